@@ -1,0 +1,392 @@
+// Depthwise causal convolution with SiLU over packed sequences, forward and
+// backward, and its single-token form on a cache addressed by slot, for gfx950.
+//
+//   pre[t, c] = b[c] + sum_k w[c, k] x[t - K + 1 + k, c],   out = silu(pre)
+// with the taps before a sequence's first row taken from its window (the last K
+// inputs it has seen, in the cache's slot) or zero.  Backward, g = dout silu'(pre):
+//   dx[t] = sum_k w[k] g[t + K - 1 - k] inside the sequence,
+//   dw[c, k] = sum_t g[t] x[t - K + 1 + k],  db[c] = sum_t g[t].
+//
+// About 2 K + 10 operations an element against two elements moved: HBM-bound.
+// A wave owns 64 V channels of one chunk of rows and walks down them with the
+// taps in registers, so each row is read once but for the K - 1 rows before a
+// chunk (and behind one, in the backward pass).
+#include <algorithm>
+
+#include "pack.h"
+
+namespace mamba {
+
+struct ConvPk {
+    Seqs q;
+    int64_t rows;
+    int C, K;
+    bool silu, fill;
+    const void* x; int64_t x_st;
+    const void* dout; int64_t dout_st;
+    const float* w; const float* b;
+    void* out; int64_t out_st;      // out, or dx
+    float* state; int64_t nslots; const int32_t* slots;
+    int64_t chunk, nchunk;
+    float* part;                    // [nchunk][K + 1][C]
+    float* dw; float* db;
+};
+
+__device__ __forceinline__ float conv_sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
+
+// KT = K as a constant, or 0: any K up to kMaxTaps (the taps then wait in a ring
+// that is shifted by one each row all the same).
+constexpr int kMaxTaps = 64;
+
+template <typename T, int KT, int V>
+__global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
+    constexpr int KM = KT ? KT : kMaxTaps;
+    const int K = KT ? KT : p.K;
+    const int lane = threadIdx.x & 63;
+    const int nblk = (p.C + 64 * V - 1) / (64 * V);
+    const int64_t item = blockIdx.x * 4ll + wave_id();
+    const int64_t ck = item / nblk;
+    if (ck >= p.nchunk) return;
+    const int c = ((int)(item - ck * nblk) * 64 + lane) * V, nc = min(V, p.C - c);
+    if (nc <= 0) return;
+    const T* x = static_cast<const T*>(p.x) + c;
+    T* out = static_cast<T*>(p.out) + c;
+    float w[KM][V], bias[V], tap[KM][V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        bias[v] = p.b && v < nc ? p.b[c + v] : 0.f;
+        for (int k = 0; k < K; ++k) w[k][v] = v < nc ? p.w[(int64_t)(c + v) * K + k] : 0.f;
+    }
+    const int64_t c0 = ck * p.chunk, c1 = min(p.rows, c0 + p.chunk);
+    int64_t t = c0;
+    const float zero[V] = {};
+    for (int s = p.q.after(c0); s < p.q.n && t < c1; ++s) {
+        const int64_t st = p.q.begin(s), en = p.q.end(s);
+        if (en <= t) continue;
+        for (; p.fill && t < min(st, c1); ++t) st_run<V, T>(out + t * p.out_st, nc, zero);
+        t = max(t, st);
+        if (t >= c1) break;
+        // the K - 1 taps before row t
+        const int64_t slot = p.state ? slot_of(p.slots, s, p.nslots) : -1;
+        for (int k = 0; k < K - 1; ++k) {
+            const int64_t at = t - (K - 1) + k;
+            if (at >= st) {
+                ld_run<V, T>(x + at * p.x_st, nc, tap[k]);
+            } else {
+                const int col = (int)(K + at - st);
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    tap[k][v] = slot >= 0 && v < nc ? p.state[(slot * p.C + c + v) * K + col] : 0.f;
+            }
+        }
+        const int64_t stop = min(en, c1);
+        for (; t < stop; ++t) {
+            ld_run<V, T>(x + t * p.x_st, nc, tap[K - 1]);
+            float o[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float acc = bias[v];
+                for (int k = 0; k < K; ++k) acc = __builtin_fmaf(w[k][v], tap[k][v], acc);
+                o[v] = p.silu ? acc * conv_sigmoid(acc) : acc;
+            }
+            st_run<V, T>(out + t * p.out_st, nc, o);
+            for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) tap[k][v] = tap[k + 1][v];
+        }
+    }
+    for (; p.fill && t < c1; ++t) st_run<V, T>(out + t * p.out_st, nc, zero);
+}
+
+// The windows after the call: window[k] = old window[k + length], then the last
+// inputs.  After the forward kernel, which reads the old ones.
+template <typename T>
+__global__ __launch_bounds__(256) void conv_pk_window(ConvPk p) {
+    const int64_t total = (int64_t)p.q.n * p.C;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+        const int s = (int)(i / p.C), c = (int)(i - (int64_t)s * p.C);
+        const int64_t slot = slot_of(p.slots, s, p.nslots);
+        const int64_t st = p.q.begin(s), en = p.q.end(s), len = en - st;
+        if (slot < 0 || len == 0) continue;
+        float* win = p.state + (slot * p.C + c) * p.K;
+        const T* x = static_cast<const T*>(p.x) + c;
+        for (int k = 0; k < p.K; ++k)
+            win[k] = k + len < p.K ? win[k + len] : load_f32<T>(x + (en - p.K + k) * p.x_st);
+    }
+}
+
+template <typename T, int KT, int V>
+__global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
+    constexpr int KM = KT ? KT : kMaxTaps;
+    const int K = KT ? KT : p.K;
+    const int lane = threadIdx.x & 63;
+    const int nblk = (p.C + 64 * V - 1) / (64 * V);
+    const int64_t item = blockIdx.x * 4ll + wave_id();
+    const int64_t ck = item / nblk;
+    if (ck >= p.nchunk) return;
+    const int c = ((int)(item - ck * nblk) * 64 + lane) * V, nc = min(V, p.C - c);
+    if (nc <= 0) return;
+    const T* x = static_cast<const T*>(p.x) + c;
+    const T* dout = static_cast<const T*>(p.dout) + c;
+    T* dx = static_cast<T*>(p.out) + c;
+    float w[KM][V], bias[V], tap[KM][V], g[KM][V], dw[KM][V], db[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        bias[v] = p.b && v < nc ? p.b[c + v] : 0.f;
+        db[v] = 0.f;
+        for (int k = 0; k < K; ++k) {
+            w[k][v] = v < nc ? p.w[(int64_t)(c + v) * K + k] : 0.f;
+            dw[k][v] = 0.f;
+        }
+    }
+    const int64_t c0 = ck * p.chunk, c1 = min(p.rows, c0 + p.chunk);
+    int64_t t = c0;
+    const float zero[V] = {};
+    for (int s = p.q.after(c0); s < p.q.n && t < c1; ++s) {
+        const int64_t st = p.q.begin(s), en = p.q.end(s);
+        if (en <= t) continue;
+        for (; p.out && p.fill && t < min(st, c1); ++t) st_run<V, T>(dx + t * p.out_st, nc, zero);
+        t = max(t, st);
+        if (t >= c1) break;
+        for (int k = 0; k < K - 1; ++k) {
+            const int64_t at = t - (K - 1) + k;
+            if (at >= st) {
+                ld_run<V, T>(x + at * p.x_st, nc, tap[k]);
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v) tap[k][v] = 0.f;
+            }
+        }
+        // g[k]: of row r - k; rows of this run give dw, the K - 1 behind it dx only
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) g[k][v] = 0.f;
+        const int64_t stop = min(en, c1);
+        for (int64_t r = t; r < stop + K - 1; ++r) {
+            for (int k = K - 1; k > 0; --k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) g[k][v] = g[k - 1][v];
+            if (r < en) {
+                float d[V];
+                ld_run<V, T>(x + r * p.x_st, nc, tap[K - 1]);
+                ld_run<V, T>(dout + r * p.dout_st, nc, d);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float acc = bias[v];
+                    for (int k = 0; k < K; ++k) acc = __builtin_fmaf(w[k][v], tap[k][v], acc);
+                    if (p.silu) {
+                        const float sg = conv_sigmoid(acc);
+                        d[v] *= sg * (1.f + acc * (1.f - sg));
+                    }
+                    g[0][v] = d[v];
+                    if (r < stop) {
+                        db[v] += d[v];
+                        for (int k = 0; k < K; ++k) dw[k][v] = __builtin_fmaf(d[v], tap[k][v], dw[k][v]);
+                    }
+                }
+                for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) tap[k][v] = tap[k + 1][v];
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v) g[0][v] = 0.f;
+            }
+            const int64_t at = r - (K - 1);
+            if (p.out && at >= t) {
+                float o[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    o[v] = 0.f;
+                    for (int k = 0; k < K; ++k) o[v] = __builtin_fmaf(w[k][v], g[k][v], o[v]);
+                }
+                st_run<V, T>(dx + at * p.out_st, nc, o);
+            }
+        }
+        t = stop;
+    }
+    for (; p.out && p.fill && t < c1; ++t) st_run<V, T>(dx + t * p.out_st, nc, zero);
+    if (!p.part) return;
+    float* part = p.part + (ck * (K + 1)) * (int64_t)p.C + c;
+    for (int k = 0; k < K; ++k) st_run<V, float>(part + (int64_t)k * p.C, nc, dw[k]);
+    st_run<V, float>(part + (int64_t)K * p.C, nc, db);
+}
+
+// The chunks' sums in order: the same result every time.
+__global__ __launch_bounds__(256) void conv_pk_join(ConvPk p) {
+    __shared__ float red[4][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6, k = blockIdx.y;
+    float s = 0.f;
+    if (c < p.C)
+        for (int64_t i = q; i < p.nchunk; i += 4) s += p.part[(i * (p.K + 1) + k) * (int64_t)p.C + c];
+    red[q][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (q == 0 && c < p.C) {
+        const int l = threadIdx.x;
+        s = (red[0][l] + red[1][l]) + (red[2][l] + red[3][l]);
+        if (k < p.K) {
+            if (p.dw) p.dw[(int64_t)c * p.K + k] = s;
+        } else if (p.db) {
+            p.db[c] = s;
+        }
+    }
+}
+
+// One token per row: the window of the row's slot moves on by it.
+struct ConvSlotParams {
+    int nb, C, K;
+    bool silu;
+    const void* x; int64_t x_sb;
+    float* state; int64_t nslots; const int32_t* slots;
+    const float* w; const float* b;
+    void* out; int64_t out_sb;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void conv_slot_step(ConvSlotParams p) {
+    const int b = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= p.C) return;
+    const int64_t slot = slot_of(p.slots, b, p.nslots);
+    T* out = static_cast<T*>(p.out) + b * p.out_sb + c;
+    if (slot < 0) {
+        store_f32<T>(out, 0.f);
+        return;
+    }
+    float* win = p.state + (slot * p.C + c) * p.K;
+    const float* w = p.w + (int64_t)c * p.K;
+    const float xv = load_f32<T>(static_cast<const T*>(p.x) + b * p.x_sb + c);
+    float acc = p.b ? p.b[c] : 0.f;
+    for (int k = 0; k < p.K; ++k) {
+        const float v = k + 1 < p.K ? win[k + 1] : xv;
+        win[k] = v;
+        acc = __builtin_fmaf(v, w[k], acc);
+    }
+    store_f32<T>(out, p.silu ? acc * conv_sigmoid(acc) : acc);
+}
+
+static int conv_pk_make(const mamba_conv1d_packed_args* a, ConvPk* o) {
+    MAMBA_CHECK_ARG(a != nullptr, "args is NULL");
+    MAMBA_CHECK_ARG(a->rows >= 0 && a->rows < (1ll << 31), "rows must be in [0, 2^31)");
+    MAMBA_CHECK_ARG(a->channels >= 1 && a->channels <= (1 << 20), "channels must be in [1, 2^20]");
+    MAMBA_CHECK_ARG(a->kernel >= 1 && a->kernel <= kMaxTaps, "kernel must be in [1, 64]");
+    MAMBA_CHECK_ARG(a->nseq >= 0, "nseq must be >= 0");
+    MAMBA_CHECK_ARG(a->io_dtype == MAMBA_F32 || a->io_dtype == MAMBA_BF16, "io_dtype must be f32 or bf16");
+    MAMBA_CHECK_ARG(a->w != nullptr, "w is required");
+    MAMBA_CHECK_ARG(a->cu_seqlens != nullptr, "cu_seqlens is required");
+    ConvPk& p = *o;
+    p = ConvPk{};
+    p.q = Seqs{a->cu_seqlens, a->nseq, a->rows};
+    p.rows = a->rows; p.C = a->channels; p.K = a->kernel;
+    p.silu = a->silu != 0; p.fill = a->fill_outside != 0;
+    p.x = a->x; p.x_st = a->x_st; p.w = a->w; p.b = a->bias;
+    // chunks of rows: long ones re-read fewer rows at their edges, as many as keep the chip full
+    // (and at most 2^20 items of 64 channels, which keeps the grid small)
+    p.chunk = 32;
+    while ((a->rows + p.chunk - 1) / p.chunk * ceil_div(p.C, 64) > (1ll << 20)) p.chunk *= 2;
+    p.nchunk = (a->rows + p.chunk - 1) / p.chunk;
+    return MAMBA_OK;
+}
+
+template <typename T, int KT>
+static uint32_t conv_pk_grid(const ConvPk& p, int V) {
+    return (uint32_t)((p.nchunk * ((p.C + 64 * V - 1) / (64 * V)) + 3) / 4);
+}
+
+template <typename T>
+static void conv_pk_fwd_launch(const ConvPk& p, hipStream_t s) {
+    switch (p.K) {
+        case 2: hipLaunchKernelGGL((conv_pk_fwd<T, 2, 4>), dim3(conv_pk_grid<T, 2>(p, 4)), dim3(256), 0, s, p); break;
+        case 3: hipLaunchKernelGGL((conv_pk_fwd<T, 3, 4>), dim3(conv_pk_grid<T, 3>(p, 4)), dim3(256), 0, s, p); break;
+        case 4: hipLaunchKernelGGL((conv_pk_fwd<T, 4, 4>), dim3(conv_pk_grid<T, 4>(p, 4)), dim3(256), 0, s, p); break;
+        default: hipLaunchKernelGGL((conv_pk_fwd<T, 0, 1>), dim3(conv_pk_grid<T, 0>(p, 1)), dim3(256), 0, s, p);
+    }
+}
+
+template <typename T>
+static void conv_pk_bwd_launch(const ConvPk& p, hipStream_t s) {
+    switch (p.K) {
+        case 2: hipLaunchKernelGGL((conv_pk_bwd<T, 2, 4>), dim3(conv_pk_grid<T, 2>(p, 4)), dim3(256), 0, s, p); break;
+        case 3: hipLaunchKernelGGL((conv_pk_bwd<T, 3, 4>), dim3(conv_pk_grid<T, 3>(p, 4)), dim3(256), 0, s, p); break;
+        case 4: hipLaunchKernelGGL((conv_pk_bwd<T, 4, 4>), dim3(conv_pk_grid<T, 4>(p, 4)), dim3(256), 0, s, p); break;
+        default: hipLaunchKernelGGL((conv_pk_bwd<T, 0, 1>), dim3(conv_pk_grid<T, 0>(p, 1)), dim3(256), 0, s, p);
+    }
+}
+
+}  // namespace mamba
+
+using namespace mamba;
+
+extern "C" int mamba_conv1d_packed_fwd(const mamba_conv1d_packed_args* a, mamba_stream_t stream) {
+    ConvPk p;
+    int st = conv_pk_make(a, &p);
+    if (st != MAMBA_OK) return st;
+    if (p.rows == 0) return MAMBA_OK;
+    MAMBA_CHECK_ARG(a->x && a->out, "x and out are required");
+    MAMBA_CHECK_ARG(a->out_st >= p.C || p.rows == 1, "rows of out overlap");
+    MAMBA_CHECK_ARG(a->state == nullptr || a->slots != nullptr || a->nslots >= a->nseq,
+                    "without slots the state needs a row per sequence");
+    p.out = a->out; p.out_st = a->out_st;
+    p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
+    hipStream_t s = (hipStream_t)stream;
+    const bool bf16 = a->io_dtype == MAMBA_BF16;
+    if (bf16) conv_pk_fwd_launch<bf16_t>(p, s);
+    else conv_pk_fwd_launch<float>(p, s);
+    MAMBA_CHECK_LAUNCH();
+    if (p.state && p.q.n) {
+        const dim3 grid((uint32_t)std::min<int64_t>(((int64_t)p.q.n * p.C + 255) / 256, 1 << 16));
+        if (bf16) hipLaunchKernelGGL(conv_pk_window<bf16_t>, grid, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL(conv_pk_window<float>, grid, dim3(256), 0, s, p);
+        MAMBA_CHECK_LAUNCH();
+    }
+    return MAMBA_OK;
+}
+
+extern "C" size_t mamba_conv1d_packed_bwd_workspace_size(const mamba_conv1d_packed_args* a) {
+    ConvPk p;
+    if (conv_pk_make(a, &p) != MAMBA_OK || (!a->dw && !a->dbias)) return 0;
+    return (size_t)p.nchunk * (p.K + 1) * p.C * 4;
+}
+
+extern "C" int mamba_conv1d_packed_bwd(const mamba_conv1d_packed_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {
+    ConvPk p;
+    int st = conv_pk_make(a, &p);
+    if (st != MAMBA_OK) return st;
+    MAMBA_CHECK_ARG(a->state == nullptr, "the gradient is of sequences without a window");
+    MAMBA_CHECK_ARG(p.rows == 0 || (a->x && a->dout), "x and dout are required");
+    MAMBA_CHECK_ARG(a->dx == nullptr || a->dx_st >= p.C || p.rows <= 1, "rows of dx overlap");
+    const size_t need = mamba_conv1d_packed_bwd_workspace_size(a);
+    if (need && (ws == nullptr || ws_bytes < need)) {
+        set_error("mamba_conv1d_packed_bwd: workspace missing or too small");
+        return MAMBA_ERR_WORKSPACE;
+    }
+    p.dout = a->dout; p.dout_st = a->dout_st; p.out = a->dx; p.out_st = a->dx_st;
+    p.part = need ? static_cast<float*>(ws) : nullptr; p.dw = a->dw; p.db = a->dbias;
+    hipStream_t s = (hipStream_t)stream;
+    if (p.rows) {
+        if (a->io_dtype == MAMBA_BF16) conv_pk_bwd_launch<bf16_t>(p, s);
+        else conv_pk_bwd_launch<float>(p, s);
+    }
+    if (p.dw || p.db) hipLaunchKernelGGL(conv_pk_join, dim3(ceil_div(p.C, 64), p.K + 1), dim3(256), 0, s, p);
+    MAMBA_CHECK_LAUNCH();
+    return MAMBA_OK;
+}
+
+extern "C" int mamba_conv1d_step_slots(const mamba_conv1d_step_slots_args* a, mamba_stream_t stream) {
+    MAMBA_CHECK_ARG(a != nullptr, "args is NULL");
+    MAMBA_CHECK_ARG(a->batch >= 0 && a->batch <= 65535, "batch must be in [0, 65535]");
+    MAMBA_CHECK_ARG(a->channels >= 1, "channels must be >= 1");
+    MAMBA_CHECK_ARG(a->kernel >= 1 && a->kernel <= kMaxTaps, "kernel must be in [1, 64]");
+    MAMBA_CHECK_ARG(a->io_dtype == MAMBA_F32 || a->io_dtype == MAMBA_BF16, "io_dtype must be f32 or bf16");
+    if (a->batch == 0) return MAMBA_OK;
+    MAMBA_CHECK_ARG(a->x && a->state && a->w && a->out, "x, state, w and out are required");
+    MAMBA_CHECK_ARG(a->slots != nullptr || a->nslots >= a->batch, "without slots the state needs a row per token");
+    MAMBA_CHECK_ARG(a->out_sb >= a->channels || a->batch == 1, "rows of out overlap");
+    ConvSlotParams p{};
+    p.nb = a->batch; p.C = a->channels; p.K = a->kernel; p.silu = a->silu != 0;
+    p.x = a->x; p.x_sb = a->x_sb; p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
+    p.w = a->w; p.b = a->bias; p.out = a->out; p.out_sb = a->out_sb;
+    const dim3 grid(ceil_div(p.C, 256), p.nb);
+    if (a->io_dtype == MAMBA_BF16) hipLaunchKernelGGL(conv_slot_step<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, p);
+    else hipLaunchKernelGGL(conv_slot_step<float>, grid, dim3(256), 0, (hipStream_t)stream, p);
+    MAMBA_CHECK_LAUNCH();
+    return MAMBA_OK;
+}

@@ -1,0 +1,82 @@
+// Runs of consecutive elements of an f32 or bf16 row as f32 values, and the
+// sequences of a packed batch: shared by the norm, dropout, convolution and
+// packed scan kernels.
+#pragma once
+
+#include "common.h"
+
+namespace mamba {
+
+// V consecutive elements at p (V sizeof(T) = 4, 8, 16 or 32 bytes; any element
+// alignment: the memory system takes unaligned vectors), the first n of them
+// read (n >= V: one vector), the others 0.
+template <int V, typename T>
+__device__ __forceinline__ void ld_run(const T* p, int n, float (&v)[V]) {
+    if (n >= V) {
+        T r[V];
+        __builtin_memcpy(r, p, V * sizeof(T));
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = load_f32<T>(&r[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = i < n ? load_f32<T>(p + i) : 0.f;
+    }
+}
+
+template <int V, typename T>
+__device__ __forceinline__ void st_run(T* p, int n, const float (&v)[V]) {
+    if (n >= V) {
+        T r[V];
+        if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const uint32_t w = pack_bf16x2(v[i], v[i + 1]);
+                r[i] = (T)w;
+                r[i + 1] = (T)(w >> 16);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) store_f32<T>(&r[i], v[i]);
+        }
+        __builtin_memcpy(p, r, V * sizeof(T));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) store_f32<T>(p + i, v[i]);
+    }
+}
+
+// ------------------------------------------------- packed sequences ---
+// Sequence s is rows cu[s] .. cu[s + 1] - 1 of a tensor of `rows` rows; rows
+// outside every sequence belong to none.  The offsets live on the device, where
+// the host cannot check them: each is clamped, so that a wrong one gives a wrong
+// result and no access out of range.
+struct Seqs {
+    const int32_t* cu;
+    int n;
+    int64_t rows;
+    __device__ __forceinline__ int64_t begin(int s) const {
+        return min(max((int64_t)cu[s], (int64_t)0), rows);
+    }
+    __device__ __forceinline__ int64_t end(int s) const {
+        return max(begin(s), min((int64_t)cu[s + 1], rows));
+    }
+    // the first sequence that ends behind row t, n if none does (t uniform)
+    __device__ __forceinline__ int after(int64_t t) const {
+        int lo = 0, hi = n;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if ((int64_t)cu[mid + 1] > t) hi = mid;
+            else lo = mid + 1;
+        }
+        return lo;
+    }
+};
+
+// Row of a cache that sequence s keeps its state in, -1: none (a slot out of range).
+__device__ __forceinline__ int64_t slot_of(const int32_t* slots, int s, int64_t nslots) {
+    const int64_t r = slots ? (int64_t)slots[s] : (int64_t)s;
+    return r >= 0 && r < nslots ? r : -1;
+}
+
+}  // namespace mamba

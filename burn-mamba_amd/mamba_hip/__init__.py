@@ -6,8 +6,8 @@ library; nothing here computes on the CPU.
 """
 
 from ._lib import MambaHipError, exported_symbols, lib  # noqa: F401
-from .mamba1 import (Mamba1, Mamba1Cache, Mamba1Config, conv1d_fwd, conv1d_step, mamba1_scan, scan_step,  # noqa: F401
-                     selective_scan, selective_scan_step)
+from .mamba1 import (Mamba1, Mamba1Cache, Mamba1Config, Mamba1Layer, conv1d_fwd, conv1d_step, mamba1_scan,  # noqa: F401
+                     scan_step, selective_scan, selective_scan_step)
 from .ssd import Mamba2SsdInput, Mamba2SsdPath, ssd2_fast_path, ssd2_fwd  # noqa: F401
 from .ssd import ssd2_autograd, ssd2_bwd  # noqa: F401
 from .step import (Mamba2, Mamba2Cache, Mamba2Config, Mamba2Layer, Mamba2Stack, linear, pack_linear,  # noqa: F401
@@ -23,3 +23,6 @@ from .mamba3 import prep_args as mamba3_prep_args, prep_fast_path as mamba3_prep
 from .mamba3 import double_inputs as mamba3_double_inputs  # noqa: F401
 from .mamba3 import fused_args as mamba3_fused_args, fused_supported as mamba3_fused_supported  # noqa: F401
 from .mamba3 import fused_run as mamba3_fused_run, ssd_fused_fwd as mamba3_ssd_fused_fwd  # noqa: F401
+from .packed import (conv1d_packed, conv1d_packed_autograd, conv1d_packed_bwd, conv1d_step_slots,  # noqa: F401
+                     mamba1_scan_packed, mamba1_scan_packed_autograd, mamba1_scan_packed_bwd, scan_step_slots)
+from .norm import (dropout, dropout_autograd, layer_norm, layer_norm_autograd, layer_norm_bwd)  # noqa: F401

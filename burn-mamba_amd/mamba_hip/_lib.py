@@ -299,6 +299,113 @@ class Mamba2LayerArgs(ctypes.Structure):
     ]
 
 
+class Conv1dPackedArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64),
+        ("nseq", c_i32), ("channels", c_i32), ("kernel", c_i32), ("io_dtype", c_i32),
+        ("silu", c_i32), ("fill_outside", c_i32),
+        ("cu_seqlens", c_vp),
+        ("x", c_vp), ("x_st", c_i64),
+        ("w", c_vp), ("bias", c_vp),
+        ("state", c_vp), ("nslots", c_i64), ("slots", c_vp),
+        ("out", c_vp), ("out_st", c_i64),
+        ("dout", c_vp), ("dout_st", c_i64),
+        ("dx", c_vp), ("dx_st", c_i64),
+        ("dw", c_vp), ("dbias", c_vp),
+    ]
+
+
+class Conv1dStepSlotsArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_i32), ("channels", c_i32), ("kernel", c_i32), ("io_dtype", c_i32), ("silu", c_i32),
+        ("x", c_vp), ("x_sb", c_i64),
+        ("state", c_vp), ("nslots", c_i64), ("slots", c_vp),
+        ("w", c_vp), ("bias", c_vp),
+        ("out", c_vp), ("out_sb", c_i64),
+    ]
+
+
+class Mamba1ScanPackedArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64),
+        ("nseq", c_i32), ("dim", c_i32), ("dstate", c_i32), ("io_dtype", c_i32),
+        ("delta_softplus", c_i32), ("fill_outside", c_i32), ("max_seqlen", c_i32),
+        ("cu_seqlens", c_vp),
+        ("u", c_vp), ("u_st", c_i64),
+        ("delta", c_vp), ("delta_st", c_i64),
+        ("A", c_vp),
+        ("B", c_vp), ("B_st", c_i64),
+        ("C", c_vp), ("C_st", c_i64),
+        ("D", c_vp),
+        ("z", c_vp), ("z_st", c_i64),
+        ("delta_bias", c_vp),
+        ("state", c_vp), ("nslots", c_i64), ("slots", c_vp),
+        ("y", c_vp), ("y_st", c_i64),
+    ]
+
+
+class Mamba1ScanPackedBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", Mamba1ScanPackedArgs),
+        ("initial_state", c_vp),
+        ("dy", c_vp), ("dy_st", c_i64),
+        ("d_final_state", c_vp),
+        ("du", c_vp), ("du_st", c_i64),
+        ("ddelta", c_vp), ("ddelta_st", c_i64),
+        ("dz", c_vp), ("dz_st", c_i64),
+        ("dB", c_vp), ("dB_st", c_i64),
+        ("dC", c_vp), ("dC_st", c_i64),
+        ("dA", c_vp), ("dD", c_vp), ("d_delta_bias", c_vp), ("d_initial_state", c_vp),
+    ]
+
+
+class Mamba1ScanStepSlotsArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_i32), ("dim", c_i32), ("dstate", c_i32), ("io_dtype", c_i32), ("delta_softplus", c_i32),
+        ("u", c_vp), ("u_sb", c_i64),
+        ("delta", c_vp), ("delta_sb", c_i64),
+        ("A", c_vp),
+        ("B", c_vp), ("B_sb", c_i64),
+        ("C", c_vp), ("C_sb", c_i64),
+        ("D", c_vp),
+        ("z", c_vp), ("z_sb", c_i64),
+        ("delta_bias", c_vp),
+        ("state", c_vp), ("nslots", c_i64), ("slots", c_vp),
+        ("y", c_vp), ("y_sb", c_i64),
+    ]
+
+
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64), ("cols", c_i32), ("io_dtype", c_i32), ("eps", ctypes.c_float),
+        ("x", c_vp), ("x_sr", c_i64),
+        ("weight", c_vp), ("bias", c_vp),
+        ("y", c_vp), ("y_sr", c_i64),
+        ("mean", c_vp), ("rstd", c_vp),
+    ]
+
+
+class LayerNormBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64), ("cols", c_i32), ("io_dtype", c_i32),
+        ("x", c_vp), ("x_sr", c_i64),
+        ("dy", c_vp), ("dy_sr", c_i64),
+        ("weight", c_vp), ("mean", c_vp), ("rstd", c_vp),
+        ("dx", c_vp), ("dx_sr", c_i64),
+        ("dweight", c_vp), ("dbias", c_vp),
+    ]
+
+
+class DropoutArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64), ("cols", c_i64), ("io_dtype", c_i32), ("p", ctypes.c_double),
+        ("x", c_vp), ("x_sr", c_i64),
+        ("residual", c_vp), ("residual_sr", c_i64),
+        ("out", c_vp), ("out_sr", c_i64),
+        ("rng", c_vp), ("offset", c_i64),
+    ]
+
+
 # name -> (argtypes, restype); the exported symbol set of include/mamba_hip.h
 _SIGNATURES = {
     "mamba_last_error": ([], ctypes.c_char_p),
@@ -366,6 +473,19 @@ _SIGNATURES = {
     "mamba2_stack_step_timed": ([ctypes.POINTER(Mamba2LayerArgs), c_i32, c_vp, ctypes.c_size_t, c_vp,
                                  ctypes.POINTER(c_vp), ctypes.POINTER(c_vp)], ctypes.c_int),
     "mamba2_stack_step_noalloc": ([ctypes.POINTER(Mamba2LayerArgs), c_i32, c_vp], ctypes.c_int),
+    "mamba_conv1d_packed_fwd": ([ctypes.POINTER(Conv1dPackedArgs), c_vp], ctypes.c_int),
+    "mamba_conv1d_packed_bwd_workspace_size": ([ctypes.POINTER(Conv1dPackedArgs)], ctypes.c_size_t),
+    "mamba_conv1d_packed_bwd": ([ctypes.POINTER(Conv1dPackedArgs), c_vp, ctypes.c_size_t, c_vp], ctypes.c_int),
+    "mamba_conv1d_step_slots": ([ctypes.POINTER(Conv1dStepSlotsArgs), c_vp], ctypes.c_int),
+    "mamba1_scan_packed_workspace_size": ([ctypes.POINTER(Mamba1ScanPackedArgs)], ctypes.c_size_t),
+    "mamba1_scan_packed_fwd": ([ctypes.POINTER(Mamba1ScanPackedArgs), c_vp, ctypes.c_size_t, c_vp], ctypes.c_int),
+    "mamba1_scan_packed_bwd_workspace_size": ([ctypes.POINTER(Mamba1ScanPackedBwdArgs)], ctypes.c_size_t),
+    "mamba1_scan_packed_bwd": ([ctypes.POINTER(Mamba1ScanPackedBwdArgs), c_vp, ctypes.c_size_t, c_vp], ctypes.c_int),
+    "mamba1_scan_step_slots": ([ctypes.POINTER(Mamba1ScanStepSlotsArgs), c_vp], ctypes.c_int),
+    "mamba_layernorm_fwd": ([ctypes.POINTER(LayerNormArgs), c_vp], ctypes.c_int),
+    "mamba_layernorm_bwd_workspace_size": ([ctypes.POINTER(LayerNormBwdArgs)], ctypes.c_size_t),
+    "mamba_layernorm_bwd": ([ctypes.POINTER(LayerNormBwdArgs), c_vp, ctypes.c_size_t, c_vp], ctypes.c_int),
+    "mamba_dropout": ([ctypes.POINTER(DropoutArgs), c_vp], ctypes.c_int),
 }
 
 _lib = None

@@ -321,6 +321,18 @@ def _wt(w: torch.Tensor, attr: str, col0: int) -> torch.Tensor:
     return _derived(w, attr, lambda t: t[:, col0:].t().contiguous())
 
 
+def _cast(w: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """w in dtype, made once and remade when the weight changes, where no gradient is wanted."""
+    from .step import _derived
+    return w if w.dtype == dtype else _derived(w, "_mamba_cast_" + str(dtype)[6:], lambda t: t.detach().to(dtype))
+
+
+def _decay(a_log: torch.Tensor) -> torch.Tensor:
+    """A = -exp(a_log) (mamba1.rs:627) of the parameter's present values."""
+    from .step import _derived
+    return _derived(a_log, "_mamba_A", lambda t: -torch.exp(t.detach()))
+
+
 @dataclass
 class Mamba1:
     """Mamba1 block, forward and step (parameters of src/mamba1/mamba1.rs:124-227);
@@ -394,11 +406,51 @@ class Mamba1:
             return mm_f32(yt.transpose(1, 2), self.out_proj_w.expand(b, -1, -1)), cache
         return torch.matmul(yt.transpose(1, 2), self.out_proj_w), cache
 
-    def step(self, x: torch.Tensor, cache: Optional[Mamba1Cache] = None):
+    def forward_packed(self, x: torch.Tensor, cu_seqlens: torch.Tensor, cache: Optional[Mamba1Cache] = None,
+                       slots: Optional[torch.Tensor] = None, max_seqlen: int = 0) -> torch.Tensor:
+        """Mamba1::forward over packed sequences of different lengths (mamba_hip.packed):
+        x [rows, d_model] f32 or bf16 -> y [rows, d_model], zero on rows outside the
+        sequences (but for a projection's bias).  With a ``cache`` (rows by ``slots``) the
+        sequences go on from it and it is updated in place, which autograd does not
+        follow; without one they start from zero and the call is differentiable, in x
+        and in every parameter that requires it."""
+        from .packed import (conv1d_packed, conv1d_packed_autograd, mamba1_scan_packed, mamba1_scan_packed_autograd)
+        c = self.cfg
+        di, r, n = c.d_inner, c.dt_rank, c.state_rank
+        if x.dim() != 2 or x.shape[1] != c.d_model:
+            raise _lib.MambaHipError(f"x: shape {tuple(x.shape)}, expected [rows, {c.d_model}]")
+        params = (self.in_proj_w, self.conv_w, self.conv_b, self.x_proj_w, self.dt_proj_w, self.dt_proj_b, self.a_log, self.d,
+                  self.out_proj_w)
+        grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, *params))
+        if grad and cache is not None:
+            raise _lib.MambaHipError("a cache is not differentiable: call under torch.no_grad(), or without one")
+        w = (lambda t: t.to(x.dtype)) if grad else (lambda t: _cast(t, x.dtype))
+        xz = torch.mm(x, w(self.in_proj_w))
+        xs, z = xz[:, :di], xz[:, di:]
+        if grad:
+            u = conv1d_packed_autograd(xs, self.conv_w, cu_seqlens, self.conv_b)
+        else:
+            u = conv1d_packed(xs, self.conv_w, cu_seqlens, self.conv_b, True, None if cache is None else cache.conv_bik, slots)
+        x_dbl = torch.mm(u, w(self.x_proj_w))
+        delta = torch.mm(x_dbl[:, :r], w(self.dt_proj_w))
+        B, C = x_dbl[:, r:r + n], x_dbl[:, r + n:]
+        if grad:  # A from its parameter, which the gradient goes to
+            y, _ = mamba1_scan_packed_autograd(u, delta, -torch.exp(self.a_log), B, C, cu_seqlens, self.d, z, self.dt_proj_b, True,
+                                               max_seqlen=max_seqlen)
+        else:
+            y = mamba1_scan_packed(u, delta, _decay(self.a_log), B, C, cu_seqlens, self.d, z, self.dt_proj_b, True,
+                                   None if cache is None else cache.ssm_bir, slots, max_seqlen)
+        return torch.mm(y, w(self.out_proj_w))
+
+    def step(self, x: torch.Tensor, cache: Optional[Mamba1Cache] = None, slots: Optional[torch.Tensor] = None):
         """Mamba1::step (mamba1.rs:533-612): returns (y [b, d_model], cache); the cache
-        is updated in place."""
+        is updated in place.  With ``slots`` [b] int32 token i's state is row slots[i] of
+        the cache, whose rows may be more, and x may be bf16 (products and y then are
+        too); without, the cache has a row per token."""
         c = self.cfg
         b = x.shape[0]
+        if slots is not None:
+            return self._step_slots(x, cache, slots), cache
         if cache is None:
             cache = self.new_cache(b)
         xr = torch.mm(x.float(), self.in_proj_w)                     # [b, 2 d_inner]
@@ -410,3 +462,53 @@ class Mamba1:
         y = scan_step(u, delta, self.A, x_dbl[:, r:r + n], x_dbl[:, r + n:], cache.ssm_bir, D=self.d, z=res,
                       delta_bias=self.dt_proj_b, delta_softplus=True)
         return torch.mm(y, self.out_proj_w), cache
+
+    def _step_slots(self, x: torch.Tensor, cache: Optional[Mamba1Cache], slots: torch.Tensor) -> torch.Tensor:
+        from .packed import conv1d_step_slots, scan_step_slots
+        if cache is None:
+            raise _lib.MambaHipError("slots without a cache")
+        c = self.cfg
+        di, r, n = c.d_inner, c.dt_rank, c.state_rank
+        w = lambda t: _cast(t, x.dtype)  # noqa: E731
+        xz = torch.mm(x, w(self.in_proj_w))
+        u = conv1d_step_slots(xz[:, :di], cache.conv_bik, slots, self.conv_w, self.conv_b)
+        x_dbl = torch.mm(u, w(self.x_proj_w))
+        delta = torch.mm(x_dbl[:, :r], w(self.dt_proj_w))
+        y = scan_step_slots(u, delta, _decay(self.a_log), x_dbl[:, r:r + n], x_dbl[:, r + n:], cache.ssm_bir, slots, self.d, xz[:, di:],
+                            self.dt_proj_b, True)
+        return torch.mm(y, w(self.out_proj_w))
+
+
+@dataclass
+class Mamba1Layer:
+    """Pre-norm residual layer (the form of src/modules/layer.rs:224-232, with layer norm for
+    its RmsNorm and dropout on the block's output) around a Mamba1 block, on packed
+    sequences: x + dropout(mixer(layer_norm(x)))."""
+    norm_w: torch.Tensor   # [d_model] f32
+    norm_b: Optional[torch.Tensor]
+    mixer: Mamba1
+    p: float = 0.0         # dropout, where a call has an rng
+    eps: float = 1e-5
+
+    @staticmethod
+    def init(cfg: Mamba1Config, device, p: float = 0.0, generator: Optional[torch.Generator] = None) -> "Mamba1Layer":
+        return Mamba1Layer(torch.ones(cfg.d_model, device=device), torch.zeros(cfg.d_model, device=device),
+                           cfg.init(device, generator), p)
+
+    def forward_packed(self, x: torch.Tensor, cu_seqlens: torch.Tensor, cache: Optional[Mamba1Cache] = None,
+                       slots: Optional[torch.Tensor] = None, max_seqlen: int = 0, rng: Optional[torch.Tensor] = None,
+                       offset: int = 0) -> torch.Tensor:
+        """x [rows, d_model] f32 or bf16 -> the same; cache and slots as in
+        ``Mamba1.forward_packed``.  ``rng`` and ``offset`` (``mamba_hip.dropout``) are given in
+        training: each layer of a stack its own offset."""
+        from .norm import dropout_autograd, layer_norm_autograd
+        y = self.mixer.forward_packed(layer_norm_autograd(x, self.norm_w, self.norm_b, self.eps), cu_seqlens, cache, slots, max_seqlen)
+        if rng is None or self.p == 0.0:
+            return x + y
+        return dropout_autograd(y, self.p, rng, offset, x)
+
+    def step(self, x: torch.Tensor, cache: Mamba1Cache, slots: Optional[torch.Tensor] = None):
+        """One token per row of x [b, d_model] on ``cache`` (``Mamba1.step``)."""
+        from .norm import layer_norm
+        y, cache = self.mixer.step(layer_norm(x, self.norm_w, self.norm_b, self.eps), cache, slots)
+        return x + y, cache

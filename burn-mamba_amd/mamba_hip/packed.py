@@ -1,0 +1,344 @@
+"""Mamba-1's short convolution and selective scan over packed sequences, their
+gradients, and their single-token steps on a cache addressed by slot.
+
+Packed: the rows of several sequences one behind the other in [rows, .] tensors,
+sequence s being rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (``cu_seqlens`` int32
+on the device; sequences may be empty).  Rows outside every sequence (padding) are
+left as they were in an output that the caller gives, and are zero in one that is
+made here.
+
+A cache is addressed by slot: sequence (or token) s keeps its state in row
+``slots[s]`` (int32; None: row s) of the cache tensor, updated in place.  The slots
+of one call are distinct; one out of range is no state (zero at the start, nothing
+kept).  A slot's row is zeroed by the caller before its first sequence.
+
+Reference: ``Mamba1::forward`` layer 2 (src/mamba1/mamba1.rs:300-340),
+``Mamba1::selective_scan`` (mamba1.rs:422-523), ``Mamba1::step``
+(mamba1.rs:533-733), which take sequences of one length and a cache row for each.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import (Conv1dPackedArgs, Conv1dStepSlotsArgs, Mamba1ScanPackedArgs, Mamba1ScanPackedBwdArgs,
+                   Mamba1ScanStepSlotsArgs, check)
+from .ssd import _dtype_code, _stream, workspace
+
+
+def _fail(msg: str):
+    raise _lib.MambaHipError(msg)
+
+
+def _need(ok: bool, msg: str):
+    if not ok:
+        _fail(msg)
+
+
+def _rows(t: torch.Tensor, name: str, rows: Optional[int] = None, cols: Optional[int] = None, dtype=None):
+    """A [rows, cols] tensor whose last axis is contiguous."""
+    _need(t.dim() == 2 and (rows is None or t.shape[0] == rows) and (cols is None or t.shape[1] == cols),
+          f"{name}: shape {tuple(t.shape)}, expected [{'rows' if rows is None else rows}, {'cols' if cols is None else cols}]")
+    _need(t.dtype == dtype if dtype is not None else t.dtype in (torch.float32, torch.bfloat16),
+          f"{name}: dtype {t.dtype}, expected {dtype or 'float32 or bfloat16'}")
+    _need(t.stride(1) == 1 or t.shape[1] <= 1, f"{name}: the last axis must be contiguous")
+
+
+def _param(t: Optional[torch.Tensor], name: str, *shape: int):
+    if t is not None:
+        _need(t.dtype == torch.float32 and t.is_contiguous() and tuple(t.shape) == shape,
+              f"{name} must be a contiguous float32 tensor of shape {shape}")
+
+
+def _sequences(cu_seqlens: torch.Tensor, slots: Optional[torch.Tensor], state: Optional[torch.Tensor], name: str, *tail: int) -> int:
+    _need(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1 and cu_seqlens.is_contiguous(),
+          "cu_seqlens must be a contiguous int32 tensor of one more entry than sequences")
+    n = cu_seqlens.numel() - 1
+    _slots(n, slots, state, name, *tail)
+    return n
+
+
+def _slots(n: int, slots, state, name: str, *tail: int):
+    if state is not None:
+        _need(state.dtype == torch.float32 and state.is_contiguous() and tuple(state.shape[1:]) == tail,
+              f"{name} must be a contiguous float32 tensor of shape (slots, {', '.join(map(str, tail))})")
+        _need(slots is not None or state.shape[0] >= n, f"{name} needs a row per sequence where no slots are given")
+    if slots is not None:
+        _need(state is not None, "slots without a state")
+        _need(slots.dtype == torch.int32 and tuple(slots.shape) == (n,) and slots.is_contiguous(),
+              f"slots must be a contiguous int32 tensor of {n} entries")
+
+
+def _one_device(*ts: Optional[torch.Tensor]):
+    """Every operand on one GPU, which becomes the current device for the call."""
+    ts = [t for t in ts if t is not None]
+    dev = ts[0].get_device()  # below 0: not a GPU
+    _need(dev >= 0 and all(t.get_device() == dev for t in ts), "operands on one GPU device required")
+    return torch.cuda.device(dev) if dev != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _p(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _st(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.stride(0)
+
+
+def _like_rows(dy: torch.Tensor) -> torch.Tensor:
+    """A gradient as the kernels read it (autograd hands on expanded ones)."""
+    return dy if dy.stride(-1) == 1 or dy.shape[-1] <= 1 else dy.contiguous()
+
+
+# ------------------------------------------------------------- convolution ---
+
+def _conv_args(x, w, cu_seqlens, bias, silu, state=None, slots=None) -> Conv1dPackedArgs:
+    _rows(x, "x")
+    rows, c = x.shape
+    _need(w.dim() == 2, "w must be [channels, kernel]")
+    k = w.shape[1]
+    _param(w, "w", c, k)
+    _param(bias, "bias", c)
+    a = Conv1dPackedArgs()
+    a.nseq = _sequences(cu_seqlens, slots, state, "state", c, k)
+    a.rows, a.channels, a.kernel, a.io_dtype, a.silu = rows, c, k, _dtype_code(x), int(bool(silu))
+    a.cu_seqlens = cu_seqlens.data_ptr()
+    a.x, a.x_st, a.w, a.bias = x.data_ptr(), x.stride(0), w.data_ptr(), _p(bias)
+    a.state, a.nslots, a.slots = _p(state), 0 if state is None else state.shape[0], _p(slots)
+    return a
+
+
+def conv1d_packed(x: torch.Tensor, w: torch.Tensor, cu_seqlens: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                  silu: bool = True, state: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Depthwise causal convolution (+ SiLU) of packed sequences: x [rows, c] f32 or bf16,
+    w [c, K], bias [c] f32 -> [rows, c] of x's type.  ``state`` [slots, c, K] f32: the
+    windows (the last K inputs) that the sequences go on from, moved on in place."""
+    a = _conv_args(x, w, cu_seqlens, bias, silu, state, slots)
+    a.fill_outside = int(out is None)
+    if out is not None:
+        _rows(out, "out", x.shape[0], x.shape[1], x.dtype)
+    with _one_device(x, w, cu_seqlens, bias, state, slots, out):
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        a.out, a.out_st = out.data_ptr(), out.stride(0)
+        check(_lib.lib().mamba_conv1d_packed_fwd(ctypes.byref(a), _stream(x.device)), "mamba_conv1d_packed_fwd")
+    return out
+
+
+def conv1d_packed_bwd(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, cu_seqlens: torch.Tensor,
+                      bias: Optional[torch.Tensor] = None, silu: bool = True) -> dict:
+    """Gradients of ``conv1d_packed`` without a state: dict(dx [rows, c] of x's type, zero
+    outside the sequences; dw [c, K], dbias [c] f32)."""
+    a = _conv_args(x, w, cu_seqlens, bias, silu)
+    _rows(dout, "dout", x.shape[0], x.shape[1], x.dtype)
+    with _one_device(dout, x, w, cu_seqlens, bias):
+        out = dict(dx=torch.empty(x.shape, dtype=x.dtype, device=x.device), dw=torch.empty_like(w),
+                   dbias=None if bias is None else torch.empty_like(bias))
+        a.fill_outside = 1
+        a.dout, a.dout_st = dout.data_ptr(), dout.stride(0)
+        a.dx, a.dx_st, a.dw, a.dbias = out["dx"].data_ptr(), out["dx"].stride(0), out["dw"].data_ptr(), _p(out["dbias"])
+        L = _lib.lib()
+        ws = workspace(x.device, L.mamba_conv1d_packed_bwd_workspace_size(ctypes.byref(a)))
+        check(L.mamba_conv1d_packed_bwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), _stream(x.device)),
+              "mamba_conv1d_packed_bwd")
+    return out
+
+
+class _Conv1dPacked(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, cu_seqlens, bias, silu):
+        ctx.silu = silu
+        ctx.save_for_backward(x, w, cu_seqlens, bias)
+        return conv1d_packed(x, w, cu_seqlens, bias, silu)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, w, cu_seqlens, bias = ctx.saved_tensors
+        g = conv1d_packed_bwd(_like_rows(dout), x, w, cu_seqlens, bias, ctx.silu)
+        return g["dx"], g["dw"], None, g["dbias"], None
+
+
+def conv1d_packed_autograd(x, w, cu_seqlens, bias=None, silu: bool = True) -> torch.Tensor:
+    """``conv1d_packed`` as a differentiable op: gradients of x, w and bias."""
+    return _Conv1dPacked.apply(x, w, cu_seqlens, bias, silu)
+
+
+def conv1d_step_slots(x: torch.Tensor, state: torch.Tensor, slots: Optional[torch.Tensor], w: torch.Tensor,
+                      bias: Optional[torch.Tensor] = None, silu: bool = True, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``conv1d_step`` on a cache of slots: x [b, c] f32 or bf16, state [slots, c, K] f32 (in
+    place), slots [b] int32.  Returns out [b, c] of x's type; a row whose slot is out of
+    range is zero."""
+    _rows(x, "x")
+    b, c = x.shape
+    _need(w.dim() == 2, "w must be [channels, kernel]")
+    k = w.shape[1]
+    _param(w, "w", c, k)
+    _param(bias, "bias", c)
+    _slots(b, slots, state, "state", c, k)
+    if out is not None:
+        _rows(out, "out", b, c, x.dtype)
+    with _one_device(x, state, slots, w, bias, out):
+        if out is None:
+            out = torch.empty((b, c), dtype=x.dtype, device=x.device)
+        a = Conv1dStepSlotsArgs()
+        a.batch, a.channels, a.kernel, a.io_dtype, a.silu = b, c, k, _dtype_code(x), int(bool(silu))
+        a.x, a.x_sb, a.state, a.nslots, a.slots = x.data_ptr(), x.stride(0), state.data_ptr(), state.shape[0], _p(slots)
+        a.w, a.bias, a.out, a.out_sb = w.data_ptr(), _p(bias), out.data_ptr(), out.stride(0)
+        check(_lib.lib().mamba_conv1d_step_slots(ctypes.byref(a), _stream(x.device)), "mamba_conv1d_step_slots")
+    return out
+
+
+# --------------------------------------------------------------------- scan ---
+
+def _scan_operands(u, delta, A, B, C, D, z, delta_bias):
+    """Checks shared by the packed scan and the step; (rows, dim, dstate)."""
+    _rows(u, "u")
+    rows, d = u.shape
+    _need(A.dim() == 2, "A must be [dim, dstate]")
+    n = A.shape[1]
+    _param(A, "A", d, n)
+    _rows(delta, "delta", rows, d, u.dtype)
+    _rows(B, "B", rows, n, u.dtype)
+    _rows(C, "C", rows, n, u.dtype)
+    if z is not None:
+        _rows(z, "z", rows, d, u.dtype)
+    _param(D, "D", d)
+    _param(delta_bias, "delta_bias", d)
+    return rows, d, n
+
+
+def _scan_args(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, delta_softplus, max_seqlen, state=None, slots=None):
+    a = Mamba1ScanPackedArgs()
+    a.rows, a.dim, a.dstate = _scan_operands(u, delta, A, B, C, D, z, delta_bias)
+    a.nseq = _sequences(cu_seqlens, slots, state, "state", a.dim, a.dstate)
+    a.io_dtype, a.delta_softplus, a.max_seqlen = _dtype_code(u), int(bool(delta_softplus)), int(max_seqlen)
+    a.cu_seqlens = cu_seqlens.data_ptr()
+    for name, t in (("u", u), ("delta", delta), ("B", B), ("C", C), ("z", z)):
+        setattr(a, name, _p(t))
+        setattr(a, name + "_st", _st(t))
+    a.A, a.D, a.delta_bias = A.data_ptr(), _p(D), _p(delta_bias)
+    a.state, a.nslots, a.slots = _p(state), 0 if state is None else state.shape[0], _p(slots)
+    return a
+
+
+def mamba1_scan_packed(u, delta, A, B, C, cu_seqlens, D=None, z=None, delta_bias=None, delta_softplus: bool = False,
+                       state: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None, max_seqlen: int = 0,
+                       y: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The selective scan of packed sequences: u, delta, z [rows, d] and B, C [rows, n] f32
+    or bf16 (one type, any row strides), A [d, n], D, delta_bias [d] f32, n <= 64.
+    ``state`` [slots, d, n] f32 holds what the sequences start from and is overwritten
+    with what they end in; None starts from zero.  ``max_seqlen``, a bound on the longest
+    sequence where the caller knows one, helps to choose the schedule (0: unknown).
+    Returns y [rows, d] of u's type."""
+    a = _scan_args(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, delta_softplus, max_seqlen, state, slots)
+    a.fill_outside = int(y is None)
+    if y is not None:
+        _rows(y, "y", u.shape[0], u.shape[1], u.dtype)
+    with _one_device(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, state, slots, y):
+        if y is None:
+            y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+        a.y, a.y_st = y.data_ptr(), y.stride(0)
+        L = _lib.lib()
+        need = L.mamba1_scan_packed_workspace_size(ctypes.byref(a))
+        ws = workspace(u.device, need) if need else None
+        check(L.mamba1_scan_packed_fwd(ctypes.byref(a), _p(ws), need, _stream(u.device)), "mamba1_scan_packed_fwd")
+    return y
+
+
+def mamba1_scan_packed_bwd(dy, u, delta, A, B, C, cu_seqlens, D=None, z=None, delta_bias=None, delta_softplus: bool = False,
+                           initial_state=None, d_final_state=None, max_seqlen: int = 0) -> dict:
+    """Gradients of the packed scan from its inputs (every intermediate is found again).
+    ``initial_state`` and ``d_final_state`` [sequences, d, n] f32 or None.  Returns
+    dict(du, ddelta, dz, dB, dC of their tensors' type, zero outside the sequences; dA,
+    dD, d_delta_bias, d_initial_state f32; None for what was not given).  The same inputs
+    give the same bits."""
+    a = Mamba1ScanPackedBwdArgs()
+    a.fwd = _scan_args(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, delta_softplus, max_seqlen)
+    d, n, s = A.shape[0], A.shape[1], cu_seqlens.numel() - 1
+    _rows(dy, "dy", u.shape[0], d, u.dtype)
+    _param(initial_state, "initial_state", s, d, n)
+    _param(d_final_state, "d_final_state", s, d, n)
+    with _one_device(dy, u, delta, A, B, C, cu_seqlens, D, z, delta_bias, initial_state, d_final_state):
+        def new(t):
+            return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+        out = dict(du=new(u), ddelta=new(delta), dz=new(z), dB=new(B), dC=new(C), dA=new(A), dD=new(D),
+                   d_delta_bias=new(delta_bias), d_initial_state=None)
+        if initial_state is not None:  # an empty sequence ends in what it starts from
+            out["d_initial_state"] = torch.zeros_like(initial_state) if d_final_state is None else d_final_state.clone()
+        a.initial_state, a.d_final_state = _p(initial_state), _p(d_final_state)
+        a.dy, a.dy_st = dy.data_ptr(), dy.stride(0)
+        for name in ("du", "ddelta", "dz", "dB", "dC"):
+            setattr(a, name, _p(out[name]))
+            setattr(a, name + "_st", _st(out[name]))
+        for name in ("dA", "dD", "d_delta_bias", "d_initial_state"):
+            setattr(a, name, _p(out[name]))
+        L = _lib.lib()
+        need = L.mamba1_scan_packed_bwd_workspace_size(ctypes.byref(a))
+        ws = workspace(u.device, need)
+        check(L.mamba1_scan_packed_bwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), _stream(u.device)),
+              "mamba1_scan_packed_bwd")
+    return out
+
+
+class _ScanPacked(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, u, delta, A, B, C, cu_seqlens, D, z, delta_bias, initial_state, delta_softplus, max_seqlen):
+        shape = (cu_seqlens.numel() - 1, *A.shape)
+        _param(initial_state, "initial_state", *shape)
+        final = torch.zeros(shape, dtype=torch.float32, device=u.device) if initial_state is None else initial_state.clone()
+        y = mamba1_scan_packed(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, delta_softplus, final, None, max_seqlen)
+        ctx.save_for_backward(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, initial_state)
+        ctx.set_materialize_grads(False)
+        ctx.opts = (delta_softplus, max_seqlen)
+        return y, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dfinal):
+        u, delta, A, B, C, cu_seqlens, D, z, delta_bias, h0 = ctx.saved_tensors
+        if dy is None and dfinal is None:
+            return (None,) * 12
+        dy = torch.zeros(u.shape, dtype=u.dtype, device=u.device) if dy is None else _like_rows(dy)
+        g = mamba1_scan_packed_bwd(dy, u, delta, A, B, C, cu_seqlens, D, z, delta_bias, ctx.opts[0], h0,
+                                   None if dfinal is None else dfinal.contiguous(), ctx.opts[1])
+        return (g["du"], g["ddelta"], g["dA"], g["dB"], g["dC"], None, g["dD"], g["dz"], g["d_delta_bias"],
+                g["d_initial_state"], None, None)
+
+
+def mamba1_scan_packed_autograd(u, delta, A, B, C, cu_seqlens, D=None, z=None, delta_bias=None, delta_softplus: bool = False,
+                                initial_state=None, max_seqlen: int = 0):
+    """``mamba1_scan_packed`` as a differentiable op: (y, final_state [sequences, d, n]) from
+    ``initial_state`` [sequences, d, n] (None: zero), with gradients of every float input."""
+    return _ScanPacked.apply(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, initial_state, delta_softplus, max_seqlen)
+
+
+def scan_step_slots(u, delta, A, B, C, state: torch.Tensor, slots: Optional[torch.Tensor], D=None, z=None, delta_bias=None,
+                    delta_softplus: bool = False, y: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``scan_step`` on a cache of slots: u, delta, z [b, d] and B, C [b, n] f32 or bf16 (one
+    type), state [slots, d, n] f32 (in place), slots [b] int32.  Returns y [b, d] of u's
+    type; a row whose slot is out of range is zero."""
+    b, d, n = _scan_operands(u, delta, A, B, C, D, z, delta_bias)
+    _slots(b, slots, state, "state", d, n)
+    if y is not None:
+        _rows(y, "y", b, d, u.dtype)
+    with _one_device(u, delta, A, B, C, state, slots, D, z, delta_bias, y):
+        if y is None:
+            y = torch.empty((b, d), dtype=u.dtype, device=u.device)
+        a = Mamba1ScanStepSlotsArgs()
+        a.batch, a.dim, a.dstate, a.io_dtype, a.delta_softplus = b, d, n, _dtype_code(u), int(bool(delta_softplus))
+        for name, t in (("u", u), ("delta", delta), ("B", B), ("C", C), ("z", z), ("y", y)):
+            setattr(a, name, _p(t))
+            setattr(a, name + "_sb", _st(t))
+        a.A, a.D, a.delta_bias = A.data_ptr(), _p(D), _p(delta_bias)
+        a.state, a.nslots, a.slots = state.data_ptr(), state.shape[0], _p(slots)
+        check(_lib.lib().mamba1_scan_step_slots(ctypes.byref(a), _stream(u.device)), "mamba1_scan_step_slots")
+    return y

@@ -47,6 +47,11 @@
  *                          depthwise conv1d + SiLU over xBC, dt softplus/clamp, conv-cache update
  *   mamba2_gated_rmsnorm <- RmsNormGated::forward (src/modules/norm/rms_norm_gated.rs:70-135),
  *                          step 7 of Mamba2::forward (src/mamba2/mamba2.rs:776)
+ * Beside them, for training and serving a Mamba-1 layer on packed sequences:
+ *   mamba_conv1d_packed_fwd / _bwd, mamba1_scan_packed_fwd / _bwd (sequences of
+ *   different lengths, gradients), mamba_conv1d_step_slots and
+ *   mamba1_scan_step_slots (single tokens on a cache addressed by slot),
+ *   mamba_layernorm_fwd / _bwd and mamba_dropout.
  */
 #ifndef MAMBA_HIP_H
 #define MAMBA_HIP_H
@@ -842,6 +847,201 @@ typedef struct mamba2_gated_norm_args {
 } mamba2_gated_norm_args;
 
 int mamba2_gated_rmsnorm(const mamba2_gated_norm_args* args, mamba_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* Packed sequences: the rows of several sequences one behind the other in     */
+/* [rows, .] tensors.  Sequence s is rows cu_seqlens[s] .. cu_seqlens[s + 1]-1 */
+/* (cu_seqlens: nseq + 1 non-decreasing int32 on the device; a sequence may be */
+/* empty); rows outside all of them are left as they were, or zeroed with      */
+/* fill_outside.  A cache is addressed by slot: sequence (token) s keeps its   */
+/* state in row slots[s] of [nslots, ...] (NULL: row s).  A slot out of range  */
+/* is no state: the sequence starts from zero and keeps nothing.  The slots of */
+/* one call are distinct.  Rows are strided, their last axis contiguous.       */
+/* ------------------------------------------------------------------------- */
+
+/* Depthwise causal convolution + SiLU (layer 2 of Mamba1::forward,            */
+/* src/mamba1/mamba1.rs:300-340, for packed rows):                             */
+/*   pre[t, c] = bias[c] + sum_k w[c, k] x[t - K + 1 + k, c]; out = silu(pre)  */
+/* with the inputs before a sequence from its window state[slot, c, :] (the    */
+/* last K inputs, updated in place) or zero.  The backward takes dout, x, w    */
+/* and bias (state NULL) and writes dx [rows, c] (rows outside zeroed with     */
+/* fill_outside), dw [c, K], dbias [c]; each may be NULL.                      */
+typedef struct mamba_conv1d_packed_args {
+    int64_t rows;
+    int32_t nseq, channels, kernel, io_dtype; /* kernel 1..64                 */
+    int32_t silu, fill_outside;
+    const int32_t* cu_seqlens;
+    const void* x;      int64_t x_st;         /* [rows, c] of io_dtype        */
+    const float* w;                           /* [c, K]                       */
+    const float* bias;                        /* [c] or NULL                  */
+    float* state;                             /* [nslots, c, K] or NULL       */
+    int64_t nslots;
+    const int32_t* slots;                     /* [nseq] or NULL               */
+    void* out;          int64_t out_st;
+    const void* dout;   int64_t dout_st;      /* backward                     */
+    void* dx;           int64_t dx_st;
+    float* dw;
+    float* dbias;
+} mamba_conv1d_packed_args;
+
+int mamba_conv1d_packed_fwd(const mamba_conv1d_packed_args* args, mamba_stream_t stream);
+size_t mamba_conv1d_packed_bwd_workspace_size(const mamba_conv1d_packed_args* args);
+int mamba_conv1d_packed_bwd(const mamba_conv1d_packed_args* args, void* workspace, size_t workspace_bytes,
+                            mamba_stream_t stream);
+
+/* mamba_conv1d_step with the windows of slots: one token per row of x.  The   */
+/* output row of a slot out of range is zero.                                  */
+typedef struct mamba_conv1d_step_slots_args {
+    int32_t batch, channels, kernel, io_dtype, silu;
+    const void* x;      int64_t x_sb;
+    float* state;                             /* [nslots, c, K]               */
+    int64_t nslots;
+    const int32_t* slots;                     /* [batch] or NULL              */
+    const float* w;
+    const float* bias;
+    void* out;          int64_t out_sb;
+} mamba_conv1d_step_slots_args;
+
+int mamba_conv1d_step_slots(const mamba_conv1d_step_slots_args* args, mamba_stream_t stream);
+
+/* Selective scan (Mamba1::selective_scan, src/mamba1/mamba1.rs:422-523, with  */
+/* the dt_proj bias + softplus and the silu gate, as mamba1_scan_fwd):         */
+/*   h_t = exp(d_t A) h_{t-1} + d_t u_t B_t,  y_t = (sum_n C h_t + D u_t) silu(z_t) */
+/* dstate 1..64.  state is read for a sequence's start and overwritten with    */
+/* its end; NULL starts from zero and keeps nothing.  max_seqlen: a bound on   */
+/* the longest sequence that the caller knows, or 0 (a hint: it chooses the    */
+/* schedule, never the result's meaning).                                      */
+typedef struct mamba1_scan_packed_args {
+    int64_t rows;
+    int32_t nseq, dim, dstate, io_dtype;
+    int32_t delta_softplus, fill_outside, max_seqlen;
+    const int32_t* cu_seqlens;
+    const void* u;      int64_t u_st;         /* [rows, d] of io_dtype        */
+    const void* delta;  int64_t delta_st;     /* [rows, d]                    */
+    const float* A;                           /* [d, n]                       */
+    const void* B;      int64_t B_st;         /* [rows, n]                    */
+    const void* C;      int64_t C_st;         /* [rows, n]                    */
+    const float* D;                           /* [d] or NULL                  */
+    const void* z;      int64_t z_st;         /* [rows, d] or NULL            */
+    const float* delta_bias;                  /* [d] or NULL                  */
+    float* state;                             /* [nslots, d, n] or NULL       */
+    int64_t nslots;
+    const int32_t* slots;                     /* [nseq] or NULL               */
+    void* y;            int64_t y_st;         /* [rows, d]                    */
+} mamba1_scan_packed_args;
+
+size_t mamba1_scan_packed_workspace_size(const mamba1_scan_packed_args* args);
+int mamba1_scan_packed_fwd(const mamba1_scan_packed_args* args, void* workspace, size_t workspace_bytes,
+                           mamba_stream_t stream);
+
+/* Its gradients from the inputs (fwd.state and fwd.slots NULL, fwd.y unused), */
+/* every intermediate found again.  initial_state and d_final_state [nseq, d,  */
+/* n] or NULL (zero).  du, ddelta, dz, dB and dC are of io_dtype, zero outside */
+/* the sequences; dD, d_delta_bias and d_initial_state may be NULL, and        */
+/* d_initial_state's rows of empty sequences are left as they were.  Sums are  */
+/* taken in a fixed order: the same inputs give the same bits.                 */
+typedef struct mamba1_scan_packed_bwd_args {
+    mamba1_scan_packed_args fwd;
+    const float* initial_state;
+    const void* dy;     int64_t dy_st;
+    const float* d_final_state;
+    void* du;           int64_t du_st;
+    void* ddelta;       int64_t ddelta_st;
+    void* dz;           int64_t dz_st;
+    void* dB;           int64_t dB_st;
+    void* dC;           int64_t dC_st;
+    float* dA;
+    float* dD;
+    float* d_delta_bias;
+    float* d_initial_state;
+} mamba1_scan_packed_bwd_args;
+
+size_t mamba1_scan_packed_bwd_workspace_size(const mamba1_scan_packed_bwd_args* args);
+int mamba1_scan_packed_bwd(const mamba1_scan_packed_bwd_args* args, void* workspace, size_t workspace_bytes,
+                           mamba_stream_t stream);
+
+/* mamba1_scan_step with the states of slots: one token per row.  The output   */
+/* row of a slot out of range is zero.                                         */
+typedef struct mamba1_scan_step_slots_args {
+    int32_t batch, dim, dstate, io_dtype, delta_softplus; /* dstate 1..1024   */
+    const void* u;      int64_t u_sb;
+    const void* delta;  int64_t delta_sb;
+    const float* A;                           /* [d, n]                       */
+    const void* B;      int64_t B_sb;
+    const void* C;      int64_t C_sb;
+    const float* D;
+    const void* z;      int64_t z_sb;
+    const float* delta_bias;
+    float* state;                             /* [nslots, d, n]               */
+    int64_t nslots;
+    const int32_t* slots;                     /* [batch] or NULL              */
+    void* y;            int64_t y_sb;
+} mamba1_scan_step_slots_args;
+
+int mamba1_scan_step_slots(const mamba1_scan_step_slots_args* args, mamba_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* Layer norm over rows (cols contiguous elements of io_dtype):                */
+/*   xh = (x - mean) rstd, rstd = 1 / sqrt(mean((x - mean)^2) + eps),          */
+/*   y = xh weight + bias                                                      */
+/* weight NULL is 1, bias NULL 0.  mean and rstd [rows] f32 are written if     */
+/* given; the backward needs them:                                             */
+/*   g = dy weight, dx = rstd (g - mean(g) - xh mean(g xh)),                   */
+/*   dweight = sum over rows of dy xh, dbias = sum of dy                       */
+/* (dx, dweight and dbias each may be NULL; sums in a fixed order).  The       */
+/* normalisation beside the reference's RmsNorm (mamba_rmsnorm).               */
+/* ------------------------------------------------------------------------- */
+typedef struct mamba_layernorm_args {
+    int64_t rows;
+    int32_t cols, io_dtype;
+    float eps;
+    const void* x;      int64_t x_sr;
+    const float* weight;
+    const float* bias;
+    void* y;            int64_t y_sr;
+    float* mean;
+    float* rstd;
+} mamba_layernorm_args;
+
+int mamba_layernorm_fwd(const mamba_layernorm_args* args, mamba_stream_t stream);
+
+typedef struct mamba_layernorm_bwd_args {
+    int64_t rows;
+    int32_t cols, io_dtype;
+    const void* x;      int64_t x_sr;
+    const void* dy;     int64_t dy_sr;
+    const float* weight;
+    const float* mean;
+    const float* rstd;
+    void* dx;           int64_t dx_sr;
+    float* dweight;
+    float* dbias;
+} mamba_layernorm_bwd_args;
+
+size_t mamba_layernorm_bwd_workspace_size(const mamba_layernorm_bwd_args* args);
+int mamba_layernorm_bwd(const mamba_layernorm_bwd_args* args, void* workspace, size_t workspace_bytes,
+                        mamba_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* Dropout: out[i] = residual[i] + (word(i) >= p 2^32 ? x[i] / (1 - p) : 0),   */
+/* word(i) = word i % 4 of Philox 4x32-10 at counter (i / 4, rng[1] + offset), */
+/* key rng[0], i the row-major place of the element: the mask is a function    */
+/* of (rng, offset, place) and is never stored.  rng: two int64 on the device. */
+/* Applied to dy (residual NULL) with the same rng and offset it is the        */
+/* gradient of x.  out may be x or residual.                                   */
+/* ------------------------------------------------------------------------- */
+typedef struct mamba_dropout_args {
+    int64_t rows, cols;
+    int32_t io_dtype;
+    double p;                                 /* in [0, 1]                    */
+    const void* x;          int64_t x_sr;
+    const void* residual;   int64_t residual_sr;
+    void* out;              int64_t out_sr;
+    const int64_t* rng;
+    int64_t offset;
+} mamba_dropout_args;
+
+int mamba_dropout(const mamba_dropout_args* args, mamba_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -812,6 +812,254 @@ impl Default for Mamba2GatedNormArgs {
     }
 }
 
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct MambaConv1dPackedArgs {
+    pub rows: i64,
+    pub nseq: i32,
+    pub channels: i32,
+    pub kernel: i32,
+    pub io_dtype: i32,
+    pub silu: i32,
+    pub fill_outside: i32,
+    pub cu_seqlens: *const i32,
+    pub x: *const c_void,
+    pub x_st: i64,
+    pub w: *const f32,
+    pub bias: *const f32,
+    pub state: *mut f32,
+    pub nslots: i64,
+    pub slots: *const i32,
+    pub out: *mut c_void,
+    pub out_st: i64,
+    pub dout: *const c_void,
+    pub dout_st: i64,
+    pub dx: *mut c_void,
+    pub dx_st: i64,
+    pub dw: *mut f32,
+    pub dbias: *mut f32,
+}
+
+impl Default for MambaConv1dPackedArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct MambaConv1dStepSlotsArgs {
+    pub batch: i32,
+    pub channels: i32,
+    pub kernel: i32,
+    pub io_dtype: i32,
+    pub silu: i32,
+    pub x: *const c_void,
+    pub x_sb: i64,
+    pub state: *mut f32,
+    pub nslots: i64,
+    pub slots: *const i32,
+    pub w: *const f32,
+    pub bias: *const f32,
+    pub out: *mut c_void,
+    pub out_sb: i64,
+}
+
+impl Default for MambaConv1dStepSlotsArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Mamba1ScanPackedArgs {
+    pub rows: i64,
+    pub nseq: i32,
+    pub dim: i32,
+    pub dstate: i32,
+    pub io_dtype: i32,
+    pub delta_softplus: i32,
+    pub fill_outside: i32,
+    pub max_seqlen: i32,
+    pub cu_seqlens: *const i32,
+    pub u: *const c_void,
+    pub u_st: i64,
+    pub delta: *const c_void,
+    pub delta_st: i64,
+    pub A: *const f32,
+    pub B: *const c_void,
+    pub B_st: i64,
+    pub C: *const c_void,
+    pub C_st: i64,
+    pub D: *const f32,
+    pub z: *const c_void,
+    pub z_st: i64,
+    pub delta_bias: *const f32,
+    pub state: *mut f32,
+    pub nslots: i64,
+    pub slots: *const i32,
+    pub y: *mut c_void,
+    pub y_st: i64,
+}
+
+impl Default for Mamba1ScanPackedArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Mamba1ScanPackedBwdArgs {
+    pub fwd: Mamba1ScanPackedArgs,
+    pub initial_state: *const f32,
+    pub dy: *const c_void,
+    pub dy_st: i64,
+    pub d_final_state: *const f32,
+    pub du: *mut c_void,
+    pub du_st: i64,
+    pub ddelta: *mut c_void,
+    pub ddelta_st: i64,
+    pub dz: *mut c_void,
+    pub dz_st: i64,
+    pub dB: *mut c_void,
+    pub dB_st: i64,
+    pub dC: *mut c_void,
+    pub dC_st: i64,
+    pub dA: *mut f32,
+    pub dD: *mut f32,
+    pub d_delta_bias: *mut f32,
+    pub d_initial_state: *mut f32,
+}
+
+impl Default for Mamba1ScanPackedBwdArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Mamba1ScanStepSlotsArgs {
+    pub batch: i32,
+    pub dim: i32,
+    pub dstate: i32,
+    pub io_dtype: i32,
+    pub delta_softplus: i32,
+    pub u: *const c_void,
+    pub u_sb: i64,
+    pub delta: *const c_void,
+    pub delta_sb: i64,
+    pub A: *const f32,
+    pub B: *const c_void,
+    pub B_sb: i64,
+    pub C: *const c_void,
+    pub C_sb: i64,
+    pub D: *const f32,
+    pub z: *const c_void,
+    pub z_sb: i64,
+    pub delta_bias: *const f32,
+    pub state: *mut f32,
+    pub nslots: i64,
+    pub slots: *const i32,
+    pub y: *mut c_void,
+    pub y_sb: i64,
+}
+
+impl Default for Mamba1ScanStepSlotsArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct MambaLayernormArgs {
+    pub rows: i64,
+    pub cols: i32,
+    pub io_dtype: i32,
+    pub eps: f32,
+    pub x: *const c_void,
+    pub x_sr: i64,
+    pub weight: *const f32,
+    pub bias: *const f32,
+    pub y: *mut c_void,
+    pub y_sr: i64,
+    pub mean: *mut f32,
+    pub rstd: *mut f32,
+}
+
+impl Default for MambaLayernormArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct MambaLayernormBwdArgs {
+    pub rows: i64,
+    pub cols: i32,
+    pub io_dtype: i32,
+    pub x: *const c_void,
+    pub x_sr: i64,
+    pub dy: *const c_void,
+    pub dy_sr: i64,
+    pub weight: *const f32,
+    pub mean: *const f32,
+    pub rstd: *const f32,
+    pub dx: *mut c_void,
+    pub dx_sr: i64,
+    pub dweight: *mut f32,
+    pub dbias: *mut f32,
+}
+
+impl Default for MambaLayernormBwdArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct MambaDropoutArgs {
+    pub rows: i64,
+    pub cols: i64,
+    pub io_dtype: i32,
+    pub p: f64,
+    pub x: *const c_void,
+    pub x_sr: i64,
+    pub residual: *const c_void,
+    pub residual_sr: i64,
+    pub out: *mut c_void,
+    pub out_sr: i64,
+    pub rng: *const i64,
+    pub offset: i64,
+}
+
+impl Default for MambaDropoutArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
 extern "C" {
     pub fn mamba_last_error() -> *const c_char;
     pub fn mamba_version() -> *const c_char;
@@ -874,4 +1122,17 @@ extern "C" {
     pub fn mamba_rmsnorm(args: *const MambaRmsnormArgs, stream: MambaStream) -> c_int;
     pub fn mamba2_conv_fwd(args: *const Mamba2ConvArgs, stream: MambaStream) -> c_int;
     pub fn mamba2_gated_rmsnorm(args: *const Mamba2GatedNormArgs, stream: MambaStream) -> c_int;
+    pub fn mamba_conv1d_packed_fwd(args: *const MambaConv1dPackedArgs, stream: MambaStream) -> c_int;
+    pub fn mamba_conv1d_packed_bwd_workspace_size(args: *const MambaConv1dPackedArgs) -> usize;
+    pub fn mamba_conv1d_packed_bwd(args: *const MambaConv1dPackedArgs, workspace: *mut c_void, workspace_bytes: usize, stream: MambaStream) -> c_int;
+    pub fn mamba_conv1d_step_slots(args: *const MambaConv1dStepSlotsArgs, stream: MambaStream) -> c_int;
+    pub fn mamba1_scan_packed_workspace_size(args: *const Mamba1ScanPackedArgs) -> usize;
+    pub fn mamba1_scan_packed_fwd(args: *const Mamba1ScanPackedArgs, workspace: *mut c_void, workspace_bytes: usize, stream: MambaStream) -> c_int;
+    pub fn mamba1_scan_packed_bwd_workspace_size(args: *const Mamba1ScanPackedBwdArgs) -> usize;
+    pub fn mamba1_scan_packed_bwd(args: *const Mamba1ScanPackedBwdArgs, workspace: *mut c_void, workspace_bytes: usize, stream: MambaStream) -> c_int;
+    pub fn mamba1_scan_step_slots(args: *const Mamba1ScanStepSlotsArgs, stream: MambaStream) -> c_int;
+    pub fn mamba_layernorm_fwd(args: *const MambaLayernormArgs, stream: MambaStream) -> c_int;
+    pub fn mamba_layernorm_bwd_workspace_size(args: *const MambaLayernormBwdArgs) -> usize;
+    pub fn mamba_layernorm_bwd(args: *const MambaLayernormBwdArgs, workspace: *mut c_void, workspace_bytes: usize, stream: MambaStream) -> c_int;
+    pub fn mamba_dropout(args: *const MambaDropoutArgs, stream: MambaStream) -> c_int;
 }

@@ -18,13 +18,23 @@
 // chunk's end is carried: scan_pk_state finds the state a chunk leaves behind
 // when it starts from zero (or from the sequence's own start) and the sum of d
 // over it, scan_pk_carry walks the chunks, h <- exp(A sum d) h + own, and
-// scan_pk_out scans again from there.  In the backward the gradient of the state
-// is carried the same way from the last chunk to the first.
+// scan_pk_out scans again from there.
+//
+// Backward: scan_pk_state_bwd finds both carries of a chunk on one set of exps
+// (the gradient of the state that enters it is sum_t P_t C_t e_t, P_t the product
+// of the decays up to row t, so it walks forwards too) and keeps the state at
+// every 8th row; scan_pk_bwd then takes 8 rows at a time from the last to the
+// first, finds their states and decays again in registers and walks back over
+// them.  dB and dC are sums over channels: over a wave's by lane exchanges, over
+// the workgroup's in LDS, over the workgroups in scan_pk_join_bc; every sum is in a
+// fixed order.
 //
 // A workgroup of 256 threads holds CPB = 1024 / NP channels, NP = the states
 // padded to 16, 32 or 64; a channel is spread over NS = NP / 4 lanes with 4 states
-// each.  Tiles of NP rows are staged through LDS as f32 with the element-wise
-// work (softplus, d u) done once per element.
+// each.  Tiles of 16 rows are staged through LDS as f32 with the element-wise
+// work (softplus, d u, the gate) done once per element; rows past a tile's end
+// and channels past D are staged as zeros, which are steps that change nothing.
+// The next tile's rows are loaded while a tile is scanned.
 #include <algorithm>
 
 #include "pack.h"
@@ -51,10 +61,13 @@ struct ScanPk {
     // leaves it), the sum of d [nchunk][D], and the state that its last sequence
     // began from [nchunk][D][NP] (the cache's slot may be written meanwhile)
     float* E; float* sumd; float* h0c;
+    int32_t* ends;                  // per chunk: kIn | kOut | kThrough
     // backward
     const void* dy; int64_t dy_st;
     const float* h0; const float* dhT;
     float* G;                       // [nchunk][D][NP]: gradient of the state that enters a chunk
+    float* ckh; float* ckd;         // [rows / kSub + 1][D][NP], [rows / kSub + 1][D]: the state at every
+                                    // kSub rows of a sequence's part of a chunk, from zero, and sum of d
     float* pA; float* pD; float* pb;  // [nchunk][D][NP], [nchunk][D] x 2: partial dA, dD, dbias
     float* pBC;                     // [channel blocks][rows][2][NP]: partial dB, dC
     void* du; int64_t du_st;
@@ -91,32 +104,78 @@ __device__ __forceinline__ float group_sum_all(float v) {
     return v;
 }
 
+constexpr int kTile = 16;  // rows of a tile
+
 template <int NP>
 struct ScanShape {
-    static constexpr int NS = NP / 4, CPB = 256 / NS, TT = NP;  // TT CPB = 1024: four elements a thread
+    static constexpr int NS = NP / 4, CPB = 256 / NS, EV = kTile * CPB / 256;  // EV elements a thread
 };
 
-// The element-wise mapping: row tid / (CPB / 4) of the tile, 4 channels from
-// 4 (tid % (CPB / 4)).  Channels past D are staged as zeros (with A = 0 their
-// states stay 0), so that sums over a wave's channels need no mask.
+// V (1, 2 or 4) consecutive elements of a row as they lie in memory, so that a
+// load may stay in flight until they are used.
+template <typename T, int V>
+struct Elems {
+    static constexpr int W = (V * (int)sizeof(T) + 3) / 4;
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const T* p, int n) {
+        if (n >= V) {
+            if constexpr (V * sizeof(T) == 2) w[0] = *p;
+            else __builtin_memcpy(w, p, V * sizeof(T));
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i] = 0u;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < n) {
+                    if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
+                    else w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
+                }
+        }
+    }
+    __device__ __forceinline__ void get(float (&o)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if constexpr (sizeof(T) == 4) o[i] = __uint_as_float(w[i]);
+            else o[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        }
+    }
+};
+
+// The element-wise mapping: row tid / (CPB / EV) of the tile, EV channels from
+// EV (tid % (CPB / EV)); with A = 0 the states of channels past D stay 0, so that
+// sums over a wave's channels need no mask.
 template <int NP>
 struct ElemMap {
-    int row, c4;
+    int row, ch;
     __device__ __forceinline__ ElemMap() {
-        constexpr int W = ScanShape<NP>::CPB / 4;
+        constexpr int W = ScanShape<NP>::CPB / ScanShape<NP>::EV;
         row = threadIdx.x / W;
-        c4 = 4 * (threadIdx.x % W);
+        ch = ScanShape<NP>::EV * (threadIdx.x % W);
     }
 };
 
-// B or C of rows t0 .. into [row][NP] (zero past n rows and N states)
+// B or C of a tile: element i = tid + 256 k of [kTile rows][NP states]
 template <typename T, int NP>
-__device__ __forceinline__ void stage_bc(const void* src, int64_t st, int64_t t0, int n, int N, float (*dst)[NP]) {
-    for (int i = threadIdx.x; i < n * NP; i += 256) {
-        const int r = i / NP, k = i % NP;
-        dst[r][k] = k < N ? load_f32<T>(static_cast<const T*>(src) + (t0 + r) * st + k) : 0.f;
+struct BcTile {
+    static constexpr int K = kTile * NP / 256;
+    T v[K];
+    __device__ __forceinline__ void load(const void* src, int64_t st, int64_t t0, int n, int N) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = threadIdx.x + 256 * k, r = i / NP, c = i % NP;
+            v[k] = r < n && c < N ? static_cast<const T*>(src)[(t0 + r) * st + c] : (T)0;
+        }
     }
-}
+    __device__ __forceinline__ void stage(float (*dst)[NP]) const {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int i = threadIdx.x + 256 * k;
+            dst[i / NP][i % NP] = load_f32<T>(&v[k]);
+        }
+    }
+};
+
+enum { kIn = 1, kOut = 2, kThrough = 4 };
 
 // What chunk ck does at its two ends: the sequence that crosses into it and the
 // one that crosses out of it (-1: none).
@@ -136,44 +195,8 @@ struct ChunkEnds {
         }
         through = in && last == first;
     }
+    __device__ __forceinline__ int flags() const { return (in ? kIn : 0) | (last >= 0 ? kOut : 0) | (through ? kThrough : 0); }
 };
-
-// Rows [a, b) of one sequence from state h: the state behind them, and sum of d.
-template <typename T, int NP>
-__device__ __forceinline__ void scan_state_run(const ScanPk& p, int64_t a, int64_t b, int d0, const float (&A2)[4],
-                                               float (&h)[4], float& sumd, float2 (*s_dd)[ScanShape<NP>::CPB],
-                                               float (*s_B)[NP]) {
-    constexpr int NS = ScanShape<NP>::NS, TT = ScanShape<NP>::TT;
-    const ElemMap<NP> m;
-    const int c = threadIdx.x / NS, ng = threadIdx.x % NS;
-    const int nc = p.D - (d0 + m.c4);
-    for (int64_t t0 = a; t0 < b; t0 += TT) {
-        const int n = (int)min((int64_t)TT, b - t0);
-        if (m.row < n) {
-            float uv[4], dv[4];
-            ld_run<4, T>(static_cast<const T*>(p.u) + (t0 + m.row) * p.u_st + d0 + m.c4, nc, uv);
-            ld_run<4, T>(static_cast<const T*>(p.dl) + (t0 + m.row) * p.dl_st + d0 + m.c4, nc, dv);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (p.bias && e < nc) dv[e] += p.bias[d0 + m.c4 + e];
-                if (p.softplus) dv[e] = pk_softplus(dv[e]);
-                s_dd[m.row][m.c4 + e] = make_float2(dv[e], dv[e] * uv[e]);
-            }
-        }
-        stage_bc<T, NP>(p.B, p.B_st, t0, n, p.N, s_B);
-        __syncthreads();
-        for (int t = 0; t < n; ++t) {
-            const float2 dd = s_dd[t][c];
-            const float4 bv = *(const float4*)&s_B[t][4 * ng];
-            sumd += dd.x;
-            h[0] = __builtin_fmaf(h[0], __builtin_amdgcn_exp2f(dd.x * A2[0]), dd.y * bv.x);
-            h[1] = __builtin_fmaf(h[1], __builtin_amdgcn_exp2f(dd.x * A2[1]), dd.y * bv.y);
-            h[2] = __builtin_fmaf(h[2], __builtin_amdgcn_exp2f(dd.x * A2[2]), dd.y * bv.z);
-            h[3] = __builtin_fmaf(h[3], __builtin_amdgcn_exp2f(dd.x * A2[3]), dd.y * bv.w);
-        }
-        __syncthreads();
-    }
-}
 
 template <int NP>
 __device__ __forceinline__ void load_A2(const ScanPk& p, int d, int ng, float (&A2)[4]) {
@@ -203,55 +226,129 @@ template <int NP>
 __device__ __forceinline__ float4* plane(float* base, int64_t ck, const ScanPk& p, int d, int ng) {
     return reinterpret_cast<float4*>(base + ((ck * p.D + d) * NP + 4 * ng));
 }
+template <int NP>
+__device__ __forceinline__ void load_plane(float* base, int64_t ck, const ScanPk& p, int d, int ng, float (&h)[4]) {
+    const float4 v = d < p.D ? *plane<NP>(base, ck, p, d, ng) : make_float4(0.f, 0.f, 0.f, 0.f);
+    h[0] = v.x; h[1] = v.y; h[2] = v.z; h[3] = v.w;
+}
+template <int NP>
+__device__ __forceinline__ void store_plane(float* base, int64_t ck, const ScanPk& p, int d, int ng, const float (&h)[4]) {
+    if (d < p.D) *plane<NP>(base, ck, p, d, ng) = make_float4(h[0], h[1], h[2], h[3]);
+}
 
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_state(ScanPk p) {
-    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, TT = ScanShape<NP>::TT;
+    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = kTile;
     __shared__ float2 s_dd[TT][CPB];
     __shared__ __align__(16) float s_B[TT][NP];
     const int nblk = (p.D + CPB - 1) / CPB;
     const int64_t ck = blockIdx.x / nblk;
     const int d0 = (int)(blockIdx.x % nblk) * CPB;
     const ChunkEnds e(p, ck);
+    if (d0 == 0 && threadIdx.x == 0) p.ends[ck] = e.flags();
     if (e.last < 0) return;  // nothing crosses its end
+    const ElemMap<NP> m;
     const int c = threadIdx.x / NS, ng = threadIdx.x % NS, d = d0 + c;
-    float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, sumd = 0.f;
+    const int nc = p.D - (d0 + m.ch);
+    float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, sumd = 0.f, bias[EV];
     load_A2<NP>(p, d, ng, A2);
-    const int64_t st = p.q.begin(e.last);
+#pragma unroll
+    for (int k = 0; k < EV; ++k) bias[k] = p.bias && k < nc ? p.bias[d0 + m.ch + k] : 0.f;
+    const int64_t st = p.q.begin(e.last), a = max(st, e.c0);
     if (st >= e.c0 && p.state) {
         load_state(p.state, slot_of(p.slots, e.last, p.nslots), p, d, ng, h);
-        if (d < p.D) *plane<NP>(p.h0c, ck, p, d, ng) = make_float4(h[0], h[1], h[2], h[3]);
+        store_plane<NP>(p.h0c, ck, p, d, ng, h);
     }
-    scan_state_run<T, NP>(p, max(st, e.c0), e.c1, d0, A2, h, sumd, s_dd, s_B);
-    if (d < p.D) {
-        *plane<NP>(p.E, ck, p, d, ng) = make_float4(h[0], h[1], h[2], h[3]);
-        if (ng == 0) p.sumd[ck * p.D + d] = sumd;
+    Elems<T, EV> ru, rd;
+    BcTile<T, NP> rB;
+    auto fetch = [&](int64_t t0) {
+        const int n = (int)min((int64_t)TT, e.c1 - t0);
+        const int q = m.row < n ? nc : 0;
+        ru.load(static_cast<const T*>(p.u) + (t0 + m.row) * p.u_st + d0 + m.ch, q);
+        rd.load(static_cast<const T*>(p.dl) + (t0 + m.row) * p.dl_st + d0 + m.ch, q);
+        rB.load(p.B, p.B_st, t0, n, p.N);
+    };
+    fetch(a);
+    for (int64_t t0 = a; t0 < e.c1; t0 += TT) {
+        const int n = (int)min((int64_t)TT, e.c1 - t0);
+        float uv[EV], dv[EV];
+        ru.get(uv);
+        rd.get(dv);
+#pragma unroll
+        for (int k = 0; k < EV; ++k) {
+            dv[k] += bias[k];
+            if (p.softplus) dv[k] = pk_softplus(dv[k]);
+            if (m.row >= n) dv[k] = 0.f;
+            s_dd[m.row][m.ch + k] = make_float2(dv[k], dv[k] * uv[k]);
+        }
+        rB.stage(s_B);
+        __syncthreads();
+        if (t0 + TT < e.c1) fetch(t0 + TT);
+#pragma unroll 1
+        for (int t = 0; t < n; t += 4) {
+            float2 dd[4];
+            float4 bv[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                dd[i] = s_dd[t + i][c];
+                bv[i] = *(const float4*)&s_B[t + i][4 * ng];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sumd += dd[i].x;
+                h[0] = __builtin_fmaf(h[0], __builtin_amdgcn_exp2f(dd[i].x * A2[0]), dd[i].y * bv[i].x);
+                h[1] = __builtin_fmaf(h[1], __builtin_amdgcn_exp2f(dd[i].x * A2[1]), dd[i].y * bv[i].y);
+                h[2] = __builtin_fmaf(h[2], __builtin_amdgcn_exp2f(dd[i].x * A2[2]), dd[i].y * bv[i].z);
+                h[3] = __builtin_fmaf(h[3], __builtin_amdgcn_exp2f(dd[i].x * A2[3]), dd[i].y * bv[i].w);
+            }
+        }
+        __syncthreads();
+    }
+    store_plane<NP>(p.E, ck, p, d, ng, h);
+    if (d < p.D && ng == 0) p.sumd[ck * p.D + d] = sumd;
+}
+
+// A thread per (channel, state) walks the chunks: E[ck] <- the state that leaves
+// chunk ck, or (BACK, from the last) G[ck] <- the gradient of the state that
+// enters it.  kAhead chunks' values are loaded at a time.
+template <int NP, bool BACK>
+__device__ __forceinline__ void carry_walk(const ScanPk& p, int i) {
+    constexpr int kAhead = 8;
+    const int d = i / NP, n = i % NP;
+    if (d >= p.D) return;
+    const float A2 = n < p.N ? p.A[(int64_t)d * p.N + n] * kLog2e : 0.f;
+    float* X = (BACK ? p.G : p.E) + (int64_t)d * NP + n;
+    const int64_t pitch = (int64_t)p.D * NP, steps = p.nchunk - 1;
+    const int have = BACK ? kIn : kOut;
+    float v = 0.f;
+    for (int64_t j = 0; j < steps; j += kAhead) {
+        float own[kAhead], sd[kAhead];
+        int f[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int64_t ck = BACK ? p.nchunk - 1 - (j + k) : j + k;
+            f[k] = j + k < steps ? p.ends[ck] : 0;
+            own[k] = f[k] & have ? X[ck * pitch] : 0.f;
+            sd[k] = f[k] & kThrough ? p.sumd[ck * p.D + d] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int64_t ck = BACK ? p.nchunk - 1 - (j + k) : j + k;
+            if (!(f[k] & have)) continue;
+            v = f[k] & kThrough ? __builtin_fmaf(__builtin_amdgcn_exp2f(sd[k] * A2), v, own[k]) : own[k];
+            X[ck * pitch] = v;
+        }
     }
 }
 
-// E[ck] <- the state that leaves chunk ck.  A thread per (channel, state).
 template <int NP>
-__global__ __launch_bounds__(256) void scan_pk_carry(ScanPk p) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    const int d = i / NP, n = i % NP;
-    const bool live = d < p.D;
-    const float A2 = live && n < p.N ? p.A[(int64_t)d * p.N + n] * kLog2e : 0.f;
-    float h = 0.f;
-    for (int64_t ck = 0; ck + 1 < p.nchunk; ++ck) {
-        const ChunkEnds e(p, ck);
-        if (e.last < 0) continue;
-        if (!live) continue;
-        float* E = p.E + (ck * p.D + d) * NP + n;
-        float own = *E;
-        if (e.through) own = __builtin_fmaf(__builtin_amdgcn_exp2f(p.sumd[ck * p.D + d] * A2), h, own);
-        h = own;
-        *E = h;
-    }
+__global__ __launch_bounds__(64) void scan_pk_carry(ScanPk p) {
+    carry_walk<NP, false>(p, blockIdx.x * 64 + threadIdx.x);
 }
 
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
-    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, TT = ScanShape<NP>::TT;
+    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = kTile;
     __shared__ float2 s_dd[TT][CPB];
     __shared__ __align__(16) float s_y[TT][CPB];
     __shared__ __align__(16) float s_B[TT][NP];
@@ -262,13 +359,29 @@ __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
     const ChunkEnds e(p, ck);
     const ElemMap<NP> m;
     const int c = threadIdx.x / NS, ng = threadIdx.x % NS, d = d0 + c;
-    const int nc = p.D - (d0 + m.c4);
-    float A2[4], h[4];
+    const int nc = p.D - (d0 + m.ch);
+    float A2[4], h[4], bias[EV], Dv[EV];
     load_A2<NP>(p, d, ng, A2);
-    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < EV; ++k) {
+        bias[k] = p.bias && k < nc ? p.bias[d0 + m.ch + k] : 0.f;
+        Dv[k] = p.Dv && k < nc ? p.Dv[d0 + m.ch + k] : 0.f;
+    }
+    const float zero[EV] = {};
     auto outside = [&](int64_t a, int64_t b) {  // rows of no sequence
         for (int64_t t = a + m.row; p.fill && t < b; t += TT)
-            st_run<4, T>(static_cast<T*>(p.y) + t * p.y_st + d0 + m.c4, nc, zero);
+            st_run<EV, T>(static_cast<T*>(p.y) + t * p.y_st + d0 + m.ch, nc, zero);
+    };
+    Elems<T, EV> ru, rd, rz;
+    BcTile<T, NP> rB, rC;
+    auto fetch = [&](int64_t t0, int64_t b) {
+        const int n = (int)min((int64_t)TT, b - t0);
+        const int q = m.row < n ? nc : 0;
+        ru.load(static_cast<const T*>(p.u) + (t0 + m.row) * p.u_st + d0 + m.ch, q);
+        rd.load(static_cast<const T*>(p.dl) + (t0 + m.row) * p.dl_st + d0 + m.ch, q);
+        if (p.z) rz.load(static_cast<const T*>(p.z) + (t0 + m.row) * p.z_st + d0 + m.ch, q);
+        rB.load(p.B, p.B_st, t0, n, p.N);
+        rC.load(p.C, p.C_st, t0, n, p.N);
     };
     int64_t t = e.c0;
     for (int s = e.first; s < p.q.n && t < e.c1; ++s) {
@@ -280,51 +393,63 @@ __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
             if (t >= e.c1) break;
         }
         const int64_t b = min(en, e.c1), slot = p.state ? slot_of(p.slots, s, p.nslots) : -1;
+        fetch(t, b);
         if (e.in && t == e.c0) {  // goes on from the chunk before
-            const float4 v = d < p.D ? *plane<NP>(p.E, ck - 1, p, d, ng) : make_float4(0.f, 0.f, 0.f, 0.f);
-            h[0] = v.x; h[1] = v.y; h[2] = v.z; h[3] = v.w;
+            load_plane<NP>(p.E, ck - 1, p, d, ng, h);
         } else if (en > e.c1 && p.state) {
-            const float4 v = d < p.D ? *plane<NP>(p.h0c, ck, p, d, ng) : make_float4(0.f, 0.f, 0.f, 0.f);
-            h[0] = v.x; h[1] = v.y; h[2] = v.z; h[3] = v.w;
+            load_plane<NP>(p.h0c, ck, p, d, ng, h);
         } else {
             load_state(p.state, slot, p, d, ng, h);
         }
         for (int64_t t0 = t; t0 < b; t0 += TT) {
             const int n = (int)min((int64_t)TT, b - t0);
-            float Du[4], gate[4];
-            if (m.row < n) {
-                float uv[4], dv[4];
-                ld_run<4, T>(static_cast<const T*>(p.u) + (t0 + m.row) * p.u_st + d0 + m.c4, nc, uv);
-                ld_run<4, T>(static_cast<const T*>(p.dl) + (t0 + m.row) * p.dl_st + d0 + m.c4, nc, dv);
-                if (p.z) ld_run<4, T>(static_cast<const T*>(p.z) + (t0 + m.row) * p.z_st + d0 + m.c4, nc, gate);
+            float Du[EV], gate[EV], uv[EV], dv[EV];
+            ru.get(uv);
+            rd.get(dv);
+            if (p.z) rz.get(gate);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (p.bias && k < nc) dv[k] += p.bias[d0 + m.c4 + k];
-                    if (p.softplus) dv[k] = pk_softplus(dv[k]);
-                    s_dd[m.row][m.c4 + k] = make_float2(dv[k], dv[k] * uv[k]);
-                    Du[k] = p.Dv && k < nc ? p.Dv[d0 + m.c4 + k] * uv[k] : 0.f;
-                    gate[k] = p.z ? gate[k] * pk_sigmoid(gate[k]) : 1.f;
-                }
+            for (int k = 0; k < EV; ++k) {
+                dv[k] += bias[k];
+                if (p.softplus) dv[k] = pk_softplus(dv[k]);
+                if (m.row >= n) dv[k] = 0.f;
+                s_dd[m.row][m.ch + k] = make_float2(dv[k], dv[k] * uv[k]);
+                Du[k] = Dv[k] * uv[k];
+                gate[k] = p.z ? gate[k] * pk_sigmoid(gate[k]) : 1.f;
             }
-            stage_bc<T, NP>(p.B, p.B_st, t0, n, p.N, s_B);
-            stage_bc<T, NP>(p.C, p.C_st, t0, n, p.N, s_C);
+            rB.stage(s_B);
+            rC.stage(s_C);
             __syncthreads();
-            for (int r = 0; r < n; ++r) {
-                const float2 dd = s_dd[r][c];
-                const float4 bv = *(const float4*)&s_B[r][4 * ng], cv = *(const float4*)&s_C[r][4 * ng];
-                h[0] = __builtin_fmaf(h[0], __builtin_amdgcn_exp2f(dd.x * A2[0]), dd.y * bv.x);
-                h[1] = __builtin_fmaf(h[1], __builtin_amdgcn_exp2f(dd.x * A2[1]), dd.y * bv.y);
-                h[2] = __builtin_fmaf(h[2], __builtin_amdgcn_exp2f(dd.x * A2[2]), dd.y * bv.z);
-                h[3] = __builtin_fmaf(h[3], __builtin_amdgcn_exp2f(dd.x * A2[3]), dd.y * bv.w);
-                const float part = __builtin_fmaf(cv.w, h[3], __builtin_fmaf(cv.z, h[2], __builtin_fmaf(cv.y, h[1], cv.x * h[0])));
-                s_y[r][c] = group_sum_all<NS>(part);
+            if (t0 + TT < b) fetch(t0 + TT, b);
+#pragma unroll 1
+            for (int r = 0; r < n; r += 4) {
+                float2 dd[4];
+                float4 bv[4], cv[4];
+                float yq[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    dd[i] = s_dd[r + i][c];
+                    bv[i] = *(const float4*)&s_B[r + i][4 * ng];
+                    cv[i] = *(const float4*)&s_C[r + i][4 * ng];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    h[0] = __builtin_fmaf(h[0], __builtin_amdgcn_exp2f(dd[i].x * A2[0]), dd[i].y * bv[i].x);
+                    h[1] = __builtin_fmaf(h[1], __builtin_amdgcn_exp2f(dd[i].x * A2[1]), dd[i].y * bv[i].y);
+                    h[2] = __builtin_fmaf(h[2], __builtin_amdgcn_exp2f(dd[i].x * A2[2]), dd[i].y * bv[i].z);
+                    h[3] = __builtin_fmaf(h[3], __builtin_amdgcn_exp2f(dd[i].x * A2[3]), dd[i].y * bv[i].w);
+                    yq[i] = __builtin_fmaf(cv[i].w, h[3], __builtin_fmaf(cv[i].z, h[2], __builtin_fmaf(cv[i].y, h[1], cv[i].x * h[0])));
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) yq[i] = group_sum_all<NS>(yq[i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s_y[r + i][c] = yq[i];  // the same value from each of the channel's lanes
             }
             __syncthreads();
             if (m.row < n) {
-                const float4 yv = *(const float4*)&s_y[m.row][m.c4];
-                const float o[4] = {(yv.x + Du[0]) * gate[0], (yv.y + Du[1]) * gate[1], (yv.z + Du[2]) * gate[2],
-                                    (yv.w + Du[3]) * gate[3]};
-                st_run<4, T>(static_cast<T*>(p.y) + (t0 + m.row) * p.y_st + d0 + m.c4, nc, o);
+                float o[EV];
+#pragma unroll
+                for (int k = 0; k < EV; ++k) o[k] = (s_y[m.row][m.ch + k] + Du[k]) * gate[k];
+                st_run<EV, T>(static_cast<T*>(p.y) + (t0 + m.row) * p.y_st + d0 + m.ch, nc, o);
             }
         }
         if (b == en) store_state(p.state, slot, p, d, ng, h);
@@ -335,126 +460,172 @@ __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
 
 // ---------------------------------------------------------------- backward ---
 
-// Both carries of a chunk, each from zero: E (forward, rows of the sequence that
-// crosses its end) and G (the gradient of the state that enters it, from the rows
-// of the sequence that crosses its start): with P_t the product of the decays from
-// the chunk's start, G = sum_t P_t C_t e_t, so both walk forwards on the same exp.
+constexpr int kSub = 8;  // rows whose states and decays wait in registers
+
+// Both carries of a chunk, each from zero: E as in the forward, G the gradient of
+// the state that enters it; and the state before every kSub-th row of each
+// sequence's part (from zero where the sequence came in, with the sum of d up to
+// there: scan_pk_bwd adds what came in).  Row a + kSub i, i >= 1, of a part that
+// begins at a is kept at place (a + kSub i) / kSub: no two parts share one.
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_state_bwd(ScanPk p) {
-    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, TT = ScanShape<NP>::TT;
-    __shared__ float s_d[TT][CPB], s_du[TT][CPB], s_e[TT][CPB];
+    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = kTile;
+    __shared__ float2 s_dd[TT][CPB];
+    __shared__ float s_e[TT][CPB];
     __shared__ __align__(16) float s_B[TT][NP];
     __shared__ __align__(16) float s_C[TT][NP];
     const int nblk = (p.D + CPB - 1) / CPB;
     const int64_t ck = blockIdx.x / nblk;
     const int d0 = (int)(blockIdx.x % nblk) * CPB;
     const ChunkEnds e(p, ck);
+    if (d0 == 0 && threadIdx.x == 0) p.ends[ck] = e.flags();
     const ElemMap<NP> m;
     const int c = threadIdx.x / NS, ng = threadIdx.x % NS, d = d0 + c;
-    const int nc = p.D - (d0 + m.c4);
-    float A2[4], h[4], P[4], G[4], sumd;
+    const int nc = p.D - (d0 + m.ch);
+    float A2[4], h[4], P[4], G[4], sumd, bias[EV];
     load_A2<NP>(p, d, ng, A2);
-    auto run = [&](int64_t a, int64_t b) {
+#pragma unroll
+    for (int k = 0; k < EV; ++k) bias[k] = p.bias && k < nc ? p.bias[d0 + m.ch + k] : 0.f;
+    Elems<T, EV> ru, rd, re, rz;
+    BcTile<T, NP> rB, rC;
+    auto fetch = [&](int64_t t0, int64_t b) {
+        const int n = (int)min((int64_t)TT, b - t0);
+        const int q = m.row < n ? nc : 0;
+        ru.load(static_cast<const T*>(p.u) + (t0 + m.row) * p.u_st + d0 + m.ch, q);
+        rd.load(static_cast<const T*>(p.dl) + (t0 + m.row) * p.dl_st + d0 + m.ch, q);
+        re.load(static_cast<const T*>(p.dy) + (t0 + m.row) * p.dy_st + d0 + m.ch, q);
+        if (p.z) rz.load(static_cast<const T*>(p.z) + (t0 + m.row) * p.z_st + d0 + m.ch, q);
+        rB.load(p.B, p.B_st, t0, n, p.N);
+        rC.load(p.C, p.C_st, t0, n, p.N);
+    };
+    int64_t t = e.c0;
+    for (int s = e.first; s < p.q.n && t < e.c1; ++s) {
+        const int64_t st = p.q.begin(s), en = p.q.end(s);
+        if (en <= t) continue;
+        t = max(t, st);
+        if (t >= e.c1) break;
+        const int64_t b = min(en, e.c1);
+        const bool in = e.in && t == e.c0;
+        fetch(t, b);
+        if (in) h[0] = h[1] = h[2] = h[3] = 0.f;
+        else load_state(p.h0, s, p, d, ng, h);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             P[k] = 1.f;
             G[k] = 0.f;
         }
         sumd = 0.f;
-        for (int64_t t0 = a; t0 < b; t0 += TT) {
+        for (int64_t t0 = t; t0 < b; t0 += TT) {
             const int n = (int)min((int64_t)TT, b - t0);
-            if (m.row < n) {
-                float uv[4], dv[4], ev[4], zv[4];
-                ld_run<4, T>(static_cast<const T*>(p.u) + (t0 + m.row) * p.u_st + d0 + m.c4, nc, uv);
-                ld_run<4, T>(static_cast<const T*>(p.dl) + (t0 + m.row) * p.dl_st + d0 + m.c4, nc, dv);
-                ld_run<4, T>(static_cast<const T*>(p.dy) + (t0 + m.row) * p.dy_st + d0 + m.c4, nc, ev);
-                if (p.z) ld_run<4, T>(static_cast<const T*>(p.z) + (t0 + m.row) * p.z_st + d0 + m.c4, nc, zv);
+            float uv[EV], dv[EV], ev[EV], zv[EV];
+            ru.get(uv);
+            rd.get(dv);
+            re.get(ev);
+            if (p.z) rz.get(zv);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (p.bias && k < nc) dv[k] += p.bias[d0 + m.c4 + k];
-                    if (p.softplus) dv[k] = pk_softplus(dv[k]);
-                    if (p.z) ev[k] *= zv[k] * pk_sigmoid(zv[k]);
-                    s_d[m.row][m.c4 + k] = dv[k];
-                    s_du[m.row][m.c4 + k] = dv[k] * uv[k];
-                    s_e[m.row][m.c4 + k] = ev[k];
+            for (int k = 0; k < EV; ++k) {
+                dv[k] += bias[k];
+                if (p.softplus) dv[k] = pk_softplus(dv[k]);
+                if (p.z) ev[k] *= zv[k] * pk_sigmoid(zv[k]);
+                if (m.row >= n) dv[k] = ev[k] = 0.f;
+                s_dd[m.row][m.ch + k] = make_float2(dv[k], dv[k] * uv[k]);
+                s_e[m.row][m.ch + k] = ev[k];
+            }
+            rB.stage(s_B);
+            rC.stage(s_C);
+            __syncthreads();
+            if (t0 + TT < b) fetch(t0 + TT, b);
+#pragma unroll 1
+            for (int r0 = 0; r0 < n; r0 += 4) {
+                if (r0 % kSub == 0 && t0 + r0 > t) {
+                    const int64_t at = (t0 + r0) / kSub;
+                    store_plane<NP>(p.ckh, at, p, d, ng, h);
+                    if (ng == 0 && d < p.D) p.ckd[at * p.D + d] = sumd;
+                }
+                float2 dd[4];
+                float ee[4];
+                float4 bq[4], cq[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    dd[i] = s_dd[r0 + i][c];
+                    ee[i] = s_e[r0 + i][c];
+                    bq[i] = *(const float4*)&s_B[r0 + i][4 * ng];
+                    cq[i] = *(const float4*)&s_C[r0 + i][4 * ng];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float bv[4] = {bq[i].x, bq[i].y, bq[i].z, bq[i].w}, cv[4] = {cq[i].x, cq[i].y, cq[i].z, cq[i].w};
+                    sumd += dd[i].x;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float a = __builtin_amdgcn_exp2f(dd[i].x * A2[k]);
+                        h[k] = __builtin_fmaf(h[k], a, dd[i].y * bv[k]);
+                        P[k] *= a;
+                        G[k] = __builtin_fmaf(P[k], cv[k] * ee[i], G[k]);
+                    }
                 }
             }
-            stage_bc<T, NP>(p.B, p.B_st, t0, n, p.N, s_B);
-            stage_bc<T, NP>(p.C, p.C_st, t0, n, p.N, s_C);
             __syncthreads();
-            for (int t = 0; t < n; ++t) {
-                const float dv = s_d[t][c], du = s_du[t][c], ev = s_e[t][c];
-                const float4 bq = *(const float4*)&s_B[t][4 * ng], cq = *(const float4*)&s_C[t][4 * ng];
-                const float bv[4] = {bq.x, bq.y, bq.z, bq.w}, cv[4] = {cq.x, cq.y, cq.z, cq.w};
-                sumd += dv;
+        }
+        if (in) {
+            if (b == en && p.dhT) {  // the sequence ends here: its own gradient comes in
+                float g[4];
+                load_state(p.dhT, s, p, d, ng, g);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float a = __builtin_amdgcn_exp2f(dv * A2[k]);
-                    h[k] = __builtin_fmaf(h[k], a, du * bv[k]);
-                    P[k] *= a;
-                    G[k] = __builtin_fmaf(P[k], cv[k] * ev, G[k]);
-                }
+                for (int k = 0; k < 4; ++k) G[k] = __builtin_fmaf(P[k], g[k], G[k]);
             }
-            __syncthreads();
+            store_plane<NP>(p.G, ck, p, d, ng, G);
         }
-    };
-    if (e.in) {
-        const int64_t en = p.q.end(e.first);
-        h[0] = h[1] = h[2] = h[3] = 0.f;
-        run(e.c0, min(en, e.c1));
-        if (en <= e.c1 && p.dhT) {  // the sequence ends here: its own gradient comes in
-            float g[4];
-            load_state(p.dhT, e.first, p, d, ng, g);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) G[k] = __builtin_fmaf(P[k], g[k], G[k]);
+        if (s == e.last) {
+            store_plane<NP>(p.E, ck, p, d, ng, h);
+            if (ng == 0 && d < p.D) p.sumd[ck * p.D + d] = sumd;
         }
-        if (d < p.D) *plane<NP>(p.G, ck, p, d, ng) = make_float4(G[0], G[1], G[2], G[3]);
+        t = b;
     }
-    if (e.last >= 0) {
-        if (!e.through) {
-            load_state(p.h0, e.last, p, d, ng, h);
-            run(p.q.begin(e.last), e.c1);
-        }
-        if (d < p.D) *plane<NP>(p.E, ck, p, d, ng) = make_float4(h[0], h[1], h[2], h[3]);
-    }
-    if (e.through && d < p.D && ng == 0) p.sumd[ck * p.D + d] = sumd;
 }
 
-// blockIdx.y 0: E as in the forward; 1: G from the last chunk to the first.
 template <int NP>
-__global__ __launch_bounds__(256) void scan_pk_carry_bwd(ScanPk p) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    const int d = i / NP, n = i % NP;
-    if (d >= p.D) return;
-    const float A2 = n < p.N ? p.A[(int64_t)d * p.N + n] * kLog2e : 0.f;
-    float v = 0.f;
-    for (int64_t j = 0; j + 1 < p.nchunk; ++j) {
-        const bool fwd = blockIdx.y == 0;
-        const int64_t ck = fwd ? j : p.nchunk - 1 - j;
-        const ChunkEnds e(p, ck);
-        if (fwd ? e.last < 0 : !e.in) continue;
-        float* X = (fwd ? p.E : p.G) + (ck * p.D + d) * NP + n;
-        float own = *X;
-        if (e.through) own = __builtin_fmaf(__builtin_amdgcn_exp2f(p.sumd[ck * p.D + d] * A2), v, own);
-        v = own;
-        *X = v;
+__global__ __launch_bounds__(64) void scan_pk_carry_bwd(ScanPk p) {
+    const int i = blockIdx.x * 64 + threadIdx.x;
+    if (blockIdx.y == 0) carry_walk<NP, false>(p, i);
+    else carry_walk<NP, true>(p, i);
+}
+
+// Sums over the wave's channels (lanes ng, ng + NS, ...) of v[0..3] and w[0..3].
+// The halves and then the rows of 16 lanes are exchanged with half of the values
+// each (a swap and an add for two of them), so that row R of lanes ends with
+// element R % 2 of v (R < 2) or w in x0, and 2 + R % 2 in x1.
+template <int NS>
+__device__ __forceinline__ void channel_sums(const float (&v)[4], const float (&w)[4], float& x0, float& x1) {
+    float y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[k]), __float_as_uint(w[k]), false, false);
+        y[k] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(y[0]), __float_as_uint(y[1]), false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(y[2]), __float_as_uint(y[3]), false, false);
+    x0 = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    x1 = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+    if (NS <= 8) {
+        x0 += pk_dpp<0x128>(x0);  // row_ror:8
+        x1 += pk_dpp<0x128>(x1);
+    }
+    if (NS <= 4) {
+        x0 += pk_dpp<0x124>(x0);  // row_ror:4
+        x1 += pk_dpp<0x124>(x1);
     }
 }
 
-constexpr int kSub = 8;    // rows whose states and decays wait in registers
-constexpr int kBwdChunk = 64;
-
-// The chunk itself: forwards over its rows once for the state at every kSub rows,
-// then backwards, kSub rows at a time, the states in between found again.  The
-// staged d, d u and e of a row are overwritten by its s, sum_n g a h A and sum_n C h.
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
-    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, TT = ScanShape<NP>::TT, Q = kBwdChunk;
-    constexpr int NK = Q / kSub;
-    __shared__ __align__(16) float s_d[Q][CPB], s_du[Q][CPB], s_e[Q][CPB];
-    __shared__ __align__(16) float s_B[Q][NP];
-    __shared__ __align__(16) float s_C[Q][NP];
-    __shared__ __align__(16) float s_bc[4][kSub][2 * NP];
+    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = kTile;
+    __shared__ __align__(16) float2 s_dd[TT][CPB];
+    __shared__ __align__(16) float s_e[TT][CPB];
+    __shared__ __align__(16) float s_sB[TT][CPB], s_sA[TT][CPB], s_sC[TT][CPB];
+    __shared__ __align__(16) float s_B[TT][NP];
+    __shared__ __align__(16) float s_C[TT][NP];
+    __shared__ __align__(16) float s_bc[4][TT][2 * NP];
     const int nblk = (p.D + CPB - 1) / CPB;
     const int64_t ck = blockIdx.x / nblk;
     const int blk = (int)(blockIdx.x % nblk), d0 = blk * CPB;
@@ -462,25 +633,40 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
     const ElemMap<NP> m;
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int c = threadIdx.x / NS, ng = threadIdx.x % NS, d = d0 + c;
-    const int nc = p.D - (d0 + m.c4);
+    const int nc = p.D - (d0 + m.ch);
+    // where this lane's channel sums go: element lane / 16 % 2 (and + 2) of B's (C's) four states
+    const int bc_at = (lane >> 5) * NP + 4 * ng + ((lane >> 4) & 1);
+    const bool bc_lane = (lane & 15) < NS;
     float A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f};
     load_A2<NP>(p, d, ng, A2);
-    float Dv[4], bias[4], dD[4], db[4];
+    float Dv[EV], bias[EV], dD[EV], db[EV];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        Dv[k] = p.Dv && k < nc ? p.Dv[d0 + m.c4 + k] : 0.f;
-        bias[k] = p.bias && k < nc ? p.bias[d0 + m.c4 + k] : 0.f;
+    for (int k = 0; k < EV; ++k) {
+        Dv[k] = p.Dv && k < nc ? p.Dv[d0 + m.ch + k] : 0.f;
+        bias[k] = p.bias && k < nc ? p.bias[d0 + m.ch + k] : 0.f;
         dD[k] = db[k] = 0.f;
     }
-    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    const float zero[EV] = {};
     float* pBC = p.pBC + (int64_t)blk * p.rows * 2 * NP;
     auto outside = [&](int64_t a, int64_t b) {
         for (int64_t t = a + m.row; t < b; t += TT) {
-            st_run<4, T>(static_cast<T*>(p.du) + t * p.du_st + d0 + m.c4, nc, zero);
-            st_run<4, T>(static_cast<T*>(p.ddl) + t * p.ddl_st + d0 + m.c4, nc, zero);
-            if (p.z) st_run<4, T>(static_cast<T*>(p.dz) + t * p.dz_st + d0 + m.c4, nc, zero);
+            st_run<EV, T>(static_cast<T*>(p.du) + t * p.du_st + d0 + m.ch, nc, zero);
+            st_run<EV, T>(static_cast<T*>(p.ddl) + t * p.ddl_st + d0 + m.ch, nc, zero);
+            if (p.z) st_run<EV, T>(static_cast<T*>(p.dz) + t * p.dz_st + d0 + m.ch, nc, zero);
         }
         for (int64_t i = a * 2 * NP + threadIdx.x; i < b * 2 * NP; i += 256) pBC[i] = 0.f;
+    };
+    Elems<T, EV> ru, rd, re, rz;
+    BcTile<T, NP> rB, rC;
+    auto fetch = [&](int64_t t0, int64_t b) {
+        const int n = (int)min((int64_t)TT, b - t0);
+        const int q = m.row < n ? nc : 0;
+        ru.load(static_cast<const T*>(p.u) + (t0 + m.row) * p.u_st + d0 + m.ch, q);
+        rd.load(static_cast<const T*>(p.dl) + (t0 + m.row) * p.dl_st + d0 + m.ch, q);
+        re.load(static_cast<const T*>(p.dy) + (t0 + m.row) * p.dy_st + d0 + m.ch, q);
+        if (p.z) rz.load(static_cast<const T*>(p.z) + (t0 + m.row) * p.z_st + d0 + m.ch, q);
+        rB.load(p.B, p.B_st, t0, n, p.N);
+        rC.load(p.C, p.C_st, t0, n, p.N);
     };
     int64_t t = e.c0;
     for (int s = e.first; s < p.q.n && t < e.c1; ++s) {
@@ -492,173 +678,142 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
             if (t >= e.c1) break;
         }
         const int64_t b = min(en, e.c1);
-        const int n = (int)(b - t);
-        // ---- the run's elements
-        for (int r = m.row; r < n; r += TT) {
-            float uv[4], dv[4], ev[4], zv[4];
-            ld_run<4, T>(static_cast<const T*>(p.u) + (t + r) * p.u_st + d0 + m.c4, nc, uv);
-            ld_run<4, T>(static_cast<const T*>(p.dl) + (t + r) * p.dl_st + d0 + m.c4, nc, dv);
-            ld_run<4, T>(static_cast<const T*>(p.dy) + (t + r) * p.dy_st + d0 + m.c4, nc, ev);
-            if (p.z) ld_run<4, T>(static_cast<const T*>(p.z) + (t + r) * p.z_st + d0 + m.c4, nc, zv);
+        const bool in = e.in && t == e.c0;
+        const int len = (int)(b - t), tiles = (len + TT - 1) / TT;
+        fetch(t + (int64_t)(tiles - 1) * TT, b);
+        float h0[4], g[4], hn[4], dn = 0.f;  // hn, dn: the next part's kept state and sum of d
+        if (in) load_plane<NP>(p.E, ck - 1, p, d, ng, h0);
+        else load_state(p.h0, s, p, d, ng, h0);
+        if (en > e.c1) load_plane<NP>(p.G, ck + 1, p, d, ng, g);
+        else load_state(p.dhT, s, p, d, ng, g);
+        auto kept = [&](int q) {  // before row kSub q of the run
+            if (q <= 0) return;
+            const int64_t at = (t + q * kSub) / kSub;
+            load_plane<NP>(p.ckh, at, p, d, ng, hn);
+            if (in) dn = d < p.D ? p.ckd[at * p.D + d] : 0.f;
+        };
+        kept((len - 1) / kSub);
+        for (int tl = tiles - 1; tl >= 0; --tl) {
+            const int64_t t0 = t + (int64_t)tl * TT;
+            const int n = (int)min((int64_t)TT, b - t0);
+            float uv[EV], dv[EV], yv[EV], zv[EV];
+            ru.get(uv);
+            rd.get(dv);
+            re.get(yv);
+            if (p.z) rz.get(zv);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < EV; ++k) {
                 dv[k] += bias[k];
-                if (p.softplus) dv[k] = pk_softplus(dv[k]);
-                if (p.z) ev[k] *= zv[k] * pk_sigmoid(zv[k]);
-                s_d[r][m.c4 + k] = dv[k];
-                s_du[r][m.c4 + k] = dv[k] * uv[k];
-                s_e[r][m.c4 + k] = ev[k];
+                float dt = p.softplus ? pk_softplus(dv[k]) : dv[k];
+                float ev = p.z ? yv[k] * (zv[k] * pk_sigmoid(zv[k])) : yv[k];
+                if (m.row >= n) dt = ev = 0.f;
+                s_dd[m.row][m.ch + k] = make_float2(dt, dt * uv[k]);
+                s_e[m.row][m.ch + k] = ev;
             }
-        }
-        stage_bc<T, NP>(p.B, p.B_st, t, n, p.N, s_B);
-        stage_bc<T, NP>(p.C, p.C_st, t, n, p.N, s_C);
-        float h[4], g[4];
-        if (e.in && t == e.c0) {  // goes on from the chunk before
-            const float4 v = d < p.D ? *plane<NP>(p.E, ck - 1, p, d, ng) : make_float4(0.f, 0.f, 0.f, 0.f);
-            h[0] = v.x; h[1] = v.y; h[2] = v.z; h[3] = v.w;
-        } else {
-            load_state(p.h0, s, p, d, ng, h);
-        }
-        if (en > e.c1) {
-            const float4 v = d < p.D ? *plane<NP>(p.G, ck + 1, p, d, ng) : make_float4(0.f, 0.f, 0.f, 0.f);
-            g[0] = v.x; g[1] = v.y; g[2] = v.z; g[3] = v.w;
-        } else {
-            load_state(p.dhT, s, p, d, ng, g);
-        }
-        __syncthreads();
-        // ---- forwards: the state at every kSub rows
-        float ck_h[NK][4];
+            rB.stage(s_B);
+            rC.stage(s_C);
+            __syncthreads();
+            if (tl > 0) fetch(t0 - TT, b);
+#pragma unroll 1
+            for (int r0 = (n - 1) / kSub * kSub; r0 >= 0; r0 -= kSub) {
+                const int q = tl * (TT / kSub) + r0 / kSub;
+                float hs[kSub + 1][4], as[kSub][4];
+                // the state before row r0: the run's own start, or the kept one and what came in
 #pragma unroll
-        for (int j = 0; j < NK; ++j) {
+                for (int k = 0; k < 4; ++k)
+                    hs[0][k] = q == 0 ? h0[k] : in ? __builtin_fmaf(__builtin_amdgcn_exp2f(dn * A2[k]), h0[k], hn[k]) : hn[k];
+                kept(q - 1);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) ck_h[j][k] = h[k];
-            if ((j + 1) * kSub < n)
-                for (int r = j * kSub; r < (j + 1) * kSub; ++r) {
-                    const float dv = s_d[r][c], du = s_du[r][c];
-                    const float4 bq = *(const float4*)&s_B[r][4 * ng];
+                for (int i = 0; i < kSub; ++i) {
+                    const float2 dd = s_dd[r0 + i][c];
+                    const float4 bq = *(const float4*)&s_B[r0 + i][4 * ng];
                     const float bv[4] = {bq.x, bq.y, bq.z, bq.w};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) h[k] = __builtin_fmaf(h[k], __builtin_amdgcn_exp2f(dv * A2[k]), du * bv[k]);
-                }
-        }
-        // ---- backwards
-#pragma unroll
-        for (int j = NK - 1; j >= 0; --j) {
-            if (j * kSub >= n) continue;
-            float hs[kSub + 1][4], as[kSub][4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) hs[0][k] = ck_h[j][k];
-#pragma unroll
-            for (int i = 0; i < kSub; ++i) {
-                const int r = j * kSub + i;
-                const bool in = r < n;
-                const float dv = in ? s_d[r][c] : 0.f, du = in ? s_du[r][c] : 0.f;
-                const float4 bq = *(const float4*)&s_B[r][4 * ng];
-                const float bv[4] = {bq.x, bq.y, bq.z, bq.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    as[i][k] = __builtin_amdgcn_exp2f(dv * A2[k]);
-                    hs[i + 1][k] = __builtin_fmaf(hs[i][k], as[i][k], in ? du * bv[k] : 0.f);
-                }
-            }
-#pragma unroll
-            for (int i = kSub - 1; i >= 0; --i) {
-                const int r = j * kSub + i;
-                if (r >= n) continue;
-                const float dv = s_d[r][c], du = s_du[r][c], ev = s_e[r][c];
-                const float4 bq = *(const float4*)&s_B[r][4 * ng], cq = *(const float4*)&s_C[r][4 * ng];
-                const float bv[4] = {bq.x, bq.y, bq.z, bq.w}, cv[4] = {cq.x, cq.y, cq.z, cq.w};
-                float sB = 0.f, sA = 0.f, sC = 0.f, vb[4], vc[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float gk = __builtin_fmaf(cv[k], ev, g[k]);
-                    vb[k] = gk * du;
-                    vc[k] = hs[i + 1][k] * ev;
-                    sB = __builtin_fmaf(gk, bv[k], sB);
-                    sC = __builtin_fmaf(cv[k], hs[i + 1][k], sC);
-                    g[k] = gk * as[i][k];
-                    const float x = g[k] * hs[i][k];
-                    sA = __builtin_fmaf(x, A2[k], sA);
-                    dA[k] = __builtin_fmaf(x, dv, dA[k]);
-                }
-                sB = group_sum_all<NS>(sB);
-                sA = group_sum_all<NS>(sA);
-                sC = group_sum_all<NS>(sC);
-                if (ng == 0) {
-                    s_d[r][c] = sB;
-                    s_du[r][c] = sA * (1.f / kLog2e);
-                    s_e[r][c] = sC;
-                }
-                // over the wave's channels: lanes ng, ng + NS, ...
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-#pragma unroll
-                    for (int o = NS; o < 64; o <<= 1) {
-                        vb[k] += __shfl_xor(vb[k], o, 64);
-                        vc[k] += __shfl_xor(vc[k], o, 64);
+                    for (int k = 0; k < 4; ++k) {
+                        as[i][k] = __builtin_amdgcn_exp2f(dd.x * A2[k]);
+                        hs[i + 1][k] = __builtin_fmaf(hs[i][k], as[i][k], dd.y * bv[k]);
                     }
                 }
-                if (lane < NS) {
-                    *(float4*)&s_bc[wave][i][4 * ng] = make_float4(vb[0], vb[1], vb[2], vb[3]);
-                    *(float4*)&s_bc[wave][i][NP + 4 * ng] = make_float4(vc[0], vc[1], vc[2], vc[3]);
-                }
-            }
-            __syncthreads();
-            for (int i = threadIdx.x; i < kSub * 2 * NP; i += 256) {
-                const int r = i / (2 * NP), k = i % (2 * NP);
-                if (j * kSub + r < n)
-                    pBC[(t + j * kSub + r) * 2 * NP + k] =
-                        (s_bc[0][r][k] + s_bc[1][r][k]) + (s_bc[2][r][k] + s_bc[3][r][k]);
-            }
-            __syncthreads();
-        }
-        // ---- the gradients of the elements
-        for (int r = m.row; r < n; r += TT) {
-            float uv[4], dv[4], yv[4], zv[4], o1[4], o2[4], o3[4];
-            ld_run<4, T>(static_cast<const T*>(p.u) + (t + r) * p.u_st + d0 + m.c4, nc, uv);
-            ld_run<4, T>(static_cast<const T*>(p.dl) + (t + r) * p.dl_st + d0 + m.c4, nc, dv);
-            ld_run<4, T>(static_cast<const T*>(p.dy) + (t + r) * p.dy_st + d0 + m.c4, nc, yv);
-            if (p.z) ld_run<4, T>(static_cast<const T*>(p.z) + (t + r) * p.z_st + d0 + m.c4, nc, zv);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float raw = dv[k] + bias[k];
-                const float dt = p.softplus ? pk_softplus(raw) : raw;
-                const float sB = s_d[r][m.c4 + k], sA = s_du[r][m.c4 + k], sC = s_e[r][m.c4 + k];
-                float ev = yv[k];
-                if (p.z) {
-                    const float sg = pk_sigmoid(zv[k]);
-                    ev *= zv[k] * sg;
-                    o3[k] = yv[k] * __builtin_fmaf(Dv[k], uv[k], sC) * (sg * (1.f + zv[k] * (1.f - sg)));
+                for (int i = kSub - 1; i >= 0; --i) {
+                    const float2 dd = s_dd[r0 + i][c];
+                    const float ev = s_e[r0 + i][c];
+                    const float4 bq = *(const float4*)&s_B[r0 + i][4 * ng], cq = *(const float4*)&s_C[r0 + i][4 * ng];
+                    const float bv[4] = {bq.x, bq.y, bq.z, bq.w}, cv[4] = {cq.x, cq.y, cq.z, cq.w};
+                    float sB = 0.f, sA = 0.f, sC = 0.f, vb[4], vc[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float gk = __builtin_fmaf(cv[k], ev, g[k]);
+                        vb[k] = gk * dd.y;
+                        vc[k] = hs[i + 1][k] * ev;
+                        sB = __builtin_fmaf(gk, bv[k], sB);
+                        sC = __builtin_fmaf(cv[k], hs[i + 1][k], sC);
+                        g[k] = gk * as[i][k];
+                        const float x = g[k] * hs[i][k];
+                        sA = __builtin_fmaf(x, A2[k], sA);
+                        dA[k] = __builtin_fmaf(x, dd.x, dA[k]);
+                    }
+                    sB = group_sum_all<NS>(sB);
+                    sA = group_sum_all<NS>(sA);
+                    sC = group_sum_all<NS>(sC);
+                    float x0, x1;
+                    channel_sums<NS>(vb, vc, x0, x1);
+                    if (ng == 0) {
+                        s_sB[r0 + i][c] = sB;
+                        s_sA[r0 + i][c] = sA;
+                        s_sC[r0 + i][c] = sC;
+                    }
+                    if (bc_lane) {
+                        s_bc[wave][r0 + i][bc_at] = x0;
+                        s_bc[wave][r0 + i][bc_at + 2] = x1;
+                    }
                 }
-                o1[k] = __builtin_fmaf(sB, dt, Dv[k] * ev);
-                o2[k] = __builtin_fmaf(sB, uv[k], sA);
-                if (p.softplus) o2[k] *= pk_sigmoid(raw);
-                dD[k] = __builtin_fmaf(ev, uv[k], dD[k]);
-                db[k] += o2[k];
             }
-            st_run<4, T>(static_cast<T*>(p.du) + (t + r) * p.du_st + d0 + m.c4, nc, o1);
-            st_run<4, T>(static_cast<T*>(p.ddl) + (t + r) * p.ddl_st + d0 + m.c4, nc, o2);
-            if (p.z) st_run<4, T>(static_cast<T*>(p.dz) + (t + r) * p.dz_st + d0 + m.c4, nc, o3);
+            __syncthreads();
+            // ---- the tile's dB and dC over the workgroup, and the gradients of its elements
+            for (int i = threadIdx.x; i < n * 2 * NP; i += 256) {
+                const int r = i / (2 * NP), k = i % (2 * NP);
+                pBC[t0 * 2 * NP + i] = (s_bc[0][r][k] + s_bc[1][r][k]) + (s_bc[2][r][k] + s_bc[3][r][k]);
+            }
+            if (m.row < n) {
+                float o1[EV], o2[EV], o3[EV];
+#pragma unroll
+                for (int k = 0; k < EV; ++k) {
+                    const float sB = s_sB[m.row][m.ch + k], sA = s_sA[m.row][m.ch + k] * (1.f / kLog2e), sC = s_sC[m.row][m.ch + k];
+                    const float dt = s_dd[m.row][m.ch + k].x, ev = s_e[m.row][m.ch + k];
+                    if (p.z) {
+                        const float sg = pk_sigmoid(zv[k]);
+                        o3[k] = yv[k] * __builtin_fmaf(Dv[k], uv[k], sC) * (sg * (1.f + zv[k] * (1.f - sg)));
+                    }
+                    o1[k] = __builtin_fmaf(sB, dt, Dv[k] * ev);
+                    o2[k] = __builtin_fmaf(sB, uv[k], sA);
+                    if (p.softplus) o2[k] *= pk_sigmoid(dv[k]);
+                    dD[k] = __builtin_fmaf(ev, uv[k], dD[k]);
+                    db[k] += o2[k];
+                }
+                st_run<EV, T>(static_cast<T*>(p.du) + (t0 + m.row) * p.du_st + d0 + m.ch, nc, o1);
+                st_run<EV, T>(static_cast<T*>(p.ddl) + (t0 + m.row) * p.ddl_st + d0 + m.ch, nc, o2);
+                if (p.z) st_run<EV, T>(static_cast<T*>(p.dz) + (t0 + m.row) * p.dz_st + d0 + m.ch, nc, o3);
+            }
         }
         if (t == st) store_state(p.dh0, s, p, d, ng, g);
         t = b;
-        __syncthreads();
     }
     outside(t, e.c1);
     // ---- the chunk's share of dA, dD and dbias
-    if (d < p.D) *plane<NP>(p.pA, ck, p, d, ng) = make_float4(dA[0], dA[1], dA[2], dA[3]);
+    store_plane<NP>(p.pA, ck, p, d, ng, dA);
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        s_d[m.row][m.c4 + k] = dD[k];
-        s_du[m.row][m.c4 + k] = db[k];
+    for (int k = 0; k < EV; ++k) {
+        s_sB[m.row][m.ch + k] = dD[k];
+        s_sA[m.row][m.ch + k] = db[k];
     }
     __syncthreads();
     if (threadIdx.x < CPB && d0 + (int)threadIdx.x < p.D) {
         float x = 0.f, y = 0.f;
         for (int r = 0; r < TT; ++r) {
-            x += s_d[r][threadIdx.x];
-            y += s_du[r][threadIdx.x];
+            x += s_sB[r][threadIdx.x];
+            y += s_sA[r][threadIdx.x];
         }
         p.pD[ck * p.D + d0 + threadIdx.x] = x;
         p.pb[ck * p.D + d0 + threadIdx.x] = y;
@@ -787,7 +942,7 @@ static void scan_pk_fwd_plan(ScanPk& p) {
     p.nchunk = (p.rows + p.chunk - 1) / p.chunk;
 }
 static void scan_pk_bwd_plan(ScanPk& p) {
-    p.chunk = kBwdChunk;
+    p.chunk = 128;
     p.nchunk = (p.rows + p.chunk - 1) / p.chunk;
 }
 // a grid's threads stay below 2^32
@@ -805,7 +960,7 @@ static void scan_pk_fwd_launch(const ScanPk& p, hipStream_t s) {
     const uint32_t nblk = ceil_div(p.D, ScanShape<NP>::CPB);
     if (p.nchunk > 1) {
         hipLaunchKernelGGL((scan_pk_state<T, NP>), dim3(nblk * (uint32_t)(p.nchunk - 1)), dim3(256), 0, s, p);
-        hipLaunchKernelGGL((scan_pk_carry<NP>), dim3(ceil_div(p.D * NP, 256)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((scan_pk_carry<NP>), dim3(ceil_div(p.D * NP, 64)), dim3(64), 0, s, p);
     }
     hipLaunchKernelGGL((scan_pk_out<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
 }
@@ -813,11 +968,9 @@ static void scan_pk_fwd_launch(const ScanPk& p, hipStream_t s) {
 template <typename T, int NP>
 static void scan_pk_bwd_launch(const ScanPk& p, hipStream_t s) {
     const uint32_t nblk = ceil_div(p.D, ScanShape<NP>::CPB);
-    if (p.nchunk > 1) {
-        hipLaunchKernelGGL((scan_pk_state_bwd<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
-        hipLaunchKernelGGL((scan_pk_carry_bwd<NP>), dim3(ceil_div(p.D * NP, 256), 2), dim3(256), 0, s, p);
-    }
     if (p.rows) {
+        hipLaunchKernelGGL((scan_pk_state_bwd<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
+        if (p.nchunk > 1) hipLaunchKernelGGL((scan_pk_carry_bwd<NP>), dim3(ceil_div(p.D * NP, 64), 2), dim3(64), 0, s, p);
         hipLaunchKernelGGL((scan_pk_bwd<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
         const int64_t n = p.rows * 2 * NP;
         hipLaunchKernelGGL((scan_pk_join_bc<T, NP>), dim3((uint32_t)std::min<int64_t>((n + 255) / 256, 8192)), dim3(256), 0, s, p,
@@ -840,13 +993,40 @@ static void scan_pk_bwd_launch(const ScanPk& p, hipStream_t s) {
         }                                                \
     } while (0)
 
-// floats of the forward's planes
-static size_t scan_pk_fwd_floats(const ScanPk& p) {
-    return p.nchunk > 1 ? (size_t)p.nchunk * p.D * (2 * scan_np(p.N) + 1) : 0;
+// Workspaces: planes of floats, each of a multiple of four (16 bytes).
+struct ScanPlanes {
+    float* base; size_t used = 0;
+    explicit ScanPlanes(void* ws) : base(static_cast<float*>(ws)) {}
+    float* take(size_t n) {
+        float* at = base ? base + used : nullptr;
+        used += (n + 3) / 4 * 4;
+        return at;
+    }
+};
+static size_t scan_pk_fwd_planes(ScanPk& p, void* ws) {
+    if (p.nchunk <= 1) return 0;
+    ScanPlanes w(ws);
+    const size_t nd = (size_t)p.nchunk * p.D, np = scan_np(p.N);
+    p.E = w.take(nd * np);
+    p.h0c = w.take(nd * np);
+    p.sumd = w.take(nd);
+    p.ends = reinterpret_cast<int32_t*>(w.take(p.nchunk));
+    return w.used * 4;
 }
-static size_t scan_pk_bwd_floats(const ScanPk& p) {
-    const size_t np = scan_np(p.N), nblk = ceil_div(p.D, 1024 / (int)np);
-    return (size_t)p.nchunk * p.D * (3 * np + 3) + nblk * (size_t)p.rows * 2 * np;
+static size_t scan_pk_bwd_planes(ScanPk& p, void* ws) {
+    ScanPlanes w(ws);
+    const size_t nd = (size_t)p.nchunk * p.D, np = scan_np(p.N), nk = (size_t)p.rows / kSub + 1;
+    p.E = w.take(nd * np);
+    p.G = w.take(nd * np);
+    p.pA = w.take(nd * np);
+    p.sumd = w.take(nd);
+    p.pD = w.take(nd);
+    p.pb = w.take(nd);
+    p.ends = reinterpret_cast<int32_t*>(w.take(p.nchunk));
+    p.ckh = w.take(nk * p.D * np);
+    p.ckd = w.take(nk * p.D);
+    p.pBC = w.take((size_t)ceil_div(p.D, 1024 / (int)np) * p.rows * 2 * np);
+    return w.used * 4;
 }
 
 }  // namespace mamba
@@ -857,7 +1037,7 @@ extern "C" size_t mamba1_scan_packed_workspace_size(const mamba1_scan_packed_arg
     ScanPk p;
     if (scan_pk_make(a, &p) != MAMBA_OK) return 0;
     scan_pk_fwd_plan(p);
-    return scan_pk_fwd_floats(p) * 4;
+    return scan_pk_fwd_planes(p, nullptr);
 }
 
 extern "C" int mamba1_scan_packed_fwd(const mamba1_scan_packed_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {
@@ -873,16 +1053,12 @@ extern "C" int mamba1_scan_packed_fwd(const mamba1_scan_packed_args* a, void* ws
     p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
     scan_pk_fwd_plan(p);
     if ((st = scan_pk_grid_ok(p)) != MAMBA_OK) return st;
-    const size_t need = scan_pk_fwd_floats(p) * 4;
+    const size_t need = scan_pk_fwd_planes(p, ws);
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");
     if (need && (ws == nullptr || ws_bytes < need)) {
         set_error("mamba1_scan_packed_fwd: workspace missing or too small");
         return MAMBA_ERR_WORKSPACE;
     }
-    const size_t pl = (size_t)p.nchunk * p.D * scan_np(p.N);
-    p.E = static_cast<float*>(ws);
-    p.h0c = p.E + pl;
-    p.sumd = p.h0c + pl;
     SCAN_PK_DISPATCH(scan_pk_fwd_launch, scan_np(p.N), a->io_dtype == MAMBA_BF16, p, (hipStream_t)stream);
     MAMBA_CHECK_LAUNCH();
     return MAMBA_OK;
@@ -892,7 +1068,7 @@ extern "C" size_t mamba1_scan_packed_bwd_workspace_size(const mamba1_scan_packed
     ScanPk p;
     if (a == nullptr || scan_pk_make(&a->fwd, &p) != MAMBA_OK) return 0;
     scan_pk_bwd_plan(p);
-    return scan_pk_bwd_floats(p) * 4;
+    return scan_pk_bwd_planes(p, nullptr);
 }
 
 extern "C" int mamba1_scan_packed_bwd(const mamba1_scan_packed_bwd_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {
@@ -914,21 +1090,13 @@ extern "C" int mamba1_scan_packed_bwd(const mamba1_scan_packed_bwd_args* a, void
     p.dA = a->dA; p.dD = a->dD; p.db = a->d_delta_bias; p.dh0 = a->d_initial_state;
     scan_pk_bwd_plan(p);
     if ((st = scan_pk_grid_ok(p)) != MAMBA_OK) return st;
-    const size_t need = scan_pk_bwd_floats(p) * 4;
+    const size_t need = scan_pk_bwd_planes(p, ws);
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");
     if (need && (ws == nullptr || ws_bytes < need)) {
         set_error("mamba1_scan_packed_bwd: workspace missing or too small");
         return MAMBA_ERR_WORKSPACE;
     }
-    const size_t np = scan_np(p.N), nd = (size_t)p.nchunk * p.D;
-    p.E = static_cast<float*>(ws);
-    p.G = p.E + nd * np;
-    p.pA = p.G + nd * np;
-    p.pBC = p.pA + nd * np;
-    p.sumd = p.pBC + (size_t)ceil_div(p.D, 1024 / (int)np) * p.rows * 2 * np;
-    p.pD = p.sumd + nd;
-    p.pb = p.pD + nd;
-    SCAN_PK_DISPATCH(scan_pk_bwd_launch, (int)np, a->fwd.io_dtype == MAMBA_BF16, p, (hipStream_t)stream);
+    SCAN_PK_DISPATCH(scan_pk_bwd_launch, scan_np(p.N), a->fwd.io_dtype == MAMBA_BF16, p, (hipStream_t)stream);
     MAMBA_CHECK_LAUNCH();
     return MAMBA_OK;
 }

@@ -57,31 +57,31 @@ __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
         bias[v] = p.b && v < nc ? p.b[c + v] : 0.f;
         for (int k = 0; k < K; ++k) w[k][v] = v < nc ? p.w[(int64_t)(c + v) * K + k] : 0.f;
     }
-    const int64_t c0 = ck * p.chunk, c1 = min(p.rows, c0 + p.chunk);
-    int64_t t = c0;
+    const int c0 = (int)(ck * p.chunk), c1 = (int)min(p.rows, ck * p.chunk + p.chunk);
+    int t = c0;
     const float zero[V] = {};
     for (int s = p.q.after(c0); s < p.q.n && t < c1; ++s) {
-        const int64_t st = p.q.begin(s), en = p.q.end(s);
+        const int st = p.q.begin(s), en = p.q.end(s);
         if (en <= t) continue;
-        for (; p.fill && t < min(st, c1); ++t) st_run<V, T>(out + t * p.out_st, nc, zero);
+        for (; p.fill && t < min(st, c1); ++t) st_run<V, T>(out + (int64_t)t * p.out_st, nc, zero);
         t = max(t, st);
         if (t >= c1) break;
         // the K - 1 taps before row t
         const int64_t slot = p.state ? slot_of(p.slots, s, p.nslots) : -1;
         for (int k = 0; k < K - 1; ++k) {
-            const int64_t at = t - (K - 1) + k;
+            const int at = t - (K - 1) + k;
             if (at >= st) {
-                ld_run<V, T>(x + at * p.x_st, nc, tap[k]);
+                ld_run<V, T>(x + (int64_t)at * p.x_st, nc, tap[k]);
             } else {
-                const int col = (int)(K + at - st);
+                const int col = K + at - st;
 #pragma unroll
                 for (int v = 0; v < V; ++v)
                     tap[k][v] = slot >= 0 && v < nc ? p.state[(slot * p.C + c + v) * K + col] : 0.f;
             }
         }
-        const int64_t stop = min(en, c1);
+        const int stop = min(en, c1);
         for (; t < stop; ++t) {
-            ld_run<V, T>(x + t * p.x_st, nc, tap[K - 1]);
+            ld_run<V, T>(x + (int64_t)t * p.x_st, nc, tap[K - 1]);
             float o[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
@@ -89,14 +89,17 @@ __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
                 for (int k = 0; k < K; ++k) acc = __builtin_fmaf(w[k][v], tap[k][v], acc);
                 o[v] = p.silu ? acc * conv_sigmoid(acc) : acc;
             }
-            st_run<V, T>(out + t * p.out_st, nc, o);
+            st_run<V, T>(out + (int64_t)t * p.out_st, nc, o);
             for (int k = 0; k < K - 1; ++k)
 #pragma unroll
                 for (int v = 0; v < V; ++v) tap[k][v] = tap[k + 1][v];
         }
     }
-    for (; p.fill && t < c1; ++t) st_run<V, T>(out + t * p.out_st, nc, zero);
+    for (; p.fill && t < c1; ++t) st_run<V, T>(out + (int64_t)t * p.out_st, nc, zero);
 }
+
+// an offset of a sequence that differs between the lanes
+__device__ __forceinline__ int seq_at(const Seqs& q, int s) { return min(max(q.cu[s], 0), q.rows); }
 
 // The windows after the call: window[k] = old window[k + length], then the last
 // inputs.  After the forward kernel, which reads the old ones.
@@ -106,12 +109,12 @@ __global__ __launch_bounds__(256) void conv_pk_window(ConvPk p) {
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
         const int s = (int)(i / p.C), c = (int)(i - (int64_t)s * p.C);
         const int64_t slot = slot_of(p.slots, s, p.nslots);
-        const int64_t st = p.q.begin(s), en = p.q.end(s), len = en - st;
+        const int st = seq_at(p.q, s), en = max(st, seq_at(p.q, s + 1)), len = en - st;
         if (slot < 0 || len == 0) continue;
         float* win = p.state + (slot * p.C + c) * p.K;
         const T* x = static_cast<const T*>(p.x) + c;
         for (int k = 0; k < p.K; ++k)
-            win[k] = k + len < p.K ? win[k + len] : load_f32<T>(x + (en - p.K + k) * p.x_st);
+            win[k] = k + len < p.K ? win[k + len] : load_f32<T>(x + (int64_t)(en - p.K + k) * p.x_st);
     }
 }
 
@@ -139,19 +142,19 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
             dw[k][v] = 0.f;
         }
     }
-    const int64_t c0 = ck * p.chunk, c1 = min(p.rows, c0 + p.chunk);
-    int64_t t = c0;
+    const int c0 = (int)(ck * p.chunk), c1 = (int)min(p.rows, ck * p.chunk + p.chunk);
+    int t = c0;
     const float zero[V] = {};
     for (int s = p.q.after(c0); s < p.q.n && t < c1; ++s) {
-        const int64_t st = p.q.begin(s), en = p.q.end(s);
+        const int st = p.q.begin(s), en = p.q.end(s);
         if (en <= t) continue;
-        for (; p.out && p.fill && t < min(st, c1); ++t) st_run<V, T>(dx + t * p.out_st, nc, zero);
+        for (; p.out && p.fill && t < min(st, c1); ++t) st_run<V, T>(dx + (int64_t)t * p.out_st, nc, zero);
         t = max(t, st);
         if (t >= c1) break;
         for (int k = 0; k < K - 1; ++k) {
-            const int64_t at = t - (K - 1) + k;
+            const int at = t - (K - 1) + k;
             if (at >= st) {
-                ld_run<V, T>(x + at * p.x_st, nc, tap[k]);
+                ld_run<V, T>(x + (int64_t)at * p.x_st, nc, tap[k]);
             } else {
 #pragma unroll
                 for (int v = 0; v < V; ++v) tap[k][v] = 0.f;
@@ -161,15 +164,15 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int v = 0; v < V; ++v) g[k][v] = 0.f;
-        const int64_t stop = min(en, c1);
-        for (int64_t r = t; r < stop + K - 1; ++r) {
+        const int stop = min(en, c1);
+        for (int r = t; r < stop + K - 1; ++r) {
             for (int k = K - 1; k > 0; --k)
 #pragma unroll
                 for (int v = 0; v < V; ++v) g[k][v] = g[k - 1][v];
             if (r < en) {
                 float d[V];
-                ld_run<V, T>(x + r * p.x_st, nc, tap[K - 1]);
-                ld_run<V, T>(dout + r * p.dout_st, nc, d);
+                ld_run<V, T>(x + (int64_t)r * p.x_st, nc, tap[K - 1]);
+                ld_run<V, T>(dout + (int64_t)r * p.dout_st, nc, d);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     float acc = bias[v];
@@ -191,7 +194,7 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) g[0][v] = 0.f;
             }
-            const int64_t at = r - (K - 1);
+            const int at = r - (K - 1);
             if (p.out && at >= t) {
                 float o[V];
 #pragma unroll
@@ -199,12 +202,12 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
                     o[v] = 0.f;
                     for (int k = 0; k < K; ++k) o[v] = __builtin_fmaf(w[k][v], g[k][v], o[v]);
                 }
-                st_run<V, T>(dx + at * p.out_st, nc, o);
+                st_run<V, T>(dx + (int64_t)at * p.out_st, nc, o);
             }
         }
         t = stop;
     }
-    for (; p.out && p.fill && t < c1; ++t) st_run<V, T>(dx + t * p.out_st, nc, zero);
+    for (; p.out && p.fill && t < c1; ++t) st_run<V, T>(dx + (int64_t)t * p.out_st, nc, zero);
     if (!p.part) return;
     float* part = p.part + (ck * (K + 1)) * (int64_t)p.C + c;
     for (int k = 0; k < K; ++k) st_run<V, float>(part + (int64_t)k * p.C, nc, dw[k]);
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(256) void conv_slot_step(ConvSlotParams p) {
 
 static int conv_pk_make(const mamba_conv1d_packed_args* a, ConvPk* o) {
     MAMBA_CHECK_ARG(a != nullptr, "args is NULL");
-    MAMBA_CHECK_ARG(a->rows >= 0 && a->rows < (1ll << 31), "rows must be in [0, 2^31)");
+    MAMBA_CHECK_ARG(a->rows >= 0 && a->rows < kMaxRows, "rows must be in [0, 2^31 - 2^20)");
     MAMBA_CHECK_ARG(a->channels >= 1 && a->channels <= (1 << 20), "channels must be in [1, 2^20]");
     MAMBA_CHECK_ARG(a->kernel >= 1 && a->kernel <= kMaxTaps, "kernel must be in [1, 64]");
     MAMBA_CHECK_ARG(a->nseq >= 0, "nseq must be >= 0");
@@ -274,7 +277,7 @@ static int conv_pk_make(const mamba_conv1d_packed_args* a, ConvPk* o) {
     MAMBA_CHECK_ARG(a->cu_seqlens != nullptr, "cu_seqlens is required");
     ConvPk& p = *o;
     p = ConvPk{};
-    p.q = Seqs{a->cu_seqlens, a->nseq, a->rows};
+    p.q = Seqs{a->cu_seqlens, a->nseq, (int)a->rows};
     p.rows = a->rows; p.C = a->channels; p.K = a->kernel;
     p.silu = a->silu != 0; p.fill = a->fill_outside != 0;
     p.x = a->x; p.x_st = a->x_st; p.w = a->w; p.b = a->bias;

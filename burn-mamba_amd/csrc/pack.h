@@ -53,25 +53,26 @@ __device__ __forceinline__ void st_run(T* p, int n, const float (&v)[V]) {
 // result and no access out of range.
 struct Seqs {
     const int32_t* cu;
-    int n;
-    int64_t rows;
-    __device__ __forceinline__ int64_t begin(int s) const {
-        return min(max((int64_t)cu[s], (int64_t)0), rows);
-    }
-    __device__ __forceinline__ int64_t end(int s) const {
-        return max(begin(s), min((int64_t)cu[s + 1], rows));
-    }
-    // the first sequence that ends behind row t, n if none does (t uniform)
-    __device__ __forceinline__ int after(int64_t t) const {
+    int n, rows;
+    // in scalar registers: s and t are uniform over a wave
+    __device__ __forceinline__ int at(int s) const { return min(max(__builtin_amdgcn_readfirstlane(cu[s]), 0), rows); }
+    __device__ __forceinline__ int begin(int s) const { return at(s); }
+    __device__ __forceinline__ int end(int s) const { return max(at(s), at(s + 1)); }
+    // the first sequence that ends behind row t, n if none does
+    __device__ __forceinline__ int after(int t) const {
         int lo = 0, hi = n;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if ((int64_t)cu[mid + 1] > t) hi = mid;
+            if (__builtin_amdgcn_readfirstlane(cu[mid + 1]) > t) hi = mid;
             else lo = mid + 1;
         }
         return lo;
     }
 };
+// rows of a packed tensor: a chunk's last row and one more chunk still fit an int
+constexpr int64_t kMaxRows = (1ll << 31) - (1ll << 20);
+// elements between rows: 16 rows' offsets fit 32 bits of bytes
+constexpr int64_t kMaxStride = 1ll << 25;
 
 // Row of a cache that sequence s keeps its state in, -1: none (a slot out of range).
 __device__ __forceinline__ int64_t slot_of(const int32_t* slots, int s, int64_t nslots) {

@@ -56,7 +56,7 @@ struct ScanPk {
     const float* A; const float* Dv; const float* bias;
     void* y; int64_t y_st;
     float* state; int64_t nslots; const int32_t* slots;
-    int chunk; int64_t nchunk;
+    int chunk, nchunk;
     // per chunk: what it leaves behind [nchunk][D][NP] (then, carried, what
     // leaves it), the sum of d [nchunk][D], and the state that its last sequence
     // began from [nchunk][D][NP] (the cache's slot may be written meanwhile)
@@ -79,12 +79,13 @@ struct ScanPk {
 };
 
 // softplus(x) = log(1 + e^x), x itself above 20 (equal in f32); log1p through the
-// hardware log with Goldberg's correction, log(v) e / (v - 1) for v = 1 + e
+// hardware log with Goldberg's correction, log(v) e / (v - 1) for v = 1 + e.
+// Without a branch, which would part the elements in the schedule.
 __device__ __forceinline__ float pk_softplus(float x) {
-    if (x > 20.f) return x;
-    const float e = __expf(x);
+    const float e = __expf(fminf(x, 20.f));
     const float v = 1.f + e;
-    return v == 1.f ? e : __logf(v) * (e * __builtin_amdgcn_rcpf(v - 1.f));
+    const float l = __logf(v) * (e * __builtin_amdgcn_rcpf(v - 1.f));
+    return x > 20.f ? x : v == 1.f ? e : l;
 }
 __device__ __forceinline__ float pk_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
 
@@ -117,20 +118,19 @@ template <typename T, int V>
 struct Elems {
     static constexpr int W = (V * (int)sizeof(T) + 3) / 4;
     uint32_t w[W];
-    __device__ __forceinline__ void load(const T* p, int n) {
-        if (n >= V) {
-            if constexpr (V * sizeof(T) == 2) w[0] = *p;
-            else __builtin_memcpy(w, p, V * sizeof(T));
-        } else {
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (V * sizeof(T) == 2) w[0] = *p;
+        else __builtin_memcpy(w, p, V * sizeof(T));
+    }
+    __device__ __forceinline__ void load_part(const T* p, int n) {
 #pragma unroll
-            for (int i = 0; i < W; ++i) w[i] = 0u;
+        for (int i = 0; i < W; ++i) w[i] = 0u;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i < n) {
-                    if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
-                    else w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
-                }
-        }
+        for (int i = 0; i < V; ++i)
+            if (i < n) {
+                if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
+                else w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
+            }
     }
     __device__ __forceinline__ void get(float (&o)[V]) const {
 #pragma unroll
@@ -159,11 +159,12 @@ template <typename T, int NP>
 struct BcTile {
     static constexpr int K = kTile * NP / 256;
     T v[K];
-    __device__ __forceinline__ void load(const void* src, int64_t st, int64_t t0, int n, int N) {
+    __device__ __forceinline__ void load(const void* src, int64_t st, int t0, int n, int N) {
+        const T* base = static_cast<const T*>(src) + t0 * st;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int i = threadIdx.x + 256 * k, r = i / NP, c = i % NP;
-            v[k] = r < n && c < N ? static_cast<const T*>(src)[(t0 + r) * st + c] : (T)0;
+            v[k] = r < n && c < N ? base[(uint32_t)(r * (int)st + c)] : (T)0;
         }
     }
     __device__ __forceinline__ void stage(float (*dst)[NP]) const {
@@ -180,12 +181,12 @@ enum { kIn = 1, kOut = 2, kThrough = 4 };
 // What chunk ck does at its two ends: the sequence that crosses into it and the
 // one that crosses out of it (-1: none).
 struct ChunkEnds {
-    int64_t c0, c1;
+    int c0, c1;
     int first, last;   // first sequence with rows in the chunk, and the one that crosses c1
     bool in, through;  // the first one began before c0; it fills the chunk and goes on
     __device__ __forceinline__ ChunkEnds(const ScanPk& p, int64_t ck) {
-        c0 = ck * p.chunk;
-        c1 = min(p.rows, c0 + p.chunk);
+        c0 = (int)(ck * p.chunk);
+        c1 = min((int)p.rows, c0 + p.chunk);
         first = p.q.after(c0);
         in = first < p.q.n && p.q.begin(first) < c0;
         last = -1;
@@ -224,7 +225,7 @@ __device__ __forceinline__ void store_state(float* base, int64_t row, const Scan
 }
 template <int NP>
 __device__ __forceinline__ float4* plane(float* base, int64_t ck, const ScanPk& p, int d, int ng) {
-    return reinterpret_cast<float4*>(base + ((ck * p.D + d) * NP + 4 * ng));
+    return reinterpret_cast<float4*>(base + ((ck * p.D + d) * (int64_t)NP + 4 * ng));
 }
 template <int NP>
 __device__ __forceinline__ void load_plane(float* base, int64_t ck, const ScanPk& p, int d, int ng, float (&h)[4]) {
@@ -242,42 +243,53 @@ __global__ __launch_bounds__(256) void scan_pk_state(ScanPk p) {
     __shared__ float2 s_dd[TT][CPB];
     __shared__ __align__(16) float s_B[TT][NP];
     const int nblk = (p.D + CPB - 1) / CPB;
-    const int64_t ck = blockIdx.x / nblk;
-    const int d0 = (int)(blockIdx.x % nblk) * CPB;
+    const int ck = (int)(blockIdx.x / (uint32_t)nblk);
+    const int d0 = (int)(blockIdx.x % (uint32_t)nblk) * CPB;
     const ChunkEnds e(p, ck);
     if (d0 == 0 && threadIdx.x == 0) p.ends[ck] = e.flags();
     if (e.last < 0) return;  // nothing crosses its end
     const ElemMap<NP> m;
+    // this thread's place in a tile (32 bits, beside a scalar base)
+    auto at = [&](int64_t st) { return (uint32_t)(m.row * (int)st + m.ch); };
     const int c = threadIdx.x / NS, ng = threadIdx.x % NS, d = d0 + c;
     const int nc = p.D - (d0 + m.ch);
     float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, sumd = 0.f, bias[EV];
     load_A2<NP>(p, d, ng, A2);
 #pragma unroll
     for (int k = 0; k < EV; ++k) bias[k] = p.bias && k < nc ? p.bias[d0 + m.ch + k] : 0.f;
-    const int64_t st = p.q.begin(e.last), a = max(st, e.c0);
+    const int st = p.q.begin(e.last), a = max(st, e.c0);
     if (st >= e.c0 && p.state) {
         load_state(p.state, slot_of(p.slots, e.last, p.nslots), p, d, ng, h);
         store_plane<NP>(p.h0c, ck, p, d, ng, h);
     }
     Elems<T, EV> ru, rd;
     BcTile<T, NP> rB;
-    auto fetch = [&](int64_t t0) {
-        const int n = (int)min((int64_t)TT, e.c1 - t0);
-        const int q = m.row < n ? nc : 0;
-        ru.load(static_cast<const T*>(p.u) + (t0 + m.row) * p.u_st + d0 + m.ch, q);
-        rd.load(static_cast<const T*>(p.dl) + (t0 + m.row) * p.dl_st + d0 + m.ch, q);
+    auto fetch = [&](int t0) {
+        const int n = min(TT, e.c1 - t0);
+        if (m.row < n && nc >= EV) {
+            ru.load(static_cast<const T*>(p.u) + (t0 * p.u_st + d0) + at(p.u_st));
+            rd.load(static_cast<const T*>(p.dl) + (t0 * p.dl_st + d0) + at(p.dl_st));
+        } else {
+            const int q = m.row < n ? nc : 0;
+            ru.load_part(static_cast<const T*>(p.u) + (t0 * p.u_st + d0) + at(p.u_st), q);
+            rd.load_part(static_cast<const T*>(p.dl) + (t0 * p.dl_st + d0) + at(p.dl_st), q);
+        }
         rB.load(p.B, p.B_st, t0, n, p.N);
     };
     fetch(a);
-    for (int64_t t0 = a; t0 < e.c1; t0 += TT) {
-        const int n = (int)min((int64_t)TT, e.c1 - t0);
+    for (int t0 = a; t0 < e.c1; t0 += TT) {
+        const int n = min(TT, e.c1 - t0);
         float uv[EV], dv[EV];
         ru.get(uv);
         rd.get(dv);
 #pragma unroll
+        for (int k = 0; k < EV; ++k) dv[k] += bias[k];
+        if (p.softplus) {
+#pragma unroll
+            for (int k = 0; k < EV; ++k) dv[k] = pk_softplus(dv[k]);
+        }
+#pragma unroll
         for (int k = 0; k < EV; ++k) {
-            dv[k] += bias[k];
-            if (p.softplus) dv[k] = pk_softplus(dv[k]);
             if (m.row >= n) dv[k] = 0.f;
             s_dd[m.row][m.ch + k] = make_float2(dv[k], dv[k] * uv[k]);
         }
@@ -305,7 +317,7 @@ __global__ __launch_bounds__(256) void scan_pk_state(ScanPk p) {
         __syncthreads();
     }
     store_plane<NP>(p.E, ck, p, d, ng, h);
-    if (d < p.D && ng == 0) p.sumd[ck * p.D + d] = sumd;
+    if (d < p.D && ng == 0) p.sumd[(int64_t)ck * p.D + d] = sumd;
 }
 
 // A thread per (channel, state) walks the chunks: E[ck] <- the state that leaves
@@ -354,10 +366,12 @@ __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
     __shared__ __align__(16) float s_B[TT][NP];
     __shared__ __align__(16) float s_C[TT][NP];
     const int nblk = (p.D + CPB - 1) / CPB;
-    const int64_t ck = blockIdx.x / nblk;
-    const int d0 = (int)(blockIdx.x % nblk) * CPB;
+    const int ck = (int)(blockIdx.x / (uint32_t)nblk);
+    const int d0 = (int)(blockIdx.x % (uint32_t)nblk) * CPB;
     const ChunkEnds e(p, ck);
     const ElemMap<NP> m;
+    // this thread's place in a tile (32 bits, beside a scalar base)
+    auto at = [&](int64_t st) { return (uint32_t)(m.row * (int)st + m.ch); };
     const int c = threadIdx.x / NS, ng = threadIdx.x % NS, d = d0 + c;
     const int nc = p.D - (d0 + m.ch);
     float A2[4], h[4], bias[EV], Dv[EV];
@@ -368,31 +382,38 @@ __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
         Dv[k] = p.Dv && k < nc ? p.Dv[d0 + m.ch + k] : 0.f;
     }
     const float zero[EV] = {};
-    auto outside = [&](int64_t a, int64_t b) {  // rows of no sequence
-        for (int64_t t = a + m.row; p.fill && t < b; t += TT)
-            st_run<EV, T>(static_cast<T*>(p.y) + t * p.y_st + d0 + m.ch, nc, zero);
+    auto outside = [&](int a, int b) {  // rows of no sequence
+        for (int t = a + m.row; p.fill && t < b; t += TT)
+            st_run<EV, T>(static_cast<T*>(p.y) + (int64_t)t * p.y_st + d0 + m.ch, nc, zero);
     };
     Elems<T, EV> ru, rd, rz;
     BcTile<T, NP> rB, rC;
-    auto fetch = [&](int64_t t0, int64_t b) {
-        const int n = (int)min((int64_t)TT, b - t0);
-        const int q = m.row < n ? nc : 0;
-        ru.load(static_cast<const T*>(p.u) + (t0 + m.row) * p.u_st + d0 + m.ch, q);
-        rd.load(static_cast<const T*>(p.dl) + (t0 + m.row) * p.dl_st + d0 + m.ch, q);
-        if (p.z) rz.load(static_cast<const T*>(p.z) + (t0 + m.row) * p.z_st + d0 + m.ch, q);
+    auto fetch = [&](int t0, int b) {
+        const int n = min(TT, b - t0);
+        if (m.row < n && nc >= EV) {
+            ru.load(static_cast<const T*>(p.u) + (t0 * p.u_st + d0) + at(p.u_st));
+            rd.load(static_cast<const T*>(p.dl) + (t0 * p.dl_st + d0) + at(p.dl_st));
+            if (p.z) rz.load(static_cast<const T*>(p.z) + (t0 * p.z_st + d0) + at(p.z_st));
+        } else {
+            const int q = m.row < n ? nc : 0;
+            ru.load_part(static_cast<const T*>(p.u) + (t0 * p.u_st + d0) + at(p.u_st), q);
+            rd.load_part(static_cast<const T*>(p.dl) + (t0 * p.dl_st + d0) + at(p.dl_st), q);
+            if (p.z) rz.load_part(static_cast<const T*>(p.z) + (t0 * p.z_st + d0) + at(p.z_st), q);
+        }
         rB.load(p.B, p.B_st, t0, n, p.N);
         rC.load(p.C, p.C_st, t0, n, p.N);
     };
-    int64_t t = e.c0;
+    int t = e.c0;
     for (int s = e.first; s < p.q.n && t < e.c1; ++s) {
-        const int64_t st = p.q.begin(s), en = p.q.end(s);
+        const int st = p.q.begin(s), en = p.q.end(s);
         if (en <= t) continue;
         if (st > t) {
             outside(t, min(st, e.c1));
             t = min(st, e.c1);
             if (t >= e.c1) break;
         }
-        const int64_t b = min(en, e.c1), slot = p.state ? slot_of(p.slots, s, p.nslots) : -1;
+        const int b = min(en, e.c1);
+        const int64_t slot = p.state ? slot_of(p.slots, s, p.nslots) : -1;
         fetch(t, b);
         if (e.in && t == e.c0) {  // goes on from the chunk before
             load_plane<NP>(p.E, ck - 1, p, d, ng, h);
@@ -401,20 +422,30 @@ __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
         } else {
             load_state(p.state, slot, p, d, ng, h);
         }
-        for (int64_t t0 = t; t0 < b; t0 += TT) {
-            const int n = (int)min((int64_t)TT, b - t0);
+        for (int t0 = t; t0 < b; t0 += TT) {
+            const int n = min(TT, b - t0);
             float Du[EV], gate[EV], uv[EV], dv[EV];
             ru.get(uv);
             rd.get(dv);
             if (p.z) rz.get(gate);
 #pragma unroll
+            for (int k = 0; k < EV; ++k) dv[k] += bias[k];
+            if (p.softplus) {
+#pragma unroll
+                for (int k = 0; k < EV; ++k) dv[k] = pk_softplus(dv[k]);
+            }
+#pragma unroll
             for (int k = 0; k < EV; ++k) {
-                dv[k] += bias[k];
-                if (p.softplus) dv[k] = pk_softplus(dv[k]);
                 if (m.row >= n) dv[k] = 0.f;
                 s_dd[m.row][m.ch + k] = make_float2(dv[k], dv[k] * uv[k]);
                 Du[k] = Dv[k] * uv[k];
-                gate[k] = p.z ? gate[k] * pk_sigmoid(gate[k]) : 1.f;
+            }
+            if (p.z) {
+#pragma unroll
+                for (int k = 0; k < EV; ++k) gate[k] *= pk_sigmoid(gate[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < EV; ++k) gate[k] = 1.f;
             }
             rB.stage(s_B);
             rC.stage(s_C);
@@ -449,7 +480,7 @@ __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
                 float o[EV];
 #pragma unroll
                 for (int k = 0; k < EV; ++k) o[k] = (s_y[m.row][m.ch + k] + Du[k]) * gate[k];
-                st_run<EV, T>(static_cast<T*>(p.y) + (t0 + m.row) * p.y_st + d0 + m.ch, nc, o);
+                st_run<EV, T>(static_cast<T*>(p.y) + (t0 * p.y_st + d0) + at(p.y_st), nc, o);
             }
         }
         if (b == en) store_state(p.state, slot, p, d, ng, h);
@@ -475,11 +506,13 @@ __global__ __launch_bounds__(256) void scan_pk_state_bwd(ScanPk p) {
     __shared__ __align__(16) float s_B[TT][NP];
     __shared__ __align__(16) float s_C[TT][NP];
     const int nblk = (p.D + CPB - 1) / CPB;
-    const int64_t ck = blockIdx.x / nblk;
-    const int d0 = (int)(blockIdx.x % nblk) * CPB;
+    const int ck = (int)(blockIdx.x / (uint32_t)nblk);
+    const int d0 = (int)(blockIdx.x % (uint32_t)nblk) * CPB;
     const ChunkEnds e(p, ck);
     if (d0 == 0 && threadIdx.x == 0) p.ends[ck] = e.flags();
     const ElemMap<NP> m;
+    // this thread's place in a tile (32 bits, beside a scalar base)
+    auto at = [&](int64_t st) { return (uint32_t)(m.row * (int)st + m.ch); };
     const int c = threadIdx.x / NS, ng = threadIdx.x % NS, d = d0 + c;
     const int nc = p.D - (d0 + m.ch);
     float A2[4], h[4], P[4], G[4], sumd, bias[EV];
@@ -488,23 +521,30 @@ __global__ __launch_bounds__(256) void scan_pk_state_bwd(ScanPk p) {
     for (int k = 0; k < EV; ++k) bias[k] = p.bias && k < nc ? p.bias[d0 + m.ch + k] : 0.f;
     Elems<T, EV> ru, rd, re, rz;
     BcTile<T, NP> rB, rC;
-    auto fetch = [&](int64_t t0, int64_t b) {
-        const int n = (int)min((int64_t)TT, b - t0);
-        const int q = m.row < n ? nc : 0;
-        ru.load(static_cast<const T*>(p.u) + (t0 + m.row) * p.u_st + d0 + m.ch, q);
-        rd.load(static_cast<const T*>(p.dl) + (t0 + m.row) * p.dl_st + d0 + m.ch, q);
-        re.load(static_cast<const T*>(p.dy) + (t0 + m.row) * p.dy_st + d0 + m.ch, q);
-        if (p.z) rz.load(static_cast<const T*>(p.z) + (t0 + m.row) * p.z_st + d0 + m.ch, q);
+    auto fetch = [&](int t0, int b) {
+        const int n = min(TT, b - t0);
+        if (m.row < n && nc >= EV) {
+            ru.load(static_cast<const T*>(p.u) + (t0 * p.u_st + d0) + at(p.u_st));
+            rd.load(static_cast<const T*>(p.dl) + (t0 * p.dl_st + d0) + at(p.dl_st));
+            re.load(static_cast<const T*>(p.dy) + (t0 * p.dy_st + d0) + at(p.dy_st));
+            if (p.z) rz.load(static_cast<const T*>(p.z) + (t0 * p.z_st + d0) + at(p.z_st));
+        } else {
+            const int q = m.row < n ? nc : 0;
+            ru.load_part(static_cast<const T*>(p.u) + (t0 * p.u_st + d0) + at(p.u_st), q);
+            rd.load_part(static_cast<const T*>(p.dl) + (t0 * p.dl_st + d0) + at(p.dl_st), q);
+            re.load_part(static_cast<const T*>(p.dy) + (t0 * p.dy_st + d0) + at(p.dy_st), q);
+            if (p.z) rz.load_part(static_cast<const T*>(p.z) + (t0 * p.z_st + d0) + at(p.z_st), q);
+        }
         rB.load(p.B, p.B_st, t0, n, p.N);
         rC.load(p.C, p.C_st, t0, n, p.N);
     };
-    int64_t t = e.c0;
+    int t = e.c0;
     for (int s = e.first; s < p.q.n && t < e.c1; ++s) {
-        const int64_t st = p.q.begin(s), en = p.q.end(s);
+        const int st = p.q.begin(s), en = p.q.end(s);
         if (en <= t) continue;
         t = max(t, st);
         if (t >= e.c1) break;
-        const int64_t b = min(en, e.c1);
+        const int b = min(en, e.c1);
         const bool in = e.in && t == e.c0;
         fetch(t, b);
         if (in) h[0] = h[1] = h[2] = h[3] = 0.f;
@@ -515,18 +555,25 @@ __global__ __launch_bounds__(256) void scan_pk_state_bwd(ScanPk p) {
             G[k] = 0.f;
         }
         sumd = 0.f;
-        for (int64_t t0 = t; t0 < b; t0 += TT) {
-            const int n = (int)min((int64_t)TT, b - t0);
+        for (int t0 = t; t0 < b; t0 += TT) {
+            const int n = min(TT, b - t0);
             float uv[EV], dv[EV], ev[EV], zv[EV];
             ru.get(uv);
             rd.get(dv);
             re.get(ev);
             if (p.z) rz.get(zv);
 #pragma unroll
+            for (int k = 0; k < EV; ++k) dv[k] += bias[k];
+            if (p.softplus) {
+#pragma unroll
+                for (int k = 0; k < EV; ++k) dv[k] = pk_softplus(dv[k]);
+            }
+            if (p.z) {
+#pragma unroll
+                for (int k = 0; k < EV; ++k) ev[k] *= zv[k] * pk_sigmoid(zv[k]);
+            }
+#pragma unroll
             for (int k = 0; k < EV; ++k) {
-                dv[k] += bias[k];
-                if (p.softplus) dv[k] = pk_softplus(dv[k]);
-                if (p.z) ev[k] *= zv[k] * pk_sigmoid(zv[k]);
                 if (m.row >= n) dv[k] = ev[k] = 0.f;
                 s_dd[m.row][m.ch + k] = make_float2(dv[k], dv[k] * uv[k]);
                 s_e[m.row][m.ch + k] = ev[k];
@@ -538,9 +585,9 @@ __global__ __launch_bounds__(256) void scan_pk_state_bwd(ScanPk p) {
 #pragma unroll 1
             for (int r0 = 0; r0 < n; r0 += 4) {
                 if (r0 % kSub == 0 && t0 + r0 > t) {
-                    const int64_t at = (t0 + r0) / kSub;
-                    store_plane<NP>(p.ckh, at, p, d, ng, h);
-                    if (ng == 0 && d < p.D) p.ckd[at * p.D + d] = sumd;
+                    const int place = (t0 + r0) / kSub;
+                    store_plane<NP>(p.ckh, place, p, d, ng, h);
+                    if (ng == 0 && d < p.D) p.ckd[(int64_t)place * p.D + d] = sumd;
                 }
                 float2 dd[4];
                 float ee[4];
@@ -578,7 +625,7 @@ __global__ __launch_bounds__(256) void scan_pk_state_bwd(ScanPk p) {
         }
         if (s == e.last) {
             store_plane<NP>(p.E, ck, p, d, ng, h);
-            if (ng == 0 && d < p.D) p.sumd[ck * p.D + d] = sumd;
+            if (ng == 0 && d < p.D) p.sumd[(int64_t)ck * p.D + d] = sumd;
         }
         t = b;
     }
@@ -627,16 +674,17 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
     __shared__ __align__(16) float s_C[TT][NP];
     __shared__ __align__(16) float s_bc[4][TT][2 * NP];
     const int nblk = (p.D + CPB - 1) / CPB;
-    const int64_t ck = blockIdx.x / nblk;
-    const int blk = (int)(blockIdx.x % nblk), d0 = blk * CPB;
+    const int ck = (int)(blockIdx.x / (uint32_t)nblk);
+    const int blk = (int)(blockIdx.x % (uint32_t)nblk), d0 = blk * CPB;
     const ChunkEnds e(p, ck);
     const ElemMap<NP> m;
+    // this thread's place in a tile (32 bits, beside a scalar base)
+    auto at = [&](int64_t st) { return (uint32_t)(m.row * (int)st + m.ch); };
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int c = threadIdx.x / NS, ng = threadIdx.x % NS, d = d0 + c;
     const int nc = p.D - (d0 + m.ch);
     // where this lane's channel sums go: element lane / 16 % 2 (and + 2) of B's (C's) four states
     const int bc_at = (lane >> 5) * NP + 4 * ng + ((lane >> 4) & 1);
-    const bool bc_lane = (lane & 15) < NS;
     float A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f};
     load_A2<NP>(p, d, ng, A2);
     float Dv[EV], bias[EV], dD[EV], db[EV];
@@ -648,39 +696,46 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
     }
     const float zero[EV] = {};
     float* pBC = p.pBC + (int64_t)blk * p.rows * 2 * NP;
-    auto outside = [&](int64_t a, int64_t b) {
-        for (int64_t t = a + m.row; t < b; t += TT) {
-            st_run<EV, T>(static_cast<T*>(p.du) + t * p.du_st + d0 + m.ch, nc, zero);
-            st_run<EV, T>(static_cast<T*>(p.ddl) + t * p.ddl_st + d0 + m.ch, nc, zero);
-            if (p.z) st_run<EV, T>(static_cast<T*>(p.dz) + t * p.dz_st + d0 + m.ch, nc, zero);
+    auto outside = [&](int a, int b) {
+        for (int t = a + m.row; t < b; t += TT) {
+            st_run<EV, T>(static_cast<T*>(p.du) + (int64_t)t * p.du_st + d0 + m.ch, nc, zero);
+            st_run<EV, T>(static_cast<T*>(p.ddl) + (int64_t)t * p.ddl_st + d0 + m.ch, nc, zero);
+            if (p.z) st_run<EV, T>(static_cast<T*>(p.dz) + (int64_t)t * p.dz_st + d0 + m.ch, nc, zero);
         }
-        for (int64_t i = a * 2 * NP + threadIdx.x; i < b * 2 * NP; i += 256) pBC[i] = 0.f;
+        for (int64_t i = (int64_t)a * 2 * NP + threadIdx.x; i < (int64_t)b * 2 * NP; i += 256) pBC[i] = 0.f;
     };
     Elems<T, EV> ru, rd, re, rz;
     BcTile<T, NP> rB, rC;
-    auto fetch = [&](int64_t t0, int64_t b) {
-        const int n = (int)min((int64_t)TT, b - t0);
-        const int q = m.row < n ? nc : 0;
-        ru.load(static_cast<const T*>(p.u) + (t0 + m.row) * p.u_st + d0 + m.ch, q);
-        rd.load(static_cast<const T*>(p.dl) + (t0 + m.row) * p.dl_st + d0 + m.ch, q);
-        re.load(static_cast<const T*>(p.dy) + (t0 + m.row) * p.dy_st + d0 + m.ch, q);
-        if (p.z) rz.load(static_cast<const T*>(p.z) + (t0 + m.row) * p.z_st + d0 + m.ch, q);
+    auto fetch = [&](int t0, int b) {
+        const int n = min(TT, b - t0);
+        if (m.row < n && nc >= EV) {
+            ru.load(static_cast<const T*>(p.u) + (t0 * p.u_st + d0) + at(p.u_st));
+            rd.load(static_cast<const T*>(p.dl) + (t0 * p.dl_st + d0) + at(p.dl_st));
+            re.load(static_cast<const T*>(p.dy) + (t0 * p.dy_st + d0) + at(p.dy_st));
+            if (p.z) rz.load(static_cast<const T*>(p.z) + (t0 * p.z_st + d0) + at(p.z_st));
+        } else {
+            const int q = m.row < n ? nc : 0;
+            ru.load_part(static_cast<const T*>(p.u) + (t0 * p.u_st + d0) + at(p.u_st), q);
+            rd.load_part(static_cast<const T*>(p.dl) + (t0 * p.dl_st + d0) + at(p.dl_st), q);
+            re.load_part(static_cast<const T*>(p.dy) + (t0 * p.dy_st + d0) + at(p.dy_st), q);
+            if (p.z) rz.load_part(static_cast<const T*>(p.z) + (t0 * p.z_st + d0) + at(p.z_st), q);
+        }
         rB.load(p.B, p.B_st, t0, n, p.N);
         rC.load(p.C, p.C_st, t0, n, p.N);
     };
-    int64_t t = e.c0;
+    int t = e.c0;
     for (int s = e.first; s < p.q.n && t < e.c1; ++s) {
-        const int64_t st = p.q.begin(s), en = p.q.end(s);
+        const int st = p.q.begin(s), en = p.q.end(s);
         if (en <= t) continue;
         if (st > t) {
             outside(t, min(st, e.c1));
             t = min(st, e.c1);
             if (t >= e.c1) break;
         }
-        const int64_t b = min(en, e.c1);
+        const int b = min(en, e.c1);
         const bool in = e.in && t == e.c0;
-        const int len = (int)(b - t), tiles = (len + TT - 1) / TT;
-        fetch(t + (int64_t)(tiles - 1) * TT, b);
+        const int len = b - t, tiles = (len + TT - 1) / TT;
+        fetch(t + (tiles - 1) * TT, b);
         float h0[4], g[4], hn[4], dn = 0.f;  // hn, dn: the next part's kept state and sum of d
         if (in) load_plane<NP>(p.E, ck - 1, p, d, ng, h0);
         else load_state(p.h0, s, p, d, ng, h0);
@@ -688,27 +743,41 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
         else load_state(p.dhT, s, p, d, ng, g);
         auto kept = [&](int q) {  // before row kSub q of the run
             if (q <= 0) return;
-            const int64_t at = (t + q * kSub) / kSub;
-            load_plane<NP>(p.ckh, at, p, d, ng, hn);
-            if (in) dn = d < p.D ? p.ckd[at * p.D + d] : 0.f;
+            const int place = (t + q * kSub) / kSub;
+            load_plane<NP>(p.ckh, place, p, d, ng, hn);
+            if (in) dn = d < p.D ? p.ckd[(int64_t)place * p.D + d] : 0.f;
         };
         kept((len - 1) / kSub);
         for (int tl = tiles - 1; tl >= 0; --tl) {
-            const int64_t t0 = t + (int64_t)tl * TT;
-            const int n = (int)min((int64_t)TT, b - t0);
+            const int t0 = t + tl * TT;
+            const int n = min(TT, b - t0);
             float uv[EV], dv[EV], yv[EV], zv[EV];
             ru.get(uv);
             rd.get(dv);
             re.get(yv);
             if (p.z) rz.get(zv);
 #pragma unroll
+            for (int k = 0; k < EV; ++k) dv[k] += bias[k];
+            float dt[EV], ev[EV];
+            if (p.softplus) {
+#pragma unroll
+                for (int k = 0; k < EV; ++k) dt[k] = pk_softplus(dv[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < EV; ++k) dt[k] = dv[k];
+            }
+            if (p.z) {
+#pragma unroll
+                for (int k = 0; k < EV; ++k) ev[k] = yv[k] * (zv[k] * pk_sigmoid(zv[k]));
+            } else {
+#pragma unroll
+                for (int k = 0; k < EV; ++k) ev[k] = yv[k];
+            }
+#pragma unroll
             for (int k = 0; k < EV; ++k) {
-                dv[k] += bias[k];
-                float dt = p.softplus ? pk_softplus(dv[k]) : dv[k];
-                float ev = p.z ? yv[k] * (zv[k] * pk_sigmoid(zv[k])) : yv[k];
-                if (m.row >= n) dt = ev = 0.f;
-                s_dd[m.row][m.ch + k] = make_float2(dt, dt * uv[k]);
-                s_e[m.row][m.ch + k] = ev;
+                if (m.row >= n) dt[k] = ev[k] = 0.f;
+                s_dd[m.row][m.ch + k] = make_float2(dt[k], dt[k] * uv[k]);
+                s_e[m.row][m.ch + k] = ev[k];
             }
             rB.stage(s_B);
             rC.stage(s_C);
@@ -758,42 +827,47 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
                     sC = group_sum_all<NS>(sC);
                     float x0, x1;
                     channel_sums<NS>(vb, vc, x0, x1);
-                    if (ng == 0) {
-                        s_sB[r0 + i][c] = sB;
-                        s_sA[r0 + i][c] = sA;
-                        s_sC[r0 + i][c] = sC;
-                    }
-                    if (bc_lane) {
-                        s_bc[wave][r0 + i][bc_at] = x0;
-                        s_bc[wave][r0 + i][bc_at + 2] = x1;
-                    }
+                    // every lane that holds a sum writes it (the same value to the same
+                    // place): a branch here would keep the rows apart in the schedule
+                    s_sB[r0 + i][c] = sB;
+                    s_sA[r0 + i][c] = sA;
+                    s_sC[r0 + i][c] = sC;
+                    s_bc[wave][r0 + i][bc_at] = x0;
+                    s_bc[wave][r0 + i][bc_at + 2] = x1;
                 }
             }
             __syncthreads();
             // ---- the tile's dB and dC over the workgroup, and the gradients of its elements
             for (int i = threadIdx.x; i < n * 2 * NP; i += 256) {
                 const int r = i / (2 * NP), k = i % (2 * NP);
-                pBC[t0 * 2 * NP + i] = (s_bc[0][r][k] + s_bc[1][r][k]) + (s_bc[2][r][k] + s_bc[3][r][k]);
+                pBC[(int64_t)t0 * 2 * NP + i] = (s_bc[0][r][k] + s_bc[1][r][k]) + (s_bc[2][r][k] + s_bc[3][r][k]);
             }
             if (m.row < n) {
                 float o1[EV], o2[EV], o3[EV];
 #pragma unroll
                 for (int k = 0; k < EV; ++k) {
-                    const float sB = s_sB[m.row][m.ch + k], sA = s_sA[m.row][m.ch + k] * (1.f / kLog2e), sC = s_sC[m.row][m.ch + k];
+                    const float sB = s_sB[m.row][m.ch + k], sA = s_sA[m.row][m.ch + k] * (1.f / kLog2e);
                     const float dt = s_dd[m.row][m.ch + k].x, ev = s_e[m.row][m.ch + k];
-                    if (p.z) {
-                        const float sg = pk_sigmoid(zv[k]);
-                        o3[k] = yv[k] * __builtin_fmaf(Dv[k], uv[k], sC) * (sg * (1.f + zv[k] * (1.f - sg)));
-                    }
                     o1[k] = __builtin_fmaf(sB, dt, Dv[k] * ev);
                     o2[k] = __builtin_fmaf(sB, uv[k], sA);
-                    if (p.softplus) o2[k] *= pk_sigmoid(dv[k]);
                     dD[k] = __builtin_fmaf(ev, uv[k], dD[k]);
-                    db[k] += o2[k];
                 }
-                st_run<EV, T>(static_cast<T*>(p.du) + (t0 + m.row) * p.du_st + d0 + m.ch, nc, o1);
-                st_run<EV, T>(static_cast<T*>(p.ddl) + (t0 + m.row) * p.ddl_st + d0 + m.ch, nc, o2);
-                if (p.z) st_run<EV, T>(static_cast<T*>(p.dz) + (t0 + m.row) * p.dz_st + d0 + m.ch, nc, o3);
+                if (p.softplus) {
+#pragma unroll
+                    for (int k = 0; k < EV; ++k) o2[k] *= pk_sigmoid(dv[k]);
+                }
+                if (p.z) {
+#pragma unroll
+                    for (int k = 0; k < EV; ++k) {
+                        const float sg = pk_sigmoid(zv[k]);
+                        o3[k] = yv[k] * __builtin_fmaf(Dv[k], uv[k], s_sC[m.row][m.ch + k]) * (sg * (1.f + zv[k] * (1.f - sg)));
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < EV; ++k) db[k] += o2[k];
+                st_run<EV, T>(static_cast<T*>(p.du) + (t0 * p.du_st + d0) + at(p.du_st), nc, o1);
+                st_run<EV, T>(static_cast<T*>(p.ddl) + (t0 * p.ddl_st + d0) + at(p.ddl_st), nc, o2);
+                if (p.z) st_run<EV, T>(static_cast<T*>(p.dz) + (t0 * p.dz_st + d0) + at(p.dz_st), nc, o3);
             }
         }
         if (t == st) store_state(p.dh0, s, p, d, ng, g);
@@ -815,8 +889,8 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
             x += s_sB[r][threadIdx.x];
             y += s_sA[r][threadIdx.x];
         }
-        p.pD[ck * p.D + d0 + threadIdx.x] = x;
-        p.pb[ck * p.D + d0 + threadIdx.x] = y;
+        p.pD[(int64_t)ck * p.D + d0 + threadIdx.x] = x;
+        p.pb[(int64_t)ck * p.D + d0 + threadIdx.x] = y;
     }
 }
 
@@ -915,7 +989,7 @@ static int scan_np(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
 static int scan_pk_make(const mamba1_scan_packed_args* a, ScanPk* o) {
     MAMBA_CHECK_ARG(a != nullptr, "args is NULL");
-    MAMBA_CHECK_ARG(a->rows >= 0 && a->rows < (1ll << 31), "rows must be in [0, 2^31)");
+    MAMBA_CHECK_ARG(a->rows >= 0 && a->rows < kMaxRows, "rows must be in [0, 2^31 - 2^20)");
     MAMBA_CHECK_ARG(a->dim >= 1 && a->dim <= (1 << 20), "dim must be in [1, 2^20]");
     MAMBA_CHECK_ARG(a->dstate >= 1, "dstate must be >= 1");
     MAMBA_CHECK_ARG(a->nseq >= 0, "nseq must be >= 0");
@@ -926,9 +1000,11 @@ static int scan_pk_make(const mamba1_scan_packed_args* a, ScanPk* o) {
     }
     MAMBA_CHECK_ARG(a->cu_seqlens != nullptr && a->A != nullptr, "cu_seqlens and A are required");
     MAMBA_CHECK_ARG(a->rows == 0 || (a->u && a->delta && a->B && a->C), "u, delta, B and C are required");
+    for (int64_t st : {a->u_st, a->delta_st, a->z_st, a->B_st, a->C_st})
+        MAMBA_CHECK_ARG(a->rows <= 1 || (st >= 0 && st < kMaxStride), "row strides must be in [0, 2^25)");
     ScanPk& p = *o;
     p = ScanPk{};
-    p.q = Seqs{a->cu_seqlens, a->nseq, a->rows};
+    p.q = Seqs{a->cu_seqlens, a->nseq, (int)a->rows};
     p.rows = a->rows; p.D = a->dim; p.N = a->dstate;
     p.softplus = a->delta_softplus != 0; p.fill = a->fill_outside != 0;
     p.u = a->u; p.u_st = a->u_st; p.dl = a->delta; p.dl_st = a->delta_st; p.z = a->z; p.z_st = a->z_st;
@@ -939,16 +1015,16 @@ static int scan_pk_make(const mamba1_scan_packed_args* a, ScanPk* o) {
 
 static void scan_pk_fwd_plan(ScanPk& p) {
     p.chunk = 128;
-    p.nchunk = (p.rows + p.chunk - 1) / p.chunk;
+    p.nchunk = (int)((p.rows + p.chunk - 1) / p.chunk);
 }
 static void scan_pk_bwd_plan(ScanPk& p) {
     p.chunk = 128;
-    p.nchunk = (p.rows + p.chunk - 1) / p.chunk;
+    p.nchunk = (int)((p.rows + p.chunk - 1) / p.chunk);
 }
 // a grid's threads stay below 2^32
 static int scan_pk_grid_ok(const ScanPk& p) {
     const int64_t nblk = ceil_div(p.D, 1024 / scan_np(p.N));
-    if (p.nchunk * nblk >= (1ll << 24)) {
+    if ((int64_t)p.nchunk * nblk >= (1ll << 24)) {
         set_error("mamba1_scan_packed: rows * dim is too large for one call");
         return MAMBA_ERR_UNSUPPORTED;
     }
@@ -1046,7 +1122,7 @@ extern "C" int mamba1_scan_packed_fwd(const mamba1_scan_packed_args* a, void* ws
     if (st != MAMBA_OK) return st;
     if (p.rows == 0) return MAMBA_OK;
     MAMBA_CHECK_ARG(a->y != nullptr, "y is required");
-    MAMBA_CHECK_ARG(a->y_st >= p.D || p.rows == 1, "rows of y overlap");
+    MAMBA_CHECK_ARG((a->y_st >= p.D && a->y_st < kMaxStride) || p.rows == 1, "rows of y overlap (or lie 2^25 elements apart)");
     MAMBA_CHECK_ARG(a->state == nullptr || a->slots != nullptr || a->nslots >= a->nseq,
                     "without slots the state needs a row per sequence");
     p.y = a->y; p.y_st = a->y_st;
@@ -1084,6 +1160,8 @@ extern "C" int mamba1_scan_packed_bwd(const mamba1_scan_packed_bwd_args* a, void
     MAMBA_CHECK_ARG(p.rows <= 1 || (a->du_st >= p.D && a->ddelta_st >= p.D && (!a->dz || a->dz_st >= p.D)),
                     "rows of du, ddelta or dz overlap");
     MAMBA_CHECK_ARG(p.rows <= 1 || (a->dB_st >= p.N && a->dC_st >= p.N), "rows of dB or dC overlap");
+    for (int64_t st : {a->dy_st, a->du_st, a->ddelta_st, a->dz_st, a->dB_st, a->dC_st})
+        MAMBA_CHECK_ARG(p.rows <= 1 || (st >= 0 && st < kMaxStride), "row strides must be in [0, 2^25)");
     p.dy = a->dy; p.dy_st = a->dy_st; p.h0 = a->initial_state; p.dhT = a->d_final_state;
     p.du = a->du; p.du_st = a->du_st; p.ddl = a->ddelta; p.ddl_st = a->ddelta_st; p.dz = a->dz; p.dz_st = a->dz_st;
     p.dB = a->dB; p.dB_st = a->dB_st; p.dC = a->dC; p.dC_st = a->dC_st;

@@ -12,6 +12,7 @@
 // taps in registers, so each row is read once but for the K - 1 rows before a
 // chunk (and behind one, in the backward pass).
 #include <algorithm>
+#include <type_traits>
 
 #include "pack.h"
 
@@ -37,10 +38,35 @@ __device__ __forceinline__ float conv_sigmoid(float v) { return __builtin_amdgcn
 // KT = K as a constant, or 0: any K up to kMaxTaps (the taps then wait in a ring
 // that is shifted by one each row all the same).
 constexpr int kMaxTaps = 64;
+constexpr int kConvRows = 4;  // rows whose loads are in flight together
+
+// V channels' weights and bias; taps[k] = the input of row t - (K - 1) + k, k < K - 1
+template <int V, int KM>
+__device__ __forceinline__ void conv_weights(const ConvPk& p, int K, int c, int nc, float (&w)[KM][V], float (&bias)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        bias[v] = p.b && v < nc ? p.b[c + v] : 0.f;
+        for (int k = 0; k < K; ++k) w[k][v] = v < nc ? p.w[(int64_t)(c + v) * K + k] : 0.f;
+    }
+}
+template <typename T, int V, int KM>
+__device__ __forceinline__ void conv_taps(const ConvPk& p, const T* x, int K, int s, int st, int t, int c, int nc, float (&tap)[KM][V]) {
+    const int64_t slot = p.state ? slot_of(p.slots, s, p.nslots) : -1;
+    for (int k = 0; k < K - 1; ++k) {
+        const int at = t - (K - 1) + k;
+        if (at >= st) {
+            ld_run<V, T>(x + (int64_t)at * p.x_st, nc, tap[k]);
+        } else {
+            const int col = K + at - st;
+#pragma unroll
+            for (int v = 0; v < V; ++v) tap[k][v] = slot >= 0 && v < nc ? p.state[(slot * p.C + c + v) * K + col] : 0.f;
+        }
+    }
+}
 
 template <typename T, int KT, int V>
 __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
-    constexpr int KM = KT ? KT : kMaxTaps;
+    constexpr int KM = KT ? KT : kMaxTaps, R = KT ? kConvRows : 1;  // rows in flight
     const int K = KT ? KT : p.K;
     const int lane = threadIdx.x & 63;
     const int nblk = (p.C + 64 * V - 1) / (64 * V);
@@ -51,49 +77,50 @@ __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
     if (nc <= 0) return;
     const T* x = static_cast<const T*>(p.x) + c;
     T* out = static_cast<T*>(p.out) + c;
-    float w[KM][V], bias[V], tap[KM][V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        bias[v] = p.b && v < nc ? p.b[c + v] : 0.f;
-        for (int k = 0; k < K; ++k) w[k][v] = v < nc ? p.w[(int64_t)(c + v) * K + k] : 0.f;
-    }
+    float w[KM][V], bias[V], tap[KM + R - 1][V];
+    conv_weights<V, KM>(p, K, c, nc, w, bias);
     const int c0 = (int)(ck * p.chunk), c1 = (int)min(p.rows, ck * p.chunk + p.chunk);
     int t = c0;
     const float zero[V] = {};
+    // rows t .. t + r - 1 (r <= R) of a sequence; the last K - 1 inputs move to the front
+    auto rows = [&](auto whole, int r) __attribute__((always_inline)) {
+        constexpr bool W = decltype(whole)::value;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (W || i < r) ld_run<V, T>(x + (int64_t)(t + i) * p.x_st, nc, tap[K - 1 + i]);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (!W && i >= r) break;
+            float o[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float acc = bias[v];
+                for (int k = 0; k < K; ++k) acc = __builtin_fmaf(w[k][v], tap[i + k][v], acc);
+                o[v] = acc;
+            }
+            if (p.silu) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) o[v] *= conv_sigmoid(o[v]);
+            }
+            st_run<V, T>(out + (int64_t)(t + i) * p.out_st, nc, o);
+        }
+        if (W) {
+            for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) tap[k][v] = tap[k + R][v];
+        }
+        t += W ? R : r;
+    };
     for (int s = p.q.after(c0); s < p.q.n && t < c1; ++s) {
         const int st = p.q.begin(s), en = p.q.end(s);
         if (en <= t) continue;
         for (; p.fill && t < min(st, c1); ++t) st_run<V, T>(out + (int64_t)t * p.out_st, nc, zero);
         t = max(t, st);
         if (t >= c1) break;
-        // the K - 1 taps before row t
-        const int64_t slot = p.state ? slot_of(p.slots, s, p.nslots) : -1;
-        for (int k = 0; k < K - 1; ++k) {
-            const int at = t - (K - 1) + k;
-            if (at >= st) {
-                ld_run<V, T>(x + (int64_t)at * p.x_st, nc, tap[k]);
-            } else {
-                const int col = K + at - st;
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    tap[k][v] = slot >= 0 && v < nc ? p.state[(slot * p.C + c + v) * K + col] : 0.f;
-            }
-        }
+        conv_taps<T, V, KM + R - 1>(p, x, K, s, st, t, c, nc, tap);
         const int stop = min(en, c1);
-        for (; t < stop; ++t) {
-            ld_run<V, T>(x + (int64_t)t * p.x_st, nc, tap[K - 1]);
-            float o[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float acc = bias[v];
-                for (int k = 0; k < K; ++k) acc = __builtin_fmaf(w[k][v], tap[k][v], acc);
-                o[v] = p.silu ? acc * conv_sigmoid(acc) : acc;
-            }
-            st_run<V, T>(out + (int64_t)t * p.out_st, nc, o);
-            for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-                for (int v = 0; v < V; ++v) tap[k][v] = tap[k + 1][v];
-        }
+        while (t + R <= stop) rows(std::true_type{}, R);
+        if (t < stop) rows(std::false_type{}, stop - t);
     }
     for (; p.fill && t < c1; ++t) st_run<V, T>(out + (int64_t)t * p.out_st, nc, zero);
 }
@@ -120,7 +147,7 @@ __global__ __launch_bounds__(256) void conv_pk_window(ConvPk p) {
 
 template <typename T, int KT, int V>
 __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
-    constexpr int KM = KT ? KT : kMaxTaps;
+    constexpr int KM = KT ? KT : kMaxTaps, R = KT ? kConvRows : 1;
     const int K = KT ? KT : p.K;
     const int lane = threadIdx.x & 63;
     const int nblk = (p.C + 64 * V - 1) / (64 * V);
@@ -132,16 +159,14 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
     const T* x = static_cast<const T*>(p.x) + c;
     const T* dout = static_cast<const T*>(p.dout) + c;
     T* dx = static_cast<T*>(p.out) + c;
-    float w[KM][V], bias[V], tap[KM][V], g[KM][V], dw[KM][V], db[V];
+    // tap[K - 1 + i]: row r + i of x; g[i + k]: of row r + i - (K - 1) + k
+    float w[KM][V], bias[V], tap[KM + R - 1][V], g[KM + R - 1][V], dw[KM][V], db[V];
+    conv_weights<V, KM>(p, K, c, nc, w, bias);
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        bias[v] = p.b && v < nc ? p.b[c + v] : 0.f;
-        db[v] = 0.f;
-        for (int k = 0; k < K; ++k) {
-            w[k][v] = v < nc ? p.w[(int64_t)(c + v) * K + k] : 0.f;
-            dw[k][v] = 0.f;
-        }
-    }
+        for (int v = 0; v < V; ++v) dw[k][v] = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) db[v] = 0.f;
     const int c0 = (int)(ck * p.chunk), c1 = (int)min(p.rows, ck * p.chunk + p.chunk);
     int t = c0;
     const float zero[V] = {};
@@ -151,60 +176,70 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
         for (; p.out && p.fill && t < min(st, c1); ++t) st_run<V, T>(dx + (int64_t)t * p.out_st, nc, zero);
         t = max(t, st);
         if (t >= c1) break;
-        for (int k = 0; k < K - 1; ++k) {
-            const int at = t - (K - 1) + k;
-            if (at >= st) {
-                ld_run<V, T>(x + (int64_t)at * p.x_st, nc, tap[k]);
-            } else {
-#pragma unroll
-                for (int v = 0; v < V; ++v) tap[k][v] = 0.f;
-            }
-        }
-        // g[k]: of row r - k; rows of this run give dw, the K - 1 behind it dx only
-        for (int k = 0; k < K; ++k)
+        conv_taps<T, V, KM + R - 1>(p, x, K, s, st, t, c, nc, tap);
+        for (int k = 0; k < K - 1; ++k)
 #pragma unroll
             for (int v = 0; v < V; ++v) g[k][v] = 0.f;
         const int stop = min(en, c1);
-        for (int r = t; r < stop + K - 1; ++r) {
-            for (int k = K - 1; k > 0; --k)
+        // R rows from r: g of them, and dx of the rows K - 1 before.  Rows of this part give
+        // dw; the K - 1 behind it, where the sequence goes on, dx only.
+        int r = t;
+        auto rows = [&](auto whole) __attribute__((always_inline)) {
+            constexpr bool W = decltype(whole)::value;  // all R rows in the part
+            float d[R][V];
 #pragma unroll
-                for (int v = 0; v < V; ++v) g[k][v] = g[k - 1][v];
-            if (r < en) {
-                float d[V];
-                ld_run<V, T>(x + (int64_t)r * p.x_st, nc, tap[K - 1]);
-                ld_run<V, T>(dout + (int64_t)r * p.dout_st, nc, d);
+            for (int i = 0; i < R; ++i) {
+                if (W || r + i < en) {
+                    ld_run<V, T>(x + (int64_t)(r + i) * p.x_st, nc, tap[K - 1 + i]);
+                    ld_run<V, T>(dout + (int64_t)(r + i) * p.dout_st, nc, d[i]);
+                }
+            }
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    float acc = bias[v];
-                    for (int k = 0; k < K; ++k) acc = __builtin_fmaf(w[k][v], tap[k][v], acc);
+            for (int i = 0; i < R; ++i) {
+                if (W || r + i < en) {
                     if (p.silu) {
-                        const float sg = conv_sigmoid(acc);
-                        d[v] *= sg * (1.f + acc * (1.f - sg));
+#pragma unroll
+                        for (int v = 0; v < V; ++v) {
+                            float acc = bias[v];
+                            for (int k = 0; k < K; ++k) acc = __builtin_fmaf(w[k][v], tap[i + k][v], acc);
+                            const float sg = conv_sigmoid(acc);
+                            d[i][v] *= sg * __builtin_fmaf(acc, 1.f - sg, 1.f);
+                        }
                     }
-                    g[0][v] = d[v];
-                    if (r < stop) {
-                        db[v] += d[v];
-                        for (int k = 0; k < K; ++k) dw[k][v] = __builtin_fmaf(d[v], tap[k][v], dw[k][v]);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) g[K - 1 + i][v] = d[i][v];
+                    if (W || r + i < stop) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) {
+                            db[v] += d[i][v];
+                            for (int k = 0; k < K; ++k) dw[k][v] = __builtin_fmaf(d[i][v], tap[i + k][v], dw[k][v]);
+                        }
                     }
+                } else {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) g[K - 1 + i][v] = 0.f;
                 }
-                for (int k = 0; k < K - 1; ++k)
+                const int at = r + i - (K - 1);
+                if (p.out && at >= t && (W || at < stop)) {
+                    float o[V];
 #pragma unroll
-                    for (int v = 0; v < V; ++v) tap[k][v] = tap[k + 1][v];
-            } else {
-#pragma unroll
-                for (int v = 0; v < V; ++v) g[0][v] = 0.f;
+                    for (int v = 0; v < V; ++v) {
+                        o[v] = 0.f;
+                        for (int k = 0; k < K; ++k) o[v] = __builtin_fmaf(w[K - 1 - k][v], g[i + k][v], o[v]);
+                    }
+                    st_run<V, T>(dx + (int64_t)at * p.out_st, nc, o);
+                }
             }
-            const int at = r - (K - 1);
-            if (p.out && at >= t) {
-                float o[V];
+            for (int k = 0; k < K - 1; ++k)
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    o[v] = 0.f;
-                    for (int k = 0; k < K; ++k) o[v] = __builtin_fmaf(w[k][v], g[k][v], o[v]);
+                    tap[k][v] = tap[k + R][v];
+                    g[k][v] = g[k + R][v];
                 }
-                st_run<V, T>(dx + (int64_t)at * p.out_st, nc, o);
-            }
-        }
+            r += R;
+        };
+        while (r + R <= stop) rows(std::true_type{});
+        while (r < stop + K - 1) rows(std::false_type{});
         t = stop;
     }
     for (; p.out && p.fill && t < c1; ++t) st_run<V, T>(dx + (int64_t)t * p.out_st, nc, zero);
@@ -214,22 +249,31 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
     st_run<V, float>(part + (int64_t)K * p.C, nc, db);
 }
 
-// The chunks' sums in order: the same result every time.
+// The chunks' sums in order: the same result every time.  16 threads a column,
+// four loads in flight each.
 __global__ __launch_bounds__(256) void conv_pk_join(ConvPk p) {
-    __shared__ float red[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6, k = blockIdx.y;
-    float s = 0.f;
-    if (c < p.C)
-        for (int64_t i = q; i < p.nchunk; i += 4) s += p.part[(i * (p.K + 1) + k) * (int64_t)p.C + c];
-    red[q][threadIdx.x & 63] = s;
+    __shared__ float red[16][17];
+    const int x = threadIdx.x & 15, q = threadIdx.x >> 4, c = blockIdx.x * 16 + x, k = blockIdx.y;
+    const int64_t pitch = (int64_t)(p.K + 1) * p.C;
+    const float* src = p.part + (int64_t)k * p.C + c;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < p.C) {
+        int64_t i = q;
+        for (; i + 48 < p.nchunk; i += 64) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += src[(i + 16 * j) * pitch];
+        }
+        for (; i < p.nchunk; i += 16) s[0] += src[i * pitch];
+    }
+    red[q][x] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
     if (q == 0 && c < p.C) {
-        const int l = threadIdx.x;
-        s = (red[0][l] + red[1][l]) + (red[2][l] + red[3][l]);
+        float a = 0.f;
+        for (int j = 0; j < 16; ++j) a += red[j][x];
         if (k < p.K) {
-            if (p.dw) p.dw[(int64_t)c * p.K + k] = s;
+            if (p.dw) p.dw[(int64_t)c * p.K + k] = a;
         } else if (p.db) {
-            p.db[c] = s;
+            p.db[c] = a;
         }
     }
 }
@@ -244,7 +288,8 @@ struct ConvSlotParams {
     void* out; int64_t out_sb;
 };
 
-template <typename T>
+// KT: 4 or 2 with 16- or 8-byte windows, or 0 for any width.
+template <typename T, int KT>
 __global__ __launch_bounds__(256) void conv_slot_step(ConvSlotParams p) {
     const int b = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
     if (c >= p.C) return;
@@ -254,16 +299,38 @@ __global__ __launch_bounds__(256) void conv_slot_step(ConvSlotParams p) {
         store_f32<T>(out, 0.f);
         return;
     }
-    float* win = p.state + (slot * p.C + c) * p.K;
-    const float* w = p.w + (int64_t)c * p.K;
+    const int K = KT ? KT : p.K;
+    float* win = p.state + (slot * p.C + c) * K;
+    const float* w = p.w + (int64_t)c * K;
     const float xv = load_f32<T>(static_cast<const T*>(p.x) + b * p.x_sb + c);
     float acc = p.b ? p.b[c] : 0.f;
-    for (int k = 0; k < p.K; ++k) {
-        const float v = k + 1 < p.K ? win[k + 1] : xv;
-        win[k] = v;
-        acc = __builtin_fmaf(v, w[k], acc);
+    if constexpr (KT != 0) {
+        float v[KT], wv[KT];
+        __builtin_memcpy(v, __builtin_assume_aligned(win, 4 * KT), 4 * KT);
+        __builtin_memcpy(wv, __builtin_assume_aligned(w, 4 * KT), 4 * KT);
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+            v[k] = k + 1 < KT ? v[k + 1] : xv;
+            acc = __builtin_fmaf(v[k], wv[k], acc);
+        }
+        __builtin_memcpy(__builtin_assume_aligned(win, 4 * KT), v, 4 * KT);
+    } else {
+        for (int k = 0; k < K; ++k) {
+            const float v = k + 1 < K ? win[k + 1] : xv;
+            win[k] = v;
+            acc = __builtin_fmaf(v, w[k], acc);
+        }
     }
     store_f32<T>(out, p.silu ? acc * conv_sigmoid(acc) : acc);
+}
+
+template <typename T>
+static void conv_slot_launch(const ConvSlotParams& p, hipStream_t s) {
+    const dim3 grid(ceil_div(p.C, 256), p.nb);
+    const uintptr_t at = (uintptr_t)p.state | (uintptr_t)p.w;
+    if (p.K == 4 && (at & 15u) == 0) hipLaunchKernelGGL((conv_slot_step<T, 4>), grid, dim3(256), 0, s, p);
+    else if (p.K == 2 && (at & 7u) == 0) hipLaunchKernelGGL((conv_slot_step<T, 2>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((conv_slot_step<T, 0>), grid, dim3(256), 0, s, p);
 }
 
 static int conv_pk_make(const mamba_conv1d_packed_args* a, ConvPk* o) {
@@ -289,7 +356,6 @@ static int conv_pk_make(const mamba_conv1d_packed_args* a, ConvPk* o) {
     return MAMBA_OK;
 }
 
-template <typename T, int KT>
 static uint32_t conv_pk_grid(const ConvPk& p, int V) {
     return (uint32_t)((p.nchunk * ((p.C + 64 * V - 1) / (64 * V)) + 3) / 4);
 }
@@ -297,20 +363,20 @@ static uint32_t conv_pk_grid(const ConvPk& p, int V) {
 template <typename T>
 static void conv_pk_fwd_launch(const ConvPk& p, hipStream_t s) {
     switch (p.K) {
-        case 2: hipLaunchKernelGGL((conv_pk_fwd<T, 2, 4>), dim3(conv_pk_grid<T, 2>(p, 4)), dim3(256), 0, s, p); break;
-        case 3: hipLaunchKernelGGL((conv_pk_fwd<T, 3, 4>), dim3(conv_pk_grid<T, 3>(p, 4)), dim3(256), 0, s, p); break;
-        case 4: hipLaunchKernelGGL((conv_pk_fwd<T, 4, 4>), dim3(conv_pk_grid<T, 4>(p, 4)), dim3(256), 0, s, p); break;
-        default: hipLaunchKernelGGL((conv_pk_fwd<T, 0, 1>), dim3(conv_pk_grid<T, 0>(p, 1)), dim3(256), 0, s, p);
+        case 2: hipLaunchKernelGGL((conv_pk_fwd<T, 2, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
+        case 3: hipLaunchKernelGGL((conv_pk_fwd<T, 3, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
+        case 4: hipLaunchKernelGGL((conv_pk_fwd<T, 4, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
+        default: hipLaunchKernelGGL((conv_pk_fwd<T, 0, 1>), dim3(conv_pk_grid(p, 1)), dim3(256), 0, s, p);
     }
 }
 
 template <typename T>
 static void conv_pk_bwd_launch(const ConvPk& p, hipStream_t s) {
     switch (p.K) {
-        case 2: hipLaunchKernelGGL((conv_pk_bwd<T, 2, 4>), dim3(conv_pk_grid<T, 2>(p, 4)), dim3(256), 0, s, p); break;
-        case 3: hipLaunchKernelGGL((conv_pk_bwd<T, 3, 4>), dim3(conv_pk_grid<T, 3>(p, 4)), dim3(256), 0, s, p); break;
-        case 4: hipLaunchKernelGGL((conv_pk_bwd<T, 4, 4>), dim3(conv_pk_grid<T, 4>(p, 4)), dim3(256), 0, s, p); break;
-        default: hipLaunchKernelGGL((conv_pk_bwd<T, 0, 1>), dim3(conv_pk_grid<T, 0>(p, 1)), dim3(256), 0, s, p);
+        case 2: hipLaunchKernelGGL((conv_pk_bwd<T, 2, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
+        case 3: hipLaunchKernelGGL((conv_pk_bwd<T, 3, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
+        case 4: hipLaunchKernelGGL((conv_pk_bwd<T, 4, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
+        default: hipLaunchKernelGGL((conv_pk_bwd<T, 0, 1>), dim3(conv_pk_grid(p, 1)), dim3(256), 0, s, p);
     }
 }
 
@@ -368,7 +434,7 @@ extern "C" int mamba_conv1d_packed_bwd(const mamba_conv1d_packed_args* a, void* 
         if (a->io_dtype == MAMBA_BF16) conv_pk_bwd_launch<bf16_t>(p, s);
         else conv_pk_bwd_launch<float>(p, s);
     }
-    if (p.dw || p.db) hipLaunchKernelGGL(conv_pk_join, dim3(ceil_div(p.C, 64), p.K + 1), dim3(256), 0, s, p);
+    if (p.dw || p.db) hipLaunchKernelGGL(conv_pk_join, dim3(ceil_div(p.C, 16), p.K + 1), dim3(256), 0, s, p);
     MAMBA_CHECK_LAUNCH();
     return MAMBA_OK;
 }
@@ -387,9 +453,8 @@ extern "C" int mamba_conv1d_step_slots(const mamba_conv1d_step_slots_args* a, ma
     p.nb = a->batch; p.C = a->channels; p.K = a->kernel; p.silu = a->silu != 0;
     p.x = a->x; p.x_sb = a->x_sb; p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
     p.w = a->w; p.b = a->bias; p.out = a->out; p.out_sb = a->out_sb;
-    const dim3 grid(ceil_div(p.C, 256), p.nb);
-    if (a->io_dtype == MAMBA_BF16) hipLaunchKernelGGL(conv_slot_step<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(conv_slot_step<float>, grid, dim3(256), 0, (hipStream_t)stream, p);
+    if (a->io_dtype == MAMBA_BF16) conv_slot_launch<bf16_t>(p, (hipStream_t)stream);
+    else conv_slot_launch<float>(p, (hipStream_t)stream);
     MAMBA_CHECK_LAUNCH();
     return MAMBA_OK;
 }

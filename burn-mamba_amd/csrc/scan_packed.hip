@@ -952,8 +952,9 @@ struct ScanSlotParams {
     void* y; int64_t y_sb;
 };
 
+// Any dstate: a thread per channel.
 template <typename T>
-__global__ __launch_bounds__(256) void scan_slot_step(ScanSlotParams p) {
+__global__ __launch_bounds__(256) void scan_slot_any(ScanSlotParams p) {
     const int b = blockIdx.y, d = blockIdx.x * 256 + threadIdx.x;
     if (d >= p.D) return;
     T* y = static_cast<T*>(p.y) + b * p.y_sb + d;
@@ -981,6 +982,88 @@ __global__ __launch_bounds__(256) void scan_slot_step(ScanSlotParams p) {
         acc *= zv * pk_sigmoid(zv);
     }
     store_f32<T>(y, acc);
+}
+
+// dstate 8, 16, 32 or 64: a channel over N / 4 lanes with 16 bytes of its state
+// each, CPT channels a thread.  The state is read and written once (HBM-bound:
+// 8 N bytes a channel against some 12 of everything else), so its loads are
+// issued first and none waits under a branch: what is optional is read through a
+// pointer to something that is there, and dropped.
+template <typename T, int N, int CPT>
+__global__ __launch_bounds__(256) void scan_slot_step(ScanSlotParams p) {
+    constexpr int LPC = N / 4, CPB = 256 / LPC;
+    const int b = blockIdx.y, q = threadIdx.x % LPC;
+    const int64_t slot = slot_of(p.slots, b, p.nslots);
+    const int base = blockIdx.x * CPB * CPT + threadIdx.x / LPC;
+    T* y = static_cast<T*>(p.y) + b * p.y_sb;
+    if (slot < 0) {
+#pragma unroll
+        for (int k = 0; k < CPT; ++k)
+            if (q == 0 && base + k * CPB < p.D) store_f32<T>(y + base + k * CPB, 0.f);
+        return;
+    }
+    const T* u = static_cast<const T*>(p.u) + b * p.u_sb;
+    const T* dl = static_cast<const T*>(p.dl) + b * p.dl_sb;
+    const T* z = p.z ? static_cast<const T*>(p.z) + b * p.z_sb : dl;
+    float4* state = reinterpret_cast<float4*>(p.state + slot * p.D * N) + q;
+    float4 h[CPT], A[CPT];
+    float uv[CPT], dv[CPT], zv[CPT], Dv[CPT], bias[CPT];
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) {
+        const int d = min(base + k * CPB, p.D - 1);
+        h[k] = ld_nt4(state + (int64_t)d * LPC);
+        A[k] = *(reinterpret_cast<const float4*>(p.A + (int64_t)d * N) + q);
+        dv[k] = load_f32<T>(dl + d);
+        uv[k] = load_f32<T>(u + d);
+        zv[k] = load_f32<T>(z + d);
+        Dv[k] = *(p.Dv ? p.Dv + d : p.A);
+        bias[k] = *(p.bias ? p.bias + d : p.A);
+    }
+    float bv[4], cv[4];
+    ld_run<4, T>(static_cast<const T*>(p.B) + b * p.B_sb + 4 * q, 4, bv);
+    ld_run<4, T>(static_cast<const T*>(p.C) + b * p.C_sb + 4 * q, 4, cv);
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) {
+        if (p.bias) dv[k] += bias[k];
+        if (p.softplus) dv[k] = pk_softplus(dv[k]);
+        const float du = dv[k] * uv[k], d2 = dv[k] * kLog2e;
+        h[k].x = __builtin_fmaf(h[k].x, __builtin_amdgcn_exp2f(d2 * A[k].x), du * bv[0]);
+        h[k].y = __builtin_fmaf(h[k].y, __builtin_amdgcn_exp2f(d2 * A[k].y), du * bv[1]);
+        h[k].z = __builtin_fmaf(h[k].z, __builtin_amdgcn_exp2f(d2 * A[k].z), du * bv[2]);
+        h[k].w = __builtin_fmaf(h[k].w, __builtin_amdgcn_exp2f(d2 * A[k].w), du * bv[3]);
+        float acc = __builtin_fmaf(h[k].w, cv[3], __builtin_fmaf(h[k].z, cv[2], __builtin_fmaf(h[k].y, cv[1], h[k].x * cv[0])));
+        acc = group_sum_last<LPC>(acc);
+        const int d = base + k * CPB;
+        if (d >= p.D) continue;
+        st_nt4(state + (int64_t)d * LPC, h[k]);
+        if (q == LPC - 1) {
+            if (p.Dv) acc = __builtin_fmaf(Dv[k], uv[k], acc);
+            if (p.z) acc *= zv[k] * pk_sigmoid(zv[k]);
+            store_f32<T>(y + d, acc);
+        }
+    }
+}
+
+template <typename T, int N>
+static void scan_slot_launch(const ScanSlotParams& p, hipStream_t s) {
+    // four channels a thread while that leaves two workgroups a CU, else one
+    constexpr int CPB = 256 / (N / 4);
+    if ((int64_t)ceil_div(p.D, 4 * CPB) * p.nb >= 512)
+        hipLaunchKernelGGL((scan_slot_step<T, N, 4>), dim3(ceil_div(p.D, 4 * CPB), p.nb), dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((scan_slot_step<T, N, 1>), dim3(ceil_div(p.D, CPB), p.nb), dim3(256), 0, s, p);
+}
+
+template <typename T>
+static void scan_slot_dispatch(const ScanSlotParams& p, hipStream_t s) {
+    const bool aligned = (((uintptr_t)p.state | (uintptr_t)p.A) & 15u) == 0;
+    switch (aligned ? p.N : 0) {
+        case 8: scan_slot_launch<T, 8>(p, s); break;
+        case 16: scan_slot_launch<T, 16>(p, s); break;
+        case 32: scan_slot_launch<T, 32>(p, s); break;
+        case 64: scan_slot_launch<T, 64>(p, s); break;
+        default: hipLaunchKernelGGL(scan_slot_any<T>, dim3(ceil_div(p.D, 256), p.nb), dim3(256), 0, s, p);
+    }
 }
 
 // ---------------------------------------------------------------- dispatch ---
@@ -1196,9 +1279,8 @@ extern "C" int mamba1_scan_step_slots(const mamba1_scan_step_slots_args* a, mamb
     p.B = a->B; p.B_sb = a->B_sb; p.C = a->C; p.C_sb = a->C_sb;
     p.A = a->A; p.Dv = a->D; p.bias = a->delta_bias;
     p.state = a->state; p.nslots = a->nslots; p.slots = a->slots; p.y = a->y; p.y_sb = a->y_sb;
-    const dim3 grid(ceil_div(p.D, 256), p.nb);
-    if (a->io_dtype == MAMBA_BF16) hipLaunchKernelGGL(scan_slot_step<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(scan_slot_step<float>, grid, dim3(256), 0, (hipStream_t)stream, p);
+    if (a->io_dtype == MAMBA_BF16) scan_slot_dispatch<bf16_t>(p, (hipStream_t)stream);
+    else scan_slot_dispatch<float>(p, (hipStream_t)stream);
     MAMBA_CHECK_LAUNCH();
     return MAMBA_OK;
 }

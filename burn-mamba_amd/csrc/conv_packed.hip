@@ -38,7 +38,7 @@ __device__ __forceinline__ float conv_sigmoid(float v) { return __builtin_amdgcn
 // KT = K as a constant, or 0: any K up to kMaxTaps (the taps then wait in a ring
 // that is shifted by one each row all the same).
 constexpr int kMaxTaps = 64;
-constexpr int kConvRows = 4;  // rows whose loads are in flight together
+constexpr int kConvRows = 4;  // rows whose loads are in flight while four others are computed
 
 // V channels' weights and bias; taps[k] = the input of row t - (K - 1) + k, k < K - 1
 template <int V, int KM>
@@ -50,12 +50,12 @@ __device__ __forceinline__ void conv_weights(const ConvPk& p, int K, int c, int 
     }
 }
 template <typename T, int V, int KM>
-__device__ __forceinline__ void conv_taps(const ConvPk& p, const T* x, int K, int s, int st, int t, int c, int nc, float (&tap)[KM][V]) {
+__device__ __forceinline__ void conv_taps(const ConvPk& p, int K, int s, int st, int t, int c, int nc, float (&tap)[KM][V]) {
     const int64_t slot = p.state ? slot_of(p.slots, s, p.nslots) : -1;
     for (int k = 0; k < K - 1; ++k) {
         const int at = t - (K - 1) + k;
         if (at >= st) {
-            ld_run<V, T>(x + (int64_t)at * p.x_st, nc, tap[k]);
+            ld_run<V, T>(static_cast<const T*>(p.x) + (int64_t)at * p.x_st + c, nc, tap[k]);
         } else {
             const int col = K + at - st;
 #pragma unroll
@@ -63,10 +63,22 @@ __device__ __forceinline__ void conv_taps(const ConvPk& p, const T* x, int K, in
         }
     }
 }
+// A row of V channels from c: FULL where C is a multiple of V, so that all V are there.
+// The row's base is in scalar registers, the lane's place 32 bits.
+template <typename T, int V, bool FULL>
+__device__ __forceinline__ void conv_load(const void* src, int64_t st, int t, int c, int nc, Elems<T, V>& e) {
+    const T* row = static_cast<const T*>(src) + t * st;
+    if (FULL) e.load(row + (uint32_t)c);
+    else e.load_part(row + (uint32_t)c, nc);
+}
+template <typename T, int V, bool FULL>
+__device__ __forceinline__ void conv_store(void* dst, int64_t st, int t, int c, int nc, const float (&o)[V]) {
+    st_run<V, T>(static_cast<T*>(dst) + t * st + (uint32_t)c, FULL ? V : nc, o);
+}
 
-template <typename T, int KT, int V>
+template <typename T, int KT, int V, bool FULL>
 __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
-    constexpr int KM = KT ? KT : kMaxTaps, R = KT ? kConvRows : 1;  // rows in flight
+    constexpr int KM = KT ? KT : kMaxTaps, R = KT ? kConvRows : 1;
     const int K = KT ? KT : p.K;
     const int lane = threadIdx.x & 63;
     const int nblk = (p.C + 64 * V - 1) / (64 * V);
@@ -75,54 +87,53 @@ __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
     if (ck >= p.nchunk) return;
     const int c = ((int)(item - ck * nblk) * 64 + lane) * V, nc = min(V, p.C - c);
     if (nc <= 0) return;
-    const T* x = static_cast<const T*>(p.x) + c;
-    T* out = static_cast<T*>(p.out) + c;
     float w[KM][V], bias[V], tap[KM + R - 1][V];
     conv_weights<V, KM>(p, K, c, nc, w, bias);
     const int c0 = (int)(ck * p.chunk), c1 = (int)min(p.rows, ck * p.chunk + p.chunk);
     int t = c0;
     const float zero[V] = {};
-    // rows t .. t + r - 1 (r <= R) of a sequence; the last K - 1 inputs move to the front
-    auto rows = [&](auto whole, int r) __attribute__((always_inline)) {
-        constexpr bool W = decltype(whole)::value;
+    Elems<T, V> raw[R];
+    auto fetch = [&](int t0, int stop) {  // rows t0 .. of those before stop
 #pragma unroll
         for (int i = 0; i < R; ++i)
-            if (W || i < r) ld_run<V, T>(x + (int64_t)(t + i) * p.x_st, nc, tap[K - 1 + i]);
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            if (!W && i >= r) break;
-            float o[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float acc = bias[v];
-                for (int k = 0; k < K; ++k) acc = __builtin_fmaf(w[k][v], tap[i + k][v], acc);
-                o[v] = acc;
-            }
-            if (p.silu) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) o[v] *= conv_sigmoid(o[v]);
-            }
-            st_run<V, T>(out + (int64_t)(t + i) * p.out_st, nc, o);
-        }
-        if (W) {
-            for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-                for (int v = 0; v < V; ++v) tap[k][v] = tap[k + R][v];
-        }
-        t += W ? R : r;
+            if (t0 + i < stop) conv_load<T, V, FULL>(p.x, p.x_st, t0 + i, c, nc, raw[i]);
     };
     for (int s = p.q.after(c0); s < p.q.n && t < c1; ++s) {
         const int st = p.q.begin(s), en = p.q.end(s);
         if (en <= t) continue;
-        for (; p.fill && t < min(st, c1); ++t) st_run<V, T>(out + (int64_t)t * p.out_st, nc, zero);
+        for (; p.fill && t < min(st, c1); ++t) conv_store<T, V, FULL>(p.out, p.out_st, t, c, nc, zero);
         t = max(t, st);
         if (t >= c1) break;
-        conv_taps<T, V, KM + R - 1>(p, x, K, s, st, t, c, nc, tap);
         const int stop = min(en, c1);
-        while (t + R <= stop) rows(std::true_type{}, R);
-        if (t < stop) rows(std::false_type{}, stop - t);
+        fetch(t, stop);
+        conv_taps<T, V, KM + R - 1>(p, K, s, st, t, c, nc, tap);
+        for (; t < stop; t += R) {
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (t + i < stop) raw[i].get(tap[K - 1 + i]);
+            fetch(t + R, stop);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                if (t + i >= stop) break;
+                float o[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    o[v] = bias[v];
+                    for (int k = 0; k < K; ++k) o[v] = __builtin_fmaf(w[k][v], tap[i + k][v], o[v]);
+                }
+                if (p.silu) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) o[v] *= conv_sigmoid(o[v]);
+                }
+                conv_store<T, V, FULL>(p.out, p.out_st, t + i, c, nc, o);
+            }
+            for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) tap[k][v] = tap[k + R][v];
+        }
+        t = stop;
     }
-    for (; p.fill && t < c1; ++t) st_run<V, T>(out + (int64_t)t * p.out_st, nc, zero);
+    for (; p.fill && t < c1; ++t) conv_store<T, V, FULL>(p.out, p.out_st, t, c, nc, zero);
 }
 
 // an offset of a sequence that differs between the lanes
@@ -145,7 +156,7 @@ __global__ __launch_bounds__(256) void conv_pk_window(ConvPk p) {
     }
 }
 
-template <typename T, int KT, int V>
+template <typename T, int KT, int V, bool FULL>
 __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
     constexpr int KM = KT ? KT : kMaxTaps, R = KT ? kConvRows : 1;
     const int K = KT ? KT : p.K;
@@ -156,9 +167,6 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
     if (ck >= p.nchunk) return;
     const int c = ((int)(item - ck * nblk) * 64 + lane) * V, nc = min(V, p.C - c);
     if (nc <= 0) return;
-    const T* x = static_cast<const T*>(p.x) + c;
-    const T* dout = static_cast<const T*>(p.dout) + c;
-    T* dx = static_cast<T*>(p.out) + c;
     // tap[K - 1 + i]: row r + i of x; g[i + k]: of row r + i - (K - 1) + k
     float w[KM][V], bias[V], tap[KM + R - 1][V], g[KM + R - 1][V], dw[KM][V], db[V];
     conv_weights<V, KM>(p, K, c, nc, w, bias);
@@ -170,64 +178,72 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
     const int c0 = (int)(ck * p.chunk), c1 = (int)min(p.rows, ck * p.chunk + p.chunk);
     int t = c0;
     const float zero[V] = {};
+    Elems<T, V> rx[R], rg[R];
+    auto fetch = [&](int r, int last) {  // rows r .. of those before last
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (r + i >= last) break;
+            conv_load<T, V, FULL>(p.x, p.x_st, r + i, c, nc, rx[i]);
+            conv_load<T, V, FULL>(p.dout, p.dout_st, r + i, c, nc, rg[i]);
+        }
+    };
     for (int s = p.q.after(c0); s < p.q.n && t < c1; ++s) {
         const int st = p.q.begin(s), en = p.q.end(s);
         if (en <= t) continue;
-        for (; p.out && p.fill && t < min(st, c1); ++t) st_run<V, T>(dx + (int64_t)t * p.out_st, nc, zero);
+        for (; p.out && p.fill && t < min(st, c1); ++t) conv_store<T, V, FULL>(p.out, p.out_st, t, c, nc, zero);
         t = max(t, st);
         if (t >= c1) break;
-        conv_taps<T, V, KM + R - 1>(p, x, K, s, st, t, c, nc, tap);
+        // rows of this part give dw; the K - 1 behind it, where the sequence goes on, dx only
+        const int stop = min(en, c1), last = min(en, stop + K - 1);
+        fetch(t, last);
+        conv_taps<T, V, KM + R - 1>(p, K, s, st, t, c, nc, tap);
         for (int k = 0; k < K - 1; ++k)
 #pragma unroll
             for (int v = 0; v < V; ++v) g[k][v] = 0.f;
-        const int stop = min(en, c1);
-        // R rows from r: g of them, and dx of the rows K - 1 before.  Rows of this part give
-        // dw; the K - 1 behind it, where the sequence goes on, dx only.
+        // R rows from r: g of them, and dx of the rows K - 1 before.  W: all of these are
+        // in the part, and nothing is asked row by row (which would part the rows in the
+        // schedule).
         int r = t;
         auto rows = [&](auto whole) __attribute__((always_inline)) {
-            constexpr bool W = decltype(whole)::value;  // all R rows in the part
-            float d[R][V];
+            constexpr bool W = decltype(whole)::value;
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                if (W || r + i < en) {
-                    ld_run<V, T>(x + (int64_t)(r + i) * p.x_st, nc, tap[K - 1 + i]);
-                    ld_run<V, T>(dout + (int64_t)(r + i) * p.dout_st, nc, d[i]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                if (W || r + i < en) {
-                    if (p.silu) {
-#pragma unroll
-                        for (int v = 0; v < V; ++v) {
-                            float acc = bias[v];
-                            for (int k = 0; k < K; ++k) acc = __builtin_fmaf(w[k][v], tap[i + k][v], acc);
-                            const float sg = conv_sigmoid(acc);
-                            d[i][v] *= sg * __builtin_fmaf(acc, 1.f - sg, 1.f);
-                        }
-                    }
-#pragma unroll
-                    for (int v = 0; v < V; ++v) g[K - 1 + i][v] = d[i][v];
-                    if (W || r + i < stop) {
-#pragma unroll
-                        for (int v = 0; v < V; ++v) {
-                            db[v] += d[i][v];
-                            for (int k = 0; k < K; ++k) dw[k][v] = __builtin_fmaf(d[i][v], tap[i + k][v], dw[k][v]);
-                        }
-                    }
+                if (W || r + i < last) {
+                    rx[i].get(tap[K - 1 + i]);
+                    rg[i].get(g[K - 1 + i]);
                 } else {
 #pragma unroll
                     for (int v = 0; v < V; ++v) g[K - 1 + i][v] = 0.f;
                 }
+            }
+            fetch(r + R, last);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                if (p.silu && (W || r + i < last)) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        float acc = bias[v];
+                        for (int k = 0; k < K; ++k) acc = __builtin_fmaf(w[k][v], tap[i + k][v], acc);
+                        const float sg = conv_sigmoid(acc);
+                        g[K - 1 + i][v] *= sg * __builtin_fmaf(acc, 1.f - sg, 1.f);
+                    }
+                }
+                if (W || r + i < stop) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        db[v] += g[K - 1 + i][v];
+                        for (int k = 0; k < K; ++k) dw[k][v] = __builtin_fmaf(g[K - 1 + i][v], tap[i + k][v], dw[k][v]);
+                    }
+                }
                 const int at = r + i - (K - 1);
-                if (p.out && at >= t && (W || at < stop)) {
+                if (p.out && (W || (at >= t && at < stop))) {
                     float o[V];
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
                         o[v] = 0.f;
                         for (int k = 0; k < K; ++k) o[v] = __builtin_fmaf(w[K - 1 - k][v], g[i + k][v], o[v]);
                     }
-                    st_run<V, T>(dx + (int64_t)at * p.out_st, nc, o);
+                    conv_store<T, V, FULL>(p.out, p.out_st, at, c, nc, o);
                 }
             }
             for (int k = 0; k < K - 1; ++k)
@@ -238,11 +254,12 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
                 }
             r += R;
         };
+        while (r < min(t + K - 1, stop + K - 1)) rows(std::false_type{});
         while (r + R <= stop) rows(std::true_type{});
         while (r < stop + K - 1) rows(std::false_type{});
         t = stop;
     }
-    for (; p.out && p.fill && t < c1; ++t) st_run<V, T>(dx + (int64_t)t * p.out_st, nc, zero);
+    for (; p.out && p.fill && t < c1; ++t) conv_store<T, V, FULL>(p.out, p.out_st, t, c, nc, zero);
     if (!p.part) return;
     float* part = p.part + (ck * (K + 1)) * (int64_t)p.C + c;
     for (int k = 0; k < K; ++k) st_run<V, float>(part + (int64_t)k * p.C, nc, dw[k]);
@@ -350,7 +367,7 @@ static int conv_pk_make(const mamba_conv1d_packed_args* a, ConvPk* o) {
     p.x = a->x; p.x_st = a->x_st; p.w = a->w; p.b = a->bias;
     // chunks of rows: long ones re-read fewer rows at their edges, as many as keep the chip full
     // (and at most 2^20 items of 64 channels, which keeps the grid small)
-    p.chunk = 32;
+    p.chunk = 64;
     while ((a->rows + p.chunk - 1) / p.chunk * ceil_div(p.C, 64) > (1ll << 20)) p.chunk *= 2;
     p.nchunk = (a->rows + p.chunk - 1) / p.chunk;
     return MAMBA_OK;
@@ -360,23 +377,25 @@ static uint32_t conv_pk_grid(const ConvPk& p, int V) {
     return (uint32_t)((p.nchunk * ((p.C + 64 * V - 1) / (64 * V)) + 3) / 4);
 }
 
-template <typename T>
-static void conv_pk_fwd_launch(const ConvPk& p, hipStream_t s) {
-    switch (p.K) {
-        case 2: hipLaunchKernelGGL((conv_pk_fwd<T, 2, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
-        case 3: hipLaunchKernelGGL((conv_pk_fwd<T, 3, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
-        case 4: hipLaunchKernelGGL((conv_pk_fwd<T, 4, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
-        default: hipLaunchKernelGGL((conv_pk_fwd<T, 0, 1>), dim3(conv_pk_grid(p, 1)), dim3(256), 0, s, p);
+template <typename T, int KT, int V>
+static void conv_pk_launch(const ConvPk& p, bool back, hipStream_t s) {
+    const dim3 grid(conv_pk_grid(p, V));
+    if (p.C % V == 0) {
+        if (back) hipLaunchKernelGGL((conv_pk_bwd<T, KT, V, true>), grid, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((conv_pk_fwd<T, KT, V, true>), grid, dim3(256), 0, s, p);
+    } else {
+        if (back) hipLaunchKernelGGL((conv_pk_bwd<T, KT, V, false>), grid, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((conv_pk_fwd<T, KT, V, false>), grid, dim3(256), 0, s, p);
     }
 }
 
 template <typename T>
-static void conv_pk_bwd_launch(const ConvPk& p, hipStream_t s) {
+static void conv_pk_dispatch(const ConvPk& p, bool back, hipStream_t s) {
     switch (p.K) {
-        case 2: hipLaunchKernelGGL((conv_pk_bwd<T, 2, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
-        case 3: hipLaunchKernelGGL((conv_pk_bwd<T, 3, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
-        case 4: hipLaunchKernelGGL((conv_pk_bwd<T, 4, 4>), dim3(conv_pk_grid(p, 4)), dim3(256), 0, s, p); break;
-        default: hipLaunchKernelGGL((conv_pk_bwd<T, 0, 1>), dim3(conv_pk_grid(p, 1)), dim3(256), 0, s, p);
+        case 2: conv_pk_launch<T, 2, 4>(p, back, s); break;
+        case 3: conv_pk_launch<T, 3, 4>(p, back, s); break;
+        case 4: conv_pk_launch<T, 4, 4>(p, back, s); break;
+        default: conv_pk_launch<T, 0, 1>(p, back, s);
     }
 }
 
@@ -397,8 +416,8 @@ extern "C" int mamba_conv1d_packed_fwd(const mamba_conv1d_packed_args* a, mamba_
     p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
     hipStream_t s = (hipStream_t)stream;
     const bool bf16 = a->io_dtype == MAMBA_BF16;
-    if (bf16) conv_pk_fwd_launch<bf16_t>(p, s);
-    else conv_pk_fwd_launch<float>(p, s);
+    if (bf16) conv_pk_dispatch<bf16_t>(p, false, s);
+    else conv_pk_dispatch<float>(p, false, s);
     MAMBA_CHECK_LAUNCH();
     if (p.state && p.q.n) {
         const dim3 grid((uint32_t)std::min<int64_t>(((int64_t)p.q.n * p.C + 255) / 256, 1 << 16));
@@ -431,8 +450,8 @@ extern "C" int mamba_conv1d_packed_bwd(const mamba_conv1d_packed_args* a, void* 
     p.part = need ? static_cast<float*>(ws) : nullptr; p.dw = a->dw; p.db = a->dbias;
     hipStream_t s = (hipStream_t)stream;
     if (p.rows) {
-        if (a->io_dtype == MAMBA_BF16) conv_pk_bwd_launch<bf16_t>(p, s);
-        else conv_pk_bwd_launch<float>(p, s);
+        if (a->io_dtype == MAMBA_BF16) conv_pk_dispatch<bf16_t>(p, true, s);
+        else conv_pk_dispatch<float>(p, true, s);
     }
     if (p.dw || p.db) hipLaunchKernelGGL(conv_pk_join, dim3(ceil_div(p.C, 16), p.K + 1), dim3(256), 0, s, p);
     MAMBA_CHECK_LAUNCH();

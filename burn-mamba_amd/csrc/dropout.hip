@@ -62,10 +62,71 @@ __global__ __launch_bounds__(256) void dropout_any(DropoutParams p) {
     }
 }
 
+// Rows one behind the other (rows = 1), or of a multiple of V columns: V = 8
+// (bf16) or 4 (f32) elements, 16 bytes, a thread and turn, two turns' loads in
+// flight.  The generator takes about 30 32-bit operations an element (a 32 x 32
+// -> 64 product counts four), which bf16's 4 to 6 bytes an element only just
+// cover: HBM-bound, with little to spare.
+template <typename T, int V, bool RES>
+__global__ __launch_bounds__(256) void dropout_vec(DropoutParams p) {
+    const int64_t n = p.rows * p.cols, units = (n + V - 1) / V, per = (p.cols + V - 1) / V;
+    const uint64_t seed = (uint64_t)p.rng[0], call = (uint64_t)p.rng[1] + p.offset;
+    const int64_t stride = gridDim.x * 256ll;
+    constexpr int U = 2;
+    for (int64_t k0 = blockIdx.x * 256ll + threadIdx.x; k0 < units; k0 += U * stride) {
+        Elems<T, V> x[U], r[U];
+        int64_t row[U], c[U];
+        int left[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t k = k0 + u * stride;
+            row[u] = p.rows > 1 ? k / per : 0;
+            c[u] = (k - row[u] * per) * V;
+            left[u] = k < units ? (int)min((int64_t)V, p.cols - c[u]) : 0;
+            const T* xs = static_cast<const T*>(p.x) + row[u] * p.x_sr + c[u];
+            const T* rs = static_cast<const T*>(p.res) + row[u] * p.res_sr + c[u];
+            if (left[u] >= V) {
+                x[u].load(xs);
+                if (RES) r[u].load(rs);
+            } else {
+                x[u].load_part(xs, left[u]);
+                if (RES) r[u].load_part(rs, left[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (left[u] <= 0) break;
+            const int64_t first = (k0 + u * stride) * (V / 4);  // its first block of the generator
+            float xv[V], rv[V];
+            x[u].get(xv);
+            if (RES) r[u].get(rv);
+#pragma unroll
+            for (int b = 0; b < V / 4; ++b) {
+                uint32_t w[4];
+                philox4x32((uint64_t)(first + b), call, seed, w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = w[e] >= p.threshold ? xv[4 * b + e] * p.scale : 0.f;
+                    if (RES) v += rv[4 * b + e];
+                    xv[4 * b + e] = v;
+                }
+            }
+            st_run<V, T>(static_cast<T*>(p.out) + row[u] * p.out_sr + c[u], left[u], xv);
+        }
+    }
+}
+
 template <typename T>
 static void dropout_launch(const DropoutParams& p, hipStream_t s) {
-    const int64_t blocks = (p.rows * p.cols + 3) / 4;
-    hipLaunchKernelGGL(dropout_any<T>, dim3((uint32_t)std::min<int64_t>((blocks + 255) / 256, 8192)), dim3(256), 0, s, p);
+    constexpr int V = 16 / sizeof(T);
+    auto grid = [](int64_t threads) { return dim3((uint32_t)std::min<int64_t>((threads + 255) / 256, 16384)); };
+    if (p.rows == 1 || p.cols % V == 0) {
+        const int64_t units = (p.rows * p.cols + V - 1) / V;
+        if (p.res) hipLaunchKernelGGL((dropout_vec<T, V, true>), grid((units + 1) / 2), dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((dropout_vec<T, V, false>), grid((units + 1) / 2), dim3(256), 0, s, p);
+    } else {
+        hipLaunchKernelGGL(dropout_any<T>, grid((p.rows * p.cols + 3) / 4), dim3(256), 0, s, p);
+    }
 }
 
 }  // namespace mamba

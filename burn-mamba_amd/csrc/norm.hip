@@ -4,8 +4,15 @@
 //   xh = (x - mean) rstd,  rstd = 1 / sqrt(mean((x - mean)^2) + eps),  y = xh w + b
 //   g = dy w:  dx = rstd (g - mean(g) - xh mean(g xh)),  dw = sum_r dy xh,  db = sum_r dy
 //
-// The variance is the mean of the squared distances from the mean (a second
-// sweep over the row), not a difference of two large sums.
+// The variance is the mean of the squared distances from the mean, not a
+// difference of two large sums.
+//
+// About ten operations an element against two elements moved (forward) or three
+// (backward): HBM-bound.  Rows of up to 10240 elements stay in registers (each
+// element is read once): G lanes hold a row, 8 (bf16) or 4 (f32) consecutive
+// elements a lane and step, G = 16, 64 or 256 by the row's width.  The backward's
+// workgroups take rows in turn and sum dw and db of their columns in registers,
+// joined in LDS and, over the workgroups, by ln_dw_join, in a fixed order.
 #include <algorithm>
 
 #include "pack.h"
@@ -109,29 +116,251 @@ __global__ __launch_bounds__(256) void ln_dw_wide(LnParams p) {
     }
 }
 
-// The parts in order of their number: the same sums every time.
-__global__ __launch_bounds__(256) void ln_dw_join(LnParams p) {
-    __shared__ float red[2][4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-    float sw = 0.f, sb = 0.f;
-    if (c < p.cols)
-        for (int i = q; i < p.parts; i += 4) {
-            sw += p.part[(int64_t)(2 * i) * p.cols + c];
-            sb += p.part[(int64_t)(2 * i + 1) * p.cols + c];
-        }
-    red[0][q][threadIdx.x & 63] = sw;
-    red[1][q][threadIdx.x & 63] = sb;
-    __syncthreads();
-    if (q < 2 && c < p.cols) {
-        const int l = threadIdx.x & 63;
-        float* out = q ? p.db : p.dw;
-        if (out) out[c] = (red[q][0][l] + red[q][1][l]) + (red[q][2][l] + red[q][3][l]);
+// ---- rows in registers
+// Sum over aligned groups of G lanes in every lane; over the workgroup for G = 256
+// (red: 8 floats; the caller's calls alternate halves, so one barrier is enough).
+template <int CTRL>
+__device__ __forceinline__ float ln_dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int G>
+__device__ __forceinline__ float ln_sum(float v, float* red) {
+    if constexpr (G == 16) {
+        v += ln_dpp<0xB1>(v);   // xor 1
+        v += ln_dpp<0x4E>(v);   // xor 2
+        v += ln_dpp<0x141>(v);  // the other quad of the half row
+        v += ln_dpp<0x140>(v);  // the other half row
+        return v;
+    } else if constexpr (G == 64) {
+        return wave_sum_dpp(v);
+    } else {
+        v = wave_sum_dpp(v);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        return (red[0] + red[1]) + (red[2] + red[3]);
     }
+}
+
+// elements of a lane and step: 16 bytes
+template <typename T>
+constexpr int kLnE = 16 / (int)sizeof(T);
+
+// G lanes a row, V steps: cols <= G V kLnE.
+template <typename T, int G, int V>
+__global__ __launch_bounds__(256) void ln_fwd_rows(LnParams p) {
+    constexpr int E = kLnE<T>;
+    __shared__ float red[8];
+    const int l = threadIdx.x % G;
+    const int64_t r = blockIdx.x * (int64_t)(256 / G) + threadIdx.x / G;
+    if (r >= p.rows) return;  // whole groups (for G = 256 the grid is the rows)
+    const T* x = static_cast<const T*>(p.x) + r * p.x_sr;
+    T* y = static_cast<T*>(p.out) + r * p.out_sr;
+    float v[V][E];
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int c = (k * G + l) * E;
+        ld_run<E, T>(x + c, p.cols - c, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+#pragma unroll
+        for (int i = 0; i < E; ++i) s += v[k][i];
+    const float inv = 1.f / (float)p.cols, mean = ln_sum<G>(s, red) * inv;
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int c = (k * G + l) * E;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            v[k][i] = c + i < p.cols ? v[k][i] - mean : 0.f;
+            s = __builtin_fmaf(v[k][i], v[k][i], s);
+        }
+    }
+    const float rstd = 1.f / sqrtf(ln_sum<G>(s, red + 4) * inv + p.eps);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int c = (k * G + l) * E, n = p.cols - c;
+        if (n <= 0) break;
+        float w[E], b[E];
+        if (p.w) ld_run<E, float>(p.w + c, n, w);
+        if (p.b) ld_run<E, float>(p.b + c, n, b);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            float o = v[k][i] * rstd;
+            if (p.w) o *= w[i];
+            if (p.b) o += b[i];
+            v[k][i] = o;
+        }
+        st_run<E, T>(y + c, n, v[k]);
+    }
+    if (l == 0) {
+        if (p.mean) p.mean[r] = mean;
+        if (p.rstd) p.rstd[r] = rstd;
+    }
+}
+
+// The workgroups take their rows in turn, the next row's loads issued before this
+// one's sums; part[blockIdx.x] gets the workgroup's dw and db.
+template <typename T, int G, int V>
+__global__ __launch_bounds__(256) void ln_bwd_rows(LnParams p) {
+    constexpr int E = kLnE<T>, RB = 256 / G;  // rows at a time
+    __shared__ float red[16];
+    __shared__ float s_w[G < 256 ? G * V * E : 1], s_b[G < 256 ? G * V * E : 1];
+    const int l = threadIdx.x % G, sub = threadIdx.x / G;
+    float w[V][E], dw[V][E], db[V][E];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int c = (k * G + l) * E;
+        if (p.w) ld_run<E, float>(p.w + c, p.cols - c, w[k]);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            if (!p.w) w[k][i] = 1.f;
+            dw[k][i] = db[k][i] = 0.f;
+        }
+    }
+    const float inv = 1.f / (float)p.cols;
+    Elems<T, E> rx[V], rg[V];
+    float mean = 0.f, rstd = 0.f;
+    auto fetch = [&](int64_t r) {
+        if (r >= p.rows) return;
+        const T* x = static_cast<const T*>(p.x) + r * p.x_sr;
+        const T* dy = static_cast<const T*>(p.dy) + r * p.dy_sr;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E, n = p.cols - c;
+            if (n >= E) {
+                rx[k].load(x + c);
+                rg[k].load(dy + c);
+            } else {
+                rx[k].load_part(x + c, n);
+                rg[k].load_part(dy + c, n);
+            }
+        }
+        mean = p.mean[r];
+        rstd = p.rstd[r];
+    };
+    const int64_t step = (int64_t)gridDim.x * RB;
+    int odd = 0;
+    fetch(blockIdx.x * (int64_t)RB + sub);
+    // every group of a workgroup makes the same number of turns (the sums of G = 256 meet at a barrier)
+    for (int64_t r0 = blockIdx.x * (int64_t)RB; r0 < p.rows; r0 += step) {
+        const int64_t r = r0 + sub;
+        const bool live = r < p.rows;
+        float xh[V][E], g[V][E];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E;
+            rx[k].get(xh[k]);
+            rg[k].get(g[k]);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const bool in = live && c + i < p.cols;
+                xh[k][i] = in ? (xh[k][i] - mean) * rstd : 0.f;
+                g[k][i] = in ? g[k][i] : 0.f;
+                dw[k][i] = __builtin_fmaf(g[k][i], xh[k][i], dw[k][i]);
+                db[k][i] += g[k][i];
+                g[k][i] *= w[k][i];
+                s1 += g[k][i];
+                s2 = __builtin_fmaf(g[k][i], xh[k][i], s2);
+            }
+        }
+        const float rs = rstd;
+        fetch(r + step);
+        if (!p.out) continue;
+        s1 = ln_sum<G>(s1, red + 8 * odd) * inv;
+        s2 = ln_sum<G>(s2, red + 8 * odd + 4) * inv;
+        odd ^= 1;
+        if (!live) continue;
+        T* dx = static_cast<T*>(p.out) + r * p.out_sr;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E, n = p.cols - c;
+            if (n <= 0) break;
+#pragma unroll
+            for (int i = 0; i < E; ++i) g[k][i] = rs * (g[k][i] - s1 - xh[k][i] * s2);
+            st_run<E, T>(dx + c, n, g[k]);
+        }
+    }
+    if (!p.part) return;
+    float* part = p.part + (int64_t)blockIdx.x * 2 * p.cols;
+    // the workgroup's groups, one behind the other
+    if constexpr (G < 256) {
+        for (int q = 0; q < RB; ++q) {
+            if (sub == q) {
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) {
+                        const int at = (k * E + i) * G + l;
+                        s_w[at] = q ? s_w[at] + dw[k][i] : dw[k][i];
+                        s_b[at] = q ? s_b[at] + db[k][i] : db[k][i];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < p.cols; c += 256) {
+            const int k = c / (G * E), at = (k * E + c % E) * G + c / E % G;
+            part[c] = s_w[at];
+            part[p.cols + c] = s_b[at];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E, n = p.cols - c;
+            if (n <= 0) break;
+            st_run<E, float>(part + c, n, dw[k]);
+            st_run<E, float>(part + p.cols + c, n, db[k]);
+        }
+    }
+}
+
+// The parts in order of their number: the same sums every time.  16 threads a
+// column, four loads in flight each.
+__global__ __launch_bounds__(256) void ln_dw_join(LnParams p) {
+    __shared__ float red[16][17];
+    const int x = threadIdx.x & 15, q = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
+    // columns 0 .. cols - 1: dw, cols .. 2 cols - 1: db
+    const bool live = c < 2 * p.cols;
+    const int64_t pitch = 2ll * p.cols;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+        const float* src = p.part + c;
+        int i = q;
+        for (; i + 48 < p.parts; i += 64) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += src[(i + 16 * j) * pitch];
+        }
+        for (; i < p.parts; i += 16) s[0] += src[i * pitch];
+    }
+    red[q][x] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (q || !live) return;
+    float a = 0.f;
+    for (int j = 0; j < 16; ++j) a += red[j][x];
+    float* out = c < p.cols ? p.dw : p.db;
+    if (out) out[c < p.cols ? c : c - p.cols] = a;
 }
 
 // workgroups of a kernel that takes a row each in turn
 static uint32_t ln_grid(int64_t rows) { return (uint32_t)std::min<int64_t>(rows, 1 << 20); }
-static int ln_parts(int64_t rows) { return (int)std::min<int64_t>(256, (rows + 31) / 32); }
+// steps of 16 bytes a lane that the columns take with G lanes a row
+template <typename T>
+static int ln_steps(int cols, int G) { return ceil_div(cols, G * kLnE<T>); }
+// Lanes a row, 0: the row is not held in registers.  16 lanes where one step of them
+// is enough, a wave for five steps of it (2560 bf16 elements), then a workgroup.
+template <typename T>
+static int ln_lanes(int cols) {
+    return ln_steps<T>(cols, 16) <= 1 ? 16 : ln_steps<T>(cols, 64) <= 5 ? 64 : ln_steps<T>(cols, 256) <= 5 ? 256 : 0;
+}
+// Workgroups of the backward: four a CU where the rows are enough for it, and
+// some eight rows a group at least, so that the parts stay few beside the rows.
+static int ln_parts(int64_t rows, int cols, bool bf16) {
+    const int G = bf16 ? ln_lanes<bf16_t>(cols) : ln_lanes<float>(cols);
+    if (G == 0) return (int)std::min<int64_t>(256, (rows + 31) / 32);
+    return (int)std::min<int64_t>(1024, (rows + 8 * (256 / G) - 1) / (8 * (256 / G)));
+}
 
 // rows x cols with these row strides: rows overlap nowhere and every element
 // offset fits 63 bits
@@ -139,17 +368,45 @@ static bool ln_rows_ok(int64_t rows, int cols, int64_t sr) {
     return sr >= cols || rows <= 1;
 }
 
+template <typename T, int G, int V>
+static void ln_rows_launch(const LnParams& p, bool back, hipStream_t s) {
+    if (back) hipLaunchKernelGGL((ln_bwd_rows<T, G, V>), dim3(p.parts), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((ln_fwd_rows<T, G, V>), dim3((uint32_t)((p.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, s, p);
+}
+
+// rows in registers; false where they are too wide (or, forward, too many for one grid)
+template <typename T>
+static bool ln_rows(const LnParams& p, bool back, hipStream_t s) {
+    const int G = ln_lanes<T>(p.cols);
+    if (G == 0 || (!back && p.rows >= (1ll << 24))) return false;
+    switch (G * 8 + ln_steps<T>(p.cols, G)) {
+        case 16 * 8 + 1: ln_rows_launch<T, 16, 1>(p, back, s); break;
+        case 64 * 8 + 1: ln_rows_launch<T, 64, 1>(p, back, s); break;
+        case 64 * 8 + 2: ln_rows_launch<T, 64, 2>(p, back, s); break;
+        case 64 * 8 + 3: ln_rows_launch<T, 64, 3>(p, back, s); break;
+        case 64 * 8 + 4: ln_rows_launch<T, 64, 4>(p, back, s); break;
+        case 64 * 8 + 5: ln_rows_launch<T, 64, 5>(p, back, s); break;
+        case 256 * 8 + 2: ln_rows_launch<T, 256, 2>(p, back, s); break;
+        case 256 * 8 + 3: ln_rows_launch<T, 256, 3>(p, back, s); break;
+        case 256 * 8 + 4: ln_rows_launch<T, 256, 4>(p, back, s); break;
+        default: ln_rows_launch<T, 256, 5>(p, back, s);
+    }
+    return true;
+}
+
 template <typename T>
 static void ln_fwd_launch(const LnParams& p, hipStream_t s) {
-    hipLaunchKernelGGL(ln_fwd_wide<T>, dim3(ln_grid(p.rows)), dim3(256), 0, s, p);
+    if (!ln_rows<T>(p, false, s)) hipLaunchKernelGGL(ln_fwd_wide<T>, dim3(ln_grid(p.rows)), dim3(256), 0, s, p);
 }
 
 template <typename T>
 static void ln_bwd_launch(const LnParams& p, hipStream_t s) {
-    if (p.out) hipLaunchKernelGGL(ln_dx_wide<T>, dim3(ln_grid(p.rows)), dim3(256), 0, s, p);
-    if (!p.dw && !p.db) return;
-    hipLaunchKernelGGL(ln_dw_wide<T>, dim3(ceil_div(p.cols, 64), p.parts), dim3(256), 0, s, p);
-    hipLaunchKernelGGL(ln_dw_join, dim3(ceil_div(p.cols, 64)), dim3(256), 0, s, p);
+    const bool sums = p.dw || p.db;
+    if (!ln_rows<T>(p, true, s)) {
+        if (p.out) hipLaunchKernelGGL(ln_dx_wide<T>, dim3(ln_grid(p.rows)), dim3(256), 0, s, p);
+        if (sums) hipLaunchKernelGGL(ln_dw_wide<T>, dim3(ceil_div(p.cols, 64), p.parts), dim3(256), 0, s, p);
+    }
+    if (sums) hipLaunchKernelGGL(ln_dw_join, dim3(ceil_div(2 * p.cols, 16)), dim3(256), 0, s, p);
 }
 
 }  // namespace mamba
@@ -159,7 +416,7 @@ using namespace mamba;
 extern "C" int mamba_layernorm_fwd(const mamba_layernorm_args* a, mamba_stream_t stream) {
     MAMBA_CHECK_ARG(a != nullptr, "args is NULL");
     MAMBA_CHECK_ARG(a->rows >= 0 && a->rows < (1ll << 31), "rows must be in [0, 2^31)");
-    MAMBA_CHECK_ARG(a->cols >= 1, "cols must be >= 1");
+    MAMBA_CHECK_ARG(a->cols >= 1 && a->cols <= (1 << 28), "cols must be in [1, 2^28]");
     MAMBA_CHECK_ARG(a->io_dtype == MAMBA_F32 || a->io_dtype == MAMBA_BF16, "io_dtype must be f32 or bf16");
     MAMBA_CHECK_ARG(a->eps >= 0.f, "eps must be >= 0");
     if (a->rows == 0) return MAMBA_OK;
@@ -178,14 +435,14 @@ extern "C" int mamba_layernorm_fwd(const mamba_layernorm_args* a, mamba_stream_t
 static int ln_bwd_check(const mamba_layernorm_bwd_args* a) {
     MAMBA_CHECK_ARG(a != nullptr, "args is NULL");
     MAMBA_CHECK_ARG(a->rows >= 0 && a->rows < (1ll << 31), "rows must be in [0, 2^31)");
-    MAMBA_CHECK_ARG(a->cols >= 1, "cols must be >= 1");
+    MAMBA_CHECK_ARG(a->cols >= 1 && a->cols <= (1 << 28), "cols must be in [1, 2^28]");
     MAMBA_CHECK_ARG(a->io_dtype == MAMBA_F32 || a->io_dtype == MAMBA_BF16, "io_dtype must be f32 or bf16");
     return MAMBA_OK;
 }
 
 extern "C" size_t mamba_layernorm_bwd_workspace_size(const mamba_layernorm_bwd_args* a) {
     if (ln_bwd_check(a) != MAMBA_OK || (!a->dweight && !a->dbias)) return 0;
-    return (size_t)ln_parts(a->rows) * 2 * a->cols * 4;
+    return (size_t)ln_parts(a->rows, a->cols, a->io_dtype == MAMBA_BF16) * 2 * a->cols * 4;
 }
 
 extern "C" int mamba_layernorm_bwd(const mamba_layernorm_bwd_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {
@@ -203,10 +460,10 @@ extern "C" int mamba_layernorm_bwd(const mamba_layernorm_bwd_args* a, void* ws, 
     p.x = a->x; p.x_sr = a->x_sr; p.dy = a->dy; p.dy_sr = a->dy_sr; p.w = a->weight;
     p.out = a->rows ? a->dx : nullptr; p.out_sr = a->dx_sr;
     p.mean = const_cast<float*>(a->mean); p.rstd = const_cast<float*>(a->rstd);
-    p.part = static_cast<float*>(ws); p.parts = ln_parts(a->rows);
+    p.part = need ? static_cast<float*>(ws) : nullptr; p.parts = ln_parts(a->rows, a->cols, a->io_dtype == MAMBA_BF16);
     p.dw = a->dweight; p.db = a->dbias;
     if (a->rows == 0) {  // the sums of no rows: zeros
-        if (p.dw || p.db) hipLaunchKernelGGL(ln_dw_join, dim3(ceil_div(p.cols, 64)), dim3(256), 0, (hipStream_t)stream, p);
+        if (p.dw || p.db) hipLaunchKernelGGL(ln_dw_join, dim3(ceil_div(2 * p.cols, 16)), dim3(256), 0, (hipStream_t)stream, p);
     } else if (a->io_dtype == MAMBA_BF16) {
         ln_bwd_launch<bf16_t>(p, (hipStream_t)stream);
     } else {

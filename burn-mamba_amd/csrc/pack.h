@@ -46,6 +46,35 @@ __device__ __forceinline__ void st_run(T* p, int n, const float (&v)[V]) {
     }
 }
 
+// V consecutive elements of a row as they lie in memory, so that a
+// load may stay in flight until they are used.
+template <typename T, int V>
+struct Elems {
+    static constexpr int W = (V * (int)sizeof(T) + 3) / 4;
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (V * sizeof(T) == 2) w[0] = *p;
+        else __builtin_memcpy(w, p, V * sizeof(T));
+    }
+    __device__ __forceinline__ void load_part(const T* p, int n) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = 0u;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) {
+                if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
+                else w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
+            }
+    }
+    __device__ __forceinline__ void get(float (&o)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if constexpr (sizeof(T) == 4) o[i] = __uint_as_float(w[i]);
+            else o[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        }
+    }
+};
+
 // ------------------------------------------------- packed sequences ---
 // Sequence s is rows cu[s] .. cu[s + 1] - 1 of a tensor of `rows` rows; rows
 // outside every sequence belong to none.  The offsets live on the device, where

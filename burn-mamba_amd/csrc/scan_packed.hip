@@ -112,35 +112,6 @@ struct ScanShape {
     static constexpr int NS = NP / 4, CPB = 256 / NS, EV = kTile * CPB / 256;  // EV elements a thread
 };
 
-// V (1, 2 or 4) consecutive elements of a row as they lie in memory, so that a
-// load may stay in flight until they are used.
-template <typename T, int V>
-struct Elems {
-    static constexpr int W = (V * (int)sizeof(T) + 3) / 4;
-    uint32_t w[W];
-    __device__ __forceinline__ void load(const T* p) {
-        if constexpr (V * sizeof(T) == 2) w[0] = *p;
-        else __builtin_memcpy(w, p, V * sizeof(T));
-    }
-    __device__ __forceinline__ void load_part(const T* p, int n) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = 0u;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (i < n) {
-                if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(p[i]);
-                else w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
-            }
-    }
-    __device__ __forceinline__ void get(float (&o)[V]) const {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if constexpr (sizeof(T) == 4) o[i] = __uint_as_float(w[i]);
-            else o[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-        }
-    }
-};
-
 // The element-wise mapping: row tid / (CPB / EV) of the tile, EV channels from
 // EV (tid % (CPB / EV)); with A = 0 the states of channels past D stay 0, so that
 // sums over a wave's channels need no mask.

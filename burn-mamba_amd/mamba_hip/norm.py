@@ -15,22 +15,26 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import DropoutArgs, LayerNormArgs, LayerNormBwdArgs, check
-from .packed import _need, _one_device, _p, _param
-from .ssd import _dtype_code, _stream, workspace
+from .packed import _IO, _fail, _need, _one_device, _p, _param, _raw_stream
+from .ssd import _dtype_code, workspace
 
 
 def _matrix(t: torch.Tensor, name: str) -> torch.Tensor:
     """t as [rows, cols] rows of its last axis, in place where its strides allow."""
-    _need(t.dim() >= 1 and t.shape[-1] >= 1, f"{name}: a last axis of at least one element required")
-    _need(t.dtype in (torch.float32, torch.bfloat16), f"{name}: dtype {t.dtype}, expected float32 or bfloat16")
-    m = t.reshape(-1, t.shape[-1])
+    shape = t.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        _fail(f"{name}: a last axis of at least one element required")
+    if t.dtype not in _IO:
+        _fail(f"{name}: dtype {t.dtype}, expected float32 or bfloat16")
+    m = t if len(shape) == 2 else t.reshape(-1, shape[-1])
     return m if m.stride(1) == 1 or m.shape[1] == 1 else m.contiguous()
 
 
-def _into(out: Optional[torch.Tensor], x: torch.Tensor) -> torch.Tensor:
+def _into(out: Optional[torch.Tensor], x: torch.Tensor) -> tuple:
     """The result tensor and its rows; one that is given has to be written in place."""
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return out, out if out.dim() == 2 else out.view(-1, out.shape[-1])
     _need(out.shape == x.shape and out.dtype == x.dtype, "out must match x")
     m = _matrix(out, "out")
     _need(m.data_ptr() == out.data_ptr(), "out must be rows of contiguous elements")
@@ -56,7 +60,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[t
         a.rows, a.cols, a.io_dtype, a.eps = rows, cols, _dtype_code(m), float(eps)
         a.x, a.x_sr, a.weight, a.bias = m.data_ptr(), m.stride(0), _p(weight), _p(bias)
         a.y, a.y_sr, a.mean, a.rstd = o.data_ptr(), o.stride(0), _p(mean), _p(rstd)
-        check(_lib.lib().mamba_layernorm_fwd(ctypes.byref(a), _stream(x.device)), "mamba_layernorm_fwd")
+        check(_lib.lib().mamba_layernorm_fwd(ctypes.byref(a), _raw_stream(x)), "mamba_layernorm_fwd")
     return out
 
 
@@ -81,7 +85,7 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Ten
         a.dx, a.dx_sr, a.dweight, a.dbias = out["dx"].data_ptr(), cols, out["dweight"].data_ptr(), out["dbias"].data_ptr()
         L = _lib.lib()
         ws = workspace(x.device, L.mamba_layernorm_bwd_workspace_size(ctypes.byref(a)))
-        check(L.mamba_layernorm_bwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), _stream(x.device)),
+        check(L.mamba_layernorm_bwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), _raw_stream(x)),
               "mamba_layernorm_bwd")
     return out
 
@@ -120,30 +124,33 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, offset: int = 0, resid
     the same call gives the same mask, and the gradient of x is this call on dy.  A program
     gives each of a step's calls its own ``offset`` and adds their count to rng[1] after the
     step's backward; in a captured graph rng is read at each replay."""
-    _need(x.dtype in (torch.float32, torch.bfloat16), f"x: dtype {x.dtype}, expected float32 or bfloat16")
+    if x.dtype not in _IO:
+        _fail(f"x: dtype {x.dtype}, expected float32 or bfloat16")
     _need(0.0 <= p <= 1.0, "p must be in [0, 1]")
-    _need(rng.dtype == torch.int64 and tuple(rng.shape) == (2,) and rng.is_contiguous(), "rng must be two int64: (seed, call number)")
+    _need(rng.dtype == torch.int64 and rng.shape == (2,) and rng.is_contiguous(), "rng must be two int64: (seed, call number)")
     _need(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), "residual must match x")
     _need(out is None or (out.shape == x.shape and out.dtype == x.dtype), "out must match x")
     with _one_device(x, rng, residual, out):
         if out is None:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if x.numel() == 0:
+        n = x.numel()
+        if n == 0:
             return out
-        ts = [x, residual, out]
-        if all(t is None or t.is_contiguous() for t in ts):
-            ts = [None if t is None else t.view(1, -1) for t in ts]
-        else:
-            ts = [None if t is None else _matrix(t.reshape(1) if t.dim() == 0 else t, "x") for t in ts]
-            _need(ts[2].data_ptr() == out.data_ptr(), "out must be rows of contiguous elements")
-        m, r, o = ts
         a = DropoutArgs()
-        (a.rows, a.cols), a.io_dtype, a.p = m.shape, _dtype_code(m), float(p)
-        a.x, a.x_sr, a.out, a.out_sr = m.data_ptr(), m.stride(0), o.data_ptr(), o.stride(0)
-        if r is not None:
-            a.residual, a.residual_sr = r.data_ptr(), r.stride(0)
-        a.rng, a.offset = rng.data_ptr(), int(offset)
-        check(_lib.lib().mamba_dropout(ctypes.byref(a), _stream(x.device)), "mamba_dropout")
+        a.io_dtype, a.p = _dtype_code(x), p
+        a.rng, a.offset = rng.data_ptr(), offset
+        if x.is_contiguous() and out.is_contiguous() and (residual is None or residual.is_contiguous()):
+            a.rows, a.cols, m, r = 1, n, x, residual  # one row
+            a.x, a.out, a.residual = x.data_ptr(), out.data_ptr(), _p(residual)
+        else:
+            m, o = _matrix(x, "x"), _matrix(out, "out")
+            _need(o.data_ptr() == out.data_ptr(), "out must be rows of contiguous elements")
+            a.rows, a.cols = m.shape
+            a.x, a.x_sr, a.out, a.out_sr = m.data_ptr(), m.stride(0), o.data_ptr(), o.stride(0)
+            if residual is not None:
+                r = _matrix(residual, "residual")
+                a.residual, a.residual_sr = r.data_ptr(), r.stride(0)
+        check(_lib.lib().mamba_dropout(ctypes.byref(a), _raw_stream(x)), "mamba_dropout")
     return out
 
 

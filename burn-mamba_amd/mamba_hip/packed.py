@@ -29,12 +29,14 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from ._lib import (Conv1dPackedArgs, Conv1dStepSlotsArgs, Mamba1ScanPackedArgs, Mamba1ScanPackedBwdArgs,
                    Mamba1ScanStepSlotsArgs, check)
-from .ssd import _dtype_code, _stream, workspace
+from .ssd import _dtype_code, workspace
 
 
 def _fail(msg: str):
     raise _lib.MambaHipError(msg)
 
+
+# The checks run on every call of a step: they build a message only to raise it.
 
 def _need(ok: bool, msg: str):
     if not ok:
@@ -43,44 +45,61 @@ def _need(ok: bool, msg: str):
 
 def _rows(t: torch.Tensor, name: str, rows: Optional[int] = None, cols: Optional[int] = None, dtype=None):
     """A [rows, cols] tensor whose last axis is contiguous."""
-    _need(t.dim() == 2 and (rows is None or t.shape[0] == rows) and (cols is None or t.shape[1] == cols),
-          f"{name}: shape {tuple(t.shape)}, expected [{'rows' if rows is None else rows}, {'cols' if cols is None else cols}]")
-    _need(t.dtype == dtype if dtype is not None else t.dtype in (torch.float32, torch.bfloat16),
-          f"{name}: dtype {t.dtype}, expected {dtype or 'float32 or bfloat16'}")
-    _need(t.stride(1) == 1 or t.shape[1] <= 1, f"{name}: the last axis must be contiguous")
+    shape = t.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (cols is not None and shape[1] != cols):
+        _fail(f"{name}: shape {tuple(shape)}, expected [{'rows' if rows is None else rows}, {'cols' if cols is None else cols}]")
+    if t.dtype != dtype if dtype is not None else t.dtype not in _IO:
+        _fail(f"{name}: dtype {t.dtype}, expected {dtype or 'float32 or bfloat16'}")
+    if t.stride(1) != 1 and shape[1] > 1:
+        _fail(f"{name}: the last axis must be contiguous")
+
+
+_IO = (torch.float32, torch.bfloat16)
 
 
 def _param(t: Optional[torch.Tensor], name: str, *shape: int):
-    if t is not None:
-        _need(t.dtype == torch.float32 and t.is_contiguous() and tuple(t.shape) == shape,
-              f"{name} must be a contiguous float32 tensor of shape {shape}")
+    if t is not None and (t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous()):
+        _fail(f"{name} must be a contiguous float32 tensor of shape {shape}")
 
 
 def _sequences(cu_seqlens: torch.Tensor, slots: Optional[torch.Tensor], state: Optional[torch.Tensor], name: str, *tail: int) -> int:
-    _need(cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1 and cu_seqlens.is_contiguous(),
-          "cu_seqlens must be a contiguous int32 tensor of one more entry than sequences")
+    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or not cu_seqlens.is_contiguous():
+        _fail("cu_seqlens must be a contiguous int32 tensor of one more entry than sequences")
     n = cu_seqlens.numel() - 1
-    _slots(n, slots, state, name, *tail)
+    if state is not None or slots is not None:
+        _slots(n, slots, state, name, *tail)
     return n
 
 
 def _slots(n: int, slots, state, name: str, *tail: int):
-    if state is not None:
-        _need(state.dtype == torch.float32 and state.is_contiguous() and tuple(state.shape[1:]) == tail,
-              f"{name} must be a contiguous float32 tensor of shape (slots, {', '.join(map(str, tail))})")
-        _need(slots is not None or state.shape[0] >= n, f"{name} needs a row per sequence where no slots are given")
-    if slots is not None:
-        _need(state is not None, "slots without a state")
-        _need(slots.dtype == torch.int32 and tuple(slots.shape) == (n,) and slots.is_contiguous(),
-              f"slots must be a contiguous int32 tensor of {n} entries")
+    if state is None:
+        _fail("slots without a state")
+    if state.dtype != torch.float32 or state.shape[1:] != tail or not state.is_contiguous():
+        _fail(f"{name} must be a contiguous float32 tensor of shape (slots, {', '.join(map(str, tail))})")
+    if slots is None:
+        if state.shape[0] < n:
+            _fail(f"{name} needs a row per sequence where no slots are given")
+    elif slots.dtype != torch.int32 or slots.shape != (n,) or not slots.is_contiguous():
+        _fail(f"slots must be a contiguous int32 tensor of {n} entries")
 
 
-def _one_device(*ts: Optional[torch.Tensor]):
+_SAME = contextlib.nullcontext()
+
+
+def _one_device(first: torch.Tensor, *ts: Optional[torch.Tensor]):
     """Every operand on one GPU, which becomes the current device for the call."""
-    ts = [t for t in ts if t is not None]
-    dev = ts[0].get_device()  # below 0: not a GPU
-    _need(dev >= 0 and all(t.get_device() == dev for t in ts), "operands on one GPU device required")
-    return torch.cuda.device(dev) if dev != torch.cuda.current_device() else contextlib.nullcontext()
+    dev = first.get_device()  # below 0: not a GPU
+    if dev < 0:
+        _fail("operands on one GPU device required")
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            _fail("operands on one GPU device required")
+    return _SAME if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+def _raw_stream(t: torch.Tensor) -> int:
+    """The current stream of t's device as a handle."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _p(t: Optional[torch.Tensor]):
@@ -128,7 +147,7 @@ def conv1d_packed(x: torch.Tensor, w: torch.Tensor, cu_seqlens: torch.Tensor, bi
         if out is None:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         a.out, a.out_st = out.data_ptr(), out.stride(0)
-        check(_lib.lib().mamba_conv1d_packed_fwd(ctypes.byref(a), _stream(x.device)), "mamba_conv1d_packed_fwd")
+        check(_lib.lib().mamba_conv1d_packed_fwd(ctypes.byref(a), _raw_stream(x)), "mamba_conv1d_packed_fwd")
     return out
 
 
@@ -146,7 +165,7 @@ def conv1d_packed_bwd(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, cu_s
         a.dx, a.dx_st, a.dw, a.dbias = out["dx"].data_ptr(), out["dx"].stride(0), out["dw"].data_ptr(), _p(out["dbias"])
         L = _lib.lib()
         ws = workspace(x.device, L.mamba_conv1d_packed_bwd_workspace_size(ctypes.byref(a)))
-        check(L.mamba_conv1d_packed_bwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), _stream(x.device)),
+        check(L.mamba_conv1d_packed_bwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), _raw_stream(x)),
               "mamba_conv1d_packed_bwd")
     return out
 
@@ -192,7 +211,7 @@ def conv1d_step_slots(x: torch.Tensor, state: torch.Tensor, slots: Optional[torc
         a.batch, a.channels, a.kernel, a.io_dtype, a.silu = b, c, k, _dtype_code(x), int(bool(silu))
         a.x, a.x_sb, a.state, a.nslots, a.slots = x.data_ptr(), x.stride(0), state.data_ptr(), state.shape[0], _p(slots)
         a.w, a.bias, a.out, a.out_sb = w.data_ptr(), _p(bias), out.data_ptr(), out.stride(0)
-        check(_lib.lib().mamba_conv1d_step_slots(ctypes.byref(a), _stream(x.device)), "mamba_conv1d_step_slots")
+        check(_lib.lib().mamba_conv1d_step_slots(ctypes.byref(a), _raw_stream(x)), "mamba_conv1d_step_slots")
     return out
 
 
@@ -221,9 +240,10 @@ def _scan_args(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, delta_softplus, 
     a.nseq = _sequences(cu_seqlens, slots, state, "state", a.dim, a.dstate)
     a.io_dtype, a.delta_softplus, a.max_seqlen = _dtype_code(u), int(bool(delta_softplus)), int(max_seqlen)
     a.cu_seqlens = cu_seqlens.data_ptr()
-    for name, t in (("u", u), ("delta", delta), ("B", B), ("C", C), ("z", z)):
-        setattr(a, name, _p(t))
-        setattr(a, name + "_st", _st(t))
+    a.u, a.u_st, a.delta, a.delta_st = u.data_ptr(), u.stride(0), delta.data_ptr(), delta.stride(0)
+    a.B, a.B_st, a.C, a.C_st = B.data_ptr(), B.stride(0), C.data_ptr(), C.stride(0)
+    if z is not None:
+        a.z, a.z_st = z.data_ptr(), z.stride(0)
     a.A, a.D, a.delta_bias = A.data_ptr(), _p(D), _p(delta_bias)
     a.state, a.nslots, a.slots = _p(state), 0 if state is None else state.shape[0], _p(slots)
     return a
@@ -249,7 +269,7 @@ def mamba1_scan_packed(u, delta, A, B, C, cu_seqlens, D=None, z=None, delta_bias
         L = _lib.lib()
         need = L.mamba1_scan_packed_workspace_size(ctypes.byref(a))
         ws = workspace(u.device, need) if need else None
-        check(L.mamba1_scan_packed_fwd(ctypes.byref(a), _p(ws), need, _stream(u.device)), "mamba1_scan_packed_fwd")
+        check(L.mamba1_scan_packed_fwd(ctypes.byref(a), _p(ws), need, _raw_stream(u)), "mamba1_scan_packed_fwd")
     return y
 
 
@@ -284,7 +304,7 @@ def mamba1_scan_packed_bwd(dy, u, delta, A, B, C, cu_seqlens, D=None, z=None, de
         L = _lib.lib()
         need = L.mamba1_scan_packed_bwd_workspace_size(ctypes.byref(a))
         ws = workspace(u.device, need)
-        check(L.mamba1_scan_packed_bwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), _stream(u.device)),
+        check(L.mamba1_scan_packed_bwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), _raw_stream(u)),
               "mamba1_scan_packed_bwd")
     return out
 
@@ -335,10 +355,12 @@ def scan_step_slots(u, delta, A, B, C, state: torch.Tensor, slots: Optional[torc
             y = torch.empty((b, d), dtype=u.dtype, device=u.device)
         a = Mamba1ScanStepSlotsArgs()
         a.batch, a.dim, a.dstate, a.io_dtype, a.delta_softplus = b, d, n, _dtype_code(u), int(bool(delta_softplus))
-        for name, t in (("u", u), ("delta", delta), ("B", B), ("C", C), ("z", z), ("y", y)):
-            setattr(a, name, _p(t))
-            setattr(a, name + "_sb", _st(t))
+        a.u, a.u_sb, a.delta, a.delta_sb = u.data_ptr(), u.stride(0), delta.data_ptr(), delta.stride(0)
+        a.B, a.B_sb, a.C, a.C_sb = B.data_ptr(), B.stride(0), C.data_ptr(), C.stride(0)
+        a.y, a.y_sb = y.data_ptr(), y.stride(0)
+        if z is not None:
+            a.z, a.z_sb = z.data_ptr(), z.stride(0)
         a.A, a.D, a.delta_bias = A.data_ptr(), _p(D), _p(delta_bias)
         a.state, a.nslots, a.slots = state.data_ptr(), state.shape[0], _p(slots)
-        check(_lib.lib().mamba1_scan_step_slots(ctypes.byref(a), _stream(u.device)), "mamba1_scan_step_slots")
+        check(_lib.lib().mamba1_scan_step_slots(ctypes.byref(a), _raw_stream(u)), "mamba1_scan_step_slots")
     return y

@@ -305,9 +305,15 @@ struct ConvSlotParams {
     void* out; int64_t out_sb;
 };
 
-// KT: 4 or 2 with 16- or 8-byte windows, or 0 for any width.
+// KT: 4 or 2 with 16- or 8-byte windows, or 0 for any width.  HBM-bound (8 K bytes
+// of window an element), so the arithmetic may be the plain composition's: each
+// product rounded, pairs of them summed first, then the bias, and SiLU with a
+// correctly rounded division (silu_f32).  A bf16 output then rounds the way the
+// composition's does, and the state that the scan keeps from it in f32 does not
+// differ by bf16 steps.
 template <typename T, int KT>
 __global__ __launch_bounds__(256) void conv_slot_step(ConvSlotParams p) {
+#pragma clang fp contract(off)
     const int b = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
     if (c >= p.C) return;
     const int64_t slot = slot_of(p.slots, b, p.nslots);
@@ -320,25 +326,28 @@ __global__ __launch_bounds__(256) void conv_slot_step(ConvSlotParams p) {
     float* win = p.state + (slot * p.C + c) * K;
     const float* w = p.w + (int64_t)c * K;
     const float xv = load_f32<T>(static_cast<const T*>(p.x) + b * p.x_sb + c);
-    float acc = p.b ? p.b[c] : 0.f;
+    float acc;
     if constexpr (KT != 0) {
         float v[KT], wv[KT];
         __builtin_memcpy(v, __builtin_assume_aligned(win, 4 * KT), 4 * KT);
         __builtin_memcpy(wv, __builtin_assume_aligned(w, 4 * KT), 4 * KT);
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            v[k] = k + 1 < KT ? v[k + 1] : xv;
-            acc = __builtin_fmaf(v[k], wv[k], acc);
-        }
+        for (int k = 0; k < KT; ++k) v[k] = k + 1 < KT ? v[k + 1] : xv;
+        acc = v[0] * wv[0] + v[1] * wv[1];
+        if constexpr (KT == 4) acc = acc + (v[2] * wv[2] + v[3] * wv[3]);
         __builtin_memcpy(__builtin_assume_aligned(win, 4 * KT), v, 4 * KT);
     } else {
+        // even taps and odd ones
+        float s[2] = {0.f, 0.f};
         for (int k = 0; k < K; ++k) {
             const float v = k + 1 < K ? win[k + 1] : xv;
             win[k] = v;
-            acc = __builtin_fmaf(v, w[k], acc);
+            s[k & 1] = s[k & 1] + v * w[k];
         }
+        acc = s[0] + s[1];
     }
-    store_f32<T>(out, p.silu ? acc * conv_sigmoid(acc) : acc);
+    if (p.b) acc = acc + p.b[c];
+    store_f32<T>(out, p.silu ? silu_f32(acc) : acc);
 }
 
 template <typename T>

@@ -11,11 +11,10 @@ import ctypes
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import DropoutArgs, LayerNormArgs, LayerNormBwdArgs, check
-from .packed import _IO, _fail, _need, _one_device, _p, _param, _raw_stream
+from .packed import _IO, _fail, _need, _once, _one_device, _p, _param, _raw_stream
 from .ssd import _dtype_code, workspace
 
 
@@ -75,38 +74,44 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Ten
     _param(mean, "mean", rows)
     _param(rstd, "rstd", rows)
     with _one_device(m, g, weight, mean, rstd):
-        f32 = dict(dtype=torch.float32, device=x.device)
-        out = dict(dx=torch.empty(x.shape, dtype=x.dtype, device=x.device), dweight=torch.empty(cols, **f32),
-                   dbias=torch.empty(cols, **f32))
-        a = LayerNormBwdArgs()
-        a.rows, a.cols, a.io_dtype = rows, cols, _dtype_code(m)
-        a.x, a.x_sr, a.dy, a.dy_sr = m.data_ptr(), m.stride(0), g.data_ptr(), g.stride(0)
-        a.weight, a.mean, a.rstd = _p(weight), mean.data_ptr(), rstd.data_ptr()
-        a.dx, a.dx_sr, a.dweight, a.dbias = out["dx"].data_ptr(), cols, out["dweight"].data_ptr(), out["dbias"].data_ptr()
-        L = _lib.lib()
-        ws = workspace(x.device, L.mamba_layernorm_bwd_workspace_size(ctypes.byref(a)))
-        check(L.mamba_layernorm_bwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), _raw_stream(x)),
-              "mamba_layernorm_bwd")
-    return out
+        dx, dweight, dbias = _ln_bwd(g, m, weight, mean.data_ptr(), rstd.data_ptr(), x.shape)
+    return dict(dx=dx, dweight=dweight, dbias=dbias)
+
+
+def _ln_bwd(g, m, weight, mean: int, rstd: int, shape):
+    """``layer_norm_bwd`` after its checks, the statistics as pointers."""
+    a = LayerNormBwdArgs()
+    rows, cols = m.shape
+    dx = torch.empty(shape, dtype=m.dtype, device=m.device)
+    dweight, dbias = torch.empty((2, cols), dtype=torch.float32, device=m.device).unbind()
+    a.rows, a.cols, a.io_dtype = rows, cols, _dtype_code(m)
+    a.x, a.x_sr, a.dy, a.dy_sr = m.data_ptr(), m.stride(0), g.data_ptr(), g.stride(0)
+    a.weight, a.mean, a.rstd = _p(weight), mean, rstd
+    a.dx, a.dx_sr, a.dweight, a.dbias = dx.data_ptr(), cols, dweight.data_ptr(), dbias.data_ptr()
+    L = _lib.lib()
+    ref = ctypes.byref(a)
+    ws = workspace(m.device, L.mamba_layernorm_bwd_workspace_size(ref))
+    check(L.mamba_layernorm_bwd(ref, ws.data_ptr(), ws.numel(), _raw_stream(m)), "mamba_layernorm_bwd")
+    return dx, dweight, dbias
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         rows = x.numel() // max(x.shape[-1], 1) if x.dim() else 0
-        mean = torch.empty(rows, dtype=torch.float32, device=x.device)
-        rstd = torch.empty_like(mean)
-        y = layer_norm(x, weight, bias, eps, stats=(mean, rstd))
-        ctx.save_for_backward(x, weight, mean, rstd)
+        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        y = layer_norm(x, weight, bias, eps, stats=stats.unbind())
+        ctx.save_for_backward(x, weight, stats)
         ctx.has_bias = bias is not None
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        g = layer_norm_bwd(dy, x, weight, mean, rstd)
-        return g["dx"], None if weight is None else g["dweight"], g["dbias"] if ctx.has_bias else None, None
+        x, weight, stats = ctx.saved_tensors
+        m, g, at = _matrix(x, "x"), _matrix(dy, "dy"), stats.data_ptr()
+        with _one_device(g):
+            dx, dweight, dbias = _ln_bwd(g, m, weight, at, at + 4 * m.shape[0], x.shape)
+        return dx, None if weight is None else dweight, dbias if ctx.has_bias else None, None
 
 
 def layer_norm_autograd(x, weight, bias=None, eps: float = 1e-5) -> torch.Tensor:
@@ -161,8 +166,7 @@ class _Dropout(torch.autograd.Function):
         ctx.call = (p, offset, residual is not None)
         return dropout(x, p, rng, offset, residual)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         (rng,), (p, offset, has_residual) = ctx.saved_tensors, ctx.call
         dx = dropout(dy, p, rng, offset) if ctx.needs_input_grad[0] else None

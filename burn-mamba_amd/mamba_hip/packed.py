@@ -110,6 +110,13 @@ def _st(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.stride(0)
 
 
+def _once(fn):
+    """A backward that is differentiable once: autograd's guard where a graph of the gradient
+    is wanted, the function itself (which that guard would slow down) where none is."""
+    guarded = once_differentiable(fn)
+    return staticmethod(lambda ctx, *g: guarded(ctx, *g) if torch.is_grad_enabled() else fn(ctx, *g))
+
+
 def _like_rows(dy: torch.Tensor) -> torch.Tensor:
     """A gradient as the kernels read it (autograd hands on expanded ones)."""
     return dy if dy.stride(-1) == 1 or dy.shape[-1] <= 1 else dy.contiguous()
@@ -158,16 +165,22 @@ def conv1d_packed_bwd(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, cu_s
     a = _conv_args(x, w, cu_seqlens, bias, silu)
     _rows(dout, "dout", x.shape[0], x.shape[1], x.dtype)
     with _one_device(dout, x, w, cu_seqlens, bias):
-        out = dict(dx=torch.empty(x.shape, dtype=x.dtype, device=x.device), dw=torch.empty_like(w),
-                   dbias=None if bias is None else torch.empty_like(bias))
-        a.fill_outside = 1
-        a.dout, a.dout_st = dout.data_ptr(), dout.stride(0)
-        a.dx, a.dx_st, a.dw, a.dbias = out["dx"].data_ptr(), out["dx"].stride(0), out["dw"].data_ptr(), _p(out["dbias"])
-        L = _lib.lib()
-        ws = workspace(x.device, L.mamba_conv1d_packed_bwd_workspace_size(ctypes.byref(a)))
-        check(L.mamba_conv1d_packed_bwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), _raw_stream(x)),
-              "mamba_conv1d_packed_bwd")
-    return out
+        dx, dw, dbias = _conv_bwd(a, dout, x, w, bias)
+    return dict(dx=dx, dw=dw, dbias=dbias)
+
+
+def _conv_bwd(a: Conv1dPackedArgs, dout, x, w, bias):
+    """``conv1d_packed_bwd`` after its checks."""
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw, dbias = torch.empty_like(w), None if bias is None else torch.empty_like(bias)
+    a.fill_outside = 1
+    a.dout, a.dout_st = dout.data_ptr(), dout.stride(0)
+    a.dx, a.dx_st, a.dw, a.dbias = dx.data_ptr(), dx.stride(0), dw.data_ptr(), _p(dbias)
+    L = _lib.lib()
+    ref = ctypes.byref(a)
+    ws = workspace(x.device, L.mamba_conv1d_packed_bwd_workspace_size(ref))
+    check(L.mamba_conv1d_packed_bwd(ref, ws.data_ptr(), ws.numel(), _raw_stream(x)), "mamba_conv1d_packed_bwd")
+    return dx, dw, dbias
 
 
 class _Conv1dPacked(torch.autograd.Function):
@@ -177,12 +190,13 @@ class _Conv1dPacked(torch.autograd.Function):
         ctx.save_for_backward(x, w, cu_seqlens, bias)
         return conv1d_packed(x, w, cu_seqlens, bias, silu)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         x, w, cu_seqlens, bias = ctx.saved_tensors
-        g = conv1d_packed_bwd(_like_rows(dout), x, w, cu_seqlens, bias, ctx.silu)
-        return g["dx"], g["dw"], None, g["dbias"], None
+        dout = _like_rows(dout)
+        with _one_device(dout):
+            dx, dw, dbias = _conv_bwd(_conv_args(x, w, cu_seqlens, bias, ctx.silu), dout, x, w, bias)
+        return dx, dw, None, dbias, None
 
 
 def conv1d_packed_autograd(x, w, cu_seqlens, bias=None, silu: bool = True) -> torch.Tensor:
@@ -287,25 +301,29 @@ def mamba1_scan_packed_bwd(dy, u, delta, A, B, C, cu_seqlens, D=None, z=None, de
     _param(initial_state, "initial_state", s, d, n)
     _param(d_final_state, "d_final_state", s, d, n)
     with _one_device(dy, u, delta, A, B, C, cu_seqlens, D, z, delta_bias, initial_state, d_final_state):
-        def new(t):
-            return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        return _scan_bwd(a, dy, u, delta, A, B, C, D, z, delta_bias, initial_state, d_final_state)
 
-        out = dict(du=new(u), ddelta=new(delta), dz=new(z), dB=new(B), dC=new(C), dA=new(A), dD=new(D),
-                   d_delta_bias=new(delta_bias), d_initial_state=None)
-        if initial_state is not None:  # an empty sequence ends in what it starts from
-            out["d_initial_state"] = torch.zeros_like(initial_state) if d_final_state is None else d_final_state.clone()
-        a.initial_state, a.d_final_state = _p(initial_state), _p(d_final_state)
-        a.dy, a.dy_st = dy.data_ptr(), dy.stride(0)
-        for name in ("du", "ddelta", "dz", "dB", "dC"):
-            setattr(a, name, _p(out[name]))
-            setattr(a, name + "_st", _st(out[name]))
-        for name in ("dA", "dD", "d_delta_bias", "d_initial_state"):
-            setattr(a, name, _p(out[name]))
-        L = _lib.lib()
-        need = L.mamba1_scan_packed_bwd_workspace_size(ctypes.byref(a))
-        ws = workspace(u.device, need)
-        check(L.mamba1_scan_packed_bwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), _raw_stream(u)),
-              "mamba1_scan_packed_bwd")
+
+def _scan_bwd(a: Mamba1ScanPackedBwdArgs, dy, u, delta, A, B, C, D, z, delta_bias, initial_state, d_final_state) -> dict:
+    """``mamba1_scan_packed_bwd`` after its checks."""
+    def new(t):
+        return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+    out = dict(du=new(u), ddelta=new(delta), dz=new(z), dB=new(B), dC=new(C), dA=new(A), dD=new(D),
+               d_delta_bias=new(delta_bias), d_initial_state=None)
+    if initial_state is not None:  # an empty sequence ends in what it starts from
+        out["d_initial_state"] = torch.zeros_like(initial_state) if d_final_state is None else d_final_state.clone()
+    a.initial_state, a.d_final_state = _p(initial_state), _p(d_final_state)
+    a.dy, a.dy_st = dy.data_ptr(), dy.stride(0)
+    a.du, a.du_st, a.ddelta, a.ddelta_st = out["du"].data_ptr(), u.shape[1], out["ddelta"].data_ptr(), u.shape[1]
+    a.dB, a.dB_st, a.dC, a.dC_st = out["dB"].data_ptr(), B.shape[1], out["dC"].data_ptr(), C.shape[1]
+    if z is not None:
+        a.dz, a.dz_st = out["dz"].data_ptr(), z.shape[1]
+    a.dA, a.dD, a.d_delta_bias, a.d_initial_state = out["dA"].data_ptr(), _p(out["dD"]), _p(out["d_delta_bias"]), _p(out["d_initial_state"])
+    L = _lib.lib()
+    ref = ctypes.byref(a)
+    ws = workspace(u.device, L.mamba1_scan_packed_bwd_workspace_size(ref))
+    check(L.mamba1_scan_packed_bwd(ref, ws.data_ptr(), ws.numel(), _raw_stream(u)), "mamba1_scan_packed_bwd")
     return out
 
 
@@ -321,15 +339,16 @@ class _ScanPacked(torch.autograd.Function):
         ctx.opts = (delta_softplus, max_seqlen)
         return y, final
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dfinal):
         u, delta, A, B, C, cu_seqlens, D, z, delta_bias, h0 = ctx.saved_tensors
         if dy is None and dfinal is None:
             return (None,) * 12
         dy = torch.zeros(u.shape, dtype=u.dtype, device=u.device) if dy is None else _like_rows(dy)
-        g = mamba1_scan_packed_bwd(dy, u, delta, A, B, C, cu_seqlens, D, z, delta_bias, ctx.opts[0], h0,
-                                   None if dfinal is None else dfinal.contiguous(), ctx.opts[1])
+        a = Mamba1ScanPackedBwdArgs()
+        a.fwd = _scan_args(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, *ctx.opts)
+        with _one_device(dy):
+            g = _scan_bwd(a, dy, u, delta, A, B, C, D, z, delta_bias, h0, None if dfinal is None else dfinal.contiguous())
         return (g["du"], g["ddelta"], g["dA"], g["dB"], g["dC"], None, g["dD"], g["dz"], g["d_delta_bias"],
                 g["d_initial_state"], None, None)
 

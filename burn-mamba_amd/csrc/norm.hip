@@ -118,7 +118,8 @@ __global__ __launch_bounds__(256) void ln_dw_wide(LnParams p) {
 
 // ---- rows in registers
 // Sum over aligned groups of G lanes in every lane; over the workgroup for G = 256
-// (red: 8 floats; the caller's calls alternate halves, so one barrier is enough).
+// (red: 4 floats, which no wave may still read from a sum before
+// the last barrier: the callers alternate between four places).
 template <int CTRL>
 __device__ __forceinline__ float ln_dpp(float v) {
     return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
@@ -145,58 +146,80 @@ __device__ __forceinline__ float ln_sum(float v, float* red) {
 template <typename T>
 constexpr int kLnE = 16 / (int)sizeof(T);
 
-// G lanes a row, V steps: cols <= G V kLnE.
+// G lanes a row, V steps: G (V - 1) kLnE < cols <= G V kLnE, so that only the last
+// step can pass the row's end (G = 16: cols <= 16 kLnE).  The workgroups take their rows in
+// turn, the next row's loads in flight while this one is summed; weight and bias
+// stay in registers.
 template <typename T, int G, int V>
 __global__ __launch_bounds__(256) void ln_fwd_rows(LnParams p) {
-    constexpr int E = kLnE<T>;
-    __shared__ float red[8];
-    const int l = threadIdx.x % G;
-    const int64_t r = blockIdx.x * (int64_t)(256 / G) + threadIdx.x / G;
-    if (r >= p.rows) return;  // whole groups (for G = 256 the grid is the rows)
-    const T* x = static_cast<const T*>(p.x) + r * p.x_sr;
-    T* y = static_cast<T*>(p.out) + r * p.out_sr;
-    float v[V][E];
-    float s = 0.f;
+    constexpr int E = kLnE<T>, RB = 256 / G;
+    __shared__ float red[16];
+    const int l = threadIdx.x % G, sub = threadIdx.x / G;
+    Elems<T, E> rx[V];
+    auto fetch = [&](int64_t r) {
+        if (r >= p.rows) return;
+        const T* x = static_cast<const T*>(p.x) + r * p.x_sr;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E, n = p.cols - c;
+            if (k < V - 1 || n >= E) rx[k].load(x + c);
+            else rx[k].load_part(x + c, n);
+        }
+    };
+    fetch(blockIdx.x * (int64_t)RB + sub);
+    float w[V][E], b[V][E];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
         const int c = (k * G + l) * E;
-        ld_run<E, T>(x + c, p.cols - c, v[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-#pragma unroll
-        for (int i = 0; i < E; ++i) s += v[k][i];
-    const float inv = 1.f / (float)p.cols, mean = ln_sum<G>(s, red) * inv;
-    s = 0.f;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int c = (k * G + l) * E;
+        if (p.w) ld_run<E, float>(p.w + c, k < V - 1 ? E : p.cols - c, w[k]);
+        if (p.b) ld_run<E, float>(p.b + c, k < V - 1 ? E : p.cols - c, b[k]);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            v[k][i] = c + i < p.cols ? v[k][i] - mean : 0.f;
-            s = __builtin_fmaf(v[k][i], v[k][i], s);
+            if (!p.w) w[k][i] = 1.f;
+            if (!p.b) b[k][i] = 0.f;
         }
     }
-    const float rstd = 1.f / sqrtf(ln_sum<G>(s, red + 4) * inv + p.eps);
+    const float inv = 1.f / (float)p.cols;
+    const int64_t step = (int64_t)gridDim.x * RB;
+    int odd = 0;
+    // every group of a workgroup makes the same number of turns (the sums of G = 256 meet at a barrier)
+    for (int64_t r0 = blockIdx.x * (int64_t)RB; r0 < p.rows; r0 += step) {
+        const int64_t r = r0 + sub;
+        float v[V][E], s = 0.f;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int c = (k * G + l) * E, n = p.cols - c;
-        if (n <= 0) break;
-        float w[E], b[E];
-        if (p.w) ld_run<E, float>(p.w + c, n, w);
-        if (p.b) ld_run<E, float>(p.b + c, n, b);
+        for (int k = 0; k < V; ++k) rx[k].get(v[k]);
+        fetch(r + step);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            float o = v[k][i] * rstd;
-            if (p.w) o *= w[i];
-            if (p.b) o += b[i];
-            v[k][i] = o;
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+            for (int i = 0; i < E; ++i) s += v[k][i];  // zeros past the row's end
+        const float mean = ln_sum<G>(s, red + 8 * odd) * inv;
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                v[k][i] = k < V - 1 || c + i < p.cols ? v[k][i] - mean : 0.f;
+                s = __builtin_fmaf(v[k][i], v[k][i], s);
+            }
         }
-        st_run<E, T>(y + c, n, v[k]);
-    }
-    if (l == 0) {
-        if (p.mean) p.mean[r] = mean;
-        if (p.rstd) p.rstd[r] = rstd;
+        const float rstd = 1.f / sqrtf(ln_sum<G>(s, red + 8 * odd + 4) * inv + p.eps);
+        odd ^= 1;
+        if (r >= p.rows) continue;
+        T* y = static_cast<T*>(p.out) + r * p.out_sr;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E, n = k < V - 1 ? E : p.cols - c;
+            if (n <= 0) break;
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[k][i] = __builtin_fmaf(v[k][i] * rstd, w[k][i], b[k][i]);
+            st_run<E, T>(y + c, n, v[k]);
+        }
+        if (l == 0) {
+            if (p.mean) p.mean[r] = mean;
+            if (p.rstd) p.rstd[r] = rstd;
+        }
     }
 }
 
@@ -206,19 +229,18 @@ template <typename T, int G, int V>
 __global__ __launch_bounds__(256) void ln_bwd_rows(LnParams p) {
     constexpr int E = kLnE<T>, RB = 256 / G;  // rows at a time
     __shared__ float red[16];
-    __shared__ float s_w[G < 256 ? G * V * E : 1], s_b[G < 256 ? G * V * E : 1];
+    // the weights, place (k E + i) G + l for element i of lane l's step k (they would take
+    // the registers that a second wave needs); after the rows, the groups' sums
+    __shared__ float s_w[G * V * E], s_b[G < 256 ? G * V * E : 1];
     const int l = threadIdx.x % G, sub = threadIdx.x / G;
-    float w[V][E], dw[V][E], db[V][E];
+    float dw[V][E], db[V][E];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const int c = (k * G + l) * E;
-        if (p.w) ld_run<E, float>(p.w + c, p.cols - c, w[k]);
+    for (int k = 0; k < V; ++k)
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            if (!p.w) w[k][i] = 1.f;
-            dw[k][i] = db[k][i] = 0.f;
-        }
-    }
+        for (int i = 0; i < E; ++i) dw[k][i] = db[k][i] = 0.f;
+    for (int c = threadIdx.x; c < G * V * E; c += 256)
+        s_w[(c / (G * E) * E + c % E) * G + c / E % G] = c < p.cols ? (p.w ? p.w[c] : 1.f) : 0.f;
+    __syncthreads();
     const float inv = 1.f / (float)p.cols;
     Elems<T, E> rx[V], rg[V];
     float mean = 0.f, rstd = 0.f;
@@ -229,7 +251,7 @@ __global__ __launch_bounds__(256) void ln_bwd_rows(LnParams p) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const int c = (k * G + l) * E, n = p.cols - c;
-            if (n >= E) {
+            if (k < V - 1 || n >= E) {
                 rx[k].load(x + c);
                 rg[k].load(dy + c);
             } else {
@@ -247,46 +269,67 @@ __global__ __launch_bounds__(256) void ln_bwd_rows(LnParams p) {
     for (int64_t r0 = blockIdx.x * (int64_t)RB; r0 < p.rows; r0 += step) {
         const int64_t r = r0 + sub;
         const bool live = r < p.rows;
-        float xh[V][E], g[V][E];
-        float s1 = 0.f, s2 = 0.f;
+        asm volatile("" ::: "memory");  // the weights stay in LDS: in registers they would cost a wave
+        Elems<T, E> cx[V], cg[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const int c = (k * G + l) * E;
-            rx[k].get(xh[k]);
-            rg[k].get(g[k]);
+            cx[k] = rx[k];
+            cg[k] = rg[k];
+        }
+        const float mu = mean, rs = rstd;
+        fetch(r + step);
+        // xh and dy of step k, from the row as it was loaded (kept in f32 between the two
+        // sweeps they would take twice the registers)
+        auto values = [&](int k, float (&xh)[E], float (&g)[E]) __attribute__((always_inline)) {
+            cx[k].get(xh);
+            cg[k].get(g);
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const bool in = live && c + i < p.cols;
-                xh[k][i] = in ? (xh[k][i] - mean) * rstd : 0.f;
-                g[k][i] = in ? g[k][i] : 0.f;
-                dw[k][i] = __builtin_fmaf(g[k][i], xh[k][i], dw[k][i]);
-                db[k][i] += g[k][i];
-                g[k][i] *= w[k][i];
-                s1 += g[k][i];
-                s2 = __builtin_fmaf(g[k][i], xh[k][i], s2);
+                xh[i] = (xh[i] - mu) * rs;
+                if (k == V - 1 && (k * G + l) * E + i >= p.cols) xh[i] = 0.f;  // g is 0 there
+            }
+        };
+        float s1 = 0.f, s2 = 0.f;
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                float xh[E], g[E];
+                values(k, xh, g);
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    dw[k][i] = __builtin_fmaf(g[i], xh[i], dw[k][i]);
+                    db[k][i] += g[i];
+                    g[i] *= s_w[(k * E + i) * G + l];
+                    s1 += g[i];
+                    s2 = __builtin_fmaf(g[i], xh[i], s2);
+                }
             }
         }
-        const float rs = rstd;
-        fetch(r + step);
         if (!p.out) continue;
         s1 = ln_sum<G>(s1, red + 8 * odd) * inv;
         s2 = ln_sum<G>(s2, red + 8 * odd + 4) * inv;
         odd ^= 1;
         if (!live) continue;
         T* dx = static_cast<T*>(p.out) + r * p.out_sr;
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const int c = (k * G + l) * E, n = p.cols - c;
-            if (n <= 0) break;
 #pragma unroll
-            for (int i = 0; i < E; ++i) g[k][i] = rs * (g[k][i] - s1 - xh[k][i] * s2);
-            st_run<E, T>(dx + c, n, g[k]);
+            for (int j = 0; j < Elems<T, E>::W; ++j) asm volatile("" : "+v"(cx[k].w[j]), "+v"(cg[k].w[j]));
+            const int c = (k * G + l) * E, n = k < V - 1 ? E : p.cols - c;
+            if (n <= 0) break;
+            float xh[E], g[E];
+            values(k, xh, g);
+#pragma unroll
+            for (int i = 0; i < E; ++i) g[i] = rs * (g[i] * s_w[(k * E + i) * G + l] - s1 - xh[i] * s2);
+            st_run<E, T>(dx + c, n, g);
         }
     }
     if (!p.part) return;
     float* part = p.part + (int64_t)blockIdx.x * 2 * p.cols;
     // the workgroup's groups, one behind the other
     if constexpr (G < 256) {
+        __syncthreads();
         for (int q = 0; q < RB; ++q) {
             if (sub == q) {
 #pragma unroll
@@ -354,6 +397,8 @@ template <typename T>
 static int ln_lanes(int cols) {
     return ln_steps<T>(cols, 16) <= 1 ? 16 : ln_steps<T>(cols, 64) <= 5 ? 64 : ln_steps<T>(cols, 256) <= 5 ? 256 : 0;
 }
+// Workgroups of the forward: four a CU (16384 x 2560 bf16: 31 us; 34 with six or three), or one for each group of rows.
+static uint32_t ln_fwd_grid(int64_t rows, int G) { return (uint32_t)std::min<int64_t>((rows + 256 / G - 1) / (256 / G), 1024); }
 // Workgroups of the backward: four a CU where the rows are enough for it, and
 // some eight rows a group at least, so that the parts stay few beside the rows.
 static int ln_parts(int64_t rows, int cols, bool bf16) {
@@ -371,14 +416,14 @@ static bool ln_rows_ok(int64_t rows, int cols, int64_t sr) {
 template <typename T, int G, int V>
 static void ln_rows_launch(const LnParams& p, bool back, hipStream_t s) {
     if (back) hipLaunchKernelGGL((ln_bwd_rows<T, G, V>), dim3(p.parts), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((ln_fwd_rows<T, G, V>), dim3((uint32_t)((p.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((ln_fwd_rows<T, G, V>), dim3(ln_fwd_grid(p.rows, G)), dim3(256), 0, s, p);
 }
 
-// rows in registers; false where they are too wide (or, forward, too many for one grid)
+// rows in registers; false where they are too wide
 template <typename T>
 static bool ln_rows(const LnParams& p, bool back, hipStream_t s) {
     const int G = ln_lanes<T>(p.cols);
-    if (G == 0 || (!back && p.rows >= (1ll << 24))) return false;
+    if (G == 0) return false;
     switch (G * 8 + ln_steps<T>(p.cols, G)) {
         case 16 * 8 + 1: ln_rows_launch<T, 16, 1>(p, back, s); break;
         case 64 * 8 + 1: ln_rows_launch<T, 64, 1>(p, back, s); break;

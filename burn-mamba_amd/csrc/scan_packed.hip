@@ -36,6 +36,7 @@
 // and channels past D are staged as zeros, which are steps that change nothing.
 // The next tile's rows are loaded while a tile is scanned.
 #include <algorithm>
+#include <cmath>
 
 #include "pack.h"
 
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(256) void scan_pk_state(ScanPk p) {
 // enters it.  kAhead chunks' values are loaded at a time.
 template <int NP, bool BACK>
 __device__ __forceinline__ void carry_walk(const ScanPk& p, int i) {
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 16;
     const int d = i / NP, n = i % NP;
     if (d >= p.D) return;
     const float A2 = n < p.N ? p.A[(int64_t)d * p.N + n] * kLog2e : 0.f;
@@ -729,7 +730,7 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
             if (p.z) rz.get(zv);
 #pragma unroll
             for (int k = 0; k < EV; ++k) dv[k] += bias[k];
-            float dt[EV], ev[EV];
+            float dt[EV], ev[EV], sz[EV];  // sz: sigmoid(z)
             if (p.softplus) {
 #pragma unroll
                 for (int k = 0; k < EV; ++k) dt[k] = pk_softplus(dv[k]);
@@ -739,7 +740,10 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
             }
             if (p.z) {
 #pragma unroll
-                for (int k = 0; k < EV; ++k) ev[k] = yv[k] * (zv[k] * pk_sigmoid(zv[k]));
+                for (int k = 0; k < EV; ++k) {
+                    sz[k] = pk_sigmoid(zv[k]);
+                    ev[k] = yv[k] * (zv[k] * sz[k]);
+                }
             } else {
 #pragma unroll
                 for (int k = 0; k < EV; ++k) ev[k] = yv[k];
@@ -830,8 +834,8 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
                 if (p.z) {
 #pragma unroll
                     for (int k = 0; k < EV; ++k) {
-                        const float sg = pk_sigmoid(zv[k]);
-                        o3[k] = yv[k] * __builtin_fmaf(Dv[k], uv[k], s_sC[m.row][m.ch + k]) * (sg * (1.f + zv[k] * (1.f - sg)));
+                        o3[k] = yv[k] * __builtin_fmaf(Dv[k], uv[k], s_sC[m.row][m.ch + k]) *
+                                (sz[k] * __builtin_fmaf(zv[k], 1.f - sz[k], 1.f));
                     }
                 }
 #pragma unroll
@@ -865,20 +869,27 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
     }
 }
 
-// The joins, each in a fixed order: dB and dC over the channel blocks (a thread
-// per row and state) ...
+// The joins, each in a fixed order: dB and dC over the channel blocks ...
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_join_bc(ScanPk p, int nblk) {
-    const int64_t total = p.rows * 2 * NP;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-        float s = 0.f;
-        for (int b = 0; b < nblk; ++b) s += p.pBC[b * total + i];
-        const int64_t t = i / (2 * NP);
-        const int k = (int)(i - t * 2 * NP), n = k % NP;
-        if (n >= p.N) continue;
-        if (k < NP) store_f32<T>(static_cast<T*>(p.dB) + t * p.dB_st + n, s);
-        else store_f32<T>(static_cast<T*>(p.dC) + t * p.dC_st + n, s);
+    // 64 values a workgroup, a quarter of the channel blocks each of its waves
+    __shared__ float red[4][64];
+    const int64_t total = p.rows * 2 * NP, i = blockIdx.x * 64ll + (threadIdx.x & 63);
+    const int q = wave_id();
+    float s = 0.f;
+    if (i < total) {
+#pragma unroll 8
+        for (int b = q; b < nblk; b += 4) s += p.pBC[b * total + i];
     }
+    red[q][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (q || i >= total) return;
+    s = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+    const int64_t t = i / (2 * NP);
+    const int k = (int)(i - t * 2 * NP), n = k % NP;
+    if (n >= p.N) return;
+    if (k < NP) store_f32<T>(static_cast<T*>(p.dB) + t * p.dB_st + n, s);
+    else store_f32<T>(static_cast<T*>(p.dC) + t * p.dC_st + n, s);
 }
 
 // ... and dA, dD, dbias over the chunks: column j of [D][NP] | [D] | [D].
@@ -1067,18 +1078,23 @@ static int scan_pk_make(const mamba1_scan_packed_args* a, ScanPk* o) {
     return MAMBA_OK;
 }
 
-static void scan_pk_fwd_plan(ScanPk& p) {
-    p.chunk = 128;
-    p.nchunk = (int)((p.rows + p.chunk - 1) / p.chunk);
-}
-static void scan_pk_bwd_plan(ScanPk& p) {
-    p.chunk = 128;
+// Rows of a chunk: four workgroups a CU where the rows are enough for it, at most
+// 256 rows (longer ones gain nothing), and at least about 0.6 sqrt(rows), where the
+// carry's walk over the chunks (0.15 us each) and the scan of one (0.2 us a row and
+// pass) weigh alike.  us, forward, at 1024 / 2048 / 4096 workgroups: 8192 x 5120
+// 325 / 328 / 323, 4000 x 2560 103 / 107 / 114, 2000 x 2560 63 / 67 / 72; at 16 / 32
+// rows at least: 1000 x 1024 40 / 33, 300 x 2560 25 / 24, 77 x 512 15.6 / 18.
+static void scan_pk_plan(ScanPk& p) {
+    const int64_t nblk = ceil_div(p.D, 1024 / scan_np(p.N));
+    const int64_t fill = (p.rows * nblk + 1023) / 1024, least = (int64_t)(0.6 * std::sqrt((double)p.rows));
+    const int64_t rows = std::max<int64_t>(1, std::max(fill, least));
+    p.chunk = (int)std::min<int64_t>(256, (rows + kTile - 1) / kTile * kTile);
     p.nchunk = (int)((p.rows + p.chunk - 1) / p.chunk);
 }
 // a grid's threads stay below 2^32
 static int scan_pk_grid_ok(const ScanPk& p) {
     const int64_t nblk = ceil_div(p.D, 1024 / scan_np(p.N));
-    if ((int64_t)p.nchunk * nblk >= (1ll << 24)) {
+    if (p.nchunk * nblk >= (1ll << 24) || p.rows * 2 * scan_np(p.N) >= (1ll << 30)) {
         set_error("mamba1_scan_packed: rows * dim is too large for one call");
         return MAMBA_ERR_UNSUPPORTED;
     }
@@ -1102,9 +1118,7 @@ static void scan_pk_bwd_launch(const ScanPk& p, hipStream_t s) {
         hipLaunchKernelGGL((scan_pk_state_bwd<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
         if (p.nchunk > 1) hipLaunchKernelGGL((scan_pk_carry_bwd<NP>), dim3(ceil_div(p.D * NP, 64), 2), dim3(64), 0, s, p);
         hipLaunchKernelGGL((scan_pk_bwd<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
-        const int64_t n = p.rows * 2 * NP;
-        hipLaunchKernelGGL((scan_pk_join_bc<T, NP>), dim3((uint32_t)std::min<int64_t>((n + 255) / 256, 8192)), dim3(256), 0, s, p,
-                           (int)nblk);
+        hipLaunchKernelGGL((scan_pk_join_bc<T, NP>), dim3((uint32_t)((p.rows * 2 * NP + 63) / 64)), dim3(256), 0, s, p, (int)nblk);
     }
     hipLaunchKernelGGL((scan_pk_join_par<NP>), dim3((uint32_t)(((int64_t)p.D * (NP + 2) + 63) / 64)), dim3(256), 0, s, p);
 }
@@ -1166,7 +1180,7 @@ using namespace mamba;
 extern "C" size_t mamba1_scan_packed_workspace_size(const mamba1_scan_packed_args* a) {
     ScanPk p;
     if (scan_pk_make(a, &p) != MAMBA_OK) return 0;
-    scan_pk_fwd_plan(p);
+    scan_pk_plan(p);
     return scan_pk_fwd_planes(p, nullptr);
 }
 
@@ -1181,7 +1195,7 @@ extern "C" int mamba1_scan_packed_fwd(const mamba1_scan_packed_args* a, void* ws
                     "without slots the state needs a row per sequence");
     p.y = a->y; p.y_st = a->y_st;
     p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
-    scan_pk_fwd_plan(p);
+    scan_pk_plan(p);
     if ((st = scan_pk_grid_ok(p)) != MAMBA_OK) return st;
     const size_t need = scan_pk_fwd_planes(p, ws);
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");
@@ -1197,7 +1211,7 @@ extern "C" int mamba1_scan_packed_fwd(const mamba1_scan_packed_args* a, void* ws
 extern "C" size_t mamba1_scan_packed_bwd_workspace_size(const mamba1_scan_packed_bwd_args* a) {
     ScanPk p;
     if (a == nullptr || scan_pk_make(&a->fwd, &p) != MAMBA_OK) return 0;
-    scan_pk_bwd_plan(p);
+    scan_pk_plan(p);
     return scan_pk_bwd_planes(p, nullptr);
 }
 
@@ -1220,7 +1234,7 @@ extern "C" int mamba1_scan_packed_bwd(const mamba1_scan_packed_bwd_args* a, void
     p.du = a->du; p.du_st = a->du_st; p.ddl = a->ddelta; p.ddl_st = a->ddelta_st; p.dz = a->dz; p.dz_st = a->dz_st;
     p.dB = a->dB; p.dB_st = a->dB_st; p.dC = a->dC; p.dC_st = a->dC_st;
     p.dA = a->dA; p.dD = a->dD; p.db = a->d_delta_bias; p.dh0 = a->d_initial_state;
-    scan_pk_bwd_plan(p);
+    scan_pk_plan(p);
     if ((st = scan_pk_grid_ok(p)) != MAMBA_OK) return st;
     const size_t need = scan_pk_bwd_planes(p, ws);
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");

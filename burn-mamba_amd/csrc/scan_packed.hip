@@ -18,7 +18,9 @@
 // chunk's end is carried: scan_pk_state finds the state a chunk leaves behind
 // when it starts from zero (or from the sequence's own start) and the sum of d
 // over it, scan_pk_carry walks the chunks, h <- exp(A sum d) h + own, and
-// scan_pk_out scans again from there.
+// scan_pk_out scans again from there.  Where the sequences are many and the longest
+// is known to be short, scan_pk_out takes whole sequences instead and nothing is
+// carried.
 //
 // Backward: scan_pk_state_bwd finds both carries of a chunk on one set of exps
 // (the gradient of the state that enters it is sum_t P_t C_t e_t, P_t the product
@@ -58,6 +60,7 @@ struct ScanPk {
     void* y; int64_t y_st;
     float* state; int64_t nslots; const int32_t* slots;
     int chunk, nchunk;
+    bool whole;                     // a workgroup takes a sequence: nchunk = the sequences
     // per chunk: what it leaves behind [nchunk][D][NP] (then, carried, what
     // leaves it), the sum of d [nchunk][D], and the state that its last sequence
     // began from [nchunk][D][NP] (the cache's slot may be written meanwhile)
@@ -157,6 +160,14 @@ struct ChunkEnds {
     int first, last;   // first sequence with rows in the chunk, and the one that crosses c1
     bool in, through;  // the first one began before c0; it fills the chunk and goes on
     __device__ __forceinline__ ChunkEnds(const ScanPk& p, int64_t ck) {
+        if (p.whole) {
+            first = (int)ck;
+            c0 = p.q.begin(first);
+            c1 = p.q.end(first);
+            in = through = false;
+            last = -1;
+            return;
+        }
         c0 = (int)(ck * p.chunk);
         c1 = min((int)p.rows, c0 + p.chunk);
         first = p.q.after(c0);
@@ -458,7 +469,12 @@ __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
         if (b == en) store_state(p.state, slot, p, d, ng, h);
         t = b;
     }
-    outside(t, e.c1);
+    if (p.whole) {  // the rows between this sequence and the next, and before the first
+        outside(e.c1, ck + 1 < p.nchunk ? p.q.begin(ck + 1) : (int)p.rows);
+        if (ck == 0) outside(0, e.c0);
+    } else {
+        outside(t, e.c1);
+    }
 }
 
 // ---------------------------------------------------------------- backward ---
@@ -1091,6 +1107,20 @@ static void scan_pk_plan(ScanPk& p) {
     p.chunk = (int)std::min<int64_t>(256, (rows + kTile - 1) / kTile * kTile);
     p.nchunk = (int)((p.rows + p.chunk - 1) / p.chunk);
 }
+// Whole sequences, a workgroup of CPB channels each, where the longest is known to
+// be short beside all the rows' work (its rows take some 0.15 us one behind the
+// other; in chunks most rows are scanned twice), or 96 rows at most, which take no
+// longer than three launches.  us, forward, whole / in chunks: 8 sequences of 2048
+// x 5120 468 / 580, 4 of them 360 / 301, 16 of 512 191 / 271, 16 of 256 x 2560 67 /
+// 103; 16 of unlike length, the longest about 2000, 473 / 306; 5 of 120 x 2560 21 / 34.
+static void scan_pk_fwd_plan(ScanPk& p, int max_seqlen) {
+    scan_pk_plan(p);
+    const int64_t nblk = ceil_div(p.D, 1024 / scan_np(p.N));
+    if (p.nchunk > 1 && max_seqlen > 0 && p.q.n > 0 && max_seqlen <= std::max<int64_t>(96, p.rows * nblk / 384)) {
+        p.whole = true;
+        p.nchunk = p.q.n;
+    }
+}
 // a grid's threads stay below 2^32
 static int scan_pk_grid_ok(const ScanPk& p) {
     const int64_t nblk = ceil_div(p.D, 1024 / scan_np(p.N));
@@ -1104,7 +1134,7 @@ static int scan_pk_grid_ok(const ScanPk& p) {
 template <typename T, int NP>
 static void scan_pk_fwd_launch(const ScanPk& p, hipStream_t s) {
     const uint32_t nblk = ceil_div(p.D, ScanShape<NP>::CPB);
-    if (p.nchunk > 1) {
+    if (p.nchunk > 1 && !p.whole) {
         hipLaunchKernelGGL((scan_pk_state<T, NP>), dim3(nblk * (uint32_t)(p.nchunk - 1)), dim3(256), 0, s, p);
         hipLaunchKernelGGL((scan_pk_carry<NP>), dim3(ceil_div(p.D * NP, 64)), dim3(64), 0, s, p);
     }
@@ -1148,7 +1178,7 @@ struct ScanPlanes {
     }
 };
 static size_t scan_pk_fwd_planes(ScanPk& p, void* ws) {
-    if (p.nchunk <= 1) return 0;
+    if (p.nchunk <= 1 || p.whole) return 0;
     ScanPlanes w(ws);
     const size_t nd = (size_t)p.nchunk * p.D, np = scan_np(p.N);
     p.E = w.take(nd * np);
@@ -1180,7 +1210,7 @@ using namespace mamba;
 extern "C" size_t mamba1_scan_packed_workspace_size(const mamba1_scan_packed_args* a) {
     ScanPk p;
     if (scan_pk_make(a, &p) != MAMBA_OK) return 0;
-    scan_pk_plan(p);
+    scan_pk_fwd_plan(p, a->max_seqlen);
     return scan_pk_fwd_planes(p, nullptr);
 }
 
@@ -1195,7 +1225,7 @@ extern "C" int mamba1_scan_packed_fwd(const mamba1_scan_packed_args* a, void* ws
                     "without slots the state needs a row per sequence");
     p.y = a->y; p.y_st = a->y_st;
     p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
-    scan_pk_plan(p);
+    scan_pk_fwd_plan(p, a->max_seqlen);
     if ((st = scan_pk_grid_ok(p)) != MAMBA_OK) return st;
     const size_t need = scan_pk_fwd_planes(p, ws);
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");

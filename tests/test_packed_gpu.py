@@ -228,6 +228,31 @@ def test_rows_outside_and_slots_out_of_range(dev):
     torch.cuda.synchronize()
 
 
+def test_scan_of_whole_sequences(dev):
+    """A known bound on the lengths: a workgroup takes whole sequences and nothing is carried.
+    Rows before, between and behind the sequences, a wrong bound, and slots."""
+    lens, d, n = [40, 0, 96, 1, 64, 30], 30, 16
+    rows = 5 + sum(lens) + 7
+    t = scan_inputs([rows], d, n, BF16, dev, seed=23)
+    starts = [5]
+    for k in lens:
+        starts.append(starts[-1] + k)
+    c = torch.tensor(starts, dtype=torch.int32, device=dev)
+    slots = torch.tensor([3, 6, 0, 1, 5, 2], dtype=torch.int32, device=dev)
+    state = torch.randn(7, d, n, generator=gen(24)).to(dev)
+    inner = {k: (v[5:] if k in ("u", "delta", "B", "C", "z") else v) for k, v in t.items()}
+    ref = po.scan(lens, h0=state.cpu()[slots.long().cpu()], **oracle_args(inner, True))
+    for most in (96, 1, 0):  # known, wrong (the schedule only), unknown
+        h, y = state.clone(), torch.full((rows, d), 7.0, dtype=BF16, device=dev)
+        mamba_hip.mamba1_scan_packed(**t, cu_seqlens=c, delta_softplus=True, state=h, slots=slots, max_seqlen=most, y=y)
+        po.close(y[5:-7], ref["y"][0][:-7], ref["y"][1][:-7], roundings(lens), "y")
+        assert (y[:5] == 7).all() and (y[-7:] == 7).all()
+        po.close(h[slots.long()], *ref["hT"], roundings(lens), "state")
+        assert torch.equal(h[4], state[4])
+        y = mamba_hip.mamba1_scan_packed(**t, cu_seqlens=c, delta_softplus=True, max_seqlen=most)
+        assert not y[:5].any() and not y[-7:].any() and y[5:-7].any()
+
+
 CONV = [("one", 3, 4, F32, 0, True), ("mixed", 130, 4, BF16, 3, True), ("borders", 600, 3, F32, 0, True),
         ("long", 77, 2, BF16, 5, False), ("mixed", 9, 1, F32, 0, True), ("tokens", 260, 4, F32, 0, True),
         ("mixed", 70, 7, F32, 2, True), ("short", 5, 64, BF16, 0, True)]

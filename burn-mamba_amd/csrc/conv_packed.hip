@@ -33,7 +33,10 @@ struct ConvPk {
     float* dw; float* db;
 };
 
-__device__ __forceinline__ float conv_sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
+// the hardware's exp2 and reciprocal (a float below the normal ones adds 0 to 1)
+__device__ __forceinline__ float conv_sigmoid(float v) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+}
 
 // KT = K as a constant, or 0: any K up to kMaxTaps (the taps then wait in a ring
 // that is shifted by one each row all the same).

@@ -83,15 +83,19 @@ struct ScanPk {
 };
 
 // softplus(x) = log(1 + e^x), x itself above 20 (equal in f32); log1p through the
-// hardware log with Goldberg's correction, log(v) e / (v - 1) for v = 1 + e.
+// hardware log with Goldberg's correction, log(v) e / (v - 1) for v = 1 + e.  The
+// hardware's exp2, log2 and reciprocal as they are (1 <= v, and an e below the normal
+// floats is 0): the library's cases for the smallest floats cost as much again.
 // Without a branch, which would part the elements in the schedule.
 __device__ __forceinline__ float pk_softplus(float x) {
-    const float e = __expf(fminf(x, 20.f));
+    const float e = __builtin_amdgcn_exp2f(fminf(x, 20.f) * kLog2e);
     const float v = 1.f + e;
-    const float l = __logf(v) * (e * __builtin_amdgcn_rcpf(v - 1.f));
+    const float l = __builtin_amdgcn_logf(v) * (1.f / kLog2e) * (e * __builtin_amdgcn_rcpf(v - 1.f));
     return x > 20.f ? x : v == 1.f ? e : l;
 }
-__device__ __forceinline__ float pk_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
+__device__ __forceinline__ float pk_sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -kLog2e));
+}
 
 template <int CTRL>
 __device__ __forceinline__ float pk_dpp(float v) {

@@ -103,7 +103,10 @@ __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
     };
     for (int s = p.q.after(c0); s < p.q.n && t < c1; ++s) {
         const int st = p.q.begin(s), en = p.q.end(s);
-        if (en <= t) continue;
+        if (en <= t) {
+            s = p.q.skip(s, t);
+            continue;
+        }
         for (; p.fill && t < min(st, c1); ++t) conv_store<T, V, FULL>(p.out, p.out_st, t, c, nc, zero);
         t = max(t, st);
         if (t >= c1) break;
@@ -192,7 +195,10 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
     };
     for (int s = p.q.after(c0); s < p.q.n && t < c1; ++s) {
         const int st = p.q.begin(s), en = p.q.end(s);
-        if (en <= t) continue;
+        if (en <= t) {
+            s = p.q.skip(s, t);
+            continue;
+        }
         for (; p.out && p.fill && t < min(st, c1); ++t) conv_store<T, V, FULL>(p.out, p.out_st, t, c, nc, zero);
         t = max(t, st);
         if (t >= c1) break;
@@ -426,6 +432,8 @@ extern "C" int mamba_conv1d_packed_fwd(const mamba_conv1d_packed_args* a, mamba_
     MAMBA_CHECK_ARG(a->out_st >= p.C || p.rows == 1, "rows of out overlap");
     MAMBA_CHECK_ARG(a->state == nullptr || a->slots != nullptr || a->nslots >= a->nseq,
                     "without slots the state needs a row per sequence");
+    MAMBA_CHECK_ARG(!rows_clash(a->out, a->out_st, a->x, a->x_st, p.C, p.C, p.rows, a->io_dtype == MAMBA_BF16 ? 2 : 4, false),
+                    "out overlaps x, whose rows are read by their successors");
     p.out = a->out; p.out_st = a->out_st;
     p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
     hipStream_t s = (hipStream_t)stream;
@@ -455,6 +463,10 @@ extern "C" int mamba_conv1d_packed_bwd(const mamba_conv1d_packed_args* a, void* 
     MAMBA_CHECK_ARG(a->state == nullptr, "the gradient is of sequences without a window");
     MAMBA_CHECK_ARG(p.rows == 0 || (a->x && a->dout), "x and dout are required");
     MAMBA_CHECK_ARG(a->dx == nullptr || a->dx_st >= p.C || p.rows <= 1, "rows of dx overlap");
+    const size_t e = a->io_dtype == MAMBA_BF16 ? 2 : 4;
+    MAMBA_CHECK_ARG(!rows_clash(a->dx, a->dx_st, a->x, a->x_st, p.C, p.C, p.rows, e, false) &&
+                        !rows_clash(a->dx, a->dx_st, a->dout, a->dout_st, p.C, p.C, p.rows, e, false),
+                    "dx overlaps x or dout");
     const size_t need = mamba_conv1d_packed_bwd_workspace_size(a);
     if (need && (ws == nullptr || ws_bytes < need)) {
         set_error("mamba_conv1d_packed_bwd: workspace missing or too small");
@@ -482,6 +494,9 @@ extern "C" int mamba_conv1d_step_slots(const mamba_conv1d_step_slots_args* a, ma
     MAMBA_CHECK_ARG(a->x && a->state && a->w && a->out, "x, state, w and out are required");
     MAMBA_CHECK_ARG(a->slots != nullptr || a->nslots >= a->batch, "without slots the state needs a row per token");
     MAMBA_CHECK_ARG(a->out_sb >= a->channels || a->batch == 1, "rows of out overlap");
+    MAMBA_CHECK_ARG(!rows_clash(a->out, a->out_sb, a->x, a->x_sb, a->channels, a->channels, a->batch,
+                                a->io_dtype == MAMBA_BF16 ? 2 : 4, true),
+                    "out overlaps x (it may be x itself)");
     ConvSlotParams p{};
     p.nb = a->batch; p.C = a->channels; p.K = a->kernel; p.silu = a->silu != 0;
     p.x = a->x; p.x_sb = a->x_sb; p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;

@@ -142,6 +142,10 @@ extern "C" int mamba_dropout(const mamba_dropout_args* a, mamba_stream_t stream)
     MAMBA_CHECK_ARG(a->cols < (1ll << 46) / a->rows, "rows * cols must be below 2^46");
     MAMBA_CHECK_ARG(a->x && a->out && a->rng, "x, out and rng are required");
     MAMBA_CHECK_ARG(a->rows == 1 || a->out_sr >= a->cols, "rows of out overlap");
+    const size_t e = a->io_dtype == MAMBA_BF16 ? 2 : 4;
+    MAMBA_CHECK_ARG(!rows_clash(a->out, a->out_sr, a->x, a->x_sr, a->cols, a->cols, a->rows, e, true) &&
+                        !rows_clash(a->out, a->out_sr, a->residual, a->residual_sr, a->cols, a->cols, a->rows, e, true),
+                    "out overlaps x or residual (it may be either itself)");
     DropoutParams p{};
     p.rows = a->rows; p.cols = a->cols;
     p.x = a->x; p.x_sr = a->x_sr; p.res = a->residual; p.res_sr = a->residual_sr;

@@ -467,6 +467,8 @@ extern "C" int mamba_layernorm_fwd(const mamba_layernorm_args* a, mamba_stream_t
     if (a->rows == 0) return MAMBA_OK;
     MAMBA_CHECK_ARG(a->x && a->y, "x and y are required");
     MAMBA_CHECK_ARG(ln_rows_ok(a->rows, a->cols, a->y_sr), "rows of y overlap");
+    MAMBA_CHECK_ARG(!rows_clash(a->y, a->y_sr, a->x, a->x_sr, a->cols, a->cols, a->rows, a->io_dtype == MAMBA_BF16 ? 2 : 4, true),
+                    "y overlaps x (it may be x itself)");
     LnParams p{};
     p.rows = a->rows; p.cols = a->cols; p.eps = a->eps;
     p.x = a->x; p.x_sr = a->x_sr; p.w = a->weight; p.b = a->bias;
@@ -496,6 +498,10 @@ extern "C" int mamba_layernorm_bwd(const mamba_layernorm_bwd_args* a, void* ws, 
     const size_t need = mamba_layernorm_bwd_workspace_size(a);
     MAMBA_CHECK_ARG(a->rows == 0 || (a->x && a->dy && a->mean && a->rstd), "x, dy, mean and rstd are required");
     MAMBA_CHECK_ARG(!a->dx || ln_rows_ok(a->rows, a->cols, a->dx_sr), "rows of dx overlap");
+    const size_t e = a->io_dtype == MAMBA_BF16 ? 2 : 4;
+    MAMBA_CHECK_ARG(!rows_clash(a->dx, a->dx_sr, a->x, a->x_sr, a->cols, a->cols, a->rows, e, false) &&
+                        !rows_clash(a->dx, a->dx_sr, a->dy, a->dy_sr, a->cols, a->cols, a->rows, e, false),
+                    "dx overlaps x or dy");
     if (need && (ws == nullptr || ws_bytes < need)) {
         set_error("mamba_layernorm_bwd: workspace missing or too small");
         return MAMBA_ERR_WORKSPACE;

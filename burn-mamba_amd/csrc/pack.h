@@ -87,6 +87,9 @@ struct Seqs {
     __device__ __forceinline__ int at(int s) const { return min(max(__builtin_amdgcn_readfirstlane(cu[s]), 0), rows); }
     __device__ __forceinline__ int begin(int s) const { return at(s); }
     __device__ __forceinline__ int end(int s) const { return max(at(s), at(s + 1)); }
+    // s + 1 is the next sequence to look at behind an empty one s at row t: many empty
+    // ones are passed over at once (and s never goes back, whatever the offsets are)
+    __device__ __forceinline__ int skip(int s, int t) const { return max(s, after(t) - 1); }
     // the first sequence that ends behind row t, n if none does
     __device__ __forceinline__ int after(int t) const {
         int lo = 0, hi = n;
@@ -98,6 +101,23 @@ struct Seqs {
         return lo;
     }
 };
+// What an output may share with an input: nothing, or (same = true) exactly its own
+// rows, where each element is read by the thread that writes it.  Rows of a wider
+// tensor beside one another (one stride, disjoint columns) share nothing.
+inline bool rows_clash(const void* a, int64_t a_st, const void* b, int64_t b_st, int64_t a_cols, int64_t b_cols,
+                       int64_t rows, size_t esize, bool same) {
+    if (a == nullptr || b == nullptr || rows <= 0) return false;
+    const char *pa = static_cast<const char*>(a), *pb = static_cast<const char*>(b);
+    const int64_t e = (int64_t)esize;
+    if (pa + ((rows - 1) * a_st + a_cols) * e <= pb || pb + ((rows - 1) * b_st + b_cols) * e <= pa) return false;
+    if (rows == 1) return !(same && pa == pb);
+    if (a_st != b_st || a_st <= 0 || (pa - pb) % e != 0) return true;
+    int64_t off = (pb - pa) / e % a_st;  // b's first column behind a's, in a row of a_st
+    if (off < 0) off += a_st;
+    if (off == 0) return !(same && pa == pb);
+    return off < a_cols || a_st - off < b_cols;
+}
+
 // rows of a packed tensor: a chunk's last row and one more chunk still fit an int
 constexpr int64_t kMaxRows = (1ll << 31) - (1ll << 20);
 // elements between rows: 16 rows' offsets fit 32 bits of bytes

@@ -393,7 +393,10 @@ __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
     int t = e.c0;
     for (int s = e.first; s < p.q.n && t < e.c1; ++s) {
         const int st = p.q.begin(s), en = p.q.end(s);
-        if (en <= t) continue;
+        if (en <= t) {
+            s = p.q.skip(s, t);
+            continue;
+        }
         if (st > t) {
             outside(t, min(st, e.c1));
             t = min(st, e.c1);
@@ -533,7 +536,10 @@ __global__ __launch_bounds__(256) void scan_pk_state_bwd(ScanPk p) {
     int t = e.c0;
     for (int s = e.first; s < p.q.n && t < e.c1; ++s) {
         const int st = p.q.begin(s), en = p.q.end(s);
-        if (en <= t) continue;
+        if (en <= t) {
+            s = p.q.skip(s, t);
+            continue;
+        }
         t = max(t, st);
         if (t >= e.c1) break;
         const int b = min(en, e.c1);
@@ -718,7 +724,10 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
     int t = e.c0;
     for (int s = e.first; s < p.q.n && t < e.c1; ++s) {
         const int st = p.q.begin(s), en = p.q.end(s);
-        if (en <= t) continue;
+        if (en <= t) {
+            s = p.q.skip(s, t);
+            continue;
+        }
         if (st > t) {
             outside(t, min(st, e.c1));
             t = min(st, e.c1);
@@ -1227,6 +1236,13 @@ extern "C" int mamba1_scan_packed_fwd(const mamba1_scan_packed_args* a, void* ws
     MAMBA_CHECK_ARG((a->y_st >= p.D && a->y_st < kMaxStride) || p.rows == 1, "rows of y overlap (or lie 2^25 elements apart)");
     MAMBA_CHECK_ARG(a->state == nullptr || a->slots != nullptr || a->nslots >= a->nseq,
                     "without slots the state needs a row per sequence");
+    const size_t e = a->io_dtype == MAMBA_BF16 ? 2 : 4;
+    MAMBA_CHECK_ARG(!rows_clash(a->y, a->y_st, a->u, a->u_st, p.D, p.D, p.rows, e, true) &&
+                        !rows_clash(a->y, a->y_st, a->delta, a->delta_st, p.D, p.D, p.rows, e, true) &&
+                        !rows_clash(a->y, a->y_st, a->z, a->z_st, p.D, p.D, p.rows, e, true) &&
+                        !rows_clash(a->y, a->y_st, a->B, a->B_st, p.D, p.N, p.rows, e, false) &&
+                        !rows_clash(a->y, a->y_st, a->C, a->C_st, p.D, p.N, p.rows, e, false),
+                    "y overlaps an input (it may be u, delta or z itself)");
     p.y = a->y; p.y_st = a->y_st;
     p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
     scan_pk_fwd_plan(p, a->max_seqlen);
@@ -1264,6 +1280,18 @@ extern "C" int mamba1_scan_packed_bwd(const mamba1_scan_packed_bwd_args* a, void
     MAMBA_CHECK_ARG(p.rows <= 1 || (a->dB_st >= p.N && a->dC_st >= p.N), "rows of dB or dC overlap");
     for (int64_t st : {a->dy_st, a->du_st, a->ddelta_st, a->dz_st, a->dB_st, a->dC_st})
         MAMBA_CHECK_ARG(p.rows <= 1 || (st >= 0 && st < kMaxStride), "row strides must be in [0, 2^25)");
+    struct Rows { const void* p; int64_t st; int cols; };
+    const Rows ins[] = {{a->fwd.u, a->fwd.u_st, p.D}, {a->fwd.delta, a->fwd.delta_st, p.D}, {a->fwd.z, a->fwd.z_st, p.D},
+                        {a->dy, a->dy_st, p.D}, {a->fwd.B, a->fwd.B_st, p.N}, {a->fwd.C, a->fwd.C_st, p.N}};
+    const Rows outs[] = {{a->du, a->du_st, p.D}, {a->ddelta, a->ddelta_st, p.D}, {a->dz, a->dz_st, p.D},
+                         {a->dB, a->dB_st, p.N}, {a->dC, a->dC_st, p.N}};
+    const size_t es = a->fwd.io_dtype == MAMBA_BF16 ? 2 : 4;
+    for (const Rows& o : outs) {
+        for (const Rows& i : ins)
+            MAMBA_CHECK_ARG(!rows_clash(o.p, o.st, i.p, i.st, o.cols, i.cols, p.rows, es, false), "a gradient overlaps an input");
+        for (const Rows* q = outs; q != &o; ++q)
+            MAMBA_CHECK_ARG(!rows_clash(o.p, o.st, q->p, q->st, o.cols, q->cols, p.rows, es, false), "two gradients overlap");
+    }
     p.dy = a->dy; p.dy_st = a->dy_st; p.h0 = a->initial_state; p.dhT = a->d_final_state;
     p.du = a->du; p.du_st = a->du_st; p.ddl = a->ddelta; p.ddl_st = a->ddelta_st; p.dz = a->dz; p.dz_st = a->dz_st;
     p.dB = a->dB; p.dB_st = a->dB_st; p.dC = a->dC; p.dC_st = a->dC_st;
@@ -1292,6 +1320,13 @@ extern "C" int mamba1_scan_step_slots(const mamba1_scan_step_slots_args* a, mamb
                     "u, delta, A, B, C, state and y are required");
     MAMBA_CHECK_ARG(a->slots != nullptr || a->nslots >= a->batch, "without slots the state needs a row per token");
     MAMBA_CHECK_ARG(a->y_sb >= a->dim || a->batch == 1, "rows of y overlap");
+    const size_t e = a->io_dtype == MAMBA_BF16 ? 2 : 4;
+    MAMBA_CHECK_ARG(!rows_clash(a->y, a->y_sb, a->u, a->u_sb, a->dim, a->dim, a->batch, e, true) &&
+                        !rows_clash(a->y, a->y_sb, a->delta, a->delta_sb, a->dim, a->dim, a->batch, e, true) &&
+                        !rows_clash(a->y, a->y_sb, a->z, a->z_sb, a->dim, a->dim, a->batch, e, true) &&
+                        !rows_clash(a->y, a->y_sb, a->B, a->B_sb, a->dim, a->dstate, a->batch, e, false) &&
+                        !rows_clash(a->y, a->y_sb, a->C, a->C_sb, a->dim, a->dstate, a->batch, e, false),
+                    "y overlaps an input (it may be u, delta or z itself)");
     ScanSlotParams p{};
     p.nb = a->batch; p.D = a->dim; p.N = a->dstate; p.softplus = a->delta_softplus != 0;
     p.u = a->u; p.u_sb = a->u_sb; p.dl = a->delta; p.dl_sb = a->delta_sb; p.z = a->z; p.z_sb = a->z_sb;

@@ -131,12 +131,20 @@ def _conv_args(x, w, cu_seqlens, bias, silu, state=None, slots=None) -> Conv1dPa
     k = w.shape[1]
     _param(w, "w", c, k)
     _param(bias, "bias", c)
+    _sequences(cu_seqlens, slots, state, "state", c, k)
+    a = _conv_fill(x, w, cu_seqlens, bias, silu)
+    if state is not None:
+        a.state, a.nslots, a.slots = state.data_ptr(), state.shape[0], _p(slots)
+    return a
+
+
+def _conv_fill(x, w, cu_seqlens, bias, silu) -> Conv1dPackedArgs:
+    """The arguments of operands that have been checked."""
     a = Conv1dPackedArgs()
-    a.nseq = _sequences(cu_seqlens, slots, state, "state", c, k)
+    (rows, c), k, a.nseq = x.shape, w.shape[1], cu_seqlens.shape[0] - 1
     a.rows, a.channels, a.kernel, a.io_dtype, a.silu = rows, c, k, _dtype_code(x), int(bool(silu))
     a.cu_seqlens = cu_seqlens.data_ptr()
     a.x, a.x_st, a.w, a.bias = x.data_ptr(), x.stride(0), w.data_ptr(), _p(bias)
-    a.state, a.nslots, a.slots = _p(state), 0 if state is None else state.shape[0], _p(slots)
     return a
 
 
@@ -195,7 +203,7 @@ class _Conv1dPacked(torch.autograd.Function):
         x, w, cu_seqlens, bias = ctx.saved_tensors
         dout = _like_rows(dout)
         with _one_device(dout):
-            dx, dw, dbias = _conv_bwd(_conv_args(x, w, cu_seqlens, bias, ctx.silu), dout, x, w, bias)
+            dx, dw, dbias = _conv_bwd(_conv_fill(x, w, cu_seqlens, bias, ctx.silu), dout, x, w, bias)
         return dx, dw, None, dbias, None
 
 
@@ -249,9 +257,18 @@ def _scan_operands(u, delta, A, B, C, D, z, delta_bias):
 
 
 def _scan_args(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, delta_softplus, max_seqlen, state=None, slots=None):
+    _, d, n = _scan_operands(u, delta, A, B, C, D, z, delta_bias)
+    _sequences(cu_seqlens, slots, state, "state", d, n)
     a = Mamba1ScanPackedArgs()
-    a.rows, a.dim, a.dstate = _scan_operands(u, delta, A, B, C, D, z, delta_bias)
-    a.nseq = _sequences(cu_seqlens, slots, state, "state", a.dim, a.dstate)
+    _scan_fill(a, u, delta, A, B, C, cu_seqlens, D, z, delta_bias, delta_softplus, max_seqlen)
+    if state is not None:
+        a.state, a.nslots, a.slots = state.data_ptr(), state.shape[0], _p(slots)
+    return a
+
+
+def _scan_fill(a: Mamba1ScanPackedArgs, u, delta, A, B, C, cu_seqlens, D, z, delta_bias, delta_softplus, max_seqlen):
+    """The arguments of operands that have been checked."""
+    (a.rows, a.dim), a.dstate, a.nseq = u.shape, A.shape[1], cu_seqlens.shape[0] - 1
     a.io_dtype, a.delta_softplus, a.max_seqlen = _dtype_code(u), int(bool(delta_softplus)), int(max_seqlen)
     a.cu_seqlens = cu_seqlens.data_ptr()
     a.u, a.u_st, a.delta, a.delta_st = u.data_ptr(), u.stride(0), delta.data_ptr(), delta.stride(0)
@@ -259,8 +276,6 @@ def _scan_args(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, delta_softplus, 
     if z is not None:
         a.z, a.z_st = z.data_ptr(), z.stride(0)
     a.A, a.D, a.delta_bias = A.data_ptr(), _p(D), _p(delta_bias)
-    a.state, a.nslots, a.slots = _p(state), 0 if state is None else state.shape[0], _p(slots)
-    return a
 
 
 def mamba1_scan_packed(u, delta, A, B, C, cu_seqlens, D=None, z=None, delta_bias=None, delta_softplus: bool = False,
@@ -346,7 +361,7 @@ class _ScanPacked(torch.autograd.Function):
             return (None,) * 12
         dy = torch.zeros(u.shape, dtype=u.dtype, device=u.device) if dy is None else _like_rows(dy)
         a = Mamba1ScanPackedBwdArgs()
-        a.fwd = _scan_args(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, *ctx.opts)
+        _scan_fill(a.fwd, u, delta, A, B, C, cu_seqlens, D, z, delta_bias, *ctx.opts)
         with _one_device(dy):
             g = _scan_bwd(a, dy, u, delta, A, B, C, D, z, delta_bias, h0, None if dfinal is None else dfinal.contiguous())
         return (g["du"], g["ddelta"], g["dA"], g["dB"], g["dC"], None, g["dD"], g["dz"], g["d_delta_bias"],

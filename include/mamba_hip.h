@@ -856,7 +856,9 @@ int mamba2_gated_rmsnorm(const mamba2_gated_norm_args* args, mamba_stream_t stre
 /* fill_outside.  A cache is addressed by slot: sequence (token) s keeps its   */
 /* state in row slots[s] of [nslots, ...] (NULL: row s).  A slot out of range  */
 /* is no state: the sequence starts from zero and keeps nothing.  The slots of */
-/* one call are distinct.  Rows are strided, their last axis contiguous.       */
+/* one call are distinct.  Rows are strided (less than 2^25 elements apart in  */
+/* the scan), their last axis contiguous.  Outputs share no memory with inputs */
+/* but where a call says so; an output that does is refused.                   */
 /* ------------------------------------------------------------------------- */
 
 /* Depthwise causal convolution + SiLU (layer 2 of Mamba1::forward,            */
@@ -910,7 +912,7 @@ int mamba_conv1d_step_slots(const mamba_conv1d_step_slots_args* args, mamba_stre
 /* dstate 1..64.  state is read for a sequence's start and overwritten with    */
 /* its end; NULL starts from zero and keeps nothing.  max_seqlen: a bound on   */
 /* the longest sequence that the caller knows, or 0 (a hint: it chooses the    */
-/* schedule, never the result's meaning).                                      */
+/* schedule, never the result's meaning).  y may be u, delta or z itself.      */
 typedef struct mamba1_scan_packed_args {
     int64_t rows;
     int32_t nseq, dim, dstate, io_dtype;
@@ -985,7 +987,7 @@ int mamba1_scan_step_slots(const mamba1_scan_step_slots_args* args, mamba_stream
 /*   xh = (x - mean) rstd, rstd = 1 / sqrt(mean((x - mean)^2) + eps),          */
 /*   y = xh weight + bias                                                      */
 /* weight NULL is 1, bias NULL 0.  mean and rstd [rows] f32 are written if     */
-/* given; the backward needs them:                                             */
+/* given (y may be x itself); the backward needs them:                         */
 /*   g = dy weight, dx = rstd (g - mean(g) - xh mean(g xh)),                   */
 /*   dweight = sum over rows of dy xh, dbias = sum of dy                       */
 /* (dx, dweight and dbias each may be NULL; sums in a fixed order).  The       */

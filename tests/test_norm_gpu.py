@@ -154,6 +154,18 @@ def test_dropout_gradient_and_masks(dev):
     assert mamba_hip.dropout(torch.empty(0, 3, device=dev), 0.5, rng).shape == (0, 3)
 
 
+def test_in_place(dev):
+    x, r = (torch.randn(37, 90, generator=torch.Generator().manual_seed(i)).to(dev) for i in (31, 32))
+    w = torch.linspace(-1, 1, 90, device=dev)
+    y = x.clone()
+    assert torch.equal(mamba_hip.layer_norm(y, w, out=y), mamba_hip.layer_norm(x, w))
+    rng = torch.tensor([5, 6], device=dev)
+    want = mamba_hip.dropout(x, 0.3, rng, residual=r)
+    for k in range(2):
+        mine = [x.clone(), r.clone()]
+        assert torch.equal(mamba_hip.dropout(mine[0], 0.3, rng, residual=mine[1], out=mine[k]), want)
+
+
 def test_graph(dev):
     """A captured step draws a new mask at each replay after the state moved on."""
     x, r, dy = (rand(300, 96, seed=s).to(BF16).to(dev) for s in (17, 18, 19))

@@ -354,6 +354,55 @@ def test_nothing_to_do(dev):
     assert mamba_hip.conv1d_step_slots(e(0, 6), e(2, 6, 4), none, e(6, 4)).shape == (0, 6)
 
 
+def test_outputs_in_place(dev):
+    """y over u, delta or z, and beside them in one tensor."""
+    lens, d, n = LENS["mixed"], 40, 16
+    t = scan_inputs(lens, d, n, BF16, dev, seed=25)
+    want = mamba_hip.mamba1_scan_packed(**t, cu_seqlens=cu(lens, dev), delta_softplus=True)
+    for k in ("u", "delta", "z"):
+        mine = {key: v.clone() for key, v in t.items()}
+        y = mamba_hip.mamba1_scan_packed(**mine, cu_seqlens=cu(lens, dev), delta_softplus=True, y=mine[k])
+        assert y is mine[k] and torch.equal(y, want), k
+    both = torch.zeros(sum(lens), 2 * d, dtype=BF16, device=dev)
+    both[:, :d] = t["u"]
+    mamba_hip.mamba1_scan_packed(**{**t, "u": both[:, :d]}, cu_seqlens=cu(lens, dev), delta_softplus=True, y=both[:, d:])
+    assert torch.equal(both[:, d:], want) and torch.equal(both[:, :d], t["u"])
+
+
+def test_many_empty_sequences(dev):
+    """Empty ones in the middle are passed over, and end in what they start from."""
+    lens = [70] + [0] * 5000 + [70]
+    t = scan_inputs([140], 16, 16, F32, dev, seed=26)
+    c = cu(lens, dev)
+    state = torch.randn(len(lens), 16, 16, generator=gen(27)).to(dev)
+    before = state.clone()
+    y = mamba_hip.mamba1_scan_packed(**t, cu_seqlens=c, delta_softplus=True, state=state)
+    ends = [0, len(lens) - 1]
+    ref = po.scan([70, 70], h0=before.cpu()[ends], **oracle_args(t, True))
+    po.close(y, *ref["y"], roundings([70]), "y")
+    po.close(state[ends], *ref["hT"], roundings([70]), "state")
+    assert torch.equal(state[1:-1], before[1:-1])
+    dy, dhT = torch.ones_like(y), torch.randn(len(lens), 16, 16, generator=gen(28)).to(dev)
+    g = mamba_hip.mamba1_scan_packed_bwd(dy, **t, cu_seqlens=c, delta_softplus=True, initial_state=before, d_final_state=dhT)
+    assert torch.equal(g["d_initial_state"][1:-1], dhT[1:-1])
+    ref = po.scan([70, 70], h0=before.cpu()[ends], dy=dy, dhT=dhT.cpu()[ends], **oracle_args(t, True))
+    po.close(g["d_initial_state"][ends], *ref["dh0"], 2 * roundings([70]), "dh0")
+    w = torch.randn(16, 4, generator=gen(29)).to(dev)
+    x = t["u"]
+    po.close(mamba_hip.conv1d_packed(x, w, c), *po.conv([70, 70], x, w)["y"], 12, "conv")
+
+
+def test_twice_differentiated(dev):
+    """A second derivative is refused, not wrong."""
+    lens = [9, 30]
+    t = {k: v.detach().requires_grad_() for k, v in scan_inputs(lens, 8, 16, F32, dev, seed=30).items()}
+    y, _ = mamba_hip.mamba1_scan_packed_autograd(**t, cu_seqlens=cu(lens, dev), delta_softplus=True)
+    dy = torch.ones_like(y).requires_grad_()
+    g, = torch.autograd.grad(y, [t["u"]], dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
 def test_graph_and_streams(dev):
     """Captured and replayed on other values, with eager calls on another stream between."""
     lens, d, n = [40, 200, 1], 64, 16

@@ -133,8 +133,8 @@ def test_the_library_refuses_by_itself():
     b = _lib.Mamba1ScanPackedBwdArgs()
     b.fwd = a
     assert L.mamba1_scan_packed_bwd(ctypes.byref(b), None, 0, None) == 1 and b"dA" in L.mamba_last_error()
-    for k in ("dA", "dy", "du", "ddelta", "dB", "dC"):
-        setattr(b, k, P)
+    for i, k in enumerate(("dA", "dy", "du", "ddelta", "dB", "dC")):
+        setattr(b, k, P + (i + 1) * 300 * 64 * 4)
     for k in ("du_st", "ddelta_st", "dB_st", "dC_st"):
         setattr(b, k, 64)
     need = L.mamba1_scan_packed_bwd_workspace_size(ctypes.byref(b))
@@ -163,6 +163,54 @@ def test_the_library_refuses_by_itself():
     assert L.mamba_dropout(ctypes.byref(o), None) == 1
     o.p = 0.5
     assert L.mamba_dropout(ctypes.byref(o), None) == 1 and b"rng" in L.mamba_last_error()
+
+
+def test_the_library_refuses_outputs_on_inputs():
+    """An output that shares memory with an input: refused but where a thread reads what it
+    writes.  The workspace's absence tells that the rest was taken."""
+    L, P = _lib.lib(), 1 << 20  # never dereferenced
+    a = _lib.Mamba1ScanPackedArgs()
+    a.rows, a.nseq, a.dim, a.dstate = 300, 2, 64, 16
+    for i, k in enumerate(("cu_seqlens", "u", "delta", "A", "B", "C", "z")):
+        setattr(a, k, P * (i + 1))
+    for k in ("u_st", "delta_st", "z_st", "B_st", "C_st"):
+        setattr(a, k, 128)
+    scan = lambda y, st: (setattr(a, "y", y), setattr(a, "y_st", st), L.mamba1_scan_packed_fwd(ctypes.byref(a), None, 0, None))[2]  # noqa: E731
+    for ok in ((9 * P, 64), (a.u, 128), (a.z, 128), (a.delta, 128), (a.u + 64 * 4, 128), (a.B + 16 * 4, 128), (a.C + 64 * 4, 128)):
+        assert scan(*ok) == 3, ok
+    for bad in ((a.u, 64), (a.u + 4, 128), (a.u + 128 * 4, 128), (a.z - 63 * 4, 128), (a.B, 128), (a.B + 15 * 4, 128), (a.C - 4, 128),
+                (a.C + 300 * 128 * 4 - 112 * 4 - 4, 128)):
+        assert scan(*bad) == 1 and b"overlaps" in L.mamba_last_error(), bad
+    c = _lib.Conv1dPackedArgs()
+    c.rows, c.nseq, c.channels, c.kernel, c.w, c.cu_seqlens, c.x, c.x_st = 10, 1, 4, 4, P, 2 * P, 3 * P, 8
+    for out, st in ((3 * P, 8), (3 * P + 12, 8), (3 * P - 4, 4)):
+        c.out, c.out_st = out, st
+        assert L.mamba_conv1d_packed_fwd(ctypes.byref(c), None) == 1 and b"overlaps" in L.mamba_last_error()
+    n = _lib.LayerNormArgs()
+    n.rows, n.cols, n.x, n.x_sr, n.y, n.y_sr = 4, 8, P, 8, P + 4, 8
+    assert L.mamba_layernorm_fwd(ctypes.byref(n), None) == 1 and b"overlaps" in L.mamba_last_error()
+    o = _lib.DropoutArgs()
+    o.rows, o.cols, o.p, o.rng, o.x, o.residual, o.out = 1, 8, 0.5, P, 2 * P, 3 * P, 3 * P + 4
+    assert L.mamba_dropout(ctypes.byref(o), None) == 1 and b"overlaps" in L.mamba_last_error()
+    g = _lib.Mamba1ScanPackedBwdArgs()
+    g.fwd, outs = a, ("du", "ddelta", "dz", "dB", "dC")
+    g.dA, g.dy, g.dy_st = P, 19 * P, 128
+    for i, k in enumerate(outs):
+        setattr(g, k, P * (20 + i))
+        setattr(g, k + "_st", 128)
+    bwd = lambda: L.mamba1_scan_packed_bwd(ctypes.byref(g), None, 0, None)  # noqa: E731
+    assert bwd() == 3
+    for k in outs:
+        mine = getattr(g, k)
+        for on in (a.u, a.z, g.dy, a.C + 4, P * 20 if k != "du" else P * 22):
+            setattr(g, k, on)
+            assert bwd() == 1 and b"overlap" in L.mamba_last_error(), (k, on)
+        setattr(g, k, mine)
+    c.dout, c.dout_st, c.dx, c.dx_st = 4 * P, 8, 4 * P, 8
+    assert L.mamba_conv1d_packed_bwd(ctypes.byref(c), None, 0, None) == 1 and b"overlaps" in L.mamba_last_error()
+    b = _lib.LayerNormBwdArgs()
+    b.rows, b.cols, b.x, b.x_sr, b.dy, b.dy_sr, b.mean, b.rstd, b.dx, b.dx_sr = 4, 8, P, 8, 2 * P, 8, 3 * P, 4 * P, 2 * P, 8
+    assert L.mamba_layernorm_bwd(ctypes.byref(b), None, 0, None) == 1 and b"overlaps" in L.mamba_last_error()
 
 
 @pytest.mark.parametrize("cls_name,c_name", [("Conv1dPackedArgs", "mamba_conv1d_packed_args"), ("Conv1dStepSlotsArgs", "mamba_conv1d_step_slots_args"),

@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -327,6 +327,9 @@ def _cast(w: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return w if w.dtype == dtype else _derived(w, "_mamba_cast_" + str(dtype)[6:], lambda t: t.detach().to(dtype))
 
 
+_CACHE_GRAD = "a cache is not differentiable: call under torch.no_grad(), or without one"
+
+
 def _decay(a_log: torch.Tensor) -> torch.Tensor:
     """A = -exp(a_log) (mamba1.rs:627) of the parameter's present values."""
     from .step import _derived
@@ -347,10 +350,18 @@ class Mamba1:
     a_log: torch.Tensor          # [d_inner, n]
     d: torch.Tensor              # [d_inner]
     out_proj_w: torch.Tensor     # [d_inner, d_model]
-    A: torch.Tensor = field(init=False, repr=False)
 
     def __post_init__(self):
-        self.A = -torch.exp(self.a_log)  # mamba1.rs:627
+        _decay(self.a_log)  # made here, so that a capture finds it
+
+    @property
+    def A(self) -> torch.Tensor:
+        return _decay(self.a_log)
+
+    def _wants_grad(self, x: torch.Tensor) -> bool:
+        return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (
+            x, self.in_proj_w, self.conv_w, self.conv_b, self.x_proj_w, self.dt_proj_w, self.dt_proj_b, self.a_log, self.d,
+            self.out_proj_w))
 
     def new_cache(self, batch: int) -> Mamba1Cache:
         c, dev = self.cfg, self.in_proj_w.device
@@ -419,11 +430,9 @@ class Mamba1:
         di, r, n = c.d_inner, c.dt_rank, c.state_rank
         if x.dim() != 2 or x.shape[1] != c.d_model:
             raise _lib.MambaHipError(f"x: shape {tuple(x.shape)}, expected [rows, {c.d_model}]")
-        params = (self.in_proj_w, self.conv_w, self.conv_b, self.x_proj_w, self.dt_proj_w, self.dt_proj_b, self.a_log, self.d,
-                  self.out_proj_w)
-        grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, *params))
+        grad = self._wants_grad(x)
         if grad and cache is not None:
-            raise _lib.MambaHipError("a cache is not differentiable: call under torch.no_grad(), or without one")
+            raise _lib.MambaHipError(_CACHE_GRAD)
         w = (lambda t: t.to(x.dtype)) if grad else (lambda t: _cast(t, x.dtype))
         xz = torch.mm(x, w(self.in_proj_w))
         xs, z = xz[:, :di], xz[:, di:]
@@ -446,7 +455,7 @@ class Mamba1:
         """Mamba1::step (mamba1.rs:533-612): returns (y [b, d_model], cache); the cache
         is updated in place.  With ``slots`` [b] int32 token i's state is row slots[i] of
         the cache, whose rows may be more, and x may be bf16 (products and y then are
-        too); without, the cache has a row per token."""
+        too); without, the cache has a row per token.  Gradients do not pass it."""
         c = self.cfg
         b = x.shape[0]
         if slots is not None:
@@ -467,6 +476,8 @@ class Mamba1:
         from .packed import conv1d_step_slots, scan_step_slots
         if cache is None:
             raise _lib.MambaHipError("slots without a cache")
+        if self._wants_grad(x):
+            raise _lib.MambaHipError(_CACHE_GRAD)
         c = self.cfg
         di, r, n = c.d_inner, c.dt_rank, c.state_rank
         w = lambda t: _cast(t, x.dtype)  # noqa: E731
@@ -510,5 +521,7 @@ class Mamba1Layer:
     def step(self, x: torch.Tensor, cache: Mamba1Cache, slots: Optional[torch.Tensor] = None):
         """One token per row of x [b, d_model] on ``cache`` (``Mamba1.step``)."""
         from .norm import layer_norm
+        if self.mixer._wants_grad(x):
+            raise _lib.MambaHipError(_CACHE_GRAD)
         y, cache = self.mixer.step(layer_norm(x, self.norm_w, self.norm_b, self.eps), cache, slots)
         return x + y, cache

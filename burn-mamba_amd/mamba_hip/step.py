@@ -278,13 +278,17 @@ def _derived(w: torch.Tensor, attr: str, make):
     tensor itself (so it lives exactly as long) and remade when the weight
     changes.  Making it launches device work, which must not be recorded into
     a captured HIP graph: a capture that finds no current copy raises, and the
-    caller derives the copies before capturing (``Mamba3.pack_products``)."""
+    caller derives the copies before capturing (``Mamba3.pack_products``).
+    The copy is finished before it is handed out: calls on other streams use
+    it too."""
     key = _weight_key(w)
     hit = getattr(w, attr, None)
     if hit is None or hit[0] != key:
         if w.is_cuda and torch.cuda.is_current_stream_capturing():
             raise _lib.MambaHipError(f"{attr[1:]}: the weight copy must be made before HIP graph capture")
         hit = (key, make(w))
+        if w.is_cuda:
+            torch.cuda.current_stream(w.device).synchronize()
         setattr(w, attr, hit)
     return hit[1]
 

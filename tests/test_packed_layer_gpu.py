@@ -133,9 +133,37 @@ def test_trained_parameters_are_the_ones_served(dev):
     ref = plain(layer, [po.d(t) for t in params(layer)], po.d(x), LENS)[0]
     near(layer.forward_packed(x, cu), ref, 1e-5, "f32")
     y = layer.forward_packed(x.to(BF16), cu)
-    # bf16 products and rows: some ten roundings of 2^-9 between x and y
+    # bf16 products and rows: some ten half steps of 2^-8 between x and y
     near(y, ref, 10 * 2.0 ** -8, "bf16")
     assert not torch.equal(y, first[1])
+    # tokens too, with slots and without
+    ps, token = [po.d(t) for t in params(layer)], x[:3]
+    cache = layer.mixer.new_cache(3)
+    for t in (cache.conv_bik, cache.ssm_bir):
+        t.normal_()
+    want, _, _ = plain(layer, ps, po.d(token), [1] * 3, window=po.d(cache.conv_bik), state=po.d(cache.ssm_bir))
+    for slots in (None, torch.arange(3, dtype=torch.int32, device=dev)):
+        mine = mamba_hip.Mamba1Cache(cache.conv_bik.clone(), cache.ssm_bir.clone())
+        near(layer.step(token, mine, slots)[0], want, 1e-5, "token")
+
+
+def test_two_streams_share_a_weight_copy(dev):
+    """The second call finds the copy that the first has ordered behind other work."""
+    layer, x, cu = make(dev, d_model=256)
+    xb = x.to(BF16)
+    want = layer.forward_packed(xb, cu)
+    for name in NAMES:
+        getattr(layer.mixer, name).mul_(1.0)  # the same values, new copies
+    torch.cuda.synchronize()
+    s1, s2, big = torch.cuda.Stream(), torch.cuda.Stream(), torch.randn(4096, 4096, device=dev)
+    with torch.cuda.stream(s1):
+        for _ in range(20):
+            big = torch.tanh(big @ big)
+        first = layer.forward_packed(xb, cu)
+    with torch.cuda.stream(s2):
+        second = layer.forward_packed(xb, cu)
+    torch.cuda.synchronize()
+    assert torch.equal(first, want) and torch.equal(second, want)
 
 
 def test_refusals(dev):
@@ -150,3 +178,7 @@ def test_refusals(dev):
     layer.mixer.d.requires_grad_()
     with pytest.raises(mamba_hip.MambaHipError, match="differentiable"):
         layer.forward_packed(x, cu, layer.mixer.new_cache(5))
+    with pytest.raises(mamba_hip.MambaHipError, match="differentiable"):
+        layer.step(x[:2], cache, torch.zeros(2, dtype=torch.int32, device=dev))
+    with torch.no_grad():
+        layer.step(x[:2], cache, torch.arange(2, dtype=torch.int32, device=dev))

@@ -10,7 +10,9 @@
 // About 2 K + 10 operations an element against two elements moved: HBM-bound.
 // A wave owns 64 V channels of one chunk of rows and walks down them with the
 // taps in registers, so each row is read once but for the K - 1 rows before a
-// chunk (and behind one, in the backward pass).
+// chunk (and behind one, in the backward pass).  Where V does not divide the
+// channels the last lane's run begins earlier, over channels that its neighbour has
+// too: both compute and store the same values, and no load or store is in parts.
 #include <algorithm>
 #include <type_traits>
 
@@ -38,48 +40,47 @@ __device__ __forceinline__ float conv_sigmoid(float v) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
 }
 
-// KT = K as a constant, or 0: any K up to kMaxTaps (the taps then wait in a ring
-// that is shifted by one each row all the same).
+// KT = K as a constant, or 0: any K up to kMaxTaps, the taps in a ring in scratch
+// memory that is shifted by one each row all the same (16384 x 5120 bf16: forward
+// 75 us with K = 7 as a constant, 1074 without; backward 137, 3276).
 constexpr int kMaxTaps = 64;
 constexpr int kConvRows = 4;  // rows whose loads are in flight while four others are computed
 
 // V channels' weights and bias; taps[k] = the input of row t - (K - 1) + k, k < K - 1
 template <int V, int KM>
-__device__ __forceinline__ void conv_weights(const ConvPk& p, int K, int c, int nc, float (&w)[KM][V], float (&bias)[V]) {
+__device__ __forceinline__ void conv_weights(const ConvPk& p, int K, int c, float (&w)[KM][V], float (&bias)[V]) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        bias[v] = p.b && v < nc ? p.b[c + v] : 0.f;
-        for (int k = 0; k < K; ++k) w[k][v] = v < nc ? p.w[(int64_t)(c + v) * K + k] : 0.f;
+        bias[v] = p.b ? p.b[c + v] : 0.f;
+        for (int k = 0; k < K; ++k) w[k][v] = p.w[(int64_t)(c + v) * K + k];
     }
 }
 template <typename T, int V, int KM>
-__device__ __forceinline__ void conv_taps(const ConvPk& p, int K, int s, int st, int t, int c, int nc, float (&tap)[KM][V]) {
+__device__ __forceinline__ void conv_taps(const ConvPk& p, int K, int s, int st, int t, int c, float (&tap)[KM][V]) {
     const int64_t slot = p.state ? slot_of(p.slots, s, p.nslots) : -1;
     for (int k = 0; k < K - 1; ++k) {
         const int at = t - (K - 1) + k;
         if (at >= st) {
-            ld_run<V, T>(static_cast<const T*>(p.x) + (int64_t)at * p.x_st + c, nc, tap[k]);
+            ld_run<V, T>(static_cast<const T*>(p.x) + (int64_t)at * p.x_st + c, V, tap[k]);
         } else {
             const int col = K + at - st;
 #pragma unroll
-            for (int v = 0; v < V; ++v) tap[k][v] = slot >= 0 && v < nc ? p.state[(slot * p.C + c + v) * K + col] : 0.f;
+            for (int v = 0; v < V; ++v) tap[k][v] = slot >= 0 ? p.state[(slot * p.C + c + v) * K + col] : 0.f;
         }
     }
 }
-// A row of V channels from c: FULL where C is a multiple of V, so that all V are there.
-// The row's base is in scalar registers, the lane's place 32 bits.
-template <typename T, int V, bool FULL>
-__device__ __forceinline__ void conv_load(const void* src, int64_t st, int t, int c, int nc, Elems<T, V>& e) {
-    const T* row = static_cast<const T*>(src) + t * st;
-    if (FULL) e.load(row + (uint32_t)c);
-    else e.load_part(row + (uint32_t)c, nc);
+// A row of V channels from c.  The row's base is in scalar registers, the lane's place
+// 32 bits.
+template <typename T, int V>
+__device__ __forceinline__ void conv_load(const void* src, int64_t st, int t, int c, Elems<T, V>& e) {
+    e.load(static_cast<const T*>(src) + t * st + (uint32_t)c);
 }
-template <typename T, int V, bool FULL>
-__device__ __forceinline__ void conv_store(void* dst, int64_t st, int t, int c, int nc, const float (&o)[V]) {
-    st_run<V, T>(static_cast<T*>(dst) + t * st + (uint32_t)c, FULL ? V : nc, o);
+template <typename T, int V>
+__device__ __forceinline__ void conv_store(void* dst, int64_t st, int t, int c, const float (&o)[V]) {
+    st_run<V, T>(static_cast<T*>(dst) + t * st + (uint32_t)c, V, o);
 }
 
-template <typename T, int KT, int V, bool FULL>
+template <typename T, int KT, int V>
 __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
     constexpr int KM = KT ? KT : kMaxTaps, R = KT ? kConvRows : 1;
     const int K = KT ? KT : p.K;
@@ -88,10 +89,10 @@ __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
     const int64_t item = blockIdx.x * 4ll + wave_id();
     const int64_t ck = item / nblk;
     if (ck >= p.nchunk) return;
-    const int c = ((int)(item - ck * nblk) * 64 + lane) * V, nc = min(V, p.C - c);
-    if (nc <= 0) return;
+    const int at_c = ((int)(item - ck * nblk) * 64 + lane) * V, c = min(at_c, p.C - V);
+    if (at_c >= p.C) return;
     float w[KM][V], bias[V], tap[KM + R - 1][V];
-    conv_weights<V, KM>(p, K, c, nc, w, bias);
+    conv_weights<V, KM>(p, K, c, w, bias);
     const int c0 = (int)(ck * p.chunk), c1 = (int)min(p.rows, ck * p.chunk + p.chunk);
     int t = c0;
     const float zero[V] = {};
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
     auto fetch = [&](int t0, int stop) {  // rows t0 .. of those before stop
 #pragma unroll
         for (int i = 0; i < R; ++i)
-            if (t0 + i < stop) conv_load<T, V, FULL>(p.x, p.x_st, t0 + i, c, nc, raw[i]);
+            if (t0 + i < stop) conv_load<T, V>(p.x, p.x_st, t0 + i, c, raw[i]);
     };
     for (int s = p.q.after(c0); s < p.q.n && t < c1; ++s) {
         const int st = p.q.begin(s), en = p.q.end(s);
@@ -107,12 +108,12 @@ __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
             s = p.q.skip(s, t);
             continue;
         }
-        for (; p.fill && t < min(st, c1); ++t) conv_store<T, V, FULL>(p.out, p.out_st, t, c, nc, zero);
+        for (; p.fill && t < min(st, c1); ++t) conv_store<T, V>(p.out, p.out_st, t, c, zero);
         t = max(t, st);
         if (t >= c1) break;
         const int stop = min(en, c1);
         fetch(t, stop);
-        conv_taps<T, V, KM + R - 1>(p, K, s, st, t, c, nc, tap);
+        conv_taps<T, V, KM + R - 1>(p, K, s, st, t, c, tap);
         for (; t < stop; t += R) {
 #pragma unroll
             for (int i = 0; i < R; ++i)
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
 #pragma unroll
                     for (int v = 0; v < V; ++v) o[v] *= conv_sigmoid(o[v]);
                 }
-                conv_store<T, V, FULL>(p.out, p.out_st, t + i, c, nc, o);
+                conv_store<T, V>(p.out, p.out_st, t + i, c, o);
             }
             for (int k = 0; k < K - 1; ++k)
 #pragma unroll
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
         }
         t = stop;
     }
-    for (; p.fill && t < c1; ++t) conv_store<T, V, FULL>(p.out, p.out_st, t, c, nc, zero);
+    for (; p.fill && t < c1; ++t) conv_store<T, V>(p.out, p.out_st, t, c, zero);
 }
 
 // an offset of a sequence that differs between the lanes
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(256) void conv_pk_window(ConvPk p) {
     }
 }
 
-template <typename T, int KT, int V, bool FULL>
+template <typename T, int KT, int V>
 __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
     constexpr int KM = KT ? KT : kMaxTaps, R = KT ? kConvRows : 1;
     const int K = KT ? KT : p.K;
@@ -171,11 +172,11 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
     const int64_t item = blockIdx.x * 4ll + wave_id();
     const int64_t ck = item / nblk;
     if (ck >= p.nchunk) return;
-    const int c = ((int)(item - ck * nblk) * 64 + lane) * V, nc = min(V, p.C - c);
-    if (nc <= 0) return;
+    const int at_c = ((int)(item - ck * nblk) * 64 + lane) * V, c = min(at_c, p.C - V);
+    if (at_c >= p.C) return;
     // tap[K - 1 + i]: row r + i of x; g[i + k]: of row r + i - (K - 1) + k
     float w[KM][V], bias[V], tap[KM + R - 1][V], g[KM + R - 1][V], dw[KM][V], db[V];
-    conv_weights<V, KM>(p, K, c, nc, w, bias);
+    conv_weights<V, KM>(p, K, c, w, bias);
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int v = 0; v < V; ++v) dw[k][v] = 0.f;
@@ -189,8 +190,8 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             if (r + i >= last) break;
-            conv_load<T, V, FULL>(p.x, p.x_st, r + i, c, nc, rx[i]);
-            conv_load<T, V, FULL>(p.dout, p.dout_st, r + i, c, nc, rg[i]);
+            conv_load<T, V>(p.x, p.x_st, r + i, c, rx[i]);
+            conv_load<T, V>(p.dout, p.dout_st, r + i, c, rg[i]);
         }
     };
     for (int s = p.q.after(c0); s < p.q.n && t < c1; ++s) {
@@ -199,13 +200,13 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
             s = p.q.skip(s, t);
             continue;
         }
-        for (; p.out && p.fill && t < min(st, c1); ++t) conv_store<T, V, FULL>(p.out, p.out_st, t, c, nc, zero);
+        for (; p.out && p.fill && t < min(st, c1); ++t) conv_store<T, V>(p.out, p.out_st, t, c, zero);
         t = max(t, st);
         if (t >= c1) break;
         // rows of this part give dw; the K - 1 behind it, where the sequence goes on, dx only
         const int stop = min(en, c1), last = min(en, stop + K - 1);
         fetch(t, last);
-        conv_taps<T, V, KM + R - 1>(p, K, s, st, t, c, nc, tap);
+        conv_taps<T, V, KM + R - 1>(p, K, s, st, t, c, tap);
         for (int k = 0; k < K - 1; ++k)
 #pragma unroll
             for (int v = 0; v < V; ++v) g[k][v] = 0.f;
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
                         o[v] = 0.f;
                         for (int k = 0; k < K; ++k) o[v] = __builtin_fmaf(w[K - 1 - k][v], g[i + k][v], o[v]);
                     }
-                    conv_store<T, V, FULL>(p.out, p.out_st, at, c, nc, o);
+                    conv_store<T, V>(p.out, p.out_st, at, c, o);
                 }
             }
             for (int k = 0; k < K - 1; ++k)
@@ -268,11 +269,11 @@ __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
         while (r < stop + K - 1) rows(std::false_type{});
         t = stop;
     }
-    for (; p.out && p.fill && t < c1; ++t) conv_store<T, V, FULL>(p.out, p.out_st, t, c, nc, zero);
+    for (; p.out && p.fill && t < c1; ++t) conv_store<T, V>(p.out, p.out_st, t, c, zero);
     if (!p.part) return;
     float* part = p.part + (ck * (K + 1)) * (int64_t)p.C + c;
-    for (int k = 0; k < K; ++k) st_run<V, float>(part + (int64_t)k * p.C, nc, dw[k]);
-    st_run<V, float>(part + (int64_t)K * p.C, nc, db);
+    for (int k = 0; k < K; ++k) st_run<V, float>(part + (int64_t)k * p.C, V, dw[k]);
+    st_run<V, float>(part + (int64_t)K * p.C, V, db);
 }
 
 // The chunks' sums in order: the same result every time.  16 threads a column,
@@ -368,7 +369,7 @@ static void conv_slot_launch(const ConvSlotParams& p, hipStream_t s) {
     else hipLaunchKernelGGL((conv_slot_step<T, 0>), grid, dim3(256), 0, s, p);
 }
 
-static int conv_pk_make(const mamba_conv1d_packed_args* a, ConvPk* o) {
+static int conv_pk_make(const mamba_conv1d_packed_args* a, bool back, ConvPk* o) {
     MAMBA_CHECK_ARG(a != nullptr, "args is NULL");
     MAMBA_CHECK_ARG(a->rows >= 0 && a->rows < kMaxRows, "rows must be in [0, 2^31 - 2^20)");
     MAMBA_CHECK_ARG(a->channels >= 1 && a->channels <= (1 << 20), "channels must be in [1, 2^20]");
@@ -383,11 +384,19 @@ static int conv_pk_make(const mamba_conv1d_packed_args* a, ConvPk* o) {
     p.rows = a->rows; p.C = a->channels; p.K = a->kernel;
     p.silu = a->silu != 0; p.fill = a->fill_outside != 0;
     p.x = a->x; p.x_st = a->x_st; p.w = a->w; p.b = a->bias;
-    // rows of a chunk: four waves a SIMD where the rows are enough for it; 8 to 64 (long
-    // chunks read fewer rows twice at their edges; 16384 x 5120 forward 60 us with 64, 70
-    // with 32), and at most 2^20 items of 64 channels, which keeps the grid small
-    const int64_t fill = a->rows * ceil_div(p.C, 256) / 4096;
-    p.chunk = std::min<int64_t>(64, std::max<int64_t>(8, fill / 4 * 4));
+    // Rows of a chunk, and at most 2^20 items of 64 channels, which keeps the grid small.
+    // Forward: four waves a SIMD where the rows are enough for it; 8 to 64 (long chunks
+    // read fewer rows twice at their edges; 16384 x 5120 60 us with 64, 70 with 32).
+    // Backward: rounds of three waves a SIMD, which is what its registers allow, of at
+    // most 128 rows, so that the last round is a whole one (16384 x 5120 bf16 with the
+    // join: 108 rows, one round, 126 us; 64 rows, 1.7 rounds, 136; 36 rows, 3 rounds, 145).
+    if (back) {
+        const int64_t fill = std::max<int64_t>(1, a->rows * ceil_div(p.C, 256) / 3072), rounds = (fill + 127) / 128;
+        p.chunk = std::max<int64_t>(8, (fill / rounds + 4) / 4 * 4);
+    } else {
+        const int64_t fill = a->rows * ceil_div(p.C, 256) / 4096;
+        p.chunk = std::min<int64_t>(64, std::max<int64_t>(8, fill / 4 * 4));
+    }
     while ((a->rows + p.chunk - 1) / p.chunk * ceil_div(p.C, 64) > (1ll << 20)) p.chunk *= 2;
     p.nchunk = (a->rows + p.chunk - 1) / p.chunk;
     return MAMBA_OK;
@@ -400,21 +409,20 @@ static uint32_t conv_pk_grid(const ConvPk& p, int V) {
 template <typename T, int KT, int V>
 static void conv_pk_launch(const ConvPk& p, bool back, hipStream_t s) {
     const dim3 grid(conv_pk_grid(p, V));
-    if (p.C % V == 0) {
-        if (back) hipLaunchKernelGGL((conv_pk_bwd<T, KT, V, true>), grid, dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((conv_pk_fwd<T, KT, V, true>), grid, dim3(256), 0, s, p);
-    } else {
-        if (back) hipLaunchKernelGGL((conv_pk_bwd<T, KT, V, false>), grid, dim3(256), 0, s, p);
-        else hipLaunchKernelGGL((conv_pk_fwd<T, KT, V, false>), grid, dim3(256), 0, s, p);
-    }
+    if (back) hipLaunchKernelGGL((conv_pk_bwd<T, KT, V>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((conv_pk_fwd<T, KT, V>), grid, dim3(256), 0, s, p);
 }
 
 template <typename T>
 static void conv_pk_dispatch(const ConvPk& p, bool back, hipStream_t s) {
-    switch (p.K) {
+    switch (p.C >= 4 ? p.K : 0) {
         case 2: conv_pk_launch<T, 2, 4>(p, back, s); break;
         case 3: conv_pk_launch<T, 3, 4>(p, back, s); break;
         case 4: conv_pk_launch<T, 4, 4>(p, back, s); break;
+        case 5: conv_pk_launch<T, 5, 2>(p, back, s); break;
+        case 6: conv_pk_launch<T, 6, 2>(p, back, s); break;
+        case 7: conv_pk_launch<T, 7, 2>(p, back, s); break;
+        case 8: conv_pk_launch<T, 8, 2>(p, back, s); break;
         default: conv_pk_launch<T, 0, 1>(p, back, s);
     }
 }
@@ -425,7 +433,7 @@ using namespace mamba;
 
 extern "C" int mamba_conv1d_packed_fwd(const mamba_conv1d_packed_args* a, mamba_stream_t stream) {
     ConvPk p;
-    int st = conv_pk_make(a, &p);
+    int st = conv_pk_make(a, false, &p);
     if (st != MAMBA_OK) return st;
     if (p.rows == 0) return MAMBA_OK;
     MAMBA_CHECK_ARG(a->x && a->out, "x and out are required");
@@ -452,13 +460,13 @@ extern "C" int mamba_conv1d_packed_fwd(const mamba_conv1d_packed_args* a, mamba_
 
 extern "C" size_t mamba_conv1d_packed_bwd_workspace_size(const mamba_conv1d_packed_args* a) {
     ConvPk p;
-    if (conv_pk_make(a, &p) != MAMBA_OK || (!a->dw && !a->dbias)) return 0;
+    if (conv_pk_make(a, true, &p) != MAMBA_OK || (!a->dw && !a->dbias)) return 0;
     return (size_t)p.nchunk * (p.K + 1) * p.C * 4;
 }
 
 extern "C" int mamba_conv1d_packed_bwd(const mamba_conv1d_packed_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {
     ConvPk p;
-    int st = conv_pk_make(a, &p);
+    int st = conv_pk_make(a, true, &p);
     if (st != MAMBA_OK) return st;
     MAMBA_CHECK_ARG(a->state == nullptr, "the gradient is of sequences without a window");
     MAMBA_CHECK_ARG(p.rows == 0 || (a->x && a->dout), "x and dout are required");

@@ -19,6 +19,7 @@ LENS = {
     "borders": [64, 64, 128, 1, 127],
     "long": [700],
     "tokens": [1] * 70,
+    "thousands": [30000, 1, 20011],
 }
 
 
@@ -255,7 +256,9 @@ def test_scan_of_whole_sequences(dev):
 
 CONV = [("one", 3, 4, F32, 0, True), ("mixed", 130, 4, BF16, 3, True), ("borders", 600, 3, F32, 0, True),
         ("long", 77, 2, BF16, 5, False), ("mixed", 9, 1, F32, 0, True), ("tokens", 260, 4, F32, 0, True),
-        ("mixed", 70, 7, F32, 2, True), ("short", 5, 64, BF16, 0, True)]
+        ("mixed", 70, 7, F32, 2, True), ("short", 5, 64, BF16, 0, True),
+        ("mixed", 129, 8, F32, 0, True), ("borders", 131, 5, BF16, 3, True), ("mixed", 2, 6, F32, 2, False), ("long", 5, 4, BF16, 0, True),
+        ("tokens", 33, 9, F32, 0, True), ("thousands", 5, 4, F32, 7, True)]
 
 
 @pytest.mark.parametrize("name,c,k,dtype,pad,act", CONV)

@@ -32,11 +32,17 @@
 // fixed order.
 //
 // A workgroup of 256 threads holds CPB = 1024 / NP channels, NP = the states
-// padded to 16, 32 or 64; a channel is spread over NS = NP / 4 lanes with 4 states
-// each.  Tiles of 16 rows are staged through LDS as f32 with the element-wise
+// padded to 8, 16, 32 or 64; a channel is spread over NS = NP / 4 lanes with 4 states
+// each.  Tiles of 16 rows (8 for NP = 8) are staged through LDS as f32 with the element-wise
 // work (softplus, d u, the gate) done once per element; rows past a tile's end
 // and channels past D are staged as zeros, which are steps that change nothing.
 // The next tile's rows are loaded while a tile is scanned.
+//
+// Measured at 8192 rows x 5120 channels, 16 states, bf16, six sequences (us, then
+// the share of cycles that the vector units issue in; HBM moves what each reads and
+// writes in a fraction of its time): state pass 114, all of them; out 176, 0.98;
+// backward state pass 209, all; backward 574, 0.86; the carries 11 and 14, the joins
+// 18 and 6.  Their bytes alone would take 31, 68, 136 and 200 us at the rate of a copy.
 #include <algorithm>
 #include <cmath>
 
@@ -105,19 +111,20 @@ __device__ __forceinline__ float pk_dpp(float v) {
 // then the mirrors of half rows and rows.
 template <int NS>
 __device__ __forceinline__ float group_sum_all(float v) {
-    static_assert(NS == 4 || NS == 8 || NS == 16, "4, 8 or 16 lanes");
+    static_assert(NS == 2 || NS == 4 || NS == 8 || NS == 16, "2, 4, 8 or 16 lanes");
     v += pk_dpp<0xB1>(v);
-    v += pk_dpp<0x4E>(v);
+    if (NS >= 4) v += pk_dpp<0x4E>(v);
     if (NS >= 8) v += pk_dpp<0x141>(v);
     if (NS >= 16) v += pk_dpp<0x140>(v);
     return v;
 }
 
-constexpr int kTile = 16;  // rows of a tile
+constexpr int kTile = 16;  // rows of a chunk come in multiples of this
 
+// NS lanes a channel, CPB channels a workgroup, tiles of TT rows, EV elements a thread
 template <int NP>
 struct ScanShape {
-    static constexpr int NS = NP / 4, CPB = 256 / NS, EV = kTile * CPB / 256;  // EV elements a thread
+    static constexpr int NS = NP / 4, CPB = 256 / NS, TT = NP == 8 ? 8 : kTile, EV = TT * CPB / 256;
 };
 
 // The element-wise mapping: row tid / (CPB / EV) of the tile, EV channels from
@@ -133,10 +140,10 @@ struct ElemMap {
     }
 };
 
-// B or C of a tile: element i = tid + 256 k of [kTile rows][NP states]
+// B or C of a tile: element i = tid + 256 k of [TT rows][NP states]
 template <typename T, int NP>
 struct BcTile {
-    static constexpr int K = kTile * NP / 256;
+    static constexpr int TT = ScanShape<NP>::TT, K = (TT * NP + 255) / 256;
     T v[K];
     __device__ __forceinline__ void load(const void* src, int64_t st, int t0, int n, int N) {
         const T* base = static_cast<const T*>(src) + t0 * st;
@@ -150,7 +157,7 @@ struct BcTile {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int i = threadIdx.x + 256 * k;
-            dst[i / NP][i % NP] = load_f32<T>(&v[k]);
+            if (TT * NP % 256 == 0 || i < TT * NP) dst[i / NP][i % NP] = load_f32<T>(&v[k]);
         }
     }
 };
@@ -224,9 +231,13 @@ __device__ __forceinline__ void store_plane(float* base, int64_t ck, const ScanP
     if (d < p.D) *plane<NP>(base, ck, p, d, ng) = make_float4(h[0], h[1], h[2], h[3]);
 }
 
+// The state that chunk ck leaves to the next, from zero or from its last sequence's own
+// start, and the sum of d.  Four rows' operands are read from LDS before the four
+// dependent steps.  114 us at 8192 x 5120 bf16: 52 M wave instructions, of which 10.5 M
+// exps at about four times a multiply's time, leave the vector units no idle cycle.
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_state(ScanPk p) {
-    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = kTile;
+    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = ScanShape<NP>::TT;
     __shared__ float2 s_dd[TT][CPB];
     __shared__ __align__(16) float s_B[TT][NP];
     const int nblk = (p.D + CPB - 1) / CPB;
@@ -309,7 +320,8 @@ __global__ __launch_bounds__(256) void scan_pk_state(ScanPk p) {
 
 // A thread per (channel, state) walks the chunks: E[ck] <- the state that leaves
 // chunk ck, or (BACK, from the last) G[ck] <- the gradient of the state that
-// enters it.  kAhead chunks' values are loaded at a time.
+// enters it.  kAhead chunks' values are loaded at a time: the walk is one round of
+// memory latency per 16 chunks (11 us for 37 chunks x 5120 x 16, 14 backward).
 template <int NP, bool BACK>
 __device__ __forceinline__ void carry_walk(const ScanPk& p, int i) {
     constexpr int kAhead = 16;
@@ -345,9 +357,13 @@ __global__ __launch_bounds__(64) void scan_pk_carry(ScanPk p) {
     carry_walk<NP, false>(p, blockIdx.x * 64 + threadIdx.x);
 }
 
+// The outputs of a chunk (or of a whole sequence) from the state that enters it.  A
+// row's sum over the states stays inside NS lanes (DPP); it goes through LDS to the
+// element-wise mapping for D u, the gate and a wide store.  176 us at 8192 x 5120
+// bf16: 0.98 of the vector units' cycles.
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
-    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = kTile;
+    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = ScanShape<NP>::TT;
     __shared__ float2 s_dd[TT][CPB];
     __shared__ __align__(16) float s_y[TT][CPB];
     __shared__ __align__(16) float s_B[TT][NP];
@@ -493,9 +509,12 @@ constexpr int kSub = 8;  // rows whose states and decays wait in registers
 // sequence's part (from zero where the sequence came in, with the sum of d up to
 // there: scan_pk_bwd adds what came in).  Row a + kSub i, i >= 1, of a part that
 // begins at a is kept at place (a + kSub i) / kSub: no two parts share one.
+// 209 us at 8192 x 5120 bf16, the vector units busy throughout; 357 MB written, 8 rows'
+// states apart (every 4th row's would be 690 MB, every 16th's would not fit the
+// registers of scan_pk_bwd).
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_state_bwd(ScanPk p) {
-    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = kTile;
+    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = ScanShape<NP>::TT;
     __shared__ float2 s_dd[TT][CPB];
     __shared__ float s_e[TT][CPB];
     __shared__ __align__(16) float s_B[TT][NP];
@@ -660,11 +679,15 @@ __device__ __forceinline__ void channel_sums(const float (&v)[4], const float (&
         x0 += pk_dpp<0x124>(x0);  // row_ror:4
         x1 += pk_dpp<0x124>(x1);
     }
+    if (NS <= 2) {
+        x0 += pk_dpp<0x122>(x0);  // row_ror:2
+        x1 += pk_dpp<0x122>(x1);
+    }
 }
 
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
-    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = kTile;
+    constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = ScanShape<NP>::TT;
     __shared__ __align__(16) float2 s_dd[TT][CPB];
     __shared__ __align__(16) float s_e[TT][CPB];
     __shared__ __align__(16) float s_sB[TT][CPB], s_sA[TT][CPB], s_sC[TT][CPB];
@@ -999,7 +1022,8 @@ __global__ __launch_bounds__(256) void scan_slot_any(ScanSlotParams p) {
 // each, CPT channels a thread.  The state is read and written once (HBM-bound:
 // 8 N bytes a channel against some 12 of everything else), so its loads are
 // issued first and none waits under a branch: what is optional is read through a
-// pointer to something that is there, and dropped.
+// pointer to something that is there, and dropped.  256 tokens x 5120 x 16, bf16: 35.6
+// us, 178 MB, 5.0 TB/s.
 template <typename T, int N, int CPT>
 __global__ __launch_bounds__(256) void scan_slot_step(ScanSlotParams p) {
     constexpr int LPC = N / 4, CPB = 256 / LPC;
@@ -1079,7 +1103,8 @@ static void scan_slot_dispatch(const ScanSlotParams& p, hipStream_t s) {
 
 // ---------------------------------------------------------------- dispatch ---
 
-static int scan_np(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : 64; }
+// (8192 x 5120 bf16 with 8 states: 224 us forward and 537 backward, 312 and 835 padded to 16)
+static int scan_np(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
 static int scan_pk_make(const mamba1_scan_packed_args* a, ScanPk* o) {
     MAMBA_CHECK_ARG(a != nullptr, "args is NULL");
@@ -1168,7 +1193,10 @@ static void scan_pk_bwd_launch(const ScanPk& p, hipStream_t s) {
 
 #define SCAN_PK_DISPATCH(fn, np, bf16, ...)              \
     do {                                                 \
-        if ((np) == 16) {                                \
+        if ((np) == 8) {                                 \
+            if (bf16) fn<bf16_t, 8>(__VA_ARGS__);        \
+            else fn<float, 8>(__VA_ARGS__);              \
+        } else if ((np) == 16) {                         \
             if (bf16) fn<bf16_t, 16>(__VA_ARGS__);       \
             else fn<float, 16>(__VA_ARGS__);             \
         } else if ((np) == 32) {                         \

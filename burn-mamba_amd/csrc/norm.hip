@@ -147,7 +147,7 @@ template <typename T>
 constexpr int kLnE = 16 / (int)sizeof(T);
 
 // G lanes a row, V steps: G (V - 1) kLnE < cols <= G V kLnE, so that only the last
-// step can pass the row's end (G = 16: cols <= 16 kLnE).  The workgroups take their rows in
+// step can pass the row's end.  The workgroups take their rows in
 // turn, the next row's loads in flight while this one is summed; weight and bias
 // stay in registers.
 template <typename T, int G, int V>
@@ -391,18 +391,21 @@ static uint32_t ln_grid(int64_t rows) { return (uint32_t)std::min<int64_t>(rows,
 // steps of 16 bytes a lane that the columns take with G lanes a row
 template <typename T>
 static int ln_steps(int cols, int G) { return ceil_div(cols, G * kLnE<T>); }
-// Lanes a row, 0: the row is not held in registers.  16 lanes where one step of them
-// is enough, a wave for five steps of it (2560 bf16 elements), then a workgroup.
+// Lanes a row, 0: the row is not held in registers.  16 lanes where four steps of them
+// are enough (backward: one, for sixteen groups' sums meet at its end), a wave for
+// five steps of it (2560 bf16 elements), then a workgroup.  us with 16 lanes / a wave, bf16,
+// forward: 65536 x 192 11 / 21, x 384 17 / 22, x 512 23 / 24; backward: 65536 x 256
+// 30 / 36, but 16384 x 256 21 / 17 and 16384 x 512 32 / 19.
 template <typename T>
-static int ln_lanes(int cols) {
-    return ln_steps<T>(cols, 16) <= 1 ? 16 : ln_steps<T>(cols, 64) <= 5 ? 64 : ln_steps<T>(cols, 256) <= 5 ? 256 : 0;
+static int ln_lanes(int cols, bool back) {
+    return ln_steps<T>(cols, 16) <= (back ? 1 : 4) ? 16 : ln_steps<T>(cols, 64) <= 5 ? 64 : ln_steps<T>(cols, 256) <= 5 ? 256 : 0;
 }
 // Workgroups of the forward: four a CU (16384 x 2560 bf16: 31 us; 34 with six or three), or one for each group of rows.
 static uint32_t ln_fwd_grid(int64_t rows, int G) { return (uint32_t)std::min<int64_t>((rows + 256 / G - 1) / (256 / G), 1024); }
 // Workgroups of the backward: four a CU where the rows are enough for it, and
 // some eight rows a group at least, so that the parts stay few beside the rows.
 static int ln_parts(int64_t rows, int cols, bool bf16) {
-    const int G = bf16 ? ln_lanes<bf16_t>(cols) : ln_lanes<float>(cols);
+    const int G = bf16 ? ln_lanes<bf16_t>(cols, true) : ln_lanes<float>(cols, true);
     if (G == 0) return (int)std::min<int64_t>(256, (rows + 31) / 32);
     return (int)std::min<int64_t>(1024, (rows + 8 * (256 / G) - 1) / (8 * (256 / G)));
 }
@@ -415,17 +418,25 @@ static bool ln_rows_ok(int64_t rows, int cols, int64_t sr) {
 
 template <typename T, int G, int V>
 static void ln_rows_launch(const LnParams& p, bool back, hipStream_t s) {
-    if (back) hipLaunchKernelGGL((ln_bwd_rows<T, G, V>), dim3(p.parts), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((ln_fwd_rows<T, G, V>), dim3(ln_fwd_grid(p.rows, G)), dim3(256), 0, s, p);
+    if constexpr (G > 16 || V == 1) {
+        if (back) {
+            hipLaunchKernelGGL((ln_bwd_rows<T, G, V>), dim3(p.parts), dim3(256), 0, s, p);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((ln_fwd_rows<T, G, V>), dim3(ln_fwd_grid(p.rows, G)), dim3(256), 0, s, p);
 }
 
 // rows in registers; false where they are too wide
 template <typename T>
 static bool ln_rows(const LnParams& p, bool back, hipStream_t s) {
-    const int G = ln_lanes<T>(p.cols);
+    const int G = ln_lanes<T>(p.cols, back);
     if (G == 0) return false;
     switch (G * 8 + ln_steps<T>(p.cols, G)) {
         case 16 * 8 + 1: ln_rows_launch<T, 16, 1>(p, back, s); break;
+        case 16 * 8 + 2: ln_rows_launch<T, 16, 2>(p, back, s); break;
+        case 16 * 8 + 3: ln_rows_launch<T, 16, 3>(p, back, s); break;
+        case 16 * 8 + 4: ln_rows_launch<T, 16, 4>(p, back, s); break;
         case 64 * 8 + 1: ln_rows_launch<T, 64, 1>(p, back, s); break;
         case 64 * 8 + 2: ln_rows_launch<T, 64, 2>(p, back, s); break;
         case 64 * 8 + 3: ln_rows_launch<T, 64, 3>(p, back, s); break;

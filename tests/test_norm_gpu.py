@@ -42,7 +42,8 @@ def ln_oracle(x, w, b, eps, dy=None):
 
 LN = [(1, 1, F32, True), (1, 2560, BF16, True), (3, 7, F32, False), (33, 769, F32, True), (130, 100, BF16, True),
       (17, 128, F32, True), (65, 512, BF16, True), (40, 1000, BF16, True), (500, 257, F32, False), (9, 4097, F32, True),
-      (6, 5120, BF16, True), (5, 20000, F32, True), (2, 33001, BF16, True), (1100, 2560, BF16, True), (70, 1536, F32, True)]
+      (6, 5120, BF16, True), (5, 20000, F32, True), (2, 33001, BF16, True), (1100, 2560, BF16, True), (70, 1536, F32, True),
+      (37, 200, BF16, True), (300, 384, BF16, False), (65, 130, F32, True), (19, 255, F32, True)]
 
 
 @pytest.mark.parametrize("rows,cols,dtype,affine", LN)

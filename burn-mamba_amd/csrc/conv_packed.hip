@@ -80,6 +80,7 @@ __device__ __forceinline__ void conv_store(void* dst, int64_t st, int t, int c, 
     st_run<V, T>(static_cast<T*>(dst) + t * st + (uint32_t)c, V, o);
 }
 
+// 16384 x 5120 bf16, K = 4: 63 us, 336 MB (5.3 TB/s).
 template <typename T, int KT, int V>
 __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
     constexpr int KM = KT ? KT : kMaxTaps, R = KT ? kConvRows : 1;
@@ -163,6 +164,8 @@ __global__ __launch_bounds__(256) void conv_pk_window(ConvPk p) {
     }
 }
 
+// dx, and a chunk's share of dw and db in registers.  16384 x 5120 bf16, K = 4: 119 us, 520
+// MB and 16 of parts (4.5 TB/s; the vector units issue 0.6 of the time), the join 7.
 template <typename T, int KT, int V>
 __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
     constexpr int KM = KT ? KT : kMaxTaps, R = KT ? kConvRows : 1;
@@ -320,7 +323,7 @@ struct ConvSlotParams {
 // product rounded, pairs of them summed first, then the bias, and SiLU with a
 // correctly rounded division (silu_f32).  A bf16 output then rounds the way the
 // composition's does, and the state that the scan keeps from it in f32 does not
-// differ by bf16 steps.
+// differ by bf16 steps.  256 tokens x 5120, K = 4, bf16: 8.7 us, 47 MB (5.4 TB/s).
 template <typename T, int KT>
 __global__ __launch_bounds__(256) void conv_slot_step(ConvSlotParams p) {
 #pragma clang fp contract(off)

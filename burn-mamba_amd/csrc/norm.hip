@@ -42,25 +42,56 @@ __device__ __forceinline__ float ln_block_sum(float v, float* red) {
     return s;
 }
 
-// Any width: a workgroup per row, the row read once per sweep.
+// elements of a lane and step: 16 bytes
+template <typename T>
+constexpr int kLnE = 16 / (int)sizeof(T);
+
+// E weights from column c of those up to cols, 1 where there are none
+template <int E>
+__device__ __forceinline__ void ln_weights(const float* w, int c, int cols, float (&v)[E]) {
+    if (w) {
+        ld_run<E, float>(w + c, cols - c, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = 1.f;
+    }
+}
+
+// Any width: a workgroup per row, the row read once per sweep.  4096 x 16384 bf16 138 us,
+// f32 201: the three sweeps and the store at 3.9 TB/s (512 or 768 workgroups, whose
+// rows the L2 would hold, take longer).
 template <typename T>
 __global__ __launch_bounds__(256) void ln_fwd_wide(LnParams p) {
+    constexpr int E = kLnE<T>, S = 256 * E;
     __shared__ float red[4];
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const T* x = static_cast<const T*>(p.x) + r * p.x_sr;
         T* y = static_cast<T*>(p.out) + r * p.out_sr;
-        float s = 0.f;
-        for (int c = threadIdx.x; c < p.cols; c += 256) s += load_f32<T>(x + c);
+        float s = 0.f, v[E];
+        for (int c = threadIdx.x * E; c < p.cols; c += S) {
+            ld_run<E, T>(x + c, p.cols - c, v);
+#pragma unroll
+            for (int i = 0; i < E; ++i) s += v[i];
+        }
         const float mean = ln_block_sum(s, red) / (float)p.cols;
         s = 0.f;
-        for (int c = threadIdx.x; c < p.cols; c += 256) {
-            const float d = load_f32<T>(x + c) - mean;
-            s += d * d;
+        for (int c = threadIdx.x * E; c < p.cols; c += S) {
+            ld_run<E, T>(x + c, p.cols - c, v);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float d = c + i < p.cols ? v[i] - mean : 0.f;
+                s = __builtin_fmaf(d, d, s);
+            }
         }
         const float rstd = 1.f / sqrtf(ln_block_sum(s, red) / (float)p.cols + p.eps);
-        for (int c = threadIdx.x; c < p.cols; c += 256) {
-            const float v = (load_f32<T>(x + c) - mean) * rstd;
-            store_f32<T>(y + c, v * (p.w ? p.w[c] : 1.f) + (p.b ? p.b[c] : 0.f));
+        for (int c = threadIdx.x * E; c < p.cols; c += S) {
+            float w[E], b[E];
+            ld_run<E, T>(x + c, p.cols - c, v);
+            ln_weights<E>(p.w, c, p.cols, w);
+            if (p.b) ld_run<E, float>(p.b + c, p.cols - c, b);
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] = __builtin_fmaf((v[i] - mean) * rstd, w[i], p.b ? b[i] : 0.f);
+            st_run<E, T>(y + c, p.cols - c, v);
         }
         if (threadIdx.x == 0) {
             if (p.mean) p.mean[r] = mean;
@@ -69,50 +100,81 @@ __global__ __launch_bounds__(256) void ln_fwd_wide(LnParams p) {
     }
 }
 
+// 4096 x 16384 with ln_dw_wide and the join: bf16 260 us, f32 369
 template <typename T>
 __global__ __launch_bounds__(256) void ln_dx_wide(LnParams p) {
+    constexpr int E = kLnE<T>, S = 256 * E;
     __shared__ float red[4];
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const T* x = static_cast<const T*>(p.x) + r * p.x_sr;
         const T* dy = static_cast<const T*>(p.dy) + r * p.dy_sr;
         T* dx = static_cast<T*>(p.out) + r * p.out_sr;
         const float mean = p.mean[r], rstd = p.rstd[r];
-        float s1 = 0.f, s2 = 0.f;
-        for (int c = threadIdx.x; c < p.cols; c += 256) {
-            const float g = load_f32<T>(dy + c) * (p.w ? p.w[c] : 1.f);
-            s1 += g;
-            s2 += g * (load_f32<T>(x + c) - mean) * rstd;
+        float s1 = 0.f, s2 = 0.f, v[E], g[E], w[E];
+        auto load = [&](int c) __attribute__((always_inline)) {  // dy is 0 past the row's end
+            ld_run<E, T>(x + c, p.cols - c, v);
+            ld_run<E, T>(dy + c, p.cols - c, g);
+            ln_weights<E>(p.w, c, p.cols, w);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                g[i] *= w[i];
+                v[i] = c + i < p.cols ? (v[i] - mean) * rstd : 0.f;
+            }
+        };
+        for (int c = threadIdx.x * E; c < p.cols; c += S) {
+            load(c);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                s1 += g[i];
+                s2 = __builtin_fmaf(g[i], v[i], s2);
+            }
         }
         s1 = ln_block_sum(s1, red) / (float)p.cols;
         s2 = ln_block_sum(s2, red) / (float)p.cols;
-        for (int c = threadIdx.x; c < p.cols; c += 256) {
-            const float g = load_f32<T>(dy + c) * (p.w ? p.w[c] : 1.f);
-            store_f32<T>(dx + c, rstd * (g - s1 - (load_f32<T>(x + c) - mean) * rstd * s2));
+        for (int c = threadIdx.x * E; c < p.cols; c += S) {
+            load(c);
+#pragma unroll
+            for (int i = 0; i < E; ++i) g[i] = rstd * (g[i] - s1 - v[i] * s2);
+            st_run<E, T>(dx + c, p.cols - c, g);
         }
     }
 }
 
-// dw and db of 64 columns over one part of the rows: thread (c, q) takes every
-// fourth row.
+// dw and db of 64 runs of columns over one part of the rows: thread (run, q) takes
+// every fourth row.
 template <typename T>
 __global__ __launch_bounds__(256) void ln_dw_wide(LnParams p) {
-    __shared__ float red[2][4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+    constexpr int E = kLnE<T>;
+    __shared__ float red[2][4][E][64];
+    const int l = threadIdx.x & 63, c = (blockIdx.x * 64 + l) * E, q = threadIdx.x >> 6;
     const int64_t per = (p.rows + p.parts - 1) / p.parts;
     const int64_t r0 = blockIdx.y * per, r1 = min(p.rows, r0 + per);
-    float sw = 0.f, sb = 0.f;
+    float sw[E], sb[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) sw[i] = sb[i] = 0.f;
     if (c < p.cols)
         for (int64_t r = r0 + q; r < r1; r += 4) {
-            const float dy = load_f32<T>(static_cast<const T*>(p.dy) + r * p.dy_sr + c);
-            sb += dy;
-            sw += dy * (load_f32<T>(static_cast<const T*>(p.x) + r * p.x_sr + c) - p.mean[r]) * p.rstd[r];
+            float v[E], g[E];
+            ld_run<E, T>(static_cast<const T*>(p.x) + r * p.x_sr + c, p.cols - c, v);
+            ld_run<E, T>(static_cast<const T*>(p.dy) + r * p.dy_sr + c, p.cols - c, g);
+            const float mean = p.mean[r], rstd = p.rstd[r];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                sb[i] += g[i];
+                sw[i] = __builtin_fmaf(g[i], (v[i] - mean) * rstd, sw[i]);
+            }
         }
-    red[0][q][threadIdx.x & 63] = sw;
-    red[1][q][threadIdx.x & 63] = sb;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        red[0][q][i][l] = sw[i];
+        red[1][q][i][l] = sb[i];
+    }
     __syncthreads();
-    if (q < 2 && c < p.cols) {
-        const int l = threadIdx.x & 63;
-        p.part[((int64_t)blockIdx.y * 2 + q) * p.cols + c] = (red[q][0][l] + red[q][1][l]) + (red[q][2][l] + red[q][3][l]);
+    if (q < 2) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (c + i < p.cols)
+                p.part[((int64_t)blockIdx.y * 2 + q) * p.cols + c + i] = (red[q][0][i][l] + red[q][1][i][l]) + (red[q][2][i][l] + red[q][3][i][l]);
     }
 }
 
@@ -142,14 +204,11 @@ __device__ __forceinline__ float ln_sum(float v, float* red) {
     }
 }
 
-// elements of a lane and step: 16 bytes
-template <typename T>
-constexpr int kLnE = 16 / (int)sizeof(T);
-
 // G lanes a row, V steps: G (V - 1) kLnE < cols <= G V kLnE, so that only the last
 // step can pass the row's end.  The workgroups take their rows in
 // turn, the next row's loads in flight while this one is summed; weight and bias
-// stay in registers.
+// stay in registers.  16384 x 2560 bf16: 27 us, 168 MB (6 TB/s, part of it out of the
+// last-level cache).
 template <typename T, int G, int V>
 __global__ __launch_bounds__(256) void ln_fwd_rows(LnParams p) {
     constexpr int E = kLnE<T>, RB = 256 / G;
@@ -224,7 +283,8 @@ __global__ __launch_bounds__(256) void ln_fwd_rows(LnParams p) {
 }
 
 // The workgroups take their rows in turn, the next row's loads issued before this
-// one's sums; part[blockIdx.x] gets the workgroup's dw and db.
+// one's sums; part[blockIdx.x] gets the workgroup's dw and db.  16384 x 2560 bf16: 51
+// us, 252 MB and 10 of parts (5.1 TB/s), the join 5.
 template <typename T, int G, int V>
 __global__ __launch_bounds__(256) void ln_bwd_rows(LnParams p) {
     constexpr int E = kLnE<T>, RB = 256 / G;  // rows at a time
@@ -460,7 +520,7 @@ static void ln_bwd_launch(const LnParams& p, hipStream_t s) {
     const bool sums = p.dw || p.db;
     if (!ln_rows<T>(p, true, s)) {
         if (p.out) hipLaunchKernelGGL(ln_dx_wide<T>, dim3(ln_grid(p.rows)), dim3(256), 0, s, p);
-        if (sums) hipLaunchKernelGGL(ln_dw_wide<T>, dim3(ceil_div(p.cols, 64), p.parts), dim3(256), 0, s, p);
+        if (sums) hipLaunchKernelGGL(ln_dw_wide<T>, dim3(ceil_div(p.cols, 64 * kLnE<T>), p.parts), dim3(256), 0, s, p);
     }
     if (sums) hipLaunchKernelGGL(ln_dw_join, dim3(ceil_div(2 * p.cols, 16)), dim3(256), 0, s, p);
 }

@@ -28,7 +28,7 @@
 // every 8th row; scan_pk_bwd then takes 8 rows at a time from the last to the
 // first, finds their states and decays again in registers and walks back over
 // them.  dB and dC are sums over channels: over a wave's by lane exchanges, over
-// the workgroup's in LDS, over the workgroups in scan_pk_join_bc; every sum is in a
+// the workgroup's in LDS, over the workgroups in scan_pk_join; every sum is in a
 // fixed order.
 //
 // A workgroup of 256 threads holds CPB = 1024 / NP channels, NP = the states
@@ -41,8 +41,8 @@
 // Measured at 8192 rows x 5120 channels, 16 states, bf16, six sequences (us, then
 // the share of cycles that the vector units issue in; HBM moves what each reads and
 // writes in a fraction of its time): state pass 114, all of them; out 176, 0.98;
-// backward state pass 209, all; backward 574, 0.86; the carries 11 and 14, the joins
-// 18 and 6.  Their bytes alone would take 31, 68, 136 and 200 us at the rate of a copy.
+// backward state pass 209, all; backward 574, 0.86; the carries 11 and 14, the join
+// 20.  Their bytes alone would take 31, 68, 136 and 200 us at the rate of a copy.
 #include <algorithm>
 #include <cmath>
 
@@ -925,53 +925,42 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
     }
 }
 
-// The joins, each in a fixed order: dB and dC over the channel blocks ...
+// The joins, each in a fixed order, 64 values a workgroup and a quarter of their terms
+// each of its waves: workgroups 0 .. par - 1 dA, dD and dbias over the chunks, column j
+// of [D][NP] | [D] | [D]; those behind them dB and dC over the channel blocks.  Their
+// bytes are read once, as they were written (8192 x 5120 x 16: 84 + 12 MB, 20.5 us).
 template <typename T, int NP>
-__global__ __launch_bounds__(256) void scan_pk_join_bc(ScanPk p, int nblk) {
-    // 64 values a workgroup, a quarter of the channel blocks each of its waves
+__global__ __launch_bounds__(256) void scan_pk_join(ScanPk p, int nblk, uint32_t par) {
     __shared__ float red[4][64];
-    const int64_t total = p.rows * 2 * NP, i = blockIdx.x * 64ll + (threadIdx.x & 63);
-    const int q = wave_id();
+    const int q = wave_id(), l = threadIdx.x & 63;
+    const bool params = blockIdx.x < par;
+    const int64_t i = (params ? blockIdx.x : blockIdx.x - par) * 64ll + l, nA = (int64_t)p.D * NP;
+    const int64_t total = params ? nA + 2 * p.D : p.rows * 2 * NP;
+    const float* src = !params ? p.pBC + i : i < nA ? p.pA + i : i < nA + p.D ? p.pD + (i - nA) : p.pb + (i - nA - p.D);
+    const int64_t pitch = !params ? total : i < nA ? nA : p.D;
+    const int count = params ? p.nchunk : nblk;
     float s = 0.f;
     if (i < total) {
 #pragma unroll 8
-        for (int b = q; b < nblk; b += 4) s += p.pBC[b * total + i];
+        for (int k = q; k < count; k += 4) s += src[k * pitch];
     }
-    red[q][threadIdx.x & 63] = s;
+    red[q][l] = s;
     __syncthreads();
     if (q || i >= total) return;
-    s = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
-    const int64_t t = i / (2 * NP);
-    const int k = (int)(i - t * 2 * NP), n = k % NP;
-    if (n >= p.N) return;
-    if (k < NP) store_f32<T>(static_cast<T*>(p.dB) + t * p.dB_st + n, s);
-    else store_f32<T>(static_cast<T*>(p.dC) + t * p.dC_st + n, s);
-}
-
-// ... and dA, dD, dbias over the chunks: column j of [D][NP] | [D] | [D].
-template <int NP>
-__global__ __launch_bounds__(256) void scan_pk_join_par(ScanPk p) {
-    __shared__ float red[4][64];
-    const int64_t j = blockIdx.x * 64ll + (threadIdx.x & 63), nA = (int64_t)p.D * NP;
-    const int q = threadIdx.x >> 6;
-    const float* src = j < nA ? p.pA + j : j < nA + p.D ? p.pD + (j - nA) : p.pb + (j - nA - p.D);
-    const int64_t pitch = j < nA ? nA : p.D;
-    const bool live = j < nA + 2 * p.D;
-    float s = 0.f;
-    if (live)
-        for (int64_t ck = q; ck < p.nchunk; ck += 4) s += src[ck * pitch];
-    red[q][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (q || !live) return;
-    s = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
-    if (j < nA) {
-        const int64_t d = j / NP;
-        const int n = (int)(j % NP);
-        if (n < p.N) p.dA[d * p.N + n] = s;
-    } else if (j < nA + p.D) {
-        if (p.dD) p.dD[j - nA] = s;
+    s = (red[0][l] + red[1][l]) + (red[2][l] + red[3][l]);
+    if (!params) {
+        const int64_t t = i / (2 * NP);
+        const int k = (int)(i - t * 2 * NP), n = k % NP;
+        if (n >= p.N) return;
+        if (k < NP) store_f32<T>(static_cast<T*>(p.dB) + t * p.dB_st + n, s);
+        else store_f32<T>(static_cast<T*>(p.dC) + t * p.dC_st + n, s);
+    } else if (i < nA) {
+        const int n = (int)(i % NP);
+        if (n < p.N) p.dA[i / NP * p.N + n] = s;
+    } else if (i < nA + p.D) {
+        if (p.dD) p.dD[i - nA] = s;
     } else if (p.db) {
-        p.db[j - nA - p.D] = s;
+        p.db[i - nA - p.D] = s;
     }
 }
 
@@ -1166,7 +1155,8 @@ static void scan_pk_fwd_plan(ScanPk& p, int max_seqlen) {
 // a grid's threads stay below 2^32
 static int scan_pk_grid_ok(const ScanPk& p) {
     const int64_t nblk = ceil_div(p.D, 1024 / scan_np(p.N));
-    if (p.nchunk * nblk >= (1ll << 24) || p.rows * 2 * scan_np(p.N) >= (1ll << 30)) {
+    const int64_t np = scan_np(p.N), joined = p.rows * 2 * np + p.D * (np + 2) + 128;  // 64 a workgroup
+    if (p.nchunk * nblk >= (1ll << 24) || joined > (1ll << 30)) {
         set_error("mamba1_scan_packed: rows * dim is too large for one call");
         return MAMBA_ERR_UNSUPPORTED;
     }
@@ -1190,9 +1180,9 @@ static void scan_pk_bwd_launch(const ScanPk& p, hipStream_t s) {
         hipLaunchKernelGGL((scan_pk_state_bwd<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
         if (p.nchunk > 1) hipLaunchKernelGGL((scan_pk_carry_bwd<NP>), dim3(ceil_div(p.D * NP, 64), 2), dim3(64), 0, s, p);
         hipLaunchKernelGGL((scan_pk_bwd<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
-        hipLaunchKernelGGL((scan_pk_join_bc<T, NP>), dim3((uint32_t)((p.rows * 2 * NP + 63) / 64)), dim3(256), 0, s, p, (int)nblk);
     }
-    hipLaunchKernelGGL((scan_pk_join_par<NP>), dim3((uint32_t)(((int64_t)p.D * (NP + 2) + 63) / 64)), dim3(256), 0, s, p);
+    const uint32_t par = (uint32_t)(((int64_t)p.D * (NP + 2) + 63) / 64);
+    hipLaunchKernelGGL((scan_pk_join<T, NP>), dim3(par + (uint32_t)((p.rows * 2 * NP + 63) / 64)), dim3(256), 0, s, p, (int)nblk, par);
 }
 
 #define SCAN_PK_DISPATCH(fn, np, bf16, ...)              \

@@ -80,7 +80,7 @@ __device__ __forceinline__ void conv_store(void* dst, int64_t st, int t, int c, 
     st_run<V, T>(static_cast<T*>(dst) + t * st + (uint32_t)c, V, o);
 }
 
-// 16384 x 5120 bf16, K = 4: 63 us, 336 MB (5.3 TB/s).
+// 16384 x 5120 bf16, K = 4: 61 us, 344 MB (5.6 TB/s).
 template <typename T, int KT, int V>
 __global__ __launch_bounds__(256) void conv_pk_fwd(ConvPk p) {
     constexpr int KM = KT ? KT : kMaxTaps, R = KT ? kConvRows : 1;
@@ -164,8 +164,8 @@ __global__ __launch_bounds__(256) void conv_pk_window(ConvPk p) {
     }
 }
 
-// dx, and a chunk's share of dw and db in registers.  16384 x 5120 bf16, K = 4: 119 us, 520
-// MB and 16 of parts (4.5 TB/s; the vector units issue 0.6 of the time), the join 7.
+// dx, and a chunk's share of dw and db in registers.  16384 x 5120 bf16, K = 4: 111 us, 519
+// MB and 16 of parts (4.8 TB/s; the vector units issue 0.7 of the time), the join 6.6.
 template <typename T, int KT, int V>
 __global__ __launch_bounds__(256) void conv_pk_bwd(ConvPk p) {
     constexpr int KM = KT ? KT : kMaxTaps, R = KT ? kConvRows : 1;

@@ -394,7 +394,7 @@ static int conv_pk_make(const mamba_conv1d_packed_args* a, bool back, ConvPk* o)
     // most 128 rows, so that the last round is a whole one (16384 x 5120 bf16 with the
     // join: 108 rows, one round, 126 us; 64 rows, 1.7 rounds, 136; 36 rows, 3 rounds, 145).
     if (back) {
-        const int64_t fill = std::max<int64_t>(1, a->rows * ceil_div(p.C, 256) / 3072), rounds = (fill + 127) / 128;
+        const int64_t fill = std::max<int64_t>(1, a->rows * ceil_div(p.C, 256) / (3 * 1024)), rounds = (fill + 127) / 128;
         p.chunk = std::max<int64_t>(8, (fill / rounds + 4) / 4 * 4);
     } else {
         const int64_t fill = a->rows * ceil_div(p.C, 256) / 4096;

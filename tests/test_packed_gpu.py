@@ -443,3 +443,64 @@ def test_graph_and_streams(dev):
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+
+
+def test_slots_far_into_a_cache(dev):
+    """Slots whose states lie behind 2^31 elements, as in a small cache."""
+    d, n, k, far, wide = 5120, 16, 4, 26999, 104999
+    t = scan_inputs([40, 3], d, n, BF16, dev, seed=31)
+    c, w = cu([40, 3], dev), torch.randn(d, k, generator=gen(32)).to(dev)
+    near, there = torch.tensor([1, 0], dtype=torch.int32, device=dev), torch.tensor([far, 2], dtype=torch.int32, device=dev)
+    small = torch.randn(2, d, n, generator=gen(33)).to(dev)
+    state = torch.empty(far + 1, d, n, device=dev)
+    state[there.long()] = small[near.long()]
+    assert state[far].storage_offset() > 2 ** 31
+    for call in (lambda h, slots: mamba_hip.mamba1_scan_packed(**t, cu_seqlens=c, delta_softplus=True, state=h, slots=slots),
+                 lambda h, slots: mamba_hip.mamba1_scan_packed(**t, cu_seqlens=c, delta_softplus=True, state=h, slots=slots, max_seqlen=40),
+                 lambda h, slots: mamba_hip.scan_step_slots(**{key: v[:2] if key in ("u", "delta", "B", "C", "z") else v for key, v in t.items()},
+                                                            state=h, slots=slots, delta_softplus=True)):
+        assert torch.equal(call(state, there), call(small, near))
+        assert torch.equal(state[there.long()], small[near.long()])
+    del state
+    there[0] = wide
+    small = torch.randn(2, d, k, generator=gen(34)).to(dev)
+    window = torch.empty(wide + 1, d, k, device=dev)
+    window[there.long()] = small[near.long()]
+    assert window[wide].storage_offset() > 2 ** 31
+    assert torch.equal(mamba_hip.conv1d_packed(t["u"], w, c, state=window, slots=there),
+                       mamba_hip.conv1d_packed(t["u"], w, c, state=small, slots=near))
+    assert torch.equal(mamba_hip.conv1d_step_slots(t["u"][:2], window, there, w), mamba_hip.conv1d_step_slots(t["u"][:2], small, near, w))
+    assert torch.equal(window[there.long()], small[near.long()])
+
+
+def test_rows_far_apart(dev):
+    """Rows behind 2^31 elements, read and written."""
+    rows, d, n, pitch = 70, 40, 16, 2 ** 25 - 8
+    t = scan_inputs([rows], d, n, BF16, dev, seed=35)
+    base = torch.empty(rows * pitch, dtype=BF16, device=dev)
+    at = 0
+
+    def apart(v):
+        nonlocal at
+        out = base.as_strided((rows, v.shape[1]), (pitch, 1), at)
+        at += v.shape[1] + 3
+        return out.copy_(v)
+    far = {k: apart(v) if k in ("u", "delta", "B", "C", "z") else v for k, v in t.items()}
+    c, y, out = cu([30, 40], dev), apart(t["u"]), apart(t["u"])
+    assert y[-1].storage_offset() > 2 ** 31
+    kw = dict(cu_seqlens=c, delta_softplus=True)
+    assert mamba_hip.mamba1_scan_packed(**far, **kw, y=y) is y
+    want = mamba_hip.mamba1_scan_packed(**t, **kw)
+    assert torch.equal(y, want)
+    a, b = mamba_hip.mamba1_scan_packed_bwd(y, **far, **kw), mamba_hip.mamba1_scan_packed_bwd(want, **t, **kw)
+    assert all(v is None or torch.equal(v, b[k]) for k, v in a.items())
+    w = torch.randn(d, 4, generator=gen(36)).to(dev)
+    assert torch.equal(mamba_hip.conv1d_packed(far["u"], w, c, out=out), mamba_hip.conv1d_packed(t["u"], w, c))
+    a, b = mamba_hip.conv1d_packed_bwd(y, far["u"], w, c), mamba_hip.conv1d_packed_bwd(want, t["u"], w, c)
+    assert all(v is None or torch.equal(v, b[k]) for k, v in a.items())
+    scale, stats = torch.randn(d, generator=gen(37)).to(dev), [tuple(torch.empty(rows, device=dev) for _ in range(2)) for _ in range(2)]
+    assert torch.equal(mamba_hip.layer_norm(far["u"], scale, out=out, stats=stats[0]), mamba_hip.layer_norm(t["u"], scale, stats=stats[1]))
+    a, b = mamba_hip.layer_norm_bwd(y, far["u"], scale, *stats[0]), mamba_hip.layer_norm_bwd(want, t["u"], scale, *stats[1])
+    assert all(torch.equal(v, b[k]) for k, v in a.items())
+    rng = torch.tensor([3, 4], device=dev)
+    assert torch.equal(mamba_hip.dropout(far["u"], 0.4, rng, residual=far["z"], out=out), mamba_hip.dropout(t["u"], 0.4, rng, residual=t["z"]))

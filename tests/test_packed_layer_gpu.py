@@ -147,6 +147,39 @@ def test_trained_parameters_are_the_ones_served(dev):
         near(layer.step(token, mine, slots)[0], want, 1e-5, "token")
 
 
+def test_training_step_in_a_graph(dev):
+    """Forward and gradients captured, no eager graph of the leaves alive; replayed on other
+    rows and other dropout masks, with eager steps between."""
+    layer, x, cu = make(dev, p=0.3)
+    rng, dy = torch.tensor([5, 9], device=dev), torch.randn(x.shape, generator=torch.Generator().manual_seed(4)).to(dev)
+    leaves = [t.requires_grad_() for t in params(layer)] + [x.requires_grad_()]
+
+    def step():
+        y = layer.forward_packed(x, cu, rng=rng)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for k in range(3):
+        with torch.no_grad():
+            x.mul_(0.9)
+            layer.mixer.a_log.add_(0.01)
+        rng += 1
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), k
+
+
 def test_two_streams_share_a_weight_copy(dev):
     """The second call finds the copy that the first has ordered behind other work."""
     layer, x, cu = make(dev, d_model=256)

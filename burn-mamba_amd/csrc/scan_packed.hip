@@ -17,8 +17,9 @@
 // that a batch of unequal ones loads the chip evenly.  A sequence that crosses a
 // chunk's end is carried: scan_pk_state finds the state a chunk leaves behind
 // when it starts from zero (or from the sequence's own start) and the sum of d
-// over it, scan_pk_carry walks the chunks, h <- exp(A sum d) h + own, and
-// scan_pk_out scans again from there.  Where the sequences are many and the longest
+// over it, a walk over the chunks, h <- exp(A sum d) h + own, finds what comes into each
+// (in scan_pk_out, or for many chunks in scan_pk_carry), and scan_pk_out scans again
+// from there.  Where the sequences are many and the longest
 // is known to be short, scan_pk_out takes whole sequences instead and nothing is
 // carried.
 //
@@ -66,6 +67,7 @@ struct ScanPk {
     void* y; int64_t y_st;
     float* state; int64_t nslots; const int32_t* slots;
     int chunk, nchunk;
+    bool walk;                      // chunks find what comes into them by themselves
     bool whole;                     // a workgroup takes a sequence: nchunk = the sequences
     // per chunk: what it leaves behind [nchunk][D][NP] (then, carried, what
     // leaves it), the sum of d [nchunk][D], and the state that its last sequence
@@ -229,6 +231,32 @@ __device__ __forceinline__ void load_plane(float* base, int64_t ck, const ScanPk
 template <int NP>
 __device__ __forceinline__ void store_plane(float* base, int64_t ck, const ScanPk& p, int d, int ng, const float (&h)[4]) {
     if (d < p.D) *plane<NP>(base, ck, p, d, ng) = make_float4(h[0], h[1], h[2], h[3]);
+}
+
+// What comes into a chunk over the chunks of its sequence before it (or, for a
+// gradient, behind it): X[from], then X[j] + exp(A sum d of j) times what came so far,
+// to chunk `to`.  With the carries already walked (p.walk false), X[to] itself.
+template <int NP>
+__device__ __forceinline__ void load_carry(float* X, int from, int to, const ScanPk& p, int d, int ng, const float (&A2)[4], float (&h)[4]) {
+    constexpr int kAhead = 4;
+    if (!p.walk) from = to;
+    const int step = to >= from ? 1 : -1, count = (to - from) * step;
+    load_plane<NP>(X, from, p, d, ng, h);
+    for (int j = 1; j <= count; j += kAhead) {
+        float own[kAhead][4], sd[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int ck = from + min(j + i, count) * step;
+            load_plane<NP>(X, ck, p, d, ng, own[i]);
+            sd[i] = d < p.D ? p.sumd[(int64_t)ck * p.D + d] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (j + i > count) break;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(sd[i] * A2[k]), h[k], own[i][k]);
+        }
+    }
 }
 
 // The state that chunk ck leaves to the next, from zero or from its last sequence's own
@@ -422,7 +450,7 @@ __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
         const int64_t slot = p.state ? slot_of(p.slots, s, p.nslots) : -1;
         fetch(t, b);
         if (e.in && t == e.c0) {  // goes on from the chunk before
-            load_plane<NP>(p.E, ck - 1, p, d, ng, h);
+            load_carry<NP>(p.E, min(st / p.chunk, ck - 1), ck - 1, p, d, ng, A2, h);
         } else if (en > e.c1 && p.state) {
             load_plane<NP>(p.h0c, ck, p, d, ng, h);
         } else {
@@ -765,9 +793,9 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
         const int len = b - t, tiles = (len + TT - 1) / TT;
         fetch(t + (tiles - 1) * TT, b);
         float h0[4], g[4], hn[4], dn = 0.f;  // hn, dn: the next part's kept state and sum of d
-        if (in) load_plane<NP>(p.E, ck - 1, p, d, ng, h0);
+        if (in) load_carry<NP>(p.E, min(st / p.chunk, ck - 1), ck - 1, p, d, ng, A2, h0);
         else load_state(p.h0, s, p, d, ng, h0);
-        if (en > e.c1) load_plane<NP>(p.G, ck + 1, p, d, ng, g);
+        if (en > e.c1) load_carry<NP>(p.G, (en - 1) / p.chunk, ck + 1, p, d, ng, A2, g);
         else load_state(p.dhT, s, p, d, ng, g);
         auto kept = [&](int q) {  // before row kSub q of the run
             if (q <= 0) return;
@@ -1126,28 +1154,34 @@ static int scan_pk_make(const mamba1_scan_packed_args* a, ScanPk* o) {
 }
 
 // Rows of a chunk: four workgroups a CU where the rows are enough for it, at most
-// 256 rows (longer ones gain nothing), and at least about 0.6 sqrt(rows), where the
-// carry's walk over the chunks (0.15 us each) and the scan of one (0.2 us a row and
-// pass) weigh alike.  us, forward, at 1024 / 2048 / 4096 workgroups: 8192 x 5120
-// 325 / 328 / 323, 4000 x 2560 103 / 107 / 114, 2000 x 2560 63 / 67 / 72; at 16 / 32
-// rows at least: 1000 x 1024 40 / 33, 300 x 2560 25 / 24, 77 x 512 15.6 / 18.
+// 256 rows (longer ones gain nothing), and at least about 0.6 sqrt(rows), where a
+// chunk's walk over those before it and its own scan (0.2 us a row and pass) weigh alike.
+// us, forward, at 1024 / 2048 / 4096 workgroups: 8192 x 5120 325 / 328 / 323, 4000 x
+// 2560 103 / 107 / 114, 2000 x 2560 63 / 67 / 72; at 0.3 / 0.45 / 0.6 / 0.85 sqrt(rows):
+// 8192 x 256 89 / 72 / 50 / 48, with the backward 218 / 185 / 137 / 139, 1023 x 777 31 / 31 / 25 / 25.
+// Up to 128 chunks find what comes into them by themselves; the walk of all of them in a
+// kernel of its own takes 10 to 14 us more where they are few (forward and backward,
+// 1023 x 777 84 against 71; 4000 x 2560 340 against 325; 8192 x 256, 128 chunks, 158
+// against 137), but each walks over half of them on average.
 static void scan_pk_plan(ScanPk& p) {
     const int64_t nblk = ceil_div(p.D, 1024 / scan_np(p.N));
     const int64_t fill = (p.rows * nblk + 1023) / 1024, least = (int64_t)(0.6 * std::sqrt((double)p.rows));
     const int64_t rows = std::max<int64_t>(1, std::max(fill, least));
     p.chunk = (int)std::min<int64_t>(256, (rows + kTile - 1) / kTile * kTile);
     p.nchunk = (int)((p.rows + p.chunk - 1) / p.chunk);
+    p.walk = p.nchunk <= 128;
 }
 // Whole sequences, a workgroup of CPB channels each, where the longest is known to
-// be short beside all the rows' work (its rows take some 0.15 us one behind the
-// other; in chunks most rows are scanned twice), or 96 rows at most, which take no
-// longer than three launches.  us, forward, whole / in chunks: 8 sequences of 2048
-// x 5120 468 / 580, 4 of them 360 / 301, 16 of 512 191 / 271, 16 of 256 x 2560 67 /
-// 103; 16 of unlike length, the longest about 2000, 473 / 306; 5 of 120 x 2560 21 / 34.
+// be short beside all the rows' work: its rows take some 0.15 us one behind the
+// other, and in chunks most rows are scanned twice.  Up to 96 rows in any case: the
+// chunks' second launch and workspace cost a call as much as they save.  us, forward, whole /
+// in chunks: 8 sequences of 2048 x 5120 466 / 558, 4 of them 352 / 285, 16 of 512 190 /
+// 259, 16 of 256 x 2560 64 / 91, 8 of 512 95 / 95, 16 of 128 x 1024 23 / 31, 8 of them
+// 22 / 21, one of 77 x 512 15 / 13, of 40 10 / 12.
 static void scan_pk_fwd_plan(ScanPk& p, int max_seqlen) {
     scan_pk_plan(p);
     const int64_t nblk = ceil_div(p.D, 1024 / scan_np(p.N));
-    if (p.nchunk > 1 && max_seqlen > 0 && p.q.n > 0 && max_seqlen <= std::max<int64_t>(96, p.rows * nblk / 384)) {
+    if (p.nchunk > 1 && max_seqlen > 0 && p.q.n > 0 && max_seqlen <= std::max<int64_t>(96, 64 + p.rows * nblk / 384)) {
         p.whole = true;
         p.nchunk = p.q.n;
     }
@@ -1168,7 +1202,7 @@ static void scan_pk_fwd_launch(const ScanPk& p, hipStream_t s) {
     const uint32_t nblk = ceil_div(p.D, ScanShape<NP>::CPB);
     if (p.nchunk > 1 && !p.whole) {
         hipLaunchKernelGGL((scan_pk_state<T, NP>), dim3(nblk * (uint32_t)(p.nchunk - 1)), dim3(256), 0, s, p);
-        hipLaunchKernelGGL((scan_pk_carry<NP>), dim3(ceil_div(p.D * NP, 64)), dim3(64), 0, s, p);
+        if (!p.walk) hipLaunchKernelGGL((scan_pk_carry<NP>), dim3(ceil_div(p.D * NP, 64)), dim3(64), 0, s, p);
     }
     hipLaunchKernelGGL((scan_pk_out<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
 }
@@ -1178,7 +1212,7 @@ static void scan_pk_bwd_launch(const ScanPk& p, hipStream_t s) {
     const uint32_t nblk = ceil_div(p.D, ScanShape<NP>::CPB);
     if (p.rows) {
         hipLaunchKernelGGL((scan_pk_state_bwd<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
-        if (p.nchunk > 1) hipLaunchKernelGGL((scan_pk_carry_bwd<NP>), dim3(ceil_div(p.D * NP, 64), 2), dim3(64), 0, s, p);
+        if (!p.walk) hipLaunchKernelGGL((scan_pk_carry_bwd<NP>), dim3(ceil_div(p.D * NP, 64), 2), dim3(64), 0, s, p);
         hipLaunchKernelGGL((scan_pk_bwd<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
     }
     const uint32_t par = (uint32_t)(((int64_t)p.D * (NP + 2) + 63) / 64);

@@ -20,6 +20,7 @@ LENS = {
     "long": [700],
     "tokens": [1] * 70,
     "thousands": [30000, 1, 20011],
+    "many chunks": [6000, 1, 0, 199],
 }
 
 
@@ -66,7 +67,7 @@ def roundings(lens):
 CASES = [("one", 1, 1, F32, 0, True), ("short", 5, 16, BF16, 2, False), ("mixed", 70, 16, F32, 3, True),
          ("mixed", 64, 16, BF16, 0, True), ("borders", 37, 20, F32, 0, True), ("long", 65, 5, BF16, 1, False),
          ("mixed", 33, 32, BF16, 0, True), ("borders", 18, 64, F32, 2, True), ("short", 9, 33, F32, 0, True),
-         ("tokens", 40, 16, F32, 0, True)]
+         ("tokens", 40, 16, F32, 0, True), ("mixed", 130, 8, BF16, 3, True), ("many chunks", 8, 5, F32, 0, True)]
 
 
 @pytest.mark.parametrize("name,d,n,dtype,pad,full", CASES)

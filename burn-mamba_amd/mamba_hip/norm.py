@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import DropoutArgs, LayerNormArgs, LayerNormBwdArgs, check
-from .packed import _IO, _fail, _need, _once, _one_device, _p, _param, _raw_stream
+from .packed import _IO, _fail, _need, _new, _once, _one_device, _p, _param, _raw_stream
 from .ssd import _dtype_code, workspace
 
 
@@ -32,7 +32,7 @@ def _matrix(t: torch.Tensor, name: str) -> torch.Tensor:
 def _into(out: Optional[torch.Tensor], x: torch.Tensor) -> tuple:
     """The result tensor and its rows; one that is given has to be written in place."""
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _new(x)
         return out, out if out.dim() == 2 else out.view(-1, out.shape[-1])
     _need(out.shape == x.shape and out.dtype == x.dtype, "out must match x")
     m = _matrix(out, "out")
@@ -46,19 +46,24 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[t
     and bias [cols] f32 or None).  ``stats``: two f32 tensors of a value per row that take
     the mean and the reciprocal standard deviation, for ``layer_norm_bwd``."""
     m = _matrix(x, "x")
+    mean, rstd = stats if stats is not None else (None, None)
+    _param(mean, "mean", m.shape[0])
+    _param(rstd, "rstd", m.shape[0])
+    return _ln_fwd(m, x, weight, bias, eps, out, mean, rstd, _p(mean), _p(rstd))
+
+
+def _ln_fwd(m, x, weight, bias, eps, out, mean, rstd, mean_at, rstd_at):
+    """``layer_norm`` of the rows m of x, the statistics' places as pointers."""
     rows, cols = m.shape
     _param(weight, "weight", cols)
     _param(bias, "bias", cols)
-    mean, rstd = stats if stats is not None else (None, None)
-    _param(mean, "mean", rows)
-    _param(rstd, "rstd", rows)
     _need(eps >= 0, "eps must be >= 0")
     with _one_device(m, weight, bias, mean, rstd, out):
         out, o = _into(out, x)
         a = LayerNormArgs()
         a.rows, a.cols, a.io_dtype, a.eps = rows, cols, _dtype_code(m), float(eps)
         a.x, a.x_sr, a.weight, a.bias = m.data_ptr(), m.stride(0), _p(weight), _p(bias)
-        a.y, a.y_sr, a.mean, a.rstd = o.data_ptr(), o.stride(0), _p(mean), _p(rstd)
+        a.y, a.y_sr, a.mean, a.rstd = o.data_ptr(), o.stride(0), mean_at, rstd_at
         check(_lib.lib().mamba_layernorm_fwd(ctypes.byref(a), _raw_stream(x)), "mamba_layernorm_fwd")
     return out
 
@@ -74,16 +79,17 @@ def layer_norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Ten
     _param(mean, "mean", rows)
     _param(rstd, "rstd", rows)
     with _one_device(m, g, weight, mean, rstd):
-        dx, dweight, dbias = _ln_bwd(g, m, weight, mean.data_ptr(), rstd.data_ptr(), x.shape)
+        dx, dweight, dbias = _ln_bwd(g, m, weight, mean.data_ptr(), rstd.data_ptr(), x)
     return dict(dx=dx, dweight=dweight, dbias=dbias)
 
 
-def _ln_bwd(g, m, weight, mean: int, rstd: int, shape):
-    """``layer_norm_bwd`` after its checks, the statistics as pointers."""
+def _ln_bwd(g, m, weight, mean: int, rstd: int, x):
+    """``layer_norm_bwd`` after its checks (m: the rows of x), the statistics as pointers."""
     a = LayerNormBwdArgs()
     rows, cols = m.shape
-    dx = torch.empty(shape, dtype=m.dtype, device=m.device)
-    dweight, dbias = torch.empty((2, cols), dtype=torch.float32, device=m.device).unbind()
+    dx = _new(x)
+    dweight = m.new_empty(cols, dtype=torch.float32) if weight is None else _new(weight)
+    dbias = _new(dweight)
     a.rows, a.cols, a.io_dtype = rows, cols, _dtype_code(m)
     a.x, a.x_sr, a.dy, a.dy_sr = m.data_ptr(), m.stride(0), g.data_ptr(), g.stride(0)
     a.weight, a.mean, a.rstd = _p(weight), mean, rstd
@@ -98,9 +104,10 @@ def _ln_bwd(g, m, weight, mean: int, rstd: int, shape):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        rows = x.numel() // max(x.shape[-1], 1) if x.dim() else 0
-        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-        y = layer_norm(x, weight, bias, eps, stats=stats.unbind())
+        m = _matrix(x, "x")
+        stats = m.new_empty((2, m.shape[0]), dtype=torch.float32)
+        at = stats.data_ptr()
+        y = _ln_fwd(m, x, weight, bias, eps, None, None, None, at, at + 4 * m.shape[0])
         ctx.save_for_backward(x, weight, stats)
         ctx.has_bias = bias is not None
         return y
@@ -110,7 +117,7 @@ class _LayerNorm(torch.autograd.Function):
         x, weight, stats = ctx.saved_tensors
         m, g, at = _matrix(x, "x"), _matrix(dy, "dy"), stats.data_ptr()
         with _one_device(g):
-            dx, dweight, dbias = _ln_bwd(g, m, weight, at, at + 4 * m.shape[0], x.shape)
+            dx, dweight, dbias = _ln_bwd(g, m, weight, at, at + 4 * m.shape[0], x)
         return dx, None if weight is None else dweight, dbias if ctx.has_bias else None, None
 
 
@@ -137,7 +144,7 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, offset: int = 0, resid
     _need(out is None or (out.shape == x.shape and out.dtype == x.dtype), "out must match x")
     with _one_device(x, rng, residual, out):
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            out = _new(x)
         n = x.numel()
         if n == 0:
             return out

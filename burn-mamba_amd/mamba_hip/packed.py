@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -102,6 +103,11 @@ def _raw_stream(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
+# an uninitialised tensor of t's shape and type with rows one behind the other (a few us
+# less than one from shape, type and device)
+_new = functools.partial(torch.empty_like, memory_format=torch.contiguous_format)
+
+
 def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -160,7 +166,7 @@ def conv1d_packed(x: torch.Tensor, w: torch.Tensor, cu_seqlens: torch.Tensor, bi
         _rows(out, "out", x.shape[0], x.shape[1], x.dtype)
     with _one_device(x, w, cu_seqlens, bias, state, slots, out):
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            out = _new(x)
         a.out, a.out_st = out.data_ptr(), out.stride(0)
         check(_lib.lib().mamba_conv1d_packed_fwd(ctypes.byref(a), _raw_stream(x)), "mamba_conv1d_packed_fwd")
     return out
@@ -179,7 +185,7 @@ def conv1d_packed_bwd(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, cu_s
 
 def _conv_bwd(a: Conv1dPackedArgs, dout, x, w, bias):
     """``conv1d_packed_bwd`` after its checks."""
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _new(x)
     dw, dbias = torch.empty_like(w), None if bias is None else torch.empty_like(bias)
     a.fill_outside = 1
     a.dout, a.dout_st = dout.data_ptr(), dout.stride(0)
@@ -228,7 +234,7 @@ def conv1d_step_slots(x: torch.Tensor, state: torch.Tensor, slots: Optional[torc
         _rows(out, "out", b, c, x.dtype)
     with _one_device(x, state, slots, w, bias, out):
         if out is None:
-            out = torch.empty((b, c), dtype=x.dtype, device=x.device)
+            out = _new(x)
         a = Conv1dStepSlotsArgs()
         a.batch, a.channels, a.kernel, a.io_dtype, a.silu = b, c, k, _dtype_code(x), int(bool(silu))
         a.x, a.x_sb, a.state, a.nslots, a.slots = x.data_ptr(), x.stride(0), state.data_ptr(), state.shape[0], _p(slots)
@@ -293,7 +299,7 @@ def mamba1_scan_packed(u, delta, A, B, C, cu_seqlens, D=None, z=None, delta_bias
         _rows(y, "y", u.shape[0], u.shape[1], u.dtype)
     with _one_device(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, state, slots, y):
         if y is None:
-            y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+            y = _new(u)
         a.y, a.y_st = y.data_ptr(), y.stride(0)
         L = _lib.lib()
         need = L.mamba1_scan_packed_workspace_size(ctypes.byref(a))
@@ -321,11 +327,9 @@ def mamba1_scan_packed_bwd(dy, u, delta, A, B, C, cu_seqlens, D=None, z=None, de
 
 def _scan_bwd(a: Mamba1ScanPackedBwdArgs, dy, u, delta, A, B, C, D, z, delta_bias, initial_state, d_final_state) -> dict:
     """``mamba1_scan_packed_bwd`` after its checks."""
-    def new(t):
-        return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-    out = dict(du=new(u), ddelta=new(delta), dz=new(z), dB=new(B), dC=new(C), dA=new(A), dD=new(D),
-               d_delta_bias=new(delta_bias), d_initial_state=None)
+    out = dict(du=_new(u), ddelta=_new(delta), dz=None if z is None else _new(z), dB=_new(B), dC=_new(C), dA=_new(A),
+               dD=None if D is None else _new(D), d_delta_bias=None if delta_bias is None else _new(delta_bias),
+               d_initial_state=None)
     if initial_state is not None:  # an empty sequence ends in what it starts from
         out["d_initial_state"] = torch.zeros_like(initial_state) if d_final_state is None else d_final_state.clone()
     a.initial_state, a.d_final_state = _p(initial_state), _p(d_final_state)
@@ -386,7 +390,7 @@ def scan_step_slots(u, delta, A, B, C, state: torch.Tensor, slots: Optional[torc
         _rows(y, "y", b, d, u.dtype)
     with _one_device(u, delta, A, B, C, state, slots, D, z, delta_bias, y):
         if y is None:
-            y = torch.empty((b, d), dtype=u.dtype, device=u.device)
+            y = _new(u)
         a = Mamba1ScanStepSlotsArgs()
         a.batch, a.dim, a.dstate, a.io_dtype, a.delta_softplus = b, d, n, _dtype_code(u), int(bool(delta_softplus))
         a.u, a.u_sb, a.delta, a.delta_sb = u.data_ptr(), u.stride(0), delta.data_ptr(), delta.stride(0)

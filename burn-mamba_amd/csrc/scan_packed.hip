@@ -41,9 +41,9 @@
 //
 // Measured at 8192 rows x 5120 channels, 16 states, bf16, six sequences (us, then
 // the share of cycles that the vector units issue in; HBM moves what each reads and
-// writes in a fraction of its time): state pass 114, all of them; out 176, 0.98;
-// backward state pass 209, all; backward 574, 0.86; the carries 11 and 14, the join
-// 20.  Their bytes alone would take 31, 68, 136 and 200 us at the rate of a copy.
+// writes in a fraction of its time): state pass 113, all of them; out 180, 0.98;
+// backward state pass 209, all; backward 587, 0.85; the join 20.6.  Their bytes alone
+// would take 32, 71, 139 and 213 us at the rate of a copy.
 #include <algorithm>
 #include <cmath>
 
@@ -261,7 +261,7 @@ __device__ __forceinline__ void load_carry(float* X, int from, int to, const Sca
 
 // The state that chunk ck leaves to the next, from zero or from its last sequence's own
 // start, and the sum of d.  Four rows' operands are read from LDS before the four
-// dependent steps.  114 us at 8192 x 5120 bf16: 52 M wave instructions, of which 10.5 M
+// dependent steps.  113 us at 8192 x 5120 bf16: 52 M wave instructions, of which 10.5 M
 // exps at about four times a multiply's time, leave the vector units no idle cycle.
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_state(ScanPk p) {
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(64) void scan_pk_carry(ScanPk p) {
 
 // The outputs of a chunk (or of a whole sequence) from the state that enters it.  A
 // row's sum over the states stays inside NS lanes (DPP); it goes through LDS to the
-// element-wise mapping for D u, the gate and a wide store.  176 us at 8192 x 5120
+// element-wise mapping for D u, the gate and a wide store.  180 us at 8192 x 5120
 // bf16: 0.98 of the vector units' cycles.
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
@@ -713,8 +713,8 @@ __device__ __forceinline__ void channel_sums(const float (&v)[4], const float (&
     }
 }
 
-// The gradients of a chunk's rows, from the last to the first, kSub at a time.  574 us at
-// 8192 x 5120 bf16: 252 M wave instructions at two waves a SIMD (220 registers), 0.86
+// The gradients of a chunk's rows, from the last to the first, kSub at a time.  587 us at
+// 8192 x 5120 bf16: 256 M wave instructions at two waves a SIMD (223 registers), 0.85
 // of the vector units' cycles; three waves (161 registers, the rows' operands read
 // from LDS again) took 4 % longer.
 template <typename T, int NP>

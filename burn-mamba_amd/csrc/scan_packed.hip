@@ -1171,6 +1171,7 @@ static void scan_pk_plan(ScanPk& p) {
     p.nchunk = (int)((p.rows + p.chunk - 1) / p.chunk);
     p.walk = p.nchunk <= 128;
 }
+constexpr int64_t kMaxGroups = 1ll << 24;  // a grid's threads stay below 2^32
 // Whole sequences, a workgroup of CPB channels each, where the longest is known to
 // be short beside all the rows' work: its rows take some 0.15 us one behind the
 // other, and in chunks most rows are scanned twice.  Up to 96 rows in any case: the
@@ -1181,16 +1182,15 @@ static void scan_pk_plan(ScanPk& p) {
 static void scan_pk_fwd_plan(ScanPk& p, int max_seqlen) {
     scan_pk_plan(p);
     const int64_t nblk = ceil_div(p.D, 1024 / scan_np(p.N));
-    if (p.nchunk > 1 && max_seqlen > 0 && p.q.n > 0 && max_seqlen <= std::max<int64_t>(96, 64 + p.rows * nblk / 384)) {
+    if (p.nchunk > 1 && max_seqlen > 0 && p.q.n > 0 && p.q.n * nblk < kMaxGroups && max_seqlen <= std::max<int64_t>(96, 64 + p.rows * nblk / 384)) {
         p.whole = true;
         p.nchunk = p.q.n;
     }
 }
-// a grid's threads stay below 2^32
-static int scan_pk_grid_ok(const ScanPk& p) {
+static int scan_pk_grid_ok(const ScanPk& p, bool back) {
     const int64_t nblk = ceil_div(p.D, 1024 / scan_np(p.N));
-    const int64_t np = scan_np(p.N), joined = p.rows * 2 * np + p.D * (np + 2) + 128;  // 64 a workgroup
-    if (p.nchunk * nblk >= (1ll << 24) || joined > (1ll << 30)) {
+    const int64_t np = scan_np(p.N), joined = back ? p.rows * 2 * np + p.D * (np + 2) + 128 : 0;
+    if (p.nchunk * nblk >= kMaxGroups || joined > 64 * kMaxGroups) {  // the join: 64 values a workgroup
         set_error("mamba1_scan_packed: rows * dim is too large for one call");
         return MAMBA_ERR_UNSUPPORTED;
     }
@@ -1302,7 +1302,7 @@ extern "C" int mamba1_scan_packed_fwd(const mamba1_scan_packed_args* a, void* ws
     p.y = a->y; p.y_st = a->y_st;
     p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
     scan_pk_fwd_plan(p, a->max_seqlen);
-    if ((st = scan_pk_grid_ok(p)) != MAMBA_OK) return st;
+    if ((st = scan_pk_grid_ok(p, false)) != MAMBA_OK) return st;
     const size_t need = scan_pk_fwd_planes(p, ws);
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");
     if (need && (ws == nullptr || ws_bytes < need)) {
@@ -1353,7 +1353,7 @@ extern "C" int mamba1_scan_packed_bwd(const mamba1_scan_packed_bwd_args* a, void
     p.dB = a->dB; p.dB_st = a->dB_st; p.dC = a->dC; p.dC_st = a->dC_st;
     p.dA = a->dA; p.dD = a->dD; p.db = a->d_delta_bias; p.dh0 = a->d_initial_state;
     scan_pk_plan(p);
-    if ((st = scan_pk_grid_ok(p)) != MAMBA_OK) return st;
+    if ((st = scan_pk_grid_ok(p, true)) != MAMBA_OK) return st;
     const size_t need = scan_pk_bwd_planes(p, ws);
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");
     if (need && (ws == nullptr || ws_bytes < need)) {

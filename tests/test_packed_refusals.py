@@ -165,6 +165,31 @@ def test_the_library_refuses_by_itself():
     assert L.mamba_dropout(ctypes.byref(o), None) == 1 and b"rng" in L.mamba_last_error()
 
 
+def test_many_sequences_and_many_rows():
+    """A bound on the lengths never refuses what is taken without one (here: up to the
+    missing workspace), and the rows that the gradients cannot take the forward can."""
+    L, P = _lib.lib(), 1 << 20  # never dereferenced
+    a = _lib.Mamba1ScanPackedArgs()
+    a.rows, a.nseq, a.dim, a.dstate = 10_000_000, 3_000_000, 512, 16
+    for i, k in enumerate(("cu_seqlens", "u", "delta", "A", "B", "C", "y")):
+        setattr(a, k, P << (20 + i))
+    for k in ("u_st", "delta_st", "B_st", "C_st", "y_st"):
+        setattr(a, k, 512)
+    for most in (0, 10, 10_000_000):
+        a.max_seqlen = most
+        assert L.mamba1_scan_packed_workspace_size(ctypes.byref(a)) > 0
+        assert L.mamba1_scan_packed_fwd(ctypes.byref(a), None, 0, None) == 3
+    a.max_seqlen, a.rows, a.dim = 0, 40_000_000, 64
+    assert L.mamba1_scan_packed_fwd(ctypes.byref(a), None, 0, None) == 3
+    b = _lib.Mamba1ScanPackedBwdArgs()
+    b.fwd = a
+    for i, k in enumerate(("dA", "dy", "du", "ddelta", "dB", "dC")):
+        setattr(b, k, P << (30 + i))
+    for k in ("dy_st", "du_st", "ddelta_st", "dB_st", "dC_st"):
+        setattr(b, k, 64)
+    assert L.mamba1_scan_packed_bwd(ctypes.byref(b), None, 0, None) == 2 and b"too large" in L.mamba_last_error()
+
+
 def test_the_library_refuses_outputs_on_inputs():
     """An output that shares memory with an input: refused but where a thread reads what it
     writes.  The workspace's absence tells that the rest was taken."""

@@ -1007,36 +1007,65 @@ struct ScanSlotParams {
     void* y; int64_t y_sb;
 };
 
-// Any dstate: a thread per channel (256 tokens x 5120 x 12: 86 us, 1.6 TB/s).
+// Any dstate up to 1024: the states of CH = 1024 / N channels lie one behind the other, so
+// the workgroup takes them four a thread whatever N is, and adds h C up by channel
+// in LDS, Q lanes each.  256 tokens x 5120, bf16: 12 states 43 us, 20 states 68 (3.2 TB/s; a
+// thread per channel 90 and 211).
+constexpr int kSlotRun = 1024;
 template <typename T>
 __global__ __launch_bounds__(256) void scan_slot_any(ScanSlotParams p) {
-    const int b = blockIdx.y, d = blockIdx.x * 256 + threadIdx.x;
-    if (d >= p.D) return;
-    T* y = static_cast<T*>(p.y) + b * p.y_sb + d;
+    __shared__ float2 s_dd[kSlotRun];
+    __shared__ float s_u[kSlotRun], s_p[kSlotRun], s_B[kSlotRun], s_C[kSlotRun];
+    const int N = p.N, CH = kSlotRun / N, d0 = blockIdx.x * CH, nc = min(CH, p.D - d0), b = blockIdx.y;
+    T* y = static_cast<T*>(p.y) + b * p.y_sb + d0;
     const int64_t slot = slot_of(p.slots, b, p.nslots);
     if (slot < 0) {
-        store_f32<T>(y, 0.f);
+        for (int c = threadIdx.x; c < nc; c += 256) store_f32<T>(y + c, 0.f);
         return;
     }
-    const float u = load_f32<T>(static_cast<const T*>(p.u) + b * p.u_sb + d);
-    float dv = load_f32<T>(static_cast<const T*>(p.dl) + b * p.dl_sb + d);
-    if (p.bias) dv += p.bias[d];
-    if (p.softplus) dv = pk_softplus(dv);
-    float* h = p.state + (slot * p.D + d) * p.N;
-    float acc = 0.f;
-    for (int n = 0; n < p.N; ++n) {
-        const float bv = load_f32<T>(static_cast<const T*>(p.B) + b * p.B_sb + n);
-        const float cv = load_f32<T>(static_cast<const T*>(p.C) + b * p.C_sb + n);
-        const float hn = __builtin_fmaf(h[n], __builtin_amdgcn_exp2f(dv * (p.A[(int64_t)d * p.N + n] * kLog2e)), dv * u * bv);
-        h[n] = hn;
-        acc = __builtin_fmaf(hn, cv, acc);
+    const int e0 = 4 * threadIdx.x, left = nc * N - e0;
+    float* state = p.state + (slot * p.D + d0) * N + e0;
+    float h[4], A[4];
+    ld_run<4, float>(state, left, h);
+    ld_run<4, float>(p.A + (int64_t)d0 * N + e0, left, A);
+    for (int c = threadIdx.x; c < nc; c += 256) {
+        const float u = load_f32<T>(static_cast<const T*>(p.u) + b * p.u_sb + d0 + c);
+        float dv = load_f32<T>(static_cast<const T*>(p.dl) + b * p.dl_sb + d0 + c);
+        if (p.bias) dv += p.bias[d0 + c];
+        if (p.softplus) dv = pk_softplus(dv);
+        s_dd[c] = make_float2(dv, dv * u);
+        s_u[c] = u;
     }
-    if (p.Dv) acc = __builtin_fmaf(p.Dv[d], u, acc);
-    if (p.z) {
-        const float zv = load_f32<T>(static_cast<const T*>(p.z) + b * p.z_sb + d);
-        acc *= zv * pk_sigmoid(zv);
+    for (int n = threadIdx.x; n < N; n += 256) {
+        s_B[n] = load_f32<T>(static_cast<const T*>(p.B) + b * p.B_sb + n);
+        s_C[n] = load_f32<T>(static_cast<const T*>(p.C) + b * p.C_sb + n);
     }
-    store_f32<T>(y, acc);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (k >= left) break;
+        const int c = (e0 + k) / N, n = e0 + k - c * N;
+        const float2 dd = s_dd[c];
+        h[k] = __builtin_fmaf(h[k], __builtin_amdgcn_exp2f(dd.x * (A[k] * kLog2e)), dd.y * s_B[n]);
+        s_p[e0 + k] = h[k] * s_C[n];
+    }
+    if (left > 0) st_run<4, float>(state, left, h);
+    __syncthreads();
+    int Q = 1;
+    while (Q < 64 && 2 * Q * CH <= 256) Q *= 2;
+    for (int i0 = 0; i0 < nc * Q; i0 += 256) {
+        const int c = (i0 + (int)threadIdx.x) / Q, q = threadIdx.x % Q;
+        float acc = 0.f;
+        for (int n = q; c < nc && n < N; n += Q) acc += s_p[c * N + n];
+        for (int o = Q / 2; o > 0; o >>= 1) acc += __shfl_xor(acc, o);
+        if (q || c >= nc) continue;
+        if (p.Dv) acc = __builtin_fmaf(p.Dv[d0 + c], s_u[c], acc);
+        if (p.z) {
+            const float zv = load_f32<T>(static_cast<const T*>(p.z) + b * p.z_sb + d0 + c);
+            acc *= zv * pk_sigmoid(zv);
+        }
+        store_f32<T>(y + c, acc);
+    }
 }
 
 // dstate 8, 16, 32 or 64: a channel over N / 4 lanes with 16 bytes of its state
@@ -1118,7 +1147,7 @@ static void scan_slot_dispatch(const ScanSlotParams& p, hipStream_t s) {
         case 16: scan_slot_launch<T, 16>(p, s); break;
         case 32: scan_slot_launch<T, 32>(p, s); break;
         case 64: scan_slot_launch<T, 64>(p, s); break;
-        default: hipLaunchKernelGGL(scan_slot_any<T>, dim3(ceil_div(p.D, 256), p.nb), dim3(256), 0, s, p);
+        default: hipLaunchKernelGGL(scan_slot_any<T>, dim3(ceil_div(p.D, kSlotRun / p.N), p.nb), dim3(256), 0, s, p);
     }
 }
 

@@ -318,7 +318,7 @@ struct ConvSlotParams {
     void* out; int64_t out_sb;
 };
 
-// KT: 4 or 2 with 16- or 8-byte windows, or 0 for any width.  HBM-bound (8 K bytes
+// KT = K up to 8 (4 and 2 with windows of 16 and 8 aligned bytes), or 0 for any width.  HBM-bound (8 K bytes
 // of window an element), so the arithmetic may be the plain composition's: each
 // product rounded, pairs of them summed first, then the bias, and SiLU with a
 // correctly rounded division (silu_f32).  A bf16 output then rounds the way the
@@ -341,16 +341,22 @@ __global__ __launch_bounds__(256) void conv_slot_step(ConvSlotParams p) {
     const float xv = load_f32<T>(static_cast<const T*>(p.x) + b * p.x_sb + c);
     float acc;
     if constexpr (KT != 0) {
+        constexpr int kAlign = KT == 4 || KT == 2 ? 4 * KT : 4;
         float v[KT], wv[KT];
-        __builtin_memcpy(v, __builtin_assume_aligned(win, 4 * KT), 4 * KT);
-        __builtin_memcpy(wv, __builtin_assume_aligned(w, 4 * KT), 4 * KT);
+        __builtin_memcpy(v, __builtin_assume_aligned(win, kAlign), 4 * KT);
+        __builtin_memcpy(wv, __builtin_assume_aligned(w, kAlign), 4 * KT);
 #pragma unroll
         for (int k = 0; k < KT; ++k) v[k] = k + 1 < KT ? v[k + 1] : xv;
-        acc = v[0] * wv[0] + v[1] * wv[1];
-        if constexpr (KT == 4) acc = acc + (v[2] * wv[2] + v[3] * wv[3]);
-        __builtin_memcpy(__builtin_assume_aligned(win, 4 * KT), v, 4 * KT);
+        if constexpr (KT == 4) {
+            acc = (v[0] * wv[0] + v[1] * wv[1]) + (v[2] * wv[2] + v[3] * wv[3]);
+        } else {  // even taps and odd ones
+            float s[2] = {0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KT; ++k) s[k & 1] = s[k & 1] + v[k] * wv[k];
+            acc = s[0] + s[1];
+        }
+        __builtin_memcpy(__builtin_assume_aligned(win, kAlign), v, 4 * KT);
     } else {
-        // even taps and odd ones
         float s[2] = {0.f, 0.f};
         for (int k = 0; k < K; ++k) {
             const float v = k + 1 < K ? win[k + 1] : xv;
@@ -367,9 +373,17 @@ template <typename T>
 static void conv_slot_launch(const ConvSlotParams& p, hipStream_t s) {
     const dim3 grid(ceil_div(p.C, 256), p.nb);
     const uintptr_t at = (uintptr_t)p.state | (uintptr_t)p.w;
-    if (p.K == 4 && (at & 15u) == 0) hipLaunchKernelGGL((conv_slot_step<T, 4>), grid, dim3(256), 0, s, p);
-    else if (p.K == 2 && (at & 7u) == 0) hipLaunchKernelGGL((conv_slot_step<T, 2>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((conv_slot_step<T, 0>), grid, dim3(256), 0, s, p);
+    const int kt = (p.K == 4 && (at & 15u)) || (p.K == 2 && (at & 7u)) ? 0 : p.K;
+    switch (kt) {
+        case 2: hipLaunchKernelGGL((conv_slot_step<T, 2>), grid, dim3(256), 0, s, p); break;
+        case 3: hipLaunchKernelGGL((conv_slot_step<T, 3>), grid, dim3(256), 0, s, p); break;
+        case 4: hipLaunchKernelGGL((conv_slot_step<T, 4>), grid, dim3(256), 0, s, p); break;
+        case 5: hipLaunchKernelGGL((conv_slot_step<T, 5>), grid, dim3(256), 0, s, p); break;
+        case 6: hipLaunchKernelGGL((conv_slot_step<T, 6>), grid, dim3(256), 0, s, p); break;
+        case 7: hipLaunchKernelGGL((conv_slot_step<T, 7>), grid, dim3(256), 0, s, p); break;
+        case 8: hipLaunchKernelGGL((conv_slot_step<T, 8>), grid, dim3(256), 0, s, p); break;
+        default: hipLaunchKernelGGL((conv_slot_step<T, 0>), grid, dim3(256), 0, s, p);
+    }
 }
 
 static int conv_pk_make(const mamba_conv1d_packed_args* a, bool back, ConvPk* o) {

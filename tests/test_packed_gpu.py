@@ -307,7 +307,7 @@ def test_conv_autograd(dev):
 @pytest.mark.parametrize("b,d,n,k,dtype,full", [(1, 1, 1, 1, F32, True), (5, 70, 16, 4, BF16, True), (33, 130, 20, 3, F32, False),
                                                 (2, 300, 64, 4, BF16, True), (3, 40, 100, 2, F32, True), (7, 256, 16, 4, F32, True),
                                                 (4, 200, 12, 4, BF16, True), (2, 1030, 1, 3, F32, True), (3, 5, 1000, 4, F32, False),
-                                                (2, 700, 3, 2, F32, True)])
+                                                (2, 700, 3, 5, F32, True), (3, 90, 8, 7, BF16, True), (2, 33, 16, 8, F32, True), (2, 33, 16, 9, F32, True)])
 def test_steps(dev, b, d, n, k, dtype, full):
     """One token per slot: the packed forms of one-row sequences are the same function."""
     g, lens = gen(15), [1] * b

@@ -434,15 +434,14 @@ class Mamba1:
         if grad and cache is not None:
             raise _lib.MambaHipError(_CACHE_GRAD)
         w = (lambda t: t.to(x.dtype)) if grad else (lambda t: _cast(t, x.dtype))
-        xz = torch.mm(x, w(self.in_proj_w))
-        xs, z = xz[:, :di], xz[:, di:]
+        # split, whose gradient is one concatenation (a slice's is a sum of padded ones)
+        xs, z = torch.mm(x, w(self.in_proj_w)).split(di, 1)
         if grad:
             u = conv1d_packed_autograd(xs, self.conv_w, cu_seqlens, self.conv_b)
         else:
             u = conv1d_packed(xs, self.conv_w, cu_seqlens, self.conv_b, True, None if cache is None else cache.conv_bik, slots)
-        x_dbl = torch.mm(u, w(self.x_proj_w))
-        delta = torch.mm(x_dbl[:, :r], w(self.dt_proj_w))
-        B, C = x_dbl[:, r:r + n], x_dbl[:, r + n:]
+        low, B, C = torch.mm(u, w(self.x_proj_w)).split((r, n, n), 1)
+        delta = torch.mm(low, w(self.dt_proj_w))
         if grad:  # A from its parameter, which the gradient goes to
             y, _ = mamba1_scan_packed_autograd(u, delta, -torch.exp(self.a_log), B, C, cu_seqlens, self.d, z, self.dt_proj_b, True,
                                                max_seqlen=max_seqlen)

@@ -462,12 +462,15 @@ static int ln_lanes(int cols, bool back) {
 }
 // Workgroups of the forward: four a CU (16384 x 2560 bf16: 31 us; 34 with six or three), or one for each group of rows.
 static uint32_t ln_fwd_grid(int64_t rows, int G) { return (uint32_t)std::min<int64_t>((rows + 256 / G - 1) / (256 / G), 1024); }
-// Workgroups of the backward: four a CU where the rows are enough for it, and
-// some eight rows a group at least, so that the parts stay few beside the rows.
+// Workgroups of the backward: two a CU where the rows are enough for it, which is what
+// the registers of wide rows leave room for (four for up to 256 columns), and some eight
+// rows a group at least, so that the parts stay few beside the rows.  us at 512 / 1024:
+// 16384 x 5120 bf16 123 / 145, 65536 x 2560 202 / 216, f32 103 / 111 at 16384 x 2560,
+// 65536 x 256 bf16 41 / 36.
 static int ln_parts(int64_t rows, int cols, bool bf16) {
     const int G = bf16 ? ln_lanes<bf16_t>(cols, true) : ln_lanes<float>(cols, true);
     if (G == 0) return (int)std::min<int64_t>(256, (rows + 31) / 32);
-    return (int)std::min<int64_t>(1024, (rows + 8 * (256 / G) - 1) / (8 * (256 / G)));
+    return (int)std::min<int64_t>(cols > 256 ? 512 : 1024, (rows + 8 * (256 / G) - 1) / (8 * (256 / G)));
 }
 
 // rows x cols with these row strides: rows overlap nowhere and every element

@@ -460,7 +460,8 @@ template <typename T>
 static int ln_lanes(int cols, bool back) {
     return ln_steps<T>(cols, 16) <= (back ? 1 : 4) ? 16 : ln_steps<T>(cols, 64) <= 5 ? 64 : ln_steps<T>(cols, 256) <= 5 ? 256 : 0;
 }
-// Workgroups of the forward: four a CU (16384 x 2560 bf16: 31 us; 34 with six or three), or one for each group of rows.
+// Workgroups of the forward: four a CU (16384 x 2560 bf16: 27.6 us; 29.5 with three, 31.5
+// with sixteen), or one for each group of rows.
 static uint32_t ln_fwd_grid(int64_t rows, int G) { return (uint32_t)std::min<int64_t>((rows + 256 / G - 1) / (256 / G), 1024); }
 // Workgroups of the backward: two a CU where the rows are enough for it, which is what
 // the registers of wide rows leave room for (four for up to 256 columns), and some eight

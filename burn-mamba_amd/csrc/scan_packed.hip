@@ -94,12 +94,13 @@ struct ScanPk {
 // hardware log with Goldberg's correction, log(v) e / (v - 1) for v = 1 + e.  The
 // hardware's exp2, log2 and reciprocal as they are (1 <= v, and an e below the normal
 // floats is 0): the library's cases for the smallest floats cost as much again.
-// Without a branch, which would part the elements in the schedule.
+// Without a branch, which would part the elements in the schedule.  The minimum of a
+// NaN and 20 is 20, so the last select asks for x <= 20: what fails it is x itself.
 __device__ __forceinline__ float pk_softplus(float x) {
     const float e = __builtin_amdgcn_exp2f(fminf(x, 20.f) * kLog2e);
     const float v = 1.f + e;
     const float l = __builtin_amdgcn_logf(v) * (1.f / kLog2e) * (e * __builtin_amdgcn_rcpf(v - 1.f));
-    return x > 20.f ? x : v == 1.f ? e : l;
+    return x <= 20.f ? (v == 1.f ? e : l) : x;
 }
 __device__ __forceinline__ float pk_sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -kLog2e));

@@ -249,6 +249,8 @@ def linear_row(x: torch.Tensor, packed_w: torch.Tensor, out: torch.Tensor, norm_
     check(_lib.lib().mamba_linear_row(ctypes.byref(a), _stream(x.device)), "mamba_linear_row")
 
 
+_wrapped = torch._C._functorch.is_functorch_wrapped_tensor
+
 # every derived copy is kept on the weight under an attribute with this prefix
 _DERIVED_PREFIX = "_mamba_"
 
@@ -266,31 +268,49 @@ def _weight_key(w: torch.Tensor):
 
 
 def drop_derived(w: torch.Tensor) -> None:
-    """Forget every derived copy made from ``w`` (the transposed, padded and
-    packed ones; needed only after an in-place update of an inference-mode
-    weight)."""
+    """Mark every derived copy made from ``w`` (the transposed, padded and packed
+    ones) as out of date: the next call that needs one makes it again (asked for only after
+    an in-place update of an inference-mode weight)."""
     for a in [a for a in vars(w) if a.startswith(_DERIVED_PREFIX)]:
-        delattr(w, a)
+        setattr(w, a, (None, *getattr(w, a)[1:]))
 
 
 def _derived(w: torch.Tensor, attr: str, make):
     """The copy of ``w`` that ``make`` builds, made once and kept on the weight
-    tensor itself (so it lives exactly as long) and remade when the weight
+    tensor itself (so it lives exactly as long) and made again when the weight
     changes.  Making it launches device work, which must not be recorded into
     a captured HIP graph: a capture that finds no current copy raises, and the
     caller derives the copies before capturing (``Mamba3.pack_products``).
     The copy is finished before it is handed out: calls on other streams use
-    it too."""
+    it too.
+
+    The new values go where the old ones were, behind everything that is launched on
+    the device: a captured graph holds the copy's address, and its replays read the weight's
+    values of the last call outside a graph.  (Not so a copy that autograd follows, or one
+    that is the weight's own memory, seen in another order.)"""
     key = _weight_key(w)
     hit = getattr(w, attr, None)
     if hit is None or hit[0] != key:
         if w.is_cuda and torch.cuda.is_current_stream_capturing():
             raise _lib.MambaHipError(f"{attr[1:]}: the weight copy must be made before HIP graph capture")
-        hit = (key, make(w))
+        copy = make(w)
+        own = (type(copy) is torch.Tensor and not copy.requires_grad and not _wrapped(copy)
+               and copy.untyped_storage().data_ptr() != w.untyped_storage().data_ptr())
+        if hit is not None and own and hit[2] and _same_layout(hit[1], copy):
+            if w.is_cuda:
+                torch.cuda.synchronize(w.device)
+            # an inference-mode tensor takes updates in that mode only
+            with torch.inference_mode(hit[1].is_inference()), torch.no_grad():
+                copy = hit[1].copy_(copy)
+        hit = (key, copy, own)
         if w.is_cuda:
             torch.cuda.current_stream(w.device).synchronize()
         setattr(w, attr, hit)
     return hit[1]
+
+
+def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.shape == b.shape and a.dtype == b.dtype and a.device == b.device and a.stride() == b.stride()
 
 
 def prefill_mm(x2d: torch.Tensor, w: torch.Tensor) -> torch.Tensor:

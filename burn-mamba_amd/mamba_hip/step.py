@@ -17,8 +17,10 @@ Nothing here computes on the CPU; a missing library raises.
 
 from __future__ import annotations
 
+import collections
 import ctypes
 import math
+import weakref
 from dataclasses import dataclass, field
 from typing import List, Optional, Tuple
 
@@ -257,22 +259,39 @@ _DERIVED_PREFIX = "_mamba_"
 
 def _weight_key(w: torch.Tensor):
     """What identifies a weight's current values for the derived-copy caches
-    below: its version counter, which every in-place update bumps.  Tensors
+    below: its version counter, which every in-place update bumps, and where and how
+    it lies, which an assignment to ``w.data`` changes (an update through ``w.data`` itself is
+    seen by neither: drop_derived(w) must follow it).  Tensors
     made under torch.inference_mode have no version counter; for them the key
     is the storage address and layout, so an in-place update of such a weight
     must be followed by drop_derived(w)."""
     try:
-        return ("version", w._version)
-    except RuntimeError:
-        return ("storage", w.data_ptr(), tuple(w.shape), tuple(w.stride()))
+        return w._version, w.data_ptr(), w.stride()
+    except RuntimeError:  # no counter, or no storage (inside a transform of the product)
+        return ("storage", w.data_ptr(), tuple(w.shape), tuple(w.stride())) if w.is_inference() else ("version", w._version)
+
+
+class _Copy:
+    """A derived copy of the weight ``of`` (weakly held) at its key ``key``; ``own``: memory
+    that is nothing else's.  It belongs to that tensor object: a weight that is copied
+    (copy.deepcopy) or loaded from a file, whose counter begins again, begins without."""
+    __slots__ = ("of", "key", "value", "own")
+
+    def __init__(self, of, key, value, own):
+        self.of, self.key, self.value, self.own = of, key, value, own
+
+    def __reduce__(self):  # what torch.load(weights_only=True) takes
+        return collections.OrderedDict, ()
 
 
 def drop_derived(w: torch.Tensor) -> None:
     """Mark every derived copy made from ``w`` (the transposed, padded and packed
     ones) as out of date: the next call that needs one makes it again (asked for only after
-    an in-place update of an inference-mode weight)."""
-    for a in [a for a in vars(w) if a.startswith(_DERIVED_PREFIX)]:
-        setattr(w, a, (None, *getattr(w, a)[1:]))
+    an in-place update that the weight's version counter does not see: of an inference-mode
+    weight, or through ``w.data``)."""
+    for a, hit in vars(w).items():
+        if a.startswith(_DERIVED_PREFIX) and isinstance(hit, _Copy):
+            hit.key = None
 
 
 def _derived(w: torch.Tensor, attr: str, make):
@@ -290,23 +309,25 @@ def _derived(w: torch.Tensor, attr: str, make):
     that is the weight's own memory, seen in another order.)"""
     key = _weight_key(w)
     hit = getattr(w, attr, None)
-    if hit is None or hit[0] != key:
+    if not isinstance(hit, _Copy) or hit.of() is not w:
+        hit = None
+    if hit is None or hit.key != key:
         if w.is_cuda and torch.cuda.is_current_stream_capturing():
             raise _lib.MambaHipError(f"{attr[1:]}: the weight copy must be made before HIP graph capture")
-        copy = make(w)
-        own = (type(copy) is torch.Tensor and not copy.requires_grad and not _wrapped(copy)
-               and copy.untyped_storage().data_ptr() != w.untyped_storage().data_ptr())
-        if hit is not None and own and hit[2] and _same_layout(hit[1], copy):
+        value = make(w)
+        own = (type(value) is torch.Tensor and not value.requires_grad and not _wrapped(value)
+               and value.untyped_storage().data_ptr() != w.untyped_storage().data_ptr())
+        if hit is not None and own and hit.own and _same_layout(hit.value, value):
             if w.is_cuda:
                 torch.cuda.synchronize(w.device)
             # an inference-mode tensor takes updates in that mode only
-            with torch.inference_mode(hit[1].is_inference()), torch.no_grad():
-                copy = hit[1].copy_(copy)
-        hit = (key, copy, own)
+            with torch.inference_mode(hit.value.is_inference()), torch.no_grad():
+                value = hit.value.copy_(value)
+        hit = _Copy(weakref.ref(w), key, value, own)
         if w.is_cuda:
             torch.cuda.current_stream(w.device).synchronize()
         setattr(w, attr, hit)
-    return hit[1]
+    return hit.value
 
 
 def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:

@@ -1,6 +1,9 @@
 """The copies that serving keeps beside a weight (its decay, its type, its layout): where
 they lie and when they are made again.  On the CPU: no kernel is reached."""
 
+import copy
+import io
+
 import pytest
 import torch
 
@@ -69,3 +72,41 @@ def test_copies_that_stay_apart():
     w.mul_(1)
     got = step._derived(w, "_mamba_test", lambda t: t.t().contiguous())
     assert torch.equal(got, w.t()) and torch.equal(owner, kept)
+
+
+def test_a_copied_block_has_its_own_copies():
+    """copy.deepcopy takes a tensor's attributes along and begins its version counter again:
+    the decay of a block copied from a copied one, after an update that nothing served since."""
+    m = copy.deepcopy(block())
+    assert m.a_log._version == copy.deepcopy(m.a_log)._version  # what the counter alone cannot tell apart
+    mamba1._decay(m.a_log)
+    m.a_log.mul_(0.5)
+    other = copy.deepcopy(m)
+    assert torch.equal(other.A, -torch.exp(m.a_log))
+    m.a_log.mul_(0.5)
+    m.A  # noqa: B018  made again, in its own memory
+    assert torch.equal(other.A, -torch.exp(other.a_log)) and not torch.equal(other.A, m.A)
+
+
+@pytest.mark.parametrize("weights_only", [True, False])
+def test_a_saved_weight_is_loaded_without_copies(weights_only):
+    w = block().a_log
+    w.add_(0)
+    mamba1._decay(w)
+    w.mul_(0.5)
+    file = io.BytesIO()
+    torch.save(w, file)
+    file.seek(0)
+    loaded = torch.load(file, weights_only=weights_only)
+    assert torch.equal(mamba1._decay(loaded), -torch.exp(w))
+
+
+def test_data_assigned():
+    """w.data = another tensor leaves the version counter where it is."""
+    m = block()
+    at = m.A.data_ptr()
+    m.a_log.data = m.a_log.data * 0.5
+    assert torch.equal(m.A, -torch.exp(m.a_log)) and m.A.data_ptr() == at
+    m.a_log.data.mul_(0.5)
+    step.drop_derived(m.a_log)
+    assert torch.equal(m.A, -torch.exp(m.a_log))

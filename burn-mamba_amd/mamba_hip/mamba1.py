@@ -358,9 +358,10 @@ class Mamba1:
     def A(self) -> torch.Tensor:
         return _decay(self.a_log)
 
-    def _wants_grad(self, x: torch.Tensor) -> bool:
+    def _wants_grad(self, *ts: Optional[torch.Tensor]) -> bool:
+        """Of one of ts (its rows, and what made them) or of a parameter."""
         return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (
-            x, self.in_proj_w, self.conv_w, self.conv_b, self.x_proj_w, self.dt_proj_w, self.dt_proj_b, self.a_log, self.d,
+            *ts, self.in_proj_w, self.conv_w, self.conv_b, self.x_proj_w, self.dt_proj_w, self.dt_proj_b, self.a_log, self.d,
             self.out_proj_w))
 
     def new_cache(self, batch: int) -> Mamba1Cache:
@@ -520,7 +521,7 @@ class Mamba1Layer:
     def step(self, x: torch.Tensor, cache: Mamba1Cache, slots: Optional[torch.Tensor] = None):
         """One token per row of x [b, d_model] on ``cache`` (``Mamba1.step``)."""
         from .norm import layer_norm
-        if self.mixer._wants_grad(x):
+        if self.mixer._wants_grad(x, self.norm_w, self.norm_b):
             raise _lib.MambaHipError(_CACHE_GRAD)
         y, cache = self.mixer.step(layer_norm(x, self.norm_w, self.norm_b, self.eps), cache, slots)
         return x + y, cache

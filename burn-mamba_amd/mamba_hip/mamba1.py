@@ -431,6 +431,8 @@ class Mamba1:
         di, r, n = c.d_inner, c.dt_rank, c.state_rank
         if x.dim() != 2 or x.shape[1] != c.d_model:
             raise _lib.MambaHipError(f"x: shape {tuple(x.shape)}, expected [rows, {c.d_model}]")
+        if slots is not None and cache is None:
+            raise _lib.MambaHipError("slots without a cache")
         grad = self._wants_grad(x)
         if grad and cache is not None:
             raise _lib.MambaHipError(_CACHE_GRAD)

@@ -521,9 +521,9 @@ class Mamba1Layer:
         return dropout_autograd(y, self.p, rng, offset, x)
 
     def step(self, x: torch.Tensor, cache: Mamba1Cache, slots: Optional[torch.Tensor] = None):
-        """One token per row of x [b, d_model] on ``cache`` (``Mamba1.step``)."""
+        """One token per row of x [b, d_model] on ``cache`` (``Mamba1.step``); y of x's type."""
         from .norm import layer_norm
         if self.mixer._wants_grad(x, self.norm_w, self.norm_b):
             raise _lib.MambaHipError(_CACHE_GRAD)
         y, cache = self.mixer.step(layer_norm(x, self.norm_w, self.norm_b, self.eps), cache, slots)
-        return x + y, cache
+        return (x + y).to(x.dtype), cache  # without slots the block is f32 throughout

@@ -518,7 +518,7 @@ class Mamba1Layer:
         y = self.mixer.forward_packed(layer_norm_autograd(x, self.norm_w, self.norm_b, self.eps), cu_seqlens, cache, slots, max_seqlen)
         if rng is None or self.p == 0.0:
             return x + y
-        return dropout_autograd(y, self.p, rng, offset, x)
+        return dropout_autograd(y.to(x.dtype), self.p, rng, offset, x)  # autocast's products are of its own type
 
     def step(self, x: torch.Tensor, cache: Mamba1Cache, slots: Optional[torch.Tensor] = None):
         """One token per row of x [b, d_model] on ``cache`` (``Mamba1.step``); y of x's type."""

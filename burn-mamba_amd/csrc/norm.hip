@@ -420,31 +420,38 @@ __global__ __launch_bounds__(256) void ln_bwd_rows(LnParams p) {
 }
 
 // The parts in order of their number: the same sums every time.  16 threads a
-// column, four loads in flight each.
+// column, four loads in flight each; 16 columns a workgroup and turn.
 __global__ __launch_bounds__(256) void ln_dw_join(LnParams p) {
     __shared__ float red[16][17];
-    const int x = threadIdx.x & 15, q = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
-    // columns 0 .. cols - 1: dw, cols .. 2 cols - 1: db
-    const bool live = c < 2 * p.cols;
+    const int x = threadIdx.x & 15, q = threadIdx.x >> 4;
     const int64_t pitch = 2ll * p.cols;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live) {
-        const float* src = p.part + c;
-        int i = q;
-        for (; i + 48 < p.parts; i += 64) {
+    // columns 0 .. cols - 1: dw, cols .. 2 cols - 1: db
+    for (int c0 = blockIdx.x * 16; c0 < 2 * p.cols; c0 += gridDim.x * 16) {
+        const int c = c0 + x;
+        const bool live = c < 2 * p.cols;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (live) {
+            const float* src = p.part + c;
+            int i = q;
+            for (; i + 48 < p.parts; i += 64) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] += src[(i + 16 * j) * pitch];
+                for (int j = 0; j < 4; ++j) s[j] += src[(i + 16 * j) * pitch];
+            }
+            for (; i < p.parts; i += 16) s[0] += src[i * pitch];
         }
-        for (; i < p.parts; i += 16) s[0] += src[i * pitch];
+        red[q][x] = (s[0] + s[1]) + (s[2] + s[3]);
+        __syncthreads();
+        if (q == 0 && live) {
+            float a = 0.f;
+            for (int j = 0; j < 16; ++j) a += red[j][x];
+            float* out = c < p.cols ? p.dw : p.db;
+            if (out) out[c < p.cols ? c : c - p.cols] = a;
+        }
+        __syncthreads();
     }
-    red[q][x] = (s[0] + s[1]) + (s[2] + s[3]);
-    __syncthreads();
-    if (q || !live) return;
-    float a = 0.f;
-    for (int j = 0; j < 16; ++j) a += red[j][x];
-    float* out = c < p.cols ? p.dw : p.db;
-    if (out) out[c < p.cols ? c : c - p.cols] = a;
 }
+// one turn up to 2^20 workgroups (a grid of 2^32 threads, reached at 2^27 columns, is none)
+static uint32_t ln_join_grid(int cols) { return (uint32_t)std::min(ceil_div(2 * cols, 16), 1 << 20); }
 
 // workgroups of a kernel that takes a row each in turn
 static uint32_t ln_grid(int64_t rows) { return (uint32_t)std::min<int64_t>(rows, 1 << 20); }
@@ -526,7 +533,7 @@ static void ln_bwd_launch(const LnParams& p, hipStream_t s) {
         if (p.out) hipLaunchKernelGGL(ln_dx_wide<T>, dim3(ln_grid(p.rows)), dim3(256), 0, s, p);
         if (sums) hipLaunchKernelGGL(ln_dw_wide<T>, dim3(ceil_div(p.cols, 64 * kLnE<T>), p.parts), dim3(256), 0, s, p);
     }
-    if (sums) hipLaunchKernelGGL(ln_dw_join, dim3(ceil_div(2 * p.cols, 16)), dim3(256), 0, s, p);
+    if (sums) hipLaunchKernelGGL(ln_dw_join, dim3(ln_join_grid(p.cols)), dim3(256), 0, s, p);
 }
 
 }  // namespace mamba
@@ -589,7 +596,7 @@ extern "C" int mamba_layernorm_bwd(const mamba_layernorm_bwd_args* a, void* ws, 
     p.part = need ? static_cast<float*>(ws) : nullptr; p.parts = ln_parts(a->rows, a->cols, a->io_dtype == MAMBA_BF16);
     p.dw = a->dweight; p.db = a->dbias;
     if (a->rows == 0) {  // the sums of no rows: zeros
-        if (p.dw || p.db) hipLaunchKernelGGL(ln_dw_join, dim3(ceil_div(2 * p.cols, 16)), dim3(256), 0, (hipStream_t)stream, p);
+        if (p.dw || p.db) hipLaunchKernelGGL(ln_dw_join, dim3(ln_join_grid(p.cols)), dim3(256), 0, (hipStream_t)stream, p);
     } else if (a->io_dtype == MAMBA_BF16) {
         ln_bwd_launch<bf16_t>(p, (hipStream_t)stream);
     } else {

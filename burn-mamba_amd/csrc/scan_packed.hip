@@ -46,6 +46,7 @@
 // would take 32, 71, 139 and 213 us at the rate of a copy.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "pack.h"
 
@@ -843,8 +844,10 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
             rC.stage(s_C);
             __syncthreads();
             if (tl > 0) fetch(t0 - TT, b);
-#pragma unroll 1
-            for (int r0 = (n - 1) / kSub * kSub; r0 >= 0; r0 -= kSub) {
+            // kSub rows from r0.  PART: the part ends among them.  Rows behind it are steps that
+            // change nothing, but an infinite state times their gradient of 0 would not be 0.
+            auto rows = [&](int r0, auto part) __attribute__((always_inline)) {
+                constexpr bool PART = decltype(part)::value;
                 const int q = tl * (TT / kSub) + r0 / kSub;
                 float hs[kSub + 1][4], as[kSub][4];
                 // the state before row r0: the run's own start, or the kept one and what came in
@@ -865,6 +868,7 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
                 }
 #pragma unroll
                 for (int i = kSub - 1; i >= 0; --i) {
+                    if (PART && r0 + i >= n) continue;
                     const float2 dd = s_dd[r0 + i][c];
                     const float ev = s_e[r0 + i][c];
                     const float4 bq = *(const float4*)&s_B[r0 + i][4 * ng], cq = *(const float4*)&s_C[r0 + i][4 * ng];
@@ -895,7 +899,11 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
                     s_bc[wave][r0 + i][bc_at] = x0;
                     s_bc[wave][r0 + i][bc_at + 2] = x1;
                 }
-            }
+            };
+            const int whole = n / kSub * kSub;
+            if (n > whole) rows(whole, std::true_type{});
+#pragma unroll 1
+            for (int r0 = whole - kSub; r0 >= 0; r0 -= kSub) rows(r0, std::false_type{});
             __syncthreads();
             // ---- the tile's dB and dC over the workgroup, and the gradients of its elements
             for (int i = threadIdx.x; i < n * 2 * NP; i += 256) {

@@ -5,11 +5,12 @@ import pytest
 import torch
 
 import mamba_hip
-from test_packed_gpu import cu, gen, scan_inputs
+import packed_oracle as po
+from test_packed_gpu import cu, gen, oracle_args, scan_inputs
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
-NAN = float("nan")
+NAN, INF = float("nan"), float("inf")
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -69,3 +70,38 @@ def test_nan_step_of_a_token(dev, name, n):
     assert torch.equal(y.isnan(), hit) and torch.equal(y[~hit], clean[~hit])
     got, want = state[slots.long()], want[slots.long()]
     assert torch.equal(got.isnan(), hit[..., None].expand_as(got)) and torch.equal(got[~hit], want[~hit])
+
+def like(got, ref, what):
+    """The same infinities, the same places that are no number, finite elsewhere."""
+    g = po.d(got)
+    assert torch.equal(g.isnan(), ref.isnan()), (what, "nan", int(g.isnan().sum()), int(ref.isnan().sum()))
+    assert torch.equal(g == INF, ref == INF) and torch.equal(g == -INF, ref == -INF), what
+
+
+def positive(lens, d, n, dev, seed):
+    """Every input that multiplies is positive, so that infinities have one sign, and the
+    decay of a sequence stays far from 0, so that an infinite state stays one."""
+    t = scan_inputs(lens, d, n, F32, dev, seed=seed)
+    for k in ("u", "B", "C", "D", "z"):
+        t[k] = t[k].abs() + 0.1
+    t["delta"] = t["delta"].clamp(-1, 1)
+    t["delta_bias"] = t["delta_bias"].clamp(-6, -4)
+    return t
+
+
+@pytest.mark.parametrize("n", [16])
+def test_infinite_input(dev, n):
+    """An infinite u makes its channel infinite from its row on, whatever the states are padded to."""
+    lens, d = [20, 60, 9], 3
+    t = positive(lens, d, n, dev, 44)
+    t["u"][30, 1] = INF
+    dy, c = torch.ones(sum(lens), d, device=dev), cu(lens, dev)
+    ref = po.scan(lens, dy=dy, **oracle_args(t, True))
+    assert ref["y"][0].isinf().sum() == 50 and not ref["y"][0].isnan().any()
+    for most in (0, 60):
+        state = torch.zeros(3, d, n, device=dev)
+        like(mamba_hip.mamba1_scan_packed(**t, cu_seqlens=c, delta_softplus=True, state=state, max_seqlen=most), ref["y"][0], "y")
+        like(state, ref["hT"][0], "state")
+    g = mamba_hip.mamba1_scan_packed_bwd(dy, **t, cu_seqlens=c, delta_softplus=True)
+    for k in ("du", "ddelta", "dz", "dB", "dC", "dA", "dD"):
+        like(g[k], ref[k][0], k)

@@ -390,8 +390,9 @@ __global__ __launch_bounds__(64) void scan_pk_carry(ScanPk p) {
 // The outputs of a chunk (or of a whole sequence) from the state that enters it.  A
 // row's sum over the states stays inside NS lanes (DPP); it goes through LDS to the
 // element-wise mapping for D u, the gate and a wide store.  180 us at 8192 x 5120
-// bf16: 0.98 of the vector units' cycles.
-template <typename T, int NP>
+// bf16: 0.98 of the vector units' cycles.  PAD: fewer states than NP.  Those past N are
+// held at 0: their B and C are 0 already, but an infinite d or d u times 0 is not a number.
+template <typename T, int NP, bool PAD>
 __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
     constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = ScanShape<NP>::TT;
     __shared__ float2 s_dd[TT][CPB];
@@ -504,6 +505,10 @@ __global__ __launch_bounds__(256) void scan_pk_out(ScanPk p) {
                     h[1] = __builtin_fmaf(h[1], __builtin_amdgcn_exp2f(dd[i].x * A2[1]), dd[i].y * bv[i].y);
                     h[2] = __builtin_fmaf(h[2], __builtin_amdgcn_exp2f(dd[i].x * A2[2]), dd[i].y * bv[i].z);
                     h[3] = __builtin_fmaf(h[3], __builtin_amdgcn_exp2f(dd[i].x * A2[3]), dd[i].y * bv[i].w);
+                    if (PAD) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) h[k] = 4 * ng + k < p.N ? h[k] : 0.f;
+                    }
                     yq[i] = __builtin_fmaf(cv[i].w, h[3], __builtin_fmaf(cv[i].z, h[2], __builtin_fmaf(cv[i].y, h[1], cv[i].x * h[0])));
                 }
 #pragma unroll
@@ -718,8 +723,9 @@ __device__ __forceinline__ void channel_sums(const float (&v)[4], const float (&
 // The gradients of a chunk's rows, from the last to the first, kSub at a time.  587 us at
 // 8192 x 5120 bf16: 256 M wave instructions at two waves a SIMD (223 registers), 0.85
 // of the vector units' cycles; three waves (161 registers, the rows' operands read
-// from LDS again) took 4 % longer.
-template <typename T, int NP>
+// from LDS again) took 4 % longer.  PAD: fewer states than NP, those past N
+// held at 0 with their gradients, as in scan_pk_out.
+template <typename T, int NP, bool PAD>
 __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
     constexpr int NS = ScanShape<NP>::NS, CPB = ScanShape<NP>::CPB, EV = ScanShape<NP>::EV, TT = ScanShape<NP>::TT;
     __shared__ __align__(16) float2 s_dd[TT][CPB];
@@ -805,7 +811,7 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
             load_plane<NP>(p.ckh, place, p, d, ng, hn);
             if (in) dn = d < p.D ? p.ckd[(int64_t)place * p.D + d] : 0.f;
         };
-        kept((len - 1) / kSub);
+        kept(len / kSub - 1);
         for (int tl = tiles - 1; tl >= 0; --tl) {
             const int t0 = t + tl * TT;
             const int n = min(TT, b - t0);
@@ -844,66 +850,92 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
             rC.stage(s_C);
             __syncthreads();
             if (tl > 0) fetch(t0 - TT, b);
-            // kSub rows from r0.  PART: the part ends among them.  Rows behind it are steps that
-            // change nothing, but an infinite state times their gradient of 0 would not be 0.
-            auto rows = [&](int r0, auto part) __attribute__((always_inline)) {
-                constexpr bool PART = decltype(part)::value;
-                const int q = tl * (TT / kSub) + r0 / kSub;
-                float hs[kSub + 1][4], as[kSub][4];
-                // the state before row r0: the run's own start, or the kept one and what came in
+            auto held = [&](float v, int k) __attribute__((always_inline)) { return !PAD || 4 * ng + k < p.N ? v : 0.f; };
+            auto step = [&](int r, const float (&h)[4], float (&a)[4], float (&after)[4]) __attribute__((always_inline)) {
+                const float2 dd = s_dd[r][c];
+                const float4 bq = *(const float4*)&s_B[r][4 * ng];
+                const float bv[4] = {bq.x, bq.y, bq.z, bq.w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    hs[0][k] = q == 0 ? h0[k] : in ? __builtin_fmaf(__builtin_amdgcn_exp2f(dn * A2[k]), h0[k], hn[k]) : hn[k];
-                kept(q - 1);
-#pragma unroll
-                for (int i = 0; i < kSub; ++i) {
-                    const float2 dd = s_dd[r0 + i][c];
-                    const float4 bq = *(const float4*)&s_B[r0 + i][4 * ng];
-                    const float bv[4] = {bq.x, bq.y, bq.z, bq.w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        as[i][k] = __builtin_amdgcn_exp2f(dd.x * A2[k]);
-                        hs[i + 1][k] = __builtin_fmaf(hs[i][k], as[i][k], dd.y * bv[k]);
-                    }
-                }
-#pragma unroll
-                for (int i = kSub - 1; i >= 0; --i) {
-                    if (PART && r0 + i >= n) continue;
-                    const float2 dd = s_dd[r0 + i][c];
-                    const float ev = s_e[r0 + i][c];
-                    const float4 bq = *(const float4*)&s_B[r0 + i][4 * ng], cq = *(const float4*)&s_C[r0 + i][4 * ng];
-                    const float bv[4] = {bq.x, bq.y, bq.z, bq.w}, cv[4] = {cq.x, cq.y, cq.z, cq.w};
-                    float sB = 0.f, sA = 0.f, sC = 0.f, vb[4], vc[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float gk = __builtin_fmaf(cv[k], ev, g[k]);
-                        vb[k] = gk * dd.y;
-                        vc[k] = hs[i + 1][k] * ev;
-                        sB = __builtin_fmaf(gk, bv[k], sB);
-                        sC = __builtin_fmaf(cv[k], hs[i + 1][k], sC);
-                        g[k] = gk * as[i][k];
-                        const float x = g[k] * hs[i][k];
-                        sA = __builtin_fmaf(x, A2[k], sA);
-                        dA[k] = __builtin_fmaf(x, dd.x, dA[k]);
-                    }
-                    sB = group_sum_all<NS>(sB);
-                    sA = group_sum_all<NS>(sA);
-                    sC = group_sum_all<NS>(sC);
-                    float x0, x1;
-                    channel_sums<NS>(vb, vc, x0, x1);
-                    // every lane that holds a sum writes it (the same value to the same
-                    // place): a branch here would keep the rows apart in the schedule
-                    s_sB[r0 + i][c] = sB;
-                    s_sA[r0 + i][c] = sA;
-                    s_sC[r0 + i][c] = sC;
-                    s_bc[wave][r0 + i][bc_at] = x0;
-                    s_bc[wave][r0 + i][bc_at + 2] = x1;
+                for (int k = 0; k < 4; ++k) {
+                    a[k] = __builtin_amdgcn_exp2f(dd.x * A2[k]);
+                    after[k] = held(__builtin_fmaf(h[k], a[k], dd.y * bv[k]), k);
                 }
             };
+            auto back = [&](int r, const float (&h)[4], const float (&a)[4], const float (&after)[4]) __attribute__((always_inline)) {
+                const float2 dd = s_dd[r][c];
+                const float ev = s_e[r][c];
+                const float4 bq = *(const float4*)&s_B[r][4 * ng], cq = *(const float4*)&s_C[r][4 * ng];
+                const float bv[4] = {bq.x, bq.y, bq.z, bq.w}, cv[4] = {cq.x, cq.y, cq.z, cq.w};
+                float sB = 0.f, sA = 0.f, sC = 0.f, vb[4], vc[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float gk = held(__builtin_fmaf(cv[k], ev, g[k]), k);
+                    vb[k] = gk * dd.y;
+                    vc[k] = after[k] * ev;
+                    sB = __builtin_fmaf(gk, bv[k], sB);
+                    sC = __builtin_fmaf(cv[k], after[k], sC);
+                    g[k] = held(gk * a[k], k);
+                    const float x = g[k] * h[k];
+                    sA = __builtin_fmaf(x, A2[k], sA);
+                    dA[k] = __builtin_fmaf(x, dd.x, dA[k]);
+                }
+                sB = group_sum_all<NS>(sB);
+                sA = group_sum_all<NS>(sA);
+                sC = group_sum_all<NS>(sC);
+                float x0, x1;
+                channel_sums<NS>(vb, vc, x0, x1);
+                // every lane that holds a sum writes it (the same value to the same
+                // place): a branch here would keep the rows apart in the schedule
+                s_sB[r][c] = sB;
+                s_sA[r][c] = sA;
+                s_sC[r][c] = sC;
+                s_bc[wave][r][bc_at] = x0;
+                s_bc[wave][r][bc_at + 2] = x1;
+            };
             const int whole = n / kSub * kSub;
-            if (n > whole) rows(whole, std::true_type{});
+            if (n > whole) {
+                // The last rows of a part, fewer than kSub: each finds its state again from the
+                // start.  (Made up to kSub by steps that change nothing, they would add an infinite
+                // state times a gradient of 0 to dA.  Their kept state is not hn: did that come from
+                // two places, the loop below would wait for the next tile's rows before its first:
+                // 826 us for 8192 x 5120 bf16 with all kernels, 792 so.)
+                float h0r[4] = {h0[0], h0[1], h0[2], h0[3]};
+                if (len > kSub) {
+                    const int place = (t0 + whole) / kSub;
+                    const float sum = in && d < p.D ? p.ckd[(int64_t)place * p.D + d] : 0.f;
+                    load_plane<NP>(p.ckh, place, p, d, ng, h0r);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (in) h0r[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(sum * A2[k]), h0[k], h0r[k]);
+                }
+                if (PAD) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) h0r[k] = held(h0r[k], k);
+                }
 #pragma unroll 1
-            for (int r0 = whole - kSub; r0 >= 0; r0 -= kSub) rows(r0, std::false_type{});
+                for (int r = n - 1; r >= whole; --r) {
+                    float h[4], a[4], after[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) h[k] = h0r[k];
+#pragma unroll 1
+                    for (int j = whole; j < r; ++j) step(j, h, a, h);
+                    step(r, h, a, after);
+                    back(r, h, a, after);
+                }
+            }
+#pragma unroll 1
+            for (int r0 = whole - kSub; r0 >= 0; r0 -= kSub) {
+                float hs[kSub + 1][4], as[kSub][4];
+                const int q = tl * (TT / kSub) + r0 / kSub;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    hs[0][k] = held(q == 0 ? h0[k] : in ? __builtin_fmaf(__builtin_amdgcn_exp2f(dn * A2[k]), h0[k], hn[k]) : hn[k], k);
+                kept(q - 1);
+#pragma unroll
+                for (int i = 0; i < kSub; ++i) step(r0 + i, hs[i], as[i], hs[i + 1]);
+#pragma unroll
+                for (int i = kSub - 1; i >= 0; --i) back(r0 + i, hs[i], as[i], hs[i + 1]);
+            }
             __syncthreads();
             // ---- the tile's dB and dC over the workgroup, and the gradients of its elements
             for (int i = threadIdx.x; i < n * 2 * NP; i += 256) {
@@ -1242,16 +1274,20 @@ static void scan_pk_fwd_launch(const ScanPk& p, hipStream_t s) {
         hipLaunchKernelGGL((scan_pk_state<T, NP>), dim3(nblk * (uint32_t)(p.nchunk - 1)), dim3(256), 0, s, p);
         if (!p.walk) hipLaunchKernelGGL((scan_pk_carry<NP>), dim3(ceil_div(p.D * NP, 64)), dim3(64), 0, s, p);
     }
-    hipLaunchKernelGGL((scan_pk_out<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
+    const dim3 grid(nblk * (uint32_t)p.nchunk);
+    if (p.N == NP) hipLaunchKernelGGL((scan_pk_out<T, NP, false>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((scan_pk_out<T, NP, true>), grid, dim3(256), 0, s, p);
 }
 
 template <typename T, int NP>
 static void scan_pk_bwd_launch(const ScanPk& p, hipStream_t s) {
     const uint32_t nblk = ceil_div(p.D, ScanShape<NP>::CPB);
     if (p.rows) {
-        hipLaunchKernelGGL((scan_pk_state_bwd<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
+        const dim3 grid(nblk * (uint32_t)p.nchunk);
+        hipLaunchKernelGGL((scan_pk_state_bwd<T, NP>), grid, dim3(256), 0, s, p);
         if (!p.walk) hipLaunchKernelGGL((scan_pk_carry_bwd<NP>), dim3(ceil_div(p.D * NP, 64), 2), dim3(64), 0, s, p);
-        hipLaunchKernelGGL((scan_pk_bwd<T, NP>), dim3(nblk * (uint32_t)p.nchunk), dim3(256), 0, s, p);
+        if (p.N == NP) hipLaunchKernelGGL((scan_pk_bwd<T, NP, false>), grid, dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((scan_pk_bwd<T, NP, true>), grid, dim3(256), 0, s, p);
     }
     const uint32_t par = (uint32_t)(((int64_t)p.D * (NP + 2) + 63) / 64);
     hipLaunchKernelGGL((scan_pk_join<T, NP>), dim3(par + (uint32_t)((p.rows * 2 * NP + 63) / 64)), dim3(256), 0, s, p, (int)nblk, par);

@@ -89,7 +89,7 @@ def positive(lens, d, n, dev, seed):
     return t
 
 
-@pytest.mark.parametrize("n", [16])
+@pytest.mark.parametrize("n", [16, 1, 5, 12, 20, 33])
 def test_infinite_input(dev, n):
     """An infinite u makes its channel infinite from its row on, whatever the states are padded to."""
     lens, d = [20, 60, 9], 3

@@ -132,8 +132,8 @@ struct ScanShape {
 };
 
 // The element-wise mapping: row tid / (CPB / EV) of the tile, EV channels from
-// EV (tid % (CPB / EV)); with A = 0 the states of channels past D stay 0, so that
-// sums over a wave's channels need no mask.
+// EV (tid % (CPB / EV)); with A, u and e = 0 the states of channels past D stay 0
+// (and B and C, in scan_pk_bwd), so that sums over a wave's channels need no mask.
 template <int NP>
 struct ElemMap {
     int row, ch;
@@ -731,8 +731,7 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
     __shared__ __align__(16) float2 s_dd[TT][CPB];
     __shared__ __align__(16) float s_e[TT][CPB];
     __shared__ __align__(16) float s_sB[TT][CPB], s_sA[TT][CPB], s_sC[TT][CPB];
-    __shared__ __align__(16) float s_B[TT][NP];
-    __shared__ __align__(16) float s_C[TT][NP];
+    __shared__ __align__(16) float s_BC[4][TT][NP];  // B, C, and zeros twice
     __shared__ __align__(16) float s_bc[4][TT][2 * NP];
     const int nblk = (p.D + CPB - 1) / CPB;
     const int ck = (int)(blockIdx.x / (uint32_t)nblk);
@@ -744,6 +743,10 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int c = threadIdx.x / NS, ng = threadIdx.x % NS, d = d0 + c;
     const int nc = p.D - (d0 + m.ch);
+    // Channels past D read zeros for B and C: an infinite one times their d u or e of 0 is not a
+    // number, and dB and dC are sums over a wave's channels.
+    const float (*const BC)[TT][NP] = s_BC + (d < p.D ? 0 : 2);
+    for (int i = threadIdx.x; i < 2 * TT * NP; i += 256) (&s_BC[2][0][0])[i] = 0.f;
     // where this lane's channel sums go: element lane / 16 % 2 (and + 2) of B's (C's) four states
     const int bc_at = (lane >> 5) * NP + 4 * ng + ((lane >> 4) & 1);
     float A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f};
@@ -846,14 +849,14 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
                 s_dd[m.row][m.ch + k] = make_float2(dt[k], dt[k] * uv[k]);
                 s_e[m.row][m.ch + k] = ev[k];
             }
-            rB.stage(s_B);
-            rC.stage(s_C);
+            rB.stage(s_BC[0]);
+            rC.stage(s_BC[1]);
             __syncthreads();
             if (tl > 0) fetch(t0 - TT, b);
             auto held = [&](float v, int k) __attribute__((always_inline)) { return !PAD || 4 * ng + k < p.N ? v : 0.f; };
             auto step = [&](int r, const float (&h)[4], float (&a)[4], float (&after)[4]) __attribute__((always_inline)) {
                 const float2 dd = s_dd[r][c];
-                const float4 bq = *(const float4*)&s_B[r][4 * ng];
+                const float4 bq = *(const float4*)&BC[0][r][4 * ng];
                 const float bv[4] = {bq.x, bq.y, bq.z, bq.w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -864,7 +867,7 @@ __global__ __launch_bounds__(256) void scan_pk_bwd(ScanPk p) {
             auto back = [&](int r, const float (&h)[4], const float (&a)[4], const float (&after)[4]) __attribute__((always_inline)) {
                 const float2 dd = s_dd[r][c];
                 const float ev = s_e[r][c];
-                const float4 bq = *(const float4*)&s_B[r][4 * ng], cq = *(const float4*)&s_C[r][4 * ng];
+                const float4 bq = *(const float4*)&BC[0][r][4 * ng], cq = *(const float4*)&BC[1][r][4 * ng];
                 const float bv[4] = {bq.x, bq.y, bq.z, bq.w}, cv[4] = {cq.x, cq.y, cq.z, cq.w};
                 float sB = 0.f, sA = 0.f, sC = 0.f, vb[4], vc[4];
 #pragma unroll

@@ -105,3 +105,18 @@ def test_infinite_input(dev, n):
     g = mamba_hip.mamba1_scan_packed_bwd(dy, **t, cu_seqlens=c, delta_softplus=True)
     for k in ("du", "ddelta", "dz", "dB", "dC", "dA", "dD"):
         like(g[k], ref[k][0], k)
+
+@pytest.mark.parametrize("name,n", [("B", 16), ("C", 16), ("B", 12), ("C", 64), ("C", 5)])
+def test_infinite_projection(dev, name, n):
+    """An infinite B or C: the channels that the last workgroup is padded with add nothing to
+    dB and dC."""
+    lens, d = [20, 60, 9], 3
+    t = positive(lens, d, n, dev, 45)
+    t[name][30, n - 1] = INF
+    dy, c = torch.ones(sum(lens), d, device=dev), cu(lens, dev)
+    ref = po.scan(lens, dy=dy, **oracle_args(t, True))
+    assert ref["dC" if name == "B" else "dB"][0].isinf().any()
+    like(mamba_hip.mamba1_scan_packed(**t, cu_seqlens=c, delta_softplus=True), ref["y"][0], "y")
+    g = mamba_hip.mamba1_scan_packed_bwd(dy, **t, cu_seqlens=c, delta_softplus=True)
+    for k in ("du", "ddelta", "dz", "dB", "dC", "dA", "dD"):
+        like(g[k], ref[k][0], k)

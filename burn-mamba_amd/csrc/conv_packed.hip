@@ -40,9 +40,10 @@ __device__ __forceinline__ float conv_sigmoid(float v) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
 }
 
-// KT = K as a constant, or 0: any K up to kMaxTaps, the taps in a ring in scratch
-// memory that is shifted by one each row all the same (16384 x 5120 bf16: forward
-// 75 us with K = 7 as a constant, 1074 without; backward 137, 3276).
+// KT = K as a constant, or 0: any K up to kMaxTaps (and fewer than 4 channels), the taps in
+// scratch memory, because registers cannot be indexed by a tap that the compiler does not know,
+// and shifted by one each row (16384 x 5120 bf16: forward 75 us with K = 7 as a
+// constant, 1074 without; backward 137, 3276).
 constexpr int kMaxTaps = 64;
 constexpr int kConvRows = 4;  // rows whose loads are in flight while four others are computed
 
@@ -404,9 +405,13 @@ static int conv_pk_make(const mamba_conv1d_packed_args* a, bool back, ConvPk* o)
     // Rows of a chunk, and at most 2^20 items of 64 channels, which keeps the grid small.
     // Forward: four waves a SIMD where the rows are enough for it; 8 to 64 (long chunks
     // read fewer rows twice at their edges; 16384 x 5120 60 us with 64, 70 with 32).
-    // Backward: rounds of three waves a SIMD, which is what its registers allow, of at
-    // most 128 rows, so that the last round is a whole one (16384 x 5120 bf16 with the
-    // join: 108 rows, one round, 126 us; 64 rows, 1.7 rounds, 136; 36 rows, 3 rounds, 145).
+    // Backward: rounds of three waves a SIMD, of at most 128 rows, so that the last round is a
+    // whole one (16384 x 5120 bf16, 4 taps, with the join: 108 rows, one round, 126 us; 64
+    // rows, 1.7 rounds, 136; 36 rows, 3 rounds, 145).  Three is what the registers of bf16 with
+    // 4 taps (136) and of f32 with 2, 3 and 8 allow; bf16 with 2, 3, 7 and 8 and f32 with 5 to 7
+    // have room for four, bf16 with 5 and 6 for five, f32 with 4 (178 registers) for two.  us at
+    // 16384 x 5120 with the join: bf16 2, 3, 4, 6, 8 taps 112, 112, 115, 132, 136; f32 208,
+    // 210, 228, 219, 227 (4.8 to 4.4 TB/s).
     if (back) {
         const int64_t fill = std::max<int64_t>(1, a->rows * ceil_div(p.C, 256) / (3 * 1024)), rounds = (fill + 127) / 128;
         p.chunk = std::max<int64_t>(8, (fill / rounds + 4) / 4 * 4);

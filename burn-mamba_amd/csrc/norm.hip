@@ -8,8 +8,8 @@
 // difference of two large sums.
 //
 // About ten operations an element against two elements moved (forward) or three
-// (backward): HBM-bound.  Rows of up to 10240 elements stay in registers (each
-// element is read once): G lanes hold a row, 8 (bf16) or 4 (f32) consecutive
+// (backward): HBM-bound.  Rows of up to 10240 bf16 or 5120 f32 elements stay in
+// registers (each element is read once): G lanes hold a row, 8 (bf16) or 4 (f32) consecutive
 // elements a lane and step, G = 16, 64 or 256 by the row's width.  The backward's
 // workgroups take rows in turn and sum dw and db of their columns in registers,
 // joined in LDS and, over the workgroups, by ln_dw_join, in a fixed order.
@@ -481,8 +481,7 @@ static int ln_parts(int64_t rows, int cols, bool bf16) {
     return (int)std::min<int64_t>(cols > 256 ? 512 : 1024, (rows + 8 * (256 / G) - 1) / (8 * (256 / G)));
 }
 
-// rows x cols with these row strides: rows overlap nowhere and every element
-// offset fits 63 bits
+// rows of cols elements with this row stride overlap nowhere
 static bool ln_rows_ok(int64_t rows, int cols, int64_t sr) {
     return sr >= cols || rows <= 1;
 }

@@ -41,8 +41,8 @@
 //
 // Measured at 8192 rows x 5120 channels, 16 states, bf16, six sequences (us, then
 // the share of cycles that the vector units issue in; HBM moves what each reads and
-// writes in a fraction of its time): state pass 113, all of them; out 180, 0.98;
-// backward state pass 209, all; backward 587, 0.85; the join 20.6.  Their bytes alone
+// writes in a fraction of its time): state pass 114, all of them; out 183, 0.98;
+// backward state pass 212, all; backward 596, 0.85; the join 20.6.  Their bytes alone
 // would take 32, 71, 139 and 213 us at the rate of a copy.
 #include <algorithm>
 #include <cmath>
@@ -263,7 +263,7 @@ __device__ __forceinline__ void load_carry(float* X, int from, int to, const Sca
 
 // The state that chunk ck leaves to the next, from zero or from its last sequence's own
 // start, and the sum of d.  Four rows' operands are read from LDS before the four
-// dependent steps.  113 us at 8192 x 5120 bf16: 52 M wave instructions, of which 10.5 M
+// dependent steps.  114 us at 8192 x 5120 bf16: 52 M wave instructions, of which 10.5 M
 // exps at about four times a multiply's time, leave the vector units no idle cycle.
 template <typename T, int NP>
 __global__ __launch_bounds__(256) void scan_pk_state(ScanPk p) {
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(64) void scan_pk_carry(ScanPk p) {
 
 // The outputs of a chunk (or of a whole sequence) from the state that enters it.  A
 // row's sum over the states stays inside NS lanes (DPP); it goes through LDS to the
-// element-wise mapping for D u, the gate and a wide store.  180 us at 8192 x 5120
+// element-wise mapping for D u, the gate and a wide store.  183 us at 8192 x 5120
 // bf16: 0.98 of the vector units' cycles.  PAD: fewer states than NP.  Those past N are
 // held at 0: their B and C are 0 already, but an infinite d or d u times 0 is not a number.
 template <typename T, int NP, bool PAD>
@@ -544,7 +544,7 @@ constexpr int kSub = 8;  // rows whose states and decays wait in registers
 // sequence's part (from zero where the sequence came in, with the sum of d up to
 // there: scan_pk_bwd adds what came in).  Row a + kSub i, i >= 1, of a part that
 // begins at a is kept at place (a + kSub i) / kSub: no two parts share one.
-// 209 us at 8192 x 5120 bf16, the vector units busy throughout; 357 MB written, 8 rows'
+// 212 us at 8192 x 5120 bf16, the vector units busy throughout; 357 MB written, 8 rows'
 // states apart (every 4th row's would be 690 MB, every 16th's would not fit the
 // registers of scan_pk_bwd).
 template <typename T, int NP>
@@ -720,8 +720,8 @@ __device__ __forceinline__ void channel_sums(const float (&v)[4], const float (&
     }
 }
 
-// The gradients of a chunk's rows, from the last to the first, kSub at a time.  587 us at
-// 8192 x 5120 bf16: 256 M wave instructions at two waves a SIMD (223 registers), 0.85
+// The gradients of a chunk's rows, from the last to the first, kSub at a time.  596 us at
+// 8192 x 5120 bf16: 256 M wave instructions at two waves a SIMD (230 registers), 0.85
 // of the vector units' cycles; three waves (161 registers, the rows' operands read
 // from LDS again) took 4 % longer.  PAD: fewer states than NP, those past N
 // held at 0 with their gradients, as in scan_pk_out.
@@ -1248,10 +1248,13 @@ constexpr int64_t kMaxGroups = 1ll << 24;  // a grid's threads stay below 2^32
 // Whole sequences, a workgroup of CPB channels each, where the longest is known to
 // be short beside all the rows' work: its rows take some 0.15 us one behind the
 // other, and in chunks most rows are scanned twice.  Up to 96 rows in any case: the
-// chunks' second launch and workspace cost a call as much as they save.  us, forward, whole /
-// in chunks: 8 sequences of 2048 x 5120 466 / 558, 4 of them 352 / 285, 16 of 512 190 /
-// 259, 16 of 256 x 2560 64 / 91, 8 of 512 95 / 95, 16 of 128 x 1024 23 / 31, 8 of them
-// 22 / 21, one of 77 x 512 15 / 13, of 40 10 / 12.
+// chunks' second launch and workspace cost a call more than they save: one call among
+// others takes 13 us whole and 17 in chunks to 64 rows, 16.5 and 17.3 at 96.  (Its time on the
+// GPU alone, which a captured graph has, turns at some 48 rows: 9.1 and 9.5 us at 40 x 512,
+// 13.8 and 10.3 at 77, 16.2 and 10.5 at 96 x 2560; a caller that knows no bound gets chunks.)
+// Longer ones, whole / in chunks: 8 sequences of 2048 x 5120 466 / 558, 4 of them 352 /
+// 285, 16 of 512 190 / 259, 16 of 256 x 2560 64 / 91, 8 of 512 95 / 95, 16 of 128 x 1024
+// 23 / 31, 8 of them 22 / 21.
 static void scan_pk_fwd_plan(ScanPk& p, int max_seqlen) {
     scan_pk_plan(p);
     const int64_t nblk = ceil_div(p.D, 1024 / scan_np(p.N));

@@ -339,7 +339,12 @@ def _decay(a_log: torch.Tensor) -> torch.Tensor:
 @dataclass
 class Mamba1:
     """Mamba1 block, forward and step (parameters of src/mamba1/mamba1.rs:124-227);
-    Linear weights in Burn's [d_in, d_out] layout."""
+    Linear weights in Burn's [d_in, d_out] layout.
+
+    Calls without gradients keep what they derive from the weights (A, bf16 and transposed
+    copies) and make it again, where it lies, when a weight has changed.  A HIP graph of such
+    calls is captured after one call outside it, and its replays follow an update of the
+    weights from the next call outside it on."""
     cfg: Mamba1Config
     in_proj_w: torch.Tensor      # [d_model, 2 d_inner]
     conv_w: torch.Tensor         # [d_inner, K]
@@ -356,6 +361,7 @@ class Mamba1:
 
     @property
     def A(self) -> torch.Tensor:
+        """-exp(a_log), one tensor whose values follow the parameter's."""
         return _decay(self.a_log)
 
     def _wants_grad(self, *ts: Optional[torch.Tensor]) -> bool:
@@ -422,7 +428,7 @@ class Mamba1:
                        slots: Optional[torch.Tensor] = None, max_seqlen: int = 0) -> torch.Tensor:
         """Mamba1::forward over packed sequences of different lengths (mamba_hip.packed):
         x [rows, d_model] f32 or bf16 -> y [rows, d_model], zero on rows outside the
-        sequences (but for a projection's bias).  With a ``cache`` (rows by ``slots``) the
+        sequences.  With a ``cache`` (rows by ``slots``) the
         sequences go on from it and it is updated in place, which autograd does not
         follow; without one they start from zero and the call is differentiable, in x
         and in every parameter that requires it."""

@@ -314,7 +314,8 @@ def mamba1_scan_packed_bwd(dy, u, delta, A, B, C, cu_seqlens, D=None, z=None, de
     ``initial_state`` and ``d_final_state`` [sequences, d, n] f32 or None.  Returns
     dict(du, ddelta, dz, dB, dC of their tensors' type, zero outside the sequences; dA,
     dD, d_delta_bias, d_initial_state f32; None for what was not given).  The same inputs
-    give the same bits."""
+    give the same bits.  While it runs it takes rows / 8 states, d x n f32 each (n as 8, 16, 32
+    or 64), and some: 0.5 GB at 8192 x 5120 x 16."""
     a = Mamba1ScanPackedBwdArgs()
     a.fwd = _scan_args(u, delta, A, B, C, cu_seqlens, D, z, delta_bias, delta_softplus, max_seqlen)
     d, n, s = A.shape[0], A.shape[1], cu_seqlens.numel() - 1

@@ -858,7 +858,8 @@ int mamba2_gated_rmsnorm(const mamba2_gated_norm_args* args, mamba_stream_t stre
 /* is no state: the sequence starts from zero and keeps nothing.  The slots of */
 /* one call are distinct.  Rows are strided (less than 2^25 elements apart in  */
 /* the scan), their last axis contiguous.  Outputs share no memory with inputs */
-/* but where a call says so; an output that does is refused.                   */
+/* but where a call says so; output rows that overlap an input's rows are      */
+/* refused.                                                                    */
 /* ------------------------------------------------------------------------- */
 
 /* Depthwise causal convolution + SiLU (layer 2 of Mamba1::forward,            */
@@ -941,7 +942,10 @@ int mamba1_scan_packed_fwd(const mamba1_scan_packed_args* args, void* workspace,
 /* n] or NULL (zero).  du, ddelta, dz, dB and dC are of io_dtype, zero outside */
 /* the sequences; dD, d_delta_bias and d_initial_state may be NULL, and        */
 /* d_initial_state's rows of empty sequences are left as they were.  Sums are  */
-/* taken in a fixed order: the same inputs give the same bits.                 */
+/* taken in a fixed order: the same inputs give the same bits.  The workspace  */
+/* holds the state at every 8th row, rows/8 x d x n' floats with n padded to   */
+/* n' = 8, 16, 32 or 64, and ceil(d n'/1024) x rows x 2n' of partial dB and dC: */
+/* 336 and 84 MB at 8192 x 5120 x 16, eight times as much at 65536 rows.       */
 typedef struct mamba1_scan_packed_bwd_args {
     mamba1_scan_packed_args fwd;
     const float* initial_state;

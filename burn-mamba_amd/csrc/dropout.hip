@@ -67,8 +67,8 @@ __global__ __launch_bounds__(256) void dropout_any(DropoutParams p) {
 // (bf16) or 4 (f32) elements, 16 bytes, a thread and turn, two turns' loads in
 // flight.  The generator takes about 30 32-bit operations an element (a 32 x 32
 // -> 64 product counts four), which bf16's 4 to 6 bytes an element only just
-// cover: HBM-bound, with little to spare.  16384 x 2560 bf16: 49 us with a residual (252
-// MB, 5.2 TB/s), 37 without (168 MB, 4.5 TB/s, the vector units issuing 0.87 of the time).
+// cover: HBM-bound, with little to spare.  16384 x 2560 bf16: 51 us with a residual (252
+// MB, 4.9 TB/s), 38 without (168 MB, 4.5 TB/s, the vector units issuing 0.86 of the time).
 template <typename T, int V, bool RES>
 __global__ __launch_bounds__(256) void dropout_vec(DropoutParams p) {
     const int64_t n = p.rows * p.cols, units = (n + V - 1) / V, per = (p.cols + V - 1) / V;

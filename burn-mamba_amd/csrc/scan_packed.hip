@@ -26,8 +26,8 @@
 // Backward: scan_pk_state_bwd finds both carries of a chunk on one set of exps
 // (the gradient of the state that enters it is sum_t P_t C_t e_t, P_t the product
 // of the decays up to row t, so it walks forwards too) and keeps the state at
-// every 8th row; scan_pk_bwd then takes 8 rows at a time from the last to the
-// first, finds their states and decays again in registers and walks back over
+// every 8th row; scan_pk_bwd then takes 8 rows at a time from the last (fewer than 8
+// at a part's end one by one) to the first, finds their states and decays again in registers and walks back over
 // them.  dB and dC are sums over channels: over a wave's by lane exchanges, over
 // the workgroup's in LDS, over the workgroups in scan_pk_join; every sum is in a
 // fixed order.

@@ -306,7 +306,8 @@ def _derived(w: torch.Tensor, attr: str, make):
     The new values go where the old ones were, behind everything that is launched on
     the device: a captured graph holds the copy's address, and its replays read the weight's
     values of the last call outside a graph.  (Not so a copy that autograd follows, or one
-    that is the weight's own memory, seen in another order.)"""
+    that is the weight's own memory, seen in another order.)  A backward whose forward read
+    the older values is refused by autograd, as for any tensor changed in place."""
     key = _weight_key(w)
     hit = getattr(w, attr, None)
     if not isinstance(hit, _Copy) or hit.of() is not w:

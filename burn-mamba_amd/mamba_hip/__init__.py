@@ -25,4 +25,7 @@ from .mamba3 import fused_args as mamba3_fused_args, fused_supported as mamba3_f
 from .mamba3 import fused_run as mamba3_fused_run, ssd_fused_fwd as mamba3_ssd_fused_fwd  # noqa: F401
 from .packed import (conv1d_packed, conv1d_packed_autograd, conv1d_packed_bwd, conv1d_step_slots,  # noqa: F401
                      mamba1_scan_packed, mamba1_scan_packed_autograd, mamba1_scan_packed_bwd, scan_step_slots)
+from .packed import (gated_scan_packed, gated_scan_packed_autograd, gated_scan_packed_bwd, gated_step_slots)  # noqa: F401
+from .norm import add_rms_norm, add_rms_norm_autograd, add_rms_norm_bwd, add_rms_norm_q8  # noqa: F401
+from .quant import PackedQ4, linear_q4, pack_linear_q4, quantize_q4  # noqa: F401
 from .norm import (dropout, dropout_autograd, layer_norm, layer_norm_autograd, layer_norm_bwd)  # noqa: F401

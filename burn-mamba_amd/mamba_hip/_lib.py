@@ -17,6 +17,8 @@ LIB_PATH = os.path.join(_HERE, "..", "lib", "libmamba_hip.so")
 
 MAMBA_F32 = 0
 MAMBA_BF16 = 1
+MAMBA_INT8 = 2
+MAMBA_E4M3 = 3
 
 c_i32 = ctypes.c_int32
 c_i64 = ctypes.c_int64
@@ -406,6 +408,96 @@ class DropoutArgs(ctypes.Structure):
     ]
 
 
+class GatedScanArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64),
+        ("nseq", c_i32), ("dim", c_i32), ("io_dtype", c_i32), ("fill_outside", c_i32),
+        ("cu_seqlens", c_vp),
+        ("x", c_vp), ("x_st", c_i64),
+        ("r", c_vp), ("r_st", c_i64),
+        ("i", c_vp), ("i_st", c_i64),
+        ("z", c_vp), ("z_st", c_i64),
+        ("A", c_vp),
+        ("state", c_vp), ("nslots", c_i64), ("slots", c_vp),
+        ("carry", c_vp),
+        ("y", c_vp), ("y_st", c_i64),
+    ]
+
+
+class GatedScanBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("fwd", GatedScanArgs),
+        ("initial_state", c_vp),
+        ("dy", c_vp), ("dy_st", c_i64),
+        ("d_final_state", c_vp),
+        ("dx", c_vp), ("dx_st", c_i64),
+        ("dr", c_vp), ("dr_st", c_i64),
+        ("di", c_vp), ("di_st", c_i64),
+        ("dz", c_vp), ("dz_st", c_i64),
+        ("dA", c_vp), ("d_initial_state", c_vp),
+    ]
+
+
+class GatedStepSlotsArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_i32), ("dim", c_i32), ("io_dtype", c_i32),
+        ("x", c_vp), ("x_sb", c_i64),
+        ("r", c_vp), ("r_sb", c_i64),
+        ("i", c_vp), ("i_sb", c_i64),
+        ("z", c_vp), ("z_sb", c_i64),
+        ("A", c_vp),
+        ("state", c_vp), ("nslots", c_i64), ("slots", c_vp),
+        ("y", c_vp), ("y_sb", c_i64),
+    ]
+
+
+class AddRmsNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64), ("cols", c_i32), ("io_dtype", c_i32), ("stream_dtype", c_i32), ("q_dtype", c_i32),
+        ("eps", ctypes.c_float),
+        ("x", c_vp), ("x_sr", c_i64),
+        ("residual", c_vp), ("residual_sr", c_i64),
+        ("weight", c_vp),
+        ("s", c_vp), ("s_sr", c_i64),
+        ("y", c_vp), ("y_sr", c_i64),
+        ("rstd", c_vp),
+        ("q", c_vp), ("q_sr", c_i64),
+        ("scale", c_vp),
+    ]
+
+
+class AddRmsNormBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_i64), ("cols", c_i32), ("io_dtype", c_i32), ("stream_dtype", c_i32),
+        ("s", c_vp), ("s_sr", c_i64),
+        ("dy", c_vp), ("dy_sr", c_i64),
+        ("ds", c_vp), ("ds_sr", c_i64),
+        ("weight", c_vp), ("rstd", c_vp),
+        ("dx", c_vp), ("dx_sr", c_i64),
+        ("dresidual", c_vp), ("dresidual_sr", c_i64),
+        ("dweight", c_vp),
+    ]
+
+
+class Q4Weight(ctypes.Structure):
+    _fields_ = [
+        ("d_in", c_i32), ("d_out", c_i32), ("group", c_i32), ("scale_dtype", c_i32),
+        ("has_zero", c_i32),
+        ("packed", c_vp),
+    ]
+
+
+class LinearQ4Args(ctypes.Structure):
+    _fields_ = [
+        ("w", Q4Weight),
+        ("rows", c_i64),
+        ("x_dtype", c_i32), ("y_dtype", c_i32),
+        ("x", c_vp), ("x_ld", c_i64),
+        ("x_scale", c_vp), ("bias", c_vp),
+        ("y", c_vp), ("y_ld", c_i64),
+    ]
+
+
 # name -> (argtypes, restype); the exported symbol set of include/mamba_hip.h
 _SIGNATURES = {
     "mamba_last_error": ([], ctypes.c_char_p),
@@ -486,6 +578,18 @@ _SIGNATURES = {
     "mamba_layernorm_bwd_workspace_size": ([ctypes.POINTER(LayerNormBwdArgs)], ctypes.c_size_t),
     "mamba_layernorm_bwd": ([ctypes.POINTER(LayerNormBwdArgs), c_vp, ctypes.c_size_t, c_vp], ctypes.c_int),
     "mamba_dropout": ([ctypes.POINTER(DropoutArgs), c_vp], ctypes.c_int),
+    "mamba_gated_scan_workspace_size": ([ctypes.POINTER(GatedScanArgs)], ctypes.c_size_t),
+    "mamba_gated_scan_fwd": ([ctypes.POINTER(GatedScanArgs), c_vp, ctypes.c_size_t, c_vp], ctypes.c_int),
+    "mamba_gated_scan_bwd_workspace_size": ([ctypes.POINTER(GatedScanBwdArgs)], ctypes.c_size_t),
+    "mamba_gated_scan_bwd": ([ctypes.POINTER(GatedScanBwdArgs), c_vp, ctypes.c_size_t, c_vp], ctypes.c_int),
+    "mamba_gated_step_slots": ([ctypes.POINTER(GatedStepSlotsArgs), c_vp], ctypes.c_int),
+    "mamba_add_rmsnorm_fwd": ([ctypes.POINTER(AddRmsNormArgs), c_vp], ctypes.c_int),
+    "mamba_add_rmsnorm_bwd_workspace_size": ([ctypes.POINTER(AddRmsNormBwdArgs)], ctypes.c_size_t),
+    "mamba_add_rmsnorm_bwd": ([ctypes.POINTER(AddRmsNormBwdArgs), c_vp, ctypes.c_size_t, c_vp], ctypes.c_int),
+    "mamba_linear_q4_packed_size": ([ctypes.POINTER(Q4Weight)], ctypes.c_size_t),
+    "mamba_linear_q4_pack": ([ctypes.POINTER(Q4Weight), c_vp, c_vp, c_vp, c_vp, c_vp], ctypes.c_int),
+    "mamba_linear_q4_workspace_size": ([ctypes.POINTER(LinearQ4Args)], ctypes.c_size_t),
+    "mamba_linear_q4_fwd": ([ctypes.POINTER(LinearQ4Args), c_vp, ctypes.c_size_t, c_vp], ctypes.c_int),
 }
 
 _lib = None

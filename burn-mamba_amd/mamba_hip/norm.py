@@ -1,7 +1,8 @@
-"""Layer norm and dropout for training a residual stack.
+"""Layer norm, RMS norm with the residual's addition, and dropout for a residual stack.
 
 ``layer_norm`` stands beside the reference's RmsNorm (src/modules/norm/rms_norm.rs;
-``rmsnorm``) for stacks that centre their rows, with its gradients; ``dropout`` (with
+``rmsnorm``) for stacks that centre their rows, with its gradients; ``add_rms_norm`` is that norm with the
+sum before it, its gradients, and rows of 8 bits for the product behind it; ``dropout`` (with
 the residual sum of src/modules/layer.rs:224-232) computes its mask where it is used.
 """
 
@@ -13,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import DropoutArgs, LayerNormArgs, LayerNormBwdArgs, check
+from ._lib import AddRmsNormArgs, AddRmsNormBwdArgs, DropoutArgs, LayerNormArgs, LayerNormBwdArgs, check
 from .packed import _IO, _fail, _need, _new, _once, _one_device, _p, _param, _raw_stream
 from .ssd import _dtype_code, workspace
 
@@ -124,6 +125,151 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm_autograd(x, weight, bias=None, eps: float = 1e-5) -> torch.Tensor:
     """``layer_norm`` as a differentiable op: gradients of x, weight and bias."""
     return _LayerNorm.apply(x, weight, bias, eps)
+
+
+def _stream_rows(x, m, residual, residual_out):
+    """The stream's rows of ``add_rms_norm``: (residual's rows, s, s's rows), None without one."""
+    if residual is None:
+        _need(residual_out is None, "residual_out without a residual")
+        return None, None, None
+    _need(residual.shape == x.shape, "residual must match x")
+    _need(residual.dtype == torch.float32 or residual.dtype == x.dtype, "residual must be float32 or of x's type")
+    return _matrix(residual, "residual"), *_into(residual_out, residual)
+
+
+def _arn_args(x, m, weight, residual, eps, residual_out, rstd):
+    """The arguments of operands on one device, and s."""
+    rows, cols = m.shape
+    _param(weight, "weight", cols)
+    _param(rstd, "rstd", rows)
+    _need(eps >= 0, "eps must be >= 0")
+    res, s, sm = _stream_rows(x, m, residual, residual_out)
+    a = AddRmsNormArgs()
+    a.rows, a.cols, a.io_dtype, a.eps = rows, cols, _dtype_code(m), float(eps)
+    a.x, a.x_sr, a.weight, a.rstd = m.data_ptr(), m.stride(0), _p(weight), _p(rstd)
+    if res is None:
+        a.stream_dtype = a.io_dtype
+        return a, x, m
+    a.stream_dtype = _dtype_code(res)
+    a.residual, a.residual_sr, a.s, a.s_sr = res.data_ptr(), res.stride(0), sm.data_ptr(), sm.stride(0)
+    return a, s, res
+
+
+def add_rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                 out: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None,
+                 rstd: Optional[torch.Tensor] = None) -> tuple:
+    """s = residual + x and y = s / sqrt(mean(s^2) + eps) * weight over the last axis: (y of x's
+    type, s of residual's).  x f32 or bf16, residual float32 or of x's type (None: s is x
+    itself), weight [cols] f32 or None.  ``residual_out`` may be residual itself; ``rstd``, a
+    value per row in f32, takes 1 / sqrt(mean(s^2) + eps) for ``add_rms_norm_bwd``."""
+    m = _matrix(x, "x")
+    with _one_device(m, weight, residual, out, residual_out, rstd):
+        a, s, _held = _arn_args(x, m, weight, residual, eps, residual_out, rstd)
+        out, o = _into(out, x)
+        a.y, a.y_sr = o.data_ptr(), o.stride(0)
+        check(_lib.lib().mamba_add_rmsnorm_fwd(ctypes.byref(a), _raw_stream(x)), "mamba_add_rmsnorm_fwd")
+    return out, s
+
+
+_Q8 = {torch.int8: _lib.MAMBA_INT8, torch.float8_e4m3fn: _lib.MAMBA_E4M3}
+
+
+def add_rms_norm_q8(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                    dtype: torch.dtype = torch.int8, out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
+                    residual_out: Optional[torch.Tensor] = None) -> tuple:
+    """``add_rms_norm`` into rows of 8 bits: (q, scale, s) with y = q * scale, q int8 or
+    float8_e4m3fn of x's shape and scale [rows] f32 (rows of the last axis) = max |y| / 127 or
+    / 448.  A row whose largest |y| is below 2^-100 has scale 0 and zeros, one with a NaN or an
+    infinity in y a NaN for its scale and zeros.  Gradients do not pass it."""
+    m = _matrix(x, "x")
+    if dtype not in _Q8:
+        _fail(f"dtype {dtype}, expected int8 or float8_e4m3fn")
+    _need(out is None or (out.shape == x.shape and out.dtype == dtype and out.is_contiguous()), "out must be contiguous, of x's shape and dtype")
+    _param(scale, "scale", m.shape[0])
+    _need(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual))),
+          "rows of 8 bits are not differentiable: call under torch.no_grad()")
+    with _one_device(m, weight, residual, out, scale, residual_out):
+        a, s, _held = _arn_args(x, m, weight, residual, eps, residual_out, None)
+        if out is None:
+            out = torch.empty(x.shape, dtype=dtype, device=x.device)
+        if scale is None:
+            scale = m.new_empty(m.shape[0], dtype=torch.float32)
+        a.q_dtype, a.q, a.q_sr, a.scale = _Q8[dtype], out.data_ptr(), m.shape[1], scale.data_ptr()
+        check(_lib.lib().mamba_add_rmsnorm_fwd(ctypes.byref(a), _raw_stream(x)), "mamba_add_rmsnorm_fwd")
+    return out, scale, s
+
+
+def add_rms_norm_bwd(dy: torch.Tensor, s: torch.Tensor, weight: Optional[torch.Tensor], rstd: torch.Tensor,
+                     ds: Optional[torch.Tensor] = None) -> dict:
+    """Gradients of ``add_rms_norm`` from s as it returned it, its rstd, dy and (of s, where it
+    was used) ds: dict(dx of dy's type, dresidual of s's, dweight [cols] f32).  Of one type dx
+    and dresidual are one tensor.  The same inputs give the same bits."""
+    m, g = _matrix(s, "s"), _matrix(dy, "dy")
+    _need(g.shape == m.shape, "dy must match s")
+    _need(s.dtype == torch.float32 or s.dtype == dy.dtype, "s must be float32 or of dy's type")
+    _need(ds is None or (ds.shape == s.shape and ds.dtype == s.dtype), "ds must match s")
+    _param(weight, "weight", m.shape[1])
+    _need(rstd is not None, "rstd is required")
+    _param(rstd, "rstd", m.shape[0])
+    with _one_device(m, g, weight, rstd, ds):
+        dx, dresidual, dweight = _arn_bwd(dy, g, s, m, weight, rstd, ds, True, True)
+    return dict(dx=dx, dresidual=dresidual, dweight=dweight)
+
+
+def _arn_bwd(dy, g, s, m, weight, rstd, ds, want_dx, want_dres):
+    """``add_rms_norm_bwd`` after its checks (g, m: the rows of dy and s)."""
+    a = AddRmsNormBwdArgs()
+    a.rows, a.cols = m.shape
+    a.io_dtype, a.stream_dtype = _dtype_code(g), _dtype_code(m)
+    a.s, a.s_sr, a.dy, a.dy_sr, a.weight, a.rstd = m.data_ptr(), m.stride(0), g.data_ptr(), g.stride(0), _p(weight), rstd.data_ptr()
+    d = None if ds is None else _matrix(ds, "ds")
+    if d is not None:
+        a.ds, a.ds_sr = d.data_ptr(), d.stride(0)
+    one = s.dtype == dy.dtype
+    dres = _new(s) if want_dres or (one and want_dx) else None
+    dx = dres if one else _new(dy) if want_dx else None
+    dweight = m.new_empty(m.shape[1], dtype=torch.float32) if weight is None else _new(weight)
+    if dres is not None:
+        a.dresidual, a.dresidual_sr = dres.data_ptr(), a.cols
+    if dx is not None and not one:
+        a.dx, a.dx_sr = dx.data_ptr(), a.cols
+    a.dweight = dweight.data_ptr()
+    L = _lib.lib()
+    ref = ctypes.byref(a)
+    ws = workspace(m.device, L.mamba_add_rmsnorm_bwd_workspace_size(ref))
+    check(L.mamba_add_rmsnorm_bwd(ref, ws.data_ptr(), ws.numel(), _raw_stream(m)), "mamba_add_rmsnorm_bwd")
+    return dx, dres, dweight
+
+
+class _AddRmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        rstd = x.new_empty(x.numel() // max(x.shape[-1], 1) if x.dim() else 1, dtype=torch.float32)
+        y, s = add_rms_norm(x, weight, residual, eps, rstd=rstd)
+        ctx.save_for_backward(s, weight, rstd)
+        ctx.io = x.dtype
+        ctx.set_materialize_grads(False)
+        return (y, s) if residual is not None else y
+
+    @_once
+    def backward(ctx, dy, ds=None):
+        s, weight, rstd = ctx.saved_tensors
+        wx, ww, wr = ctx.needs_input_grad[:3]
+        if dy is None:  # the sum alone was used
+            if ds is None:
+                return (None,) * 4
+            return ds.to(ctx.io), torch.zeros_like(weight) if ww else None, ds, None
+        m, g = _matrix(s, "s"), _matrix(dy, "dy")
+        with _one_device(g):
+            dx, dres, dweight = _arn_bwd(dy, g, s, m, weight, rstd, ds, wx, wr)
+        return dx, dweight if ww else None, dres if wr else None, None
+
+
+def add_rms_norm_autograd(x, weight, residual=None, eps: float = 1e-5) -> tuple:
+    """``add_rms_norm`` as a differentiable op: (y, s), with gradients of x, weight and residual."""
+    if residual is None:
+        return _AddRmsNorm.apply(x, weight, None, eps), x
+    return _AddRmsNorm.apply(x, weight, residual, eps)
 
 
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, offset: int = 0, residual: Optional[torch.Tensor] = None,

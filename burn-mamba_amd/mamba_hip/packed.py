@@ -1,5 +1,5 @@
-"""Mamba-1's short convolution and selective scan over packed sequences, their
-gradients, and their single-token steps on a cache addressed by slot.
+"""Mamba-1's short convolution and selective scan, and a gated linear recurrence, over
+packed sequences, their gradients, and their single-token steps on a cache addressed by slot.
 
 Packed: the rows of several sequences one behind the other in [rows, .] tensors,
 sequence s being rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (``cu_seqlens`` int32
@@ -14,7 +14,8 @@ kept).  A slot's row is zeroed by the caller before its first sequence.
 
 Reference: ``Mamba1::forward`` layer 2 (src/mamba1/mamba1.rs:300-340),
 ``Mamba1::selective_scan`` (mamba1.rs:422-523), ``Mamba1::step``
-(mamba1.rs:533-733), which take sequences of one length and a cache row for each.
+(mamba1.rs:533-733), which take sequences of one length and a cache row for each; the
+gated recurrence stands beside them, with one state a channel.
 """
 
 from __future__ import annotations
@@ -28,8 +29,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import (Conv1dPackedArgs, Conv1dStepSlotsArgs, Mamba1ScanPackedArgs, Mamba1ScanPackedBwdArgs,
-                   Mamba1ScanStepSlotsArgs, check)
+from ._lib import (Conv1dPackedArgs, Conv1dStepSlotsArgs, GatedScanArgs, GatedScanBwdArgs, GatedStepSlotsArgs,
+                   Mamba1ScanPackedArgs, Mamba1ScanPackedBwdArgs, Mamba1ScanStepSlotsArgs, check)
 from .ssd import _dtype_code, workspace
 
 
@@ -402,4 +403,164 @@ def scan_step_slots(u, delta, A, B, C, state: torch.Tensor, slots: Optional[torc
         a.A, a.D, a.delta_bias = A.data_ptr(), _p(D), _p(delta_bias)
         a.state, a.nslots, a.slots = state.data_ptr(), state.shape[0], _p(slots)
         check(_lib.lib().mamba1_scan_step_slots(ctypes.byref(a), _raw_stream(u)), "mamba1_scan_step_slots")
+    return y
+
+
+# -------------------------------------------------- gated linear recurrence ---
+
+CARRY_ROWS = 64  # rows between the states that the forward keeps for its backward
+
+
+def _gated_operands(x, r, i, A, z):
+    """Checks shared by the packed recurrence and the step; (rows, dim)."""
+    _rows(x, "x")
+    rows, d = x.shape
+    _rows(r, "r", rows, d, x.dtype)
+    _rows(i, "i", rows, d, x.dtype)
+    if z is not None:
+        _rows(z, "z", rows, d, x.dtype)
+    _param(A, "A", d)
+    return rows, d
+
+
+def _gated_args(x, r, i, A, cu_seqlens, z, carry, state=None, slots=None) -> GatedScanArgs:
+    rows, d = _gated_operands(x, r, i, A, z)
+    _sequences(cu_seqlens, slots, state, "state", d)
+    _param(carry, "carry", -(-rows // CARRY_ROWS), d)
+    a = GatedScanArgs()
+    _gated_fill(a, x, r, i, A, cu_seqlens, z, carry)
+    if state is not None:
+        a.state, a.nslots, a.slots = state.data_ptr(), state.shape[0], _p(slots)
+    return a
+
+
+def _gated_fill(a: GatedScanArgs, x, r, i, A, cu_seqlens, z, carry):
+    """The arguments of operands that have been checked."""
+    (a.rows, a.dim), a.nseq, a.io_dtype = x.shape, cu_seqlens.shape[0] - 1, _dtype_code(x)
+    a.cu_seqlens, a.A, a.carry = cu_seqlens.data_ptr(), A.data_ptr(), _p(carry)
+    a.x, a.x_st, a.r, a.r_st, a.i, a.i_st = x.data_ptr(), x.stride(0), r.data_ptr(), r.stride(0), i.data_ptr(), i.stride(0)
+    if z is not None:
+        a.z, a.z_st = z.data_ptr(), z.stride(0)
+
+
+def gated_scan_packed(x, r, i, A, cu_seqlens, z=None, state: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                      carry: Optional[torch.Tensor] = None, y: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A linear recurrence with a state for each channel, whose decay and input are gated by
+    the token, over packed sequences (s: the logistic function):
+
+        a_t = exp(A s(r_t)),  h_t = a_t h_{t-1} + sqrt(1 - a_t^2) s(i_t) x_t,  y_t = h_t silu(z_t)
+
+    x, r, i and z [rows, d] f32 or bf16 (one type, any row strides; without z, y_t = h_t), A [d]
+    f32 and at most 0.  ``state`` [slots, d] f32 holds what the sequences start from and is
+    overwritten with what they end in; None starts from zero.  ``carry``, [ceil(rows / 64), d]
+    f32, takes the states that ``gated_scan_packed_bwd`` goes on from.  Returns y [rows, d]
+    of x's type.  The same inputs give the same bits."""
+    a = _gated_args(x, r, i, A, cu_seqlens, z, carry, state, slots)
+    a.fill_outside = int(y is None)
+    if y is not None:
+        _rows(y, "y", x.shape[0], x.shape[1], x.dtype)
+    with _one_device(x, r, i, A, cu_seqlens, z, state, slots, carry, y):
+        if y is None:
+            y = _new(x)
+        _gated_fwd(a, x, y)
+    return y
+
+
+def _gated_fwd(a: GatedScanArgs, x, y):
+    a.y, a.y_st = y.data_ptr(), y.stride(0)
+    L = _lib.lib()
+    ref = ctypes.byref(a)
+    need = L.mamba_gated_scan_workspace_size(ref)
+    ws = workspace(x.device, need) if need else None
+    check(L.mamba_gated_scan_fwd(ref, _p(ws), need, _raw_stream(x)), "mamba_gated_scan_fwd")
+
+
+def gated_scan_packed_bwd(dy, x, r, i, A, cu_seqlens, carry, z=None, initial_state=None, d_final_state=None) -> dict:
+    """Gradients of ``gated_scan_packed`` from its inputs and the ``carry`` that it kept (from
+    the same initial_state).  ``initial_state`` and ``d_final_state`` [sequences, d] f32 or
+    None.  Returns dict(dx, dr, di, dz of their tensors' type, zero outside the sequences; dA,
+    d_initial_state f32; None for what was not given).  The same inputs give the same bits.
+    Where a_t is exactly 1 the input's weight is 0, and is taken not to change with a_t."""
+    _need(carry is not None, "carry is required")
+    a = GatedScanBwdArgs()
+    a.fwd = _gated_args(x, r, i, A, cu_seqlens, z, carry)
+    d, s = x.shape[1], cu_seqlens.numel() - 1
+    _rows(dy, "dy", x.shape[0], d, x.dtype)
+    _param(initial_state, "initial_state", s, d)
+    _param(d_final_state, "d_final_state", s, d)
+    with _one_device(dy, x, r, i, A, cu_seqlens, carry, z, initial_state, d_final_state):
+        return _gated_bwd(a, dy, x, A, z, initial_state, d_final_state)
+
+
+def _gated_bwd(a: GatedScanBwdArgs, dy, x, A, z, initial_state, d_final_state) -> dict:
+    """``gated_scan_packed_bwd`` after its checks."""
+    out = dict(dx=_new(x), dr=_new(x), di=_new(x), dz=None if z is None else _new(x), dA=_new(A), d_initial_state=None)
+    if initial_state is not None:  # an empty sequence ends in what it starts from
+        out["d_initial_state"] = torch.zeros_like(initial_state) if d_final_state is None else d_final_state.clone()
+    a.initial_state, a.d_final_state, a.d_initial_state = _p(initial_state), _p(d_final_state), _p(out["d_initial_state"])
+    d = x.shape[1]
+    a.dy, a.dy_st, a.dA = dy.data_ptr(), dy.stride(0), out["dA"].data_ptr()
+    a.dx, a.dx_st, a.dr, a.dr_st, a.di, a.di_st = out["dx"].data_ptr(), d, out["dr"].data_ptr(), d, out["di"].data_ptr(), d
+    if z is not None:
+        a.dz, a.dz_st = out["dz"].data_ptr(), d
+    L = _lib.lib()
+    ref = ctypes.byref(a)
+    need = L.mamba_gated_scan_bwd_workspace_size(ref)
+    ws = workspace(x.device, need) if need else None
+    check(L.mamba_gated_scan_bwd(ref, _p(ws), need, _raw_stream(x)), "mamba_gated_scan_bwd")
+    return out
+
+
+class _GatedScanPacked(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, r, i, A, cu_seqlens, z, initial_state):
+        rows, d = _gated_operands(x, r, i, A, z)
+        shape = (_sequences(cu_seqlens, None, None, "state"), d)
+        _param(initial_state, "initial_state", *shape)
+        final = A.new_zeros(shape) if initial_state is None else initial_state.clone()
+        carry = A.new_empty((-(-rows // CARRY_ROWS), d))
+        y = gated_scan_packed(x, r, i, A, cu_seqlens, z, final, None, carry)
+        ctx.save_for_backward(x, r, i, A, cu_seqlens, z, initial_state, carry)
+        ctx.set_materialize_grads(False)
+        return y, final
+
+    @_once
+    def backward(ctx, dy, dfinal):
+        x, r, i, A, cu_seqlens, z, h0, carry = ctx.saved_tensors
+        if dy is None and dfinal is None:
+            return (None,) * 7
+        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else _like_rows(dy)
+        a = GatedScanBwdArgs()
+        _gated_fill(a.fwd, x, r, i, A, cu_seqlens, z, carry)
+        with _one_device(dy):
+            g = _gated_bwd(a, dy, x, A, z, h0, None if dfinal is None else dfinal.contiguous())
+        return g["dx"], g["dr"], g["di"], g["dA"], None, g["dz"], g["d_initial_state"]
+
+
+def gated_scan_packed_autograd(x, r, i, A, cu_seqlens, z=None, initial_state=None):
+    """``gated_scan_packed`` as a differentiable op: (y, final_state [sequences, d]) from
+    ``initial_state`` [sequences, d] (None: zero), with gradients of every float input."""
+    return _GatedScanPacked.apply(x, r, i, A, cu_seqlens, z, initial_state)
+
+
+def gated_step_slots(x, r, i, A, state: torch.Tensor, slots: Optional[torch.Tensor], z=None,
+                     y: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token a row of ``gated_scan_packed`` on a cache of slots: x, r, i, z [b, d] f32 or
+    bf16 (one type), state [slots, d] f32 (in place), slots [b] int32.  Returns y [b, d] of
+    x's type; a row whose slot is out of range is zero."""
+    b, d = _gated_operands(x, r, i, A, z)
+    _slots(b, slots, state, "state", d)
+    if y is not None:
+        _rows(y, "y", b, d, x.dtype)
+    with _one_device(x, r, i, A, state, slots, z, y):
+        if y is None:
+            y = _new(x)
+        a = GatedStepSlotsArgs()
+        a.batch, a.dim, a.io_dtype = b, d, _dtype_code(x)
+        a.x, a.x_sb, a.r, a.r_sb, a.i, a.i_sb = x.data_ptr(), x.stride(0), r.data_ptr(), r.stride(0), i.data_ptr(), i.stride(0)
+        if z is not None:
+            a.z, a.z_sb = z.data_ptr(), z.stride(0)
+        a.A, a.state, a.nslots, a.slots = A.data_ptr(), state.data_ptr(), state.shape[0], _p(slots)
+        a.y, a.y_sb = y.data_ptr(), y.stride(0)
+        check(_lib.lib().mamba_gated_step_slots(ctypes.byref(a), _raw_stream(x)), "mamba_gated_step_slots")
     return y

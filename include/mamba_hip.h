@@ -51,7 +51,10 @@
  *   mamba_conv1d_packed_fwd / _bwd, mamba1_scan_packed_fwd / _bwd (sequences of
  *   different lengths, gradients), mamba_conv1d_step_slots and
  *   mamba1_scan_step_slots (single tokens on a cache addressed by slot),
- *   mamba_layernorm_fwd / _bwd and mamba_dropout.
+ *   mamba_layernorm_fwd / _bwd and mamba_dropout; for layers around a gated linear
+ *   recurrence mamba_gated_scan_fwd / _bwd and mamba_gated_step_slots,
+ *   mamba_add_rmsnorm_fwd / _bwd (also to rows of 8 bits), and mamba_linear_q4_fwd
+ *   (weights of 4 bits).
  */
 #ifndef MAMBA_HIP_H
 #define MAMBA_HIP_H
@@ -76,7 +79,9 @@ typedef enum mamba_status {
 
 typedef enum mamba_dtype {
     MAMBA_F32 = 0,
-    MAMBA_BF16 = 1
+    MAMBA_BF16 = 1,
+    MAMBA_INT8 = 2,  /* rows of 8 bits with a scale each: */
+    MAMBA_E4M3 = 3   /* mamba_add_rmsnorm_fwd, mamba_linear_q4_fwd (int8) */
 } mamba_dtype;
 
 /* Human-readable description of the last error raised on the calling thread. */
@@ -986,6 +991,80 @@ typedef struct mamba1_scan_step_slots_args {
 
 int mamba1_scan_step_slots(const mamba1_scan_step_slots_args* args, mamba_stream_t stream);
 
+/* Gated linear recurrence, one state a channel, with its decay and its input   */
+/* gated by the token (beside the selective scan; s(v) = 1 / (1 + exp(-v))):   */
+/*   a_t = exp(A s(r_t)),  h_t = a_t h_{t-1} + sqrt(1 - a_t^2) s(i_t) x_t,     */
+/*   y_t = h_t silu(z_t), or h_t where z is NULL; A <= 0                       */
+/* over packed sequences.  state is read for a sequence's start and            */
+/* overwritten with its end; NULL starts from zero and keeps nothing.  carry   */
+/* [ceil(rows / 64), d] or NULL: the states that enter rows 0, 64, 128, ...,   */
+/* which the backward takes (what it holds for a row that begins a sequence or */
+/* belongs to none is not looked at).  y may be x, r, i or z itself.           */
+typedef struct mamba_gated_scan_args {
+    int64_t rows;
+    int32_t nseq, dim, io_dtype, fill_outside;
+    const int32_t* cu_seqlens;
+    const void* x;      int64_t x_st;         /* [rows, d] of io_dtype        */
+    const void* r;      int64_t r_st;         /* [rows, d]                    */
+    const void* i;      int64_t i_st;         /* [rows, d]                    */
+    const void* z;      int64_t z_st;         /* [rows, d] or NULL            */
+    const float* A;                           /* [d]                          */
+    float* state;                             /* [nslots, d] or NULL          */
+    int64_t nslots;
+    const int32_t* slots;                     /* [nseq] or NULL               */
+    float* carry;
+    void* y;            int64_t y_st;         /* [rows, d]                    */
+} mamba_gated_scan_args;
+
+size_t mamba_gated_scan_workspace_size(const mamba_gated_scan_args* args);
+int mamba_gated_scan_fwd(const mamba_gated_scan_args* args, void* workspace, size_t workspace_bytes,
+                         mamba_stream_t stream);
+
+/* Its gradients (fwd.state and fwd.slots NULL, fwd.y unused, fwd.carry as the */
+/* forward from the same initial_state wrote it).  With g_t = dy_t silu(z_t),  */
+/* d_final_state added at a sequence's last row, u_t = s(i_t) x_t and          */
+/* m_t = sqrt(1 - a_t^2):                                                      */
+/*   dh_t = g_t + a_{t+1} dh_{t+1},  e_t = dh_t (a_t h_{t-1} - u_t a_t^2 / m_t) */
+/*   dx = dh m s(i),  di = dh m u s(-i),  dr = e A s(r) s(-r),                 */
+/*   dA = sum_t e s(r),  dz = dy h silu'(z),  d_initial_state = a dh (first)   */
+/* (u a^2 / m is taken as 0 where a is exactly 1).  initial_state and          */
+/* d_final_state [nseq, d] or NULL (zero).  dx, dr, di and dz are zero outside */
+/* the sequences; d_initial_state's rows of empty sequences are left as they   */
+/* were.  Sums in a fixed order: the same inputs give the same bits.           */
+typedef struct mamba_gated_scan_bwd_args {
+    mamba_gated_scan_args fwd;
+    const float* initial_state;
+    const void* dy;     int64_t dy_st;
+    const float* d_final_state;
+    void* dx;           int64_t dx_st;
+    void* dr;           int64_t dr_st;
+    void* di;           int64_t di_st;
+    void* dz;           int64_t dz_st;
+    float* dA;
+    float* d_initial_state;
+} mamba_gated_scan_bwd_args;
+
+size_t mamba_gated_scan_bwd_workspace_size(const mamba_gated_scan_bwd_args* args);
+int mamba_gated_scan_bwd(const mamba_gated_scan_bwd_args* args, void* workspace, size_t workspace_bytes,
+                         mamba_stream_t stream);
+
+/* One token a row on the states of slots.  The output row of a slot out of    */
+/* range is zero.  y may be x, r, i or z itself.                               */
+typedef struct mamba_gated_step_slots_args {
+    int32_t batch, dim, io_dtype;
+    const void* x;      int64_t x_sb;
+    const void* r;      int64_t r_sb;
+    const void* i;      int64_t i_sb;
+    const void* z;      int64_t z_sb;
+    const float* A;
+    float* state;                             /* [nslots, d]                  */
+    int64_t nslots;
+    const int32_t* slots;                     /* [batch] or NULL              */
+    void* y;            int64_t y_sb;
+} mamba_gated_step_slots_args;
+
+int mamba_gated_step_slots(const mamba_gated_step_slots_args* args, mamba_stream_t stream);
+
 /* ------------------------------------------------------------------------- */
 /* Layer norm over rows (cols contiguous elements of io_dtype):                */
 /*   xh = (x - mean) rstd, rstd = 1 / sqrt(mean((x - mean)^2) + eps),          */
@@ -1029,6 +1108,58 @@ int mamba_layernorm_bwd(const mamba_layernorm_bwd_args* args, void* workspace, s
                         mamba_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
+/* RMS norm with the residual's addition, over rows of cols contiguous         */
+/* elements:                                                                   */
+/*   s = residual + x,  y = s rstd weight,  rstd = 1 / sqrt(mean(s^2) + eps)   */
+/* x and y of io_dtype, residual and s of stream_dtype (f32, or bf16 with bf16 */
+/* rows).  residual NULL: s = x, and s is not written.  y is formed from the   */
+/* sum as it is before it is stored as s.  rstd [rows] is written if given.    */
+/* s may be residual itself, and x where the types agree; y may be x.          */
+/*                                                                             */
+/* The row of 8 bits (q given, y NULL) is y / scale, rounded to the nearest    */
+/* (ties to even), scale [rows] = max |y| / 127 (MAMBA_INT8) or / 448          */
+/* (MAMBA_E4M3, OCP).  A row whose largest |y| is below 2^-100 has scale 0 and */
+/* zeros; a row with a NaN or an infinity in y a NaN for its scale, and zeros. */
+/* ------------------------------------------------------------------------- */
+typedef struct mamba_add_rmsnorm_args {
+    int64_t rows;
+    int32_t cols, io_dtype, stream_dtype, q_dtype;
+    float eps;
+    const void* x;        int64_t x_sr;
+    const void* residual; int64_t residual_sr;
+    const float* weight;                      /* [cols] or NULL (1)           */
+    void* s;              int64_t s_sr;
+    void* y;              int64_t y_sr;
+    float* rstd;                              /* [rows] or NULL               */
+    void* q;              int64_t q_sr;       /* [rows, cols] bytes           */
+    float* scale;                             /* [rows]                       */
+} mamba_add_rmsnorm_args;
+
+int mamba_add_rmsnorm_fwd(const mamba_add_rmsnorm_args* args, mamba_stream_t stream);
+
+/* Its gradients from s as the forward stored it (x itself without a           */
+/* residual), rstd, dy and, if given, ds (of s, stream_dtype), xh = s rstd:    */
+/*   d = ds + rstd (dy weight - xh mean(dy weight xh)),  dweight = sum dy xh   */
+/* d is written as dx (io_dtype) and as dresidual (stream_dtype), each if      */
+/* given; dweight may be NULL.  Sums in a fixed order.                         */
+typedef struct mamba_add_rmsnorm_bwd_args {
+    int64_t rows;
+    int32_t cols, io_dtype, stream_dtype;
+    const void* s;        int64_t s_sr;
+    const void* dy;       int64_t dy_sr;
+    const void* ds;       int64_t ds_sr;
+    const float* weight;
+    const float* rstd;
+    void* dx;             int64_t dx_sr;
+    void* dresidual;      int64_t dresidual_sr;
+    float* dweight;
+} mamba_add_rmsnorm_bwd_args;
+
+size_t mamba_add_rmsnorm_bwd_workspace_size(const mamba_add_rmsnorm_bwd_args* args);
+int mamba_add_rmsnorm_bwd(const mamba_add_rmsnorm_bwd_args* args, void* workspace, size_t workspace_bytes,
+                          mamba_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
 /* Dropout: out[i] = residual[i] + (word(i) >= p 2^32 ? x[i] / (1 - p) : 0),   */
 /* word(i) = word i % 4 of Philox 4x32-10 at counter (i / 4, rng[1] + offset), */
 /* key rng[0], i the row-major place of the element: the mask is a function    */
@@ -1048,6 +1179,46 @@ typedef struct mamba_dropout_args {
 } mamba_dropout_args;
 
 int mamba_dropout(const mamba_dropout_args* args, mamba_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* Products of few rows with weights of 4 bits (beside mamba_linear_fwd):      */
+/*   y[m, n] = x_scale[m] sum_k x[m, k] (c[k, n] - zero[g, n]) scale[g, n] + bias[n], */
+/* c in 0..15, g = k / group (32, 64 or 128; the last group may be shorter),   */
+/* zero 8 where there are none.  mamba_linear_q4_pack lays the codes out once, */
+/* at load, in the order in which the kernels read them, with the scales and   */
+/* zero points in the same buffer (packed, of mamba_linear_q4_packed_size      */
+/* bytes, 16-byte aligned).                                                    */
+/* x: bf16, f32 (three bf16 parts, which hold all of it) or int8 with x_scale  */
+/* [rows]; sums are f32, of int8 rows exact within a group.  The codes are     */
+/* multiplied as they are and the zero points taken off a group's sum, so a    */
+/* row of x with a NaN or an infinity gives NaN everywhere.                    */
+/* ------------------------------------------------------------------------- */
+typedef struct mamba_q4_weight {
+    int32_t d_in, d_out, group, scale_dtype;  /* scales f32 or bf16           */
+    int32_t has_zero;
+    const void* packed;
+} mamba_q4_weight;
+
+size_t mamba_linear_q4_packed_size(const mamba_q4_weight* w);
+/* codes [d_in, d_out] (a byte each, the low four bits taken), scale [groups,  */
+/* d_out] of scale_dtype and zero [groups, d_out] bytes (0..15, with has_zero) */
+/* contiguous -> packed                                                        */
+int mamba_linear_q4_pack(const mamba_q4_weight* w, const void* codes, const void* scale, const void* zero,
+                         void* packed, mamba_stream_t stream);
+
+typedef struct mamba_linear_q4_args {
+    mamba_q4_weight w;
+    int64_t rows;
+    int32_t x_dtype, y_dtype;                 /* f32, bf16 or MAMBA_INT8; f32 or bf16 */
+    const void* x;      int64_t x_ld;         /* [rows, d_in]                 */
+    const float* x_scale;                     /* [rows], with int8            */
+    const float* bias;                        /* [d_out] or NULL              */
+    void* y;            int64_t y_ld;         /* [rows, d_out]                */
+} mamba_linear_q4_args;
+
+size_t mamba_linear_q4_workspace_size(const mamba_linear_q4_args* args);
+int mamba_linear_q4_fwd(const mamba_linear_q4_args* args, void* workspace, size_t workspace_bytes,
+                        mamba_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -15,6 +15,8 @@ pub const MAMBA_ERR_WORKSPACE: c_int = 3;
 pub const MAMBA_ERR_HIP: c_int = 4;
 pub const MAMBA_F32: c_int = 0;
 pub const MAMBA_BF16: c_int = 1;
+pub const MAMBA_INT8: c_int = 2;
+pub const MAMBA_E4M3: c_int = 3;
 pub const MAMBA2_STACK_NOALLOC_SCRATCH_BYTES: usize = 48 << 20;
 
 #[repr(C)]
@@ -985,6 +987,98 @@ impl Default for Mamba1ScanStepSlotsArgs {
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
+pub struct MambaGatedScanArgs {
+    pub rows: i64,
+    pub nseq: i32,
+    pub dim: i32,
+    pub io_dtype: i32,
+    pub fill_outside: i32,
+    pub cu_seqlens: *const i32,
+    pub x: *const c_void,
+    pub x_st: i64,
+    pub r: *const c_void,
+    pub r_st: i64,
+    pub i: *const c_void,
+    pub i_st: i64,
+    pub z: *const c_void,
+    pub z_st: i64,
+    pub A: *const f32,
+    pub state: *mut f32,
+    pub nslots: i64,
+    pub slots: *const i32,
+    pub carry: *mut f32,
+    pub y: *mut c_void,
+    pub y_st: i64,
+}
+
+impl Default for MambaGatedScanArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct MambaGatedScanBwdArgs {
+    pub fwd: MambaGatedScanArgs,
+    pub initial_state: *const f32,
+    pub dy: *const c_void,
+    pub dy_st: i64,
+    pub d_final_state: *const f32,
+    pub dx: *mut c_void,
+    pub dx_st: i64,
+    pub dr: *mut c_void,
+    pub dr_st: i64,
+    pub di: *mut c_void,
+    pub di_st: i64,
+    pub dz: *mut c_void,
+    pub dz_st: i64,
+    pub dA: *mut f32,
+    pub d_initial_state: *mut f32,
+}
+
+impl Default for MambaGatedScanBwdArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct MambaGatedStepSlotsArgs {
+    pub batch: i32,
+    pub dim: i32,
+    pub io_dtype: i32,
+    pub x: *const c_void,
+    pub x_sb: i64,
+    pub r: *const c_void,
+    pub r_sb: i64,
+    pub i: *const c_void,
+    pub i_sb: i64,
+    pub z: *const c_void,
+    pub z_sb: i64,
+    pub A: *const f32,
+    pub state: *mut f32,
+    pub nslots: i64,
+    pub slots: *const i32,
+    pub y: *mut c_void,
+    pub y_sb: i64,
+}
+
+impl Default for MambaGatedStepSlotsArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
 pub struct MambaLayernormArgs {
     pub rows: i64,
     pub cols: i32,
@@ -1037,6 +1131,68 @@ impl Default for MambaLayernormBwdArgs {
 
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
+pub struct MambaAddRmsnormArgs {
+    pub rows: i64,
+    pub cols: i32,
+    pub io_dtype: i32,
+    pub stream_dtype: i32,
+    pub q_dtype: i32,
+    pub eps: f32,
+    pub x: *const c_void,
+    pub x_sr: i64,
+    pub residual: *const c_void,
+    pub residual_sr: i64,
+    pub weight: *const f32,
+    pub s: *mut c_void,
+    pub s_sr: i64,
+    pub y: *mut c_void,
+    pub y_sr: i64,
+    pub rstd: *mut f32,
+    pub q: *mut c_void,
+    pub q_sr: i64,
+    pub scale: *mut f32,
+}
+
+impl Default for MambaAddRmsnormArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct MambaAddRmsnormBwdArgs {
+    pub rows: i64,
+    pub cols: i32,
+    pub io_dtype: i32,
+    pub stream_dtype: i32,
+    pub s: *const c_void,
+    pub s_sr: i64,
+    pub dy: *const c_void,
+    pub dy_sr: i64,
+    pub ds: *const c_void,
+    pub ds_sr: i64,
+    pub weight: *const f32,
+    pub rstd: *const f32,
+    pub dx: *mut c_void,
+    pub dx_sr: i64,
+    pub dresidual: *mut c_void,
+    pub dresidual_sr: i64,
+    pub dweight: *mut f32,
+}
+
+impl Default for MambaAddRmsnormBwdArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
 pub struct MambaDropoutArgs {
     pub rows: i64,
     pub cols: i64,
@@ -1053,6 +1209,48 @@ pub struct MambaDropoutArgs {
 }
 
 impl Default for MambaDropoutArgs {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct MambaQ4Weight {
+    pub d_in: i32,
+    pub d_out: i32,
+    pub group: i32,
+    pub scale_dtype: i32,
+    pub has_zero: i32,
+    pub packed: *const c_void,
+}
+
+impl Default for MambaQ4Weight {
+    /// Every size 0, every pointer null, every stride 0.
+    fn default() -> Self {
+        // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
+        unsafe { core::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct MambaLinearQ4Args {
+    pub w: MambaQ4Weight,
+    pub rows: i64,
+    pub x_dtype: i32,
+    pub y_dtype: i32,
+    pub x: *const c_void,
+    pub x_ld: i64,
+    pub x_scale: *const f32,
+    pub bias: *const f32,
+    pub y: *mut c_void,
+    pub y_ld: i64,
+}
+
+impl Default for MambaLinearQ4Args {
     /// Every size 0, every pointer null, every stride 0.
     fn default() -> Self {
         // SAFETY: all fields are integers, floats or raw pointers, for which zero is valid.
@@ -1131,8 +1329,20 @@ extern "C" {
     pub fn mamba1_scan_packed_bwd_workspace_size(args: *const Mamba1ScanPackedBwdArgs) -> usize;
     pub fn mamba1_scan_packed_bwd(args: *const Mamba1ScanPackedBwdArgs, workspace: *mut c_void, workspace_bytes: usize, stream: MambaStream) -> c_int;
     pub fn mamba1_scan_step_slots(args: *const Mamba1ScanStepSlotsArgs, stream: MambaStream) -> c_int;
+    pub fn mamba_gated_scan_workspace_size(args: *const MambaGatedScanArgs) -> usize;
+    pub fn mamba_gated_scan_fwd(args: *const MambaGatedScanArgs, workspace: *mut c_void, workspace_bytes: usize, stream: MambaStream) -> c_int;
+    pub fn mamba_gated_scan_bwd_workspace_size(args: *const MambaGatedScanBwdArgs) -> usize;
+    pub fn mamba_gated_scan_bwd(args: *const MambaGatedScanBwdArgs, workspace: *mut c_void, workspace_bytes: usize, stream: MambaStream) -> c_int;
+    pub fn mamba_gated_step_slots(args: *const MambaGatedStepSlotsArgs, stream: MambaStream) -> c_int;
     pub fn mamba_layernorm_fwd(args: *const MambaLayernormArgs, stream: MambaStream) -> c_int;
     pub fn mamba_layernorm_bwd_workspace_size(args: *const MambaLayernormBwdArgs) -> usize;
     pub fn mamba_layernorm_bwd(args: *const MambaLayernormBwdArgs, workspace: *mut c_void, workspace_bytes: usize, stream: MambaStream) -> c_int;
+    pub fn mamba_add_rmsnorm_fwd(args: *const MambaAddRmsnormArgs, stream: MambaStream) -> c_int;
+    pub fn mamba_add_rmsnorm_bwd_workspace_size(args: *const MambaAddRmsnormBwdArgs) -> usize;
+    pub fn mamba_add_rmsnorm_bwd(args: *const MambaAddRmsnormBwdArgs, workspace: *mut c_void, workspace_bytes: usize, stream: MambaStream) -> c_int;
     pub fn mamba_dropout(args: *const MambaDropoutArgs, stream: MambaStream) -> c_int;
+    pub fn mamba_linear_q4_packed_size(w: *const MambaQ4Weight) -> usize;
+    pub fn mamba_linear_q4_pack(w: *const MambaQ4Weight, codes: *const c_void, scale: *const c_void, zero: *const c_void, packed: *mut c_void, stream: MambaStream) -> c_int;
+    pub fn mamba_linear_q4_workspace_size(args: *const MambaLinearQ4Args) -> usize;
+    pub fn mamba_linear_q4_fwd(args: *const MambaLinearQ4Args, workspace: *mut c_void, workspace_bytes: usize, stream: MambaStream) -> c_int;
 }

@@ -41,6 +41,7 @@ FILE_FLAGS = {
     # the decode products: accumulators in VGPRs keep a wave within 128
     # registers (four waves per SIMD)
     "lin.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "lin_q4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

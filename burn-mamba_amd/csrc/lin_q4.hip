@@ -78,51 +78,257 @@ struct Q4P {
     Q4W w;
     int64_t rows;
     const void* x; int64_t x_ld;
+    int K8;                 // elements of a row of x: a multiple of 8
     const float* xs;
     const float* bias;
     void* y; int64_t y_ld; bool ybf16;
 };
 
-template <typename T>
-__device__ __forceinline__ float q4_x(const T* x) { return load_f32<T>(x); }
-template <>
-__device__ __forceinline__ float q4_x<int8_t>(const int8_t* x) { return (float)*x; }
+typedef __bf16 q4_bf16x8 __attribute__((ext_vector_type(8)));
+typedef float q4_f32x4 __attribute__((ext_vector_type(4)));
+typedef int q4_i32x4 __attribute__((ext_vector_type(4)));
 
-// A wave per row and column tile.
-template <typename T>
-__global__ __launch_bounds__(64) void q4_rows(Q4P p) {
-    const int l = threadIdx.x, col = l & 15, kq = l >> 4, n = blockIdx.x * kQ4N + col;
-    for (int64_t m = blockIdx.y; m < p.rows; m += gridDim.y) {
-        const T* x = static_cast<const T*>(p.x) + m * p.x_ld;
-        float total = 0.f;
-        for (int kb = 0; kb < p.w.KB; ++kb) {
-            const uint4 c4 = p.w.codes[((int64_t)blockIdx.x * p.w.KB + kb) * 64 + l];
-            const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+enum Q4X { Q4_BF16 = 0, Q4_F32 = 1, Q4_I8 = 2 };
+
+// Lane l's operand of 32 k of 16 rows: row l % 16, k 8 (l / 16) .. + 7.  f32 rows are three bf16
+// parts, each the upper half of what the ones before leave (8 bits of the 24), lowest first.
+template <int X> struct Q4A;
+template <> struct Q4A<Q4_BF16> {
+    static constexpr int kParts = 1, kSize = 2;
+    uint4 v;
+    __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void load(const char* p) { __builtin_memcpy(&v, p, 16); }
+    __device__ __forceinline__ q4_bf16x8 part(int) const { return __builtin_bit_cast(q4_bf16x8, v); }
+};
+template <> struct Q4A<Q4_F32> {
+    static constexpr int kParts = 3, kSize = 4;
+    float v[8];
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                const int g = (kb * kQ4K + 32 * st) / p.w.G;
-                const int64_t at = ((int64_t)blockIdx.x * p.w.NG + g) * kQ4N + col;
-                const float s = p.w.sbf16 ? bf16_to_f32(static_cast<const bf16_t*>(p.w.scale)[at]) : static_cast<const float*>(p.w.scale)[at];
-                const float z = p.w.zeros ? (float)p.w.zero[at] : 8.f;
-                float sum = 0.f, sx = 0.f;
-                for (int e = 0; e < 8; ++e) {
-                    const int k = kb * kQ4K + 32 * st + 8 * kq + e;
-                    const float v = k < p.w.K ? q4_x<T>(x + k) : 0.f;
-                    sum = __builtin_fmaf(v, (float)((c[st] >> (4 * (e / 2 + 4 * (e & 1)))) & 15u), sum);
-                    sx += v;
-                }
-                total = __builtin_fmaf(s, __builtin_fmaf(-z, sx, sum), total);
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+    __device__ __forceinline__ void load(const char* p) { __builtin_memcpy(v, p, 32); }
+    __device__ __forceinline__ q4_bf16x8 part(int k) const {
+        uint32_t d[4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float r = v[i];
+#pragma unroll
+            for (int j = k; j < 2; ++j) r -= __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+            const uint32_t h = __float_as_uint(r) >> 16;
+            d[i / 2] = i & 1 ? d[i / 2] | h << 16 : h;
+        }
+        return __builtin_bit_cast(q4_bf16x8, d);
+    }
+};
+template <> struct Q4A<Q4_I8> {
+    static constexpr int kParts = 1, kSize = 1;
+    uint2 v;
+    __device__ __forceinline__ void zero() { v = make_uint2(0, 0); }
+    __device__ __forceinline__ void load(const char* p) { __builtin_memcpy(&v, p, 8); }
+    // in the order in which the codes' bytes come: 0 4 1 5 2 6 3 7
+    __device__ __forceinline__ long part(int) const {
+        return (long)((uint64_t)__builtin_amdgcn_perm(v.y, v.x, 0x07030602u) << 32 | __builtin_amdgcn_perm(v.y, v.x, 0x05010400u));
+    }
+};
+
+// The codes of a dword, as operands.  A bf16 whose upper four bits of mantissa are the code
+// is 16 + code: one shift and one and-or a pair.
+__device__ __forceinline__ q4_bf16x8 q4_codes_bf16(uint32_t w) {
+    const uint32_t d[4] = {(w << 3 & 0x00780078u) | 0x41804180u, (w >> 1 & 0x00780078u) | 0x41804180u, (w >> 5 & 0x00780078u) | 0x41804180u,
+                           (w >> 9 & 0x00780078u) | 0x41804180u};
+    return __builtin_bit_cast(q4_bf16x8, d);
+}
+__device__ __forceinline__ long q4_codes_i8(uint32_t w) { return (long)((uint64_t)(w >> 4 & 0x0f0f0f0fu) << 32 | (w & 0x0f0f0f0fu)); }
+
+// One block of C column tiles and RT row tiles, in flight.
+template <int X, int RT, int C, int GB>
+struct Q4Block {
+    uint4 w[C];
+    float scale[C][GB], zero[C][GB];
+    Q4A<X> a[RT][4];
+};
+
+// RT row tiles of 16, C column tiles of 16 for a wave, GB groups a block, PF blocks in flight.  The
+// waves of a workgroup take stretches of k and are summed in LDS in the order of k.
+template <int X, int RT, int C, int GB, int PF>
+__global__ __launch_bounds__(512) void q4_mm(Q4P p) {
+    extern __shared__ __align__(16) q4_f32x4 q4_red[];  // [waves][RT][C][64]
+    const int nw = blockDim.x >> 6, w = wave_id(), l = threadIdx.x & 63, col = l & 15, kq = l >> 4;
+    const int j0 = blockIdx.x * C;
+    const int64_t m0 = (int64_t)blockIdx.y * (16 * RT);
+    const int per = (p.w.KB + nw - 1) / nw, kb0 = min(p.w.KB, w * per), kb1 = min(p.w.KB, kb0 + per);
+    using A = Q4A<X>;
+    const char* xrow[RT];
+    bool on[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int64_t m = m0 + 16 * i + col;  // an operand's row is the lane's low four bits, as a weight's column is
+        on[i] = m < p.rows;
+        xrow[i] = static_cast<const char*>(p.x) + (on[i] ? m : 0) * p.x_ld * A::kSize;
+    }
+    auto load = [&](Q4Block<X, RT, C, GB>& b, int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int j = min(j0 + c, p.w.NT - 1);
+            b.w[c] = p.w.codes[((int64_t)j * p.w.KB + kb) * 64 + l];
+            const int64_t at = ((int64_t)j * p.w.NG + (int64_t)kb * GB) * kQ4N + col;
+#pragma unroll
+            for (int g = 0; g < GB; ++g) {
+                b.scale[c][g] = p.w.sbf16 ? bf16_to_f32(static_cast<const bf16_t*>(p.w.scale)[at + g * kQ4N]) : static_cast<const float*>(p.w.scale)[at + g * kQ4N];
+                b.zero[c][g] = p.w.zeros ? (float)p.w.zero[at + g * kQ4N] : 8.f;
             }
         }
-        total += __shfl_xor(total, 16, 64);
-        total += __shfl_xor(total, 32, 64);
-        if (kq == 0 && n < p.w.N) {
-            if (p.xs) total *= p.xs[m];
-            if (p.bias) total += p.bias[n];
-            if (p.ybf16) store_f32<bf16_t>(static_cast<bf16_t*>(p.y) + m * p.y_ld + n, total);
-            else static_cast<float*>(p.y)[m * p.y_ld + n] = total;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                const int k = kb * kQ4K + 32 * st + 8 * kq;
+                b.a[i][st].zero();
+                if (on[i] && k < p.K8) b.a[i][st].load(xrow[i] + (int64_t)k * A::kSize);
+            }
+    };
+    q4_f32x4 tot[RT][C];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) tot[i][c] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
+    auto step = [&](const Q4Block<X, RT, C, GB>& b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < GB; ++g) {
+            if constexpr (X == Q4_I8) {
+                q4_i32x4 acc[RT][C], sx[RT];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    sx[i] = q4_i32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int c = 0; c < C; ++c) acc[i][c] = q4_i32x4{0, 0, 0, 0};
+                }
+#pragma unroll
+                for (int st = g * 4 / GB; st < (g + 1) * 4 / GB; ++st) {
+                    long a[RT];
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) {
+                        a[i] = b.a[i][st].part(0);
+                        sx[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(a[i], 0x0101010101010101l, sx[i], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        const long q = q4_codes_i8((&b.w[c].x)[st]);
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) acc[i][c] = __builtin_amdgcn_mfma_i32_16x16x32_i8(a[i], q, acc[i][c], 0, 0, 0);
+                    }
+                }
+                // whole numbers below 2^24 (128 x 127 x 15): exact up to the scale
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int c = 0; c < C; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            tot[i][c][e] = __builtin_fmaf(b.scale[c][g], (float)(acc[i][c][e] - (int)b.zero[c][g] * sx[i][e]), tot[i][c][e]);
+            } else {
+                const uint4 one4 = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+                const q4_bf16x8 one = __builtin_bit_cast(q4_bf16x8, one4);
+                q4_f32x4 acc[RT][C], sx[RT];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    sx[i] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < C; ++c) acc[i][c] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+#pragma unroll
+                for (int st = g * 4 / GB; st < (g + 1) * 4 / GB; ++st) {
+                    q4_bf16x8 q[C];
+#pragma unroll
+                    for (int c = 0; c < C; ++c) q[c] = q4_codes_bf16((&b.w[c].x)[st]);
+#pragma unroll
+                    for (int i = 0; i < RT; ++i)
+#pragma unroll
+                        for (int k = 0; k < A::kParts; ++k) {
+                            const q4_bf16x8 a = b.a[i][st].part(k);
+                            sx[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, one, sx[i], 0, 0, 0);
+#pragma unroll
+                            for (int c = 0; c < C; ++c) acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[c], acc[i][c], 0, 0, 0);
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int c = 0; c < C; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            tot[i][c][e] = __builtin_fmaf(b.scale[c][g], __builtin_fmaf(-16.f - b.zero[c][g], sx[i][e], acc[i][c][e]), tot[i][c][e]);
+            }
+        }
+    };
+    Q4Block<X, RT, C, GB> b[PF];
+#pragma unroll
+    for (int i = 0; i < PF; ++i)
+        if (kb0 + i < kb1) load(b[i], kb0 + i);
+    for (int kb = kb0; kb < kb1; kb += PF) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i)
+            if (kb + i < kb1) {
+                step(b[i]);
+                if (kb + i + PF < kb1) load(b[i], kb + i + PF);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) q4_red[((w * RT + i) * C + c) * 64 + l] = tot[i][c];
+    __syncthreads();
+    for (int u = w; u < RT * C; u += nw) {  // one wave a tile
+        const int i = u / C, c = u - i * C, n = (j0 + c) * kQ4N + col;
+        q4_f32x4 s = q4_red[(i * C + c) * 64 + l];
+        for (int k = 1; k < nw; ++k) s += q4_red[((k * RT + i) * C + c) * 64 + l];
+        if (n >= p.w.N) continue;
+        const float bias = p.bias ? p.bias[n] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t m = m0 + 16 * i + 4 * kq + e;
+            if (m >= p.rows) continue;
+            float v = s[e];
+            if (X == Q4_I8) v *= p.xs[m];
+            if (p.bias) v += bias;
+            if (p.ybf16) store_f32<bf16_t>(static_cast<bf16_t*>(p.y) + m * p.y_ld + n, v);
+            else static_cast<float*>(p.y)[m * p.y_ld + n] = v;
         }
     }
+}
+
+// Rows of a width that is no multiple of 8, copied with zeros behind them.
+template <typename T>
+__global__ __launch_bounds__(256) void q4_pad(const T* x, int64_t ld, int64_t rows, int K, int K8, T* out) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * K8; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / K8;
+        const int k = (int)(i - m * K8);
+        out[i] = k < K ? x[m * ld + k] : T(0);
+    }
+}
+
+template <int X, int RT, int C, int GB, int PF>
+static void q4_launch(const Q4P& p, int nw, hipStream_t s) {
+    const dim3 grid(ceil_div(p.w.NT, C), (uint32_t)((p.rows + 16 * RT - 1) / (16 * RT)));
+    hipLaunchKernelGGL((q4_mm<X, RT, C, GB, PF>), grid, dim3(64 * nw), (size_t)nw * RT * C * 64 * 16, s, p);
+}
+template <int X, int GB>
+static void q4_shape(const Q4P& p, hipStream_t s) {
+    const int C = p.rows <= 4 ? 1 : 2;
+    // waves: some 2048 in all, each with two blocks at least
+    int nw = 4;
+    while (nw < 8 && (int64_t)ceil_div(p.w.NT, C) * nw < 2048 && p.w.KB >= 4 * nw) nw *= 2;
+    if (p.rows <= 4) q4_launch<X, 1, 1, GB, X == Q4_F32 ? 2 : 4>(p, nw, s);
+    else if (p.rows <= 16) q4_launch<X, 1, 2, GB, 2>(p, nw, s);
+    else if (p.rows <= 32 || X == Q4_F32) q4_launch<X, 2, 2, GB, X == Q4_F32 ? 1 : 2>(p, nw, s);
+    else if constexpr (X != Q4_F32) q4_launch<X, 4, 2, GB, 1>(p, 4, s);
+}
+template <int X>
+static void q4_dispatch(const Q4P& p, hipStream_t s) {
+    if (p.w.G == 128) q4_shape<X, 1>(p, s);
+    else if (p.w.G == 64) q4_shape<X, 2>(p, s);
+    else q4_shape<X, 4>(p, s);
 }
 
 }  // namespace mamba
@@ -165,14 +371,17 @@ static int q4_check(const mamba_linear_q4_args* a, Q4P* out) {
     MAMBA_CHECK_ARG((a->x_dtype == MAMBA_INT8) == (a->x_scale != nullptr) || a->rows == 0, "x_scale goes with rows of int8");
     p.rows = a->rows; p.x = a->x; p.x_ld = a->x_ld; p.xs = a->x_scale; p.bias = a->bias;
     p.y = a->y; p.y_ld = a->y_ld; p.ybf16 = a->y_dtype == MAMBA_BF16;
+    p.K8 = (p.w.K + 7) / 8 * 8;
+    MAMBA_CHECK_ARG((p.rows + 15) / 16 <= 65535, "rows must be at most 1048560");
     *out = p;
     return MAMBA_OK;
 }
+static int q4_xsize(int x_dtype) { return x_dtype == MAMBA_F32 ? 4 : x_dtype == MAMBA_BF16 ? 2 : 1; }
 
 extern "C" size_t mamba_linear_q4_workspace_size(const mamba_linear_q4_args* a) {
     Q4P p;
     if (q4_check(a, &p) != MAMBA_OK) return 0;
-    return 0;
+    return p.K8 == p.w.K ? 0 : (size_t)p.rows * p.K8 * q4_xsize(a->x_dtype);
 }
 
 extern "C" int mamba_linear_q4_fwd(const mamba_linear_q4_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {
@@ -183,13 +392,28 @@ extern "C" int mamba_linear_q4_fwd(const mamba_linear_q4_args* a, void* ws, size
     MAMBA_CHECK_ARG(a->w.packed && p.x && p.y, "packed, x and y are required");
     MAMBA_CHECK_ARG(((uintptr_t)a->w.packed & 15u) == 0, "packed must be 16-byte aligned");
     MAMBA_CHECK_ARG(p.y_ld >= p.w.N || p.rows == 1, "rows of y overlap");
-    const size_t ex = a->x_dtype == MAMBA_F32 ? 4 : a->x_dtype == MAMBA_BF16 ? 2 : 1, ey = p.ybf16 ? 2 : 4;
+    const size_t ex = q4_xsize(a->x_dtype), ey = p.ybf16 ? 2 : 4;
     const char *px = static_cast<const char*>(p.x), *py = static_cast<const char*>(p.y);
     MAMBA_CHECK_ARG(py + ((p.rows - 1) * p.y_ld + p.w.N) * ey <= px || px + ((p.rows - 1) * p.x_ld + p.w.K) * ex <= py, "y overlaps x");
-    const dim3 grid(p.w.NT, (uint32_t)std::min<int64_t>(p.rows, 1024));
-    if (a->x_dtype == MAMBA_F32) hipLaunchKernelGGL(q4_rows<float>, grid, dim3(64), 0, (hipStream_t)stream, p);
-    else if (a->x_dtype == MAMBA_BF16) hipLaunchKernelGGL(q4_rows<bf16_t>, grid, dim3(64), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(q4_rows<int8_t>, grid, dim3(64), 0, (hipStream_t)stream, p);
+    hipStream_t s = (hipStream_t)stream;
+    const size_t need = mamba_linear_q4_workspace_size(a);
+    MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");
+    if (need && (ws == nullptr || ws_bytes < need)) {
+        set_error("mamba_linear_q4_fwd: workspace missing or too small");
+        return MAMBA_ERR_WORKSPACE;
+    }
+    if (need) {
+        const dim3 grid((uint32_t)std::min<int64_t>((p.rows * p.K8 + 255) / 256, 4096));
+        if (ex == 4) hipLaunchKernelGGL(q4_pad<uint32_t>, grid, dim3(256), 0, s, (const uint32_t*)p.x, p.x_ld, p.rows, p.w.K, p.K8, (uint32_t*)ws);
+        else if (ex == 2) hipLaunchKernelGGL(q4_pad<uint16_t>, grid, dim3(256), 0, s, (const uint16_t*)p.x, p.x_ld, p.rows, p.w.K, p.K8, (uint16_t*)ws);
+        else hipLaunchKernelGGL(q4_pad<uint8_t>, grid, dim3(256), 0, s, (const uint8_t*)p.x, p.x_ld, p.rows, p.w.K, p.K8, (uint8_t*)ws);
+        MAMBA_CHECK_LAUNCH();
+        p.x = ws;
+        p.x_ld = p.K8;
+    }
+    if (a->x_dtype == MAMBA_F32) q4_dispatch<Q4_F32>(p, s);
+    else if (a->x_dtype == MAMBA_BF16) q4_dispatch<Q4_BF16>(p, s);
+    else q4_dispatch<Q4_I8>(p, s);
     MAMBA_CHECK_LAUNCH();
     return MAMBA_OK;
 }

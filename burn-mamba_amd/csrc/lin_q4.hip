@@ -21,30 +21,27 @@ struct Q4W {
     int KB, NT, NG;         // blocks along k, column tiles, groups along k (padded to whole blocks)
     bool zeros, sbf16;
     const uint4* codes;     // [NT][KB][64]
-    const void* scale;      // [NT][NG][16]
-    const uint8_t* zero;    // [NT][NG][16]
+    const void* scale;      // [NT][NG][16] words of 4 (bf16 scales) or 8 bytes
 };
 
 static bool q4_make(const mamba_q4_weight* w, Q4W* o, size_t* bytes) {
-    if (w == nullptr || w->d_in < 1 || w->d_out < 1 || w->d_in > (1 << 24) || w->d_out > (1 << 24)) return false;
+    if (w == nullptr || w->d_in < 1 || w->d_out < 1 || w->d_in > (1 << 22) || w->d_out > (1 << 24)) return false;
     if (w->group != 32 && w->group != 64 && w->group != 128) return false;
     if (w->scale_dtype != MAMBA_F32 && w->scale_dtype != MAMBA_BF16) return false;
     Q4W q{};
     q.K = w->d_in; q.N = w->d_out; q.G = w->group;
     q.KB = ceil_div(q.K, kQ4K); q.NT = ceil_div(q.N, kQ4N); q.NG = q.KB * (kQ4K / q.G);
     q.zeros = w->has_zero != 0; q.sbf16 = w->scale_dtype == MAMBA_BF16;
-    const size_t codes = (size_t)q.NT * q.KB * 1024, scales = align_up((size_t)q.NT * q.NG * kQ4N * (q.sbf16 ? 2 : 4), 256);
+    const size_t codes = (size_t)q.NT * q.KB * 1024;
     const char* base = static_cast<const char*>(w->packed);
     q.codes = reinterpret_cast<const uint4*>(base);
     q.scale = base + codes;
-    q.zero = reinterpret_cast<const uint8_t*>(base + codes + scales);
     *o = q;
-    *bytes = codes + scales + (q.zeros ? (size_t)q.NT * q.NG * kQ4N : 0);
+    *bytes = codes + (size_t)q.NT * q.NG * kQ4N * (q.sbf16 ? 4 : 8);
     return true;
 }
 
-__global__ __launch_bounds__(256) void q4_pack(Q4W w, const uint8_t* codes, const void* scale, const uint8_t* zero, uint32_t* out, void* oscale,
-                                               uint8_t* ozero) {
+__global__ __launch_bounds__(256) void q4_pack(Q4W w, const uint8_t* codes, const void* scale, const uint8_t* zero, uint32_t* out, void* oscale) {
     const int64_t step = (int64_t)gridDim.x * 256, at0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
     // column-major in the threads, so that neighbours read neighbouring codes
     for (int64_t i = at0; i < (int64_t)w.NT * w.KB * 256; i += step) {
@@ -68,9 +65,9 @@ __global__ __launch_bounds__(256) void q4_pack(Q4W w, const uint8_t* codes, cons
         const int col = (int)(i % 16), g = (int)(i / 16 % w.NG), n = (int)(i / 16 / w.NG) * kQ4N + col;
         const bool in = g < groups && n < w.N;
         const int64_t src = (int64_t)g * w.N + n;
-        if (w.sbf16) static_cast<bf16_t*>(oscale)[i] = in ? static_cast<const bf16_t*>(scale)[src] : (bf16_t)0;
-        else static_cast<float*>(oscale)[i] = in ? static_cast<const float*>(scale)[src] : 0.f;
-        if (ozero) ozero[i] = in ? zero[src] & 15 : 0;
+        const float z = 16.f + (in ? (zero ? zero[src] & 15 : 8) : 0);
+        if (w.sbf16) static_cast<uint32_t*>(oscale)[i] = (in ? (uint32_t)static_cast<const bf16_t*>(scale)[src] << 16 : 0u) | __float_as_uint(z) >> 16;
+        else static_cast<float2*>(oscale)[i] = make_float2(in ? static_cast<const float*>(scale)[src] : 0.f, z);
     }
 }
 
@@ -90,31 +87,31 @@ typedef int q4_i32x4 __attribute__((ext_vector_type(4)));
 
 enum Q4X { Q4_BF16 = 0, Q4_F32 = 1, Q4_I8 = 2 };
 
-// Lane l's operand of 32 k of 16 rows: row l % 16, k 8 (l / 16) .. + 7.  f32 rows are three bf16
-// parts, each the upper half of what the ones before leave (8 bits of the 24), lowest first.
+// Lane l's operand of 32 k of 16 rows: row l % 16, k 8 (l / 16) .. + 7, loaded through a buffer
+// resource (an offset past its extent reads zeros).  f32 rows are three bf16 parts, each the
+// upper half of what the ones before leave (8 bits of the 24).
 template <int X> struct Q4A;
 template <> struct Q4A<Q4_BF16> {
     static constexpr int kParts = 1, kSize = 2;
     uint4 v;
-    __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void load(const char* p) { __builtin_memcpy(&v, p, 16); }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t soff) { v = buf_ld16(r, off, soff); }
     __device__ __forceinline__ q4_bf16x8 part(int) const { return __builtin_bit_cast(q4_bf16x8, v); }
 };
 template <> struct Q4A<Q4_F32> {
     static constexpr int kParts = 3, kSize = 4;
-    float v[8];
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    uint4 v[2];
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t soff) {
+        v[0] = buf_ld16(r, off, soff);
+        v[1] = buf_ld16(r, off + 16, soff);
     }
-    __device__ __forceinline__ void load(const char* p) { __builtin_memcpy(v, p, 32); }
     __device__ __forceinline__ q4_bf16x8 part(int k) const {
+        const uint32_t u[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
         uint32_t d[4];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float r = v[i];
+            float r = __uint_as_float(u[i]);
 #pragma unroll
-            for (int j = k; j < 2; ++j) r -= __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+            for (int j = 0; j < k; ++j) r -= __uint_as_float(__float_as_uint(r) & 0xffff0000u);
             const uint32_t h = __float_as_uint(r) >> 16;
             d[i / 2] = i & 1 ? d[i / 2] | h << 16 : h;
         }
@@ -124,8 +121,9 @@ template <> struct Q4A<Q4_F32> {
 template <> struct Q4A<Q4_I8> {
     static constexpr int kParts = 1, kSize = 1;
     uint2 v;
-    __device__ __forceinline__ void zero() { v = make_uint2(0, 0); }
-    __device__ __forceinline__ void load(const char* p) { __builtin_memcpy(&v, p, 8); }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t soff) {
+        v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, (int)__builtin_amdgcn_readfirstlane(soff), 0));
+    }
     // in the order in which the codes' bytes come: 0 4 1 5 2 6 3 7
     __device__ __forceinline__ long part(int) const {
         return (long)((uint64_t)__builtin_amdgcn_perm(v.y, v.x, 0x07030602u) << 32 | __builtin_amdgcn_perm(v.y, v.x, 0x05010400u));
@@ -133,41 +131,48 @@ template <> struct Q4A<Q4_I8> {
 };
 
 // The codes of a dword, as operands.  A bf16 whose upper four bits of mantissa are the code
-// is 16 + code: one shift and one and-or a pair.
+// is 16 + code: one shift and one and-or a pair.  A byte whose upper four bits are code ^ 8 is
+// 16 (code - 8).
 __device__ __forceinline__ q4_bf16x8 q4_codes_bf16(uint32_t w) {
     const uint32_t d[4] = {(w << 3 & 0x00780078u) | 0x41804180u, (w >> 1 & 0x00780078u) | 0x41804180u, (w >> 5 & 0x00780078u) | 0x41804180u,
                            (w >> 9 & 0x00780078u) | 0x41804180u};
     return __builtin_bit_cast(q4_bf16x8, d);
 }
-__device__ __forceinline__ long q4_codes_i8(uint32_t w) { return (long)((uint64_t)(w >> 4 & 0x0f0f0f0fu) << 32 | (w & 0x0f0f0f0fu)); }
+__device__ __forceinline__ long q4_codes_i8(uint32_t w) {
+    return (long)((uint64_t)((w & 0xf0f0f0f0u) ^ 0x80808080u) << 32 | ((w << 4 & 0xf0f0f0f0u) ^ 0x80808080u));
+}
 
-// One block of C column tiles and RT row tiles, in flight.
-template <int X, int RT, int C, int GB>
-struct Q4Block {
+// What a wave has in flight: a block of C column tiles, and the rows' operands of a block.
+template <int C, int GB, bool SF>
+struct Q4Codes {
     uint4 w[C];
-    float scale[C][GB], zero[C][GB];
-    Q4A<X> a[RT][4];
+    uint32_t s[C][GB];
+    float sf[C][SF ? GB : 1], zf[C][SF ? GB : 1];
 };
+template <int X, int RT>
+struct Q4Rows { Q4A<X> a[RT][4]; };
 
-// RT row tiles of 16, C column tiles of 16 for a wave, GB groups a block, PF blocks in flight.  The
-// waves of a workgroup take stretches of k and are summed in LDS in the order of k.
-template <int X, int RT, int C, int GB, int PF>
+constexpr uint32_t kQ4Out = 0x80000000u;  // past every extent
+
+// RT row tiles of 16, C column tiles of 16 for a wave, GB groups a block, PW blocks of codes and PA of
+// rows in flight, scales f32 (SF) or bf16.  The waves of a workgroup take stretches of k and are
+// summed in LDS in the order of k.
+template <int X, int RT, int C, int GB, int PW, int PA, bool SF>
 __global__ __launch_bounds__(512) void q4_mm(Q4P p) {
     extern __shared__ __align__(16) q4_f32x4 q4_red[];  // [waves][RT][C][64]
+    static_assert(PW % PA == 0, "the rings turn together");
     const int nw = blockDim.x >> 6, w = wave_id(), l = threadIdx.x & 63, col = l & 15, kq = l >> 4;
     const int j0 = blockIdx.x * C;
     const int64_t m0 = (int64_t)blockIdx.y * (16 * RT);
     const int per = (p.w.KB + nw - 1) / nw, kb0 = min(p.w.KB, w * per), kb1 = min(p.w.KB, kb0 + per);
     using A = Q4A<X>;
-    const char* xrow[RT];
-    bool on[RT];
+    const int here = (int)min((int64_t)16 * RT, p.rows - m0);  // rows of this workgroup
+    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(static_cast<const char*>(p.x) + m0 * p.x_ld * A::kSize,
+                                               (uint32_t)(((here - 1) * p.x_ld + p.K8) * A::kSize));
+    uint32_t off[RT];  // of the lane's row and k; an operand's row is the lane's low four bits, as a weight's column is
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const int64_t m = m0 + 16 * i + col;  // an operand's row is the lane's low four bits, as a weight's column is
-        on[i] = m < p.rows;
-        xrow[i] = static_cast<const char*>(p.x) + (on[i] ? m : 0) * p.x_ld * A::kSize;
-    }
-    auto load = [&](Q4Block<X, RT, C, GB>& b, int kb) __attribute__((always_inline)) {
+    for (int i = 0; i < RT; ++i) off[i] = 16 * i + col < here ? (uint32_t)((16 * i + col) * p.x_ld + 8 * kq) * A::kSize : kQ4Out;
+    auto load_codes = [&](Q4Codes<C, GB, SF>& b, int kb) __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int j = min(j0 + c, p.w.NT - 1);
@@ -175,27 +180,39 @@ __global__ __launch_bounds__(512) void q4_mm(Q4P p) {
             const int64_t at = ((int64_t)j * p.w.NG + (int64_t)kb * GB) * kQ4N + col;
 #pragma unroll
             for (int g = 0; g < GB; ++g) {
-                b.scale[c][g] = p.w.sbf16 ? bf16_to_f32(static_cast<const bf16_t*>(p.w.scale)[at + g * kQ4N]) : static_cast<const float*>(p.w.scale)[at + g * kQ4N];
-                b.zero[c][g] = p.w.zeros ? (float)p.w.zero[at + g * kQ4N] : 8.f;
+                if constexpr (SF) {
+                    const float2 v = static_cast<const float2*>(p.w.scale)[at + g * kQ4N];
+                    b.sf[c][g] = v.x;
+                    b.zf[c][g] = v.y;
+                } else {
+                    b.s[c][g] = static_cast<const uint32_t*>(p.w.scale)[at + g * kQ4N];
+                }
             }
         }
+    };
+    auto load_rows = [&](Q4Rows<X, RT>& b, int kb) __attribute__((always_inline)) {
+        const bool last = (kb + 1) * kQ4K > p.K8;  // runs of 8 behind the rows' end read zeros
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+        for (int st = 0; st < 4; ++st) {
+            const bool out = last && kb * kQ4K + 32 * st + 8 * kq >= p.K8;
 #pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                const int k = kb * kQ4K + 32 * st + 8 * kq;
-                b.a[i][st].zero();
-                if (on[i] && k < p.K8) b.a[i][st].load(xrow[i] + (int64_t)k * A::kSize);
-            }
+            for (int i = 0; i < RT; ++i) b.a[i][st].load(rx, (out ? kQ4Out : off[i]) + 32 * st * A::kSize, (uint32_t)(kb * kQ4K * A::kSize));
+        }
     };
     q4_f32x4 tot[RT][C];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int c = 0; c < C; ++c) tot[i][c] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
-    auto step = [&](const Q4Block<X, RT, C, GB>& b) __attribute__((always_inline)) {
+    auto step = [&](const Q4Codes<C, GB, SF>& b, const Q4Rows<X, RT>& x) __attribute__((always_inline)) {
 #pragma unroll
         for (int g = 0; g < GB; ++g) {
+            float scale[C], zero[C];  // zero: 16 + the zero point
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                scale[c] = SF ? b.sf[c][SF ? g : 0] : __uint_as_float(b.s[c][g] & 0xffff0000u);
+                zero[c] = SF ? b.zf[c][SF ? g : 0] : __uint_as_float(b.s[c][g] << 16);
+            }
             if constexpr (X == Q4_I8) {
                 q4_i32x4 acc[RT][C], sx[RT];
 #pragma unroll
@@ -208,9 +225,10 @@ __global__ __launch_bounds__(512) void q4_mm(Q4P p) {
                 for (int st = g * 4 / GB; st < (g + 1) * 4 / GB; ++st) {
                     long a[RT];
 #pragma unroll
-                    for (int i = 0; i < RT; ++i) {
-                        a[i] = b.a[i][st].part(0);
-                        sx[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(a[i], 0x0101010101010101l, sx[i], 0, 0, 0);
+                    for (int i = 0; i < RT; ++i) a[i] = x.a[i][st].part(0);
+                    if (p.w.zeros) {
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) sx[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(a[i], 0x0101010101010101l, sx[i], 0, 0, 0);
                     }
 #pragma unroll
                     for (int c = 0; c < C; ++c) {
@@ -219,14 +237,23 @@ __global__ __launch_bounds__(512) void q4_mm(Q4P p) {
                         for (int i = 0; i < RT; ++i) acc[i][c] = __builtin_amdgcn_mfma_i32_16x16x32_i8(a[i], q, acc[i][c], 0, 0, 0);
                     }
                 }
-                // whole numbers below 2^24 (128 x 127 x 15): exact up to the scale
+                // whole numbers of at most 128 x 127 x 128 < 2^24: exact up to the scale
+                if (p.w.zeros) {
 #pragma unroll
-                for (int i = 0; i < RT; ++i)
+                    for (int c = 0; c < C; ++c) {
+                        const int z = 16 * ((int)zero[c] - 24);
 #pragma unroll
-                    for (int c = 0; c < C; ++c)
+                        for (int i = 0; i < RT; ++i) acc[i][c] -= z * sx[i];
+                    }
+                }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            tot[i][c][e] = __builtin_fmaf(b.scale[c][g], (float)(acc[i][c][e] - (int)b.zero[c][g] * sx[i][e]), tot[i][c][e]);
+                for (int c = 0; c < C; ++c) {
+                    const float s16 = scale[c] * 0.0625f;
+#pragma unroll
+                    for (int i = 0; i < RT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) tot[i][c][e] = __builtin_fmaf(s16, (float)acc[i][c][e], tot[i][c][e]);
+                }
             } else {
                 const uint4 one4 = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
                 const q4_bf16x8 one = __builtin_bit_cast(q4_bf16x8, one4);
@@ -245,8 +272,8 @@ __global__ __launch_bounds__(512) void q4_mm(Q4P p) {
 #pragma unroll
                     for (int i = 0; i < RT; ++i)
 #pragma unroll
-                        for (int k = 0; k < A::kParts; ++k) {
-                            const q4_bf16x8 a = b.a[i][st].part(k);
+                        for (int k = A::kParts - 1; k >= 0; --k) {  // the lowest part first
+                            const q4_bf16x8 a = x.a[i][st].part(k);
                             sx[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, one, sx[i], 0, 0, 0);
 #pragma unroll
                             for (int c = 0; c < C; ++c) acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[c], acc[i][c], 0, 0, 0);
@@ -258,20 +285,25 @@ __global__ __launch_bounds__(512) void q4_mm(Q4P p) {
                     for (int c = 0; c < C; ++c)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            tot[i][c][e] = __builtin_fmaf(b.scale[c][g], __builtin_fmaf(-16.f - b.zero[c][g], sx[i][e], acc[i][c][e]), tot[i][c][e]);
+                            tot[i][c][e] = __builtin_fmaf(scale[c], __builtin_fmaf(-zero[c], sx[i][e], acc[i][c][e]), tot[i][c][e]);
             }
         }
     };
-    Q4Block<X, RT, C, GB> b[PF];
+    Q4Codes<C, GB, SF> b[PW];
+    Q4Rows<X, RT> x[PA];
 #pragma unroll
-    for (int i = 0; i < PF; ++i)
-        if (kb0 + i < kb1) load(b[i], kb0 + i);
-    for (int kb = kb0; kb < kb1; kb += PF) {
+    for (int i = 0; i < PW; ++i)
+        if (kb0 + i < kb1) load_codes(b[i], kb0 + i);
 #pragma unroll
-        for (int i = 0; i < PF; ++i)
+    for (int i = 0; i < PA; ++i)
+        if (kb0 + i < kb1) load_rows(x[i], kb0 + i);
+    for (int kb = kb0; kb < kb1; kb += PW) {
+#pragma unroll
+        for (int i = 0; i < PW; ++i)
             if (kb + i < kb1) {
-                step(b[i]);
-                if (kb + i + PF < kb1) load(b[i], kb + i + PF);
+                step(b[i], x[i % PA]);
+                if (kb + i + PA < kb1) load_rows(x[i % PA], kb + i + PA);
+                if (kb + i + PW < kb1) load_codes(b[i], kb + i + PW);
             }
     }
 #pragma unroll
@@ -298,7 +330,8 @@ __global__ __launch_bounds__(512) void q4_mm(Q4P p) {
     }
 }
 
-// Rows of a width that is no multiple of 8, copied with zeros behind them.
+// Rows of a width that is no multiple of 8 (or too far apart for the buffer's offsets), copied with
+// zeros behind them.
 template <typename T>
 __global__ __launch_bounds__(256) void q4_pad(const T* x, int64_t ld, int64_t rows, int K, int K8, T* out) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * K8; i += (int64_t)gridDim.x * 256) {
@@ -308,21 +341,21 @@ __global__ __launch_bounds__(256) void q4_pad(const T* x, int64_t ld, int64_t ro
     }
 }
 
-template <int X, int RT, int C, int GB, int PF>
+template <int X, int RT, int C, int GB, int PW, int PA>
 static void q4_launch(const Q4P& p, int nw, hipStream_t s) {
-    const dim3 grid(ceil_div(p.w.NT, C), (uint32_t)((p.rows + 16 * RT - 1) / (16 * RT)));
-    hipLaunchKernelGGL((q4_mm<X, RT, C, GB, PF>), grid, dim3(64 * nw), (size_t)nw * RT * C * 64 * 16, s, p);
+    const dim3 grid(ceil_div(p.w.NT, C), (uint32_t)((p.rows + 16 * RT - 1) / (16 * RT))), block(64 * nw);
+    const size_t lds = (size_t)nw * RT * C * 64 * 16;
+    if (p.w.sbf16) hipLaunchKernelGGL((q4_mm<X, RT, C, GB, PW, PA, false>), grid, block, lds, s, p);
+    else hipLaunchKernelGGL((q4_mm<X, RT, C, GB, PW, PA, true>), grid, block, lds, s, p);
 }
 template <int X, int GB>
 static void q4_shape(const Q4P& p, hipStream_t s) {
-    const int C = p.rows <= 4 ? 1 : 2;
     // waves: some 2048 in all, each with two blocks at least
     int nw = 4;
-    while (nw < 8 && (int64_t)ceil_div(p.w.NT, C) * nw < 2048 && p.w.KB >= 4 * nw) nw *= 2;
-    if (p.rows <= 4) q4_launch<X, 1, 1, GB, X == Q4_F32 ? 2 : 4>(p, nw, s);
-    else if (p.rows <= 16) q4_launch<X, 1, 2, GB, 2>(p, nw, s);
-    else if (p.rows <= 32 || X == Q4_F32) q4_launch<X, 2, 2, GB, X == Q4_F32 ? 1 : 2>(p, nw, s);
-    else if constexpr (X != Q4_F32) q4_launch<X, 4, 2, GB, 1>(p, 4, s);
+    while (nw < 8 && (int64_t)p.w.NT * nw < 2048 && p.w.KB >= 4 * nw) nw *= 2;
+    if (p.rows <= 16) q4_launch<X, 1, 1, GB, X == Q4_F32 ? 4 : 6, X == Q4_F32 ? 1 : 2>(p, nw, s);
+    else if (p.rows <= 32 || X == Q4_F32) q4_launch<X, 2, 2, GB, 2, X == Q4_F32 ? 1 : 2>(p, nw, s);
+    else if constexpr (X != Q4_F32) q4_launch<X, 4, 2, GB, 2, X == Q4_BF16 ? 1 : 2>(p, 4, s);
 }
 template <int X>
 static void q4_dispatch(const Q4P& p, hipStream_t s) {
@@ -330,12 +363,14 @@ static void q4_dispatch(const Q4P& p, hipStream_t s) {
     else if (p.w.G == 64) q4_shape<X, 2>(p, s);
     else q4_shape<X, 4>(p, s);
 }
+// Rows that are read in place: whole runs of 8, and 64 of them within a buffer's offsets.
+static bool q4_in_place(const Q4P& p, int size) { return p.K8 == p.w.K && p.x_ld >= 0 && (63 * p.x_ld + p.K8) * size < (1ll << 31); }
 
 }  // namespace mamba
 
 using namespace mamba;
 
-#define Q4_SHAPE "d_in and d_out in [1, 2^24], group 32, 64 or 128 and scales of f32 or bf16 required"
+#define Q4_SHAPE "d_in in [1, 2^22], d_out in [1, 2^24], group 32, 64 or 128 and scales of f32 or bf16 required"
 
 extern "C" size_t mamba_linear_q4_packed_size(const mamba_q4_weight* w) {
     Q4W q;
@@ -355,7 +390,7 @@ extern "C" int mamba_linear_q4_pack(const mamba_q4_weight* w, const void* codes,
     MAMBA_CHECK_ARG(((uintptr_t)packed & 15u) == 0, "packed must be 16-byte aligned");
     const int64_t items = (int64_t)q.NT * q.KB * 256;
     hipLaunchKernelGGL(q4_pack, dim3((uint32_t)std::min<int64_t>((items + 255) / 256, 1 << 16)), dim3(256), 0, (hipStream_t)stream, q, (const uint8_t*)codes,
-                       scale, (const uint8_t*)zero, (uint32_t*)packed, const_cast<void*>(q.scale), q.zeros ? const_cast<uint8_t*>(q.zero) : nullptr);
+                       scale, (const uint8_t*)zero, (uint32_t*)packed, const_cast<void*>(q.scale));
     MAMBA_CHECK_LAUNCH();
     return MAMBA_OK;
 }
@@ -381,7 +416,7 @@ static int q4_xsize(int x_dtype) { return x_dtype == MAMBA_F32 ? 4 : x_dtype == 
 extern "C" size_t mamba_linear_q4_workspace_size(const mamba_linear_q4_args* a) {
     Q4P p;
     if (q4_check(a, &p) != MAMBA_OK) return 0;
-    return p.K8 == p.w.K ? 0 : (size_t)p.rows * p.K8 * q4_xsize(a->x_dtype);
+    return q4_in_place(p, q4_xsize(a->x_dtype)) ? 0 : (size_t)p.rows * p.K8 * q4_xsize(a->x_dtype);
 }
 
 extern "C" int mamba_linear_q4_fwd(const mamba_linear_q4_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {

@@ -284,7 +284,7 @@ def test_c_product():
         a = args()
         setattr(a, field, bad)
         assert L.mamba_linear_q4_fwd(ctypes.byref(a), None, 0, None) == 1 and what in L.mamba_last_error(), field
-    for field, bad in (("d_in", 0), ("d_out", 0), ("d_in", (1 << 24) + 1), ("group", 16), ("group", 0), ("scale_dtype", 2)):
+    for field, bad in (("d_in", 0), ("d_out", 0), ("d_in", (1 << 22) + 1), ("group", 16), ("group", 0), ("scale_dtype", 2)):
         a = args()
         setattr(a.w, field, bad)
         assert L.mamba_linear_q4_fwd(ctypes.byref(a), None, 0, None) == 1 and b"group 32" in L.mamba_last_error(), field
@@ -297,5 +297,7 @@ def test_c_product():
     assert L.mamba_linear_q4_pack(ctypes.byref(a.w), P, P, None, None, None) == 1
     a.w.has_zero = 1
     assert L.mamba_linear_q4_pack(ctypes.byref(a.w), P, P, None, P, None) == 1 and b"zero" in L.mamba_last_error()
-    # 2 blocks of k, 4 column tiles: codes, scales (to 256 bytes), zero points
-    assert L.mamba_linear_q4_packed_size(ctypes.byref(a.w)) == 4 * 2 * 1024 + 4 * 4 * 16 * 4 + 4 * 4 * 16
+    # 2 blocks of k, 4 column tiles: codes, and a word for each group's scale and zero point
+    assert L.mamba_linear_q4_packed_size(ctypes.byref(a.w)) == 4 * 2 * 1024 + 4 * 4 * 16 * 8
+    a.w.scale_dtype = 1
+    assert L.mamba_linear_q4_packed_size(ctypes.byref(a.w)) == 4 * 2 * 1024 + 4 * 4 * 16 * 4

@@ -142,192 +142,314 @@ __device__ __forceinline__ long q4_codes_i8(uint32_t w) {
     return (long)((uint64_t)((w & 0xf0f0f0f0u) ^ 0x80808080u) << 32 | ((w << 4 & 0xf0f0f0f0u) ^ 0x80808080u));
 }
 
-// What a wave has in flight: a block of C column tiles, and the rows' operands of a block.
-template <int C, int GB, bool SF>
-struct Q4Codes {
-    uint4 w[C];
-    uint32_t s[C][GB];
-    float sf[C][SF ? GB : 1], zf[C][SF ? GB : 1];
+// The rows' operands as the products take them, kept in registers: NP parts.
+template <int X>
+struct Q4Op {
+    static constexpr int kParts = Q4A<X>::kParts;
+    q4_bf16x8 v[kParts];
+    __device__ __forceinline__ void make(const Q4A<X>& a) {
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) v[k] = a.part(k);
+    }
+};
+template <>
+struct Q4Op<Q4_I8> {
+    static constexpr int kParts = 1;
+    long v[1];
+    __device__ __forceinline__ void make(const Q4A<Q4_I8>& a) { v[0] = a.part(0); }
+};
+
+// A group's products of RT row tiles with a column tile, scaled and added to tot: st0 .. st1 - 1 its
+// steps of 32 k, q(st) their codes' dword, x(i, st) the rows' operands, zero 16 + the zero point.
+template <int X, int RT, typename Q, typename Op>
+__device__ __forceinline__ void q4_group(int st0, int st1, float scale, float zero, bool zeros, Q q, Op x, q4_f32x4 (&tot)[RT]) {
+    if constexpr (X == Q4_I8) {
+        q4_i32x4 acc[RT], sx[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[i] = sx[i] = q4_i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int st = st0; st < st1; ++st) {
+            const long c = q4_codes_i8(q(st));
+#pragma unroll
+            for (int i = 0; i < RT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x(i, st).v[0], c, acc[i], 0, 0, 0);
+        }
+        // whole numbers of at most 128 x 127 x 128 < 2^24: exact up to the scale
+        if (zeros) {
+            const int z = 16 * ((int)zero - 24);
+#pragma unroll
+            for (int st = st0; st < st1; ++st)
+#pragma unroll
+                for (int i = 0; i < RT; ++i) sx[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x(i, st).v[0], 0x0101010101010101l, sx[i], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) acc[i] -= z * sx[i];
+        }
+        const float s16 = scale * 0.0625f;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tot[i][e] = __builtin_fmaf(s16, (float)acc[i][e], tot[i][e]);
+    } else {
+        const uint32_t z2 = __float_as_uint(-zero) >> 16 | (__float_as_uint(-zero) & 0xffff0000u);
+        const q4_bf16x8 off = __builtin_bit_cast(q4_bf16x8, make_uint4(z2, z2, z2, z2));  // a whole number up to 31: a bf16
+        q4_f32x4 acc[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[i] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = st0; st < st1; ++st) {
+            const q4_bf16x8 c = q4_codes_bf16(q(st));
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int k = Q4Op<X>::kParts - 1; k >= 0; --k) {  // the lowest part first
+                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x(i, st).v[k], c, acc[i], 0, 0, 0);
+                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x(i, st).v[k], off, acc[i], 0, 0, 0);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tot[i][e] = __builtin_fmaf(scale, acc[i][e], tot[i][e]);
+    }
+}
+
+// Column tile j through buffer resources (scalar bases, 32-bit offsets): blocks behind the last,
+// and tiles behind the last, read zeros.
+struct Q4Tile {
+    __amdgpu_buffer_rsrc_t codes, scale;
+    __device__ __forceinline__ Q4Tile(const Q4W& q, int j) {
+        const int64_t at = j < q.NT ? j : 0;
+        const uint32_t kb = j < q.NT ? q.KB : 0, words = q.NG * kQ4N * (q.sbf16 ? 4 : 8);
+        codes = buf_rsrc(q.codes + at * q.KB * 64, kb * 1024u);
+        scale = buf_rsrc(static_cast<const char*>(q.scale) + at * words, kb ? words : 0u);
+    }
+};
+// A block of a column tile: its codes, and its groups' scales and zero points.
+template <int GB, bool SF>
+struct Q4Block {
+    uint4 w;
+    uint32_t s[SF ? 1 : GB];
+    uint2 sf[SF ? GB : 1];
+    __device__ __forceinline__ void load(const Q4Tile& t, int kb, int l) {
+        w = buf_ld16(t.codes, l * 16, kb * 1024);
+#pragma unroll
+        for (int g = 0; g < GB; ++g) {
+            const int soff = kb * GB * kQ4N * (SF ? 8 : 4);
+            if constexpr (SF) sf[g] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(t.scale, (l & 15) * 8 + g * kQ4N * 8, soff, 0));
+            else s[g] = __builtin_amdgcn_raw_buffer_load_b32(t.scale, (l & 15) * 4 + g * kQ4N * 4, soff, 0);
+        }
+    }
+    __device__ __forceinline__ float scale(int g) const { return __uint_as_float(SF ? sf[SF ? g : 0].x : s[SF ? 0 : g] & 0xffff0000u); }
+    __device__ __forceinline__ float zero(int g) const { return __uint_as_float(SF ? sf[SF ? g : 0].y : s[SF ? 0 : g] << 16); }
+    __device__ __forceinline__ uint32_t dword(int st) const { return st == 0 ? w.x : st == 1 ? w.y : st == 2 ? w.z : w.w; }
+};
+
+// The rows of a workgroup and where a lane's operands of them lie.
+template <int X, int RT>
+struct Q4Src {
+    __amdgpu_buffer_rsrc_t r;
+    uint32_t off[RT];
+    int K8, kq;
+    __device__ __forceinline__ Q4Src(const Q4P& p, int64_t m0, int l) : K8(p.K8), kq(l >> 4) {
+        constexpr int e = Q4A<X>::kSize;
+        const int here = (int)min((int64_t)16 * RT, p.rows - m0), col = l & 15;  // an operand's row is the lane's low four bits, as a weight's column is
+        r = buf_rsrc(static_cast<const char*>(p.x) + m0 * p.x_ld * e, (uint32_t)(((here - 1) * p.x_ld + p.K8) * e));
+#pragma unroll
+        for (int i = 0; i < RT; ++i) off[i] = 16 * i + col < here ? (uint32_t)((16 * i + col) * p.x_ld + 8 * kq) * e : 0x80000000u;  // past every extent
+    }
+    // runs of 8 behind the rows' end, and blocks behind the last (kb = KB), read zeros
+    __device__ __forceinline__ void load(Q4A<X>& a, int i, int kb, int st) const {
+        constexpr int e = Q4A<X>::kSize;
+        const bool out = kb * kQ4K + 32 * st + 8 * kq >= K8;
+        a.load(r, (out ? 0x80000000u : off[i]) + 32 * st * e, out ? 0u : (uint32_t)(kb * kQ4K * e));
+    }
+};
+
+// A column's bias, and the scales of a lane's four rows of each row tile (1 but for int8 rows): through
+// buffer resources, 0 where there is none.
+struct Q4Bias {
+    __amdgpu_buffer_rsrc_t r;
+    __device__ __forceinline__ explicit Q4Bias(const Q4P& p) : r(buf_rsrc(p.bias, p.bias ? (uint32_t)p.w.N * 4u : 0u)) {}
+    __device__ __forceinline__ float at(int n) const { return buf_ld4(r, (uint32_t)n * 4u); }
 };
 template <int X, int RT>
-struct Q4Rows { Q4A<X> a[RT][4]; };
+struct Q4Scales {
+    float v[RT][4];
+    __device__ __forceinline__ Q4Scales(const Q4P& p, int64_t m0, int l) {
+        const int here = (int)min((int64_t)16 * RT, p.rows - m0);
+        const __amdgpu_buffer_rsrc_t r = buf_rsrc(p.xs + (X == Q4_I8 ? m0 : 0), X == Q4_I8 ? here * 4u : 0u);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = X == Q4_I8 ? buf_ld4(r, (16 * i + 4 * (l >> 4) + e) * 4) : 1.f;
+    }
+};
 
-constexpr uint32_t kQ4Out = 0x80000000u;  // past every extent
+// The sums of a row tile (the lane's column and four of its rows) as results.
+template <int X>
+__device__ __forceinline__ void q4_store(const Q4P& p, int64_t m0, int n, const q4_f32x4& s, const float (&xs)[4], float bias) {
+    if (n >= p.w.N) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int64_t m = m0 + e;
+        if (m >= p.rows) continue;
+        const float v = X == Q4_I8 ? __builtin_fmaf(s[e], xs[e], bias) : s[e] + bias;
+        if (p.ybf16) store_f32<bf16_t>(static_cast<bf16_t*>(p.y) + m * p.y_ld + n, v);
+        else static_cast<float*>(p.y)[m * p.y_ld + n] = v;
+    }
+}
 
-// RT row tiles of 16, C column tiles of 16 for a wave, GB groups a block, PW blocks of codes and PA of
-// rows in flight, scales f32 (SF) or bf16.  The waves of a workgroup take stretches of k and are
-// summed in LDS in the order of k.
-template <int X, int RT, int C, int GB, int PW, int PA, bool SF>
-__global__ __launch_bounds__(512) void q4_mm(Q4P p) {
+// The rows in registers: wave w holds the operands of RT row tiles for NK blocks of k, and the
+// workgroup's waves all of k.  It takes column tiles in turn; a block's registers are loaded for
+// the next tile as soon as this one's are used.  The waves' sums meet in LDS, in the order of k, in
+// two places by turns, so that a tile has one barrier.
+template <int X, int RT, int NK, int GB, bool SF>
+__global__ __launch_bounds__(768) void q4_held(Q4P p) {
+    extern __shared__ __align__(16) q4_f32x4 q4_red[];  // [2][waves][RT][64]
+    const int nw = blockDim.x >> 6, w = wave_id(), l = threadIdx.x & 63;
+    const int64_t m0 = (int64_t)blockIdx.y * (16 * RT);
+    const int kb0 = w * NK;
+    // No load has a branch of its own, behind which the compiler would wait for every load in
+    // flight; for the same reason the rows are waited for before the tiles' loop, and the blocks are
+    // loaded in the order of their use before it as in it.
+    const Q4Src<X, RT> src(p, m0, l);
+    Q4A<X> a[NK][RT][4];
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int st = 0; st < 4; ++st) src.load(a[k][i][st], i, min(kb0 + k, p.w.KB), st);
+    __builtin_amdgcn_sched_barrier(0);
+    Q4Block<GB, SF> b[NK];
+    {
+        const Q4Tile t(p.w, blockIdx.x);
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            b[k].load(t, kb0 + k, l);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    Q4Op<X> x[NK][RT][4];
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                x[k][i][st].make(a[k][i][st]);
+#pragma unroll
+                for (int e = 0; e < Q4Op<X>::kParts; ++e) asm volatile("" : "+v"(x[k][i][st].v[e]));
+            }
+    const Q4Bias bias(p);
+    Q4Scales<X, RT> xs(p, m0, l);
+    if constexpr (X == Q4_I8) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(xs.v[i][e]));
+    }
+    int turn = 0;
+    for (int j = blockIdx.x; j < p.w.NT; j += gridDim.x, ++turn) {
+        const Q4Tile next(p.w, j + gridDim.x);
+        const float add = bias.at(j * kQ4N + (l & 15));
+        q4_f32x4 tot[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) tot[i] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+#pragma unroll
+            for (int g = 0; g < GB; ++g)
+                q4_group<X, RT>(g * 4 / GB, (g + 1) * 4 / GB, b[k].scale(g), b[k].zero(g), p.w.zeros, [&](int st) { return b[k].dword(st); },
+                                [&](int i, int st) -> const Q4Op<X>& { return x[k][i][st]; }, tot);
+            // behind the block's last use, so that its registers are these
+            __builtin_amdgcn_sched_barrier(0);
+            b[k].load(next, kb0 + k, l);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        q4_f32x4* red = q4_red + (turn & 1) * nw * RT * 64;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) red[(w * RT + i) * 64 + l] = tot[i];
+        __syncthreads();
+        if (w != turn % nw) continue;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            q4_f32x4 s = red[i * 64 + l];
+            for (int k = 1; k < nw; ++k) s += red[(k * RT + i) * 64 + l];
+            q4_store<X>(p, m0 + 16 * i + 4 * (l >> 4), j * kQ4N + (l & 15), s, xs.v[i], add);
+        }
+    }
+}
+
+// Any k: RT row tiles with C column tiles, a wave walks a stretch of k with two blocks of codes and
+// one of rows in flight.
+template <int X, int RT, int C, int GB, bool SF>
+__global__ __launch_bounds__(512) void q4_walk(Q4P p) {
     extern __shared__ __align__(16) q4_f32x4 q4_red[];  // [waves][RT][C][64]
-    static_assert(PW % PA == 0, "the rings turn together");
-    const int nw = blockDim.x >> 6, w = wave_id(), l = threadIdx.x & 63, col = l & 15, kq = l >> 4;
+    const int nw = blockDim.x >> 6, w = wave_id(), l = threadIdx.x & 63;
     const int j0 = blockIdx.x * C;
     const int64_t m0 = (int64_t)blockIdx.y * (16 * RT);
     const int per = (p.w.KB + nw - 1) / nw, kb0 = min(p.w.KB, w * per), kb1 = min(p.w.KB, kb0 + per);
-    using A = Q4A<X>;
-    const int here = (int)min((int64_t)16 * RT, p.rows - m0);  // rows of this workgroup
-    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(static_cast<const char*>(p.x) + m0 * p.x_ld * A::kSize,
-                                               (uint32_t)(((here - 1) * p.x_ld + p.K8) * A::kSize));
-    uint32_t off[RT];  // of the lane's row and k; an operand's row is the lane's low four bits, as a weight's column is
+    const Q4Src<X, RT> src(p, m0, l);
+    q4_f32x4 tot[C][RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) off[i] = 16 * i + col < here ? (uint32_t)((16 * i + col) * p.x_ld + 8 * kq) * A::kSize : kQ4Out;
-    auto load_codes = [&](Q4Codes<C, GB, SF>& b, int kb) __attribute__((always_inline)) {
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) tot[c][i] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
+    Q4Block<GB, SF> b[2][C];
+    Q4A<X> a[RT][4];
+    Q4Tile tile[C] = {Q4Tile(p.w, j0), Q4Tile(p.w, j0 + 1)};
+    static_assert(C == 2, "two tiles");
+    auto codes = [&](int q, int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) b[q][c].load(tile[c], kb, l);
+    };
+    auto rows = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int st = 0; st < 4; ++st) src.load(a[i][st], i, kb, st);
+    };
+    const int stop = p.w.KB;
+    codes(0, kb0);
+    rows(kb0 < kb1 ? kb0 : stop);
+    codes(1, kb0 + 1);
+    for (int kb = kb0; kb < kb1; kb += 2) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            Q4Op<X> x[RT][4];
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int st = 0; st < 4; ++st) x[i][st].make(a[i][st]);
+            rows(kb + q + 1 < kb1 ? kb + q + 1 : stop);
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int g = 0; g < GB; ++g)
+                    q4_group<X, RT>(g * 4 / GB, (g + 1) * 4 / GB, b[q][c].scale(g), b[q][c].zero(g), p.w.zeros,
+                                    [&](int st) { return b[q][c].dword(st); }, [&](int i, int st) -> const Q4Op<X>& { return x[i][st]; }, tot[c]);
+            __builtin_amdgcn_sched_barrier(0);
+            codes(q, kb + q + 2);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) q4_red[((w * RT + i) * C + c) * 64 + l] = tot[c][i];
+    __syncthreads();
+    const Q4Bias bias(p);
+    const Q4Scales<X, RT> xs(p, m0, l);
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int j = min(j0 + c, p.w.NT - 1);
-            b.w[c] = p.w.codes[((int64_t)j * p.w.KB + kb) * 64 + l];
-            const int64_t at = ((int64_t)j * p.w.NG + (int64_t)kb * GB) * kQ4N + col;
-#pragma unroll
-            for (int g = 0; g < GB; ++g) {
-                if constexpr (SF) {
-                    const float2 v = static_cast<const float2*>(p.w.scale)[at + g * kQ4N];
-                    b.sf[c][g] = v.x;
-                    b.zf[c][g] = v.y;
-                } else {
-                    b.s[c][g] = static_cast<const uint32_t*>(p.w.scale)[at + g * kQ4N];
-                }
-            }
+            if ((i * C + c) % nw != w) continue;  // one wave a tile
+            q4_f32x4 s = q4_red[(i * C + c) * 64 + l];
+            for (int k = 1; k < nw; ++k) s += q4_red[((k * RT + i) * C + c) * 64 + l];
+            const int n = (j0 + c) * kQ4N + (l & 15);
+            q4_store<X>(p, m0 + 16 * i + 4 * (l >> 4), n, s, xs.v[i], bias.at(n));
         }
-    };
-    auto load_rows = [&](Q4Rows<X, RT>& b, int kb) __attribute__((always_inline)) {
-        const bool last = (kb + 1) * kQ4K > p.K8;  // runs of 8 behind the rows' end read zeros
-#pragma unroll
-        for (int st = 0; st < 4; ++st) {
-            const bool out = last && kb * kQ4K + 32 * st + 8 * kq >= p.K8;
-#pragma unroll
-            for (int i = 0; i < RT; ++i) b.a[i][st].load(rx, (out ? kQ4Out : off[i]) + 32 * st * A::kSize, (uint32_t)(kb * kQ4K * A::kSize));
-        }
-    };
-    q4_f32x4 tot[RT][C];
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int c = 0; c < C; ++c) tot[i][c] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
-    auto step = [&](const Q4Codes<C, GB, SF>& b, const Q4Rows<X, RT>& x) __attribute__((always_inline)) {
-#pragma unroll
-        for (int g = 0; g < GB; ++g) {
-            float scale[C], zero[C];  // zero: 16 + the zero point
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                scale[c] = SF ? b.sf[c][SF ? g : 0] : __uint_as_float(b.s[c][g] & 0xffff0000u);
-                zero[c] = SF ? b.zf[c][SF ? g : 0] : __uint_as_float(b.s[c][g] << 16);
-            }
-            if constexpr (X == Q4_I8) {
-                q4_i32x4 acc[RT][C], sx[RT];
-#pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    sx[i] = q4_i32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int c = 0; c < C; ++c) acc[i][c] = q4_i32x4{0, 0, 0, 0};
-                }
-#pragma unroll
-                for (int st = g * 4 / GB; st < (g + 1) * 4 / GB; ++st) {
-                    long a[RT];
-#pragma unroll
-                    for (int i = 0; i < RT; ++i) a[i] = x.a[i][st].part(0);
-                    if (p.w.zeros) {
-#pragma unroll
-                        for (int i = 0; i < RT; ++i) sx[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(a[i], 0x0101010101010101l, sx[i], 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        const long q = q4_codes_i8((&b.w[c].x)[st]);
-#pragma unroll
-                        for (int i = 0; i < RT; ++i) acc[i][c] = __builtin_amdgcn_mfma_i32_16x16x32_i8(a[i], q, acc[i][c], 0, 0, 0);
-                    }
-                }
-                // whole numbers of at most 128 x 127 x 128 < 2^24: exact up to the scale
-                if (p.w.zeros) {
-#pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        const int z = 16 * ((int)zero[c] - 24);
-#pragma unroll
-                        for (int i = 0; i < RT; ++i) acc[i][c] -= z * sx[i];
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const float s16 = scale[c] * 0.0625f;
-#pragma unroll
-                    for (int i = 0; i < RT; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) tot[i][c][e] = __builtin_fmaf(s16, (float)acc[i][c][e], tot[i][c][e]);
-                }
-            } else {
-                const uint4 one4 = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-                const q4_bf16x8 one = __builtin_bit_cast(q4_bf16x8, one4);
-                q4_f32x4 acc[RT][C], sx[RT];
-#pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    sx[i] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int c = 0; c < C; ++c) acc[i][c] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
-                }
-#pragma unroll
-                for (int st = g * 4 / GB; st < (g + 1) * 4 / GB; ++st) {
-                    q4_bf16x8 q[C];
-#pragma unroll
-                    for (int c = 0; c < C; ++c) q[c] = q4_codes_bf16((&b.w[c].x)[st]);
-#pragma unroll
-                    for (int i = 0; i < RT; ++i)
-#pragma unroll
-                        for (int k = A::kParts - 1; k >= 0; --k) {  // the lowest part first
-                            const q4_bf16x8 a = x.a[i][st].part(k);
-                            sx[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, one, sx[i], 0, 0, 0);
-#pragma unroll
-                            for (int c = 0; c < C; ++c) acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[c], acc[i][c], 0, 0, 0);
-                        }
-                }
-#pragma unroll
-                for (int i = 0; i < RT; ++i)
-#pragma unroll
-                    for (int c = 0; c < C; ++c)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            tot[i][c][e] = __builtin_fmaf(scale[c], __builtin_fmaf(-zero[c], sx[i][e], acc[i][c][e]), tot[i][c][e]);
-            }
-        }
-    };
-    Q4Codes<C, GB, SF> b[PW];
-    Q4Rows<X, RT> x[PA];
-#pragma unroll
-    for (int i = 0; i < PW; ++i)
-        if (kb0 + i < kb1) load_codes(b[i], kb0 + i);
-#pragma unroll
-    for (int i = 0; i < PA; ++i)
-        if (kb0 + i < kb1) load_rows(x[i], kb0 + i);
-    for (int kb = kb0; kb < kb1; kb += PW) {
-#pragma unroll
-        for (int i = 0; i < PW; ++i)
-            if (kb + i < kb1) {
-                step(b[i], x[i % PA]);
-                if (kb + i + PA < kb1) load_rows(x[i % PA], kb + i + PA);
-                if (kb + i + PW < kb1) load_codes(b[i], kb + i + PW);
-            }
-    }
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int c = 0; c < C; ++c) q4_red[((w * RT + i) * C + c) * 64 + l] = tot[i][c];
-    __syncthreads();
-    for (int u = w; u < RT * C; u += nw) {  // one wave a tile
-        const int i = u / C, c = u - i * C, n = (j0 + c) * kQ4N + col;
-        q4_f32x4 s = q4_red[(i * C + c) * 64 + l];
-        for (int k = 1; k < nw; ++k) s += q4_red[((k * RT + i) * C + c) * 64 + l];
-        if (n >= p.w.N) continue;
-        const float bias = p.bias ? p.bias[n] : 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int64_t m = m0 + 16 * i + 4 * kq + e;
-            if (m >= p.rows) continue;
-            float v = s[e];
-            if (X == Q4_I8) v *= p.xs[m];
-            if (p.bias) v += bias;
-            if (p.ybf16) store_f32<bf16_t>(static_cast<bf16_t*>(p.y) + m * p.y_ld + n, v);
-            else static_cast<float*>(p.y)[m * p.y_ld + n] = v;
-        }
-    }
 }
 
 // Rows of a width that is no multiple of 8 (or too far apart for the buffer's offsets), copied with
@@ -341,21 +463,34 @@ __global__ __launch_bounds__(256) void q4_pad(const T* x, int64_t ld, int64_t ro
     }
 }
 
-template <int X, int RT, int C, int GB, int PW, int PA>
-static void q4_launch(const Q4P& p, int nw, hipStream_t s) {
+template <int X, int RT, int NK, int GB>
+static void q4_held_launch(const Q4P& p, hipStream_t s) {
+    const int nw = ceil_div(p.w.KB, NK), by = (int)((p.rows + 16 * RT - 1) / (16 * RT));
+    // workgroups that the chip holds at once (the registers leave room for sixteen or twelve waves a
+    // CU), each with the same number of tiles
+    constexpr int room = RT == 1 && X != Q4_F32 && GB < 4 ? 16 : 12;
+    const int most = std::max(1, 256 * std::max(1, room / nw) / by), turns = ceil_div(p.w.NT, std::min(p.w.NT, most));
+    const dim3 grid(ceil_div(p.w.NT, turns), by), block(64 * nw);
+    const size_t lds = (size_t)2 * nw * RT * 64 * 16;
+    if (p.w.sbf16) hipLaunchKernelGGL((q4_held<X, RT, NK, GB, false>), grid, block, lds, s, p);
+    else hipLaunchKernelGGL((q4_held<X, RT, NK, GB, true>), grid, block, lds, s, p);
+}
+template <int X, int RT, int C, int GB>
+static void q4_walk_launch(const Q4P& p, hipStream_t s) {
+    int nw = 4;  // some 2048 waves in all, each with two blocks at least
+    while (nw < 8 && (int64_t)p.w.NT * nw < 2048 * C && p.w.KB >= 4 * nw) nw *= 2;
     const dim3 grid(ceil_div(p.w.NT, C), (uint32_t)((p.rows + 16 * RT - 1) / (16 * RT))), block(64 * nw);
     const size_t lds = (size_t)nw * RT * C * 64 * 16;
-    if (p.w.sbf16) hipLaunchKernelGGL((q4_mm<X, RT, C, GB, PW, PA, false>), grid, block, lds, s, p);
-    else hipLaunchKernelGGL((q4_mm<X, RT, C, GB, PW, PA, true>), grid, block, lds, s, p);
+    if (p.w.sbf16) hipLaunchKernelGGL((q4_walk<X, RT, C, GB, false>), grid, block, lds, s, p);
+    else hipLaunchKernelGGL((q4_walk<X, RT, C, GB, true>), grid, block, lds, s, p);
 }
 template <int X, int GB>
 static void q4_shape(const Q4P& p, hipStream_t s) {
-    // waves: some 2048 in all, each with two blocks at least
-    int nw = 4;
-    while (nw < 8 && (int64_t)p.w.NT * nw < 2048 && p.w.KB >= 4 * nw) nw *= 2;
-    if (p.rows <= 16) q4_launch<X, 1, 1, GB, X == Q4_F32 ? 4 : 6, X == Q4_F32 ? 1 : 2>(p, nw, s);
-    else if (p.rows <= 32 || X == Q4_F32) q4_launch<X, 2, 2, GB, 2, X == Q4_F32 ? 1 : 2>(p, nw, s);
-    else if constexpr (X != Q4_F32) q4_launch<X, 4, 2, GB, 2, X == Q4_BF16 ? 1 : 2>(p, 4, s);
+    // twelve waves at most hold the rows
+    constexpr int NK1 = X == Q4_F32 ? 2 : 4, NK2 = X == Q4_I8 ? 3 : 2;
+    if (p.rows <= 16 && p.w.KB <= 12 * NK1) q4_held_launch<X, 1, NK1, GB>(p, s);
+    else if (X != Q4_F32 && p.rows > 16 && p.w.KB <= 12 * NK2) q4_held_launch<X == Q4_F32 ? Q4_BF16 : X, 2, NK2, GB>(p, s);
+    else q4_walk_launch<X, 2, 2, GB>(p, s);
 }
 template <int X>
 static void q4_dispatch(const Q4P& p, hipStream_t s) {

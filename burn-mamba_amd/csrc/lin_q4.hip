@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void q4_pack(Q4W w, const uint8_t* codes, cons
         const int col = (int)(i % 16), g = (int)(i / 16 % w.NG), n = (int)(i / 16 / w.NG) * kQ4N + col;
         const bool in = g < groups && n < w.N;
         const int64_t src = (int64_t)g * w.N + n;
-        const float z = 16.f + (in ? (zero ? zero[src] & 15 : 8) : 0);
+        const float z = -16.f - (in ? (zero ? zero[src] & 15 : 8) : 0);  // whole numbers to 31: bf16 holds them
         if (w.sbf16) static_cast<uint32_t*>(oscale)[i] = (in ? (uint32_t)static_cast<const bf16_t*>(scale)[src] << 16 : 0u) | __float_as_uint(z) >> 16;
         else static_cast<float2*>(oscale)[i] = make_float2(in ? static_cast<const float*>(scale)[src] : 0.f, z);
     }
@@ -86,6 +86,9 @@ typedef float q4_f32x4 __attribute__((ext_vector_type(4)));
 typedef int q4_i32x4 __attribute__((ext_vector_type(4)));
 
 enum Q4X { Q4_BF16 = 0, Q4_F32 = 1, Q4_I8 = 2 };
+// What lies beside the codes: bf16 scales alone, with zero points, f32 scales (with or without).
+enum Q4S { Q4_S16 = 0, Q4_S16Z = 1, Q4_S32 = 2 };
+constexpr uint32_t kQ4Out = 0x80000000u;  // a byte offset past every buffer's extent
 
 // Lane l's operand of 32 k of 16 rows: row l % 16, k 8 (l / 16) .. + 7, loaded through a buffer
 // resource (an offset past its extent reads zeros).  f32 rows are three bf16 parts, each the
@@ -131,15 +134,17 @@ template <> struct Q4A<Q4_I8> {
 };
 
 // The codes of a dword, as operands.  A bf16 whose upper four bits of mantissa are the code
-// is 16 + code: one shift and one and-or a pair.  A byte whose upper four bits are code ^ 8 is
-// 16 (code - 8).
+// is 16 + code: a shift and an and-or a pair (the mask in a vector register, for an instruction takes
+// one scalar).  A byte whose upper four bits are code ^ 8 is 16 (code - 8).
 __device__ __forceinline__ q4_bf16x8 q4_codes_bf16(uint32_t w) {
-    const uint32_t d[4] = {(w << 3 & 0x00780078u) | 0x41804180u, (w >> 1 & 0x00780078u) | 0x41804180u, (w >> 5 & 0x00780078u) | 0x41804180u,
-                           (w >> 9 & 0x00780078u) | 0x41804180u};
+    uint32_t mask = 0x00780078u;
+    asm("" : "+v"(mask));
+    const uint32_t d[4] = {(w << 3 & mask) | 0x41804180u, (w >> 1 & mask) | 0x41804180u, (w >> 5 & mask) | 0x41804180u, (w >> 9 & mask) | 0x41804180u};
     return __builtin_bit_cast(q4_bf16x8, d);
 }
 __device__ __forceinline__ long q4_codes_i8(uint32_t w) {
-    return (long)((uint64_t)((w & 0xf0f0f0f0u) ^ 0x80808080u) << 32 | ((w << 4 & 0xf0f0f0f0u) ^ 0x80808080u));
+    w ^= 0x88888888u;
+    return (long)((uint64_t)(w & 0xf0f0f0f0u) << 32 | (w << 4 & 0xf0f0f0f0u));
 }
 
 // The rows' operands as the products take them, kept in registers: NP parts.
@@ -159,59 +164,6 @@ struct Q4Op<Q4_I8> {
     __device__ __forceinline__ void make(const Q4A<Q4_I8>& a) { v[0] = a.part(0); }
 };
 
-// A group's products of RT row tiles with a column tile, scaled and added to tot: st0 .. st1 - 1 its
-// steps of 32 k, q(st) their codes' dword, x(i, st) the rows' operands, zero 16 + the zero point.
-template <int X, int RT, typename Q, typename Op>
-__device__ __forceinline__ void q4_group(int st0, int st1, float scale, float zero, bool zeros, Q q, Op x, q4_f32x4 (&tot)[RT]) {
-    if constexpr (X == Q4_I8) {
-        q4_i32x4 acc[RT], sx[RT];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) acc[i] = sx[i] = q4_i32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int st = st0; st < st1; ++st) {
-            const long c = q4_codes_i8(q(st));
-#pragma unroll
-            for (int i = 0; i < RT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x(i, st).v[0], c, acc[i], 0, 0, 0);
-        }
-        // whole numbers of at most 128 x 127 x 128 < 2^24: exact up to the scale
-        if (zeros) {
-            const int z = 16 * ((int)zero - 24);
-#pragma unroll
-            for (int st = st0; st < st1; ++st)
-#pragma unroll
-                for (int i = 0; i < RT; ++i) sx[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x(i, st).v[0], 0x0101010101010101l, sx[i], 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < RT; ++i) acc[i] -= z * sx[i];
-        }
-        const float s16 = scale * 0.0625f;
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) tot[i][e] = __builtin_fmaf(s16, (float)acc[i][e], tot[i][e]);
-    } else {
-        const uint32_t z2 = __float_as_uint(-zero) >> 16 | (__float_as_uint(-zero) & 0xffff0000u);
-        const q4_bf16x8 off = __builtin_bit_cast(q4_bf16x8, make_uint4(z2, z2, z2, z2));  // a whole number up to 31: a bf16
-        q4_f32x4 acc[RT];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) acc[i] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int st = st0; st < st1; ++st) {
-            const q4_bf16x8 c = q4_codes_bf16(q(st));
-#pragma unroll
-            for (int i = 0; i < RT; ++i)
-#pragma unroll
-                for (int k = Q4Op<X>::kParts - 1; k >= 0; --k) {  // the lowest part first
-                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x(i, st).v[k], c, acc[i], 0, 0, 0);
-                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x(i, st).v[k], off, acc[i], 0, 0, 0);
-                }
-        }
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) tot[i][e] = __builtin_fmaf(scale, acc[i][e], tot[i][e]);
-    }
-}
-
 // Column tile j through buffer resources (scalar bases, 32-bit offsets): blocks behind the last,
 // and tiles behind the last, read zeros.
 struct Q4Tile {
@@ -224,43 +176,112 @@ struct Q4Tile {
     }
 };
 // A block of a column tile: its codes, and its groups' scales and zero points.
-template <int GB, bool SF>
+template <int GB, int S>
 struct Q4Block {
     uint4 w;
-    uint32_t s[SF ? 1 : GB];
-    uint2 sf[SF ? GB : 1];
+    uint32_t s[GB];
+    uint32_t z[S == Q4_S32 ? GB : 1];
     __device__ __forceinline__ void load(const Q4Tile& t, int kb, int l) {
         w = buf_ld16(t.codes, l * 16, kb * 1024);
 #pragma unroll
         for (int g = 0; g < GB; ++g) {
-            const int soff = kb * GB * kQ4N * (SF ? 8 : 4);
-            if constexpr (SF) sf[g] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(t.scale, (l & 15) * 8 + g * kQ4N * 8, soff, 0));
-            else s[g] = __builtin_amdgcn_raw_buffer_load_b32(t.scale, (l & 15) * 4 + g * kQ4N * 4, soff, 0);
+            if constexpr (S == Q4_S32) {
+                const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(t.scale, (l & 15) * 8 + g * kQ4N * 8, kb * GB * kQ4N * 8, 0));
+                s[g] = v.x;
+                z[g] = v.y;
+            } else {
+                s[g] = __builtin_amdgcn_raw_buffer_load_b32(t.scale, (l & 15) * 4 + g * kQ4N * 4, kb * GB * kQ4N * 4, 0);
+            }
         }
     }
-    __device__ __forceinline__ float scale(int g) const { return __uint_as_float(SF ? sf[SF ? g : 0].x : s[SF ? 0 : g] & 0xffff0000u); }
-    __device__ __forceinline__ float zero(int g) const { return __uint_as_float(SF ? sf[SF ? g : 0].y : s[SF ? 0 : g] << 16); }
+    __device__ __forceinline__ float scale(int g) const { return __uint_as_float(S == Q4_S32 ? s[g] : s[g] & 0xffff0000u); }
+    // -(16 + zero point), as two bf16
+    __device__ __forceinline__ uint32_t minus2(int g) const {
+        if constexpr (S == Q4_S16) return 0xc1c0c1c0u;  // -24
+        else if constexpr (S == Q4_S16Z) return __builtin_amdgcn_perm(s[g], s[g], 0x01000100u);
+        else return __builtin_amdgcn_perm(z[S == Q4_S32 ? g : 0], z[S == Q4_S32 ? g : 0], 0x03020302u);
+    }
+    // zero point - 8
+    __device__ __forceinline__ int zero8(int g) const {
+        return -24 - (int)__uint_as_float(S == Q4_S32 ? z[S == Q4_S32 ? g : 0] : s[g] << 16);
+    }
     __device__ __forceinline__ uint32_t dword(int st) const { return st == 0 ? w.x : st == 1 ? w.y : st == 2 ? w.z : w.w; }
 };
+
+// Group g of a block against RT row tiles, scaled and added to tot.
+template <int X, int RT, int GB, int S>
+__device__ __forceinline__ void q4_group(const Q4Block<GB, S>& b, int g, bool zeros, const Q4Op<X> (&x)[RT][4], q4_f32x4 (&tot)[RT]) {
+    const float scale = b.scale(g);
+    if constexpr (X == Q4_I8) {
+        q4_i32x4 acc[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[i] = q4_i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int st = g * 4 / GB; st < (g + 1) * 4 / GB; ++st) {
+            const long c = q4_codes_i8(b.dword(st));
+#pragma unroll
+            for (int i = 0; i < RT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x[i][st].v[0], c, acc[i], 0, 0, 0);
+        }
+        // whole numbers of at most 128 x 127 x 256 < 2^23: exact up to the scale
+        if (S != Q4_S16 && zeros) {
+            const int z = -16 * b.zero8(g);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                q4_i32x4 sx = {0, 0, 0, 0};
+#pragma unroll
+                for (int st = g * 4 / GB; st < (g + 1) * 4 / GB; ++st) sx = __builtin_amdgcn_mfma_i32_16x16x32_i8(x[i][st].v[0], 0x0101010101010101l, sx, 0, 0, 0);
+                acc[i] += z * sx;
+            }
+        }
+        const float s16 = scale * 0.0625f;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tot[i][e] = __builtin_fmaf(s16, (float)acc[i][e], tot[i][e]);
+    } else {
+        const uint32_t z2 = b.minus2(g);
+        const q4_bf16x8 off = __builtin_bit_cast(q4_bf16x8, make_uint4(z2, z2, z2, z2));
+        q4_f32x4 acc[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) acc[i] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = g * 4 / GB; st < (g + 1) * 4 / GB; ++st) {
+            const q4_bf16x8 c = q4_codes_bf16(b.dword(st));
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int k = Q4Op<X>::kParts - 1; k >= 0; --k) {  // the lowest part first
+                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i][st].v[k], c, acc[i], 0, 0, 0);
+                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i][st].v[k], off, acc[i], 0, 0, 0);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tot[i][e] = __builtin_fmaf(scale, acc[i][e], tot[i][e]);
+    }
+}
 
 // The rows of a workgroup and where a lane's operands of them lie.
 template <int X, int RT>
 struct Q4Src {
+    static constexpr int e = Q4A<X>::kSize;
     __amdgpu_buffer_rsrc_t r;
     uint32_t off[RT];
-    int K8, kq;
-    __device__ __forceinline__ Q4Src(const Q4P& p, int64_t m0, int l) : K8(p.K8), kq(l >> 4) {
-        constexpr int e = Q4A<X>::kSize;
+    int K8, KB, k8;
+    __device__ __forceinline__ Q4Src(const Q4P& p, int64_t m0, int l) : K8(p.K8), KB(p.w.KB), k8(8 * (l >> 4)) {
         const int here = (int)min((int64_t)16 * RT, p.rows - m0), col = l & 15;  // an operand's row is the lane's low four bits, as a weight's column is
         r = buf_rsrc(static_cast<const char*>(p.x) + m0 * p.x_ld * e, (uint32_t)(((here - 1) * p.x_ld + p.K8) * e));
 #pragma unroll
-        for (int i = 0; i < RT; ++i) off[i] = 16 * i + col < here ? (uint32_t)((16 * i + col) * p.x_ld + 8 * kq) * e : 0x80000000u;  // past every extent
+        for (int i = 0; i < RT; ++i) off[i] = 16 * i + col < here ? ((uint32_t)(16 * i + col) * (uint32_t)p.x_ld + k8) * e : kQ4Out;
     }
-    // runs of 8 behind the rows' end, and blocks behind the last (kb = KB), read zeros
-    __device__ __forceinline__ void load(Q4A<X>& a, int i, int kb, int st) const {
-        constexpr int e = Q4A<X>::kSize;
-        const bool out = kb * kQ4K + 32 * st + 8 * kq >= K8;
-        a.load(r, (out ? 0x80000000u : off[i]) + 32 * st * e, out ? 0u : (uint32_t)(kb * kQ4K * e));
+    // block kb; runs of 8 behind the rows' end, and blocks behind the last, read zeros
+    __device__ __forceinline__ void load(Q4A<X> (&a)[RT][4], int kb) const {
+        const int left = K8 - kb * kQ4K, soff = min(kb, KB - 1) * kQ4K * e;
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int i = 0; i < RT; ++i) a[i][st].load(r, (k8 + 32 * st < left ? off[i] : kQ4Out) + 32 * st * e, soff);
     }
 };
 
@@ -302,7 +323,7 @@ __device__ __forceinline__ void q4_store(const Q4P& p, int64_t m0, int n, const 
 // workgroup's waves all of k.  It takes column tiles in turn; a block's registers are loaded for
 // the next tile as soon as this one's are used.  The waves' sums meet in LDS, in the order of k, in
 // two places by turns, so that a tile has one barrier.
-template <int X, int RT, int NK, int GB, bool SF>
+template <int X, int RT, int NK, int GB, int S>
 __global__ __launch_bounds__(768) void q4_held(Q4P p) {
     extern __shared__ __align__(16) q4_f32x4 q4_red[];  // [2][waves][RT][64]
     const int nw = blockDim.x >> 6, w = wave_id(), l = threadIdx.x & 63;
@@ -314,13 +335,9 @@ __global__ __launch_bounds__(768) void q4_held(Q4P p) {
     const Q4Src<X, RT> src(p, m0, l);
     Q4A<X> a[NK][RT][4];
 #pragma unroll
-    for (int k = 0; k < NK; ++k)
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int st = 0; st < 4; ++st) src.load(a[k][i][st], i, min(kb0 + k, p.w.KB), st);
+    for (int k = 0; k < NK; ++k) src.load(a[k], kb0 + k);
     __builtin_amdgcn_sched_barrier(0);
-    Q4Block<GB, SF> b[NK];
+    Q4Block<GB, S> b[NK];
     {
         const Q4Tile t(p.w, blockIdx.x);
 #pragma unroll
@@ -358,9 +375,7 @@ __global__ __launch_bounds__(768) void q4_held(Q4P p) {
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
 #pragma unroll
-            for (int g = 0; g < GB; ++g)
-                q4_group<X, RT>(g * 4 / GB, (g + 1) * 4 / GB, b[k].scale(g), b[k].zero(g), p.w.zeros, [&](int st) { return b[k].dword(st); },
-                                [&](int i, int st) -> const Q4Op<X>& { return x[k][i][st]; }, tot);
+            for (int g = 0; g < GB; ++g) q4_group<X, RT, GB, S>(b[k], g, p.w.zeros, x[k], tot);
             // behind the block's last use, so that its registers are these
             __builtin_amdgcn_sched_barrier(0);
             b[k].load(next, kb0 + k, l);
@@ -382,7 +397,7 @@ __global__ __launch_bounds__(768) void q4_held(Q4P p) {
 
 // Any k: RT row tiles with C column tiles, a wave walks a stretch of k with two blocks of codes and
 // one of rows in flight.
-template <int X, int RT, int C, int GB, bool SF>
+template <int X, int RT, int C, int GB, int S>
 __global__ __launch_bounds__(512) void q4_walk(Q4P p) {
     extern __shared__ __align__(16) q4_f32x4 q4_red[];  // [waves][RT][C][64]
     const int nw = blockDim.x >> 6, w = wave_id(), l = threadIdx.x & 63;
@@ -395,7 +410,7 @@ __global__ __launch_bounds__(512) void q4_walk(Q4P p) {
     for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int i = 0; i < RT; ++i) tot[c][i] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
-    Q4Block<GB, SF> b[2][C];
+    Q4Block<GB, S> b[2][C];
     Q4A<X> a[RT][4];
     Q4Tile tile[C] = {Q4Tile(p.w, j0), Q4Tile(p.w, j0 + 1)};
     static_assert(C == 2, "two tiles");
@@ -403,15 +418,9 @@ __global__ __launch_bounds__(512) void q4_walk(Q4P p) {
 #pragma unroll
         for (int c = 0; c < C; ++c) b[q][c].load(tile[c], kb, l);
     };
-    auto rows = [&](int kb) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int st = 0; st < 4; ++st) src.load(a[i][st], i, kb, st);
-    };
     const int stop = p.w.KB;
     codes(0, kb0);
-    rows(kb0 < kb1 ? kb0 : stop);
+    src.load(a, kb0 < kb1 ? kb0 : stop);
     codes(1, kb0 + 1);
     for (int kb = kb0; kb < kb1; kb += 2) {
 #pragma unroll
@@ -421,13 +430,11 @@ __global__ __launch_bounds__(512) void q4_walk(Q4P p) {
             for (int i = 0; i < RT; ++i)
 #pragma unroll
                 for (int st = 0; st < 4; ++st) x[i][st].make(a[i][st]);
-            rows(kb + q + 1 < kb1 ? kb + q + 1 : stop);
+            src.load(a, kb + q + 1 < kb1 ? kb + q + 1 : stop);
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int g = 0; g < GB; ++g)
-                    q4_group<X, RT>(g * 4 / GB, (g + 1) * 4 / GB, b[q][c].scale(g), b[q][c].zero(g), p.w.zeros,
-                                    [&](int st) { return b[q][c].dword(st); }, [&](int i, int st) -> const Q4Op<X>& { return x[i][st]; }, tot[c]);
+                for (int g = 0; g < GB; ++g) q4_group<X, RT, GB, S>(b[q][c], g, p.w.zeros, x, tot[c]);
             __builtin_amdgcn_sched_barrier(0);
             codes(q, kb + q + 2);
             __builtin_amdgcn_sched_barrier(0);
@@ -472,8 +479,9 @@ static void q4_held_launch(const Q4P& p, hipStream_t s) {
     const int most = std::max(1, 256 * std::max(1, room / nw) / by), turns = ceil_div(p.w.NT, std::min(p.w.NT, most));
     const dim3 grid(ceil_div(p.w.NT, turns), by), block(64 * nw);
     const size_t lds = (size_t)2 * nw * RT * 64 * 16;
-    if (p.w.sbf16) hipLaunchKernelGGL((q4_held<X, RT, NK, GB, false>), grid, block, lds, s, p);
-    else hipLaunchKernelGGL((q4_held<X, RT, NK, GB, true>), grid, block, lds, s, p);
+    if (!p.w.sbf16) hipLaunchKernelGGL((q4_held<X, RT, NK, GB, Q4_S32>), grid, block, lds, s, p);
+    else if (p.w.zeros) hipLaunchKernelGGL((q4_held<X, RT, NK, GB, Q4_S16Z>), grid, block, lds, s, p);
+    else hipLaunchKernelGGL((q4_held<X, RT, NK, GB, Q4_S16>), grid, block, lds, s, p);
 }
 template <int X, int RT, int C, int GB>
 static void q4_walk_launch(const Q4P& p, hipStream_t s) {
@@ -481,8 +489,9 @@ static void q4_walk_launch(const Q4P& p, hipStream_t s) {
     while (nw < 8 && (int64_t)p.w.NT * nw < 2048 * C && p.w.KB >= 4 * nw) nw *= 2;
     const dim3 grid(ceil_div(p.w.NT, C), (uint32_t)((p.rows + 16 * RT - 1) / (16 * RT))), block(64 * nw);
     const size_t lds = (size_t)nw * RT * C * 64 * 16;
-    if (p.w.sbf16) hipLaunchKernelGGL((q4_walk<X, RT, C, GB, false>), grid, block, lds, s, p);
-    else hipLaunchKernelGGL((q4_walk<X, RT, C, GB, true>), grid, block, lds, s, p);
+    if (!p.w.sbf16) hipLaunchKernelGGL((q4_walk<X, RT, C, GB, Q4_S32>), grid, block, lds, s, p);
+    else if (p.w.zeros) hipLaunchKernelGGL((q4_walk<X, RT, C, GB, Q4_S16Z>), grid, block, lds, s, p);
+    else hipLaunchKernelGGL((q4_walk<X, RT, C, GB, Q4_S16>), grid, block, lds, s, p);
 }
 template <int X, int GB>
 static void q4_shape(const Q4P& p, hipStream_t s) {

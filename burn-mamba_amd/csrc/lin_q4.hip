@@ -15,6 +15,7 @@
 namespace mamba {
 
 constexpr int kQ4N = 16, kQ4K = 128;  // columns and k of a block
+constexpr int kQ4Waves = 12;           // of a workgroup that holds the rows, at most
 
 struct Q4W {
     int K, N, G;            // group: k of a group
@@ -142,10 +143,11 @@ __device__ __forceinline__ q4_bf16x8 q4_codes_bf16(uint32_t w) {
     const uint32_t d[4] = {(w << 3 & mask) | 0x41804180u, (w >> 1 & mask) | 0x41804180u, (w >> 5 & mask) | 0x41804180u, (w >> 9 & mask) | 0x41804180u};
     return __builtin_bit_cast(q4_bf16x8, d);
 }
-__device__ __forceinline__ long q4_codes_i8(uint32_t w) {
+__device__ __forceinline__ long q4_codes_i8x16(uint32_t w) {
     w ^= 0x88888888u;
     return (long)((uint64_t)(w & 0xf0f0f0f0u) << 32 | (w << 4 & 0xf0f0f0f0u));
 }
+__device__ __forceinline__ long q4_codes_i8(uint32_t w) { return (long)((uint64_t)(w >> 4 & 0x0f0f0f0fu) << 32 | (w & 0x0f0f0f0fu)); }
 
 // The rows' operands as the products take them, kept in registers: NP parts.
 template <int X>
@@ -201,43 +203,39 @@ struct Q4Block {
         else if constexpr (S == Q4_S16Z) return __builtin_amdgcn_perm(s[g], s[g], 0x01000100u);
         else return __builtin_amdgcn_perm(z[S == Q4_S32 ? g : 0], z[S == Q4_S32 ? g : 0], 0x03020302u);
     }
-    // zero point - 8
-    __device__ __forceinline__ int zero8(int g) const {
-        return -24 - (int)__uint_as_float(S == Q4_S32 ? z[S == Q4_S32 ? g : 0] : s[g] << 16);
+    // - zero point, as eight bytes
+    __device__ __forceinline__ long minus8(int g) const {
+        const uint32_t v = 16 + (int)__uint_as_float(S == Q4_S32 ? z[S == Q4_S32 ? g : 0] : s[g] << 16);
+        const uint32_t b = __builtin_amdgcn_perm(v, v, 0u);
+        return (long)((uint64_t)b << 32 | b);
     }
     __device__ __forceinline__ uint32_t dword(int st) const { return st == 0 ? w.x : st == 1 ? w.y : st == 2 ? w.z : w.w; }
 };
 
 // Group g of a block against RT row tiles, scaled and added to tot.
 template <int X, int RT, int GB, int S>
-__device__ __forceinline__ void q4_group(const Q4Block<GB, S>& b, int g, bool zeros, const Q4Op<X> (&x)[RT][4], q4_f32x4 (&tot)[RT]) {
+__device__ __forceinline__ void q4_group(const Q4Block<GB, S>& b, int g, const Q4Op<X> (&x)[RT][4], q4_f32x4 (&tot)[RT]) {
     const float scale = b.scale(g);
     if constexpr (X == Q4_I8) {
+        const long off = S == Q4_S16 ? 0 : b.minus8(g);
         q4_i32x4 acc[RT];
 #pragma unroll
         for (int i = 0; i < RT; ++i) acc[i] = q4_i32x4{0, 0, 0, 0};
 #pragma unroll
         for (int st = g * 4 / GB; st < (g + 1) * 4 / GB; ++st) {
-            const long c = q4_codes_i8(b.dword(st));
-#pragma unroll
-            for (int i = 0; i < RT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x[i][st].v[0], c, acc[i], 0, 0, 0);
-        }
-        // whole numbers of at most 128 x 127 x 256 < 2^23: exact up to the scale
-        if (S != Q4_S16 && zeros) {
-            const int z = -16 * b.zero8(g);
+            const long c = S == Q4_S16 ? q4_codes_i8x16(b.dword(st)) : q4_codes_i8(b.dword(st));
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-                q4_i32x4 sx = {0, 0, 0, 0};
-#pragma unroll
-                for (int st = g * 4 / GB; st < (g + 1) * 4 / GB; ++st) sx = __builtin_amdgcn_mfma_i32_16x16x32_i8(x[i][st].v[0], 0x0101010101010101l, sx, 0, 0, 0);
-                acc[i] += z * sx;
+                acc[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x[i][st].v[0], c, acc[i], 0, 0, 0);
+                if constexpr (S != Q4_S16) acc[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x[i][st].v[0], off, acc[i], 0, 0, 0);
             }
         }
-        const float s16 = scale * 0.0625f;
+        // whole numbers of at most 128 x 127 x 128 < 2^24: exact up to the scale
+        const float by = S == Q4_S16 ? scale * 0.0625f : scale;
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) tot[i][e] = __builtin_fmaf(s16, (float)acc[i][e], tot[i][e]);
+            for (int e = 0; e < 4; ++e) tot[i][e] = __builtin_fmaf(by, (float)acc[i][e], tot[i][e]);
     } else {
         const uint32_t z2 = b.minus2(g);
         const q4_bf16x8 off = __builtin_bit_cast(q4_bf16x8, make_uint4(z2, z2, z2, z2));
@@ -319,21 +317,21 @@ __device__ __forceinline__ void q4_store(const Q4P& p, int64_t m0, int n, const 
     }
 }
 
-// The rows in registers: wave w holds the operands of RT row tiles for NK blocks of k, and the
+// The rows in registers: wave w holds the operands of 16 rows for NK blocks of k, and the
 // workgroup's waves all of k.  It takes column tiles in turn; a block's registers are loaded for
 // the next tile as soon as this one's are used.  The waves' sums meet in LDS, in the order of k, in
 // two places by turns, so that a tile has one barrier.
-template <int X, int RT, int NK, int GB, int S>
-__global__ __launch_bounds__(768) void q4_held(Q4P p) {
-    extern __shared__ __align__(16) q4_f32x4 q4_red[];  // [2][waves][RT][64]
+template <int X, int NK, int GB, int S>
+__global__ __launch_bounds__(64 * kQ4Waves) void q4_held(Q4P p) {
+    extern __shared__ __align__(16) q4_f32x4 q4_red[];  // [2][waves][64]
     const int nw = blockDim.x >> 6, w = wave_id(), l = threadIdx.x & 63;
-    const int64_t m0 = (int64_t)blockIdx.y * (16 * RT);
+    const int64_t m0 = (int64_t)blockIdx.y * 16;
     const int kb0 = w * NK;
     // No load has a branch of its own, behind which the compiler would wait for every load in
     // flight; for the same reason the rows are waited for before the tiles' loop, and the blocks are
     // loaded in the order of their use before it as in it.
-    const Q4Src<X, RT> src(p, m0, l);
-    Q4A<X> a[NK][RT][4];
+    const Q4Src<X, 1> src(p, m0, l);
+    Q4A<X> a[NK][1][4];
 #pragma unroll
     for (int k = 0; k < NK; ++k) src.load(a[k], kb0 + k);
     __builtin_amdgcn_sched_barrier(0);
@@ -346,52 +344,42 @@ __global__ __launch_bounds__(768) void q4_held(Q4P p) {
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    Q4Op<X> x[NK][RT][4];
+    Q4Op<X> x[NK][1][4];
 #pragma unroll
     for (int k = 0; k < NK; ++k)
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+        for (int st = 0; st < 4; ++st) {
+            x[k][0][st].make(a[k][0][st]);
 #pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                x[k][i][st].make(a[k][i][st]);
-#pragma unroll
-                for (int e = 0; e < Q4Op<X>::kParts; ++e) asm volatile("" : "+v"(x[k][i][st].v[e]));
-            }
+            for (int e = 0; e < Q4Op<X>::kParts; ++e) asm volatile("" : "+v"(x[k][0][st].v[e]));
+        }
     const Q4Bias bias(p);
-    Q4Scales<X, RT> xs(p, m0, l);
+    Q4Scales<X, 1> xs(p, m0, l);
     if constexpr (X == Q4_I8) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(xs.v[i][e]));
+        for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(xs.v[0][e]));
     }
     int turn = 0;
     for (int j = blockIdx.x; j < p.w.NT; j += gridDim.x, ++turn) {
         const Q4Tile next(p.w, j + gridDim.x);
         const float add = bias.at(j * kQ4N + (l & 15));
-        q4_f32x4 tot[RT];
-#pragma unroll
-        for (int i = 0; i < RT; ++i) tot[i] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
+        q4_f32x4 tot[1] = {q4_f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
 #pragma unroll
-            for (int g = 0; g < GB; ++g) q4_group<X, RT, GB, S>(b[k], g, p.w.zeros, x[k], tot);
+            for (int g = 0; g < GB; ++g) q4_group<X, 1, GB, S>(b[k], g, x[k], tot);
             // behind the block's last use, so that its registers are these
             __builtin_amdgcn_sched_barrier(0);
             b[k].load(next, kb0 + k, l);
             __builtin_amdgcn_sched_barrier(0);
         }
-        q4_f32x4* red = q4_red + (turn & 1) * nw * RT * 64;
-#pragma unroll
-        for (int i = 0; i < RT; ++i) red[(w * RT + i) * 64 + l] = tot[i];
+        q4_f32x4* red = q4_red + (turn & 1) * nw * 64;
+        red[w * 64 + l] = tot[0];
         __syncthreads();
         if (w != turn % nw) continue;
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            q4_f32x4 s = red[i * 64 + l];
-            for (int k = 1; k < nw; ++k) s += red[(k * RT + i) * 64 + l];
-            q4_store<X>(p, m0 + 16 * i + 4 * (l >> 4), j * kQ4N + (l & 15), s, xs.v[i], add);
-        }
+        q4_f32x4 s = red[l];
+        for (int k = 1; k < nw; ++k) s += red[k * 64 + l];
+        q4_store<X>(p, m0 + 4 * (l >> 4), j * kQ4N + (l & 15), s, xs.v[0], add);
     }
 }
 
@@ -434,7 +422,7 @@ __global__ __launch_bounds__(512) void q4_walk(Q4P p) {
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
-                for (int g = 0; g < GB; ++g) q4_group<X, RT, GB, S>(b[q][c], g, p.w.zeros, x, tot[c]);
+                for (int g = 0; g < GB; ++g) q4_group<X, RT, GB, S>(b[q][c], g, x, tot[c]);
             __builtin_amdgcn_sched_barrier(0);
             codes(q, kb + q + 2);
             __builtin_amdgcn_sched_barrier(0);
@@ -470,18 +458,15 @@ __global__ __launch_bounds__(256) void q4_pad(const T* x, int64_t ld, int64_t ro
     }
 }
 
-template <int X, int RT, int NK, int GB>
-static void q4_held_launch(const Q4P& p, hipStream_t s) {
-    const int nw = ceil_div(p.w.KB, NK), by = (int)((p.rows + 16 * RT - 1) / (16 * RT));
-    // workgroups that the chip holds at once (the registers leave room for sixteen or twelve waves a
-    // CU), each with the same number of tiles
-    constexpr int room = RT == 1 && X != Q4_F32 && GB < 4 ? 16 : 12;
-    const int most = std::max(1, 256 * std::max(1, room / nw) / by), turns = ceil_div(p.w.NT, std::min(p.w.NT, most));
-    const dim3 grid(ceil_div(p.w.NT, turns), by), block(64 * nw);
-    const size_t lds = (size_t)2 * nw * RT * 64 * 16;
-    if (!p.w.sbf16) hipLaunchKernelGGL((q4_held<X, RT, NK, GB, Q4_S32>), grid, block, lds, s, p);
-    else if (p.w.zeros) hipLaunchKernelGGL((q4_held<X, RT, NK, GB, Q4_S16Z>), grid, block, lds, s, p);
-    else hipLaunchKernelGGL((q4_held<X, RT, NK, GB, Q4_S16>), grid, block, lds, s, p);
+template <int X, int NK, int GB>
+static void q4_held_launch(const Q4P& p, int nw, hipStream_t s) {
+    const int by = (int)((p.rows + 15) / 16);
+    // the chip full once: two workgroups of four waves a CU, or one
+    const dim3 grid(std::min(p.w.NT, std::max(8, (nw == 4 ? 512 : 256) / by)), by), block(64 * nw);
+    const size_t lds = (size_t)2 * nw * 64 * 16;
+    if (!p.w.sbf16) hipLaunchKernelGGL((q4_held<X, NK, GB, Q4_S32>), grid, block, lds, s, p);
+    else if (p.w.zeros) hipLaunchKernelGGL((q4_held<X, NK, GB, Q4_S16Z>), grid, block, lds, s, p);
+    else hipLaunchKernelGGL((q4_held<X, NK, GB, Q4_S16>), grid, block, lds, s, p);
 }
 template <int X, int RT, int C, int GB>
 static void q4_walk_launch(const Q4P& p, hipStream_t s) {
@@ -493,13 +478,23 @@ static void q4_walk_launch(const Q4P& p, hipStream_t s) {
     else if (p.w.zeros) hipLaunchKernelGGL((q4_walk<X, RT, C, GB, Q4_S16Z>), grid, block, lds, s, p);
     else hipLaunchKernelGGL((q4_walk<X, RT, C, GB, Q4_S16>), grid, block, lds, s, p);
 }
+// The rows in registers wherever twelve waves hold them (60 blocks of k, f32 24), as four, eight or
+// twelve waves, which load the four SIMDs evenly; else the walk.  us held / walked, bf16 at 2560 x 10240:
+// 32 rows 12.8 / 19.9, 64 rows 16.4 / 26.7, 256 rows 41 / 78; int8 64 rows 14.5 / 23.4, at 5120 x
+// 2560 15.5 / 14.7; f32 one row 8.9 / 27.
 template <int X, int GB>
 static void q4_shape(const Q4P& p, hipStream_t s) {
-    // twelve waves at most hold the rows
-    constexpr int NK1 = X == Q4_F32 ? 2 : 4, NK2 = X == Q4_I8 ? 3 : 2;
-    if (p.rows <= 16 && p.w.KB <= 12 * NK1) q4_held_launch<X, 1, NK1, GB>(p, s);
-    else if (X != Q4_F32 && p.rows > 16 && p.w.KB <= 12 * NK2) q4_held_launch<X == Q4_F32 ? Q4_BF16 : X, 2, NK2, GB>(p, s);
-    else q4_walk_launch<X, 2, 2, GB>(p, s);
+    constexpr int most = X == Q4_F32 ? 2 : 5;  // blocks of k whose operands a wave's registers hold
+    const int nw = p.w.KB <= 4 * most ? 4 : p.w.KB <= 8 * most ? 8 : 12, NK = ceil_div(p.w.KB, nw);
+    if (NK > most) return q4_walk_launch<X, 2, 2, GB>(p, s);
+    if constexpr (X == Q4_F32) {
+        q4_held_launch<X, 2, GB>(p, nw, s);
+    } else {
+        if (NK <= 2) q4_held_launch<X, 2, GB>(p, nw, s);
+        else if (NK == 3) q4_held_launch<X, 3, GB>(p, nw, s);
+        else if (NK == 4) q4_held_launch<X, 4, GB>(p, nw, s);
+        else q4_held_launch<X, 5, GB>(p, nw, s);
+    }
 }
 template <int X>
 static void q4_dispatch(const Q4P& p, hipStream_t s) {

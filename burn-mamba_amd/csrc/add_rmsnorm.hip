@@ -7,6 +7,13 @@
 //
 // The sum is normalised as it is in f32, before it is rounded to the stream's type: y
 // then has one rounding.  The backward reads the stored s.
+//
+// Some ten operations an element against three or four elements moved: HBM-bound.  Rows of up to
+// 10240 bf16 or 5120 f32 stream elements stay in registers, so that each element is read
+// once: G lanes hold a row, E = 16 bytes of the stream a lane and step, G = 16, 64 or 256 by the
+// row's width; the next row's loads are in flight while this one is summed.  The backward's
+// workgroups take rows in turn and sum dw of their columns in registers, joined in LDS
+// and, over the workgroups, by arn_dw_join, in a fixed order.
 #include <algorithm>
 
 #include "pack.h"
@@ -65,6 +72,275 @@ __device__ __forceinline__ uint8_t arn_q8(float v, ArnScale s, bool e4m3) {
     const float t = v * s.inv;
     if (e4m3) return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(fminf(fmaxf(t, -448.f), 448.f), 0.f, 0, false);
     return (uint8_t)(int8_t)(int)rintf(fminf(fmaxf(t, -127.f), 127.f));
+}
+
+// ---- rows in registers
+// Sum, or largest, over aligned groups of G lanes in every lane; over the workgroup for G = 256
+// (red: 4 places, which no wave may still read from a sum before the last barrier: the callers
+// alternate between two sets).
+template <int CTRL>
+__device__ __forceinline__ uint32_t arn_dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true); }
+struct ArnAdd {
+    __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }
+};
+struct ArnMax {
+    __device__ __forceinline__ uint32_t operator()(uint32_t a, uint32_t b) const { return max(a, b); }
+};
+template <int G, typename Op>
+__device__ __forceinline__ uint32_t arn_all(uint32_t v, uint32_t* red, Op op) {
+    v = op(v, arn_dpp<0xB1>(v));   // xor 1
+    v = op(v, arn_dpp<0x4E>(v));   // xor 2
+    v = op(v, arn_dpp<0x141>(v));  // the other quad of the half row
+    v = op(v, arn_dpp<0x140>(v));  // the other half row
+    if constexpr (G >= 64) {
+        const uint32_t a = op((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
+        v = op(a, op((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
+    }
+    if constexpr (G == 256) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = op(op(red[0], red[1]), op(red[2], red[3]));
+    }
+    return v;
+}
+template <int G>
+__device__ __forceinline__ float arn_sum(float v, uint32_t* red) { return __uint_as_float(arn_all<G>(__float_as_uint(v), red, ArnAdd())); }
+
+// elements of a lane and step: 16 bytes of the stream
+template <typename S>
+constexpr int kArnE = 16 / (int)sizeof(S);
+
+// E consecutive results of 8 bits, the first n of them
+template <int E>
+__device__ __forceinline__ void arn_put8(uint8_t* q, int n, const float (&v)[E], ArnScale sc, bool e4m3) {
+    uint32_t w[E / 4];
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+        float t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float top = e4m3 ? 448.f : 127.f;
+            t[j] = sc.inv == 0.f ? 0.f : __builtin_amdgcn_fmed3f(v[i + j] * sc.inv, -top, top);
+        }
+        if (e4m3) {
+            const int a = __builtin_amdgcn_cvt_pk_fp8_f32(t[0], t[1], 0, false);
+            w[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], a, true);
+        } else {
+            uint32_t b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = (uint32_t)(int)rintf(t[j]) & 255u;
+            w[i / 4] = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+        }
+    }
+    if (n >= E) {
+        __builtin_memcpy(q, w, E);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (i < n) q[i] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
+    }
+}
+
+// G lanes a row, V steps: G (V - 1) E < cols <= G V E, so that only the last step can pass the row's
+// end.  Q: rows of 8 bits.
+template <typename T, typename S, int G, int V, bool Q>
+__global__ __launch_bounds__(256) void arn_fwd_rows(ArnP p) {
+    constexpr int E = kArnE<S>, RB = 256 / G;
+    __shared__ uint32_t red[16];
+    const int l = threadIdx.x % G, sub = threadIdx.x / G;
+    Elems<T, E> rx[V];
+    Elems<S, E> rr[V];
+    auto fetch = [&](int64_t r) __attribute__((always_inline)) {
+        if (r >= p.rows) return;
+        const T* x = static_cast<const T*>(p.x) + r * p.x_sr;
+        const S* res = static_cast<const S*>(p.res) + r * p.res_sr;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E, n = p.cols - c;
+            if (k < V - 1 || n >= E) {
+                rx[k].load(x + c);
+                if (p.res) rr[k].load(res + c);
+            } else {
+                rx[k].load_part(x + c, n);
+                if (p.res) rr[k].load_part(res + c, n);
+            }
+        }
+    };
+    fetch(blockIdx.x * (int64_t)RB + sub);
+    float w[V][E];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int c = (k * G + l) * E;
+        if (p.w) ld_run<E, float>(p.w + c, k < V - 1 ? E : p.cols - c, w[k]);
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (!p.w) w[k][i] = 1.f;
+    }
+    const float inv = 1.f / (float)p.cols;
+    const int64_t step = (int64_t)gridDim.x * RB;
+    int odd = 0;
+    // every group of a workgroup makes the same number of turns (the sums of G = 256 meet at a barrier)
+    for (int64_t r0 = blockIdx.x * (int64_t)RB; r0 < p.rows; r0 += step) {
+        const int64_t r = r0 + sub;
+        float v[V][E], ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            rx[k].get(v[k]);
+            if (p.res) {
+                float b[E];
+                rr[k].get(b);
+#pragma unroll
+                for (int i = 0; i < E; ++i) v[k][i] += b[i];
+            }
+        }
+        fetch(r + step);
+        if (p.s && r < p.rows) {
+            S* s = static_cast<S*>(p.s) + r * p.s_sr;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const int c = (k * G + l) * E, n = k < V - 1 ? E : p.cols - c;
+                if (n > 0) st_run<E, S>(s + c, n, v[k]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+            for (int i = 0; i < E; ++i) ss = __builtin_fmaf(v[k][i], v[k][i], ss);  // zeros past the row's end
+        const float rstd = 1.f / sqrtf(__builtin_fmaf(arn_sum<G>(ss, red + 8 * odd), inv, p.eps));
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[k][i] = v[k][i] * rstd * w[k][i];
+        ArnScale sc{};
+        if constexpr (Q) {
+            uint32_t amax = 0;
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (k < V - 1 || (k * G + l) * E + i < p.cols) amax = max(amax, __float_as_uint(v[k][i]) & 0x7fffffffu);
+            sc = arn_scale(arn_all<G>(amax, red + 8 * odd + 4, ArnMax()), p.e4m3);
+        }
+        odd ^= 1;
+        if (r >= p.rows) continue;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E, n = k < V - 1 ? E : p.cols - c;
+            if (n <= 0) break;
+            if constexpr (Q) arn_put8<E>(p.q + r * p.q_sr + c, n, v[k], sc, p.e4m3);
+            else st_run<E, T>(static_cast<T*>(p.y) + r * p.y_sr + c, n, v[k]);
+        }
+        if (l == 0) {
+            if (p.rstd) p.rstd[r] = rstd;
+            if constexpr (Q) p.scale[r] = sc.scale;
+        }
+    }
+}
+
+// The workgroups take their rows in turn; part[blockIdx.x] gets the workgroup's dw.
+template <typename T, typename S, int G, int V>
+__global__ __launch_bounds__(256) void arn_bwd_rows(ArnP p) {
+    constexpr int E = kArnE<S>, RB = 256 / G;
+    __shared__ uint32_t red[8];
+    __shared__ float s_w[G < 256 ? G * V * E : 1];  // after the rows, the groups' sums
+    const int l = threadIdx.x % G, sub = threadIdx.x / G;
+    Elems<S, E> rs[V], rd[V];
+    Elems<T, E> rg[V];
+    float rstd = 0.f, dw[V][E], w[V][E];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int c = (k * G + l) * E;
+        if (p.w) ld_run<E, float>(p.w + c, k < V - 1 ? E : p.cols - c, w[k]);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            if (!p.w) w[k][i] = 1.f;
+            dw[k][i] = 0.f;
+        }
+    }
+    auto fetch = [&](int64_t r) __attribute__((always_inline)) {
+        if (r >= p.rows) return;
+        const S* s = static_cast<const S*>(p.s) + r * p.s_sr;
+        const S* d = static_cast<const S*>(p.ds) + r * p.ds_sr;
+        const T* g = static_cast<const T*>(p.dy) + r * p.dy_sr;
+        rstd = p.rstd[r];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E, n = p.cols - c;
+            if (k < V - 1 || n >= E) {
+                rs[k].load(s + c);
+                rg[k].load(g + c);
+                if (p.ds) rd[k].load(d + c);
+            } else {
+                rs[k].load_part(s + c, n);
+                rg[k].load_part(g + c, n);
+                if (p.ds) rd[k].load_part(d + c, n);
+            }
+        }
+    };
+    const float inv = 1.f / (float)p.cols;
+    const int64_t step = (int64_t)gridDim.x * RB;
+    int odd = 0;
+    fetch(blockIdx.x * (int64_t)RB + sub);
+    for (int64_t r0 = blockIdx.x * (int64_t)RB; r0 < p.rows; r0 += step) {
+        const int64_t r = r0 + sub;
+        const bool live = r < p.rows;
+        float xh[V][E], g[V][E], d[V][E], dot = 0.f;
+        const float rsd = rstd;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            rs[k].get(xh[k]);
+            rg[k].get(g[k]);
+            if (p.ds) rd[k].get(d[k]);
+        }
+        fetch(r + step);
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+#pragma unroll
+                for (int i = 0; i < E; ++i) {  // zeros past the row's end
+                    xh[k][i] *= rsd;
+                    dw[k][i] = __builtin_fmaf(g[k][i], xh[k][i], dw[k][i]);
+                    g[k][i] *= w[k][i];
+                    dot = __builtin_fmaf(g[k][i], xh[k][i], dot);
+                }
+        }
+        dot = arn_sum<G>(dot, red + 4 * odd) * inv;
+        odd ^= 1;
+        if (!live) continue;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E, n = k < V - 1 ? E : p.cols - c;
+            if (n <= 0) break;
+            float o[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) o[i] = __builtin_fmaf(rsd, __builtin_fmaf(-xh[k][i], dot, g[k][i]), p.ds ? d[k][i] : 0.f);
+            if (p.y) st_run<E, T>(static_cast<T*>(p.y) + r * p.y_sr + c, n, o);
+            if (p.dres) st_run<E, S>(static_cast<S*>(p.dres) + r * p.dres_sr + c, n, o);
+        }
+    }
+    if (!p.part) return;
+    float* part = p.part + (int64_t)blockIdx.x * p.cols;
+    if constexpr (G < 256) {  // the workgroup's groups, one behind the other
+        for (int q = 0; q < RB; ++q) {
+            if (sub == q) {
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) {
+                        const int at = (k * E + i) * G + l;
+                        s_w[at] = q ? s_w[at] + dw[k][i] : dw[k][i];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < p.cols; c += 256) part[c] = s_w[(c / (G * E) * E + c % E) * G + c / E % G];
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * G + l) * E, n = p.cols - c;
+            if (n > 0) st_run<E, float>(part + c, n, dw[k]);
+        }
+    }
 }
 
 // Any width: a workgroup per row, the row read once per sweep.
@@ -222,16 +498,56 @@ __global__ __launch_bounds__(256) void arn_dw_join(ArnP p) {
 }
 
 static uint32_t arn_grid(int64_t rows) { return (uint32_t)std::min<int64_t>(rows, 1 << 20); }
-static int arn_parts(int64_t rows) { return (int)std::min<int64_t>(256, (rows + 31) / 32); }
+// steps of 16 stream bytes a lane that the columns take with G lanes a row
+static int arn_steps(int cols, int E, int G) { return ceil_div(cols, G * E); }
+// Lanes a row, 0: the row is not held in registers.
+static int arn_lanes(int cols, int E) {
+    return arn_steps(cols, E, 16) <= 2 ? 16 : arn_steps(cols, E, 64) <= 3 ? 64 : arn_steps(cols, E, 256) <= 5 ? 256 : 0;
+}
+static uint32_t arn_fwd_grid(int64_t rows, int G) { return (uint32_t)std::min<int64_t>((rows + 256 / G - 1) / (256 / G), 2048); }
+// Workgroups of the backward, some eight rows a group at least, so that the parts stay few beside the rows.
+static int arn_parts(int64_t rows, int cols, int E) {
+    const int G = arn_lanes(cols, E);
+    if (G == 0) return (int)std::min<int64_t>(256, (rows + 31) / 32);
+    return (int)std::min<int64_t>(1024, (rows + 8 * (256 / G) - 1) / (8 * (256 / G)));
+}
+
+template <typename T, typename S, int G, int V>
+static void arn_rows_launch(const ArnP& p, bool back, hipStream_t s) {
+    if (back) hipLaunchKernelGGL((arn_bwd_rows<T, S, G, V>), dim3(p.parts), dim3(256), 0, s, p);
+    else if (p.q) hipLaunchKernelGGL((arn_fwd_rows<T, S, G, V, true>), dim3(arn_fwd_grid(p.rows, G)), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((arn_fwd_rows<T, S, G, V, false>), dim3(arn_fwd_grid(p.rows, G)), dim3(256), 0, s, p);
+}
+// rows in registers; false where they are too wide
+template <typename T, typename S>
+static bool arn_rows(const ArnP& p, bool back, hipStream_t s) {
+    const int G = arn_lanes(p.cols, kArnE<S>);
+    if (G == 0) return false;
+    switch (G * 8 + arn_steps(p.cols, kArnE<S>, G)) {
+        case 16 * 8 + 1: arn_rows_launch<T, S, 16, 1>(p, back, s); break;
+        case 16 * 8 + 2: arn_rows_launch<T, S, 16, 2>(p, back, s); break;
+        case 64 * 8 + 1: arn_rows_launch<T, S, 64, 1>(p, back, s); break;
+        case 64 * 8 + 2: arn_rows_launch<T, S, 64, 2>(p, back, s); break;
+        case 64 * 8 + 3: arn_rows_launch<T, S, 64, 3>(p, back, s); break;
+        case 256 * 8 + 1: arn_rows_launch<T, S, 256, 1>(p, back, s); break;
+        case 256 * 8 + 2: arn_rows_launch<T, S, 256, 2>(p, back, s); break;
+        case 256 * 8 + 3: arn_rows_launch<T, S, 256, 3>(p, back, s); break;
+        case 256 * 8 + 4: arn_rows_launch<T, S, 256, 4>(p, back, s); break;
+        default: arn_rows_launch<T, S, 256, 5>(p, back, s);
+    }
+    return true;
+}
 
 template <typename T, typename S>
 static void arn_fwd_launch(const ArnP& p, hipStream_t s) {
-    hipLaunchKernelGGL((arn_fwd_wide<T, S>), dim3(arn_grid(p.rows)), dim3(256), 0, s, p);
+    if (!arn_rows<T, S>(p, false, s)) hipLaunchKernelGGL((arn_fwd_wide<T, S>), dim3(arn_grid(p.rows)), dim3(256), 0, s, p);
 }
 template <typename T, typename S>
 static void arn_bwd_launch(const ArnP& p, hipStream_t s) {
-    if (p.rows && (p.y || p.dres)) hipLaunchKernelGGL((arn_dx_wide<T, S>), dim3(arn_grid(p.rows)), dim3(256), 0, s, p);
-    if (p.rows && p.dw) hipLaunchKernelGGL((arn_dw_wide<T, S>), dim3(ceil_div(p.cols, 256), p.parts), dim3(256), 0, s, p);
+    if (p.rows && !arn_rows<T, S>(p, true, s)) {
+        if (p.y || p.dres) hipLaunchKernelGGL((arn_dx_wide<T, S>), dim3(arn_grid(p.rows)), dim3(256), 0, s, p);
+        if (p.dw) hipLaunchKernelGGL((arn_dw_wide<T, S>), dim3(ceil_div(p.cols, 256), p.parts), dim3(256), 0, s, p);
+    }
     if (p.dw) hipLaunchKernelGGL(arn_dw_join, dim3((uint32_t)std::min(ceil_div(p.cols, 16), 1 << 20)), dim3(256), 0, s, p);
 }
 
@@ -296,7 +612,7 @@ extern "C" int mamba_add_rmsnorm_fwd(const mamba_add_rmsnorm_args* a, mamba_stre
 
 extern "C" size_t mamba_add_rmsnorm_bwd_workspace_size(const mamba_add_rmsnorm_bwd_args* a) {
     if (a == nullptr || arn_check(a->rows, a->cols, a->io_dtype, a->stream_dtype) != MAMBA_OK || !a->dweight) return 0;
-    return (size_t)arn_parts(a->rows) * a->cols * 4;
+    return (size_t)arn_parts(a->rows, a->cols, a->stream_dtype == MAMBA_BF16 ? 8 : 4) * a->cols * 4;
 }
 
 extern "C" int mamba_add_rmsnorm_bwd(const mamba_add_rmsnorm_bwd_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {
@@ -321,7 +637,7 @@ extern "C" int mamba_add_rmsnorm_bwd(const mamba_add_rmsnorm_bwd_args* a, void* 
     ArnP p{};
     p.rows = R; p.cols = C; p.s = const_cast<void*>(a->s); p.s_sr = a->s_sr; p.dy = a->dy; p.dy_sr = a->dy_sr; p.ds = a->ds; p.ds_sr = a->ds_sr;
     p.w = a->weight; p.rstd = const_cast<float*>(a->rstd); p.y = a->dx; p.y_sr = a->dx_sr; p.dres = a->dresidual; p.dres_sr = a->dresidual_sr;
-    p.part = need ? static_cast<float*>(ws) : nullptr; p.parts = arn_parts(R); p.dw = a->dweight;
+    p.part = need ? static_cast<float*>(ws) : nullptr; p.parts = arn_parts(R, C, 16 / f); p.dw = a->dweight;
     ARN_DISPATCH(arn_bwd_launch, a->io_dtype, a->stream_dtype, p, (hipStream_t)stream);
     MAMBA_CHECK_LAUNCH();
     return MAMBA_OK;

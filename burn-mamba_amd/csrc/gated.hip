@@ -11,8 +11,8 @@
 //
 // With one state a channel some 30 (forward) to 90 (backward) operations stand against 8 to
 // 18 bytes an element of bf16, so memory bounds it, and every row is read once: the rows are
-// cut into tiles of 64 without regard to the sequences, a workgroup takes one tile of 128
-// channels, keeps it in registers, and finds the state that enters it while the tile is there.
+// cut into tiles (of 64; the forward of bf16: 128) without regard to the sequences, a workgroup
+// takes one tile of 128 channels, keeps it in registers, and finds the state that enters it while the tile is there.
 // A stretch of rows maps the state that enters it, h -> P h + H; P is the product of its
 // decays and H what it leaves from zero.  A lane holds R rows of two channels; its map and
 // the maps of the eight waves are joined in LDS to the tile's, which is published to the
@@ -66,7 +66,10 @@ constexpr int kCarryRows = 64;  // rows between the states that the forward keep
 constexpr int kGW = 8, kGV = 2, kGC = 64 * kGV;  // waves of a workgroup, channels of a lane and of a tile
 constexpr int kGGroup = 32;                      // tiles of a group
 constexpr uint64_t kGNone = ~0ull;               // nothing published yet
-constexpr int kGRows = kCarryRows / kGW;         // rows of a lane: a tile has kCarryRows
+// rows of a lane: a tile of the backward has kCarryRows, one of the forward as many or twice that
+constexpr int kGRows = kCarryRows / kGW;
+template <typename T>
+constexpr int kGFwdRows = sizeof(T) == 2 ? 2 * kGRows : kGRows;
 
 // s(v) = 1 / (1 + exp(-v)) and s(-v) = 1 - s(v), by the hardware's exp2 and reciprocal (one
 // step each); 0 and 1 at the ends.  s(-v) of a large v is exp(-v) s(v): the difference from 1
@@ -80,21 +83,25 @@ __device__ __forceinline__ Logistic g_logistic(float v) {
     return {s, v > 0.f ? e * s : 1.f - s};
 }
 
-// a = exp(v) and m = sqrt(1 - a^2) for v <= 0, both to a few steps of their own size.  Above
-// -1/4 from e = exp(v) - 1, the series to v^7 / 7! (its next term is 2^-29 of the sum there):
-// a = 1 + e, 1 - a^2 = -e (2 + e) keep what a difference from 1 would lose as a nears 1.
-struct Decay { float a, m; };
+// a = exp(v) and q = 1 - a^2 for v <= 0, both to a few steps of their own size.  From -1/8 up by
+// e = exp(v) - 1, the series to v^5 / 5! (its next term is 2^-24 of the sum there): a = 1 + e,
+// 1 - a^2 = -e (2 + e) keep what a difference from 1 would lose as a nears 1.  The exponential,
+// for what lies below, is passed over where no lane needs it.
+struct Decay { float a, q; };
 __device__ __forceinline__ Decay g_decay(float v) {
-    float e = 1.f / 5040.f;
-    e = __builtin_fmaf(e, v, 1.f / 720.f);
-    e = __builtin_fmaf(e, v, 1.f / 120.f);
+    float e = 1.f / 120.f;
     e = __builtin_fmaf(e, v, 1.f / 24.f);
     e = __builtin_fmaf(e, v, 1.f / 6.f);
     e = __builtin_fmaf(e, v, 0.5f);
     e = __builtin_fmaf(e, v, 1.f) * v;
-    const float far = __builtin_amdgcn_exp2f(v * 1.44269504088896341f);
-    const bool near = v >= -0.25f;
-    return {near ? 1.f + e : far, __builtin_amdgcn_sqrtf(near ? -e * (2.f + e) : __builtin_fmaf(-far, far, 1.f))};
+    Decay d = {1.f + e, -e * (2.f + e)};
+    const bool near = v >= -0.125f;  // not of a NaN
+    if (__ballot(!near)) {
+        const float far = __builtin_amdgcn_exp2f(v * 1.44269504088896341f);
+        d.a = near ? d.a : far;
+        d.q = near ? d.q : __builtin_fmaf(-far, far, 1.f);
+    }
+    return d;
 }
 
 // What the R rows from t0 are (R <= 64, t0 uniform over the wave): bit j of a mask for row
@@ -184,7 +191,7 @@ __device__ __forceinline__ void g_tile(const GatedP& p, GShared& s, int& o, int&
 // from the end of the group before o's.  Called by the whole workgroup (o > far >= 0).
 __device__ __forceinline__ void g_enter(const GatedP& p, GShared& s, int o, int ct, int far, float (&h)[kGV]) {
     const int w = wave_id(), l = threadIdx.x & 63;
-    const int64_t Dp = (int64_t)p.nct * kGC, at = (int64_t)ct * kGC + l * kGV;
+    const int64_t Dp = (int64_t)p.nct * kGC, at = (int64_t)ct * kGC + l;
     const int base = o / kGGroup * kGGroup, from = max(far, base);
     const bool group = far < base;
     const int per = (o - from + kGW - 1) / kGW, k0 = min(o, from + w * per), k1 = min(o, k0 + per);
@@ -195,18 +202,18 @@ __device__ __forceinline__ void g_enter(const GatedP& p, GShared& s, int o, int 
 #pragma unroll
     for (int i = 0; i < kGGroup / kGW; ++i)
 #pragma unroll
-        for (int v = 0; v < kGV; ++v) word[i][v] = k0 + i < k1 ? g_peek(p.map + (int64_t)(k0 + i) * Dp + at + v) : 0;
+        for (int v = 0; v < kGV; ++v) word[i][v] = k0 + i < k1 ? g_peek(p.map + (int64_t)(k0 + i) * Dp + at + 64 * v) : 0;
     const uint64_t* ends = p.ends + (int64_t)(base / kGGroup - 1) * Dp + at;
     if (group && w == 0) {
 #pragma unroll
-        for (int v = 0; v < kGV; ++v) end[v] = g_peek(ends + v);
+        for (int v = 0; v < kGV; ++v) end[v] = g_peek(ends + 64 * v);
     }
 #pragma unroll
     for (int i = 0; i < kGGroup / kGW; ++i) {
         if (k0 + i >= k1) break;
 #pragma unroll
         for (int v = 0; v < kGV; ++v) {
-            const uint64_t x = g_wait(p.map + (int64_t)(k0 + i) * Dp + at + v, word[i][v]);
+            const uint64_t x = g_wait(p.map + (int64_t)(k0 + i) * Dp + at + 64 * v, word[i][v]);
             const float P = __uint_as_float((uint32_t)x), H = __uint_as_float((uint32_t)(x >> 32));
             m.H[v] = i ? __builtin_fmaf(P, m.H[v], H) : H;
             m.P[v] = i ? P * m.P[v] : P;
@@ -214,7 +221,7 @@ __device__ __forceinline__ void g_enter(const GatedP& p, GShared& s, int o, int 
     }
     if (group && w == 0) {
 #pragma unroll
-        for (int v = 0; v < kGV; ++v) s.in[v][l] = __uint_as_float((uint32_t)(g_wait(ends + v, end[v]) >> 32));
+        for (int v = 0; v < kGV; ++v) s.in[v][l] = __uint_as_float((uint32_t)(g_wait(ends + 64 * v, end[v]) >> 32));
     }
 #pragma unroll
     for (int v = 0; v < kGV; ++v) s.P2[w][v][l] = m.P[v], s.H2[w][v][l] = m.H[v];
@@ -231,15 +238,21 @@ __device__ __forceinline__ void g_enter(const GatedP& p, GShared& s, int o, int 
 // channels; 1: an odd one, whose last lane takes the second of the two; 2: a single channel.
 template <int MODE>
 __device__ __forceinline__ int g_column(int c, int D) { return MODE == 2 ? c : min(c, D - kGV); }
+// (row: uniform; an unsigned offset keeps the address a scalar base and one register)
 template <typename T, int MODE>
 __device__ __forceinline__ void g_load(Elems<T, kGV>& e, const T* row, int cl, int n) {
-    if constexpr (MODE == 2) e.load_part(row + cl, n);
-    else e.load(row + cl);
+    const T* at = reinterpret_cast<const T*>(reinterpret_cast<const char*>(row) + (uint32_t)cl * (uint32_t)sizeof(T));
+    if constexpr (MODE == 2) e.load_part(at, n);
+    else e.load(at);
+}
+template <typename T>
+__device__ __forceinline__ void g_store(T* row, int c, int n, const float (&v)[kGV]) {
+    st_run<kGV, T>(reinterpret_cast<T*>(reinterpret_cast<char*>(row) + (uint32_t)c * (uint32_t)sizeof(T)), n, v);
 }
 
 template <typename T, int MODE>
 __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
-    constexpr int R = kGRows;
+    constexpr int R = kGFwdRows<T>;
     __shared__ GShared s;
     int o, ct;
     g_tile(p, s, o, ct);
@@ -276,7 +289,7 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
         for (int v = 0; v < kGV; ++v) {
             const Decay d = g_decay(A[v] * g_sigmoid(r[v]));
             a[j][v] = d.a;
-            b[j][v] = d.m * (g_sigmoid(i[v]) * x[v]);
+            b[j][v] = __builtin_amdgcn_sqrtf(d.q) * (g_sigmoid(i[v]) * x[v]);
         }
     }
     GMap m;
@@ -319,7 +332,7 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
     if (p.z) fetch(ez, p.z, p.z_st);
     __syncthreads();
     float h[kGV] = {0.f, 0.f};
-    const int64_t at = (int64_t)o * p.nct * kGC + c;
+    const int64_t at = ((int64_t)o * p.nct + ct) * kGC + l;
     const bool ends = (o + 1) % kGGroup == 0 && o + 1 < p.ntile;
     GMap whole;
     bool cut = false;
@@ -336,14 +349,14 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
             }
         }
 #pragma unroll
-        for (int v = 0; v < kGV; ++v) g_publish(p.map + at + v, g_word(whole.P[v], whole.H[v]));
+        for (int v = 0; v < kGV; ++v) g_publish(p.map + at + 64 * v, g_word(whole.P[v], whole.H[v]));
     }
     const int far = __builtin_amdgcn_readfirstlane(s.far);
     if (far >= 0) g_enter(p, s, o, ct, far, h);
     if (w == kGW - 1 && ends) {
 #pragma unroll
         for (int v = 0; v < kGV; ++v)
-            g_publish(p.ends + (int64_t)(o / kGGroup) * p.nct * kGC + c + v, g_word(0.f, cut ? whole.H[v] : __builtin_fmaf(whole.P[v], h[v], whole.H[v])));
+            g_publish(p.ends + ((int64_t)(o / kGGroup) * p.nct + ct) * kGC + l + 64 * v, g_word(0.f, cut ? whole.H[v] : __builtin_fmaf(whole.P[v], h[v], whole.H[v])));
     }
     for (int k = 0; k < w; ++k) {
         const bool here = s.cut[k] != 0;
@@ -362,7 +375,7 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
 #pragma unroll
             for (int v = 0; v < kGV; ++v) y[v] = h[v];
         }
-        st_run<kGV, T>(static_cast<T*>(p.y) + (t0 + j) * p.y_st + c, n, y);
+        g_store<T>(static_cast<T*>(p.y) + (t0 + j) * p.y_st, c, n, y);
     };
     if (plain) {
 #pragma unroll
@@ -374,11 +387,10 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
     } else {
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            if (j >= rows) break;
             if (!g_bit(g.live, j)) {
 #pragma unroll
                 for (int v = 0; v < kGV; ++v) h[v] = 0.f;
-                if (p.fill) st_run<kGV, T>(static_cast<T*>(p.y) + (t0 + j) * p.y_st + c, n, h);
+                if (p.fill && j < rows) g_store<T>(static_cast<T*>(p.y) + (t0 + j) * p.y_st, c, n, h);
                 continue;
             }
 #pragma unroll
@@ -423,7 +435,7 @@ __global__ __launch_bounds__(64 * kGW, 2) void gated_bwd(GatedP p) {
     ld_run<kGV, float>(p.carry + (int64_t)tile * p.D + c, n, hin);
     constexpr uint64_t full = (1ull << R) - 1;
     const bool plain = g.live == full && (g.first | g.last) == 0;
-    float a[R][kGV], m[R][kGV], b[R][kGV];  // b: m u, and then the state before the row
+    float a[R][kGV], m[R][kGV], im[R][kGV], b[R][kGV];  // im: 1 / m; b: m u, and then the state before the row
 #pragma unroll
     for (int j = 0; j < R; ++j) {
         float r[kGV], i[kGV], x[kGV];
@@ -434,8 +446,10 @@ __global__ __launch_bounds__(64 * kGW, 2) void gated_bwd(GatedP p) {
         for (int v = 0; v < kGV; ++v) {
             const Decay d = g_decay(A[v] * g_sigmoid(r[v]));
             a[j][v] = d.a;
-            m[j][v] = d.m;
-            b[j][v] = d.m * (g_sigmoid(i[v]) * x[v]);
+            const float q = d.q;
+            im[j][v] = q > 0.f ? __builtin_amdgcn_rsqf(q) : q * 0.f;  // 0 where a is 1, a NaN of a NaN
+            m[j][v] = q * im[j][v];
+            b[j][v] = m[j][v] * (g_sigmoid(i[v]) * x[v]);
         }
     }
     auto start = [&](int j, float (&h)[kGV]) __attribute__((always_inline)) {  // what the sequence of row j starts from
@@ -521,7 +535,7 @@ __global__ __launch_bounds__(64 * kGW, 2) void gated_bwd(GatedP p) {
 #pragma unroll
         for (int v = 0; v < kGV; ++v) h[v] = here ? s.H2[k][v][l] : __builtin_fmaf(s.P2[k][v][l], h[v], s.H2[k][v][l]);
     }
-    const int64_t at = (int64_t)o * p.nct * kGC + c;
+    const int64_t at = ((int64_t)o * p.nct + ct) * kGC + l;
     const bool ends = (o + 1) % kGGroup == 0 && o + 1 < p.ntile;
     GMap whole;
     bool cut = false;
@@ -538,7 +552,7 @@ __global__ __launch_bounds__(64 * kGW, 2) void gated_bwd(GatedP p) {
             }
         }
 #pragma unroll
-        for (int v = 0; v < kGV; ++v) g_publish(p.map + at + v, g_word(whole.P[v], whole.H[v]));
+        for (int v = 0; v < kGV; ++v) g_publish(p.map + at + 64 * v, g_word(whole.P[v], whole.H[v]));
     }
 #pragma unroll
     for (int j = 0; j < R; ++j) {  // b: the state before the row
@@ -562,7 +576,7 @@ __global__ __launch_bounds__(64 * kGW, 2) void gated_bwd(GatedP p) {
     if (w == 0 && ends) {
 #pragma unroll
         for (int v = 0; v < kGV; ++v)
-            g_publish(p.ends + (int64_t)(o / kGGroup) * p.nct * kGC + c + v, g_word(0.f, cut ? whole.H[v] : __builtin_fmaf(whole.P[v], qin[v], whole.H[v])));
+            g_publish(p.ends + ((int64_t)(o / kGGroup) * p.nct + ct) * kGC + l + 64 * v, g_word(0.f, cut ? whole.H[v] : __builtin_fmaf(whole.P[v], qin[v], whole.H[v])));
     }
     for (int k = kGW - 1; k > w; --k) {
         const bool here = s.cut[k] != 0;
@@ -571,7 +585,7 @@ __global__ __launch_bounds__(64 * kGW, 2) void gated_bwd(GatedP p) {
     }
     float dA[kGV] = {0.f, 0.f};
     auto put = [&](void* to, int64_t st, int j, const float (&v)[kGV]) __attribute__((always_inline)) {
-        st_run<kGV, T>(static_cast<T*>(to) + (t0 + j) * st + c, n, v);
+        g_store<T>(static_cast<T*>(to) + (t0 + j) * st, c, n, v);
     };
 #pragma unroll
     for (int j = R - 1; j >= 0; --j) {
@@ -598,7 +612,7 @@ __global__ __launch_bounds__(64 * kGW, 2) void gated_bwd(GatedP p) {
         for (int v = 0; v < kGV; ++v) {
             const Logistic sr = g_logistic(r[v]), si = g_logistic(i[v]);
             const float aj = a[j][v], mj = m[j][v], u = si.s * x[v], dh = gr[v] + qin[v], ah = aj * b[j][v], dm = dh * mj;
-            const float pull = mj > 0.f ? u * aj * aj * __builtin_amdgcn_rcpf(mj) : 0.f;
+            const float pull = u * aj * aj * im[j][v];
             const float e = dh * (ah - pull);
             dx[v] = dm * si.s;
             di[v] = dm * u * si.c;
@@ -676,7 +690,7 @@ __global__ __launch_bounds__(256) void gated_step(GatedStepP p) {
     const Decay g = g_decay(p.A[c] * g_sigmoid(load_f32<T>(static_cast<const T*>(p.r) + b * p.r_sb + c)));
     float* st = p.state + slot * p.D + c;
     const float u = g_sigmoid(load_f32<T>(static_cast<const T*>(p.i) + b * p.i_sb + c)) * load_f32<T>(static_cast<const T*>(p.x) + b * p.x_sb + c);
-    const float h = __builtin_fmaf(g.a, *st, g.m * u);
+    const float h = __builtin_fmaf(g.a, *st, __builtin_amdgcn_sqrtf(g.q) * u);
     *st = h;
     const float z = p.z ? load_f32<T>(static_cast<const T*>(p.z) + b * p.z_sb + c) : 0.f;
     store_f32<T>(y, p.z ? h * z * g_sigmoid(z) : h);
@@ -684,8 +698,9 @@ __global__ __launch_bounds__(256) void gated_step(GatedStepP p) {
 
 // The tiles of a call, and its workspace at ws (counted from NULL: its size): the ticket, the maps
 // and ends (none for one tile of rows: nothing is waited for), and the backward's sums.
-static size_t gated_plan(GatedP& p, bool back, void* ws) {
-    p.ntile = (int)((p.rows + kCarryRows - 1) / kCarryRows);
+static size_t gated_plan(GatedP& p, bool back, bool bf16, void* ws) {
+    const int tile = kGW * (back ? kGRows : bf16 ? kGFwdRows<bf16_t> : kGFwdRows<float>);
+    p.ntile = (int)((p.rows + tile - 1) / tile);
     p.nct = ceil_div(p.D, kGC);
     const int64_t Dp = (int64_t)p.nct * kGC, words = p.ntile > 1 ? (p.ntile + p.ntile / kGGroup) * Dp : 0;
     char* at = static_cast<char*>(ws);
@@ -745,7 +760,7 @@ using namespace mamba;
 extern "C" size_t mamba_gated_scan_workspace_size(const mamba_gated_scan_args* a) {
     GatedP p;
     if (gated_make(a, &p) != MAMBA_OK) return 0;
-    return gated_plan(p, false, nullptr);
+    return gated_plan(p, false, a->io_dtype == MAMBA_BF16, nullptr);
 }
 
 extern "C" int mamba_gated_scan_fwd(const mamba_gated_scan_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {
@@ -764,7 +779,7 @@ extern "C" int mamba_gated_scan_fwd(const mamba_gated_scan_args* a, void* ws, si
                         !rows_clash(a->y, a->y_st, a->z, a->z_st, p.D, p.D, p.rows, e, true),
                     "y overlaps an input (it may be x, r, i or z itself)");
     p.y = a->y; p.y_st = a->y_st; p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
-    const size_t need = gated_plan(p, false, ws);
+    const size_t need = gated_plan(p, false, a->io_dtype == MAMBA_BF16, ws);
     if ((st = gated_grid_ok(p)) != MAMBA_OK) return st;
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");
     if (need && (ws == nullptr || ws_bytes < need)) {
@@ -782,7 +797,7 @@ extern "C" int mamba_gated_scan_fwd(const mamba_gated_scan_args* a, void* ws, si
 extern "C" size_t mamba_gated_scan_bwd_workspace_size(const mamba_gated_scan_bwd_args* a) {
     GatedP p;
     if (a == nullptr || gated_make(&a->fwd, &p) != MAMBA_OK) return 0;
-    return gated_plan(p, true, nullptr);
+    return gated_plan(p, true, a->fwd.io_dtype == MAMBA_BF16, nullptr);
 }
 
 extern "C" int mamba_gated_scan_bwd(const mamba_gated_scan_bwd_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {
@@ -809,7 +824,7 @@ extern "C" int mamba_gated_scan_bwd(const mamba_gated_scan_bwd_args* a, void* ws
     p.h0 = a->initial_state; p.dhT = a->d_final_state; p.dh0 = a->d_initial_state; p.dA = a->dA;
     p.dy = a->dy; p.dy_st = a->dy_st; p.dx = a->dx; p.dx_st = a->dx_st; p.dr = a->dr; p.dr_st = a->dr_st;
     p.di = a->di; p.di_st = a->di_st; p.dz = a->dz; p.dz_st = a->dz_st;
-    const size_t need = gated_plan(p, true, ws);
+    const size_t need = gated_plan(p, true, a->fwd.io_dtype == MAMBA_BF16, ws);
     if ((st = gated_grid_ok(p)) != MAMBA_OK) return st;
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");
     if (need && (ws == nullptr || ws_bytes < need)) {

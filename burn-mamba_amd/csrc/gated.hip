@@ -11,14 +11,16 @@
 //
 // With one state a channel some 30 (forward) to 90 (backward) operations stand against 8 to
 // 18 bytes an element of bf16, so memory bounds it, and every row is read once: the rows are
-// cut into tiles (of 64; the forward of bf16: 128) without regard to the sequences, a workgroup
-// takes one tile of 128 channels, keeps it in registers, and finds the state that enters it while the tile is there.
+// cut into tiles (128 in the forward, 64 in the backward) without regard to the sequences, a
+// workgroup takes one tile of 64 channels, keeps it in registers, and finds the state that enters
+// it while the tile is there.
 // A stretch of rows maps the state that enters it, h -> P h + H; P is the product of its
-// decays and H what it leaves from zero.  A lane holds R rows of two channels; its map and
-// the maps of the eight waves are joined in LDS to the tile's, which is published to the
+// decays and H what it leaves from zero.  A lane holds R rows of one channel (two would take
+// twice the registers and leave the backward one workgroup a CU: 8192 x 5120 of bf16 360 us against
+// 245); the maps of the eight waves are joined in LDS to the tile's, which is published to the
 // other workgroups before the tile's own state is waited for.  That state is joined from the
 // published maps of the tiles before it, back to the one in which the tile's first sequence
-// begins, or to the last group of 32 tiles, whose final state its last tile publishes.  The
+// begins, or to the last group of 16 tiles, whose final state its last tile publishes.  The
 // joins follow a fixed order: the same inputs give the same bits.  The backward walks the other way
 // with q in the state's place, and finds h again from the states that the forward kept.
 //
@@ -63,13 +65,17 @@ struct GatedP {
 };
 
 constexpr int kCarryRows = 64;  // rows between the states that the forward keeps for the backward
-constexpr int kGW = 8, kGV = 2, kGC = 64 * kGV;  // waves of a workgroup, channels of a lane and of a tile
-constexpr int kGGroup = 32;                      // tiles of a group
+constexpr int kGW = 8, kGC = 64;  // waves of a workgroup; channels of a tile: one a lane
+constexpr int kGGroup = 16;                      // tiles of a group
 constexpr uint64_t kGNone = ~0ull;               // nothing published yet
-// rows of a lane: a tile of the backward has kCarryRows, one of the forward as many or twice that
-constexpr int kGRows = kCarryRows / kGW;
-template <typename T>
-constexpr int kGFwdRows = sizeof(T) == 2 ? 2 * kGRows : kGRows;
+// Rows of a lane.  What a tile costs beside its rows is the same for 8 of them: the forward of
+// 8192 x 5120 took 154 us with 8 (bf16) and 126 with 16 (f32 170 and 143).  The backward holds
+// nine values of a row where the forward holds two, and a tile of it enters with kept states.
+constexpr int kGRows = kCarryRows / kGW, kGFwdRows = 2 * kGRows;
+
+// v is formed here: the compiler moves a value to the block of its only use, and what it is
+// formed from stays in registers until then.
+__device__ __forceinline__ void g_keep(float& v) { asm volatile("" : "+v"(v)); }
 
 // s(v) = 1 / (1 + exp(-v)) and s(-v) = 1 - s(v), by the hardware's exp2 and reciprocal (one
 // step each); 0 and 1 at the ends.  s(-v) of a large v is exp(-v) s(v): the difference from 1
@@ -85,9 +91,11 @@ __device__ __forceinline__ Logistic g_logistic(float v) {
 
 // a = exp(v) and q = 1 - a^2 for v <= 0, both to a few steps of their own size.  From -1/8 up by
 // e = exp(v) - 1, the series to v^5 / 5! (its next term is 2^-24 of the sum there): a = 1 + e,
-// 1 - a^2 = -e (2 + e) keep what a difference from 1 would lose as a nears 1.  The exponential,
-// for what lies below, is passed over where no lane needs it.
+// 1 - a^2 = -e (2 + e) keep what a difference from 1 would lose as a nears 1.  FAR: with the
+// exponential for what lies below, which a tile takes only where it has such a value.
 struct Decay { float a, q; };
+__device__ __forceinline__ bool g_near(float v) { return v >= -0.125f; }  // not of a NaN
+template <bool FAR>
 __device__ __forceinline__ Decay g_decay(float v) {
     float e = 1.f / 120.f;
     e = __builtin_fmaf(e, v, 1.f / 24.f);
@@ -95,13 +103,36 @@ __device__ __forceinline__ Decay g_decay(float v) {
     e = __builtin_fmaf(e, v, 0.5f);
     e = __builtin_fmaf(e, v, 1.f) * v;
     Decay d = {1.f + e, -e * (2.f + e)};
-    const bool near = v >= -0.125f;  // not of a NaN
-    if (__ballot(!near)) {
-        const float far = __builtin_amdgcn_exp2f(v * 1.44269504088896341f);
-        d.a = near ? d.a : far;
-        d.q = near ? d.q : __builtin_fmaf(-far, far, 1.f);
+    if constexpr (FAR) {
+        float far = __builtin_amdgcn_exp2f(v * 1.44269504088896341f);
+        g_keep(far);  // for every lane: a branch of its own would cost more
+        const float q = __builtin_fmaf(-far, far, 1.f);
+        d.a = g_near(v) ? d.a : far;
+        d.q = g_near(v) ? d.q : q;
     }
     return d;
+}
+// The decays of R rows: a holds A s(r).
+template <int R>
+__device__ __forceinline__ void g_decays(float (&a)[R], float (&q)[R]) {
+    bool far = false;
+#pragma unroll
+    for (int j = 0; j < R; ++j) far |= !g_near(a[j]);
+    if (__ballot(far)) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const Decay d = g_decay<true>(a[j]);
+            a[j] = d.a;
+            q[j] = d.q;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const Decay d = g_decay<false>(a[j]);
+            a[j] = d.a;
+            q[j] = d.q;
+        }
+    }
 }
 
 // What the R rows from t0 are (R <= 64, t0 uniform over the wave): bit j of a mask for row
@@ -164,12 +195,12 @@ __global__ __launch_bounds__(256) void gated_clear(uint32_t* ticket, uint4* word
     for (int64_t k = i; k < n; k += (int64_t)gridDim.x * 256) words[k] = make_uint4(~0u, ~0u, ~0u, ~0u);
 }
 
-struct GMap { float P[kGV], H[kGV]; };
+struct GMap { float P = 1.f, H = 0.f; };
 struct GShared {
-    float P[kGW][kGV][64], H[kGW][kGV][64];    // the waves' maps
-    float P2[kGW][kGV][64], H2[kGW][kGV][64];  // joined runs of tiles; the backward's sums
-    float in[kGV][64];                         // the group's entry
-    int cut[kGW];                              // whether a wave's rows cut the state that enters them off
+    float P[kGW][64], H[kGW][64];    // the waves' maps
+    float P2[kGW][64], H2[kGW][64];  // joined runs of tiles; the backward's maps of h
+    float in[64];                    // the group's entry
+    int cut[kGW];                    // whether a wave's rows cut the state that enters them off
     int tile, far;
 };
 
@@ -186,459 +217,373 @@ __device__ __forceinline__ void g_tile(const GatedP& p, GShared& s, int& o, int&
         ct = blockIdx.x;
     }
 }
+__device__ __forceinline__ int64_t g_at(const GatedP& p, int o, int ct, int l) { return ((int64_t)o * p.nct + ct) * kGC + l; }
+
+// The waves' maps, joined onto h: the waves from .. to - 1 in the order of time, or against it.
+template <bool BACK>
+__device__ __forceinline__ void g_fold(const float (&P)[kGW][64], const float (&H)[kGW][64], const int (&cut)[kGW], int n, int l, float& h) {
+    for (int i = 0; i < n; ++i) {
+        const int k = BACK ? kGW - 1 - i : i;
+        h = cut[k] ? H[k][l] : __builtin_fmaf(P[k][l], h, H[k][l]);
+    }
+}
+// The tile's map, published by one wave; cut: whether its rows cut off what enters.
+template <bool BACK>
+__device__ __forceinline__ GMap g_publish_map(const GatedP& p, const GShared& s, int o, int ct, int l, bool& cut) {
+    GMap m;
+    g_fold<BACK>(s.P, s.H, s.cut, kGW, l, m.H);
+    cut = false;
+#pragma unroll
+    for (int k = 0; k < kGW; ++k) {
+        m.P *= s.P[k][l];
+        cut |= s.cut[k] != 0;
+    }
+    g_publish(p.map + g_at(p, o, ct, l), g_word(m.P, m.H));
+    return m;
+}
+__device__ __forceinline__ void g_publish_end(const GatedP& p, int o, int ct, int l, const GMap& m, bool cut, float h) {
+    if ((o + 1) % kGGroup == 0 && o + 1 < p.ntile)
+        g_publish(p.ends + g_at(p, o / kGGroup, ct, l), g_word(0.f, cut ? m.H : __builtin_fmaf(m.P, h, m.H)));
+}
 
 // The state that enters tile o: joined from the maps of tiles far .. o - 1, tile `far` being cut, or
 // from the end of the group before o's.  Called by the whole workgroup (o > far >= 0).
-__device__ __forceinline__ void g_enter(const GatedP& p, GShared& s, int o, int ct, int far, float (&h)[kGV]) {
+__device__ __forceinline__ float g_enter(const GatedP& p, GShared& s, int o, int ct, int far) {
     const int w = wave_id(), l = threadIdx.x & 63;
-    const int64_t Dp = (int64_t)p.nct * kGC, at = (int64_t)ct * kGC + l;
     const int base = o / kGGroup * kGGroup, from = max(far, base);
     const bool group = far < base;
     const int per = (o - from + kGW - 1) / kGW, k0 = min(o, from + w * per), k1 = min(o, k0 + per);
     GMap m;
+    uint64_t word[kGGroup / kGW], end = 0;
 #pragma unroll
-    for (int v = 0; v < kGV; ++v) m.P[v] = 1.f, m.H[v] = 0.f;
-    uint64_t word[kGGroup / kGW][kGV], end[kGV];
-#pragma unroll
-    for (int i = 0; i < kGGroup / kGW; ++i)
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) word[i][v] = k0 + i < k1 ? g_peek(p.map + (int64_t)(k0 + i) * Dp + at + 64 * v) : 0;
-    const uint64_t* ends = p.ends + (int64_t)(base / kGGroup - 1) * Dp + at;
-    if (group && w == 0) {
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) end[v] = g_peek(ends + 64 * v);
-    }
+    for (int i = 0; i < kGGroup / kGW; ++i) word[i] = k0 + i < k1 ? g_peek(p.map + g_at(p, k0 + i, ct, l)) : 0;
+    const uint64_t* ends = p.ends + g_at(p, base / kGGroup - 1, ct, l);
+    if (group && w == 0) end = g_peek(ends);
 #pragma unroll
     for (int i = 0; i < kGGroup / kGW; ++i) {
         if (k0 + i >= k1) break;
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) {
-            const uint64_t x = g_wait(p.map + (int64_t)(k0 + i) * Dp + at + 64 * v, word[i][v]);
-            const float P = __uint_as_float((uint32_t)x), H = __uint_as_float((uint32_t)(x >> 32));
-            m.H[v] = i ? __builtin_fmaf(P, m.H[v], H) : H;
-            m.P[v] = i ? P * m.P[v] : P;
-        }
+        const uint64_t x = g_wait(p.map + g_at(p, k0 + i, ct, l), word[i]);
+        const float P = __uint_as_float((uint32_t)x), H = __uint_as_float((uint32_t)(x >> 32));
+        m.H = i ? __builtin_fmaf(P, m.H, H) : H;
+        m.P = i ? P * m.P : P;
     }
-    if (group && w == 0) {
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) s.in[v][l] = __uint_as_float((uint32_t)(g_wait(ends + 64 * v, end[v]) >> 32));
-    }
-#pragma unroll
-    for (int v = 0; v < kGV; ++v) s.P2[w][v][l] = m.P[v], s.H2[w][v][l] = m.H[v];
+    if (group && w == 0) s.in[l] = __uint_as_float((uint32_t)(g_wait(ends, end) >> 32));
+    s.P2[w][l] = m.P;
+    s.H2[w][l] = m.H;
     __syncthreads();
-#pragma unroll
-    for (int v = 0; v < kGV; ++v) {
-        h[v] = group ? __builtin_fmaf(s.P2[0][v][l], s.in[v][l], s.H2[0][v][l]) : s.H2[0][v][l];  // a cut tile's P is no factor
-        for (int k = 1; k < kGW && from + k * per < o; ++k) h[v] = __builtin_fmaf(s.P2[k][v][l], h[v], s.H2[k][v][l]);
-    }
+    float h = group ? __builtin_fmaf(s.P2[0][l], s.in[l], s.H2[0][l]) : s.H2[0][l];  // a cut tile's P is no factor
+    for (int k = 1; k < kGW && from + k * per < o; ++k) h = __builtin_fmaf(s.P2[k][l], h, s.H2[k][l]);
+    return h;
 }
 
-// Two channels of a row from column c: loaded whole by every lane, those past the row's end from
-// its last two channels, so that no load has a branch of its own.  MODE 0: an even number of
-// channels; 1: an odd one, whose last lane takes the second of the two; 2: a single channel.
-template <int MODE>
-__device__ __forceinline__ int g_column(int c, int D) { return MODE == 2 ? c : min(c, D - kGV); }
-// (row: uniform; an unsigned offset keeps the address a scalar base and one register)
-template <typename T, int MODE>
-__device__ __forceinline__ void g_load(Elems<T, kGV>& e, const T* row, int cl, int n) {
-    const T* at = reinterpret_cast<const T*>(reinterpret_cast<const char*>(row) + (uint32_t)cl * (uint32_t)sizeof(T));
-    if constexpr (MODE == 2) e.load_part(at, n);
-    else e.load(at);
-}
+// A wave's rows of one tensor from row t0 on, a channel a lane, through a buffer resource: a scalar
+// offset a row (16 rows' offsets and a column fit 31 bits) and one of the lane, which lies behind the resource's
+// end for a lane without a channel.  Such a lane reads 0 and writes nothing, without a branch.
 template <typename T>
-__device__ __forceinline__ void g_store(T* row, int c, int n, const float (&v)[kGV]) {
-    st_run<kGV, T>(reinterpret_cast<T*>(reinterpret_cast<char*>(row) + (uint32_t)c * (uint32_t)sizeof(T)), n, v);
+struct GRow {
+    __amdgpu_buffer_rsrc_t r;
+    uint32_t st;
+    __device__ __forceinline__ GRow(const void* p, int64_t t0, int64_t stride)
+        : r(buf_rsrc(static_cast<const T*>(p) + t0 * stride, 0x7fffffffu)), st((uint32_t)stride * (uint32_t)sizeof(T)) {}
+    static __device__ __forceinline__ uint32_t column(int c, int D) { return c < D ? (uint32_t)c * (uint32_t)sizeof(T) : 0x80000000u; }
+    __device__ __forceinline__ uint32_t load(int j, uint32_t col) const {
+        if constexpr (sizeof(T) == 2) return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, col, j * st, 0);
+        else return __builtin_amdgcn_raw_buffer_load_b32(r, col, j * st, 0);
+    }
+    __device__ __forceinline__ void store(int j, uint32_t col, float v) const {
+        if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16((short)pack_bf16x2(v, v), r, col, j * st, 0);
+        else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, col, j * st, 0);
+    }
+};
+template <typename T>
+__device__ __forceinline__ float g_value(uint32_t w) { return __uint_as_float(sizeof(T) == 2 ? w << 16 : w); }
+// rows past the last one are read as the last
+template <typename T, int R>
+__device__ __forceinline__ void g_fetch(uint32_t (&e)[R], const GatedP& p, const void* q, int64_t st, int t0, uint32_t col) {
+    const int t = min(t0, (int)p.rows - 1), k = (int)p.rows - 1 - t;
+    const GRow<T> row(q, t, st);
+#pragma unroll
+    for (int j = 0; j < R; ++j) e[j] = row.load(min(j, k), col);
 }
 
-template <typename T, int MODE>
+template <typename T, bool Z>
 __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
-    constexpr int R = kGFwdRows<T>;
+    constexpr int R = kGFwdRows;
     __shared__ GShared s;
     int o, ct;
     g_tile(p, s, o, ct);
     const int w = wave_id(), l = threadIdx.x & 63;
-    const int row0 = o * (kGW * R), t0 = row0 + w * R, c = ct * kGC + l * kGV, n = p.D - c;
+    const int t0 = (o * kGW + w) * R, c = ct * kGC + l;
     const int rows = min(R, max(0, (int)p.rows - t0));  // of this wave
-    Elems<T, kGV> ex[R], er[R], ei[R], ez[R];
-    const int cl = g_column<MODE>(c, p.D);
-    auto fetch = [&](Elems<T, kGV> (&e)[R], const void* q, int64_t st) __attribute__((always_inline)) {
+    const uint32_t col = GRow<T>::column(c, p.D);
+    uint32_t ez[Z ? R : 1];
+    float a[R], b[R];
+    GRows g;
+    {
+        uint32_t ex[R], er[R], ei[R];
+        g_fetch<T, R>(er, p, p.r, p.r_st, t0, col);
+        g_fetch<T, R>(ei, p, p.i, p.i_st, t0, col);
+        g_fetch<T, R>(ex, p, p.x, p.x_st, t0, col);
+        g = g_rows(p.q, t0, R);
+        const float A = c < p.D ? p.A[c] : 0.f;
 #pragma unroll
-        for (int j = 0; j < R; ++j) g_load<T, MODE>(e[j], static_cast<const T*>(q) + (int64_t)min(t0 + j, (int)p.rows - 1) * st, cl, n);
-    };
-    auto get = [&](const Elems<T, kGV>& e, float (&v)[kGV]) __attribute__((always_inline)) {
-        e.get(v);
-        if (MODE == 1 && n == 1) v[0] = v[1];
-    };
-    fetch(er, p.r, p.r_st);
-    fetch(ei, p.i, p.i_st);
-    fetch(ex, p.x, p.x_st);
-    const GRows g = g_rows(p.q, t0, R);
-    float A[kGV];
+        for (int j = 0; j < R; ++j) {
+            a[j] = A * g_sigmoid(g_value<T>(er[j]));
+            g_keep(a[j]);
+        }
+        g_decays<R>(a, b);
 #pragma unroll
-    for (int v = 0; v < kGV; ++v) A[v] = v < n ? p.A[c + v] : 0.f;
-    constexpr uint64_t full = (1ull << R) - 1;
-    const bool plain = g.live == full && (g.first | g.last) == 0;
-    float a[R][kGV], b[R][kGV];
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        float r[kGV], i[kGV], x[kGV];
-        get(er[j], r);
-        get(ei[j], i);
-        get(ex[j], x);
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) {
-            const Decay d = g_decay(A[v] * g_sigmoid(r[v]));
-            a[j][v] = d.a;
-            b[j][v] = __builtin_amdgcn_sqrtf(d.q) * (g_sigmoid(i[v]) * x[v]);
+        for (int j = 0; j < R; ++j) {
+            b[j] = __builtin_amdgcn_sqrtf(b[j]) * (g_sigmoid(g_value<T>(ei[j])) * g_value<T>(ex[j]));
+            g_keep(b[j]);
         }
     }
+    constexpr uint64_t full = (1ull << R) - 1;
+    const bool plain = g.live == full && (g.first | g.last) == 0;
     GMap m;
-#pragma unroll
-    for (int v = 0; v < kGV; ++v) m.P[v] = 1.f, m.H[v] = 0.f;
     if (plain) {
 #pragma unroll
-        for (int j = 0; j < R; ++j)
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) {
-                m.H[v] = __builtin_fmaf(a[j][v], m.H[v], b[j][v]);
-                m.P[v] *= a[j][v];
-            }
+        for (int j = 0; j < R; ++j) {
+            m.H = __builtin_fmaf(a[j], m.H, b[j]);
+            m.P *= a[j];
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             if (g_bit(g.first, j)) {  // from the sequence's state on; b holds the new one
                 const int64_t slot = p.state ? slot_of(p.slots, g_lane(g.s, j), p.nslots) : -1;
-#pragma unroll
-                for (int v = 0; v < kGV; ++v) {
-                    const float h0 = slot >= 0 && v < n ? p.state[slot * p.D + c + v] : 0.f;
-                    m.H[v] = b[j][v] = __builtin_fmaf(a[j][v], h0, b[j][v]);
-                }
+                const float h0 = slot >= 0 && c < p.D ? p.state[slot * p.D + c] : 0.f;
+                m.H = b[j] = __builtin_fmaf(a[j], h0, b[j]);
             } else if (g_bit(g.live, j)) {
-#pragma unroll
-                for (int v = 0; v < kGV; ++v) {
-                    m.H[v] = __builtin_fmaf(a[j][v], m.H[v], b[j][v]);
-                    m.P[v] *= a[j][v];
-                }
+                m.H = __builtin_fmaf(a[j], m.H, b[j]);
+                m.P *= a[j];
             } else {
-#pragma unroll
-                for (int v = 0; v < kGV; ++v) m.H[v] = 0.f;
+                m.H = 0.f;
             }
         }
     }
-#pragma unroll
-    for (int v = 0; v < kGV; ++v) s.P[w][v][l] = m.P[v], s.H[w][v][l] = m.H[v];
+    s.P[w][l] = m.P;
+    s.H[w][l] = m.H;
     if (l == 0) s.cut[w] = g.live != full || g.first != 0;
-    if (w == 0 && l == 0) s.far = (g.live & ~g.first & 1) ? g.b / (kGW * R) : -1;
-    if (p.z) fetch(ez, p.z, p.z_st);
+    if (threadIdx.x == 0) s.far = (g.live & ~g.first & 1) ? g.b / (kGW * R) : -1;
+    if constexpr (Z) g_fetch<T, R>(ez, p, p.z, p.z_st, t0, col);
     __syncthreads();
-    float h[kGV] = {0.f, 0.f};
-    const int64_t at = ((int64_t)o * p.nct + ct) * kGC + l;
-    const bool ends = (o + 1) % kGGroup == 0 && o + 1 < p.ntile;
+    float h = 0.f;
     GMap whole;
     bool cut = false;
-    if (w == kGW - 1 && p.ntile > 1) {
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) whole.P[v] = 1.f, whole.H[v] = 0.f;
-        for (int k = 0; k < kGW; ++k) {
-            const bool here = s.cut[k] != 0;
-            cut |= here;
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) {
-                whole.H[v] = here ? s.H[k][v][l] : __builtin_fmaf(s.P[k][v][l], whole.H[v], s.H[k][v][l]);
-                whole.P[v] *= s.P[k][v][l];
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) g_publish(p.map + at + 64 * v, g_word(whole.P[v], whole.H[v]));
-    }
+    if (w == kGW - 1 && p.ntile > 1) whole = g_publish_map<false>(p, s, o, ct, l, cut);
     const int far = __builtin_amdgcn_readfirstlane(s.far);
-    if (far >= 0) g_enter(p, s, o, ct, far, h);
-    if (w == kGW - 1 && ends) {
-#pragma unroll
-        for (int v = 0; v < kGV; ++v)
-            g_publish(p.ends + ((int64_t)(o / kGGroup) * p.nct + ct) * kGC + l + 64 * v, g_word(0.f, cut ? whole.H[v] : __builtin_fmaf(whole.P[v], h[v], whole.H[v])));
-    }
-    for (int k = 0; k < w; ++k) {
-        const bool here = s.cut[k] != 0;
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) h[v] = here ? s.H[k][v][l] : __builtin_fmaf(s.P[k][v][l], h[v], s.H[k][v][l]);
-    }
-    if (p.carry && t0 % kCarryRows == 0 && rows > 0) st_run<kGV, float>(p.carry + (int64_t)(t0 / kCarryRows) * p.D + c, n, h);
+    if (far >= 0) h = g_enter(p, s, o, ct, far);
+    if (w == kGW - 1) g_publish_end(p, o, ct, l, whole, cut, h);
+    g_fold<false>(s.P, s.H, s.cut, w, l, h);
+    if (p.carry && t0 % kCarryRows == 0 && rows > 0 && c < p.D) p.carry[(int64_t)(t0 / kCarryRows) * p.D + c] = h;
+    const GRow<T> y(p.y, t0, p.y_st);
     auto put = [&](int j) __attribute__((always_inline)) {
-        float y[kGV];
-        if (p.z) {
-            float z[kGV];
-            get(ez[j], z);
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) y[v] = h[v] * z[v] * g_sigmoid(z[v]);
-        } else {
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) y[v] = h[v];
+        float v = h;
+        if constexpr (Z) {
+            const float z = g_value<T>(ez[j]);
+            v = h * z * g_sigmoid(z);
         }
-        g_store<T>(static_cast<T*>(p.y) + (t0 + j) * p.y_st, c, n, y);
+        y.store(j, col, v);
     };
     if (plain) {
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) h[v] = __builtin_fmaf(a[j][v], h[v], b[j][v]);
+            h = __builtin_fmaf(a[j], h, b[j]);
             put(j);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             if (!g_bit(g.live, j)) {
-#pragma unroll
-                for (int v = 0; v < kGV; ++v) h[v] = 0.f;
-                if (p.fill && j < rows) g_store<T>(static_cast<T*>(p.y) + (t0 + j) * p.y_st, c, n, h);
+                h = 0.f;
+                if (p.fill && j < rows) y.store(j, col, 0.f);
                 continue;
             }
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) h[v] = g_bit(g.first, j) ? b[j][v] : __builtin_fmaf(a[j][v], h[v], b[j][v]);
+            h = g_bit(g.first, j) ? b[j] : __builtin_fmaf(a[j], h, b[j]);
             put(j);
             if (g_bit(g.last, j) && p.state) {
                 const int64_t slot = slot_of(p.slots, g_lane(g.s, j), p.nslots);
-                if (slot >= 0) st_run<kGV, float>(p.state + slot * p.D + c, n, h);
+                if (slot >= 0 && c < p.D) p.state[slot * p.D + c] = h;
             }
         }
     }
 }
 
-template <typename T, int MODE>
-__global__ __launch_bounds__(64 * kGW, 2) void gated_bwd(GatedP p) {
+// What a row's gradients need is formed once, where its values are read: with u = s(i) x,
+//   gr = dy silu(z), zk = dy silu'(z), pull = u a^2 / m, kr = A s(r) s(-r), ui = u s(-i)
+// so that dz = h zk, dx = dh m s(i), di = dh m ui, dr = e kr, e = dh (a h_{t-1} - pull).
+template <typename T, bool Z>
+__global__ __launch_bounds__(64 * kGW, 4) void gated_bwd(GatedP p) {
     constexpr int R = kGRows;
     __shared__ GShared s;
     int o, ct;
     g_tile(p, s, o, ct);
     const int tile = p.ntile - 1 - o;  // from the last one on
     const int w = wave_id(), l = threadIdx.x & 63;
-    const int row0 = tile * kCarryRows, t0 = row0 + w * R, c = ct * kGC + l * kGV, n = p.D - c;
+    const int row0 = tile * kCarryRows, t0 = row0 + w * R, c = ct * kGC + l;
     const int rows = min(R, max(0, (int)p.rows - t0));
-    Elems<T, kGV> ex[R], er[R], ei[R], ez[R], ey[R];
-    const int cl = g_column<MODE>(c, p.D);
-    auto fetch = [&](Elems<T, kGV> (&e)[R], const void* q, int64_t st) __attribute__((always_inline)) {
+    const uint32_t col = GRow<T>::column(c, p.D);
+    // sm = m s(i), um = m ui
+    float a[R], b[R], pull[R], sr[R], kr[R], sm[R], um[R], gr[R], zk[Z ? R : 1];
+    float h = 0.f;
+    GRows g;
+    {
+        uint32_t ex[R], er[R], ei[R], ez[R], ey[R];
+        g_fetch<T, R>(er, p, p.r, p.r_st, t0, col);
+        g_fetch<T, R>(ei, p, p.i, p.i_st, t0, col);
+        g_fetch<T, R>(ex, p, p.x, p.x_st, t0, col);
+        g_fetch<T, R>(ey, p, p.dy, p.dy_st, t0, col);
+        if constexpr (Z) g_fetch<T, R>(ez, p, p.z, p.z_st, t0, col);
+        g = g_rows(p.q, t0, R);
+        const float A = c < p.D ? p.A[c] : 0.f;
+        if (c < p.D) h = p.carry[(int64_t)tile * p.D + c];
+        float q[R];
 #pragma unroll
-        for (int j = 0; j < R; ++j) g_load<T, MODE>(e[j], static_cast<const T*>(q) + (int64_t)min(t0 + j, (int)p.rows - 1) * st, cl, n);
-    };
-    auto get = [&](const Elems<T, kGV>& e, float (&v)[kGV]) __attribute__((always_inline)) {
-        e.get(v);
-        if (MODE == 1 && n == 1) v[0] = v[1];
-    };
-    fetch(er, p.r, p.r_st);
-    fetch(ei, p.i, p.i_st);
-    fetch(ex, p.x, p.x_st);
-    fetch(ey, p.dy, p.dy_st);
-    if (p.z) fetch(ez, p.z, p.z_st);
-    const GRows g = g_rows(p.q, t0, R);
-    float A[kGV], hin[kGV] = {0.f, 0.f};
-    ld_run<kGV, float>(p.A + c, n, A);
-    ld_run<kGV, float>(p.carry + (int64_t)tile * p.D + c, n, hin);
+        for (int j = 0; j < R; ++j) {
+            const Logistic r = g_logistic(g_value<T>(er[j]));
+            sr[j] = r.s;
+            a[j] = A * r.s;
+            kr[j] = a[j] * r.c;
+            g_keep(kr[j]);
+        }
+        g_decays<R>(a, q);
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const float im = q[j] > 0.f ? __builtin_amdgcn_rsqf(q[j]) : q[j] * 0.f;  // 0 where a is 1, a NaN of a NaN
+            const float m = q[j] * im;
+            const Logistic i = g_logistic(g_value<T>(ei[j]));
+            const float u = i.s * g_value<T>(ex[j]);
+            sm[j] = m * i.s;
+            um[j] = m * (u * i.c);
+            b[j] = m * u;
+            pull[j] = u * a[j] * (a[j] * im);
+            g_keep(sm[j]);
+            g_keep(um[j]);
+            g_keep(pull[j]);
+            const float dy = g_value<T>(ey[j]);
+            gr[j] = dy;
+            if constexpr (Z) {
+                const float z = g_value<T>(ez[j]);
+                const Logistic k = g_logistic(z);
+                gr[j] = dy * k.s * z;
+                zk[j] = dy * k.s * __builtin_fmaf(z, k.c, 1.f);
+                g_keep(gr[j]);
+                g_keep(zk[j]);
+            }
+        }
+    }
     constexpr uint64_t full = (1ull << R) - 1;
     const bool plain = g.live == full && (g.first | g.last) == 0;
-    float a[R][kGV], m[R][kGV], im[R][kGV], b[R][kGV];  // im: 1 / m; b: m u, and then the state before the row
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        float r[kGV], i[kGV], x[kGV];
-        get(er[j], r);
-        get(ei[j], i);
-        get(ex[j], x);
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) {
-            const Decay d = g_decay(A[v] * g_sigmoid(r[v]));
-            a[j][v] = d.a;
-            const float q = d.q;
-            im[j][v] = q > 0.f ? __builtin_amdgcn_rsqf(q) : q * 0.f;  // 0 where a is 1, a NaN of a NaN
-            m[j][v] = q * im[j][v];
-            b[j][v] = m[j][v] * (g_sigmoid(i[v]) * x[v]);
-        }
-    }
-    auto start = [&](int j, float (&h)[kGV]) __attribute__((always_inline)) {  // what the sequence of row j starts from
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) h[v] = 0.f;
-        if (p.h0) ld_run<kGV, float>(p.h0 + (int64_t)g_lane(g.s, j) * p.D + c, n, h);
+    auto start = [&](int j) __attribute__((always_inline)) {  // what the sequence of row j starts from
+        return p.h0 && c < p.D ? p.h0[(int64_t)g_lane(g.s, j) * p.D + c] : 0.f;
     };
-    // the waves' maps of h
+    // the waves' maps of h and of q
     GMap f, q;
+    if (plain) {
 #pragma unroll
-    for (int v = 0; v < kGV; ++v) f.P[v] = 1.f, f.H[v] = 0.f, q.P[v] = 1.f, q.H[v] = 0.f;
+        for (int j = 0; j < R; ++j) {
+            f.H = __builtin_fmaf(a[j], f.H, b[j]);
+            f.P *= a[j];
+            q.H = a[R - 1 - j] * (gr[R - 1 - j] + q.H);
+        }
+    } else {
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-        if (!plain && !g_bit(g.live, j)) {
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) f.H[v] = 0.f;
-        } else {
-            if (!plain && g_bit(g.first, j)) start(j, f.H);
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) {
-                f.H[v] = __builtin_fmaf(a[j][v], f.H[v], b[j][v]);
-                f.P[v] *= a[j][v];
+        for (int j = 0; j < R; ++j) {
+            if (!g_bit(g.live, j)) {
+                f.H = 0.f;
+                continue;
             }
+            if (g_bit(g.first, j)) f.H = start(j);
+            f.H = __builtin_fmaf(a[j], f.H, b[j]);
+            f.P *= a[j];
+            if (g_bit(g.last, j) && p.dhT && c < p.D) gr[j] += p.dhT[(int64_t)g_lane(g.s, j) * p.D + c];
         }
+#pragma unroll
+        for (int j = R - 1; j >= 0; --j) q.H = g_bit(g.live & ~g.first, j) ? a[j] * (gr[j] + q.H) : 0.f;
     }
-    // g of row j
-    auto grad = [&](int j, const Logistic (&sz)[kGV], const float (&z)[kGV], const float (&dy)[kGV], float (&o_)[kGV]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) o_[v] = p.z ? dy[v] * z[v] * sz[v].s : dy[v];
-        if (!plain && g_bit(g.last, j) && p.dhT) {
-            float d[kGV];
-            ld_run<kGV, float>(p.dhT + (int64_t)g_lane(g.s, j) * p.D + c, n, d);
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) o_[v] += d[v];
-        }
-    };
-    auto gate = [&](int j, Logistic (&sz)[kGV], float (&z)[kGV]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) z[v] = 0.f, sz[v] = Logistic{0.f, 0.f};
-        if (p.z) {
-            get(ez[j], z);
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) sz[v] = g_logistic(z[v]);
-        }
-    };
-    // and of q
-#pragma unroll
-    for (int j = R - 1; j >= 0; --j) {
-        if (!plain && !g_bit(g.live, j)) {
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) q.H[v] = 0.f;
-            continue;
-        }
-        Logistic sz[kGV];
-        float z[kGV], dy[kGV], gr[kGV];
-        gate(j, sz, z);
-        get(ey[j], dy);
-        grad(j, sz, z, dy, gr);
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) {
-            q.H[v] = a[j][v] * (gr[v] + q.H[v]);
-            q.P[v] *= a[j][v];
-            if (!plain && g_bit(g.first, j)) q.H[v] = 0.f;
-        }
-    }
-#pragma unroll
-    for (int v = 0; v < kGV; ++v) {
-        s.P[w][v][l] = q.P[v], s.H[w][v][l] = q.H[v];
-        s.P2[w][v][l] = f.P[v], s.H2[w][v][l] = f.H[v];
-    }
-    const bool cut_here = g.live != full || g.first != 0;
-    if (l == 0) s.cut[w] = cut_here;
-    // the tile's last row: its sequence's last tile, where that is another
-    if (w == 0 && l == 0) s.far = -1;
+    s.P[w][l] = f.P;  // one product for both
+    s.H[w][l] = q.H;
+    s.H2[w][l] = f.H;
+    if (l == 0) s.cut[w] = g.live != full || g.first != 0;
+    if (threadIdx.x == 0) s.far = -1;
     __syncthreads();
-    const int lastrow = min((int)p.rows, row0 + kCarryRows) - 1 - t0;  // of the tile, counted from this wave's first
+    // the tile's last row: its sequence's last tile, where that is another
+    const int lastrow = min((int)p.rows, row0 + kCarryRows) - 1 - t0;  // counted from this wave's first
     if (lastrow >= 0 && lastrow < R && g_bit(g.live & ~g.last, lastrow) && l == 0)
         s.far = p.ntile - 1 - (g_lane(g.e, lastrow) - 1) / kCarryRows;
-    // the state that enters this wave's rows
-    float h[kGV] = {hin[0], hin[1]};
-    for (int k = 0; k < w; ++k) {
-        const bool here = s.cut[k] != 0;
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) h[v] = here ? s.H2[k][v][l] : __builtin_fmaf(s.P2[k][v][l], h[v], s.H2[k][v][l]);
-    }
-    const int64_t at = ((int64_t)o * p.nct + ct) * kGC + l;
-    const bool ends = (o + 1) % kGGroup == 0 && o + 1 < p.ntile;
     GMap whole;
     bool cut = false;
-    if (w == 0 && p.ntile > 1) {
+    if (w == 0 && p.ntile > 1) whole = g_publish_map<true>(p, s, o, ct, l, cut);
+    g_fold<false>(s.P, s.H2, s.cut, w, l, h);  // the state that enters this wave's rows
+    const GRow<T> dz(p.dz, t0, p.dz_st);
+    // b: a h_{t-1} - pull
+    if (plain) {
 #pragma unroll
-        for (int v = 0; v < kGV; ++v) whole.P[v] = 1.f, whole.H[v] = 0.f;
-        for (int k = kGW - 1; k >= 0; --k) {
-            const bool here = s.cut[k] != 0;
-            cut |= here;
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) {
-                whole.H[v] = here ? s.H[k][v][l] : __builtin_fmaf(s.P[k][v][l], whole.H[v], s.H[k][v][l]);
-                whole.P[v] *= s.P[k][v][l];
-            }
+        for (int j = 0; j < R; ++j) {
+            const float ah = a[j] * h;
+            h = ah + b[j];
+            b[j] = ah - pull[j];
+            if constexpr (Z) dz.store(j, col, h * zk[j]);
         }
+    } else {
 #pragma unroll
-        for (int v = 0; v < kGV; ++v) g_publish(p.map + at + 64 * v, g_word(whole.P[v], whole.H[v]));
-    }
-#pragma unroll
-    for (int j = 0; j < R; ++j) {  // b: the state before the row
-        if (!plain && !g_bit(g.live, j)) {
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) h[v] = 0.f;
-        } else {
-            if (!plain && g_bit(g.first, j)) start(j, h);
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) {
-                const float after = __builtin_fmaf(a[j][v], h[v], b[j][v]);
-                b[j][v] = h[v];
-                h[v] = after;
+        for (int j = 0; j < R; ++j) {
+            const bool live = g_bit(g.live, j);
+            if (g_bit(g.first, j)) h = start(j);
+            const float ah = a[j] * h;
+            h = live ? ah + b[j] : 0.f;
+            b[j] = ah - pull[j];
+            if constexpr (Z) {
+                if (j < rows) dz.store(j, col, live ? h * zk[j] : 0.f);
             }
         }
     }
     __syncthreads();  // the waves' maps of h have been read, and far is known
-    float qin[kGV] = {0.f, 0.f};
+    float qin = 0.f;
     const int far = __builtin_amdgcn_readfirstlane(s.far);
-    if (far >= 0) g_enter(p, s, o, ct, far, qin);
-    if (w == 0 && ends) {
-#pragma unroll
-        for (int v = 0; v < kGV; ++v)
-            g_publish(p.ends + ((int64_t)(o / kGGroup) * p.nct + ct) * kGC + l + 64 * v, g_word(0.f, cut ? whole.H[v] : __builtin_fmaf(whole.P[v], qin[v], whole.H[v])));
-    }
-    for (int k = kGW - 1; k > w; --k) {
-        const bool here = s.cut[k] != 0;
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) qin[v] = here ? s.H[k][v][l] : __builtin_fmaf(s.P[k][v][l], qin[v], s.H[k][v][l]);
-    }
-    float dA[kGV] = {0.f, 0.f};
-    auto put = [&](void* to, int64_t st, int j, const float (&v)[kGV]) __attribute__((always_inline)) {
-        g_store<T>(static_cast<T*>(to) + (t0 + j) * st, c, n, v);
+    if (far >= 0) qin = g_enter(p, s, o, ct, far);
+    if (w == 0) g_publish_end(p, o, ct, l, whole, cut, qin);
+    g_fold<true>(s.P, s.H, s.cut, kGW - 1 - w, l, qin);
+    float dA = 0.f;
+    const GRow<T> dx(p.dx, t0, p.dx_st), dr(p.dr, t0, p.dr_st), di(p.di, t0, p.di_st);
+    auto put = [&](int j) __attribute__((always_inline)) {
+        const float dh = gr[j] + qin, e = dh * b[j];
+        dx.store(j, col, dh * sm[j]);
+        di.store(j, col, dh * um[j]);
+        dr.store(j, col, e * kr[j]);
+        dA = __builtin_fmaf(e, sr[j], dA);
+        qin = a[j] * dh;
     };
+    if (plain) {
 #pragma unroll
-    for (int j = R - 1; j >= 0; --j) {
-        if (j >= rows) continue;
-        if (!plain && !g_bit(g.live, j)) {
-            const float zero[kGV] = {0.f, 0.f};
-            put(p.dx, p.dx_st, j, zero);
-            put(p.dr, p.dr_st, j, zero);
-            put(p.di, p.di_st, j, zero);
-            if (p.z) put(p.dz, p.dz_st, j, zero);
+        for (int j = R - 1; j >= 0; --j) put(j);
+    } else {
 #pragma unroll
-            for (int v = 0; v < kGV; ++v) qin[v] = 0.f;
-            continue;
-        }
-        Logistic sz[kGV];
-        float z[kGV], dy[kGV], gr[kGV], r[kGV], i[kGV], x[kGV], dx[kGV], dr[kGV], di[kGV], dz[kGV];
-        gate(j, sz, z);
-        get(ey[j], dy);
-        grad(j, sz, z, dy, gr);
-        get(er[j], r);
-        get(ei[j], i);
-        get(ex[j], x);
-#pragma unroll
-        for (int v = 0; v < kGV; ++v) {
-            const Logistic sr = g_logistic(r[v]), si = g_logistic(i[v]);
-            const float aj = a[j][v], mj = m[j][v], u = si.s * x[v], dh = gr[v] + qin[v], ah = aj * b[j][v], dm = dh * mj;
-            const float pull = u * aj * aj * im[j][v];
-            const float e = dh * (ah - pull);
-            dx[v] = dm * si.s;
-            di[v] = dm * u * si.c;
-            dr[v] = e * A[v] * sr.s * sr.c;
-            dA[v] = __builtin_fmaf(e, sr.s, dA[v]);
-            dz[v] = dy[v] * __builtin_fmaf(mj, u, ah) * sz[v].s * __builtin_fmaf(z[v], sz[v].c, 1.f);
-            qin[v] = aj * dh;
-        }
-        put(p.dx, p.dx_st, j, dx);
-        put(p.dr, p.dr_st, j, dr);
-        put(p.di, p.di_st, j, di);
-        if (p.z) put(p.dz, p.dz_st, j, dz);
-        if (!plain && g_bit(g.first, j)) {
-            if (p.dh0) st_run<kGV, float>(p.dh0 + (int64_t)g_lane(g.s, j) * p.D + c, n, qin);
-#pragma unroll
-            for (int v = 0; v < kGV; ++v) qin[v] = 0.f;
+        for (int j = R - 1; j >= 0; --j) {
+            if (g_bit(g.live, j)) {
+                put(j);
+                if (g_bit(g.first, j)) {
+                    if (p.dh0 && c < p.D) p.dh0[(int64_t)g_lane(g.s, j) * p.D + c] = qin;
+                    qin = 0.f;
+                }
+            } else {
+                qin = 0.f;
+                if (j < rows) {
+                    dx.store(j, col, 0.f);
+                    di.store(j, col, 0.f);
+                    dr.store(j, col, 0.f);
+                }
+            }
         }
     }
-    __syncthreads();  // P and H have been read
-#pragma unroll
-    for (int v = 0; v < kGV; ++v) s.P[w][v][l] = dA[v];
+    __syncthreads();  // P has been read
+    s.P[w][l] = dA;
     __syncthreads();
-    if (w < kGV) {  // wave v: the channels v of the lanes
+    if (w == 0 && c < p.D) {
         float sum = 0.f;
-        for (int k = 0; k < kGW; ++k) sum += s.P[k][w][l];
-        if (w < n) p.part[(int64_t)tile * p.D + c + w] = sum;
+        for (int k = 0; k < kGW; ++k) sum += s.P[k][l];
+        p.part[(int64_t)tile * p.D + c] = sum;
     }
 }
 
@@ -687,7 +632,7 @@ __global__ __launch_bounds__(256) void gated_step(GatedStepP p) {
         store_f32<T>(y, 0.f);
         return;
     }
-    const Decay g = g_decay(p.A[c] * g_sigmoid(load_f32<T>(static_cast<const T*>(p.r) + b * p.r_sb + c)));
+    const Decay g = g_decay<true>(p.A[c] * g_sigmoid(load_f32<T>(static_cast<const T*>(p.r) + b * p.r_sb + c)));
     float* st = p.state + slot * p.D + c;
     const float u = g_sigmoid(load_f32<T>(static_cast<const T*>(p.i) + b * p.i_sb + c)) * load_f32<T>(static_cast<const T*>(p.x) + b * p.x_sb + c);
     const float h = __builtin_fmaf(g.a, *st, __builtin_amdgcn_sqrtf(g.q) * u);
@@ -698,8 +643,8 @@ __global__ __launch_bounds__(256) void gated_step(GatedStepP p) {
 
 // The tiles of a call, and its workspace at ws (counted from NULL: its size): the ticket, the maps
 // and ends (none for one tile of rows: nothing is waited for), and the backward's sums.
-static size_t gated_plan(GatedP& p, bool back, bool bf16, void* ws) {
-    const int tile = kGW * (back ? kGRows : bf16 ? kGFwdRows<bf16_t> : kGFwdRows<float>);
+static size_t gated_plan(GatedP& p, bool back, void* ws) {
+    const int tile = kGW * (back ? kGRows : kGFwdRows);
     p.ntile = (int)((p.rows + tile - 1) / tile);
     p.nct = ceil_div(p.D, kGC);
     const int64_t Dp = (int64_t)p.nct * kGC, words = p.ntile > 1 ? (p.ntile + p.ntile / kGGroup) * Dp : 0;
@@ -736,6 +681,8 @@ static int gated_make(const mamba_gated_scan_args* a, GatedP* out) {
     MAMBA_CHECK_ARG(a->io_dtype == MAMBA_F32 || a->io_dtype == MAMBA_BF16, "io_dtype must be f32 or bf16");
     MAMBA_CHECK_ARG(a->A != nullptr && a->cu_seqlens != nullptr, "A and cu_seqlens are required");
     MAMBA_CHECK_ARG(a->rows == 0 || (a->x && a->r && a->i), "x, r and i are required");
+    for (const int64_t st : {a->x_st, a->r_st, a->i_st, a->z ? a->z_st : 0})
+        MAMBA_CHECK_ARG(a->rows <= 1 || (st >= 0 && st < kMaxStride), "row strides must be in [0, 2^25)");
     GatedP& p = *out;
     p = GatedP{};
     p.q = Seqs{a->cu_seqlens, a->nseq, (int)a->rows};
@@ -749,18 +696,21 @@ static int gated_make(const mamba_gated_scan_args* a, GatedP* out) {
 
 using namespace mamba;
 
-// kernel<..., MODE>, by the number of channels
-#define GATED_MODE(kernel, grid, block, stream, p, ...)                                                          \
-    do {                                                                                                         \
-        if ((p).D % 2 == 0) hipLaunchKernelGGL((kernel<__VA_ARGS__, 0>), grid, block, 0, (hipStream_t)stream, p); \
-        else if ((p).D > 1) hipLaunchKernelGGL((kernel<__VA_ARGS__, 1>), grid, block, 0, (hipStream_t)stream, p); \
-        else hipLaunchKernelGGL((kernel<__VA_ARGS__, 2>), grid, block, 0, (hipStream_t)stream, p);               \
+#define GATED_LAUNCH(kernel, ...) \
+    hipLaunchKernelGGL((kernel<__VA_ARGS__>), dim3(p.ntile * p.nct), dim3(64 * kGW), 0, (hipStream_t)stream, p)
+// kernel<T, Z>, by the type and the gate
+#define GATED_TILES(kernel, bf16)                             \
+    do {                                                      \
+        if (bf16 && p.z) GATED_LAUNCH(kernel, bf16_t, true);  \
+        else if (bf16) GATED_LAUNCH(kernel, bf16_t, false);   \
+        else if (p.z) GATED_LAUNCH(kernel, float, true);      \
+        else GATED_LAUNCH(kernel, float, false);              \
     } while (0)
 
 extern "C" size_t mamba_gated_scan_workspace_size(const mamba_gated_scan_args* a) {
     GatedP p;
     if (gated_make(a, &p) != MAMBA_OK) return 0;
-    return gated_plan(p, false, a->io_dtype == MAMBA_BF16, nullptr);
+    return gated_plan(p, false, nullptr);
 }
 
 extern "C" int mamba_gated_scan_fwd(const mamba_gated_scan_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {
@@ -769,7 +719,7 @@ extern "C" int mamba_gated_scan_fwd(const mamba_gated_scan_args* a, void* ws, si
     if (st != MAMBA_OK) return st;
     if (p.rows == 0) return MAMBA_OK;
     MAMBA_CHECK_ARG(a->y != nullptr, "y is required");
-    MAMBA_CHECK_ARG(a->y_st >= p.D || p.rows == 1, "rows of y overlap");
+    MAMBA_CHECK_ARG((a->y_st >= p.D && a->y_st < kMaxStride) || p.rows == 1, "rows of y overlap (or lie 2^25 elements apart)");
     MAMBA_CHECK_ARG(a->state == nullptr || a->slots != nullptr || a->nslots >= a->nseq,
                     "without slots the state needs a row per sequence");
     const size_t e = a->io_dtype == MAMBA_BF16 ? 2 : 4;
@@ -779,7 +729,7 @@ extern "C" int mamba_gated_scan_fwd(const mamba_gated_scan_args* a, void* ws, si
                         !rows_clash(a->y, a->y_st, a->z, a->z_st, p.D, p.D, p.rows, e, true),
                     "y overlaps an input (it may be x, r, i or z itself)");
     p.y = a->y; p.y_st = a->y_st; p.state = a->state; p.nslots = a->nslots; p.slots = a->slots;
-    const size_t need = gated_plan(p, false, a->io_dtype == MAMBA_BF16, ws);
+    const size_t need = gated_plan(p, false, ws);
     if ((st = gated_grid_ok(p)) != MAMBA_OK) return st;
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");
     if (need && (ws == nullptr || ws_bytes < need)) {
@@ -787,9 +737,7 @@ extern "C" int mamba_gated_scan_fwd(const mamba_gated_scan_args* a, void* ws, si
         return MAMBA_ERR_WORKSPACE;
     }
     gated_clear_launch(p, (hipStream_t)stream);
-    const dim3 grid(p.ntile * p.nct), block(64 * kGW);
-    if (a->io_dtype == MAMBA_BF16) GATED_MODE(gated_fwd, grid, block, stream, p, bf16_t);
-    else GATED_MODE(gated_fwd, grid, block, stream, p, float);
+    GATED_TILES(gated_fwd, a->io_dtype == MAMBA_BF16);
     MAMBA_CHECK_LAUNCH();
     return MAMBA_OK;
 }
@@ -797,7 +745,7 @@ extern "C" int mamba_gated_scan_fwd(const mamba_gated_scan_args* a, void* ws, si
 extern "C" size_t mamba_gated_scan_bwd_workspace_size(const mamba_gated_scan_bwd_args* a) {
     GatedP p;
     if (a == nullptr || gated_make(&a->fwd, &p) != MAMBA_OK) return 0;
-    return gated_plan(p, true, a->fwd.io_dtype == MAMBA_BF16, nullptr);
+    return gated_plan(p, true, nullptr);
 }
 
 extern "C" int mamba_gated_scan_bwd(const mamba_gated_scan_bwd_args* a, void* ws, size_t ws_bytes, mamba_stream_t stream) {
@@ -810,12 +758,13 @@ extern "C" int mamba_gated_scan_bwd(const mamba_gated_scan_bwd_args* a, void* ws
     MAMBA_CHECK_ARG(a->dA != nullptr, "dA is required");
     MAMBA_CHECK_ARG(p.rows == 0 || (p.carry && a->dy && a->dx && a->dr && a->di), "carry, dy, dx, dr and di are required");
     MAMBA_CHECK_ARG(p.rows == 0 || (p.z != nullptr) == (a->dz != nullptr), "dz goes with z");
+    MAMBA_CHECK_ARG(p.rows <= 1 || (a->dy_st >= 0 && a->dy_st < kMaxStride), "row strides must be in [0, 2^25)");
     struct Rows { const void* p; int64_t st; };
     const Rows ins[] = {{p.x, p.x_st}, {p.r, p.r_st}, {p.i, p.i_st}, {p.z, p.z_st}, {a->dy, a->dy_st}};
     const Rows outs[] = {{a->dx, a->dx_st}, {a->dr, a->dr_st}, {a->di, a->di_st}, {a->dz, a->dz_st}};
     const size_t es = a->fwd.io_dtype == MAMBA_BF16 ? 2 : 4;
     for (const Rows& o : outs) {
-        MAMBA_CHECK_ARG(p.rows <= 1 || o.p == nullptr || o.st >= p.D, "rows of a gradient overlap");
+        MAMBA_CHECK_ARG(p.rows <= 1 || o.p == nullptr || (o.st >= p.D && o.st < kMaxStride), "rows of a gradient overlap (or lie 2^25 elements apart)");
         for (const Rows& i : ins)
             MAMBA_CHECK_ARG(!rows_clash(o.p, o.st, i.p, i.st, p.D, p.D, p.rows, es, false), "a gradient overlaps an input");
         for (const Rows* q = outs; q != &o; ++q)
@@ -824,7 +773,7 @@ extern "C" int mamba_gated_scan_bwd(const mamba_gated_scan_bwd_args* a, void* ws
     p.h0 = a->initial_state; p.dhT = a->d_final_state; p.dh0 = a->d_initial_state; p.dA = a->dA;
     p.dy = a->dy; p.dy_st = a->dy_st; p.dx = a->dx; p.dx_st = a->dx_st; p.dr = a->dr; p.dr_st = a->dr_st;
     p.di = a->di; p.di_st = a->di_st; p.dz = a->dz; p.dz_st = a->dz_st;
-    const size_t need = gated_plan(p, true, a->fwd.io_dtype == MAMBA_BF16, ws);
+    const size_t need = gated_plan(p, true, ws);
     if ((st = gated_grid_ok(p)) != MAMBA_OK) return st;
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");
     if (need && (ws == nullptr || ws_bytes < need)) {
@@ -832,11 +781,7 @@ extern "C" int mamba_gated_scan_bwd(const mamba_gated_scan_bwd_args* a, void* ws
         return MAMBA_ERR_WORKSPACE;
     }
     gated_clear_launch(p, (hipStream_t)stream);
-    if (p.ntile) {
-        const dim3 grid(p.ntile * p.nct), block(64 * kGW);
-        if (a->fwd.io_dtype == MAMBA_BF16) GATED_MODE(gated_bwd, grid, block, stream, p, bf16_t);
-        else GATED_MODE(gated_bwd, grid, block, stream, p, float);
-    }
+    if (p.ntile) GATED_TILES(gated_bwd, a->fwd.io_dtype == MAMBA_BF16);
     hipLaunchKernelGGL(gated_join, dim3(ceil_div(p.D, 16)), dim3(256), 0, (hipStream_t)stream, p.part, p.ntile, p.D, p.dA);
     MAMBA_CHECK_LAUNCH();
     return MAMBA_OK;

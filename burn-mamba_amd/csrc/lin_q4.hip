@@ -317,21 +317,21 @@ __device__ __forceinline__ void q4_store(const Q4P& p, int64_t m0, int n, const 
     }
 }
 
-// The rows in registers: wave w holds the operands of 16 rows for NK blocks of k, and the
-// workgroup's waves all of k.  It takes column tiles in turn; a block's registers are loaded for
+// The rows in registers: wave w holds the operands of RT row tiles of 16 for NK blocks of k, and
+// the workgroup's waves all of k.  It takes column tiles in turn; a block's registers are loaded for
 // the next tile as soon as this one's are used.  The waves' sums meet in LDS, in the order of k, in
 // two places by turns, so that a tile has one barrier.
-template <int X, int NK, int GB, int S>
-__global__ __launch_bounds__(64 * kQ4Waves) void q4_held(Q4P p) {
-    extern __shared__ __align__(16) q4_f32x4 q4_red[];  // [2][waves][64]
+template <int X, int RT, int NK, int GB, int S>
+__global__ __launch_bounds__(64 * (RT > 1 ? 8 : kQ4Waves)) void q4_held(Q4P p) {
+    extern __shared__ __align__(16) q4_f32x4 q4_red[];  // [2][RT][waves][64]
     const int nw = blockDim.x >> 6, w = wave_id(), l = threadIdx.x & 63;
-    const int64_t m0 = (int64_t)blockIdx.y * 16;
+    const int64_t m0 = (int64_t)blockIdx.y * (16 * RT);
     const int kb0 = w * NK;
     // No load has a branch of its own, behind which the compiler would wait for every load in
     // flight; for the same reason the rows are waited for before the tiles' loop, and the blocks are
     // loaded in the order of their use before it as in it.
-    const Q4Src<X, 1> src(p, m0, l);
-    Q4A<X> a[NK][1][4];
+    const Q4Src<X, RT> src(p, m0, l);
+    Q4A<X> a[NK][RT][4];
 #pragma unroll
     for (int k = 0; k < NK; ++k) src.load(a[k], kb0 + k);
     __builtin_amdgcn_sched_barrier(0);
@@ -344,42 +344,52 @@ __global__ __launch_bounds__(64 * kQ4Waves) void q4_held(Q4P p) {
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    Q4Op<X> x[NK][1][4];
+    Q4Op<X> x[NK][RT][4];
 #pragma unroll
     for (int k = 0; k < NK; ++k)
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-            x[k][0][st].make(a[k][0][st]);
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int e = 0; e < Q4Op<X>::kParts; ++e) asm volatile("" : "+v"(x[k][0][st].v[e]));
-        }
+            for (int st = 0; st < 4; ++st) {
+                x[k][i][st].make(a[k][i][st]);
+#pragma unroll
+                for (int e = 0; e < Q4Op<X>::kParts; ++e) asm volatile("" : "+v"(x[k][i][st].v[e]));
+            }
     const Q4Bias bias(p);
-    Q4Scales<X, 1> xs(p, m0, l);
+    Q4Scales<X, RT> xs(p, m0, l);
     if constexpr (X == Q4_I8) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(xs.v[0][e]));
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(xs.v[i][e]));
     }
     int turn = 0;
     for (int j = blockIdx.x; j < p.w.NT; j += gridDim.x, ++turn) {
         const Q4Tile next(p.w, j + gridDim.x);
         const float add = bias.at(j * kQ4N + (l & 15));
-        q4_f32x4 tot[1] = {q4_f32x4{0.f, 0.f, 0.f, 0.f}};
+        q4_f32x4 tot[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) tot[i] = q4_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
 #pragma unroll
-            for (int g = 0; g < GB; ++g) q4_group<X, 1, GB, S>(b[k], g, x[k], tot);
+            for (int g = 0; g < GB; ++g) q4_group<X, RT, GB, S>(b[k], g, x[k], tot);
             // behind the block's last use, so that its registers are these
             __builtin_amdgcn_sched_barrier(0);
             b[k].load(next, kb0 + k, l);
             __builtin_amdgcn_sched_barrier(0);
         }
-        q4_f32x4* red = q4_red + (turn & 1) * nw * 64;
-        red[w * 64 + l] = tot[0];
+        q4_f32x4* red = q4_red + (turn & 1) * RT * nw * 64;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) red[(i * nw + w) * 64 + l] = tot[i];
         __syncthreads();
-        if (w != turn % nw) continue;
-        q4_f32x4 s = red[l];
-        for (int k = 1; k < nw; ++k) s += red[k * 64 + l];
-        q4_store<X>(p, m0 + 4 * (l >> 4), j * kQ4N + (l & 15), s, xs.v[0], add);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            if (w != (turn * RT + i) % nw) continue;
+            q4_f32x4 s = red[i * nw * 64 + l];
+            for (int k = 1; k < nw; ++k) s += red[(i * nw + k) * 64 + l];
+            q4_store<X>(p, m0 + 16 * i + 4 * (l >> 4), j * kQ4N + (l & 15), s, xs.v[i], add);
+        }
     }
 }
 
@@ -458,15 +468,15 @@ __global__ __launch_bounds__(256) void q4_pad(const T* x, int64_t ld, int64_t ro
     }
 }
 
-template <int X, int NK, int GB>
+template <int X, int RT, int NK, int GB>
 static void q4_held_launch(const Q4P& p, int nw, hipStream_t s) {
-    const int by = (int)((p.rows + 15) / 16);
+    const int by = (int)((p.rows + 16 * RT - 1) / (16 * RT));
     // the chip full once: two workgroups of four waves a CU, or one
     const dim3 grid(std::min(p.w.NT, std::max(8, (nw == 4 ? 512 : 256) / by)), by), block(64 * nw);
-    const size_t lds = (size_t)2 * nw * 64 * 16;
-    if (!p.w.sbf16) hipLaunchKernelGGL((q4_held<X, NK, GB, Q4_S32>), grid, block, lds, s, p);
-    else if (p.w.zeros) hipLaunchKernelGGL((q4_held<X, NK, GB, Q4_S16Z>), grid, block, lds, s, p);
-    else hipLaunchKernelGGL((q4_held<X, NK, GB, Q4_S16>), grid, block, lds, s, p);
+    const size_t lds = (size_t)2 * RT * nw * 64 * 16;
+    if (!p.w.sbf16) hipLaunchKernelGGL((q4_held<X, RT, NK, GB, Q4_S32>), grid, block, lds, s, p);
+    else if (p.w.zeros) hipLaunchKernelGGL((q4_held<X, RT, NK, GB, Q4_S16Z>), grid, block, lds, s, p);
+    else hipLaunchKernelGGL((q4_held<X, RT, NK, GB, Q4_S16>), grid, block, lds, s, p);
 }
 template <int X, int RT, int C, int GB>
 static void q4_walk_launch(const Q4P& p, hipStream_t s) {
@@ -480,20 +490,29 @@ static void q4_walk_launch(const Q4P& p, hipStream_t s) {
 }
 // The rows in registers wherever twelve waves hold them (60 blocks of k, f32 24), as four, eight or
 // twelve waves, which load the four SIMDs evenly; else the walk.  us held / walked, bf16 at 2560 x 10240:
-// 32 rows 12.8 / 19.9, 64 rows 16.4 / 26.7, 256 rows 41 / 78; int8 64 rows 14.5 / 23.4, at 5120 x
-// 2560 15.5 / 14.7; f32 one row 8.9 / 27.
+// 32 rows 12.5 / 19.9, 64 rows 15.8 / 26.7, 256 rows 41 / 78; int8 64 rows 14.6 / 23.4, at 5120 x
+// 2560 11.1 / 14.7; f32 one row 9.1 / 27.
+// Two row tiles a wave take apart a block once for both, but start with twice the rows to load: where
+// a workgroup has ten tiles or more to go through.  us with one / two at 2560 x 10240: bf16 64 rows
+// (5 tiles) 15.8 / 18.7, 128 rows (10) 24.6 / 23.4, 256 rows (20) 41.0 / 35.0, int8 35.2 / 30.4; bf16
+// 64 rows at 2560 x 50001 (24) 50.3 / 42.6.
 template <int X, int GB>
 static void q4_shape(const Q4P& p, hipStream_t s) {
     constexpr int most = X == Q4_F32 ? 2 : 5;  // blocks of k whose operands a wave's registers hold
     const int nw = p.w.KB <= 4 * most ? 4 : p.w.KB <= 8 * most ? 8 : 12, NK = ceil_div(p.w.KB, nw);
     if (NK > most) return q4_walk_launch<X, 2, 2, GB>(p, s);
     if constexpr (X == Q4_F32) {
-        q4_held_launch<X, 2, GB>(p, nw, s);
+        q4_held_launch<X, 1, 2, GB>(p, nw, s);
+    } else if (nw < kQ4Waves && p.rows > 16 && ((p.rows + 15) / 16) * p.w.NT >= 5120) {
+        if (NK <= 2) q4_held_launch<X, 2, 2, GB>(p, nw, s);
+        else if (NK == 3) q4_held_launch<X, 2, 3, GB>(p, nw, s);
+        else if (NK == 4) q4_held_launch<X, 2, 4, GB>(p, nw, s);
+        else q4_held_launch<X, 2, 5, GB>(p, nw, s);
     } else {
-        if (NK <= 2) q4_held_launch<X, 2, GB>(p, nw, s);
-        else if (NK == 3) q4_held_launch<X, 3, GB>(p, nw, s);
-        else if (NK == 4) q4_held_launch<X, 4, GB>(p, nw, s);
-        else q4_held_launch<X, 5, GB>(p, nw, s);
+        if (NK <= 2) q4_held_launch<X, 1, 2, GB>(p, nw, s);
+        else if (NK == 3) q4_held_launch<X, 1, 3, GB>(p, nw, s);
+        else if (NK == 4) q4_held_launch<X, 1, 4, GB>(p, nw, s);
+        else q4_held_launch<X, 1, 5, GB>(p, nw, s);
     }
 }
 template <int X>

@@ -66,6 +66,20 @@ def test_product(dev, rows, k, n, group, zero, sdtype, dtype):
     assert bool((wide[:, :2] == 7).all()) and bool((wide[:, 2 + n:] == 7).all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32, I8])
+@pytest.mark.parametrize("rows,k,n,group,zero,sdtype", [(33, 160, 27400, 32, True, F32), (200, 1280, 6500, 64, True, BF16),
+                                                        (350, 2000, 3900, 128, False, BF16), (100, 2500, 12000, 64, False, BF16),
+                                                        (47, 5000, 27400, 128, True, BF16)])
+def test_many_rows_and_columns(dev, rows, k, n, group, zero, sdtype, dtype):
+    codes, scale, z, w = weight(dev, k, n, group, zero, sdtype)
+    x = rows_of(dev, rows, k, dtype)
+    xs = (torch.rand(rows, generator=gen(2)) + 0.1).to(dev) * 0.01 if dtype == I8 else None
+    bias = torch.randn(n, generator=gen(3)).to(dev)
+    y = mamba_hip.linear_q4(x, w, bias, xs, dtype=F32)
+    go.close(y, *go.q4(x, codes, scale, z, group, bias, xs), roundings(k, group), "y")
+    assert torch.equal(y, mamba_hip.linear_q4(x, w, bias, xs, dtype=F32))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_rows_off_centre(dev, dtype):
     """Rows with a mean beside which their spread is small: what the zero points take off is

@@ -622,23 +622,29 @@ struct GatedStepP {
     void* y; int64_t y_sb;
 };
 
+// A token a row, a channel a lane: 256 tokens of 5120 bf16 channels 8.0 us for 23.6 MB.  Bound by the
+// latency of its loads, which do not wait for the slot; two channels a lane took 9.2 us and four 7.6,
+// and a single token 2.6 and 3.0 us against 2.4.
 template <typename T>
 __global__ __launch_bounds__(256) void gated_step(GatedStepP p) {
     const int b = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
     if (c >= p.D) return;
-    const int64_t slot = slot_of(p.slots, b, p.nslots);
-    T* y = static_cast<T*>(p.y) + b * p.y_sb + c;
-    if (slot < 0) {
-        store_f32<T>(y, 0.f);
-        return;
-    }
-    const Decay g = g_decay<true>(p.A[c] * g_sigmoid(load_f32<T>(static_cast<const T*>(p.r) + b * p.r_sb + c)));
-    float* st = p.state + slot * p.D + c;
-    const float u = g_sigmoid(load_f32<T>(static_cast<const T*>(p.i) + b * p.i_sb + c)) * load_f32<T>(static_cast<const T*>(p.x) + b * p.x_sb + c);
-    const float h = __builtin_fmaf(g.a, *st, __builtin_amdgcn_sqrtf(g.q) * u);
-    *st = h;
+    const float r = load_f32<T>(static_cast<const T*>(p.r) + b * p.r_sb + c);
+    const float i = load_f32<T>(static_cast<const T*>(p.i) + b * p.i_sb + c);
+    const float x = load_f32<T>(static_cast<const T*>(p.x) + b * p.x_sb + c);
     const float z = p.z ? load_f32<T>(static_cast<const T*>(p.z) + b * p.z_sb + c) : 0.f;
-    store_f32<T>(y, p.z ? h * z * g_sigmoid(z) : h);
+    const float A = p.A[c];
+    const int64_t slot = slot_of(p.slots, b, p.nslots);
+    float y = 0.f;
+    if (slot >= 0) {
+        float* st = p.state + slot * p.D + c;
+        const float h0 = *st;
+        const Decay g = g_decay<true>(A * g_sigmoid(r));
+        y = __builtin_fmaf(g.a, h0, __builtin_amdgcn_sqrtf(g.q) * (g_sigmoid(i) * x));
+        *st = y;
+        if (p.z) y = y * z * g_sigmoid(z);
+    }
+    store_f32<T>(static_cast<T*>(p.y) + b * p.y_sb + c, y);
 }
 
 // The tiles of a call, and its workspace at ws (counted from NULL: its size): the ticket, the maps

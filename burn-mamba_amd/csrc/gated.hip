@@ -16,8 +16,7 @@
 // it while the tile is there.
 // A stretch of rows maps the state that enters it, h -> P h + H; P is the product of its
 // decays and H what it leaves from zero.  A lane holds R rows of one channel (two would take
-// twice the registers and leave the backward one workgroup a CU: 8192 x 5120 of bf16 360 us against
-// 245); the maps of the eight waves are joined in LDS to the tile's, which is published to the
+// twice the registers and leave the backward one workgroup a CU, which took half as long again); the maps of the eight waves are joined in LDS to the tile's, which is published to the
 // other workgroups before the tile's own state is waited for.  That state is joined from the
 // published maps of the tiles before it, back to the one in which the tile's first sequence
 // begins, or to the last group of 16 tiles, whose final state its last tile publishes.  The
@@ -58,7 +57,7 @@ struct GatedP {
     float* dA; float* dh0;
     // tiles of rows and of channels; the workspace
     int ntile, nct;
-    uint32_t* ticket;
+    uint32_t* ticket;                   // [nct], kGTicket words apart
     uint64_t* map;                      // [ntile][nct kGC] published maps
     uint64_t* ends;                     // [ntile / kGGroup][nct kGC] states at the ends of groups
     float* part;                        // [ntile][D] partial sums of dA
@@ -68,9 +67,10 @@ constexpr int kCarryRows = 64;  // rows between the states that the forward keep
 constexpr int kGW = 8, kGC = 64;  // waves of a workgroup; channels of a tile: one a lane
 constexpr int kGGroup = 16;                      // tiles of a group
 constexpr uint64_t kGNone = ~0ull;               // nothing published yet
-// Rows of a lane.  What a tile costs beside its rows is the same for 8 of them: the forward of
-// 8192 x 5120 took 154 us with 8 (bf16) and 126 with 16 (f32 170 and 143).  The backward holds
-// nine values of a row where the forward holds two, and a tile of it enters with kept states.
+constexpr int kGTicket = 32;                     // words between the tickets of two column tiles
+// Rows of a lane.  What a tile costs beside its rows is the same for 8 of them: with 8 the forward
+// of 8192 x 5120 takes 1.2 times as long as with 16.  The backward holds nine values of a row where
+// the forward holds two, and a tile of it enters with kept states.
 constexpr int kGRows = kCarryRows / kGW, kGFwdRows = 2 * kGRows;
 
 // v is formed here: the compiler moves a value to the block of its only use, and what it is
@@ -140,7 +140,7 @@ __device__ __forceinline__ void g_decays(float (&a)[R], float (&q)[R]) {
 // that one's first row and end.  The offsets are clamped: a wrong one gives a wrong result and
 // no access out of range.  They are searched with scalar loads, which do not queue behind the rows
 // in flight, and each lane looks for its own row only where the rows are not all of one sequence
-// (8192 x 5120 of bf16, six sequences: forward 126 us with lanes that searched, 6 more than one).
+// (lanes that searched cost 8192 x 5120 a tenth).
 struct GRows {
     uint64_t live, first, last;
     int s, b, e;
@@ -212,9 +212,9 @@ __device__ __forceinline__ uint64_t g_wait(const uint64_t* at, uint64_t v) {
     return v;
 }
 
-__global__ __launch_bounds__(256) void gated_clear(uint32_t* ticket, uint4* words, int64_t n) {
+__global__ __launch_bounds__(256) void gated_clear(uint32_t* ticket, int nct, uint4* words, int64_t n) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i == 0) *ticket = 0;
+    if (i < nct) ticket[i * kGTicket] = 0;  // nct <= n
     for (int64_t k = i; k < n; k += (int64_t)gridDim.x * 256) words[k] = make_uint4(~0u, ~0u, ~0u, ~0u);
 }
 
@@ -228,13 +228,17 @@ struct GShared {
 };
 
 // The tile of this workgroup (in the order in which the tiles wait for one another) and its channels.
+// A ticket for each column tile: one counter for all is asked by 512 workgroups at once when a
+// kernel starts (4000 x 2560 of bf16 40 us, 35 with a ticket each).  The columns turn against the
+// workgroups' numbers from a row of tiles to the next, as the numbers go around the chip's eight
+// dies: a die that kept every eighth column would go through a few channels of its L2 (8192 x 5120
+// 116 us, 106 with the turn).
 __device__ __forceinline__ void g_tile(const GatedP& p, GShared& s, int& o, int& ct) {
     if (p.ntile > 1) {
-        if (threadIdx.x == 0) s.tile = (int)atomicAdd(p.ticket, 1u);
+        ct = (blockIdx.x + blockIdx.x / p.nct) % p.nct;
+        if (threadIdx.x == 0) s.tile = (int)atomicAdd(p.ticket + ct * kGTicket, 1u);
         __syncthreads();
-        const int k = __builtin_amdgcn_readfirstlane(s.tile);
-        o = k / p.nct;
-        ct = k - o * p.nct;
+        o = __builtin_amdgcn_readfirstlane(s.tile);
     } else {
         o = 0;
         ct = blockIdx.x;
@@ -329,6 +333,10 @@ __device__ __forceinline__ void g_fetch(uint32_t (&e)[R], const GatedP& p, const
     for (int j = 0; j < R; ++j) e[j] = row.load(min(j, k), col);
 }
 
+// 8192 x 5120: bf16 with z 106 us (420 MB, 4.0 TB/s), f32 without 132 (671 MB, 5.1: what a copy
+// reaches).  bf16: half the time is issue of vector instructions (46 a row, 7 of them at a quarter
+// of the rate), the rest a tile's latencies (ticket, rows, the states that enter), which two
+// workgroups a CU hide in part; three (80 registers) spill and take 1.2 times as long.
 template <typename T, bool Z>
 __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
     constexpr int R = kGFwdRows;
@@ -436,6 +444,8 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
 // What a row's gradients need is formed once, where its values are read: with u = s(i) x,
 //   gr = dy silu(z), zk = dy silu'(z), pull = u a^2 / m, kr = A s(r) s(-r), ui = u s(-i)
 // so that dz = h zk, dx = dh m s(i), di = dh m ui, dr = e kr, e = dh (a h_{t-1} - pull).
+// 8192 x 5120: bf16 with z 207 us with the join (755 MB, 3.6 TB/s), f32 without 236 (1174 MB, 5.0).
+// Bound as the forward is: some 95 vector instructions a row.
 template <typename T, bool Z>
 __global__ __launch_bounds__(64 * kGW, 4) void gated_bwd(GatedP p) {
     constexpr int R = kGRows;
@@ -685,7 +695,7 @@ static size_t gated_plan(GatedP& p, bool back, void* ws) {
         return q;
     };
     if (words) {
-        p.ticket = reinterpret_cast<uint32_t*>(take(4));
+        p.ticket = reinterpret_cast<uint32_t*>(take((size_t)p.nct * kGTicket * 4));
         p.map = reinterpret_cast<uint64_t*>(take(8 * words));
         p.ends = p.map + p.ntile * Dp;
     }
@@ -695,7 +705,7 @@ static size_t gated_plan(GatedP& p, bool back, void* ws) {
 static void gated_clear_launch(const GatedP& p, hipStream_t s) {
     if (p.ntile <= 1) return;
     const int64_t n = (int64_t)(p.ntile + p.ntile / kGGroup) * p.nct * kGC / 2;  // kGC words are whole 16 bytes
-    hipLaunchKernelGGL(gated_clear, dim3((uint32_t)std::min<int64_t>((n + 255) / 256, 2048)), dim3(256), 0, s, p.ticket, reinterpret_cast<uint4*>(p.map), n);
+    hipLaunchKernelGGL(gated_clear, dim3((uint32_t)std::min<int64_t>((n + 255) / 256, 2048)), dim3(256), 0, s, p.ticket, p.nct, reinterpret_cast<uint4*>(p.map), n);
 }
 static int gated_grid_ok(const GatedP& p) {
     MAMBA_CHECK_ARG((int64_t)p.ntile * p.nct * 64 * kGW < (1ll << 32), "rows x dim is too large for one call");

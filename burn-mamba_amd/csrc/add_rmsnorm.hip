@@ -6,7 +6,9 @@
 //   g = dy w,  xh = s rstd:  d = ds + rstd (g - xh mean(g xh)),  dw = sum_r dy xh
 //
 // The sum is normalised as it is in f32, before it is rounded to the stream's type: y
-// then has one rounding.  The backward reads the stored s.
+// then has one rounding.  The backward reads the stored s, or, where that one was rounded to bf16,
+// the two rows that it was the sum of (16384 x 2560 91 us against 80): from the rounded s dw is off
+// by 2e-3 of itself, from the sum by 1e-7.
 //
 // Some ten operations an element against three or four elements moved: HBM-bound.  Rows of up to
 // 10240 bf16 or 5120 f32 stream elements stay in registers, so that each element is read
@@ -237,15 +239,16 @@ __global__ __launch_bounds__(256) void arn_fwd_rows(ArnP p) {
     }
 }
 
-// The workgroups take their rows in turn; part[blockIdx.x] gets the workgroup's dw.
-template <typename T, typename S, int G, int V>
+// The workgroups take their rows in turn; part[blockIdx.x] gets the workgroup's dw.  SUM: s + x in
+// the place of s.
+template <typename T, typename S, int G, int V, bool SUM>
 __global__ __launch_bounds__(256) void arn_bwd_rows(ArnP p) {
     constexpr int E = kArnE<S>, RB = 256 / G;
     __shared__ uint32_t red[8];
     __shared__ float s_w[G < 256 ? G * V * E : 1];  // after the rows, the groups' sums
     const int l = threadIdx.x % G, sub = threadIdx.x / G;
     Elems<S, E> rs[V], rd[V];
-    Elems<T, E> rg[V];
+    Elems<T, E> rg[V], rx[SUM ? V : 1];
     float rstd = 0.f, dw[V][E], w[V][E];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
@@ -262,6 +265,7 @@ __global__ __launch_bounds__(256) void arn_bwd_rows(ArnP p) {
         const S* s = static_cast<const S*>(p.s) + r * p.s_sr;
         const S* d = static_cast<const S*>(p.ds) + r * p.ds_sr;
         const T* g = static_cast<const T*>(p.dy) + r * p.dy_sr;
+        const T* x = static_cast<const T*>(p.x) + r * p.x_sr;
         rstd = p.rstd[r];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -270,10 +274,12 @@ __global__ __launch_bounds__(256) void arn_bwd_rows(ArnP p) {
                 rs[k].load(s + c);
                 rg[k].load(g + c);
                 if (p.ds) rd[k].load(d + c);
+                if constexpr (SUM) rx[k].load(x + c);
             } else {
                 rs[k].load_part(s + c, n);
                 rg[k].load_part(g + c, n);
                 if (p.ds) rd[k].load_part(d + c, n);
+                if constexpr (SUM) rx[k].load_part(x + c, n);
             }
         }
     };
@@ -291,6 +297,12 @@ __global__ __launch_bounds__(256) void arn_bwd_rows(ArnP p) {
             rs[k].get(xh[k]);
             rg[k].get(g[k]);
             if (p.ds) rd[k].get(d[k]);
+            if constexpr (SUM) {
+                float x[E];
+                rx[k].get(x);
+#pragma unroll
+                for (int i = 0; i < E; ++i) xh[k][i] += x[i];
+            }
         }
         fetch(r + step);
         if (live) {
@@ -402,6 +414,20 @@ __global__ __launch_bounds__(256) void arn_fwd_wide(ArnP p) {
     }
 }
 
+// the backward's s from column c of a row on
+template <typename T, typename S, int E>
+__device__ __forceinline__ void arn_sum_row(const ArnP& p, const S* s, int64_t r, int c, float (&v)[E]) {
+    ld_run<E, S>(s + c, p.cols - c, v);
+    if constexpr (sizeof(S) == 2) {
+        if (p.x) {
+            float x[E];
+            ld_run<E, T>(static_cast<const T*>(p.x) + r * p.x_sr + c, p.cols - c, x);
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] += x[i];
+        }
+    }
+}
+
 template <typename T, typename S>
 __global__ __launch_bounds__(256) void arn_dx_wide(ArnP p) {
     constexpr int E = 4, ST = 256 * E;
@@ -412,7 +438,7 @@ __global__ __launch_bounds__(256) void arn_dx_wide(ArnP p) {
         const float rstd = p.rstd[r];
         float v[E], g[E], w[E];
         auto load = [&](int c) __attribute__((always_inline)) {
-            ld_run<E, S>(s + c, p.cols - c, v);
+            arn_sum_row<T, S, E>(p, s, r, c, v);
             ld_run<E, T>(dy + c, p.cols - c, g);
             if (p.w) ld_run<E, float>(p.w + c, p.cols - c, w);
 #pragma unroll
@@ -452,7 +478,7 @@ __global__ __launch_bounds__(256) void arn_dw_wide(ArnP p) {
     if (c < p.cols)
         for (int64_t r = r0 + q; r < r1; r += 4) {
             float v[E], g[E];
-            ld_run<E, S>(static_cast<const S*>(p.s) + r * p.s_sr + c, p.cols - c, v);
+            arn_sum_row<T, S, E>(p, static_cast<const S*>(p.s) + r * p.s_sr, r, c, v);
             ld_run<E, T>(static_cast<const T*>(p.dy) + r * p.dy_sr + c, p.cols - c, g);
             const float rstd = p.rstd[r];
 #pragma unroll
@@ -516,8 +542,15 @@ static int arn_parts(int64_t rows, int cols, int E) {
 
 template <typename T, typename S, int G, int V>
 static void arn_rows_launch(const ArnP& p, bool back, hipStream_t s) {
-    if (back) hipLaunchKernelGGL((arn_bwd_rows<T, S, G, V>), dim3(p.parts), dim3(256), 0, s, p);
-    else if (p.q) hipLaunchKernelGGL((arn_fwd_rows<T, S, G, V, true>), dim3(arn_fwd_grid(p.rows, G)), dim3(256), 0, s, p);
+    if (back) {
+        if constexpr (sizeof(S) == 2) {
+            if (p.x) {
+                hipLaunchKernelGGL((arn_bwd_rows<T, S, G, V, true>), dim3(p.parts), dim3(256), 0, s, p);
+                return;
+            }
+        }
+        hipLaunchKernelGGL((arn_bwd_rows<T, S, G, V, false>), dim3(p.parts), dim3(256), 0, s, p);
+    } else if (p.q) hipLaunchKernelGGL((arn_fwd_rows<T, S, G, V, true>), dim3(arn_fwd_grid(p.rows, G)), dim3(256), 0, s, p);
     else hipLaunchKernelGGL((arn_fwd_rows<T, S, G, V, false>), dim3(arn_fwd_grid(p.rows, G)), dim3(256), 0, s, p);
 }
 // rows in registers; false where they are too wide
@@ -622,11 +655,12 @@ extern "C" int mamba_add_rmsnorm_bwd(const mamba_add_rmsnorm_bwd_args* a, void* 
     int st = arn_check(a->rows, a->cols, a->io_dtype, a->stream_dtype);
     if (st != MAMBA_OK) return st;
     MAMBA_CHECK_ARG(a->rows == 0 || (a->s && a->dy && a->rstd), "s, dy and rstd are required");
+    MAMBA_CHECK_ARG(!a->x || a->stream_dtype == MAMBA_BF16, "x goes with a bf16 stream");
     const int64_t R = a->rows;
     const int C = a->cols, e = a->io_dtype == MAMBA_BF16 ? 2 : 4, f = a->stream_dtype == MAMBA_BF16 ? 2 : 4;
     MAMBA_CHECK_ARG(R <= 1 || ((!a->dx || a->dx_sr >= C) && (!a->dresidual || a->dresidual_sr >= C)), "rows of dx or dresidual overlap");
     struct Rows { const void* p; int64_t sr; int e; };
-    const Rows ins[] = {{a->s, a->s_sr, f}, {a->dy, a->dy_sr, e}, {a->ds, a->ds_sr, f}}, outs[] = {{a->dx, a->dx_sr, e}, {a->dresidual, a->dresidual_sr, f}};
+    const Rows ins[] = {{a->s, a->s_sr, f}, {a->dy, a->dy_sr, e}, {a->ds, a->ds_sr, f}, {a->x, a->x_sr, e}}, outs[] = {{a->dx, a->dx_sr, e}, {a->dresidual, a->dresidual_sr, f}};
     for (const Rows& o : outs)
         for (const Rows& i : ins)
             MAMBA_CHECK_ARG(!arn_clash(o.p, o.sr, o.e, i.p, i.sr, i.e, R, C, false), "a gradient overlaps an input");
@@ -638,7 +672,7 @@ extern "C" int mamba_add_rmsnorm_bwd(const mamba_add_rmsnorm_bwd_args* a, void* 
     }
     ArnP p{};
     p.rows = R; p.cols = C; p.s = const_cast<void*>(a->s); p.s_sr = a->s_sr; p.dy = a->dy; p.dy_sr = a->dy_sr; p.ds = a->ds; p.ds_sr = a->ds_sr;
-    p.w = a->weight; p.rstd = const_cast<float*>(a->rstd); p.y = a->dx; p.y_sr = a->dx_sr; p.dres = a->dresidual; p.dres_sr = a->dresidual_sr;
+    p.w = a->weight; p.rstd = const_cast<float*>(a->rstd); p.x = a->x; p.x_sr = a->x_sr; p.y = a->dx; p.y_sr = a->dx_sr; p.dres = a->dresidual; p.dres_sr = a->dresidual_sr;
     p.part = need ? static_cast<float*>(ws) : nullptr; p.parts = arn_parts(R, C, 16 / f); p.dw = a->dweight;
     ARN_DISPATCH(arn_bwd_launch, a->io_dtype, a->stream_dtype, p, (hipStream_t)stream);
     MAMBA_CHECK_LAUNCH();

@@ -476,6 +476,7 @@ class AddRmsNormBwdArgs(ctypes.Structure):
         ("dx", c_vp), ("dx_sr", c_i64),
         ("dresidual", c_vp), ("dresidual_sr", c_i64),
         ("dweight", c_vp),
+        ("x", c_vp), ("x_sr", c_i64),
     ]
 
 

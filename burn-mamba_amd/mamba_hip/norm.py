@@ -200,23 +200,26 @@ def add_rms_norm_q8(x: torch.Tensor, weight: Optional[torch.Tensor], residual: O
 
 
 def add_rms_norm_bwd(dy: torch.Tensor, s: torch.Tensor, weight: Optional[torch.Tensor], rstd: torch.Tensor,
-                     ds: Optional[torch.Tensor] = None) -> dict:
+                     ds: Optional[torch.Tensor] = None, x: Optional[torch.Tensor] = None) -> dict:
     """Gradients of ``add_rms_norm`` from s as it returned it, its rstd, dy and (of s, where it
-    was used) ds: dict(dx of dy's type, dresidual of s's, dweight [cols] f32).  Of one type dx
-    and dresidual are one tensor.  The same inputs give the same bits."""
+    was used) ds: dict(dx of dy's type, dresidual of s's, dweight [cols] f32).  With a bf16
+    stream s has been rounded; where ``x`` is given, s is the residual instead, and the sum is
+    formed again.  Of one type dx and dresidual are one tensor.  The same inputs give the same
+    bits."""
     m, g = _matrix(s, "s"), _matrix(dy, "dy")
     _need(g.shape == m.shape, "dy must match s")
     _need(s.dtype == torch.float32 or s.dtype == dy.dtype, "s must be float32 or of dy's type")
     _need(ds is None or (ds.shape == s.shape and ds.dtype == s.dtype), "ds must match s")
+    _need(x is None or (s.dtype == torch.bfloat16 and x.shape == s.shape and x.dtype == s.dtype), "x goes with a bfloat16 residual, and must match it")
     _param(weight, "weight", m.shape[1])
     _need(rstd is not None, "rstd is required")
     _param(rstd, "rstd", m.shape[0])
-    with _one_device(m, g, weight, rstd, ds):
-        dx, dresidual, dweight = _arn_bwd(dy, g, s, m, weight, rstd, ds, True, True)
+    with _one_device(m, g, weight, rstd, ds, x):
+        dx, dresidual, dweight = _arn_bwd(dy, g, s, m, weight, rstd, ds, x, True, True)
     return dict(dx=dx, dresidual=dresidual, dweight=dweight)
 
 
-def _arn_bwd(dy, g, s, m, weight, rstd, ds, want_dx, want_dres):
+def _arn_bwd(dy, g, s, m, weight, rstd, ds, x, want_dx, want_dres):
     """``add_rms_norm_bwd`` after its checks (g, m: the rows of dy and s)."""
     a = AddRmsNormBwdArgs()
     a.rows, a.cols = m.shape
@@ -225,6 +228,9 @@ def _arn_bwd(dy, g, s, m, weight, rstd, ds, want_dx, want_dres):
     d = None if ds is None else _matrix(ds, "ds")
     if d is not None:
         a.ds, a.ds_sr = d.data_ptr(), d.stride(0)
+    xm = None if x is None else _matrix(x, "x")
+    if xm is not None:
+        a.x, a.x_sr = xm.data_ptr(), xm.stride(0)
     one = s.dtype == dy.dtype
     dres = _new(s) if want_dres or (one and want_dx) else None
     dx = dres if one else _new(dy) if want_dx else None
@@ -246,14 +252,15 @@ class _AddRmsNorm(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps):
         rstd = x.new_empty(x.numel() // max(x.shape[-1], 1) if x.dim() else 1, dtype=torch.float32)
         y, s = add_rms_norm(x, weight, residual, eps, rstd=rstd)
-        ctx.save_for_backward(s, weight, rstd)
+        again = residual is not None and residual.dtype == torch.bfloat16  # s has been rounded
+        ctx.save_for_backward(residual if again else s, weight, rstd, x if again else None)
         ctx.io = x.dtype
         ctx.set_materialize_grads(False)
         return (y, s) if residual is not None else y
 
     @_once
     def backward(ctx, dy, ds=None):
-        s, weight, rstd = ctx.saved_tensors
+        s, weight, rstd, x = ctx.saved_tensors
         wx, ww, wr = ctx.needs_input_grad[:3]
         if dy is None:  # the sum alone was used
             if ds is None:
@@ -261,7 +268,7 @@ class _AddRmsNorm(torch.autograd.Function):
             return ds.to(ctx.io), torch.zeros_like(weight) if ww else None, ds, None
         m, g = _matrix(s, "s"), _matrix(dy, "dy")
         with _one_device(g):
-            dx, dres, dweight = _arn_bwd(dy, g, s, m, weight, rstd, ds, wx, wr)
+            dx, dres, dweight = _arn_bwd(dy, g, s, m, weight, rstd, ds, x, wx, wr)
         return dx, dweight if ww else None, dres if wr else None, None
 
 

@@ -1138,7 +1138,9 @@ typedef struct mamba_add_rmsnorm_args {
 int mamba_add_rmsnorm_fwd(const mamba_add_rmsnorm_args* args, mamba_stream_t stream);
 
 /* Its gradients from s as the forward stored it (x itself without a           */
-/* residual), rstd, dy and, if given, ds (of s, stream_dtype), xh = s rstd:    */
+/* residual), rstd, dy and, if given, ds (of s, stream_dtype), xh = s rstd.    */
+/* A stream of bf16 has rounded s: with x given, s points to residual, and the */
+/* sum is formed again.                                                        */
 /*   d = ds + rstd (dy weight - xh mean(dy weight xh)),  dweight = sum dy xh   */
 /* d is written as dx (io_dtype) and as dresidual (stream_dtype), each if      */
 /* given; dweight may be NULL.  Sums in a fixed order.                         */
@@ -1153,6 +1155,7 @@ typedef struct mamba_add_rmsnorm_bwd_args {
     void* dx;             int64_t dx_sr;
     void* dresidual;      int64_t dresidual_sr;
     float* dweight;
+    const void* x;        int64_t x_sr;       /* or NULL                      */
 } mamba_add_rmsnorm_bwd_args;
 
 size_t mamba_add_rmsnorm_bwd_workspace_size(const mamba_add_rmsnorm_bwd_args* args);
@@ -1189,9 +1192,9 @@ int mamba_dropout(const mamba_dropout_args* args, mamba_stream_t stream);
 /* zero points in the same buffer (packed, of mamba_linear_q4_packed_size      */
 /* bytes, 16-byte aligned).                                                    */
 /* x: bf16, f32 (three bf16 parts, which hold all of it) or int8 with x_scale  */
-/* [rows]; sums are f32, of int8 rows exact within a group.  The codes are     */
-/* multiplied as they are and the zero points taken off a group's sum, so a    */
-/* row of x with a NaN or an infinity gives NaN everywhere.                    */
+/* [rows]; sums are f32, of int8 rows exact within a group.  The codes and the */
+/* zero points are multiplied apart, so a row of x with a NaN or an infinity   */
+/* gives a row of NaN.                                                         */
 /* ------------------------------------------------------------------------- */
 typedef struct mamba_q4_weight {
     int32_t d_in, d_out, group, scale_dtype;  /* scales f32 or bf16           */

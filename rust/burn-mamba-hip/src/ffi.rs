@@ -1181,6 +1181,8 @@ pub struct MambaAddRmsnormBwdArgs {
     pub dresidual: *mut c_void,
     pub dresidual_sr: i64,
     pub dweight: *mut f32,
+    pub x: *const c_void,
+    pub x_sr: i64,
 }
 
 impl Default for MambaAddRmsnormBwdArgs {

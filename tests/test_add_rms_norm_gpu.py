@@ -85,29 +85,46 @@ def test_autograd(dev, io, stream):
     y, s = mamba_hip.add_rms_norm_autograd(*leaves)
     g = gen(4)
     dy, ds = torch.randn(rows, cols, generator=g).to(io).to(dev), torch.randn(rows, cols, generator=g).to(s.dtype).to(dev)
-    rstd = torch.empty(rows, device=dev)
-    mamba_hip.add_rms_norm(x, w, res, rstd=rstd)
-    ref = go.add_rms_bwd(dy, s, w, rstd, ds)
+    s0, rstd, _ = go.add_rms(x, w, res, 1e-5)  # the sum as it is, which a bf16 stream has rounded
+    rstd = rstd[:, 0]
+    ref = go.add_rms_bwd(dy, s0, w, rstd, ds)
     if res is None:  # s is x: its gradient is added by autograd, which rounds both
         grads = torch.autograd.grad(y, leaves, dy, retain_graph=True)
-        ref = go.add_rms_bwd(dy, s, w, rstd, None)
+        ref = go.add_rms_bwd(dy, s0, w, rstd, None)
     else:
         grads = torch.autograd.grad((y, s), leaves, (dy, ds), retain_graph=True)
-        go.close(grads[2], *ref["d"], roundings(cols), "dresidual")
+        go.close(grads[2], *ref["d"], 4 * roundings(cols), "dresidual")
         assert grads[2].dtype == stream
-    go.close(grads[0], *ref["d"], roundings(cols), "dx")
-    go.close(grads[1], *ref["dweight"], 8 + rows, "dweight")
+    go.close(grads[0], *ref["d"], 4 * roundings(cols), "dx")  # rstd is up to three of its factors
+    go.close(grads[1], *ref["dweight"], 8 + rows + roundings(cols), "dweight")
     assert grads[0].dtype == io and grads[1].dtype == F32
     if res is not None:
         # the sum alone, the norm alone, one leaf alone
         only = torch.autograd.grad(s, leaves, ds, retain_graph=True)
         assert torch.equal(only[0], ds.to(io)) and torch.equal(only[2], ds) and not only[1].any()
-        ref = go.add_rms_bwd(dy, s, w, rstd, None)
+        ref = go.add_rms_bwd(dy, s0, w, rstd, None)
         only = torch.autograd.grad(y, leaves[2], dy.expand(rows, cols), retain_graph=True)
-        go.close(only[0], *ref["d"], roundings(cols), "dresidual of y")
+        go.close(only[0], *ref["d"], 4 * roundings(cols), "dresidual of y")
         only = torch.autograd.grad(y.sum(), leaves[1])
-        ref = go.add_rms_bwd(torch.ones_like(dy), s, w, rstd, None)
-        go.close(only[0], *ref["dweight"], 8 + rows, "dweight of a sum")
+        ref = go.add_rms_bwd(torch.ones_like(dy), s0, w, rstd, None)
+        go.close(only[0], *ref["dweight"], 8 + rows + roundings(cols), "dweight of a sum")
+
+
+@pytest.mark.parametrize("rows,cols", SIZES + [(700, 300)])
+def test_backward_of_the_sum_as_it_is(dev, rows, cols):
+    """The two rows of a bf16 stream in the place of their rounded sum."""
+    x, w, res = make(dev, rows, cols, BF16, BF16, 14)
+    s0, rstd0, _ = go.add_rms(x, w, res, 1e-5)
+    rstd = torch.empty(rows, device=dev)
+    mamba_hip.add_rms_norm(x, w, res, 1e-5, rstd=rstd)
+    g = gen(15)
+    dy, ds = rows_of(g, rows, cols, BF16, dev, 1, 0), rows_of(g, rows, cols, BF16, dev)
+    for weight, more in ((w, ds), (None, None)):
+        got = mamba_hip.add_rms_norm_bwd(dy, res, weight, rstd, more, x=x)
+        ref = go.add_rms_bwd(dy, s0, weight, rstd0[:, 0], more)
+        go.close(got["dx"], *ref["d"], 4 * roundings(cols), "dx")  # rstd is up to three of its factors
+        assert got["dx"] is got["dresidual"]
+        go.close(got["dweight"], *ref["dweight"], 8 + rows + roundings(cols), "dweight")
 
 
 def test_gradient_by_differences(dev):

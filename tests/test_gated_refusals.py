@@ -105,7 +105,8 @@ def test_norm_outputs(monkeypatch):
     with pytest.raises(Err, match="not differentiable"):
         mamba_hip.add_rms_norm_q8(z(4, 8).requires_grad_(), z(8))
     for over, what in ((dict(dy=z(4, 7)), "dy"), (dict(s=z(4, 8, dtype=BF)), "s must"), (dict(ds=z(3, 8)), "ds"), (dict(ds=z(4, 8, dtype=BF)), "ds"),
-                       (dict(weight=z(7)), "weight"), (dict(rstd=None), "rstd"), (dict(rstd=z(3)), "rstd")):
+                       (dict(weight=z(7)), "weight"), (dict(rstd=None), "rstd"), (dict(rstd=z(3)), "rstd"), (dict(x=z(4, 8)), "x goes"),
+                       (dict(dy=z(4, 8, dtype=BF), s=z(4, 8, dtype=BF), x=z(4, 7, dtype=BF)), "x goes")):
         b = dict(dy=z(4, 8), s=z(4, 8), weight=z(8), rstd=z(4))
         b.update(over)
         with pytest.raises(Err, match=what):
@@ -261,7 +262,8 @@ def test_c_norm():
         return b
 
     for field, bad, what in (("rstd", None, b"required"), ("dy", None, b"required"), ("dx_sr", 63, b"overlap"), ("dx", FAR, b"overlaps an input"),
-                             ("dresidual", FAR + (3 << 24) + 64, b"dresidual"), ("stream_dtype", 1, b"io_dtype")):
+                             ("dresidual", FAR + (3 << 24) + 64, b"dresidual"), ("stream_dtype", 1, b"io_dtype"),
+                             ("x", FAR + (5 << 24), b"bf16 stream")):
         b = back()
         setattr(b, field, bad)
         assert L.mamba_add_rmsnorm_bwd(ctypes.byref(b), P, 1 << 20, None) == 1 and what in L.mamba_last_error(), field

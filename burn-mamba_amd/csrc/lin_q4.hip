@@ -587,7 +587,8 @@ extern "C" int mamba_linear_q4_fwd(const mamba_linear_q4_args* a, void* ws, size
     MAMBA_CHECK_ARG(p.y_ld >= p.w.N || p.rows == 1, "rows of y overlap");
     const size_t ex = q4_xsize(a->x_dtype), ey = p.ybf16 ? 2 : 4;
     const char *px = static_cast<const char*>(p.x), *py = static_cast<const char*>(p.y);
-    MAMBA_CHECK_ARG(py + ((p.rows - 1) * p.y_ld + p.w.N) * ey <= px || px + ((p.rows - 1) * p.x_ld + p.w.K) * ex <= py, "y overlaps x");
+    const bool apart = py + ((p.rows - 1) * p.y_ld + p.w.N) * ey <= px || px + ((p.rows - 1) * p.x_ld + p.w.K) * ex <= py;
+    MAMBA_CHECK_ARG(apart || (ex == ey && !rows_clash(p.y, p.y_ld, p.x, p.x_ld, p.w.N, p.w.K, p.rows, ex, false)), "y overlaps x");
     hipStream_t s = (hipStream_t)stream;
     const size_t need = mamba_linear_q4_workspace_size(a);
     MAMBA_CHECK_ARG(((uintptr_t)ws & 15u) == 0, "the workspace must be 16-byte aligned");

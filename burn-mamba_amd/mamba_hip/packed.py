@@ -450,8 +450,8 @@ def gated_scan_packed(x, r, i, A, cu_seqlens, z=None, state: Optional[torch.Tens
 
         a_t = exp(A s(r_t)),  h_t = a_t h_{t-1} + sqrt(1 - a_t^2) s(i_t) x_t,  y_t = h_t silu(z_t)
 
-    x, r, i and z [rows, d] f32 or bf16 (one type, any row strides; without z, y_t = h_t), A [d]
-    f32 and at most 0.  ``state`` [slots, d] f32 holds what the sequences start from and is
+    x, r, i and z [rows, d] f32 or bf16 (one type, rows less than 2^25 elements apart; without z,
+    y_t = h_t), A [d] f32 and at most 0.  ``state`` [slots, d] f32 holds what the sequences start from and is
     overwritten with what they end in; None starts from zero.  ``carry``, [ceil(rows / 64), d]
     f32, takes the states that ``gated_scan_packed_bwd`` goes on from.  Returns y [rows, d]
     of x's type.  The same inputs give the same bits."""

@@ -999,7 +999,9 @@ int mamba1_scan_step_slots(const mamba1_scan_step_slots_args* args, mamba_stream
 /* overwritten with its end; NULL starts from zero and keeps nothing.  carry   */
 /* [ceil(rows / 64), d] or NULL: the states that enter rows 0, 64, 128, ...,   */
 /* which the backward takes (what it holds for a row that begins a sequence or */
-/* belongs to none is not looked at).  y may be x, r, i or z itself.           */
+/* belongs to none is not looked at).  y may be x, r, i or z itself.  dim is    */
+/* at most 2^20, and a call's tiles (128 rows x 64 channels, the backward's 64 */
+/* x 64) must be fewer than 2^23.                                              */
 typedef struct mamba_gated_scan_args {
     int64_t rows;
     int32_t nseq, dim, io_dtype, fill_outside;

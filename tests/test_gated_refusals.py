@@ -171,7 +171,8 @@ def test_c_scan():
     for field, bad, what in (("rows", -1, b"rows"), ("rows", 1 << 31, b"rows"), ("nseq", -1, b"nseq"), ("dim", 0, b"dim"), ("dim", (1 << 20) + 1, b"dim"),
                              ("io_dtype", 2, b"io_dtype"), ("A", None, b"A and cu_seqlens"), ("cu_seqlens", None, b"A and cu_seqlens"),
                              ("r", None, b"x, r and i"), ("y", None, b"y is"), ("y_st", 63, b"rows of y"), ("y", FAR + 4, b"overlaps"),
-                             ("y", FAR + (3 << 24) + 128, b"overlaps")):
+                             ("y", FAR + (3 << 24) + 128, b"overlaps"), ("x_st", 1 << 25, b"strides"), ("r_st", -64, b"strides"),
+                             ("i_st", 1 << 40, b"strides"), ("z_st", 1 << 25, b"strides"), ("y_st", 1 << 25, b"2^25")):
         a = _scan_c()
         setattr(a, field, bad)
         assert L.mamba_gated_scan_fwd(ctypes.byref(a), None, 0, None) == 1 and what in L.mamba_last_error(), field
@@ -197,7 +198,8 @@ def _bwd_c():
 def test_c_scan_bwd():
     L = _lib.lib()
     for field, bad, what in (("dA", None, b"dA"), ("dy", None, b"carry, dy"), ("dz", None, b"dz goes with z"), ("dx_st", 60, b"overlap"),
-                             ("dx", FAR, b"overlaps an input"), ("dr", (FAR << 2) + 64, b"two gradients"), ("di", FAR + (5 << 24), b"overlaps an input")):
+                             ("dx", FAR, b"overlaps an input"), ("dr", (FAR << 2) + 64, b"two gradients"), ("di", FAR + (5 << 24), b"overlaps an input"),
+                             ("dy_st", 1 << 25, b"strides"), ("dy_st", -1, b"strides"), ("dz_st", 1 << 25, b"2^25")):
         b = _bwd_c()
         setattr(b, field, bad)
         assert L.mamba_gated_scan_bwd(ctypes.byref(b), None, 0, None) == 1 and what in L.mamba_last_error(), field

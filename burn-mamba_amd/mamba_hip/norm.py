@@ -191,7 +191,7 @@ def add_rms_norm_q8(x: torch.Tensor, weight: Optional[torch.Tensor], residual: O
     with _one_device(m, weight, residual, out, scale, residual_out):
         a, s, _held = _arn_args(x, m, weight, residual, eps, residual_out, None)
         if out is None:
-            out = torch.empty(x.shape, dtype=dtype, device=x.device)
+            out = _new(x, dtype=dtype)
         if scale is None:
             scale = m.new_empty(m.shape[0], dtype=torch.float32)
         a.q_dtype, a.q, a.q_sr, a.scale = _Q8[dtype], out.data_ptr(), m.shape[1], scale.data_ptr()

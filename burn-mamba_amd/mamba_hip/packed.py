@@ -414,11 +414,12 @@ CARRY_ROWS = 64  # rows between the states that the forward keeps for its backwa
 def _gated_operands(x, r, i, A, z):
     """Checks shared by the packed recurrence and the step; (rows, dim)."""
     _rows(x, "x")
-    rows, d = x.shape
-    _rows(r, "r", rows, d, x.dtype)
-    _rows(i, "i", rows, d, x.dtype)
-    if z is not None:
-        _rows(z, "z", rows, d, x.dtype)
+    shape, dtype = x.shape, x.dtype
+    rows, d = shape
+    for t, name in ((r, "r"), (i, "i"), (z, "z")):
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.stride(1) != 1):
+            _rows(t, name, rows, d, dtype)
+    _need(r is not None and i is not None, "r and i are required")
     _param(A, "A", d)
     return rows, d
 

@@ -144,8 +144,7 @@ __device__ __forceinline__ q4_bf16x8 q4_codes_bf16(uint32_t w) {
     return __builtin_bit_cast(q4_bf16x8, d);
 }
 __device__ __forceinline__ long q4_codes_i8x16(uint32_t w) {
-    w ^= 0x88888888u;
-    return (long)((uint64_t)(w & 0xf0f0f0f0u) << 32 | (w << 4 & 0xf0f0f0f0u));
+    return (long)((uint64_t)((w & 0xf0f0f0f0u) ^ 0x80808080u) << 32 | ((w << 4 & 0xf0f0f0f0u) ^ 0x80808080u));
 }
 __device__ __forceinline__ long q4_codes_i8(uint32_t w) { return (long)((uint64_t)(w >> 4 & 0x0f0f0f0fu) << 32 | (w & 0x0f0f0f0fu)); }
 
@@ -230,12 +229,12 @@ __device__ __forceinline__ void q4_group(const Q4Block<GB, S>& b, int g, const Q
                 if constexpr (S != Q4_S16) acc[i] = __builtin_amdgcn_mfma_i32_16x16x32_i8(x[i][st].v[0], off, acc[i], 0, 0, 0);
             }
         }
-        // whole numbers of at most 128 x 127 x 128 < 2^24: exact up to the scale
-        const float by = S == Q4_S16 ? scale * 0.0625f : scale;
+        // whole numbers of at most 128 x 128 x 128 < 2^24: exact up to the scale (a sixteenth of them is
+        // taken with the row's scale)
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) tot[i][e] = __builtin_fmaf(by, (float)acc[i][e], tot[i][e]);
+            for (int e = 0; e < 4; ++e) tot[i][e] = __builtin_fmaf(scale, (float)acc[i][e], tot[i][e]);
     } else {
         const uint32_t z2 = b.minus2(g);
         const q4_bf16x8 off = __builtin_bit_cast(q4_bf16x8, make_uint4(z2, z2, z2, z2));
@@ -293,13 +292,13 @@ struct Q4Bias {
 template <int X, int RT>
 struct Q4Scales {
     float v[RT][4];
-    __device__ __forceinline__ Q4Scales(const Q4P& p, int64_t m0, int l) {
+    __device__ __forceinline__ Q4Scales(const Q4P& p, int64_t m0, int l, float by) {  // by a power of two
         const int here = (int)min((int64_t)16 * RT, p.rows - m0);
         const __amdgpu_buffer_rsrc_t r = buf_rsrc(p.xs + (X == Q4_I8 ? m0 : 0), X == Q4_I8 ? here * 4u : 0u);
 #pragma unroll
         for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[i][e] = X == Q4_I8 ? buf_ld4(r, (16 * i + 4 * (l >> 4) + e) * 4) : 1.f;
+            for (int e = 0; e < 4; ++e) v[i][e] = X == Q4_I8 ? buf_ld4(r, (16 * i + 4 * (l >> 4) + e) * 4) * by : 1.f;
     }
 };
 
@@ -356,7 +355,7 @@ __global__ __launch_bounds__(64 * (RT > 1 ? 8 : kQ4Waves)) void q4_held(Q4P p) {
                 for (int e = 0; e < Q4Op<X>::kParts; ++e) asm volatile("" : "+v"(x[k][i][st].v[e]));
             }
     const Q4Bias bias(p);
-    Q4Scales<X, RT> xs(p, m0, l);
+    Q4Scales<X, RT> xs(p, m0, l, S == Q4_S16 ? 0.0625f : 1.f);
     if constexpr (X == Q4_I8) {
 #pragma unroll
         for (int i = 0; i < RT; ++i)
@@ -444,7 +443,7 @@ __global__ __launch_bounds__(512) void q4_walk(Q4P p) {
         for (int c = 0; c < C; ++c) q4_red[((w * RT + i) * C + c) * 64 + l] = tot[c][i];
     __syncthreads();
     const Q4Bias bias(p);
-    const Q4Scales<X, RT> xs(p, m0, l);
+    const Q4Scales<X, RT> xs(p, m0, l, S == Q4_S16 ? 0.0625f : 1.f);
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -490,12 +489,12 @@ static void q4_walk_launch(const Q4P& p, hipStream_t s) {
 }
 // The rows in registers wherever twelve waves hold them (60 blocks of k, f32 24), as four, eight or
 // twelve waves, which load the four SIMDs evenly; else the walk.  us held / walked, bf16 at 2560 x 10240:
-// 32 rows 12.5 / 19.9, 64 rows 15.8 / 26.7, 256 rows 41 / 78; int8 64 rows 14.6 / 23.4, at 5120 x
-// 2560 11.1 / 14.7; f32 one row 9.1 / 27.
+// 32 rows 12.4 / 19.9, 64 rows 15.6 / 26.7, 256 rows 41 / 78; int8 64 rows 14.4 / 23.4, at 5120 x
+// 2560 11.0 / 14.7; f32 one row 9.1 / 27.
 // Two row tiles a wave take apart a block once for both, but start with twice the rows to load: where
 // a workgroup has ten tiles or more to go through.  us with one / two at 2560 x 10240: bf16 64 rows
-// (5 tiles) 15.8 / 18.7, 128 rows (10) 24.6 / 23.4, 256 rows (20) 41.0 / 35.0, int8 35.2 / 30.4; bf16
-// 64 rows at 2560 x 50001 (24) 50.3 / 42.6.
+// (5 tiles) 15.8 / 18.7, 128 rows (10) 24.6 / 23.3, 256 rows (20) 41.0 / 34.4, int8 35.2 / 29.5; bf16
+// 64 rows at 2560 x 50001 (24) 50.3 / 42.4.
 template <int X, int GB>
 static void q4_shape(const Q4P& p, hipStream_t s) {
     constexpr int most = X == Q4_F32 ? 2 : 5;  // blocks of k whose operands a wave's registers hold

@@ -11,11 +11,14 @@
 // by 2e-3 of itself, from the sum by 1e-7.
 //
 // Some ten operations an element against three or four elements moved: HBM-bound.  Rows of up to
-// 10240 bf16 or 5120 f32 stream elements stay in registers, so that each element is read
-// once: G lanes hold a row, E = 16 bytes of the stream a lane and step, G = 16, 64 or 256 by the
-// row's width; the next row's loads are in flight while this one is summed.  The backward's
+// 16384 bf16 or 8192 f32 stream elements stay in registers, so that each element is read
+// once: G lanes hold a row, E = 16 bytes of the stream a lane and step, G = 16, 64, 256 or 512 by
+// the row's width; the next row's loads are in flight while this one is summed.  The backward's
 // workgroups take rows in turn and sum dw of their columns in registers, joined in LDS
-// and, over the workgroups, by arn_dw_join, in a fixed order.
+// and, over the workgroups, by arn_dw_join, in a fixed order.  16384 x 2560, bf16 rows with an f32
+// stream: forward 97 us (5.2 TB/s), backward with the join 126 (5.3), to int8 94 (4.9): what a copy
+// reaches.  4096 x 16384 of bf16 in registers / by the wide kernels below: forward 104 / 173, backward
+// 126 / 312, int8 107 / 212.
 #include <algorithm>
 
 #include "pack.h"
@@ -77,8 +80,8 @@ __device__ __forceinline__ uint8_t arn_q8(float v, ArnScale s, bool e4m3) {
 }
 
 // ---- rows in registers
-// Sum, or largest, over aligned groups of G lanes in every lane; over the workgroup for G = 256
-// (red: 4 places, which no wave may still read from a sum before the last barrier: the callers
+// Sum, or largest, over aligned groups of G lanes in every lane; over the workgroup for G = 256 and
+// 512 (red: 8 places, which no wave may still read from a sum before the last barrier: the callers
 // alternate between two sets).
 template <int CTRL>
 __device__ __forceinline__ uint32_t arn_dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true); }
@@ -98,16 +101,18 @@ __device__ __forceinline__ uint32_t arn_all(uint32_t v, uint32_t* red, Op op) {
         const uint32_t a = op((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
         v = op(a, op((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
     }
-    if constexpr (G == 256) {
+    if constexpr (G >= 256) {
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         v = op(op(red[0], red[1]), op(red[2], red[3]));
+        if constexpr (G == 512) v = op(v, op(op(red[4], red[5]), op(red[6], red[7])));
     }
     return v;
 }
 template <int G>
 __device__ __forceinline__ float arn_sum(float v, uint32_t* red) { return __uint_as_float(arn_all<G>(__float_as_uint(v), red, ArnAdd())); }
 
+constexpr int arn_block(int G) { return G > 256 ? G : 256; }
 // elements of a lane and step: 16 bytes of the stream
 template <typename S>
 constexpr int kArnE = 16 / (int)sizeof(S);
@@ -146,9 +151,9 @@ __device__ __forceinline__ void arn_put8(uint8_t* q, int n, const float (&v)[E],
 // G lanes a row, V steps: G (V - 1) E < cols <= G V E, so that only the last step can pass the row's
 // end.  Q: rows of 8 bits.
 template <typename T, typename S, int G, int V, bool Q>
-__global__ __launch_bounds__(256) void arn_fwd_rows(ArnP p) {
-    constexpr int E = kArnE<S>, RB = 256 / G;
-    __shared__ uint32_t red[16];
+__global__ __launch_bounds__(arn_block(G)) void arn_fwd_rows(ArnP p) {
+    constexpr int E = kArnE<S>, RB = arn_block(G) / G;
+    __shared__ uint32_t red[32];
     const int l = threadIdx.x % G, sub = threadIdx.x / G;
     Elems<T, E> rx[V];
     Elems<S, E> rr[V];
@@ -181,7 +186,7 @@ __global__ __launch_bounds__(256) void arn_fwd_rows(ArnP p) {
     const float inv = 1.f / (float)p.cols;
     const int64_t step = (int64_t)gridDim.x * RB;
     int odd = 0;
-    // every group of a workgroup makes the same number of turns (the sums of G = 256 meet at a barrier)
+    // every group of a workgroup makes the same number of turns (the sums of G >= 256 meet at a barrier)
     for (int64_t r0 = blockIdx.x * (int64_t)RB; r0 < p.rows; r0 += step) {
         const int64_t r = r0 + sub;
         float v[V][E], ss = 0.f;
@@ -208,7 +213,7 @@ __global__ __launch_bounds__(256) void arn_fwd_rows(ArnP p) {
         for (int k = 0; k < V; ++k)
 #pragma unroll
             for (int i = 0; i < E; ++i) ss = __builtin_fmaf(v[k][i], v[k][i], ss);  // zeros past the row's end
-        const float rstd = 1.f / sqrtf(__builtin_fmaf(arn_sum<G>(ss, red + 8 * odd), inv, p.eps));
+        const float rstd = 1.f / sqrtf(__builtin_fmaf(arn_sum<G>(ss, red + 16 * odd), inv, p.eps));
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
@@ -221,7 +226,7 @@ __global__ __launch_bounds__(256) void arn_fwd_rows(ArnP p) {
 #pragma unroll
                 for (int i = 0; i < E; ++i)
                     if (k < V - 1 || (k * G + l) * E + i < p.cols) amax = max(amax, __float_as_uint(v[k][i]) & 0x7fffffffu);
-            sc = arn_scale(arn_all<G>(amax, red + 8 * odd + 4, ArnMax()), p.e4m3);
+            sc = arn_scale(arn_all<G>(amax, red + 16 * odd + 8, ArnMax()), p.e4m3);
         }
         odd ^= 1;
         if (r >= p.rows) continue;
@@ -242,9 +247,9 @@ __global__ __launch_bounds__(256) void arn_fwd_rows(ArnP p) {
 // The workgroups take their rows in turn; part[blockIdx.x] gets the workgroup's dw.  SUM: s + x in
 // the place of s.
 template <typename T, typename S, int G, int V, bool SUM>
-__global__ __launch_bounds__(256) void arn_bwd_rows(ArnP p) {
-    constexpr int E = kArnE<S>, RB = 256 / G;
-    __shared__ uint32_t red[8];
+__global__ __launch_bounds__(arn_block(G)) void arn_bwd_rows(ArnP p) {
+    constexpr int E = kArnE<S>, RB = arn_block(G) / G;
+    __shared__ uint32_t red[16];
     __shared__ float s_w[G < 256 ? G * V * E : 1];  // after the rows, the groups' sums
     const int l = threadIdx.x % G, sub = threadIdx.x / G;
     Elems<S, E> rs[V], rd[V];
@@ -316,7 +321,7 @@ __global__ __launch_bounds__(256) void arn_bwd_rows(ArnP p) {
                     dot = __builtin_fmaf(g[k][i], xh[k][i], dot);
                 }
         }
-        dot = arn_sum<G>(dot, red + 4 * odd) * inv;
+        dot = arn_sum<G>(dot, red + 8 * odd) * inv;
         odd ^= 1;
         if (!live) continue;
 #pragma unroll
@@ -355,7 +360,8 @@ __global__ __launch_bounds__(256) void arn_bwd_rows(ArnP p) {
     }
 }
 
-// Any width: a workgroup per row, the row read once per sweep.
+// Any width: a workgroup per row, the row read once per sweep (two forward, three to 8 bits; two and
+// one more for dw backward): 2048 x 20000, bf16 with an f32 stream: 169 us, 209 and 257.
 template <typename T, typename S>
 __global__ __launch_bounds__(256) void arn_fwd_wide(ArnP p) {
     constexpr int E = 4, ST = 256 * E;
@@ -528,16 +534,20 @@ static uint32_t arn_grid(int64_t rows) { return (uint32_t)std::min<int64_t>(rows
 static int arn_steps(int cols, int E, int G) { return ceil_div(cols, G * E); }
 // Lanes a row, 0: the row is not held in registers.
 static int arn_lanes(int cols, int E) {
-    return arn_steps(cols, E, 16) <= 2 ? 16 : arn_steps(cols, E, 64) <= 3 ? 64 : arn_steps(cols, E, 256) <= 5 ? 256 : 0;
+    return arn_steps(cols, E, 16) <= 2 ? 16 : arn_steps(cols, E, 64) <= 3 ? 64 : arn_steps(cols, E, 256) <= 5 ? 256 : arn_steps(cols, E, 512) <= 4 ? 512 : 0;
 }
-static uint32_t arn_fwd_grid(int64_t rows, int G) { return (uint32_t)std::min<int64_t>((rows + 256 / G - 1) / (256 / G), 2048); }
+static uint32_t arn_fwd_grid(int64_t rows, int G) {
+    const int rb = arn_block(G) / G;
+    return (uint32_t)std::min<int64_t>((rows + rb - 1) / rb, 2048);
+}
 // Workgroups of the backward: two a CU, and some eight rows a group at least, so that the parts
 // stay few beside the rows.  us at 512 / 1024 with the join: 16384 x 2560 with an f32 stream 127 /
 // 139, bf16 82 / 91, 65536 x 256 57 / 56.
 static int arn_parts(int64_t rows, int cols, int E) {
     const int G = arn_lanes(cols, E);
     if (G == 0) return (int)std::min<int64_t>(256, (rows + 31) / 32);
-    return (int)std::min<int64_t>(512, (rows + 8 * (256 / G) - 1) / (8 * (256 / G)));
+    const int rb = arn_block(G) / G;
+    return (int)std::min<int64_t>(512, (rows + 8 * rb - 1) / (8 * rb));
 }
 
 template <typename T, typename S, int G, int V>
@@ -545,13 +555,13 @@ static void arn_rows_launch(const ArnP& p, bool back, hipStream_t s) {
     if (back) {
         if constexpr (sizeof(S) == 2) {
             if (p.x) {
-                hipLaunchKernelGGL((arn_bwd_rows<T, S, G, V, true>), dim3(p.parts), dim3(256), 0, s, p);
+                hipLaunchKernelGGL((arn_bwd_rows<T, S, G, V, true>), dim3(p.parts), dim3(arn_block(G)), 0, s, p);
                 return;
             }
         }
-        hipLaunchKernelGGL((arn_bwd_rows<T, S, G, V, false>), dim3(p.parts), dim3(256), 0, s, p);
-    } else if (p.q) hipLaunchKernelGGL((arn_fwd_rows<T, S, G, V, true>), dim3(arn_fwd_grid(p.rows, G)), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((arn_fwd_rows<T, S, G, V, false>), dim3(arn_fwd_grid(p.rows, G)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((arn_bwd_rows<T, S, G, V, false>), dim3(p.parts), dim3(arn_block(G)), 0, s, p);
+    } else if (p.q) hipLaunchKernelGGL((arn_fwd_rows<T, S, G, V, true>), dim3(arn_fwd_grid(p.rows, G)), dim3(arn_block(G)), 0, s, p);
+    else hipLaunchKernelGGL((arn_fwd_rows<T, S, G, V, false>), dim3(arn_fwd_grid(p.rows, G)), dim3(arn_block(G)), 0, s, p);
 }
 // rows in registers; false where they are too wide
 template <typename T, typename S>
@@ -568,7 +578,9 @@ static bool arn_rows(const ArnP& p, bool back, hipStream_t s) {
         case 256 * 8 + 2: arn_rows_launch<T, S, 256, 2>(p, back, s); break;
         case 256 * 8 + 3: arn_rows_launch<T, S, 256, 3>(p, back, s); break;
         case 256 * 8 + 4: arn_rows_launch<T, S, 256, 4>(p, back, s); break;
-        default: arn_rows_launch<T, S, 256, 5>(p, back, s);
+        case 256 * 8 + 5: arn_rows_launch<T, S, 256, 5>(p, back, s); break;
+        case 512 * 8 + 3: arn_rows_launch<T, S, 512, 3>(p, back, s); break;
+        default: arn_rows_launch<T, S, 512, 4>(p, back, s);
     }
     return true;
 }

@@ -36,7 +36,7 @@ def roundings(cols):
     return 30 + cols / 256
 
 
-SIZES = [(1, 1), (3, 7), (5, 100), (33, 256), (2, 513), (70, 769), (9, 1000), (40, 2560), (3, 5120), (5, 7001), (2, 20000)]
+SIZES = [(1, 1), (3, 7), (5, 100), (33, 256), (2, 513), (70, 769), (9, 1000), (40, 2560), (3, 5120), (5, 7001), (2, 20000), (3, 5121), (4, 8192), (9, 10241), (2, 16384), (1, 16385)]
 
 
 @pytest.mark.parametrize("io,stream", TYPES)

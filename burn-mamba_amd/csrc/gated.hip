@@ -169,7 +169,11 @@ __device__ __forceinline__ GRows g_rows(const Seqs& q, int t0, int R) {
         return o;
     }
     const int j = threadIdx.x & 63, t = t0 + j;
-    hi = q.n;
+    hi = lo;
+    for (uint32_t w = 1; hi < q.n && q.cu[hi + 1] <= t; w *= 2) {  // seldom far from the first row's
+        lo = hi + 1;
+        hi += (int)min(w, (uint32_t)(q.n - hi));
+    }
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (q.cu[mid + 1] > t) hi = mid;

@@ -24,6 +24,7 @@ LENS = {
     "tokens": [1] * 70,
     "groups": [2500, 1, 0, 3900, 200],  # tiles' groups crossed within a sequence, several times
     "far": [9000],
+    "crowd": [3] * 20 + [0] * 500 + [1, 0] * 100 + [40] + [0] * 1000 + [2, 90],  # many in a tile, and long runs of empty ones
 }
 
 
@@ -64,7 +65,8 @@ def roundings(lens, t):
 CASES = [("one", 1, F32, 0, True), ("short", 5, BF16, 2, False), ("mixed", 70, F32, 3, True), ("mixed", 64, BF16, 0, True),
          ("borders", 37, F32, 0, True), ("borders", 129, BF16, 70, False), ("long", 65, BF16, 1, False), ("tokens", 40, F32, 0, True),
          ("mixed", 130, BF16, 3, True), ("mixed", 257, F32, 0, False), ("groups", 6, F32, 5, True), ("groups", 9, BF16, 0, False),
-         ("far", 3, BF16, 0, True), ("none", 4, F32, 3, True), ("empties", 4, BF16, 3, True)]
+         ("far", 3, BF16, 0, True), ("none", 4, F32, 3, True), ("empties", 4, BF16, 3, True), ("crowd", 65, F32, 2, True),
+         ("crowd", 9, BF16, 0, False)]
 
 
 @pytest.mark.parametrize("name,d,dtype,pad,z", CASES)
@@ -353,6 +355,21 @@ def test_captured_and_replayed(dev):
         for a, b in zip(grads, want):
             assert torch.equal(a, b), rep
     assert torch.equal(state, eager_state)
+
+
+def test_rows_that_are_one(dev):
+    """A row that all tokens share (stride 0) is read as its copies are; so is every second row."""
+    lens, d = LENS["mixed"], 70
+    t = inputs(lens, d, F32, dev, seed=31)
+    n, c = sum(lens), cu(lens, dev)
+    one = {**t, "r": t["r"][:1].expand(n, d), "i": torch.randn(2 * n, d, generator=gen(32)).to(dev)[::2]}
+    copies = {k: v.clone(memory_format=torch.contiguous_format) for k, v in one.items()}
+    carry, carry2 = (torch.zeros(-(-n // 64), d, device=dev) for _ in range(2))
+    assert torch.equal(mamba_hip.gated_scan_packed(**one, cu_seqlens=c, carry=carry), mamba_hip.gated_scan_packed(**copies, cu_seqlens=c, carry=carry2))
+    dy = torch.randn(1, d, generator=gen(33)).to(dev).expand(n, d)
+    a = mamba_hip.gated_scan_packed_bwd(dy, **one, cu_seqlens=c, carry=carry)
+    b = mamba_hip.gated_scan_packed_bwd(dy.contiguous(), **copies, cu_seqlens=c, carry=carry2)
+    assert all(torch.equal(a[k], b[k]) for k in ("dx", "dr", "di", "dz", "dA"))
 
 
 def test_two_streams_at_once(dev):

@@ -53,24 +53,35 @@ static bool q4_make(const mamba_q4_weight* w, Q4W* o, size_t* bytes) {
     return true;
 }
 
-__global__ __launch_bounds__(256) void q4_pack(Q4W w, const uint8_t* codes, const void* scale, const uint8_t* zero, uint32_t* out, void* oscale) {
+// A thread forms what four lanes of a block hold (run q of 8 k in each 32, four columns): a dword of
+// codes a row, 16 bytes out a lane.  2560 x 50001 (196 MB) 47 us with its scales.
+__global__ __launch_bounds__(256) void q4_pack(Q4W w, const uint8_t* codes, const void* scale, const uint8_t* zero, uint4* out, void* oscale) {
     const int64_t step = (int64_t)gridDim.x * 256, at0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    // column-major in the threads, so that neighbours read neighbouring codes
-    for (int64_t i = at0; i < (int64_t)w.NT * w.KB * 256; i += step) {
-        const int col = (int)(i % 16);
-        int64_t t = i / 16;
-        const int j = (int)(t % w.NT);
-        t /= w.NT;
-        const int k8 = (int)(t % 16);  // the run of 8 k inside the block
-        const int64_t kb = t / 16;
-        const int n = j * kQ4N + col;
-        uint32_t v = 0;
-        for (int e = 0; e < 8; ++e) {
-            const int64_t k = kb * kQ4K + k8 * 8 + e;
-            const uint32_t c = k < w.K && n < w.N ? codes[k * w.N + n] & 15u : 0u;
-            v |= c << (4 * (e / 2 + 4 * (e & 1)));
-        }
-        out[((j * (int64_t)w.KB + kb) * 64 + (k8 & 3) * 16 + col) * 4 + k8 / 4] = v;
+    const int n4 = w.NT * (kQ4N / 4);
+    for (int64_t i = at0; i < (int64_t)w.KB * 4 * n4; i += step) {
+        const int n = (int)(i % n4) * 4, q = (int)(i / n4 & 3), here = w.N - n;
+        const int64_t kb = i / n4 / 4;
+        uint32_t v[4][4] = {};  // [column][dword]
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int64_t k = kb * kQ4K + 32 * st + 8 * q + e;
+                uint32_t c = 0;
+                if (k < w.K) {
+                    const uint8_t* at = codes + k * w.N + n;
+                    if (here >= 4) {
+                        __builtin_memcpy(&c, at, 4);
+                    } else {
+                        for (int m = 0; m < here; ++m) c |= (uint32_t)at[m] << (8 * m);
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < 4; ++m) v[m][st] |= (c >> (8 * m) & 15u) << (4 * (e / 2 + 4 * (e & 1)));
+            }
+        uint4* to = out + (((int64_t)(n / kQ4N) * w.KB + kb) * 64 + q * 16 + n % kQ4N);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) to[m] = make_uint4(v[m][0], v[m][1], v[m][2], v[m][3]);
     }
     const int groups = (w.K + w.G - 1) / w.G;
     for (int64_t i = at0; i < (int64_t)w.NT * w.NG * kQ4N; i += step) {
@@ -556,9 +567,9 @@ extern "C" int mamba_linear_q4_pack(const mamba_q4_weight* w, const void* codes,
     MAMBA_CHECK_ARG(q4_make(&at, &q, &bytes), Q4_SHAPE);
     MAMBA_CHECK_ARG(codes && scale && packed && (zero || !q.zeros), "codes, scale, packed and, with has_zero, zero are required");
     MAMBA_CHECK_ARG(((uintptr_t)packed & 15u) == 0, "packed must be 16-byte aligned");
-    const int64_t items = (int64_t)q.NT * q.KB * 256;
+    const int64_t items = (int64_t)q.NT * q.KB * 16;
     hipLaunchKernelGGL(q4_pack, dim3((uint32_t)std::min<int64_t>((items + 255) / 256, 1 << 16)), dim3(256), 0, (hipStream_t)stream, q, (const uint8_t*)codes,
-                       scale, (const uint8_t*)zero, (uint32_t*)packed, const_cast<void*>(q.scale));
+                       scale, (const uint8_t*)zero, (uint4*)packed, const_cast<void*>(q.scale));
     MAMBA_CHECK_LAUNCH();
     return MAMBA_OK;
 }

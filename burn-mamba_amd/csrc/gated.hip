@@ -135,12 +135,11 @@ __device__ __forceinline__ void g_decays(float (&a)[R], float (&q)[R]) {
     }
 }
 
-// What the R rows from t0 are (R <= 64, t0 uniform over the wave): bit j of a mask for row
+// What the R rows from t0 are (R < 64, t0 uniform over the wave): bit j of a mask for row
 // t0 + j, whether it is in a sequence, its first, its last; lane j holds the row's sequence and
 // that one's first row and end.  The offsets are clamped: a wrong one gives a wrong result and
 // no access out of range.  They are searched with scalar loads, which do not queue behind the rows
-// in flight, and each lane looks for its own row only where the rows are not all of one sequence
-// (lanes that searched cost 8192 x 5120 a tenth).
+// in flight (lanes that searched cost 8192 x 5120 a tenth).
 struct GRows {
     uint64_t live, first, last;
     int s, b, e;
@@ -148,48 +147,44 @@ struct GRows {
 __device__ __forceinline__ int g_offset(const Seqs& q, int s) {  // cu[s], s uniform
     return min(max(((const __attribute__((address_space(4))) int32_t*)q.cu)[s], 0), q.rows);
 }
-__device__ __forceinline__ GRows g_rows(const Seqs& q, int t0, int R) {
-    GRows o;
-    int lo = 0, hi = q.n;
-    while (lo < hi) {  // the first sequence that ends behind row t0
-        const int mid = (lo + hi) >> 1;
-        if (g_offset(q, mid + 1) > t0) hi = mid;
-        else lo = mid + 1;
-    }
-    o.s = lo;
-    o.b = o.e = 0;
-    if (lo < q.n) {
-        o.b = g_offset(q, lo);
-        o.e = max(g_offset(q, lo + 1), o.b);
-    }
-    if (t0 >= o.b && t0 + R <= o.e) {
-        o.live = (1ull << R) - 1;
-        o.first = t0 == o.b;
-        o.last = t0 + R == o.e ? 1ull << (R - 1) : 0;
-        return o;
-    }
-    const int j = threadIdx.x & 63, t = t0 + j;
-    hi = lo;
-    for (uint32_t w = 1; hi < q.n && q.cu[hi + 1] <= t; w *= 2) {  // seldom far from the first row's
-        lo = hi + 1;
-        hi += (int)min(w, (uint32_t)(q.n - hi));
-    }
+// The first sequence from lo on that ends behind row t.
+__device__ __forceinline__ int g_search(const Seqs& q, int lo, int t) {
+    int hi = q.n;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (q.cu[mid + 1] > t) hi = mid;
+        if (g_offset(q, mid + 1) > t) hi = mid;
         else lo = mid + 1;
     }
-    o.s = lo;
-    o.b = o.e = 0;
-    const bool in = j < R && t < q.rows && lo < q.n;
-    if (in) {
-        o.b = min(max(q.cu[lo], 0), q.rows);
-        o.e = min(max(q.cu[lo + 1], o.b), q.rows);
+    return lo;
+}
+__device__ __forceinline__ GRows g_rows(const Seqs& q, int t0, int R) {
+    const int j = threadIdx.x & 63;
+    GRows o{0, 0, 0, 0, 0, 0};
+    int t = t0, s = g_search(q, 0, t0);
+    if (s >= q.n) return o;
+    int b = g_offset(q, s), e = g_offset(q, s + 1);
+    while (true) {  // sequence s, b .. e, ends behind t, which grows
+        const int j0 = max(b, t) - t0, j1 = min(e - t0, R);
+        if (j0 < j1) {
+            o.live |= (1ull << j1) - (1ull << j0);
+            if (b >= t0) o.first |= 1ull << j0;
+            if (e - t0 <= R) o.last |= 1ull << (j1 - 1);
+            const bool here = j >= j0 && j < j1;
+            o.s = here ? s : o.s;
+            o.b = here ? b : o.b;
+            o.e = here ? e : o.e;
+        }
+        t = e;
+        if (t >= t0 + R || ++s >= q.n) break;
+        b = e;
+        e = g_offset(q, s + 1);
+        if (e <= t) {  // an empty one, or many
+            s = g_search(q, s + 1, t);
+            if (s >= q.n) break;
+            b = g_offset(q, s);
+            e = g_offset(q, s + 1);
+        }
     }
-    const bool live = in && t >= o.b && t < o.e;
-    o.live = __ballot(live);
-    o.first = __ballot(live && t == o.b);
-    o.last = __ballot(live && t == o.e - 1);
     return o;
 }
 __device__ __forceinline__ int g_lane(int v, int j) { return __builtin_amdgcn_readlane(v, j); }

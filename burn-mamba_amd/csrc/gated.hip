@@ -349,6 +349,8 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
     uint32_t ez[Z ? R : 1];
     float a[R], b[R];
     GRows g;
+    int j0;    // the first row here that begins a sequence, and
+    float h0;  // what that one starts from, on its way with the rows
     {
         uint32_t ex[R], er[R], ei[R];
         const float A = c < p.D ? p.A[c] : 0.f;  // first: loads come back in order
@@ -356,6 +358,9 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
         g_fetch<T, R>(ei, p, p.i, p.i_st, t0, col);
         g_fetch<T, R>(ex, p, p.x, p.x_st, t0, col);
         g = g_rows(p.q, t0, R);
+        j0 = g.first ? __builtin_ctzll(g.first) : 0;
+        const int64_t slot = p.state && g.first ? slot_of(p.slots, g_lane(g.s, j0), p.nslots) : -1;
+        h0 = buf_ld4(buf_rsrc(p.state + max(slot, (int64_t)0) * p.D, slot >= 0 ? p.D * 4u : 0u), c * 4u);
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             a[j] = A * g_sigmoid(g_value<T>(er[j]));
@@ -381,8 +386,10 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
 #pragma unroll
         for (int j = 0; j < R; ++j) {
             if (g_bit(g.first, j)) {  // from the sequence's state on; b holds the new one
-                const int64_t slot = p.state ? slot_of(p.slots, g_lane(g.s, j), p.nslots) : -1;
-                const float h0 = slot >= 0 && c < p.D ? p.state[slot * p.D + c] : 0.f;
+                if (j != j0) {
+                    const int64_t slot = p.state ? slot_of(p.slots, g_lane(g.s, j), p.nslots) : -1;
+                    h0 = slot >= 0 && c < p.D ? p.state[slot * p.D + c] : 0.f;
+                }
                 m.H = b[j] = __builtin_fmaf(a[j], h0, b[j]);
             } else if (g_bit(g.live, j)) {
                 m.H = __builtin_fmaf(a[j], m.H, b[j]);

@@ -332,8 +332,8 @@ __device__ __forceinline__ void g_fetch(uint32_t (&e)[R], const GatedP& p, const
     for (int j = 0; j < R; ++j) e[j] = row.load(min(j, k), col);
 }
 
-// 8192 x 5120: bf16 with z 106 us (420 MB, 4.0 TB/s), f32 without 132 (671 MB, 5.1: what a copy
-// reaches).  bf16: half the time is issue of vector instructions (46 a row, 7 of them at a quarter
+// 8192 x 5120: bf16 with z 104 us (420 MB, 4.0 TB/s), f32 without 131 (671 MB, 5.1: what a copy
+// reaches).  bf16: half the time is issue of vector instructions (44 a row, 7 of them at a quarter
 // of the rate), the rest a tile's latencies (ticket, rows, the states that enter), which two
 // workgroups a CU hide in part; three (80 registers) spill and take 1.2 times as long.
 template <typename T, bool Z>
@@ -450,8 +450,8 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
 // What a row's gradients need is formed once, where its values are read: with u = s(i) x,
 //   gr = dy silu(z), zk = dy silu'(z), pull = u a^2 / m, kr = A s(r) s(-r), ui = u s(-i)
 // so that dz = h zk, dx = dh m s(i), di = dh m ui, dr = e kr, e = dh (a h_{t-1} - pull).
-// 8192 x 5120: bf16 with z 207 us with the join (755 MB, 3.6 TB/s), f32 without 236 (1174 MB, 5.0).
-// Bound as the forward is: some 95 vector instructions a row.
+// 8192 x 5120: bf16 with z 202 us with the join (755 MB, 3.7 TB/s), f32 without 236 (1174 MB, 5.0).
+// Bound as the forward is: some 90 vector instructions a row.
 template <typename T, bool Z>
 __global__ __launch_bounds__(64 * kGW, 4) void gated_bwd(GatedP p) {
     constexpr int R = kGRows;

@@ -273,7 +273,8 @@ class _AddRmsNorm(torch.autograd.Function):
 
 
 def add_rms_norm_autograd(x, weight, residual=None, eps: float = 1e-5) -> tuple:
-    """``add_rms_norm`` as a differentiable op: (y, s), with gradients of x, weight and residual."""
+    """``add_rms_norm`` as a differentiable op: (y, s), with gradients of x, weight and residual.
+    The backward keeps s, or x and a bf16 residual, whose sum it forms again."""
     if residual is None:
         return _AddRmsNorm.apply(x, weight, None, eps), x
     return _AddRmsNorm.apply(x, weight, residual, eps)

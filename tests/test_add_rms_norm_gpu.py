@@ -127,6 +127,33 @@ def test_backward_of_the_sum_as_it_is(dev, rows, cols):
         go.close(got["dweight"], *ref["dweight"], 8 + rows + roundings(cols), "dweight")
 
 
+@pytest.mark.parametrize("io,stream", TYPES[:3])
+def test_gradients_of_leaves_are_their_own(dev, io, stream):
+    """x and residual have equal gradients of one type: no leaf's is another's memory, also where
+    the same tensor is both, and a second pass adds to each."""
+    x, w, res = make(dev, 20, 96, io, stream, 16)
+    x, w, res = (t.contiguous().requires_grad_() for t in (x, w, res))
+    for rep in (1, 2):
+        y, s = mamba_hip.add_rms_norm_autograd(x, w, res)
+        (y.float().sum() + 2 * s.float().sum()).backward()
+        if rep == 1:
+            first = [t.grad.clone() for t in (x, w, res)]
+    assert x.grad.data_ptr() != res.grad.data_ptr()
+    for t, g in zip((x, w, res), first):
+        assert torch.equal(t.grad, 2 * g)
+    x.grad.zero_()
+    assert torch.equal(res.grad, 2 * first[2])
+    if io == stream:
+        both = res.detach().clone().requires_grad_()
+        y, s = mamba_hip.add_rms_norm_autograd(both, w, both)
+        (one,) = torch.autograd.grad((y, s), both, (torch.ones_like(y), torch.ones_like(s)))
+        s0, rstd, _ = go.add_rms(both, w, both, 1e-5)
+        ref, mag = go.add_rms_bwd(torch.ones_like(y), s0, w, rstd[:, 0], torch.ones_like(s))["d"]
+        # twice the gradient, which each of the two has rounded to its type
+        eps = torch.finfo(io).eps
+        assert bool(((f64(one) - 2 * ref).abs() <= 2 * eps * ref.abs() + 8 * roundings(96) * 2.0 ** -23 * mag).all())
+
+
 def test_gradient_by_differences(dev):
     rows, cols = 5, 40
     x, w, res = make(dev, rows, cols, F32, F32, 5)

@@ -19,7 +19,7 @@
 // twice the registers and leave the backward one workgroup a CU, which took half as long again); the maps of the eight waves are joined in LDS to the tile's, which is published to the
 // other workgroups before the tile's own state is waited for.  That state is joined from the
 // published maps of the tiles before it, back to the one in which the tile's first sequence
-// begins, or to the last group of 16 tiles, whose final state its last tile publishes.  The
+// begins, or to the last group of 16 or 64 tiles, whose final state its last tile publishes.  The
 // joins follow a fixed order: the same inputs give the same bits.  The backward walks the other way
 // with q in the state's place, and finds h again from the states that the forward kept.
 //
@@ -56,16 +56,21 @@ struct GatedP {
     void* dz; int64_t dz_st;
     float* dA; float* dh0;
     // tiles of rows and of channels; the workspace
-    int ntile, nct;
+    int ntile, nct, group;              // group: log2 of the tiles of a group
     uint32_t* ticket;                   // [nct], kGTicket words apart
     uint64_t* map;                      // [ntile][nct kGC] published maps
-    uint64_t* ends;                     // [ntile / kGGroup][nct kGC] states at the ends of groups
+    uint64_t* ends;                     // [ntile >> group][nct kGC] states at the ends of groups
     float* part;                        // [ntile][D] partial sums of dA
 };
 
 constexpr int kCarryRows = 64;  // rows between the states that the forward keeps for the backward
 constexpr int kGW = 8, kGC = 64;  // waves of a workgroup; channels of a tile: one a lane
-constexpr int kGGroup = 16;                      // tiles of a group
+// Log2 of the tiles of a group.  The ends of groups are found one behind the other: with many of them
+// in flight that chain is the longer wait, with few the maps of a group are (64 / 16 tiles: 262144 x
+// 256 of bf16 forward 165 / 183 us, backward 336 / 373; 65536 x 512 backward 180 / 176, 8192 x 5120
+// 214 / 205).
+constexpr int kGGroup = 4, kGGroupLong = 6;
+constexpr int kGLong = 2048;                     // tiles of rows from which on groups are long
 constexpr uint64_t kGNone = ~0ull;               // nothing published yet
 constexpr int kGTicket = 32;                     // words between the tickets of two column tiles
 // Rows of a lane.  What a tile costs beside its rows is the same for 8 of them: with 8 the forward
@@ -268,25 +273,26 @@ __device__ __forceinline__ GMap g_publish_map(const GatedP& p, const GShared& s,
     return m;
 }
 __device__ __forceinline__ void g_publish_end(const GatedP& p, int o, int ct, int l, const GMap& m, bool cut, float h) {
-    if ((o + 1) % kGGroup == 0 && o + 1 < p.ntile)
-        g_publish(p.ends + g_at(p, o / kGGroup, ct, l), g_word(0.f, cut ? m.H : __builtin_fmaf(m.P, h, m.H)));
+    if (((o + 1) & ((1 << p.group) - 1)) == 0 && o + 1 < p.ntile)
+        g_publish(p.ends + g_at(p, o >> p.group, ct, l), g_word(0.f, cut ? m.H : __builtin_fmaf(m.P, h, m.H)));
 }
 
 // The state that enters tile o: joined from the maps of tiles far .. o - 1, tile `far` being cut, or
 // from the end of the group before o's.  Called by the whole workgroup (o > far >= 0).
 __device__ __forceinline__ float g_enter(const GatedP& p, GShared& s, int o, int ct, int far) {
     const int w = wave_id(), l = threadIdx.x & 63;
-    const int base = o / kGGroup * kGGroup, from = max(far, base);
+    const int base = o >> p.group << p.group, from = max(far, base);
     const bool group = far < base;
     const int per = (o - from + kGW - 1) / kGW, k0 = min(o, from + w * per), k1 = min(o, k0 + per);
     GMap m;
-    uint64_t word[kGGroup / kGW], end = 0;
+    constexpr int most = (1 << kGGroupLong) / kGW;  // maps of a wave
+    uint64_t word[most], end = 0;
 #pragma unroll
-    for (int i = 0; i < kGGroup / kGW; ++i) word[i] = k0 + i < k1 ? g_peek(p.map + g_at(p, k0 + i, ct, l)) : 0;
-    const uint64_t* ends = p.ends + g_at(p, base / kGGroup - 1, ct, l);
+    for (int i = 0; i < most; ++i) word[i] = k0 + i < k1 ? g_peek(p.map + g_at(p, k0 + i, ct, l)) : 0;
+    const uint64_t* ends = p.ends + g_at(p, (base >> p.group) - 1, ct, l);
     if (group && w == 0) end = g_peek(ends);
 #pragma unroll
-    for (int i = 0; i < kGGroup / kGW; ++i) {
+    for (int i = 0; i < most; ++i) {
         if (k0 + i >= k1) break;
         const uint64_t x = g_wait(p.map + g_at(p, k0 + i, ct, l), word[i]);
         const float P = __uint_as_float((uint32_t)x), H = __uint_as_float((uint32_t)(x >> 32));
@@ -692,7 +698,8 @@ static size_t gated_plan(GatedP& p, bool back, void* ws) {
     const int tile = kGW * (back ? kGRows : kGFwdRows);
     p.ntile = (int)((p.rows + tile - 1) / tile);
     p.nct = ceil_div(p.D, kGC);
-    const int64_t Dp = (int64_t)p.nct * kGC, words = p.ntile > 1 ? (p.ntile + p.ntile / kGGroup) * Dp : 0;
+    p.group = p.ntile >= kGLong ? kGGroupLong : kGGroup;
+    const int64_t Dp = (int64_t)p.nct * kGC, words = p.ntile > 1 ? (p.ntile + (p.ntile >> p.group)) * Dp : 0;
     char* at = static_cast<char*>(ws);
     size_t n = 0;
     auto take = [&](size_t bytes) {
@@ -710,7 +717,7 @@ static size_t gated_plan(GatedP& p, bool back, void* ws) {
 }
 static void gated_clear_launch(const GatedP& p, hipStream_t s) {
     if (p.ntile <= 1) return;
-    const int64_t n = (int64_t)(p.ntile + p.ntile / kGGroup) * p.nct * kGC / 2;  // kGC words are whole 16 bytes
+    const int64_t n = (int64_t)(p.ntile + (p.ntile >> p.group)) * p.nct * kGC / 2;  // kGC words are whole 16 bytes
     hipLaunchKernelGGL(gated_clear, dim3((uint32_t)std::min<int64_t>((n + 255) / 256, 2048)), dim3(256), 0, s, p.ticket, p.nct, reinterpret_cast<uint4*>(p.map), n);
 }
 static int gated_grid_ok(const GatedP& p) {

@@ -177,9 +177,9 @@ _Q8 = {torch.int8: _lib.MAMBA_INT8, torch.float8_e4m3fn: _lib.MAMBA_E4M3}
 def add_rms_norm_q8(x: torch.Tensor, weight: Optional[torch.Tensor], residual: Optional[torch.Tensor] = None, eps: float = 1e-5,
                     dtype: torch.dtype = torch.int8, out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
                     residual_out: Optional[torch.Tensor] = None) -> tuple:
-    """``add_rms_norm`` into rows of 8 bits: (q, scale, s) with y = q * scale, q int8 or
+    """``add_rms_norm`` into rows of 8 bits: (q, scale, s) with y near q * scale, q int8 or
     float8_e4m3fn of x's shape and scale [rows] f32 (rows of the last axis) = max |y| / 127 or
-    / 448.  A row whose largest |y| is below 2^-100 has scale 0 and zeros, one with a NaN or an
+    / 448; q is y / scale, rounded to f32 and then to the nearest code.  A row whose largest |y| is below 2^-100 has scale 0 and zeros, one with a NaN or an
     infinity in y a NaN for its scale and zeros.  Gradients do not pass it."""
     m = _matrix(x, "x")
     if dtype not in _Q8:

@@ -1118,10 +1118,11 @@ int mamba_layernorm_bwd(const mamba_layernorm_bwd_args* args, void* workspace, s
 /* sum as it is before it is stored as s.  rstd [rows] is written if given.    */
 /* s may be residual itself, and x where the types agree; y may be x.          */
 /*                                                                             */
-/* The row of 8 bits (q given, y NULL) is y / scale, rounded to the nearest    */
-/* (ties to even), scale [rows] = max |y| / 127 (MAMBA_INT8) or / 448          */
-/* (MAMBA_E4M3, OCP).  A row whose largest |y| is below 2^-100 has scale 0 and */
-/* zeros; a row with a NaN or an infinity in y a NaN for its scale, and zeros. */
+/* The row of 8 bits (q given, y NULL) is y / scale, rounded to f32 and then   */
+/* to the nearest code (ties to even); scale [rows] is max |y| / 127           */
+/* (MAMBA_INT8) or / 448 (MAMBA_E4M3, OCP).  A row whose largest |y| is below  */
+/* 2^-100 has scale 0 and zeros; one with a NaN or an infinity in y a NaN for  */
+/* its scale, and zeros.                                                       */
 /* ------------------------------------------------------------------------- */
 typedef struct mamba_add_rmsnorm_args {
     int64_t rows;

@@ -187,8 +187,8 @@ struct Q4Op<Q4_I8> {
     __device__ __forceinline__ void make(const Q4A<Q4_I8>& a) { v[0] = a.part(0); }
 };
 
-// Column tile j through buffer resources (scalar bases, 32-bit offsets): blocks behind the last,
-// and tiles behind the last, read zeros.
+// Column tile j through buffer resources (scalar bases, 32-bit offsets).  A tile behind the last
+// has no extent; whatever of the first tile's its loads bring, no result of it is stored.
 struct Q4Tile {
     __amdgpu_buffer_rsrc_t codes, scale;
     __device__ __forceinline__ Q4Tile(const Q4W& q, int j) {
@@ -198,22 +198,32 @@ struct Q4Tile {
         scale = buf_rsrc(static_cast<const char*>(q.scale) + at * words, kb ? words : 0u);
     }
 };
+// Block kb of KB, as the loads take it.  One behind the last reads zeros: that is told by the lane's own
+// offset, past the extent, while the scalar one stays inside (how far that one is checked is not relied on).
+struct Q4At {
+    int kb;
+    uint32_t out;
+    __device__ __forceinline__ Q4At(int k, int KB) : kb(k < KB ? k : 0), out(k < KB ? 0u : kQ4Out) {}
+};
 // A block of a column tile: its codes, and its groups' scales and zero points.
 template <int GB, int S>
 struct Q4Block {
     uint4 w;
     uint32_t s[GB];
     uint32_t z[S == Q4_S32 ? GB : 1];
-    __device__ __forceinline__ void load(const Q4Tile& t, int kb, int l) {
-        w = buf_ld16(t.codes, l * 16, kb * 1024);
+    __device__ __forceinline__ void load(const Q4Tile& t, const Q4At& at, int l) {
+        constexpr int word = S == Q4_S32 ? 8 : 4;
+        w = buf_ld16(t.codes, l * 16 + at.out, at.kb * 1024);
 #pragma unroll
         for (int g = 0; g < GB; ++g) {
+            const uint32_t off = (l & 15) * word + at.out + g * kQ4N * word;
+            const int soff = at.kb * GB * kQ4N * word;
             if constexpr (S == Q4_S32) {
-                const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(t.scale, (l & 15) * 8 + g * kQ4N * 8, kb * GB * kQ4N * 8, 0));
+                const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(t.scale, off, soff, 0));
                 s[g] = v.x;
                 z[g] = v.y;
             } else {
-                s[g] = __builtin_amdgcn_raw_buffer_load_b32(t.scale, (l & 15) * 4 + g * kQ4N * 4, kb * GB * kQ4N * 4, 0);
+                s[g] = __builtin_amdgcn_raw_buffer_load_b32(t.scale, off, soff, 0);
             }
         }
     }
@@ -361,7 +371,7 @@ __global__ __launch_bounds__(64 * (RT > 1 ? 8 : kQ4Waves)) void q4_held(Q4P p) {
         const Q4Tile t(p.w, blockIdx.x);
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
-            b[k].load(t, kb0 + k, l);
+            b[k].load(t, Q4At(kb0 + k, p.w.KB), l);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -397,7 +407,7 @@ __global__ __launch_bounds__(64 * (RT > 1 ? 8 : kQ4Waves)) void q4_held(Q4P p) {
             for (int g = 0; g < GB; ++g) q4_group<X, RT, GB, S>(b[k], g, x[k], tot);
             // behind the block's last use, so that its registers are these
             __builtin_amdgcn_sched_barrier(0);
-            b[k].load(next, kb0 + k, l);
+            b[k].load(next, Q4At(kb0 + k, p.w.KB), l);
             __builtin_amdgcn_sched_barrier(0);
         }
         q4_f32x4* red = q4_red + (turn & 1) * RT * nw * 64;
@@ -435,7 +445,7 @@ __global__ __launch_bounds__(512) void q4_walk(Q4P p) {
     static_assert(C == 2, "two tiles");
     auto codes = [&](int q, int kb) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) b[q][c].load(tile[c], kb, l);
+        for (int c = 0; c < C; ++c) b[q][c].load(tile[c], Q4At(kb, p.w.KB), l);
     };
     const int stop = p.w.KB;
     codes(0, kb0);

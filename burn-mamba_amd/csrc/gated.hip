@@ -495,7 +495,9 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_bwd(GatedP p) {
         g_decays<R>(a, q);
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            const float im = q[j] > 0.f ? __builtin_amdgcn_rsqf(q[j]) : q[j] * 0.f;  // 0 where a is 1, a NaN of a NaN
+            // 0 where a is 1 (of a q below the normal numbers the hardware's root is 0 and its reciprocal
+            // infinity), a NaN of a NaN
+            const float im = q[j] >= 0x1p-126f ? __builtin_amdgcn_rsqf(q[j]) : q[j] * 0.f;
             const float m = q[j] * im;
             const Logistic i = g_logistic(g_value<T>(ei[j]));
             const float u = i.s * g_value<T>(ex[j]);

@@ -481,7 +481,7 @@ def gated_scan_packed_bwd(dy, x, r, i, A, cu_seqlens, carry, z=None, initial_sta
     the same initial_state).  ``initial_state`` and ``d_final_state`` [sequences, d] f32 or
     None.  Returns dict(dx, dr, di, dz of their tensors' type, zero outside the sequences; dA,
     d_initial_state f32; None for what was not given).  The same inputs give the same bits.
-    Where a_t is exactly 1 the input's weight is 0, and is taken not to change with a_t."""
+    Where 1 - a_t^2 is below 2^-126 the input's weight is taken as 0, and not to change with a_t."""
     _need(carry is not None, "carry is required")
     a = GatedScanBwdArgs()
     a.fwd = _gated_args(x, r, i, A, cu_seqlens, z, carry)

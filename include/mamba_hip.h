@@ -1029,10 +1029,11 @@ int mamba_gated_scan_fwd(const mamba_gated_scan_args* args, void* workspace, siz
 /*   dh_t = g_t + a_{t+1} dh_{t+1},  e_t = dh_t (a_t h_{t-1} - u_t a_t^2 / m_t) */
 /*   dx = dh m s(i),  di = dh m u s(-i),  dr = e A s(r) s(-r),                 */
 /*   dA = sum_t e s(r),  dz = dy h silu'(z),  d_initial_state = a dh (first)   */
-/* (u a^2 / m is taken as 0 where a is exactly 1).  initial_state and          */
-/* d_final_state [nseq, d] or NULL (zero).  dx, dr, di and dz are zero outside */
-/* the sequences; d_initial_state's rows of empty sequences are left as they   */
-/* were.  Sums in a fixed order: the same inputs give the same bits.           */
+/* (Where 1 - a^2 is below 2^-126, m is taken as 0, by the forward too, and    */
+/* so is u a^2 / m.)  initial_state and d_final_state [nseq, d] or NULL (zero). */
+/* dx, dr, di and dz are zero outside the sequences; d_initial_state's rows of */
+/* empty sequences are left as they were.  Sums in a fixed order: the same     */
+/* inputs give the same bits.                                                  */
 typedef struct mamba_gated_scan_bwd_args {
     mamba_gated_scan_args fwd;
     const float* initial_state;

@@ -425,7 +425,7 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
         float v = h;
         if constexpr (Z) {
             const float z = g_value<T>(ez[j]);
-            v = h * z * g_sigmoid(z);
+            v = h * (z * g_sigmoid(z));  // silu first: h z may pass f32 where silu is 0
         }
         y.store(j, col, v);
     };
@@ -689,7 +689,7 @@ __global__ __launch_bounds__(256) void gated_step(GatedStepP p) {
         const Decay g = g_decay<true>(A * g_sigmoid(r));
         y = __builtin_fmaf(g.a, h0, __builtin_amdgcn_sqrtf(g.q) * (g_sigmoid(i) * x));
         *st = y;
-        if (p.z) y = y * z * g_sigmoid(z);
+        if (p.z) y = y * (z * g_sigmoid(z));
     }
     store_f32<T>(static_cast<T*>(p.y) + b * p.y_sb + c, y);
 }

@@ -7,7 +7,7 @@
 // dword st of its four the codes of k = 32 st + 8 (l / 16) + e, e = 0..7: nibble e / 2 for even
 // e, 4 + e / 2 for odd, so that two consecutive k lie 16 bits apart.  Behind the blocks, for
 // [tile][group][16], the scale and -(16 + zero point): two bf16 in a word, or with f32 scales two
-// floats.  What k and columns are padded with has scale 0.
+// floats.  What k and columns are padded with has scale 0, a group with a zero point above 16 a NaN.
 //
 // A code goes into the matrix instruction as 16 + c, which its bits give in one or two instructions,
 // and -(16 + zero) as a second operand with the same rows: no weight is formed, and no rounding but
@@ -88,9 +88,13 @@ __global__ __launch_bounds__(256) void q4_pack(Q4W w, const uint8_t* codes, cons
         const int col = (int)(i % 16), g = (int)(i / 16 % w.NG), n = (int)(i / 16 / w.NG) * kQ4N + col;
         const bool in = g < groups && n < w.N;
         const int64_t src = (int64_t)g * w.N + n;
-        const float z = -16.f - (in ? (zero ? zero[src] & 15 : 8) : 0);  // whole numbers to 31: bf16 holds them
-        if (w.sbf16) static_cast<uint32_t*>(oscale)[i] = (in ? (uint32_t)static_cast<const bf16_t*>(scale)[src] << 16 : 0u) | __float_as_uint(z) >> 16;
-        else static_cast<float2*>(oscale)[i] = make_float2(in ? static_cast<const float*>(scale)[src] : 0.f, z);
+        const int zp = in ? (zero ? zero[src] : 8) : 0;
+        const float z = -16.f - (float)min(zp, 16);  // whole numbers to 32: bf16 holds them
+        uint32_t sc = 0;
+        if (in) sc = w.sbf16 ? (uint32_t)static_cast<const bf16_t*>(scale)[src] << 16 : __float_as_uint(static_cast<const float*>(scale)[src]);
+        if (zp > 16) sc = 0x7fc00000u;
+        if (w.sbf16) static_cast<uint32_t*>(oscale)[i] = sc | __float_as_uint(z) >> 16;
+        else static_cast<float2*>(oscale)[i] = make_float2(__uint_as_float(sc), z);
     }
 }
 

@@ -63,7 +63,7 @@ def quantize_q4(weight: torch.Tensor, group: int = 64, zero_points: bool = False
 def pack_linear_q4(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None, group: Optional[int] = None) -> PackedQ4:
     """Lay a weight of 4 bits out for ``linear_q4``, once, at model load: codes [d_in, d_out]
     uint8 of 0 to 15 (the low four bits are taken), scale [groups, d_out] f32 or bf16, zero
-    [groups, d_out] uint8 or None (8 everywhere).  ``group``, the rows that share a scale, is
+    [groups, d_out] uint8 of 0 to 16 or None (8 everywhere).  ``group``, the rows that share a scale, is
     32, 64 or 128; None: d_in / groups, where that is whole."""
     _need(codes.dim() == 2 and codes.dtype == torch.uint8 and codes.numel() > 0, "codes must be a uint8 [d_in, d_out] tensor")
     d_in, d_out = codes.shape
@@ -73,6 +73,7 @@ def pack_linear_q4(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torc
     _need(group in (32, 64, 128), "group must be 32, 64 or 128")
     _need(scale.shape[0] == -(-d_in // group), "scale must have a row for each group")
     _need(zero is None or (zero.dtype == torch.uint8 and zero.shape == scale.shape), "zero must be uint8 and match scale")
+    _need(zero is None or int(zero.max()) <= 16, "zero points must be at most 16")
     with _one_device(codes, scale, zero):
         codes, scale = codes.contiguous(), scale.detach().contiguous()
         zero = None if zero is None else zero.contiguous()

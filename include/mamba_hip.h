@@ -1208,8 +1208,9 @@ typedef struct mamba_q4_weight {
 
 size_t mamba_linear_q4_packed_size(const mamba_q4_weight* w);
 /* codes [d_in, d_out] (a byte each, the low four bits taken), scale [groups,  */
-/* d_out] of scale_dtype and zero [groups, d_out] bytes (0..15, with has_zero) */
-/* contiguous -> packed                                                        */
+/* d_out] of scale_dtype and, with has_zero, zero [groups, d_out] bytes of 0 to */
+/* 16 (a format that keeps the zero point less one gives up to 16; a larger one */
+/* makes its group's scale a NaN), contiguous -> packed                        */
 int mamba_linear_q4_pack(const mamba_q4_weight* w, const void* codes, const void* scale, const void* zero,
                          void* packed, mamba_stream_t stream);
 

@@ -56,3 +56,21 @@ def test_larger_ones_through_the_c_entry(dev, sdtype):
     for x, xs in ((torch.ones(3, k, device=dev), None), (torch.ones(3, k, dtype=I8, device=dev), torch.ones(3, device=dev))):
         y = mamba_hip.linear_q4(x, w, x_scale=xs, dtype=F32)
         assert y.isnan().all(0).tolist() == bad and bool((y[:, ~torch.tensor(bad)] == k).all())
+
+
+@pytest.mark.gpu
+def test_captured(dev):
+    """Laid out in a graph, again from codes and zero points that have changed."""
+    k, n = 128, 40
+    g = torch.Generator().manual_seed(1)
+    codes = torch.randint(0, 16, (k, n), generator=g, dtype=U8).to(dev)
+    zero, scale = torch.randint(0, 17, (2, n), generator=g, dtype=U8).to(dev), torch.rand(2, n, generator=g).to(dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w = mamba_hip.pack_linear_q4(codes, scale, zero)
+    for turn in range(3):
+        codes.copy_((codes + turn).remainder(16))
+        zero.copy_((zero + turn).remainder(17))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(w.data, mamba_hip.pack_linear_q4(codes, scale, zero).data)

@@ -8,7 +8,7 @@
 //
 // The sum is normalised as it is in f32, before it is rounded to the stream's type: y
 // then has one rounding.  The backward reads the stored s, or, where that one was rounded to bf16,
-// the two rows that it was the sum of (16384 x 2560 91 us against 80): from the rounded s dw is off
+// the two rows that it was the sum of (16384 x 2560 93 us against 77): from the rounded s dw is off
 // by 2e-3 of itself, from the sum by 1e-7.
 //
 // Some ten operations an element against three or four elements moved: HBM-bound.  Rows of up to
@@ -17,9 +17,9 @@
 // the row's width; the next row's loads are in flight while this one is summed.  The backward's
 // workgroups take rows in turn and sum dw of their columns in registers, joined in LDS
 // and, over the workgroups, by arn_dw_join, in a fixed order.  16384 x 2560, bf16 rows with an f32
-// stream: forward 97 us (5.2 TB/s), backward with the join 126 (5.3), to int8 94 (4.9): what a copy
-// reaches.  4096 x 16384 of bf16 in registers / by the wide kernels below: forward 104 / 173, backward
-// 126 / 312, int8 107 / 212.
+// stream: forward 97 us (5.2 TB/s), backward with the join 127 (5.3), to int8 90 (5.1): what a copy
+// reaches.  4096 x 16384 of bf16 in registers / by the wide kernels below: forward 103 / 166, backward
+// 128 / 310, int8 106 / 211.  Times: calls back to back in a captured graph on a warm card.
 #include <algorithm>
 
 #include "pack.h"
@@ -77,8 +77,8 @@ __device__ __forceinline__ ArnScale arn_scale(uint32_t amax, bool e4m3) {
 }
 // v / (scale up), v = y up, rounded once: what a division gives, but where the quotient lies within 2^-22
 // steps of midway between two f32.  The product with inv alone is up to one and a half steps off, and of
-// values at the edge between two codes a sixth fell on its wrong side.  4000 x 2560 to e4m3 16.1 us, with the
-// product alone 15.8, with a division's steps (two remainders) 17.4.
+// values at the edge between two codes a sixth fell on its wrong side.  4000 x 2560 to e4m3 15.3 us, with the
+// product alone 15.2, with a division 17.7.
 __device__ __forceinline__ float arn_quotient(float v, const ArnScale& s) { return __builtin_fmaf(v, s.inv, v * s.lo); }
 __device__ __forceinline__ uint8_t arn_q8(float v, const ArnScale& s, bool e4m3) {
     if (s.inv == 0.f) return 0;
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(arn_block(G)) void arn_bwd_rows(ArnP p) {
 }
 
 // Any width: a workgroup per row, the row read once per sweep (two forward, three to 8 bits; two and
-// one more for dw backward): 2048 x 20000, bf16 with an f32 stream: 169 us, 209 and 257.
+// one more for dw backward): 2048 x 20000, bf16 with an f32 stream: 167 us, 203 and 257.
 template <typename T, typename S>
 __global__ __launch_bounds__(256) void arn_fwd_wide(ArnP p) {
     constexpr int E = 4, ST = 256 * E;
@@ -550,13 +550,16 @@ static int arn_steps(int cols, int E, int G) { return ceil_div(cols, G * E); }
 static int arn_lanes(int cols, int E) {
     return arn_steps(cols, E, 16) <= 2 ? 16 : arn_steps(cols, E, 64) <= 3 ? 64 : arn_steps(cols, E, 256) <= 5 ? 256 : arn_steps(cols, E, 512) <= 4 ? 512 : 0;
 }
+// Workgroups of the forward, which take rows in turn.  us at 1024 / 2048 / 16384: 16384 x 2560 with an f32
+// stream 93 / 97 / 87, 4000 x 2560 of bf16 14.3 / 14.5 / 15.3, 65536 x 256 30.6 / 31.2 / 30.8, 8192 x 5120
+// 97 / 95 / 88.
 static uint32_t arn_fwd_grid(int64_t rows, int G) {
     const int rb = arn_block(G) / G;
     return (uint32_t)std::min<int64_t>((rows + rb - 1) / rb, 2048);
 }
 // Workgroups of the backward: two a CU, and some eight rows a group at least, so that the parts
 // stay few beside the rows.  us at 512 / 1024 with the join: 16384 x 2560 with an f32 stream 127 /
-// 139, bf16 82 / 91, 65536 x 256 57 / 56.
+// 137, bf16 77 / 88, 65536 x 256 52 / 50.
 static int arn_parts(int64_t rows, int cols, int E) {
     const int G = arn_lanes(cols, E);
     if (G == 0) return (int)std::min<int64_t>(256, (rows + 31) / 32);

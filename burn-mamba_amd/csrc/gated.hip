@@ -15,18 +15,21 @@
 // workgroup takes one tile of 64 channels, keeps it in registers, and finds the state that enters
 // it while the tile is there.
 // A stretch of rows maps the state that enters it, h -> P h + H; P is the product of its
-// decays and H what it leaves from zero.  A lane holds R rows of one channel (two would take
-// twice the registers and leave the backward one workgroup a CU, which took half as long again); the maps of the eight waves are joined in LDS to the tile's, which is published to the
-// other workgroups before the tile's own state is waited for.  That state is joined from the
-// published maps of the tiles before it, back to the one in which the tile's first sequence
-// begins, or to the last group of 16 or 64 tiles, whose final state its last tile publishes.  The
-// joins follow a fixed order: the same inputs give the same bits.  The backward walks the other way
-// with q in the state's place, and finds h again from the states that the forward kept.
+// decays and H what it leaves from zero.  A lane holds R rows of one channel (two channels would take
+// twice the registers and leave the backward one workgroup a CU, which took half as long again).
+// The maps of the eight waves are joined in LDS to the tile's, which is published to the other
+// workgroups before the tile's own state is waited for.  That state is joined from the published
+// maps of the tiles before it, back to the one in which the tile's first sequence begins, or to
+// the last group of 16 or 64 tiles, whose final state its last tile publishes.  The joins follow a
+// fixed order: the same inputs give the same bits.  The backward walks the other way with q in the
+// state's place, and finds h again from the states that the forward kept.
 //
 // A map is published as one 64-bit word (P, H) and read with relaxed atomics of the whole card:
 // the word is its own flag, all ones until it is written (P of a NaN is made the usual one, so
 // that no map has that value).  A workgroup takes its tile by ticket, so the tiles that it waits
 // for belong to workgroups that run already, and those publish before they wait: every wait ends.
+//
+// Times below: calls back to back in a captured graph on a warm card, with their clear and join.
 #include <algorithm>
 
 #include "pack.h"
@@ -67,8 +70,8 @@ constexpr int kCarryRows = 64;  // rows between the states that the forward keep
 constexpr int kGW = 8, kGC = 64;  // waves of a workgroup; channels of a tile: one a lane
 // Log2 of the tiles of a group.  The ends of groups are found one behind the other: with many of them
 // in flight that chain is the longer wait, with few the maps of a group are (64 / 16 tiles: 262144 x
-// 256 of bf16 forward 165 / 183 us, backward 336 / 373; 65536 x 512 backward 180 / 176, 8192 x 5120
-// 214 / 205).
+// 256 of bf16 forward 185 / 202 us, backward 381 / 410; 65536 x 512 77 / 77 and 160 / 159, 8192 x 5120
+// 104 / 99 and 208 / 196).
 constexpr int kGGroup = 4, kGGroupLong = 6;
 constexpr int kGLong = 2048;                     // tiles of rows from which on groups are long
 constexpr uint64_t kGNone = ~0ull;               // nothing published yet
@@ -94,10 +97,14 @@ __device__ __forceinline__ Logistic g_logistic(float v) {
     return {s, v > 0.f ? e * s : 1.f - s};
 }
 
-// a = exp(v) and q = 1 - a^2 for v <= 0, both to a few steps of their own size.  From -1/8 up by
+// a = exp(v) and q = 1 - a^2 for v <= 0, both to a few steps of their own size (below -1/8 a's error
+// grows as |v|, by the rounding of the exponent).  From -1/8 up by
 // e = exp(v) - 1, the series to v^5 / 5! (its next term is 2^-24 of the sum there): a = 1 + e,
 // 1 - a^2 = -e (2 + e) keep what a difference from 1 would lose as a nears 1.  FAR: with the
-// exponential for what lies below, which a tile takes only where it has such a value.
+// exponential for what lies below, which a wave takes only where it has such a value.  Forward and
+// backward where no wave has one / every wave has one, through one channel in 64: 8192 x 5120 of bf16
+// 99 / 102 and 196 / 198 us, 2048 x 2560 22.6 / 23.3 and 38.1 / 38.3, 65536 x 512 77 / 80 and 160 / 162;
+// in f32, bound by memory, no different.
 struct Decay { float a, q; };
 __device__ __forceinline__ bool g_near(float v) { return v >= -0.125f; }  // not of a NaN
 template <bool FAR>
@@ -233,10 +240,10 @@ struct GShared {
 
 // The tile of this workgroup (in the order in which the tiles wait for one another) and its channels.
 // A ticket for each column tile: one counter for all is asked by 512 workgroups at once when a
-// kernel starts (4000 x 2560 of bf16 40 us, 35 with a ticket each).  The columns turn against the
+// kernel starts (4000 x 2560 of bf16 took 1.14 times as long).  The columns turn against the
 // workgroups' numbers from a row of tiles to the next, as the numbers go around the chip's eight
 // dies: a die that kept every eighth column would go through a few channels of its L2 (8192 x 5120
-// 116 us, 106 with the turn).
+// took 1.09 times as long).
 __device__ __forceinline__ void g_tile(const GatedP& p, GShared& s, int& o, int& ct) {
     if (p.ntile > 1) {
         ct = (blockIdx.x + blockIdx.x / p.nct) % p.nct;
@@ -338,8 +345,8 @@ __device__ __forceinline__ void g_fetch(uint32_t (&e)[R], const GatedP& p, const
     for (int j = 0; j < R; ++j) e[j] = row.load(min(j, k), col);
 }
 
-// 8192 x 5120: bf16 with z 104 us (420 MB, 4.0 TB/s), f32 without 131 (671 MB, 5.1: what a copy
-// reaches).  bf16: half the time is issue of vector instructions (44 a row, 7 of them at a quarter
+// 8192 x 5120: bf16 with z 99 us (420 MB, 4.2 TB/s), f32 without 125 (671 MB, 5.4: what a copy
+// reaches and a little from the last-level cache).  bf16: half the time is issue of vector instructions (44 a row, 7 of them at a quarter
 // of the rate), the rest a tile's latencies (ticket, rows, the states that enter), which two
 // workgroups a CU hide in part; three (80 registers) spill and take 1.2 times as long.
 template <typename T, bool Z>
@@ -456,7 +463,7 @@ __global__ __launch_bounds__(64 * kGW, 4) void gated_fwd(GatedP p) {
 // What a row's gradients need is formed once, where its values are read: with u = s(i) x,
 //   gr = dy silu(z), zk = dy silu'(z), pull = u a^2 / m, kr = A s(r) s(-r), ui = u s(-i)
 // so that dz = h zk, dx = dh m s(i), di = dh m ui, dr = e kr, e = dh (a h_{t-1} - pull).
-// 8192 x 5120: bf16 with z 202 us with the join (755 MB, 3.7 TB/s), f32 without 236 (1174 MB, 5.0).
+// 8192 x 5120: bf16 with z 196 us (755 MB, 3.9 TB/s), f32 without 229 (1174 MB, 5.1).
 // Bound as the forward is: some 90 vector instructions a row.
 template <typename T, bool Z>
 __global__ __launch_bounds__(64 * kGW, 4) void gated_bwd(GatedP p) {
@@ -669,9 +676,9 @@ struct GatedStepP {
     void* y; int64_t y_sb;
 };
 
-// A token a row, a channel a lane: 256 tokens of 5120 bf16 channels 8.0 us for 23.6 MB.  Bound by the
-// latency of its loads, which do not wait for the slot; two channels a lane took 9.2 us and four 7.6,
-// and a single token 2.6 and 3.0 us against 2.4.
+// A token a row, a channel a lane: 256 tokens of 5120 bf16 channels 6.0 us for 23.6 MB, a single one
+// 2.4.  Bound by the latency of its loads, which do not wait for the slot.  Two and four channels a lane
+// took 1.15 and 0.95 times as long for 256 tokens, 1.08 and 1.25 for one, where latency counts most.
 template <typename T>
 __global__ __launch_bounds__(256) void gated_step(GatedStepP p) {
     const int b = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;

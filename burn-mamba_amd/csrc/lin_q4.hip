@@ -11,14 +11,17 @@
 //
 // A code goes into the matrix instruction as 16 + c, which its bits give in one or two instructions,
 // and -(16 + zero) as a second operand with the same rows: no weight is formed, and no rounding but
-// that of f32 sums.  f32 rows go in as three bf16 parts.  int8 rows take the codes as bytes, and
-// their sums are whole numbers up to the scale.
+// that of f32 sums.  Those are sums of up to 31 x, of which the second operand takes most off again:
+// a step of theirs is up to 16 times one of the result's terms.  f32 rows go in as three bf16 parts.
+// int8 rows take the codes as bytes, and their sums are whole numbers up to the scale.
 //
-// Few rows are bound by the weight's bytes and a kernel's one trip to memory: 1 x 2560 x 10240 6.7 us
-// (13.9 MB; at a copy's rate 2.8), 7 x 2560 x 50001 17.7 (67 MB, 3.8 TB/s).  More rows are loaded
-// into registers before the first block is used, 16 in 2.5 us, and a turn of a workgroup (four waves
-// of five blocks, then a barrier) takes 1.3: 64 rows of int8 14.4 us, in which two waves a SIMD issue
-// two thirds of the time.
+// Few rows are bound by the weight's bytes and a kernel's trips to memory: 1 x 2560 x 10240 5.3 us
+// (13.9 MB; at a copy's rate 2.8; of its 640 column tiles 128 are a second turn of 512 workgroups), 7 x
+// 2560 x 50001 15.8 (67 MB, 4.2 TB/s).  More rows are loaded into registers before the first block is
+// used, 16 in 2.5 us, and a turn of a workgroup (four waves of five blocks, then a barrier) takes 1.3: 64
+// rows of int8 13.7 us, in which two waves a SIMD issue two thirds of the time.  A prompt's rows go the
+// same way, 16 or 32 a workgroup and every code taken apart for each: 4000 x 2560 x 10240 of bf16 378 us,
+// 555 TFLOP/s.  Times: calls back to back in a captured graph on a warm card.
 #include <algorithm>
 
 #include "pack.h"
@@ -54,7 +57,7 @@ static bool q4_make(const mamba_q4_weight* w, Q4W* o, size_t* bytes) {
 }
 
 // A thread forms what four lanes of a block hold (run q of 8 k in each 32, four columns): a dword of
-// codes a row, 16 bytes out a lane.  2560 x 50001 (196 MB) 47 us with its scales.
+// codes a row, 16 bytes out a lane.  2560 x 50001 (196 MB) 44 us with its scales.
 __global__ __launch_bounds__(256) void q4_pack(Q4W w, const uint8_t* codes, const void* scale, const uint8_t* zero, uint4* out, void* oscale) {
     const int64_t step = (int64_t)gridDim.x * 256, at0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int n4 = w.NT * (kQ4N / 4);
@@ -515,7 +518,10 @@ static void q4_held_launch(const Q4P& p, int nw, hipStream_t s) {
 }
 template <int X, int RT, int C, int GB>
 static void q4_walk_launch(const Q4P& p, hipStream_t s) {
-    int nw = 4;  // some 2048 waves in all, each with two blocks at least
+    // Some 2048 waves in all, each with two blocks at least.  us at 1024 / 2048 / 4096: one bf16 row of 10240 x
+    // 10240 22.2 / 23.8 / 23.8, x 20480 28.8 / 28.6 / 34.4; one f32 row of 5120 x 10240 31.0 / 37.7 / 37.8, x 20480
+    // 44.5 / 44.4 / 55; four bf16 rows of 10240 x 2560 13.0.
+    int nw = 4;
     while (nw < 8 && (int64_t)p.w.NT * nw < 2048 * C && p.w.KB >= 4 * nw) nw *= 2;
     const dim3 grid(ceil_div(p.w.NT, C), (uint32_t)((p.rows + 16 * RT - 1) / (16 * RT))), block(64 * nw);
     const size_t lds = (size_t)nw * RT * C * 64 * 16;
@@ -525,12 +531,12 @@ static void q4_walk_launch(const Q4P& p, hipStream_t s) {
 }
 // The rows in registers wherever twelve waves hold them (60 blocks of k, f32 24), as four, eight or
 // twelve waves, which load the four SIMDs evenly; else the walk.  us held / walked, bf16 at 2560 x 10240:
-// 32 rows 12.4 / 19.9, 64 rows 15.6 / 26.7, 256 rows 41 / 78; int8 64 rows 14.4 / 23.4, at 5120 x
-// 2560 11.0 / 14.7; f32 one row 9.1 / 27.
+// one row 5.3 / 11.1, 32 rows 11.4 / 17.5, 64 rows 14.8 / 24.8, 256 rows 34 / 78; int8 64 rows 13.7 / 22.8,
+// at 5120 x 2560 11.0 / 14.9; f32 one row 9.0 / 26.3.
 // Two row tiles a wave take apart a block once for both, but start with twice the rows to load: where
 // a workgroup has ten tiles or more to go through.  us with one / two at 2560 x 10240: bf16 64 rows
-// (5 tiles) 15.8 / 18.7, 128 rows (10) 24.6 / 23.3, 256 rows (20) 41.0 / 34.4, int8 35.2 / 29.5; bf16
-// 64 rows at 2560 x 50001 (24) 50.3 / 42.4.
+// (5 tiles) 14.8 / 17.2, 128 rows (10) 23.2 / 22.4, 256 rows (20) 39.3 / 34.2, int8 33.5 / 29.0; bf16
+// 64 rows at 2560 x 50001 (24) 46.7 / 40.6.
 template <int X, int GB>
 static void q4_shape(const Q4P& p, hipStream_t s) {
     constexpr int most = X == Q4_F32 ? 2 : 5;  // blocks of k whose operands a wave's registers hold

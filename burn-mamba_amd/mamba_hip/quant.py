@@ -96,8 +96,8 @@ def linear_q4(x: torch.Tensor, weight: PackedQ4, bias: Optional[torch.Tensor] = 
     """y = x W + bias for few rows: x [rows, d_in] bf16, f32 or, with x_scale [rows] f32 (the rows
     of ``add_rms_norm_q8``), int8; bias [d_out] f32.  Returns [rows, d_out] of ``dtype`` (f32
     or bf16; None: x's, bf16 for int8) or in ``out``.  Sums are f32, of int8 rows exact
-    within a group; a row of x with a NaN or an infinity gives a row of NaN.  Gradients do not
-    pass it."""
+    within a group; a row of x with a NaN or an infinity gives a row of NaN, and values
+    from 2^115 on, where sums of 31 |x| may pass f32, may.  Gradients do not pass it."""
     if x.dtype not in _X:
         _fail(f"x: dtype {x.dtype}, expected float32, bfloat16 or int8")
     _need(x.dim() == 2 and x.shape[1] == weight.d_in, "x must be [rows, d_in]")

@@ -1197,8 +1197,9 @@ int mamba_dropout(const mamba_dropout_args* args, mamba_stream_t stream);
 /* bytes, 16-byte aligned).                                                    */
 /* x: bf16, f32 (three bf16 parts, which hold all of it) or int8 with x_scale  */
 /* [rows]; sums are f32, of int8 rows exact within a group.  The codes and the */
-/* zero points are multiplied apart, so a row of x with a NaN or an infinity   */
-/* gives a row of NaN.                                                         */
+/* zero points are multiplied apart, in sums of up to 31 |x| a term: a row of x */
+/* with a NaN or an infinity gives a row of NaN, and values from 2^115 on, where */
+/* those sums may pass f32, may.                                               */
 /* ------------------------------------------------------------------------- */
 typedef struct mamba_q4_weight {
     int32_t d_in, d_out, group, scale_dtype;  /* scales f32 or bf16           */
